@@ -466,3 +466,57 @@ int swiglu_quant_col_chunk(int rows, int inter);   // columns of a row that one 
 cudaError_t launch_moe_bwd(const MoeBwdArgs& args, cudaStream_t stream);
 int moe_bwd_prep_col_blocks(int cols);   // PREP writes row_dot as [col_blocks, rows] partial sums
 }  // namespace ep
+
+// ------------------------------------------------------------------------------------------------ routing
+// Choice of experts and weights from gate logits, and the gradient of the weights (router.cu states the formulas).
+struct RouterArgs {
+    const void* logits;               // [num_tokens, num_experts] fp32 or bf16, row pitch ld elements
+    int64_t ld;
+    int logits_bf16;
+    int num_tokens, num_experts, num_topk;
+    int softmax;                      // scores: softmax over the experts, or the sigmoid of each
+    int renormalize;                  // weights of a token add up to scale
+    float scale;
+    const float* bias;                // [num_experts] added to the scores for the choice alone, or null
+    const uint8_t* token_mask;        // [num_tokens] 0: the token goes nowhere; or null
+    int num_groups, num_topk_groups;  // at most 32 groups of consecutive experts
+    int group_top;                    // 1 or 2 best choices make a group's score
+    void* topk_idx;                   // [num_tokens, num_topk] int64 or int32, -1 in empty places (the gradient reads it)
+    int idx_is_64;
+    float* topk_weights;              // [num_tokens, num_topk]
+    int32_t* count;                   // [num_experts] tokens that chose an expert
+    const float* d_weights;           // gradient: [num_tokens, num_topk]
+    void* d_logits;                   // gradient: [num_tokens, num_experts] contiguous, type of the logits
+};
+
+namespace ep {
+cudaError_t launch_route(const RouterArgs& args, int num_sms, cudaStream_t stream);
+cudaError_t launch_route_backward(const RouterArgs& args, int num_sms, cudaStream_t stream);
+}  // namespace ep
+
+// ------------------------------------------------------------------------------------------------ layer norm
+struct LayerNormArgs {
+    const void* x;                    // [rows, hidden] bf16 or fp32, row pitch ldx elements
+    int64_t ldx;
+    int rows, hidden;
+    int x_bf16, param_bf16;           // types of x (y, dy, dx) and of the weights (bias and their gradients): bf16 or fp32
+    const void* weight;               // [hidden]
+    const void* bias;                 // [hidden] or null
+    float eps;
+    void* y;                          // [rows, hidden] contiguous
+    float* mean;                      // [rows] written by the forward pass, read by the backward pass
+    float* rstd;
+    const void* dy;                   // gradient: [rows, hidden], row pitch lddy
+    int64_t lddy;
+    void* dx;                         // [rows, hidden] contiguous
+    void* dw;                         // [hidden]
+    void* db;                         // [hidden] or null
+    float* partial;                   // [slices, 2, hidden] sums over the rows of a slice
+    int slices;                       // layer_norm_slices
+};
+
+namespace ep {
+cudaError_t launch_layer_norm(const LayerNormArgs& args, cudaStream_t stream);
+cudaError_t launch_layer_norm_backward(const LayerNormArgs& args, cudaStream_t stream);
+int layer_norm_slices(int rows, int hidden, int num_sms);
+}  // namespace ep

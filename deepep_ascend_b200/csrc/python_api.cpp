@@ -3,6 +3,7 @@
 #include <torch/extension.h>
 
 #include "kernels/api.h"
+#include "runtime/block_ops.hpp"
 #include "runtime/coordinator.hpp"
 #include "runtime/elastic_buffer.hpp"
 #include "runtime/layout.hpp"
@@ -961,6 +962,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("swiglu_bwd", &swiglu_bwd, py::arg("d_act"), py::arg("h"), py::arg("valid"), py::arg("row_weight") = py::none());
     m.def("weighted_transpose", &weighted_transpose);
     m.def("dequant_transpose", &dequant_transpose);
+    m.def("route", &route, py::arg("logits"), py::arg("num_topk"), py::arg("softmax"), py::arg("bias"), py::arg("num_groups"), py::arg("num_topk_groups"),
+          py::arg("group_top"), py::arg("renormalize"), py::arg("scale"), py::arg("token_mask"), py::arg("idx_is_64"));
+    m.def("route_backward", &route_backward, py::arg("d_weights"), py::arg("logits"), py::arg("topk_idx"), py::arg("softmax"), py::arg("renormalize"),
+          py::arg("scale"));
+    m.def("layer_norm", &layer_norm, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("eps"));
+    m.def("layer_norm_backward", &layer_norm_backward, py::arg("dy"), py::arg("x"), py::arg("weight"), py::arg("mean"), py::arg("rstd"), py::arg("with_bias"));
     m.def("gemm_error", [](int device) { return gemm_error_flag(device).item<int>(); });
     m.def("get_dispatch_layout", &get_dispatch_layout);
     m.def("per_token_cast_to_fp8", &per_token_cast_to_fp8, py::arg("x"), py::arg("round_scale") = false,

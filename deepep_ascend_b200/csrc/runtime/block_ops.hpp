@@ -1,0 +1,159 @@
+// Tensor front end of the operators around the expert layer: argument checks, result tensors, launches on the current stream.
+#pragma once
+#include <torch/extension.h>
+
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <optional>
+#include <tuple>
+
+#include "../kernels/api.h"
+#include "elastic_buffer.hpp"
+
+namespace ep_host {
+
+inline int device_sms() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; }
+
+inline void router_logits(RouterArgs& a, const at::Tensor& logits) {
+    TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16),
+                "logits must be fp32 or bf16 [tokens, experts] on a GPU");
+    TORCH_CHECK(logits.size(1) >= 1 && logits.size(1) <= EP_MAX_EXPERTS, "between 1 and ", EP_MAX_EXPERTS, " experts");
+    TORCH_CHECK(logits.size(1) == 1 || logits.stride(1) == 1, "rows of the logits must be contiguous");
+    TORCH_CHECK(logits.size(0) <= 1 || logits.stride(0) >= logits.size(1), "rows of the logits must not overlap");
+    TORCH_CHECK(logits.size(0) < (1ll << 31), "too many tokens");
+    a.logits = logits.data_ptr();
+    a.ld = std::max(logits.stride(0), logits.size(1));
+    a.logits_bf16 = logits.scalar_type() == at::kBFloat16;
+    a.num_tokens = static_cast<int>(logits.size(0));
+    a.num_experts = static_cast<int>(logits.size(1));
+}
+
+inline std::tuple<at::Tensor, at::Tensor, at::Tensor> route(const at::Tensor& logits, int64_t num_topk, bool softmax, const std::optional<at::Tensor>& bias,
+                                                            int64_t num_groups, int64_t num_topk_groups, int64_t group_top, bool renormalize, double scale,
+                                                            const std::optional<at::Tensor>& token_mask, bool idx_is_64) {
+    RouterArgs a{};
+    router_logits(a, logits);
+    TORCH_CHECK(num_groups >= 1 && num_groups <= 32 && a.num_experts % num_groups == 0, "the experts must divide into 1 to 32 groups");
+    TORCH_CHECK(num_topk_groups >= 1 && num_topk_groups <= num_groups, "num_topk_groups must be between 1 and num_groups");
+    TORCH_CHECK(num_topk >= 1 && num_topk <= EP_MAX_TOPK && num_topk <= a.num_experts / num_groups * num_topk_groups,
+                "num_topk must be between 1 and ", EP_MAX_TOPK, ", and at most the experts of num_topk_groups groups");
+    TORCH_CHECK(num_groups == 1 || group_top == 1 || (group_top == 2 && a.num_experts / num_groups >= 2), "group_top must be 1 or 2, and at most the experts of a group");
+    const c10::cuda::CUDAGuard guard(logits.device());
+    if (bias.has_value()) {
+        TORCH_CHECK(bias->device() == logits.device() && bias->scalar_type() == at::kFloat && bias->is_contiguous() && bias->dim() == 1 && bias->size(0) == a.num_experts,
+                    "bias must be contiguous fp32 [experts] on the device of the logits");
+        a.bias = bias->data_ptr<float>();
+    }
+    if (token_mask.has_value()) {
+        TORCH_CHECK(token_mask->device() == logits.device() && token_mask->scalar_type() == at::kBool && token_mask->is_contiguous() && token_mask->dim() == 1 &&
+                        token_mask->size(0) == a.num_tokens,
+                    "token_mask must be contiguous bool [tokens] on the device of the logits");
+        a.token_mask = reinterpret_cast<const uint8_t*>(token_mask->data_ptr<bool>());
+    }
+    at::Tensor idx = at::empty({a.num_tokens, num_topk}, logits.options().dtype(idx_is_64 ? at::kLong : at::kInt));
+    at::Tensor weights = at::empty({a.num_tokens, num_topk}, logits.options().dtype(at::kFloat));
+    at::Tensor count = at::empty({a.num_experts}, logits.options().dtype(at::kInt));
+    a.num_topk = static_cast<int>(num_topk);
+    a.softmax = softmax;
+    a.renormalize = renormalize;
+    a.scale = static_cast<float>(scale);
+    a.num_groups = static_cast<int>(num_groups);
+    a.num_topk_groups = static_cast<int>(num_topk_groups);
+    a.group_top = static_cast<int>(num_groups == 1 ? 1 : group_top);
+    a.topk_idx = idx.data_ptr();
+    a.idx_is_64 = idx_is_64;
+    a.topk_weights = weights.data_ptr<float>();
+    a.count = count.data_ptr<int32_t>();
+    cuda_check(ep::launch_route(a, device_sms(), at::cuda::getCurrentCUDAStream()), "routing launch");
+    return {idx, weights, count};
+}
+
+inline at::Tensor route_backward(const at::Tensor& d_weights, const at::Tensor& logits, const at::Tensor& topk_idx, bool softmax, bool renormalize, double scale) {
+    RouterArgs a{};
+    router_logits(a, logits);
+    TORCH_CHECK(topk_idx.device() == logits.device() && topk_idx.dim() == 2 && topk_idx.is_contiguous() && topk_idx.size(0) == a.num_tokens &&
+                    topk_idx.size(1) >= 1 && topk_idx.size(1) <= EP_MAX_TOPK && (topk_idx.scalar_type() == at::kLong || topk_idx.scalar_type() == at::kInt),
+                "topk_idx must be contiguous int64 or int32 [tokens, K] on the device of the logits, K at most ", EP_MAX_TOPK);
+    TORCH_CHECK(d_weights.device() == logits.device() && d_weights.scalar_type() == at::kFloat && d_weights.is_contiguous() && d_weights.sizes() == topk_idx.sizes(),
+                "d_weights must be contiguous fp32 of topk_idx's shape on the device of the logits");
+    const c10::cuda::CUDAGuard guard(logits.device());
+    at::Tensor d_logits = at::empty({a.num_tokens, a.num_experts}, logits.options());
+    a.num_topk = static_cast<int>(topk_idx.size(1));
+    a.softmax = softmax;
+    a.renormalize = renormalize;
+    a.scale = static_cast<float>(scale);
+    a.topk_idx = topk_idx.data_ptr();
+    a.idx_is_64 = topk_idx.scalar_type() == at::kLong;
+    a.d_weights = d_weights.data_ptr<float>();
+    a.d_logits = d_logits.data_ptr();
+    cuda_check(ep::launch_route_backward(a, device_sms(), at::cuda::getCurrentCUDAStream()), "routing gradient launch");
+    return d_logits;
+}
+
+inline bool is_bf16_or_f32(const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
+
+inline void norm_rows(LayerNormArgs& a, const at::Tensor& x, const at::Tensor& weight) {
+    TORCH_CHECK(x.is_cuda() && x.dim() == 2 && is_bf16_or_f32(x), "x must be bf16 or fp32 [rows, hidden] on a GPU");
+    TORCH_CHECK(x.size(1) >= 1 && x.size(1) < (1ll << 24) && x.size(0) < (1ll << 31), "between 1 and 2^24 - 1 channels, fewer than 2^31 rows");
+    TORCH_CHECK(x.size(1) == 1 || x.stride(1) == 1, "rows of x must be contiguous");
+    TORCH_CHECK(weight.device() == x.device() && is_bf16_or_f32(weight) && weight.is_contiguous() && weight.dim() == 1 && weight.size(0) == x.size(1),
+                "weight must be contiguous bf16 or fp32 [hidden] on the device of x");
+    a.x = x.data_ptr();
+    a.ldx = x.stride(0);
+    a.rows = static_cast<int>(x.size(0));
+    a.hidden = static_cast<int>(x.size(1));
+    a.x_bf16 = x.scalar_type() == at::kBFloat16;
+    a.param_bf16 = weight.scalar_type() == at::kBFloat16;
+    a.weight = weight.data_ptr();
+}
+
+inline std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias, double eps) {
+    LayerNormArgs a{};
+    norm_rows(a, x, weight);
+    if (bias.has_value()) {
+        TORCH_CHECK(bias->device() == x.device() && bias->scalar_type() == weight.scalar_type() && bias->is_contiguous() && bias->sizes() == weight.sizes(),
+                    "bias must be like the weight");
+        a.bias = bias->data_ptr();
+    }
+    const c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor y = at::empty({x.size(0), x.size(1)}, x.options());
+    at::Tensor mean = at::empty({x.size(0)}, x.options().dtype(at::kFloat)), rstd = at::empty({x.size(0)}, mean.options());
+    a.eps = static_cast<float>(eps);
+    a.y = y.data_ptr();
+    a.mean = mean.data_ptr<float>();
+    a.rstd = rstd.data_ptr<float>();
+    cuda_check(ep::launch_layer_norm(a, at::cuda::getCurrentCUDAStream()), "layer norm launch");
+    return {y, mean, rstd};
+}
+
+inline std::tuple<at::Tensor, at::Tensor, std::optional<at::Tensor>> layer_norm_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& weight,
+                                                                                         const at::Tensor& mean, const at::Tensor& rstd, bool with_bias) {
+    LayerNormArgs a{};
+    norm_rows(a, x, weight);
+    TORCH_CHECK(dy.device() == x.device() && dy.scalar_type() == x.scalar_type() && dy.sizes() == x.sizes() && (dy.size(1) == 1 || dy.stride(1) == 1),
+                "dy must be like x, with contiguous rows");
+    for (const at::Tensor* t : {&mean, &rstd})
+        TORCH_CHECK(t->device() == x.device() && t->scalar_type() == at::kFloat && t->is_contiguous() && t->dim() == 1 && t->size(0) == x.size(0),
+                    "mean and rstd must be contiguous fp32 [rows] on the device of x");
+    const c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor dx = at::empty({x.size(0), x.size(1)}, x.options()), dw = at::empty({x.size(1)}, weight.options());
+    std::optional<at::Tensor> db;
+    if (with_bias) {
+        db = at::empty({x.size(1)}, weight.options());
+        a.db = db->data_ptr();
+    }
+    a.slices = ep::layer_norm_slices(a.rows, a.hidden, device_sms());
+    at::Tensor partial = at::empty({a.slices, 2, x.size(1)}, mean.options());
+    a.dy = dy.data_ptr();
+    a.lddy = dy.stride(0);
+    a.mean = mean.data_ptr<float>();
+    a.rstd = rstd.data_ptr<float>();
+    a.dx = dx.data_ptr();
+    a.dw = dw.data_ptr();
+    a.partial = partial.data_ptr<float>();
+    cuda_check(ep::launch_layer_norm_backward(a, at::cuda::getCurrentCUDAStream()), "layer norm gradient launch");
+    return {dx, dw, db};
+}
+
+}  // namespace ep_host
