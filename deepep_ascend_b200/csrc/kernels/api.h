@@ -520,3 +520,41 @@ cudaError_t launch_layer_norm(const LayerNormArgs& args, cudaStream_t stream);
 cudaError_t launch_layer_norm_backward(const LayerNormArgs& args, cudaStream_t stream);
 int layer_norm_slices(int rows, int hidden, int num_sms);
 }  // namespace ep
+
+// ------------------------------------------------------------------------------------------------ orthogonalised updates
+struct __half;
+// where a pipeline wait that runs out is reported (as in GemmArgs)
+struct NsReport {
+    int* error;
+    uint64_t* status;                 // or null
+    int status_rank;
+    uint64_t timeout_ns;              // 0: four seconds
+};
+// A stack of `count` matrices [rows, cols] with rows <= cols (newton_schulz.cu states the formulas).  The caller sets the first part.
+struct NsArgs {
+    const void* in;                   // bf16 or fp32: in_lines lines of in_line contiguous elements per matrix
+    int64_t in_stride_matrix, in_stride_line, in_lines;
+    int in_line, in_bf16;
+    int flip;                         // lines are columns of the matrices [rows, cols], not rows
+    void* out;                        // bf16 [count, rows, cols] contiguous, or with out_transposed [count, cols, rows]
+    int out_transposed;
+    int count, rows, cols;
+    float a, b, c, eps;
+    NsReport report;
+    // set by the launcher
+    int ld_x, ld_sq;
+    const __half *x_in, *sq_in;       // [count, rows, ld_x], [count, rows, ld_sq]
+    __half *x_out, *x_lo, *sq_out;
+    float *diag, *coef;               // [count, rows]
+    double* norm_parts;               // [count, num_norm_parts]
+    int num_norm_parts;
+};
+struct NsWorkspace {
+    int64_t bytes, ld_x, ld_sq, norm_parts;
+    int64_t norms, x[2], lo, sq[2], diag[2];        // byte offsets
+};
+
+namespace ep {
+NsWorkspace newton_schulz_workspace(int64_t count, int64_t rows, int64_t cols, int num_sms);
+cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8_t* workspace, int steps, int num_sms, cudaStream_t stream);
+}  // namespace ep

@@ -1247,22 +1247,6 @@ __global__ void __launch_bounds__(kReduceMaxThreads) gemm_reduce_kernel(const Ge
     }
 }
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn get_encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-    });
-    return fn;
-}
-
 // K-major [rows, K] operand, box = box_rows (32, 128, 224 or 256) rows x 128 bytes, 128B swizzle, out-of-range elements read as zero
 bool make_operand_map(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int64_t ld_elems, bool fp8, int box_rows) {
     EncodeTiledFn encode = get_encode_fn();
@@ -1310,6 +1294,18 @@ constexpr int kMaxSplits = 16, kMinSplitBlocks = 4, kSplitCost = 16, kSplitBytes
 constexpr int kStreamMaxRows = 56;
 
 }  // namespace
+
+EncodeTiledFn get_encode_fn() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiledFn>(p);
+    });
+    return fn;
+}
 
 bool gemm_streams_weights(const GemmArgs& g) {
     const int64_t num_m = (g.M + kBlockM - 1) / kBlockM;

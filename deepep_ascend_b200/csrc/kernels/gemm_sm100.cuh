@@ -11,6 +11,13 @@
 #include "ptx.cuh"
 
 namespace ep {
+
+// The driver's encoder of tensor maps, looked up at run time (null where there is none): this library is not linked against libcuda.
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn get_encode_fn();
+
 namespace umma {
 
 // 64-bit shared-memory matrix descriptor, K-major tile of rows x 128 bytes, 128B swizzle:
@@ -52,6 +59,7 @@ __host__ __device__ constexpr uint32_t make_instr_desc(int m, int n, int ab_form
     return (1u << 4) | (a_mn_major ? 1u << 15 : 0u) | (b_mn_major ? 1u << 16 : 0u) | (static_cast<uint32_t>(ab_format) << 7) | (static_cast<uint32_t>(ab_format) << 10) |
            (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
+constexpr int kFormatF16 = 0;    // kind::f16
 constexpr int kFormatBF16 = 1;   // kind::f16
 constexpr int kFormatE4M3 = 0;   // kind::f8f6f4
 

@@ -968,6 +968,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("scale"));
     m.def("layer_norm", &layer_norm, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("eps"));
     m.def("layer_norm_backward", &layer_norm_backward, py::arg("dy"), py::arg("x"), py::arg("weight"), py::arg("mean"), py::arg("rstd"), py::arg("with_bias"));
+    m.def("orthogonalize", [](const at::Tensor& x, int64_t steps, double a, double b, double c, double eps, const std::optional<at::Tensor>& out, int64_t num_sms,
+                              ElasticBufferCore* report_to) {
+        TORCH_CHECK(x.is_cuda(), "matrices must be on a GPU");
+        return orthogonalize(x, steps, a, b, c, eps, out, num_sms, gemm_error_flag(x.get_device()), report_to);
+    }, py::arg("x"), py::arg("steps"), py::arg("a"), py::arg("b"), py::arg("c"), py::arg("eps"), py::arg("out") = py::none(), py::arg("num_sms") = 0,
+          py::arg("report_to") = py::none());
     m.def("gemm_error", [](int device) { return gemm_error_flag(device).item<int>(); });
     m.def("get_dispatch_layout", &get_dispatch_layout);
     m.def("per_token_cast_to_fp8", &per_token_cast_to_fp8, py::arg("x"), py::arg("round_scale") = false,

@@ -156,4 +156,52 @@ inline std::tuple<at::Tensor, at::Tensor, std::optional<at::Tensor>> layer_norm_
     return {dx, dw, db};
 }
 
+// Stack of matrices [count, rows, cols], bf16 or fp32, rows or columns contiguous -> bf16 [count, rows, cols]
+inline at::Tensor orthogonalize(const at::Tensor& x, int64_t steps, double a, double b, double c, double eps, const std::optional<at::Tensor>& out, int64_t num_sms,
+                                at::Tensor error, ElasticBufferCore* report_to) {
+    TORCH_CHECK(x.is_cuda() && x.dim() == 3 && is_bf16_or_f32(x), "matrices must be bf16 or fp32 [count, rows, cols] on a GPU");
+    TORCH_CHECK(steps >= 1, "at least one step");
+    const int64_t count = x.size(0), R = x.size(1), C = x.size(2);
+    TORCH_CHECK(count <= 65535 && R < (1ll << 20) && C < (1ll << 20), "at most 65535 matrices of fewer than 2^20 rows and columns");
+    const bool by_rows = C == 1 ? R == 1 || x.stride(1) != 1 : x.stride(2) == 1;
+    TORCH_CHECK(by_rows || R == 1 || x.stride(1) == 1, "rows or columns must be contiguous");
+    const c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor res = out.has_value() ? *out : at::empty({count, R, C}, x.options().dtype(at::kBFloat16));
+    TORCH_CHECK(res.device() == x.device() && res.scalar_type() == at::kBFloat16 && res.is_contiguous() && res.sizes() == x.sizes(),
+                "out must be contiguous bf16 of the matrices' shape");
+    if (res.numel() == 0) return res;
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(res.data_ptr()) % 16 == 0, "out must start on 16 bytes");
+    NsArgs g{};
+    const bool tall = R > C;
+    g.in = x.data_ptr();
+    g.in_bf16 = x.scalar_type() == at::kBFloat16;
+    g.in_stride_matrix = x.stride(0);
+    g.in_stride_line = by_rows ? x.stride(1) : x.stride(2);
+    g.in_lines = by_rows ? R : C;
+    g.in_line = static_cast<int>(by_rows ? C : R);
+    g.flip = by_rows ? tall : !tall;
+    g.out = res.data_ptr();
+    g.out_transposed = tall;
+    g.count = static_cast<int>(count);
+    g.rows = static_cast<int>(std::min(R, C));
+    g.cols = static_cast<int>(std::max(R, C));
+    g.a = static_cast<float>(a);
+    g.b = static_cast<float>(b);
+    g.c = static_cast<float>(c);
+    g.eps = static_cast<float>(eps);
+    g.report.error = error.data_ptr<int>();
+    if (report_to != nullptr) {
+        report_to->check_status();
+        const RankCtx ctx = report_to->ctx();
+        g.report.status = ctx.status;
+        g.report.status_rank = ctx.rank;
+        g.report.timeout_ns = ctx.timeout_ns;
+    }
+    const int sms = num_sms > 0 ? static_cast<int>(num_sms) : device_sms();
+    const NsWorkspace w = ep::newton_schulz_workspace(g.count, g.rows, g.cols, sms);
+    at::Tensor workspace = at::empty({w.bytes}, x.options().dtype(at::kByte));
+    cuda_check(ep::launch_newton_schulz(g, w, workspace.data_ptr<uint8_t>(), static_cast<int>(steps), sms, at::cuda::getCurrentCUDAStream()), "orthogonalisation launch");
+    return res;
+}
+
 }  // namespace ep_host

@@ -1,0 +1,176 @@
+"""Orthogonalised updates: the kernels and the PyTorch statement against the Newton-Schulz steps in 64 bits, and what they are for."""
+import pytest
+import torch
+
+from deepep_ascend_b200.ops.muon import COEFFICIENTS, orthogonalize, orthogonalize_ref
+
+DEVICES = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def _exact(x, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+    a, b, c = coefficients
+    X = x.double()
+    X = X / (torch.linalg.matrix_norm(X, keepdim=True) + eps)
+    for _ in range(steps):
+        if X.shape[-2] <= X.shape[-1]:
+            A = X @ X.mT
+            X = a * X + (b * A + c * A @ A) @ X
+        else:
+            A = X.mT @ X
+            X = a * X + X @ (b * A + c * A @ A)
+    return X
+
+
+def _matrix(kind, count, rows, cols, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(count, rows, cols, generator=g)
+    if kind == 'strong directions':           # momentum: a few directions far above the noise
+        x = 0.1 * x + torch.randn(count, rows, 8, generator=g) @ (torch.randn(count, 8, cols, generator=g) * torch.logspace(0, -1, 8)[:, None])
+    elif kind == 'one direction':
+        x = 0.01 * x + torch.randn(count, rows, 1, generator=g) @ torch.randn(count, 1, cols, generator=g)
+    elif kind == 'rows of all sizes':
+        x = x * torch.logspace(0, -3, rows)[torch.randperm(rows, generator=g)][:, None]
+    return 1e-3 * x
+
+
+def _error(got, want):
+    """Per matrix: 2-norm of the difference over that of the result."""
+    return (torch.linalg.matrix_norm(got.double().cpu() - want.cpu()) / torch.linalg.matrix_norm(want.cpu())).max().item()
+
+
+# Rounding the result to bf16 is off by 1.7e-3 of its norm.  Simulated in 64 bits, the steps' own roundings add at most 1e-3 to that for matrices of 64 and
+# more rows (2.2e-3 where one direction holds nearly all of the norm); matrices of fewer rows are held to the same.
+BOUND = {'normal': 2.5e-3, 'strong directions': 2.7e-3, 'one direction': 3.5e-3, 'rows of all sizes': 2.5e-3}
+
+SHAPES = [(1, 64, 64), (2, 128, 256), (1, 129, 130), (3, 77, 301), (2, 300, 77), (1, 256, 1024), (1, 1000, 257), (1, 511, 513), (2, 640, 384), (5, 65, 1001), (1, 31, 2000),
+          (1, 2056, 100)]
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('kind', sorted(BOUND))
+@pytest.mark.parametrize('count,rows,cols', SHAPES)
+def test_against_64_bits(count, rows, cols, kind, device):
+    for dtype in (BF16, F32):
+        x = _matrix(kind, count, rows, cols, rows + cols).to(dtype)
+        got = orthogonalize(x.to(device))
+        assert got.dtype == BF16 and got.shape == x.shape and got.is_contiguous()
+        assert _error(got, _exact(x)) < BOUND[kind]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('count,rows,cols', [(1, 1024, 4096), (2, 2000, 1100), (9, 520, 776), (1, 264, 7168), (40, 128, 160)])
+def test_more_tiles_than_one_wave_and_few_sms(count, rows, cols):
+    x = _matrix('strong directions', count, rows, cols).bfloat16().cuda()
+    want = _exact(x)
+    got = orthogonalize(x)
+    assert _error(got, want) < BOUND['strong directions']
+    assert torch.equal(orthogonalize(x), got)                  # the same bits on every run
+    for sms in (1, 7):
+        assert _error(orthogonalize(x, num_sms=sms), want) < BOUND['strong directions']
+    # each matrix by itself: the others change nothing but the order of a sum
+    for i in range(0, count, 3):
+        assert _error(orthogonalize(x[i]), want[i]) < BOUND['strong directions']
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_tiny_matrices(device):
+    for shape in ((1, 1, 1), (3, 1, 9), (2, 9, 1), (1, 2, 2), (4, 3, 17), (2, 8, 5)):
+        x = _matrix('normal', *shape).to(device)
+        assert _error(orthogonalize(x), _exact(x)) < 3e-3
+    assert orthogonalize(torch.zeros(0, 4, 5, device=device)).shape == (0, 4, 5)
+    assert orthogonalize(torch.zeros(2, 0, 5, device=device)).shape == (2, 0, 5)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_scales_zeros_and_bad_matrices(device):
+    x = _matrix('normal', 1, 96, 200)
+    want = _exact(x, eps=0.0)
+    for scale in (1e-25, 1e-10, 1.0, 1e12, 1e16):            # the norm divides out (and is no square that leaves the range of its type)
+        if device == 'cuda' or 1e-12 < scale < 1e14:
+            assert _error(orthogonalize((x * scale).to(device), eps=0.0), want) < BOUND['normal']
+    # eps decides where the norm is smaller
+    assert _error(orthogonalize((x * 1e-9).to(device), eps=1e-3), _exact(x * 1e-9, eps=1e-3)) < BOUND['normal']
+    stack = torch.stack([x[0], torch.zeros(96, 200), x[0], x[0]]).to(device)
+    stack[2, 3, 5] = float('nan')
+    got = orthogonalize(stack)
+    assert _error(got[:1], _exact(x)) < BOUND['normal'] and not got[1].any()
+    assert torch.isnan(got[2]).all() and torch.equal(got[3], got[0])
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_strides_shapes_and_out(device):
+    wide = _matrix('strong directions', 3, 150, 310).to(device)
+    for x in (wide, wide[:, 3:140, 5:300], wide.mT, wide[::2], wide[:, ::2], wide[:1].expand(2, 150, 310), wide[0], wide[:, :, ::2], wide.transpose(0, 1)[:100],
+              wide.view(3, 1, 150, 310).expand(3, 2, 150, 310), wide[:, 3:140, 5:300].mT):
+        got = orthogonalize(x)
+        assert got.shape == x.shape and got.is_contiguous()
+        assert _error(got, _exact(x)) < 5e-3
+        out = torch.empty(x.shape, dtype=BF16, device=device)
+        assert orthogonalize(x, out=out) is out and torch.equal(out, got)
+    own = wide.bfloat16()                                     # in place
+    want = orthogonalize(own)
+    assert orthogonalize(own, out=own) is own and torch.equal(own, want)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_other_steps_and_coefficients(device):
+    x = _matrix('normal', 2, 100, 260)
+    for steps, coefficients in ((1, COEFFICIENTS), (2, COEFFICIENTS), (8, COEFFICIENTS), (12, (1.875, -1.25, 0.375)), (3, (1.5, -0.5, 0.0))):
+        assert _error(orthogonalize(x.to(device), steps, coefficients), _exact(x, steps, coefficients)) < 2.7e-3
+    # what it is for: with enough steps of the fifth-order polynomial whose fixed point is one, rows are orthonormal
+    got = orthogonalize(x.to(device), 25, (1.875, -1.25, 0.375)).float().cpu()
+    assert (got @ got.mT - torch.eye(100)).abs().max() < 0.02
+
+
+@pytest.mark.gpu
+def test_streams_and_graphs():
+    x = _matrix('strong directions', 2, 200, 520).cuda()
+    want = orthogonalize(x)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        got = orthogonalize(x)
+    torch.cuda.current_stream().wait_stream(stream)
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = orthogonalize(x)
+    x.copy_(_matrix('strong directions', 2, 200, 520, seed=5))
+    graph.replay()
+    assert torch.equal(out, orthogonalize(x))
+
+
+@pytest.mark.gpu
+def test_waits_report_to_the_buffer():
+    """A buffer's limit and status block serve the products, which end within it."""
+    from deepep_ascend_b200 import ElasticBuffer, _native
+    buf = ElasticBuffer(None, num_max_tokens_per_rank=16, hidden=256, num_topk=2)
+    try:
+        x = _matrix('normal', 1, 128, 256).cuda()
+        assert torch.equal(orthogonalize(x, buffer=buf), orthogonalize(x))
+        torch.cuda.synchronize()
+        buf.check_status()
+        assert _native.load().gemm_error(0) == 0
+    finally:
+        buf.destroy()
+
+
+@pytest.mark.gpu
+def test_refusals():
+    x = torch.randn(2, 64, 64, device='cuda')
+    for bad in (x.half(), x.double()):
+        with pytest.raises(RuntimeError):
+            orthogonalize(bad)
+    for kw in (dict(steps=0), dict(out=torch.empty_like(x)), dict(out=torch.empty(2, 64, 64, dtype=BF16)), dict(out=torch.empty(2, 64, 65, dtype=BF16, device='cuda')[:, :, :64])):
+        with pytest.raises(RuntimeError):
+            orthogonalize(x, **kw)
+    with pytest.raises(ValueError):
+        orthogonalize(x[0, 0])
+
+
+def test_refusals_of_the_statement():
+    with pytest.raises(ValueError):
+        orthogonalize(torch.randn(4))
+    with pytest.raises(ValueError):
+        orthogonalize_ref(torch.randn(4, 4), steps=0)
