@@ -511,14 +511,21 @@ struct LayerNormArgs {
     void* dx;                         // [rows, hidden] contiguous
     void* dw;                         // [hidden]
     void* db;                         // [hidden] or null
-    float* partial;                   // [slices, 2, hidden] sums over the rows of a slice
-    int slices;                       // layer_norm_slices
+    float* partial;                   // [slices, 1 or 2 (with db), hidden] sums over the rows of a slice
+    int slices;                       // set by the launcher
+};
+struct NormShape {
+    int vec, values;                  // values of an access, values of a row that a thread has (0: the row stays in memory)
+    int warp_rows;                    // a row belongs to a warp, not to a CTA
+    int threads, rows_per_cta, ctas;  // (rows_per_cta: warps of a CTA that have rows of their own)
+    int smem;                         // bytes
 };
 
 namespace ep {
-cudaError_t launch_layer_norm(const LayerNormArgs& args, cudaStream_t stream);
-cudaError_t launch_layer_norm_backward(const LayerNormArgs& args, cudaStream_t stream);
-int layer_norm_slices(int rows, int hidden, int num_sms);
+cudaError_t launch_layer_norm(const LayerNormArgs& args, int num_sms, cudaStream_t stream);
+// how the rows are laid out on threads; the gradient's sums have a slice per CTA
+NormShape layer_norm_backward_shape(const LayerNormArgs& args, int num_sms);
+cudaError_t launch_layer_norm_backward(const LayerNormArgs& args, const NormShape& shape, cudaStream_t stream);
 }  // namespace ep
 
 // ------------------------------------------------------------------------------------------------ orthogonalised updates

@@ -123,7 +123,7 @@ inline std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tenso
     a.y = y.data_ptr();
     a.mean = mean.data_ptr<float>();
     a.rstd = rstd.data_ptr<float>();
-    cuda_check(ep::launch_layer_norm(a, at::cuda::getCurrentCUDAStream()), "layer norm launch");
+    cuda_check(ep::launch_layer_norm(a, device_sms(), at::cuda::getCurrentCUDAStream()), "layer norm launch");
     return {y, mean, rstd};
 }
 
@@ -143,16 +143,16 @@ inline std::tuple<at::Tensor, at::Tensor, std::optional<at::Tensor>> layer_norm_
         db = at::empty({x.size(1)}, weight.options());
         a.db = db->data_ptr();
     }
-    a.slices = ep::layer_norm_slices(a.rows, a.hidden, device_sms());
-    at::Tensor partial = at::empty({a.slices, 2, x.size(1)}, mean.options());
     a.dy = dy.data_ptr();
     a.lddy = dy.stride(0);
+    const NormShape shape = ep::layer_norm_backward_shape(a, device_sms());
+    at::Tensor partial = at::empty({shape.ctas, with_bias ? 2 : 1, x.size(1)}, mean.options());
     a.mean = mean.data_ptr<float>();
     a.rstd = rstd.data_ptr<float>();
     a.dx = dx.data_ptr();
     a.dw = dw.data_ptr();
     a.partial = partial.data_ptr<float>();
-    cuda_check(ep::launch_layer_norm_backward(a, at::cuda::getCurrentCUDAStream()), "layer norm gradient launch");
+    cuda_check(ep::launch_layer_norm_backward(a, shape, at::cuda::getCurrentCUDAStream()), "layer norm gradient launch");
     return {dx, dw, db};
 }
 
