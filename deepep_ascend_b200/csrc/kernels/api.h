@@ -552,16 +552,19 @@ struct NsArgs {
     int ld_x, ld_sq;
     const __half *x_in, *sq_in;       // [count, rows, ld_x], [count, rows, ld_sq]
     __half *x_out, *x_lo, *sq_out;
-    float *diag, *coef;               // [count, rows]
+    float *diag, *coef;               // [count, ld_sq]
+    float* parts;                     // [k_splits, tiles, 128, 128] sums of X X^T over parts of K
+    int k_splits;
     double* norm_parts;               // [count, num_norm_parts]
     int num_norm_parts;
 };
 struct NsWorkspace {
     int64_t bytes, ld_x, ld_sq, norm_parts;
-    int64_t norms, x[2], lo, sq[2], diag[2];        // byte offsets
+    int k_splits;
+    int64_t norms, x[2], lo, sq[2], diag[2], parts;        // byte offsets
 };
 
 namespace ep {
-NsWorkspace newton_schulz_workspace(int64_t count, int64_t rows, int64_t cols, int num_sms);
+NsWorkspace newton_schulz_workspace(const NsArgs& args, int num_sms);      // (sizes alone are read)
 cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8_t* workspace, int steps, int num_sms, cudaStream_t stream);
 }  // namespace ep

@@ -25,15 +25,18 @@ namespace ep {
 namespace {
 
 constexpr int kTileM = 128, kTileK = 64;                       // one 128-byte row of fp16 per stage
-constexpr int kNsThreads = 192;                                // TMA warp, MMA warp, four epilogue warps
+constexpr int kEpiWarps = 8, kNsThreads = 64 + kEpiWarps * 32; // TMA warp, MMA warp, eight epilogue warps (two per 32 tile rows, half of the columns each)
 constexpr float kUnitX = 4096.f, kUnitLo = 2048.f, kUnitA = 1024.f;      // stored = value * unit; lo: unit of hi * kUnitLo
+constexpr int kStagingBytes = 32 * 128;                        // per epilogue warp: 32 x 32 sums, later the same values in fp16 transposed
 constexpr int kTransposePitch = 72;                            // bytes of a staged column of 32 fp16 values
-constexpr int kEpiWarpBytes = 32 * 128 + 32 * kTransposePitch; // 32 x 32 sums, and the same tile transposed
 constexpr uint64_t kNsWaitLimitNs = 4ull * 1000 * 1000 * 1000; // when the caller gives no limit
 
-__host__ __device__ constexpr int ns_stages(int block_n) { return block_n == 256 ? 4 : 5; }
+__host__ __device__ constexpr int ns_stages(int block_n) { return block_n == 256 ? 4 : 6; }
 __host__ __device__ constexpr int ns_stage_bytes(int block_n) { return (kTileM + block_n) * 128; }
-__host__ __device__ constexpr int ns_smem_bytes(int block_n) { return ns_stages(block_n) * ns_stage_bytes(block_n) + 1024 + 4 * kEpiWarpBytes; }
+__host__ __device__ constexpr int ns_smem_bytes(int block_n) { return ns_stages(block_n) * ns_stage_bytes(block_n) + 1024 + kEpiWarps * kStagingBytes; }
+
+// What a kernel makes of its sums
+enum { kGram = 0, kPoly = 1, kUpdate = 2, kGramPart = 3 };
 
 struct NsSmem {
     uint64_t full[8], empty[8], acc_full[2], acc_empty[2], quiet;
@@ -121,7 +124,7 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ void unpack_half(const int4& v, float (&f)[8]) {
+__device__ __forceinline__ void unpack_half(const uint4& v, float (&f)[8]) {
     const __half2* h = reinterpret_cast<const __half2*>(&v);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -131,16 +134,88 @@ __device__ __forceinline__ void unpack_half(const int4& v, float (&f)[8]) {
     }
 }
 
-// kMode 0: O, d = X X^T without its diagonal, and the diagonal.  1: B, coef = b A + c A A without its diagonal, and a + the diagonal.
-// 2: X <- coef X + B X.
+// 32 x 32 values of a tile lie on a warp as four rows (i * 8 + lane / 4) of eight neighbouring columns ((lane & 3) * 8) per lane: rows are read and written in
+// whole sectors.
+struct Block {
+    int row0, col0;
+    __device__ __forceinline__ int row(int i) const { return row0 + i * 8 + ((threadIdx.x & 31) >> 2); }
+    __device__ __forceinline__ int col() const { return col0 + (threadIdx.x & 3) * 8; }
+};
+// From one row per lane, as tensor memory gives them
+__device__ __forceinline__ void spread(uint8_t* staging, const uint32_t (&r)[32], float (&v)[4][8]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int p = 0; p < 8; ++p)
+        *reinterpret_cast<uint4*>(staging + lane * 128 + ((p ^ (lane & 7)) * 16)) = make_uint4(r[4 * p], r[4 * p + 1], r[4 * p + 2], r[4 * p + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int lr = i * 8 + (lane >> 2), p = (lane & 3) * 2;
+        const float4 a = *reinterpret_cast<const float4*>(staging + lr * 128 + ((p ^ (lr & 7)) * 16));
+        const float4 b = *reinterpret_cast<const float4*>(staging + lr * 128 + (((p + 1) ^ (lr & 7)) * 16));
+        v[i][0] = a.x, v[i][1] = a.y, v[i][2] = a.z, v[i][3] = a.w;
+        v[i][4] = b.x, v[i][5] = b.y, v[i][6] = b.z, v[i][7] = b.w;
+    }
+    __syncwarp();
+}
+// 16-bit values of the block (four words per row) transposed: `write(row, col, four values)` of the mirror image, eight lanes per row of 32
+template <class Write>
+__device__ __forceinline__ void transposed(uint8_t* staging, const uint32_t (&o)[4][4], const Block& b, Write write) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint16_t*>(staging + ((lane & 3) * 8 + j) * kTransposePitch + (i * 8 + (lane >> 2)) * 2) = static_cast<uint16_t>(o[i][j >> 1] >> (16 * (j & 1)));
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int lr = i * 4 + (lane >> 3), lc = (lane & 7) * 4;
+        write(b.col0 + lr, b.row0 + lc, *reinterpret_cast<const uint2*>(staging + lr * kTransposePitch + lc * 2));
+    }
+    __syncwarp();
+}
+// A symmetric result's block, and its mirror image
+__device__ __forceinline__ void store_symmetric(const NsArgs& g, uint8_t* staging, int matrix, const Block& b, const float (&v)[4][8], bool mirror) {
+    __half* out = g.sq_out + static_cast<int64_t>(matrix) * g.rows * g.ld_sq;
+    uint32_t o[4][4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][j] = pack_half(v[i][2 * j], v[i][2 * j + 1]);
+        if (b.row(i) < g.rows && b.col() < g.ld_sq)
+            *reinterpret_cast<uint4*>(out + static_cast<int64_t>(b.row(i)) * g.ld_sq + b.col()) = make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
+    }
+    if (mirror)
+        transposed(staging, o, b, [&](int row, int col, const uint2& four) {
+            if (row < g.rows && col < g.ld_sq) *reinterpret_cast<uint2*>(out + static_cast<int64_t>(row) * g.ld_sq + col) = four;
+        });
+}
+// X X^T in kUnitX^2 -> O and the diagonal.  (Columns past the end are sums of zeros.)
+__device__ __forceinline__ void finish_gram(const NsArgs& g, uint8_t* staging, int matrix, const Block& b, float (&v)[4][8], bool mirror) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (b.row(i) == b.col() + j) {
+                if (b.row(i) < g.rows) g.diag[static_cast<int64_t>(matrix) * g.ld_sq + b.row(i)] = v[i][j] * (1.f / (kUnitX * kUnitX));
+                v[i][j] = 0.f;
+            }
+            v[i][j] *= kUnitA / (kUnitX * kUnitX);
+        }
+    store_symmetric(g, staging, matrix, b, v, mirror);
+}
+
+// kGram: O, d = X X^T without its diagonal, and the diagonal; kGramPart: its sums over a part of K.  kPoly: B, coef = b A + c A A without its diagonal, and a + the
+// diagonal.  kUpdate: X <- coef X + B X.
 template <int kMode, int kBlockN>
 __global__ void __launch_bounds__(kNsThreads, 1)
 ns_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ NsArgs g) {
     extern __shared__ __align__(1024) uint8_t smem[];
     constexpr int kStages = ns_stages(kBlockN), kBytesA = kTileM * 128, kBytesB = kBlockN * 128;
-    constexpr bool kSymmetric = kMode != 2;
+    constexpr bool kSymmetric = kMode != kUpdate;
     constexpr int kTmemColumns = 2 * kBlockN;
-    constexpr uint32_t kIdesc = umma::make_instr_desc(kTileM, kBlockN, umma::kFormatF16, false, kMode == 2);
+    constexpr uint32_t kIdesc = umma::make_instr_desc(kTileM, kBlockN, umma::kFormatF16, false, kMode == kUpdate);
     uint8_t* s_a = smem;
     uint8_t* s_b = smem + kStages * kBytesA;
     NsSmem* sm = reinterpret_cast<NsSmem*>(smem + kStages * (kBytesA + kBytesB));
@@ -148,8 +223,12 @@ ns_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int num_m = (g.rows + kTileM - 1) / kTileM;
     const int per_matrix = kSymmetric ? symmetric_tiles<kBlockN>(g.rows) : num_m * ((g.cols + kBlockN - 1) / kBlockN);
-    const int num_items = per_matrix * g.count;
-    const int num_k = ((kMode == 0 ? g.cols : g.rows) + kTileK - 1) / kTileK;
+    const int num_tiles = per_matrix * g.count, num_items = kMode == kGramPart ? num_tiles * g.k_splits : num_tiles;
+    const int num_k = ((kMode == kGram || kMode == kGramPart ? g.cols : g.rows) + kTileK - 1) / kTileK;
+    // the K blocks of an item: all, or those of its part
+    auto k_begin = [&](int item) { return kMode == kGramPart ? num_k * (item / num_tiles) / g.k_splits : 0; };
+    auto k_end = [&](int item) { return kMode == kGramPart ? num_k * (item / num_tiles + 1) / g.k_splits : num_k; };
+    auto tile_of = [&](int item) { return ns_tile<kBlockN, kSymmetric>(kMode == kGramPart ? item % num_tiles : item, per_matrix, num_m); };
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < kStages; ++i) {
@@ -158,7 +237,7 @@ ns_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         }
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&sm->acc_full[i], 1);
-            ptx::mbar_init(&sm->acc_empty[i], 4);
+            ptx::mbar_init(&sm->acc_empty[i], kEpiWarps);
         }
         ptx::mbar_init(&sm->quiet, 1);
         sm->failed = 0;
@@ -182,13 +261,14 @@ ns_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             int loads = 0;
             bool ok = true;
             for (int item = blockIdx.x; item < num_items && ok; item += gridDim.x) {
-                const NsTile t = ns_tile<kBlockN, kSymmetric>(item, per_matrix, num_m);
-                for (int kb = 0; kb < num_k; ++kb) {
+                const NsTile t = tile_of(item);
+                const int kb1 = k_end(item);
+                for (int kb = k_begin(item); kb < kb1; ++kb) {
                     ok = ns_wait(&sm->empty[p.stage], p.phase ^ 1, sm, g.report, 1);
                     if (!ok) break;
                     ptx::mbar_arrive_expect_tx(&sm->full[p.stage], kBytesA + kBytesB);
                     umma::tma_load_3d(s_a + p.stage * kBytesA, &map_a, kb * kTileK, t.m * kTileM, t.g, &sm->full[p.stage]);
-                    if constexpr (kMode == 2) {
+                    if constexpr (kMode == kUpdate) {
 #pragma unroll
                         for (int i = 0; i < kBlockN / 64; ++i)
                             umma::tma_load_3d(s_b + p.stage * kBytesB + i * umma::kMnChunkBytes, &map_b, t.n * kBlockN + i * 64, kb * kTileK, t.g, &sm->full[p.stage]);
@@ -218,17 +298,18 @@ ns_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
                 ok = ns_wait(&sm->acc_empty[acc], acc_phase ^ 1, sm, g.report, 2);
                 if (!ok) break;
                 umma::fence_after_thread_sync();
-                for (int kb = 0; kb < num_k; ++kb) {
+                const int kb0 = k_begin(item), kb1 = k_end(item);
+                for (int kb = kb0; kb < kb1; ++kb) {
                     ok = ns_wait(&sm->full[p.stage], p.phase, sm, g.report, 4);
                     if (!ok) break;
                     umma::fence_after_thread_sync();
                     const uint64_t desc_a = umma::make_smem_desc_sw128(s_a + p.stage * kBytesA);
-                    const uint64_t desc_b = kMode == 2 ? umma::make_smem_desc_mn_sw128(s_b + p.stage * kBytesB) : umma::make_smem_desc_sw128(s_b + p.stage * kBytesB);
-                    constexpr int kStepB = kMode == 2 ? 16 * 128 : 32;       // 16 elements of K
+                    const uint64_t desc_b = kMode == kUpdate ? umma::make_smem_desc_mn_sw128(s_b + p.stage * kBytesB) : umma::make_smem_desc_sw128(s_b + p.stage * kBytesB);
+                    constexpr int kStepB = kMode == kUpdate ? 16 * 128 : 32;       // 16 elements of K
 #pragma unroll
                     for (int k = 0; k < kTileK / 16; ++k)
                         umma::mma_ss<false>(tmem_base + acc * kBlockN, umma::advance_desc_k(desc_a, k * 32), umma::advance_desc_k(desc_b, k * kStepB), kIdesc,
-                                            kb != 0 || k != 0);
+                                            kb != kb0 || k != 0);
                     umma::mma_commit(&sm->empty[p.stage]);
                     p.advance();
                 }
@@ -243,137 +324,158 @@ ns_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
             }
         }
     } else {
-        const int quad = warp & 3;
-        uint8_t* s_sum = s_epi + quad * kEpiWarpBytes;
-        uint8_t* s_t = s_sum + 32 * 128;
+        constexpr int kChunks = kBlockN / 2 / 32;          // 32-column blocks of a warp
+        const int quad = warp & 3, half = (warp - 2) >> 2;
+        uint8_t* staging = s_epi + (warp - 2) * kStagingBytes;
         int acc = 0;
         uint32_t acc_phase = 0;
         for (int item = blockIdx.x; item < num_items; item += gridDim.x) {
-            const NsTile t = ns_tile<kBlockN, kSymmetric>(item, per_matrix, num_m);
+            const NsTile t = tile_of(item);
+            const int64_t sq = static_cast<int64_t>(t.g) * g.rows * g.ld_sq, wide = static_cast<int64_t>(t.g) * g.rows * g.ld_x, diag = static_cast<int64_t>(t.g) * g.ld_sq;
+            const int width = kSymmetric ? g.ld_sq : g.ld_x;
+            auto block = [&](int c) { return Block{t.m * kTileM + quad * 32, t.n * kBlockN + half * (kBlockN / 2) + c * 32}; };
+            auto empty = [&](const Block& b) { return b.row0 >= g.rows || b.col0 >= width; };
+            // What the sums are combined with is requested a block ahead, that of the first one before the sums are there: waiting for it block by block
+            // took ten times as long as the products of a tile of 256 K.
+            uint4 old[2][4], low[2][4];
+            float row_value[4], col_value[2][8];
+            auto request = [&](int c, uint4 (&o)[4], uint4 (&l)[4], float (&cv)[8]) {
+                const Block b = block(c);
+                if (empty(b)) return;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool in = b.row(i) < g.rows && b.col() < width;
+                    o[i] = l[i] = make_uint4(0, 0, 0, 0);
+                    if constexpr (kMode == kPoly) {
+                        if (in) o[i] = *reinterpret_cast<const uint4*>(g.sq_in + sq + static_cast<int64_t>(b.row(i)) * g.ld_sq + b.col());
+                    } else if constexpr (kMode == kUpdate) {
+                        if (in) {
+                            const int64_t at = wide + static_cast<int64_t>(b.row(i)) * g.ld_x + b.col();
+                            o[i] = *reinterpret_cast<const uint4*>(g.x_in + at);
+                            l[i] = *reinterpret_cast<const uint4*>(g.x_lo + at);
+                        }
+                    }
+                }
+                if constexpr (kMode == kPoly) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) cv[j] = b.col() + j < g.rows ? g.diag[diag + b.col() + j] : 0.f;
+                }
+            };
+            if constexpr (kMode == kPoly || kMode == kUpdate) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int row = block(0).row(i);
+                    row_value[i] = row >= g.rows ? 0.f : kMode == kPoly ? g.diag[diag + row] : g.coef[diag + row];
+                }
+                request(0, old[0], low[0], col_value[0]);
+            }
             const bool ok = ns_wait(&sm->acc_full[acc], acc_phase, sm, g.report, 5);
             if (!__all_sync(0xffffffffu, ok)) break;
             umma::fence_after_thread_sync();
-            const int row0 = t.m * kTileM + quad * 32;
-            const int64_t sq = static_cast<int64_t>(t.g) * g.rows * g.ld_sq, wide = static_cast<int64_t>(t.g) * g.rows * g.ld_x, diag = static_cast<int64_t>(t.g) * g.rows;
-            const int width = kSymmetric ? g.ld_sq : g.ld_x;
-#pragma unroll 1
-            for (int c = 0; c < kBlockN / 32; ++c) {
-                const int col0 = t.n * kBlockN + c * 32;
-                if (col0 >= width || row0 >= g.rows) break;
-                uint32_t r[32];
-                umma::tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * kBlockN + c * 32, r);
-                umma::tmem_ld_wait();
-                // one row per lane -> four lanes with eight columns each per row
 #pragma unroll
-                for (int v = 0; v < 8; ++v)
-                    *reinterpret_cast<uint4*>(s_sum + lane * 128 + ((v ^ (lane & 7)) * 16)) = make_uint4(r[4 * v], r[4 * v + 1], r[4 * v + 2], r[4 * v + 3]);
-                __syncwarp();
+            for (int c = 0; c < kChunks; ++c) {
+                const Block b = block(c);
+                if (kMode != kGramPart && empty(b)) break;
+                if constexpr (kMode == kPoly || kMode == kUpdate)
+                    if (c + 1 < kChunks) request(c + 1, old[(c + 1) & 1], low[(c + 1) & 1], col_value[(c + 1) & 1]);
+                float v[4][8];
+                {
+                    uint32_t r[32];
+                    umma::tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * kBlockN + half * (kBlockN / 2) + c * 32, r);
+                    umma::tmem_ld_wait();
+                    spread(staging, r, v);
+                }
+                if constexpr (kMode == kGram) {
+                    finish_gram(g, staging, t.g, b, v, t.mirror);
+                } else if constexpr (kMode == kGramPart) {
+                    // [part][tile][128][kBlockN]
+                    float* part = g.parts + static_cast<int64_t>(item) * kTileM * kBlockN + (b.col0 - t.n * kBlockN + (lane & 3) * 8);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int lr = i * 8 + (lane >> 2), lc = (lane & 3) * 8, row = row0 + lr, col = col0 + lc;
-                    const float4 s0 = *reinterpret_cast<const float4*>(s_sum + lr * 128 + ((((lc >> 2)) ^ (lr & 7)) * 16));
-                    const float4 s1 = *reinterpret_cast<const float4*>(s_sum + lr * 128 + ((((lc >> 2) + 1) ^ (lr & 7)) * 16));
-                    float v[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-                    const bool in = row < g.rows && col < width;
-                    int4 out = make_int4(0, 0, 0, 0);
-                    uint32_t* o = reinterpret_cast<uint32_t*>(&out);
-                    if constexpr (kMode == 0) {
+                    for (int i = 0; i < 4; ++i) {
+                        float* p = part + (b.row(i) - t.m * kTileM) * kBlockN;
+                        *reinterpret_cast<float4*>(p) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+                        *reinterpret_cast<float4*>(p + 4) = make_float4(v[i][4], v[i][5], v[i][6], v[i][7]);
+                    }
+                } else if constexpr (kMode == kPoly) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float f[8];
+                        unpack_half(old[c & 1][i], f);
+                        const float di = row_value[i];
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            if (in && row == col + j) {
-                                g.diag[diag + row] = v[j] * (1.f / (kUnitX * kUnitX));
-                                v[j] = 0.f;
+                            if (b.row(i) == b.col() + j) {
+                                if (b.row(i) < g.rows) g.coef[diag + b.row(i)] = g.a + g.b * di + g.c * (di * di + v[i][j] * (1.f / (kUnitA * kUnitA)));
+                                v[i][j] = 0.f;
+                            } else {        // (B in kUnitA; O O in kUnitA^2)
+                                v[i][j] = (g.b + g.c * (di + col_value[c & 1][j])) * f[j] + g.c * (1.f / kUnitA) * v[i][j];
                             }
-                            v[j] *= kUnitA / (kUnitX * kUnitX);
-                        }
-                    } else if constexpr (kMode == 1) {
-                        if (in) {
-                            float old[8];
-                            unpack_half(*reinterpret_cast<const int4*>(g.sq_in + sq + static_cast<int64_t>(row) * g.ld_sq + col), old);
-                            const float di = g.diag[diag + row];
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) {
-                                const float dj = col + j < g.rows ? g.diag[diag + col + j] : 0.f;
-                                // (B in kUnitA; O O in kUnitA^2)
-                                if (row == col + j) {
-                                    g.coef[diag + row] = g.a + g.b * di + g.c * (di * di + v[j] * (1.f / (kUnitA * kUnitA)));
-                                    v[j] = 0.f;
-                                } else {
-                                    v[j] = (g.b + g.c * (di + dj)) * old[j] + g.c * (1.f / kUnitA) * v[j];
-                                }
-                            }
-                        }
-                    } else {
-                        if (in) {
-                            const int64_t at = wide + static_cast<int64_t>(row) * g.ld_x + col;
-                            float hi[8], lo[8];
-                            unpack_half(*reinterpret_cast<const int4*>(g.x_in + at), hi);
-                            unpack_half(*reinterpret_cast<const int4*>(g.x_lo + at), lo);
-                            const float k = g.coef[diag + row];
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) v[j] = k * (hi[j] + lo[j] * (1.f / kUnitLo)) + v[j] * (1.f / kUnitA);     // in kUnitX
                         }
                     }
-                    if (kMode != 2 || g.out == nullptr) {
+                    store_symmetric(g, staging, t.g, b, v, t.mirror);
+                } else {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) o[j] = pack_half(v[2 * j], v[2 * j + 1]);
-                        if (in) *reinterpret_cast<int4*>(kMode == 2 ? g.x_out + wide + static_cast<int64_t>(row) * g.ld_x + col
-                                                                     : g.sq_out + sq + static_cast<int64_t>(row) * g.ld_sq + col) = out;
-                        if (kMode == 2 && in) {
-                            float hi[8];
-                            unpack_half(out, hi);
+                    for (int i = 0; i < 4; ++i) {
+                        float hi[8], lo[8];
+                        unpack_half(old[c & 1][i], hi);
+                        unpack_half(low[c & 1][i], lo);
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) o[j] = pack_half((v[2 * j] - hi[2 * j]) * kUnitLo, (v[2 * j + 1] - hi[2 * j + 1]) * kUnitLo);
-                            *reinterpret_cast<int4*>(g.x_lo + wide + static_cast<int64_t>(row) * g.ld_x + col) = out;
+                        for (int j = 0; j < 8; ++j) v[i][j] = row_value[i] * (hi[j] + lo[j] * (1.f / kUnitLo)) + v[i][j] * (1.f / kUnitA);     // in kUnitX
+                    }
+                    if (g.out == nullptr) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t o[4], l[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                o[j] = pack_half(v[i][2 * j], v[i][2 * j + 1]);
+                                const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&o[j]));
+                                l[j] = pack_half((v[i][2 * j] - hi.x) * kUnitLo, (v[i][2 * j + 1] - hi.y) * kUnitLo);
+                            }
+                            if (b.row(i) < g.rows && b.col() < width) {
+                                const int64_t at = wide + static_cast<int64_t>(b.row(i)) * g.ld_x + b.col();
+                                *reinterpret_cast<uint4*>(g.x_out + at) = make_uint4(o[0], o[1], o[2], o[3]);
+                                *reinterpret_cast<uint4*>(g.x_lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+                            }
                         }
                     } else {
                         // the last step: the result, in the caller's orientation
-                        __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(g.out) + static_cast<int64_t>(t.g) * g.rows * g.cols;
+                        uint16_t* dst = reinterpret_cast<uint16_t*>(g.out) + static_cast<int64_t>(t.g) * g.rows * g.cols;
+                        uint32_t o[4][4];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j] * (1.f / kUnitX), v[2 * j + 1] * (1.f / kUnitX));
-                            o[j] = *reinterpret_cast<const uint32_t*>(&h);
-                        }
-                        if (in && !g.out_transposed) {
-                            dst += static_cast<int64_t>(row) * g.cols + col;
-                            if (g.cols % 8 == 0) {
-                                *reinterpret_cast<int4*>(dst) = out;
-                            } else {
+                        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                                for (int j = 0; j < 8; ++j)
-                                    if (col + j < g.cols) reinterpret_cast<uint16_t*>(dst)[j] = static_cast<uint16_t>(o[j >> 1] >> (16 * (j & 1)));
+                            for (int j = 0; j < 4; ++j) {
+                                const __nv_bfloat162 h = __floats2bfloat162_rn(v[i][2 * j] * (1.f / kUnitX), v[i][2 * j + 1] * (1.f / kUnitX));
+                                o[i][j] = *reinterpret_cast<const uint32_t*>(&h);
                             }
-                        }
-                    }
-                    if (t.mirror || (kMode == 2 && g.out != nullptr && g.out_transposed)) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            *reinterpret_cast<uint16_t*>(s_t + (lc + j) * kTransposePitch + lr * 2) = static_cast<uint16_t>(o[j >> 1] >> (16 * (j & 1)));
-                    }
-                }
-                __syncwarp();
-                if (t.mirror || (kMode == 2 && g.out != nullptr && g.out_transposed)) {
-                    // rows of the mirror image: 32 values, eight lanes with four each
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int lr = i * 4 + (lane >> 3), lc = (lane & 7) * 4, row = col0 + lr, col = row0 + lc;
-                        const uint2 v = *reinterpret_cast<const uint2*>(s_t + lr * kTransposePitch + lc * 2);
-                        if constexpr (kMode != 2) {
-                            if (row < g.rows && col < g.ld_sq) *reinterpret_cast<uint2*>(g.sq_out + sq + static_cast<int64_t>(row) * g.ld_sq + col) = v;
-                        } else {
-                            uint16_t* dst = reinterpret_cast<uint16_t*>(g.out) + static_cast<int64_t>(t.g) * g.rows * g.cols + static_cast<int64_t>(row) * g.rows + col;
-                            if (row < g.cols) {
+                        if (g.out_transposed) {
+                            transposed(staging, o, b, [&](int row, int col, const uint2& four) {
+                                if (row >= g.cols) return;
+                                uint16_t* p = dst + static_cast<int64_t>(row) * g.rows + col;
                                 if (g.rows % 4 == 0) {
-                                    if (col < g.rows) *reinterpret_cast<uint2*>(dst) = v;
+                                    if (col < g.rows) *reinterpret_cast<uint2*>(p) = four;
                                 } else {
 #pragma unroll
                                     for (int j = 0; j < 4; ++j)
-                                        if (col + j < g.rows) dst[j] = static_cast<uint16_t>((j < 2 ? v.x : v.y) >> (16 * (j & 1)));
+                                        if (col + j < g.rows) p[j] = static_cast<uint16_t>((j < 2 ? four.x : four.y) >> (16 * (j & 1)));
+                                }
+                            });
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                if (b.row(i) >= g.rows || b.col() >= width) continue;
+                                uint16_t* p = dst + static_cast<int64_t>(b.row(i)) * g.cols + b.col();
+                                if (g.cols % 8 == 0) {
+                                    *reinterpret_cast<uint4*>(p) = make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
+                                } else {
+#pragma unroll
+                                    for (int j = 0; j < 8; ++j)
+                                        if (b.col() + j < g.cols) p[j] = static_cast<uint16_t>(o[i][j >> 1] >> (16 * (j & 1)));
                                 }
                             }
                         }
                     }
-                    __syncwarp();
                 }
             }
             umma::fence_before_thread_sync();
@@ -388,6 +490,39 @@ ns_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     if (warp == 1) umma::tmem_dealloc(tmem_base, kTmemColumns);
 }
 
+// Adds the parts of X X^T in their order: a warp per 32 x 32 block of a tile
+constexpr int kAddThreads = 128;
+template <int kBlockN>
+__global__ void __launch_bounds__(kAddThreads) ns_add_kernel(const __grid_constant__ NsArgs g) {
+    __shared__ __align__(16) uint8_t s_staging[kAddThreads / 32][kStagingBytes];
+    ptx::wait_for_previous_kernel();
+    ptx::let_next_kernel_start();
+    const int lane = threadIdx.x & 31, per_matrix = symmetric_tiles<kBlockN>(g.rows), num_tiles = per_matrix * g.count;
+    const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kAddThreads / 32) + (threadIdx.x >> 5);
+    constexpr int kBlocks = (kTileM / 32) * (kBlockN / 32);
+    const int tile = static_cast<int>(unit / kBlocks), in_tile = static_cast<int>(unit % kBlocks);
+    if (tile >= num_tiles) return;
+    const NsTile t = ns_tile<kBlockN, true>(tile, per_matrix, 0);
+    const int r0 = in_tile / (kBlockN / 32) * 32, c0 = in_tile % (kBlockN / 32) * 32;
+    const Block b{t.m * kTileM + r0, t.n * kBlockN + c0};
+    if (b.row0 >= g.rows || b.col0 >= g.ld_sq) return;
+    float v[4][8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    const float* part = g.parts + (static_cast<int64_t>(tile) * kTileM + r0 + (lane >> 2)) * kBlockN + c0 + (lane & 3) * 8;
+#pragma unroll 2
+    for (int s = 0; s < g.k_splits; ++s, part += static_cast<int64_t>(num_tiles) * kTileM * kBlockN)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 x = *reinterpret_cast<const float4*>(part + i * 8 * kBlockN), y = *reinterpret_cast<const float4*>(part + i * 8 * kBlockN + 4);
+            v[i][0] += x.x, v[i][1] += x.y, v[i][2] += x.z, v[i][3] += x.w;
+            v[i][4] += y.x, v[i][5] += y.y, v[i][6] += y.z, v[i][7] += y.w;
+        }
+    finish_gram(g, s_staging[threadIdx.x >> 5], t.g, b, v, t.mirror);
+}
+
 // ------------------------------------------------------------------------------------------------ the first X
 constexpr int kNormThreads = 256, kCastTile = 64;
 
@@ -396,58 +531,111 @@ __device__ __forceinline__ float as_float(T v) {
     if constexpr (sizeof(T) == 2) return __bfloat162float(v);
     else return v;
 }
+// kWide: lines start on 16 bytes
+template <class T, bool kWide>
+__device__ __forceinline__ void load_values(const T* p, int n, float* v) {     // 16 / sizeof(T) values, the first n of them there
+    constexpr int kPer = 16 / sizeof(T);
+    if (kWide && n >= kPer) {
+        T raw[kPer];
+        *reinterpret_cast<uint4*>(raw) = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) v[i] = as_float(raw[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) v[i] = i < n ? as_float(p[i]) : 0.f;
+    }
+}
 
-// sums of squares, in 64 bits: one per CTA
-template <class T>
-__global__ void __launch_bounds__(kNormThreads) ns_norm_kernel(const NsArgs g) {
+// sums of squares, in 64 bits (squares of small or large fp32 values leave the range of 32): one per CTA
+template <class T, bool kWide>
+__global__ void __launch_bounds__(kNormThreads) ns_norm_kernel(const __grid_constant__ NsArgs g) {
     __shared__ double s_sum[kNormThreads / 32];
+    constexpr int kPer = 16 / sizeof(T);
     ptx::wait_for_previous_kernel();
     ptx::let_next_kernel_start();
     const T* src = reinterpret_cast<const T*>(g.in) + static_cast<int64_t>(blockIdx.y) * g.in_stride_matrix;
-    double sum = 0.0;
-    for (int64_t line = blockIdx.x; line < g.in_lines; line += gridDim.x) {
-        const T* p = src + line * g.in_stride_line;
-        for (int i = threadIdx.x; i < g.in_line; i += kNormThreads) {
-            const double v = as_float(p[i]);
-            sum += v * v;
-        }
-    }
+    double sum[2] = {0.0, 0.0};
+    // pieces of a line, line after line
+    const int per_line = (g.in_line + kPer - 1) / kPer;
+    const int64_t pieces = g.in_lines * per_line, stride = static_cast<int64_t>(gridDim.x) * kNormThreads;
+    int64_t at = static_cast<int64_t>(blockIdx.x) * kNormThreads + threadIdx.x, line = at / per_line;
+    int piece = static_cast<int>(at - line * per_line);
+    const int64_t line_step = stride / per_line;
+    const int piece_step = static_cast<int>(stride - line_step * per_line);
+#pragma unroll 4
+    for (; at < pieces; at += stride) {
+        float v[kPer];
+        load_values<T, kWide>(src + line * g.in_stride_line + piece * kPer, g.in_line - piece * kPer, v);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = sum;
+        for (int i = 0; i < kPer; ++i) {
+            const double d = v[i];
+            sum[i & 1] = fma(d, d, sum[i & 1]);
+        }
+        line += line_step;
+        piece += piece_step;
+        if (piece >= per_line) piece -= per_line, ++line;
+    }
+    double total = sum[0] + sum[1];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if ((threadIdx.x & 31) == 0) s_sum[threadIdx.x >> 5] = total;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < kNormThreads / 32; ++w) sum += s_sum[w];
-        g.norm_parts[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = sum;
+        for (int w = 1; w < kNormThreads / 32; ++w) total += s_sum[w];
+        g.norm_parts[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = total;
     }
 }
 
 // X = G / (norm + eps) as hi + lo, with rows <= cols; lines of the input are rows of X, or (flip) its columns.  One CTA per 64 x 64 tile.
-template <class T>
-__global__ void __launch_bounds__(kNormThreads) ns_cast_kernel(const NsArgs g) {
+template <class T, bool kWide>
+__global__ void __launch_bounds__(kNormThreads) ns_cast_kernel(const __grid_constant__ NsArgs g) {
     __shared__ float tile[kCastTile][kCastTile + 1];
+    __shared__ double s_scale;
+    constexpr int kPer = 16 / sizeof(T), kPerLine = kCastTile / kPer;
     ptx::wait_for_previous_kernel();
     ptx::let_next_kernel_start();
     const int line0 = blockIdx.y * kCastTile, at0 = blockIdx.x * kCastTile;
     const T* src = reinterpret_cast<const T*>(g.in) + static_cast<int64_t>(blockIdx.z) * g.in_stride_matrix;
-    double sum = 0.0;
-    for (int i = 0; i < g.num_norm_parts; ++i) sum += g.norm_parts[static_cast<int64_t>(blockIdx.z) * g.num_norm_parts + i];
-    const double scale = static_cast<double>(kUnitX) / (sqrt(sum) + static_cast<double>(g.eps));
-    for (int i = threadIdx.x; i < kCastTile * kCastTile; i += kNormThreads) {
-        const int l = i / kCastTile, c = i % kCastTile;
-        const float v = line0 + l < g.in_lines && at0 + c < g.in_line ? static_cast<float>(as_float(src[(line0 + l) * g.in_stride_line + at0 + c]) * scale) : 0.f;
-        if (g.flip) tile[c][l] = v;
-        else tile[l][c] = v;
+#pragma unroll
+    for (int i = 0; i < kCastTile * kPerLine / kNormThreads; ++i) {
+        const int u = i * kNormThreads + threadIdx.x, l = u / kPerLine, c = (u % kPerLine) * kPer;
+        float v[kPer];
+        load_values<T, kWide>(src + (line0 + l) * g.in_stride_line + at0 + c, line0 + l < g.in_lines ? g.in_line - at0 - c : 0, v);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            if (g.flip) tile[c + j][l] = v[j];
+            else tile[l][c + j] = v[j];
+        }
+    }
+    if (threadIdx.x < 32) {
+        double sum = 0.0;
+        for (int i = threadIdx.x; i < g.num_norm_parts; i += 32) sum += g.norm_parts[static_cast<int64_t>(blockIdx.z) * g.num_norm_parts + i];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (threadIdx.x == 0) s_scale = static_cast<double>(kUnitX) / (sqrt(sum) + static_cast<double>(g.eps));
     }
     __syncthreads();
+    const double scale = s_scale;
+    // (a factor that is an ordinary 32-bit number serves as one)
+    const float scale32 = static_cast<float>(scale);
+    const bool ordinary = scale32 > 1e-30f && scale32 < 1e30f;
     const int row0 = g.flip ? at0 : line0, col0 = g.flip ? line0 : at0;
-    for (int i = threadIdx.x; i < kCastTile * kCastTile; i += kNormThreads) {
-        const int r = i / kCastTile, c = i % kCastTile;
+#pragma unroll
+    for (int i = 0; i < kCastTile * kCastTile / 8 / kNormThreads; ++i) {
+        const int u = i * kNormThreads + threadIdx.x, r = u / (kCastTile / 8), c = (u % (kCastTile / 8)) * 8;
         if (row0 + r < g.rows && col0 + c < g.ld_x) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float a = tile[r][c + 2 * j], b = tile[r][c + 2 * j + 1];
+                const float x = ordinary ? a * scale32 : static_cast<float>(a * scale), y = ordinary ? b * scale32 : static_cast<float>(b * scale);
+                hi[j] = pack_half(x, y);
+                const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[j]));
+                lo[j] = pack_half((x - h.x) * kUnitLo, (y - h.y) * kUnitLo);
+            }
             const int64_t at = (static_cast<int64_t>(blockIdx.z) * g.rows + row0 + r) * g.ld_x + col0 + c;
-            const __half hi = __float2half_rn(tile[r][c]);
-            g.x_out[at] = hi;
-            g.x_lo[at] = __float2half_rn((tile[r][c] - __half2float(hi)) * kUnitLo);
+            *reinterpret_cast<uint4*>(g.x_out + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(g.x_lo + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
     }
 }
@@ -463,37 +651,78 @@ bool make_map(CUtensorMap* map, const __half* base, int64_t count, int64_t rows,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+int64_t symmetric_tiles_of(int rows, int block_n) { return block_n == 256 ? symmetric_tiles<256>(rows) : symmetric_tiles<128>(rows); }
+int64_t tiles_of(const NsArgs& g, int mode, int block_n) {
+    return g.count * (mode == kUpdate ? static_cast<int64_t>((g.rows + kTileM - 1) / kTileM) * ((g.cols + block_n - 1) / block_n) : symmetric_tiles_of(g.rows, block_n));
+}
+// 256-column tiles, or 128 where their waves take less time: a tile of half the columns takes about 0.6 of it.
+int block_n_of(const NsArgs& g, int mode, int num_sms) {
+    auto waves = [&](int n) { return (tiles_of(g, mode, n) + num_sms - 1) / num_sms; };
+    return 10 * waves(256) <= 6 * waves(128) ? 256 : 128;
+}
+// Parts along K of X X^T where its tiles are few and long: as in the GEMM, the K blocks that a CTA is spared against the kernel that adds the parts
+// (about 16 blocks) and the parts' way through L2 (one block per 512 KB).
+int k_splits_of(const NsArgs& g, int num_sms) {
+    const int64_t tiles = tiles_of(g, kGram, 128), num_k = (g.cols + kTileK - 1) / kTileK, most = std::min<int64_t>(num_sms / tiles, num_k / 4);
+    int64_t best = 1, gain = 0;
+    for (int64_t s = 2; s <= most; ++s) {
+        const int64_t now = num_k - (num_k + s - 1) / s - 16 - s * tiles * kTileM * 128 * 4 / (512 * 1024);
+        if (now > gain) best = s, gain = now;
+    }
+    return static_cast<int>(best);
+}
+
 template <int kMode, int kBlockN>
 cudaError_t launch_product(const CUtensorMap& map_a, const CUtensorMap& map_b, const NsArgs& g, int num_sms, cudaStream_t stream) {
     const void* fn = reinterpret_cast<const void*>(ns_kernel<kMode, kBlockN>);
     const cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, ns_smem_bytes(kBlockN));
-    if (err != cudaSuccess) return err;
-    const int64_t num_m = (g.rows + kTileM - 1) / kTileM;
-    const int64_t items = g.count * (kMode != 2 ? static_cast<int64_t>(symmetric_tiles<kBlockN>(g.rows)) : num_m * ((g.cols + kBlockN - 1) / kBlockN));
+    if (err != cudaSuccess) {
+        cudaGetLastError();      // the caller reports it
+        return err;
+    }
+    const int64_t items = tiles_of(g, kMode, kBlockN) * (kMode == kGramPart ? g.k_splits : 1);
     void* params[] = {const_cast<CUtensorMap*>(&map_a), const_cast<CUtensorMap*>(&map_b), const_cast<NsArgs*>(&g)};
     return launch_dependent(fn, dim3(static_cast<unsigned>(std::min<int64_t>(items, num_sms))), dim3(kNsThreads), params, ns_smem_bytes(kBlockN), stream);
+}
+template <int kMode>
+cudaError_t launch_product(int block_n, const CUtensorMap& map_a, const CUtensorMap& map_b, const NsArgs& g, int num_sms, cudaStream_t stream) {
+    return block_n == 256 ? launch_product<kMode, 256>(map_a, map_b, g, num_sms, stream) : launch_product<kMode, 128>(map_a, map_b, g, num_sms, stream);
 }
 
 int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 
+template <class T>
+cudaError_t launch_first(const NsArgs& g, cudaStream_t stream) {
+    const bool wide = reinterpret_cast<uintptr_t>(g.in) % 16 == 0 && g.in_stride_line * sizeof(T) % 16 == 0 && g.in_stride_matrix * sizeof(T) % 16 == 0;
+    void* params[] = {const_cast<NsArgs*>(&g)};
+    const cudaError_t err = launch_dependent(wide ? reinterpret_cast<const void*>(ns_norm_kernel<T, true>) : reinterpret_cast<const void*>(ns_norm_kernel<T, false>),
+                                             dim3(g.num_norm_parts, g.count), dim3(kNormThreads), params, 0, stream);
+    if (err != cudaSuccess) return err;
+    const dim3 grid((g.in_line + kCastTile - 1) / kCastTile, static_cast<unsigned>((g.in_lines + kCastTile - 1) / kCastTile), g.count);
+    return launch_dependent(wide ? reinterpret_cast<const void*>(ns_cast_kernel<T, true>) : reinterpret_cast<const void*>(ns_cast_kernel<T, false>), grid, dim3(kNormThreads), params, 0,
+                            stream);
+}
+
 }  // namespace
 
-// Workspace: hi of X twice and lo once, O and B, their diagonals, sums of squares.
-NsWorkspace newton_schulz_workspace(int64_t count, int64_t rows, int64_t cols, int num_sms) {
+// Workspace: hi of X twice and lo once, O and B, their diagonals, sums of squares, parts of X X^T.
+NsWorkspace newton_schulz_workspace(const NsArgs& g, int num_sms) {
     NsWorkspace w{};
-    w.ld_x = round8(cols);
-    w.ld_sq = round8(rows);
-    w.norm_parts = std::max<int64_t>(1, std::min<int64_t>(rows, 4 * num_sms / std::max<int64_t>(1, count)));
+    w.ld_x = round8(g.cols);
+    w.ld_sq = round8(g.rows);
+    w.norm_parts = std::max<int64_t>(1, std::min<int64_t>((static_cast<int64_t>(g.rows) * g.cols + 8191) / 8192, 8 * num_sms / g.count));
+    w.k_splits = k_splits_of(g, num_sms);
     auto take = [&](int64_t bytes) {
         const int64_t at = w.bytes;
         w.bytes += (bytes + 255) / 256 * 256;
         return at;
     };
-    w.norms = take(count * w.norm_parts * 8);
-    for (int64_t& x : w.x) x = take(count * rows * w.ld_x * 2);
-    w.lo = take(count * rows * w.ld_x * 2);
-    for (int64_t& s : w.sq) s = take(count * rows * w.ld_sq * 2);
-    for (int64_t& d : w.diag) d = take(count * rows * 4);
+    w.norms = take(g.count * w.norm_parts * 8);
+    for (int64_t& x : w.x) x = take(g.count * g.rows * w.ld_x * 2);
+    w.lo = take(g.count * g.rows * w.ld_x * 2);
+    for (int64_t& s : w.sq) s = take(g.count * g.rows * w.ld_sq * 2);
+    for (int64_t& d : w.diag) d = take(g.count * w.ld_sq * 4);
+    w.parts = take(w.k_splits > 1 ? w.k_splits * tiles_of(g, kGram, 128) * kTileM * 128 * 4 : 0);
     return w;
 }
 
@@ -512,40 +741,43 @@ cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8
     g.coef = reinterpret_cast<float*>(workspace + w.diag[1]);
     g.norm_parts = reinterpret_cast<double*>(workspace + w.norms);
     g.num_norm_parts = static_cast<int>(w.norm_parts);
+    g.parts = reinterpret_cast<float*>(workspace + w.parts);
+    g.k_splits = w.k_splits;
     void* out = g.out;
     g.out = nullptr;
-    constexpr int kBlockN = 256;
+    const int n_gram = g.k_splits > 1 ? 128 : block_n_of(g, kGram, num_sms), n_poly = block_n_of(g, kPoly, num_sms), n_update = block_n_of(g, kUpdate, num_sms);
     CUtensorMap x_rows[2], x_cols[2], x_mn[2], o_rows, o_cols, b_rows;
     for (int i = 0; i < 2; ++i)
-        if (!make_map(&x_rows[i], x[i], g.count, g.rows, g.cols, g.ld_x, kTileM) || !make_map(&x_cols[i], x[i], g.count, g.rows, g.cols, g.ld_x, kBlockN) ||
+        if (!make_map(&x_rows[i], x[i], g.count, g.rows, g.cols, g.ld_x, kTileM) || !make_map(&x_cols[i], x[i], g.count, g.rows, g.cols, g.ld_x, n_gram) ||
             !make_map(&x_mn[i], x[i], g.count, g.rows, g.cols, g.ld_x, 64))
             return cudaErrorInvalidValue;
-    if (!make_map(&o_rows, sq[0], g.count, g.rows, g.rows, g.ld_sq, kTileM) || !make_map(&o_cols, sq[0], g.count, g.rows, g.rows, g.ld_sq, kBlockN) ||
+    if (!make_map(&o_rows, sq[0], g.count, g.rows, g.rows, g.ld_sq, kTileM) || !make_map(&o_cols, sq[0], g.count, g.rows, g.rows, g.ld_sq, n_poly) ||
         !make_map(&b_rows, sq[1], g.count, g.rows, g.rows, g.ld_sq, kTileM))
         return cudaErrorInvalidValue;
 
-    void* params[] = {&g};
     g.x_out = x[0];
-    const dim3 norm_grid(g.num_norm_parts, g.count);
-    const dim3 cast_grid((g.in_line + kCastTile - 1) / kCastTile, static_cast<unsigned>((g.in_lines + kCastTile - 1) / kCastTile), g.count);
-    cudaError_t err = launch_dependent(g.in_bf16 ? reinterpret_cast<const void*>(ns_norm_kernel<__nv_bfloat16>) : reinterpret_cast<const void*>(ns_norm_kernel<float>), norm_grid,
-                                       dim3(kNormThreads), params, 0, stream);
-    if (err != cudaSuccess) return err;
-    err = launch_dependent(g.in_bf16 ? reinterpret_cast<const void*>(ns_cast_kernel<__nv_bfloat16>) : reinterpret_cast<const void*>(ns_cast_kernel<float>), cast_grid,
-                           dim3(kNormThreads), params, 0, stream);
+    cudaError_t err = g.in_bf16 ? launch_first<__nv_bfloat16>(g, stream) : launch_first<float>(g, stream);
     for (int s = 0; s < steps && err == cudaSuccess; ++s) {
         const int from = s & 1;
         g.sq_out = sq[0];
-        err = launch_product<0, kBlockN>(x_rows[from], x_cols[from], g, num_sms, stream);
+        if (g.k_splits > 1) {
+            err = launch_product<kGramPart, 128>(x_rows[from], x_cols[from], g, num_sms, stream);
+            if (err != cudaSuccess) break;
+            void* params[] = {&g};
+            const int64_t warps = tiles_of(g, kGram, 128) * (kTileM / 32) * (128 / 32);
+            err = launch_dependent(reinterpret_cast<const void*>(ns_add_kernel<128>), dim3(static_cast<unsigned>(warps * 32 / kAddThreads)), dim3(kAddThreads), params, 0, stream);
+        } else {
+            err = launch_product<kGram>(n_gram, x_rows[from], x_cols[from], g, num_sms, stream);
+        }
         if (err != cudaSuccess) break;
         g.sq_in = sq[0];
         g.sq_out = sq[1];
-        err = launch_product<1, kBlockN>(o_rows, o_cols, g, num_sms, stream);
+        err = launch_product<kPoly>(n_poly, o_rows, o_cols, g, num_sms, stream);
         if (err != cudaSuccess) break;
         g.x_in = x[from];
         g.x_out = x[from ^ 1];
         if (s == steps - 1) g.out = out;
-        err = launch_product<2, kBlockN>(b_rows, x_mn[from], g, num_sms, stream);
+        err = launch_product<kUpdate>(n_update, b_rows, x_mn[from], g, num_sms, stream);
     }
     return err;
 }

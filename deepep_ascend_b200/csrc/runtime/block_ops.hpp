@@ -198,7 +198,7 @@ inline at::Tensor orthogonalize(const at::Tensor& x, int64_t steps, double a, do
         g.report.timeout_ns = ctx.timeout_ns;
     }
     const int sms = num_sms > 0 ? static_cast<int>(num_sms) : device_sms();
-    const NsWorkspace w = ep::newton_schulz_workspace(g.count, g.rows, g.cols, sms);
+    const NsWorkspace w = ep::newton_schulz_workspace(g, sms);
     at::Tensor workspace = at::empty({w.bytes}, x.options().dtype(at::kByte));
     cuda_check(ep::launch_newton_schulz(g, w, workspace.data_ptr<uint8_t>(), static_cast<int>(steps), sms, at::cuda::getCurrentCUDAStream()), "orthogonalisation launch");
     return res;
