@@ -6,12 +6,13 @@
 //     groups: the sum of a group's one or two best choices; the experts of the best groups stay
 //     chosen = the num_topk best choices, equal ones by index;  w = scale * p (/ sum of the chosen p)
 //
-// One warp per token.  Lane i of a warp holds the experts i, i + 32, ...: every load of the warp is contiguous, and the sum of the
-// exponentials "upper half added to lower half" has its first levels within a lane and the others across lanes.  That order is part of the
-// definition: scores that differ in their last bit would choose another expert where two are as good.
-#include <math_constants.h>
-
+// The sum of the exponentials is a tree: the experts, padded with zeros to a power of two, are halved and the upper half is added to the lower one.
+// That order is part of the definition: scores that differ in their last bit would choose another expert where two are as good.
 #include <algorithm>
+#include <map>
+#include <mutex>
+#include <tuple>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -19,21 +20,39 @@ namespace ep {
 
 namespace {
 
-constexpr int kRouterWarps = 8;
+constexpr float kNone = -__builtin_inff();
 
 template <bool kBf16>
 __device__ __forceinline__ float load_logit(const void* row, int e) {
     return kBf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(row)[e]) : reinterpret_cast<const float*>(row)[e];
 }
 
+template <class T>
+__device__ __forceinline__ T logit_of(float v) {
+    if constexpr (sizeof(T) == 2) return __float2bfloat16_rn(v);
+    else return v;
+}
+
 __device__ __forceinline__ float sigmoid(float l) { return __frcp_rn(1.f + expf(-l)); }
 
-__device__ __forceinline__ float warp_max_nan(float v) {      // a NaN wins, as everything computed with it is one
+__device__ __forceinline__ float max_nan(float a, float b) {      // a NaN wins, as everything computed with it is one
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// over the eight lanes of a token
+template <class F>
+__device__ __forceinline__ float over8(float v, F f) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const float w = __shfl_xor_sync(0xffffffffu, v, o);
-        asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(v), "f"(w));
-    }
+    for (int o = 4; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ float sum8(float v) {
+    return over8(v, [](float a, float b) { return a + b; });
+}
+__device__ __forceinline__ float warp_max_nan(float v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 __device__ __forceinline__ float warp_sum(float v) {
@@ -41,185 +60,445 @@ __device__ __forceinline__ float warp_sum(float v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-// floats as integers of the same order (no NaN, no -0)
-__device__ __forceinline__ int order_key(float v) {
-    const int b = __float_as_int(v);
-    return b ^ ((b >> 31) & 0x7fffffff);
+
+// Eight neighbouring logits; those past the end are -inf.  kWide: rows start on 16 bytes and end with a whole eight.
+template <bool kBf16, bool kWide>
+__device__ __forceinline__ void load8(const void* row, int first, int experts, float (&v)[8]) {
+    if constexpr (kWide && kBf16) {
+        const uint4 q = *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(row) + first);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else if constexpr (kWide) {
+        const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + first);
+        const float4 b = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + first + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = first + i < experts ? load_logit<kBf16>(row, first + i) : kNone;
+    }
+}
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void fetch8(const float* p, float (&v)[8]) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
-// the row's softmax: maximum and sum of exp(l - max); v[j] becomes exp(l - max)
-template <int kVals>
-__device__ __forceinline__ void softmax_row(float (&v)[kVals], int lane, int experts, float& top, float& total) {
-    top = -CUDART_INF_F;
-#pragma unroll
-    for (int j = 0; j < kVals; ++j)
-        if (j * 32 + lane < experts) asm("max.NaN.f32 %0, %1, %2;" : "=f"(top) : "f"(top), "f"(v[j]));
-    top = warp_max_nan(top);
-    float sum[kVals];
-#pragma unroll
-    for (int j = 0; j < kVals; ++j) sum[j] = v[j] = j * 32 + lane < experts ? expf(v[j] - top) : 0.f;
-#pragma unroll
-    for (int h = kVals / 2; h > 0; h >>= 1)
-#pragma unroll
-        for (int j = 0; j < h; ++j) sum[j] += sum[j + h];
-    total = warp_sum(sum[0]);
+// Shared memory of a warp, which works on up to four tokens at a time: the choices of each, padded to whole eights; the best and second best of each eight; the
+// groups' scores; for a softmax, room for the tree.
+constexpr int kTokens = 4;
+struct RouteLayout {
+    int eights, choice, best, group, tree, warp;       // eights of a token; offsets in floats of a token's or the warp's arrays; floats of a warp
+};
+__host__ __device__ inline RouteLayout route_layout(int experts, int groups, bool softmax) {
+    RouteLayout l;
+    l.eights = (experts + 7) / 8;
+    int width = 8;                                     // experts as a power of two, eight at least
+    while (width < experts) width *= 2;
+    l.choice = 0;
+    l.best = kTokens * l.eights * 8;
+    l.group = l.best + kTokens * 2 * ((l.eights + 3) / 4 * 4);
+    l.tree = l.group + (groups > 1 ? kTokens * 32 : 0);
+    l.warp = l.tree + (softmax ? kTokens * width / 2 : 0);
+    return l;
 }
 
-template <int kVals, bool kBf16>
-__global__ void __launch_bounds__(kRouterWarps * 32) route_kernel(const RouterArgs a) {
-    extern __shared__ uint8_t router_smem[];
-    int* s_count = reinterpret_cast<int*>(router_smem);                                 // [experts]
-    float* s_choice = reinterpret_cast<float*>(s_count + a.num_experts);                // [warps][experts], with groups
+// A warp takes `tokens` (1 or 4) at a time.  Scores: a lane has eight neighbouring experts of one token.  Choice: eight lanes per token, each with kSegs eights
+// of which it knows the largest choice; a chosen expert is found, taken out, and the new largest of its eight made by the token's eight lanes together, so that the
+// shuffles of a step serve four tokens.  Bound by instruction issue: about half of what is left are the exact exponentials and reciprocals.
+// 65536 x 256 fp32, 8 of 256 in 4 of 8 groups: 59 us; one token per warp, with a maximum over the warp for every expert, took 139.
+template <int kSegs, bool kBf16, bool kWide, bool kSoftmax>
+__global__ void __launch_bounds__(256) route_kernel(const RouterArgs a, const int tokens) {
+    extern __shared__ __align__(16) float route_smem[];
+    const RouteLayout l = route_layout(a.num_experts, a.num_groups, kSoftmax);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, E = a.num_experts, K = a.num_topk, S = l.eights, G = a.num_groups;
+    float* mine = route_smem + warp * l.warp;
+    float *choice = mine + l.choice, *best = mine + l.best, *group_score = mine + l.group, *tree = mine + l.tree;
+    const int best_pitch = (S + 3) / 4 * 4;
+    float* second = best + kTokens * best_pitch;
+    float* s_bias = route_smem + warps * l.warp;                              // [S * 8]
+    int* s_count = reinterpret_cast<int*>(s_bias + S * 8);                    // [E]
+    for (int e = threadIdx.x; e < E; e += blockDim.x) s_count[e] = 0;
     ptx::wait_for_previous_kernel();
     ptx::let_next_kernel_start();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, E = a.num_experts, K = a.num_topk;
-    for (int e = threadIdx.x; e < E; e += blockDim.x) s_count[e] = 0;
+    for (int e = threadIdx.x; e < S * 8; e += blockDim.x) s_bias[e] = a.bias != nullptr && e < E ? a.bias[e] : 0.f;
+    // eights past the last one of a token, which the lanes below look at, hold nobody
+    for (int i = lane; i < 2 * kTokens * best_pitch; i += 32) best[i] = kNone;
     __syncthreads();
-    s_choice += warp * E;
-    for (int64_t t = static_cast<int64_t>(blockIdx.x) * kRouterWarps + warp; t < a.num_tokens; t += static_cast<int64_t>(gridDim.x) * kRouterWarps) {
-        int my_expert = -1;
-        float my_p = 0.f;
-        if (a.token_mask == nullptr || a.token_mask[t] != 0) {
-            const uint8_t* row = reinterpret_cast<const uint8_t*>(a.logits) + t * a.ld * (kBf16 ? 2 : 4);
-            float c[kVals];
-            uint32_t off = 0;                   // bit j: expert j * 32 + lane cannot be chosen
+    const int size = E / G;                            // experts of a group
+    const bool whole = G > 1 && size % 8 == 0;         // groups of whole eights
+    const int t8 = lane >> 3, q = lane & 7;            // token and place of the lane where eight lanes have a token
+    int seg_group[kSegs];
 #pragma unroll
-            for (int j = 0; j < kVals; ++j) {
-                const int e = j * 32 + lane;
-                c[j] = e < E ? load_logit<kBf16>(row, e) : -CUDART_INF_F;
-                if (c[j] == -CUDART_INF_F) off |= 1u << j;
+    for (int i = 0; i < kSegs; ++i) seg_group[i] = whole ? min(q * kSegs + i, S - 1) * 8 / size : 0;
+    const float inverse_s = 1.f / S, inverse_g = 1.f / G;
+    // largest and second largest choice of an eight
+    auto tops = [&](const float (&c)[8], int t, int seg) {
+        float v1 = c[0], v2 = kNone;
+#pragma unroll
+        for (int i = 1; i < 8; ++i) {
+            v2 = fmaxf(v2, fminf(v1, c[i]));
+            v1 = fmaxf(v1, c[i]);
+        }
+        best[t * best_pitch + seg] = v1;
+        second[t * best_pitch + seg] = v2;
+    };
+    // a choice that is no number, or whose logit is -inf, is nobody's
+    auto settle = [&](const float (&logit)[8], float (&c)[8]) {
+        float low = fminf(fminf(fminf(c[0], c[1]), fminf(c[2], c[3])), fminf(fminf(c[4], c[5]), fminf(c[6], c[7])));
+        float odd = ((c[0] + c[1]) + (c[2] + c[3])) + ((c[4] + c[5]) + (c[6] + c[7]));      // NaN if one of them is
+        low = fminf(low, fminf(fminf(fminf(logit[0], logit[1]), fminf(logit[2], logit[3])), fminf(fminf(logit[4], logit[5]), fminf(logit[6], logit[7]))));
+        if (!(low > kNone) || !(odd == odd)) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (!(c[i] > kNone) || !(logit[i] > kNone)) c[i] = kNone;
+        }
+    };
+
+    const int64_t step = static_cast<int64_t>(gridDim.x) * warps * tokens;
+    for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * warps + warp) * tokens; t0 < a.num_tokens; t0 += step) {
+        const int n = static_cast<int>(min(static_cast<int64_t>(tokens), a.num_tokens - t0)), units = n * S;
+        const uint8_t* rows = reinterpret_cast<const uint8_t*>(a.logits) + t0 * a.ld * (kBf16 ? 2 : 4);
+        const int64_t pitch = a.ld * (kBf16 ? 2 : 4);
+        float top = 0.f, total = 1.f;                  // of the token of this lane's eight
+        if constexpr (kSoftmax) {
+            // logits, and the largest of each eight
+            for (int u = lane; u < units; u += 32) {
+                const int t = static_cast<int>((u + 0.5f) * inverse_s), seg = u - t * S;
+                float v[8];
+                load8<kBf16, kWide>(rows + t * pitch, seg * 8, E, v);
+                store8(choice + u * 8, v);
+                best[t * best_pitch + seg] = max_nan(max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3])), max_nan(max_nan(v[4], v[5]), max_nan(v[6], v[7])));
             }
-            float top = 0.f, total = 1.f;
-            if (a.softmax) {
-                softmax_row<kVals>(c, lane, E, top, total);
-#pragma unroll
-                for (int j = 0; j < kVals; ++j) c[j] = __fdiv_rn(c[j], total);
-            } else {
-#pragma unroll
-                for (int j = 0; j < kVals; ++j) c[j] = sigmoid(c[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < kVals; ++j) {
-                const int e = j * 32 + lane;
-                if (a.bias != nullptr && e < E) c[j] += a.bias[e];
-                if (((off >> j) & 1u) != 0 || isnan(c[j])) c[j] = -CUDART_INF_F;
-            }
-            if (a.num_groups > 1) {
-                const int G = a.num_groups, size = E / G;
-#pragma unroll
-                for (int j = 0; j < kVals; ++j)
-                    if (j * 32 + lane < E) s_choice[j * 32 + lane] = c[j];
-                __syncwarp();
-                float v1 = -CUDART_INF_F, v2 = -CUDART_INF_F;
-                if (lane < G)
-                    for (int i = 0; i < size; ++i) {
-                        const float v = s_choice[lane * size + i];
-                        v2 = fmaxf(v2, fminf(v1, v));
-                        v1 = fmaxf(v1, v);
+            __syncwarp();
+            top = kNone;
+            if (t8 < n)
+                for (int s = q; s < S; s += 8) top = max_nan(top, best[t8 * best_pitch + s]);
+            top = over8(top, max_nan);
+            // exp(l - max) of the lane's experts q, q + 8, ..., and their sum by halves: the first level on the way to `tree`
+            if (t8 < n) {
+                float *e = choice + t8 * S * 8 + q, *x = tree + t8 * ((l.warp - l.tree) / kTokens) + q;
+                int half = (l.warp - l.tree) / kTokens / 8;            // eights of the padded experts, by two
+                if (half == 0) {
+                    e[0] = expf(e[0] - top);
+                    total = q < E ? e[0] : 0.f;
+                } else {
+                    for (int s = 0; s < half; ++s) {
+                        float lo = 0.f, hi = 0.f;
+                        if (s < S) lo = e[s * 8] = expf(e[s * 8] - top);
+                        if (s + half < S) hi = e[(s + half) * 8] = expf(e[(s + half) * 8] - top);
+                        x[s * 8] = lo + hi;
                     }
-                const float score = a.group_top == 2 && v2 != -CUDART_INF_F ? v1 + v2 : v1;
-                int better = 0;
-                for (int g = 0; g < G; ++g) {
-                    const float other = __shfl_sync(0xffffffffu, score, g);
-                    better += other > score || (other == score && g < lane);
+                    for (half /= 2; half > 0; half /= 2)
+                        for (int s = 0; s < half; ++s) x[s * 8] += x[(s + half) * 8];
+                    total = x[0];
                 }
-                const uint32_t keep = __ballot_sync(0xffffffffu, lane < G && better < a.num_topk_groups);
+            } else {
+                total = 0.f;
+            }
+            total = sum8(total);
+            __syncwarp();
+            for (int u0 = 0; u0 < units; u0 += 32) {
+                const int u = u0 + lane, t = min(static_cast<int>((u + 0.5f) * inverse_s), kTokens - 1), seg = u - t * S;
+                const float sum = __shfl_sync(0xffffffffu, total, t * 8);
+                if (u < units) {
+                    float logit[8], c[8];
+                    load8<kBf16, kWide>(rows + t * pitch, seg * 8, E, logit);
+                    fetch8(choice + u * 8, c);
+                    float b[8];
+                    fetch8(s_bias + seg * 8, b);
 #pragma unroll
-                for (int j = 0; j < kVals; ++j) {
-                    const int e = j * 32 + lane;
-                    if (e < E && ((keep >> (e / size)) & 1u) == 0) c[j] = -CUDART_INF_F;
+                    for (int i = 0; i < 8; ++i) c[i] = __fdiv_rn(c[i], sum) + b[i];
+                    settle(logit, c);
+                    store8(choice + u * 8, c);
+                    tops(c, t, seg);
                 }
+            }
+        } else {
+            for (int u = lane; u < units; u += 32) {
+                const int t = static_cast<int>((u + 0.5f) * inverse_s), seg = u - t * S;
+                float logit[8], c[8], b[8];
+                load8<kBf16, kWide>(rows + t * pitch, seg * 8, E, logit);
+                fetch8(s_bias + seg * 8, b);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) c[i] = sigmoid(logit[i]) + b[i];
+                settle(logit, c);
+                store8(choice + u * 8, c);
+                tops(c, t, seg);
+            }
+        }
+        __syncwarp();
+        uint32_t kept = 0xffffffffu;                   // groups of token t8 that stay
+        if (G > 1) {
+            // scores of the groups: their two best
+            for (int u = lane; u < n * G; u += 32) {
+                const int t = static_cast<int>((u + 0.5f) * inverse_g), g = u - t * G;
+                float v1 = kNone, v2 = kNone;
+                if (whole) {
+                    for (int s = g * (size / 8); s < (g + 1) * (size / 8); ++s) {
+                        const float b1 = best[t * best_pitch + s], b2 = second[t * best_pitch + s];
+                        v2 = fmaxf(fminf(v1, b1), fmaxf(v2, b2));
+                        v1 = fmaxf(v1, b1);
+                    }
+                } else {
+                    const float* c = choice + t * S * 8 + g * size;
+                    for (int i = 0; i < size; ++i) {
+                        v2 = fmaxf(v2, fminf(v1, c[i]));
+                        v1 = fmaxf(v1, c[i]);
+                    }
+                }
+                group_score[t * 32 + g] = a.group_top == 2 && v2 > kNone ? v1 + v2 : v1;
+            }
+            __syncwarp();
+            // the groups that fewer than num_topk_groups others beat, equal ones by index; eight lanes per token
+            kept = 0;
+            if (t8 < n)
+                for (int g = q; g < G; g += 8) {
+                    const float score = group_score[t8 * 32 + g];
+                    int better = 0;
+                    for (int h = 0; h < G; ++h) {
+                        const float other = group_score[t8 * 32 + h];
+                        better += other > score || (other == score && h < g);
+                    }
+                    if (better < a.num_topk_groups) kept |= 1u << g;
+                }
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) kept |= __shfl_xor_sync(0xffffffffu, kept, o);
+            if (!whole) {
+                // groups that end within an eight: their experts leave one by one
+                for (int u0 = 0; u0 < units; u0 += 32) {
+                    const int u = u0 + lane, t = min(static_cast<int>((u + 0.5f) * inverse_s), kTokens - 1), seg = u - t * S;
+                    const uint32_t stay = __shfl_sync(0xffffffffu, kept, t * 8);
+                    if (u < units) {
+                        float c[8];
+                        fetch8(choice + u * 8, c);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (((stay >> min((seg * 8 + i) / size, 31)) & 1u) == 0) c[i] = kNone;
+                        store8(choice + u * 8, c);
+                        tops(c, t, seg);
+                    }
+                }
+                kept = 0xffffffffu;
                 __syncwarp();
             }
-            for (int k = 0; k < K; ++k) {
-                float best = -CUDART_INF_F;
-                int at = E;
+        }
+        // the largest choice of each of this lane's eights
+        float m[kSegs];
+        const bool routed = t8 < n && (a.token_mask == nullptr || a.token_mask[t0 + t8] != 0);
 #pragma unroll
-                for (int j = 0; j < kVals; ++j)
-                    if (c[j] > best) best = c[j], at = j * 32 + lane;
-                const int key = order_key(best), top_key = __reduce_max_sync(0xffffffffu, key);
-                const int e = __reduce_min_sync(0xffffffffu, key == top_key ? at : E);
-                if (e >= E) break;              // nobody is left
-                if (lane == k) my_expert = e;
+        for (int i = 0; i < kSegs; ++i) {
+            const int seg = q * kSegs + i;
+            m[i] = routed && seg < S && ((kept >> seg_group[i]) & 1u) != 0 ? best[t8 * best_pitch + seg] : kNone;
+        }
+        int chosen[2] = {-1, -1};                      // experts q and q + 8 of token t8
+        float* c8 = choice + (t8 < n ? t8 : 0) * S * 8 + q;
+        for (int k = 0; k < K; ++k) {
+            float largest = m[0];
 #pragma unroll
-                for (int j = 0; j < kVals; ++j)
-                    if (j * 32 + lane == e) c[j] = -CUDART_INF_F;
+            for (int i = 1; i < kSegs; ++i) largest = fmaxf(largest, m[i]);
+            const float wanted = over8(largest, [](float x, float y) { return fmaxf(x, y); });
+            const bool some = wanted > kNone;
+            if (!__any_sync(0xffffffffu, some)) break;
+            // the first eight that has it, its first expert
+            int at = 0;
+#pragma unroll
+            for (int i = kSegs - 1; i >= 0; --i)
+                if (m[i] == wanted) at = i;
+            const uint32_t owners = __ballot_sync(0xffffffffu, largest == wanted) >> (t8 * 8) & 0xffu;
+            const int owner = __ffs(owners) - 1, seg = __shfl_sync(0xffffffffu, q * kSegs + at, t8 * 8 + owner);
+            float c = some ? c8[seg * 8] : kNone;
+            const uint32_t hits = __ballot_sync(0xffffffffu, c == wanted) >> (t8 * 8) & 0xffu;
+            const int place = __ffs(hits) - 1;
+            if (some && q == place) c8[seg * 8] = c = kNone;
+            const float next = over8(c, [](float x, float y) { return fmaxf(x, y); });
+            if (some && q == owner) {
+#pragma unroll
+                for (int i = 0; i < kSegs; ++i)
+                    if (i == at) m[i] = next;
             }
-            const float l = my_expert >= 0 ? load_logit<kBf16>(row, my_expert) : -CUDART_INF_F;
-            // renormalised softmax weights are taken relative to the largest chosen logit: also right where p itself would vanish
-            if (a.softmax && a.renormalize) top = warp_max_nan(l), total = 1.f;
-            if (my_expert >= 0) {
-                my_p = a.softmax ? __fdiv_rn(expf(l - top), total) : sigmoid(l);
-                atomicAdd(&s_count[my_expert], 1);
+            if (some && q == (k & 7)) {
+                if (k < 8) chosen[0] = seg * 8 + place;
+                else chosen[1] = seg * 8 + place;
             }
         }
-        float w = my_p;
+        // weights
+        const uint8_t* row = rows + (t8 < n ? t8 : 0) * pitch;
+        float logit[2], p[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) logit[i] = chosen[i] >= 0 ? load_logit<kBf16>(row, chosen[i]) : kNone;
+        if constexpr (kSoftmax) {
+            // renormalised weights are taken relative to the largest chosen logit: also right where p itself would vanish
+            if (a.renormalize) top = over8(max_nan(logit[0], logit[1]), max_nan), total = 1.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (chosen[i] >= 0) {
+                p[i] = kSoftmax ? __fdiv_rn(expf(logit[i] - top), total) : sigmoid(logit[i]);
+                atomicAdd(&s_count[chosen[i]], 1);
+            }
         if (a.renormalize) {
-            const float sum = warp_sum(my_p);
-            w = sum > 0.f ? __fdiv_rn(my_p, sum) : 0.f;
+            const float sum = sum8(p[0] + p[1]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) p[i] = sum > 0.f ? __fdiv_rn(p[i], sum) : 0.f;
         }
-        if (lane < K) {
-            if (a.idx_is_64) reinterpret_cast<int64_t*>(a.topk_idx)[t * K + lane] = my_expert;
-            else reinterpret_cast<int32_t*>(a.topk_idx)[t * K + lane] = my_expert;
-            a.topk_weights[t * K + lane] = w * a.scale;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int k = q + i * 8;
+            if (t8 < n && k < K) {
+                const int64_t out = (t0 + t8) * K + k;
+                if (a.idx_is_64) reinterpret_cast<int64_t*>(a.topk_idx)[out] = chosen[i];
+                else reinterpret_cast<int32_t*>(a.topk_idx)[out] = chosen[i];
+                a.topk_weights[out] = p[i] * a.scale;
+            }
         }
+        __syncwarp();
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += blockDim.x)
-        if (s_count[e] != 0) atomicAdd(&a.count[e], s_count[e]);
+    // the only CTA of a small batch has all counts; otherwise they are added to a cleared array
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
+        if (gridDim.x == 1) a.count[e] = s_count[e];
+        else if (s_count[e] != 0) atomicAdd(&a.count[e], s_count[e]);
+    }
 }
 
+// ------------------------------------------------------------------------------------------------ gradient
 // d loss / d logits of a row.  sigmoid: dp p (1 - p) at the chosen experts; softmax with renormalised weights: the other experts' scores
 // cancel, w (dw - sum dw w) at the chosen ones; softmax as it is: p (dp - sum dp p) for every expert.
-template <int kVals, bool kBf16>
-__global__ void __launch_bounds__(kRouterWarps * 32) route_backward_kernel(const RouterArgs a) {
+
+__device__ __forceinline__ int chosen_expert(const RouterArgs& a, int64_t at) {
+    const int64_t e = a.idx_is_64 ? reinterpret_cast<const int64_t*>(a.topk_idx)[at] : reinterpret_cast<const int32_t*>(a.topk_idx)[at];
+    return e >= 0 && e < a.num_experts ? static_cast<int>(e) : -1;
+}
+
+// Gradients that only chosen experts have.  A warp takes kRows tokens at a time, eight lanes for each of four; their rows, zero but for the chosen experts,
+// lie in shared memory and leave as one bulk copy (kRows rows start and end on 16 bytes for any number of experts), two sets of rows in turn.  What is
+// left to do per row is to write and clear its few values.  65536 x 256 fp32, 8 chosen: 21 us; rows put together in registers took 42.
+template <bool kBf16>
+__global__ void __launch_bounds__(256) route_backward_kernel(const RouterArgs a) {
+    using T = std::conditional_t<kBf16, __nv_bfloat16, float>;
+    constexpr int kRows = kBf16 ? 8 : 4, kSets = 2;
+    extern __shared__ __align__(16) uint8_t route_rows[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, E = a.num_experts, K = a.num_topk;
+    const int t8 = lane >> 3, q = lane & 7;
+    const int set_bytes = kRows * E * static_cast<int>(sizeof(T));
+    uint8_t* mine = route_rows + warp * kSets * set_bytes;
+    for (int i = lane; i < kSets * set_bytes / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
+    __syncwarp();
     ptx::wait_for_previous_kernel();
     ptx::let_next_kernel_start();
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, E = a.num_experts, K = a.num_topk;
-    for (int64_t t = static_cast<int64_t>(blockIdx.x) * kRouterWarps + warp; t < a.num_tokens; t += static_cast<int64_t>(gridDim.x) * kRouterWarps) {
-        const uint8_t* row = reinterpret_cast<const uint8_t*>(a.logits) + t * a.ld * (kBf16 ? 2 : 4);
-        int expert = -1;
-        float dw = 0.f;
-        if (lane < K) {
-            const int64_t e = a.idx_is_64 ? reinterpret_cast<const int64_t*>(a.topk_idx)[t * K + lane] : reinterpret_cast<const int32_t*>(a.topk_idx)[t * K + lane];
-            if (e >= 0 && e < E) {
-                expert = static_cast<int>(e);
-                dw = a.d_weights[t * K + lane] * a.scale;
+    constexpr int kParts = kRows / 4;
+    int held[kSets][kParts][2];                        // where this lane's values lie
+#pragma unroll
+    for (int s = 0; s < kSets; ++s)
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) held[s][p][0] = held[s][p][1] = -1;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * warps * kRows;
+    int64_t t0 = (static_cast<int64_t>(blockIdx.x) * warps + warp) * kRows;
+    while (t0 < a.num_tokens) {
+#pragma unroll
+        for (int s = 0; s < kSets; ++s) {
+            if (t0 >= a.num_tokens) break;
+            const int n = static_cast<int>(min(static_cast<int64_t>(kRows), a.num_tokens - t0));
+            T* rows = reinterpret_cast<T*>(mine + s * set_bytes);
+            float d[kParts][2];
+            int expert[kParts][2];
+#pragma unroll
+            for (int p = 0; p < kParts; ++p) {
+                const int t = p * 4 + t8;
+                float w[2] = {0.f, 0.f}, dw[2] = {0.f, 0.f}, logit[2], slope[2] = {1.f, 1.f};
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int k = q + i * 8;
+                    expert[p][i] = t < n && k < K ? chosen_expert(a, (t0 + t) * K + k) : -1;
+                    logit[i] = kNone;
+                    if (expert[p][i] >= 0) {
+                        dw[i] = a.d_weights[(t0 + t) * K + k] * a.scale;
+                        logit[i] = load_logit<kBf16>(reinterpret_cast<const uint8_t*>(a.logits) + (t0 + t) * a.ld * sizeof(T), expert[p][i]);
+                    }
+                }
+                // relative to the largest chosen logit: w = p / sum p needs no other
+                const float top = a.softmax ? over8(max_nan(logit[0], logit[1]), max_nan) : 0.f;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (expert[p][i] >= 0) {
+                        w[i] = a.softmax ? expf(logit[i] - top) : sigmoid(logit[i]);
+                        if (!a.softmax) slope[i] = sigmoid(-logit[i]);
+                    }
+                float along = 0.f;
+                if (a.renormalize) {
+                    const float sum = sum8(w[0] + w[1]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) w[i] = sum > 0.f ? __fdiv_rn(w[i], sum) : 0.f;
+                    along = sum8(dw[0] * w[0] + dw[1] * w[1]);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) d[p][i] = w[i] * (dw[i] - along) * slope[i];
             }
+            // the copy that last read this set has ended; its values go, the new ones come
+            if (lane == 0) ptx::bulk_wait_read<kSets - 1>();
+            __syncwarp();
+#pragma unroll
+            for (int p = 0; p < kParts; ++p)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (held[s][p][i] >= 0) rows[held[s][p][i]] = logit_of<T>(0.f);
+            __syncwarp();
+#pragma unroll
+            for (int p = 0; p < kParts; ++p)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    held[s][p][i] = expert[p][i] >= 0 ? (p * 4 + t8) * E + expert[p][i] : -1;
+                    if (expert[p][i] >= 0) rows[held[s][p][i]] = logit_of<T>(d[p][i]);
+                }
+            T* out = reinterpret_cast<T*>(a.d_logits) + t0 * E;
+            const int bytes = n * E * static_cast<int>(sizeof(T));
+            if (bytes % 16 == 0) {
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) ptx::bulk_store(out, rows, bytes);
+            } else {
+                __syncwarp();
+                for (int i = lane; i < n * E; i += 32) out[i] = rows[i];
+            }
+            if (lane == 0) ptx::bulk_commit();
+            t0 += step;
         }
+    }
+    if (lane == 0) ptx::bulk_wait_read<0>();
+}
+
+// Softmax weights as they are: every expert's logit has a gradient.  One warp per token; lane i has the experts i, i + 32, ...
+template <int kVals, bool kBf16>
+__global__ void __launch_bounds__(256) route_backward_all_kernel(const RouterArgs a) {
+    ptx::wait_for_previous_kernel();
+    ptx::let_next_kernel_start();
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5, E = a.num_experts, K = a.num_topk;
+    for (int64_t t = static_cast<int64_t>(blockIdx.x) * warps + (threadIdx.x >> 5); t < a.num_tokens; t += static_cast<int64_t>(gridDim.x) * warps) {
+        const uint8_t* row = reinterpret_cast<const uint8_t*>(a.logits) + t * a.ld * (kBf16 ? 2 : 4);
+        const int expert = lane < K ? chosen_expert(a, t * K + lane) : -1;
         float out[kVals];
 #pragma unroll
         for (int j = 0; j < kVals; ++j) out[j] = 0.f;
         if (__ballot_sync(0xffffffffu, expert >= 0) != 0) {
-            const float l = expert >= 0 ? load_logit<kBf16>(row, expert) : 0.f;
-            float d;
-            if (!a.softmax || a.renormalize) {
-                float p = 0.f, slope = 1.f;
-                if (a.softmax) {
-                    // relative to the largest chosen logit: w = p / sum p needs no other
-                    const float top = warp_max_nan(expert >= 0 ? l : -CUDART_INF_F);
-                    p = expert >= 0 ? expf(l - top) : 0.f;
-                } else if (expert >= 0) {
-                    p = sigmoid(l);
-                    slope = sigmoid(-l);
-                }
-                if (a.renormalize) {
-                    const float sum = warp_sum(p), w = sum > 0.f ? __fdiv_rn(p, sum) : 0.f;
-                    d = w * (dw - warp_sum(dw * w)) * slope;
-                } else {
-                    d = dw * p * slope;
-                }
-            } else {
-                float c[kVals], top, total;
+            const float dw = expert >= 0 ? a.d_weights[t * K + lane] * a.scale : 0.f;
+            float top = kNone, sum = 0.f;
 #pragma unroll
-                for (int j = 0; j < kVals; ++j) c[j] = j * 32 + lane < E ? load_logit<kBf16>(row, j * 32 + lane) : 0.f;
-                softmax_row<kVals>(c, lane, E, top, total);
-                const float p = expert >= 0 ? __fdiv_rn(expf(l - top), total) : 0.f;
-                const float along = warp_sum(dw * p);
-#pragma unroll
-                for (int j = 0; j < kVals; ++j) out[j] = -along * __fdiv_rn(c[j], total);
-                d = p * dw;
+            for (int j = 0; j < kVals; ++j) {
+                out[j] = j * 32 + lane < E ? load_logit<kBf16>(row, j * 32 + lane) : kNone;
+                top = max_nan(top, out[j]);
             }
+            top = warp_max_nan(top);
+#pragma unroll
+            for (int j = 0; j < kVals; ++j) sum += out[j] = expf(out[j] - top);
+            const float inverse = 1.f / warp_sum(sum);
+            const float d = expert >= 0 ? expf(load_logit<kBf16>(row, expert) - top) * inverse * dw : 0.f;
+            const float along = -warp_sum(d) * inverse;
+#pragma unroll
+            for (int j = 0; j < kVals; ++j) out[j] *= along;
             for (int k = 0; k < K; ++k) {
                 const int e = __shfl_sync(0xffffffffu, expert, k);
                 const float v = __shfl_sync(0xffffffffu, d, k);
@@ -239,43 +518,104 @@ __global__ void __launch_bounds__(kRouterWarps * 32) route_backward_kernel(const
     }
 }
 
+using RouteKernel = void (*)(RouterArgs, int);
+template <bool kBf16, bool kWide, bool kSoftmax>
+RouteKernel route_kernel_of(int experts) {
+    if (experts <= 64) return route_kernel<1, kBf16, kWide, kSoftmax>;
+    if (experts <= 128) return route_kernel<2, kBf16, kWide, kSoftmax>;
+    if (experts <= 256) return route_kernel<4, kBf16, kWide, kSoftmax>;
+    if (experts <= 512) return route_kernel<8, kBf16, kWide, kSoftmax>;
+    return route_kernel<16, kBf16, kWide, kSoftmax>;
+}
+template <bool kBf16>
+RouteKernel route_kernel_of(int experts, bool wide, bool softmax) {
+    if (wide) return softmax ? route_kernel_of<kBf16, true, true>(experts) : route_kernel_of<kBf16, true, false>(experts);
+    return softmax ? route_kernel_of<kBf16, false, true>(experts) : route_kernel_of<kBf16, false, false>(experts);
+}
 using RouterKernel = void (*)(RouterArgs);
-template <bool kBackward, bool kBf16>
-RouterKernel router_kernel(int experts) {
-    if (experts <= 32) return kBackward ? route_backward_kernel<1, kBf16> : route_kernel<1, kBf16>;
-    if (experts <= 64) return kBackward ? route_backward_kernel<2, kBf16> : route_kernel<2, kBf16>;
-    if (experts <= 128) return kBackward ? route_backward_kernel<4, kBf16> : route_kernel<4, kBf16>;
-    if (experts <= 256) return kBackward ? route_backward_kernel<8, kBf16> : route_kernel<8, kBf16>;
-    if (experts <= 512) return kBackward ? route_backward_kernel<16, kBf16> : route_kernel<16, kBf16>;
-    return kBackward ? route_backward_kernel<32, kBf16> : route_kernel<32, kBf16>;
+template <bool kBf16>
+RouterKernel backward_all_of(int experts) {
+    if (experts <= 32) return route_backward_all_kernel<1, kBf16>;
+    if (experts <= 64) return route_backward_all_kernel<2, kBf16>;
+    if (experts <= 128) return route_backward_all_kernel<4, kBf16>;
+    if (experts <= 256) return route_backward_all_kernel<8, kBf16>;
+    if (experts <= 512) return route_backward_all_kernel<16, kBf16>;
+    return route_backward_all_kernel<32, kBf16>;
 }
 
 bool bad_router_args(const RouterArgs& a) {
     return a.num_experts < 1 || a.num_experts > EP_MAX_EXPERTS || a.num_topk < 1 || a.num_topk > EP_MAX_TOPK || a.num_tokens < 0 || a.ld < a.num_experts;
 }
 
+// CTAs of a kernel that fit on an SM, asked for once per kernel and shape
+int resident_ctas(const void* fn, int threads, int smem) {
+    static std::mutex lock;
+    static std::map<std::tuple<const void*, int, int>, int> known;
+    const std::lock_guard<std::mutex> guard(lock);
+    int& n = known[{fn, threads, smem}];
+    if (n == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, threads, smem) != cudaSuccess) cudaGetLastError();
+        n = std::max(1, n);
+    }
+    return n;
+}
+cudaError_t allow_smem(const void* fn, int bytes) {
+    if (bytes <= 48 * 1024) return cudaSuccess;
+    const cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (err != cudaSuccess) cudaGetLastError();      // the caller reports it
+    return err;
+}
+// warps of a CTA: eight, or as many as have room
+int warps_of(int bytes_per_warp, int bytes) { return std::max(1, std::min(8, (200 * 1024 - bytes) / bytes_per_warp)); }
+
 }  // namespace
 
-cudaError_t launch_route(const RouterArgs& a, int num_sms, cudaStream_t stream) {
+cudaError_t launch_route(const RouterArgs& args, int num_sms, cudaStream_t stream) {
+    RouterArgs a = args;
     if (bad_router_args(a) || a.num_groups < 1 || a.num_groups > 32 || a.num_experts % a.num_groups != 0 || a.num_topk_groups < 1 || a.num_topk_groups > a.num_groups ||
         a.group_top < 1 || a.group_top > 2)
         return cudaErrorInvalidValue;
-    cudaError_t err = cudaMemsetAsync(a.count, 0, sizeof(int32_t) * a.num_experts, stream);
-    if (err != cudaSuccess || a.num_tokens == 0) return err;
-    const RouterKernel fn = a.logits_bf16 ? router_kernel<false, true>(a.num_experts) : router_kernel<false, false>(a.num_experts);
-    const size_t smem = sizeof(int) * a.num_experts * (a.num_groups > 1 ? 1 + kRouterWarps : 1);
-    const int64_t ctas = (a.num_tokens + kRouterWarps - 1) / kRouterWarps;
-    void* params[] = {const_cast<RouterArgs*>(&a)};
-    return launch_dependent(reinterpret_cast<const void*>(fn), dim3(static_cast<unsigned>(std::min<int64_t>(ctas, 8ll * num_sms))), dim3(kRouterWarps * 32), params, smem, stream);
+    if (a.num_tokens == 0) return cudaMemsetAsync(a.count, 0, sizeof(int32_t) * a.num_experts, stream);
+    const int size = a.logits_bf16 ? 2 : 4;
+    const bool wide = a.num_experts % 8 == 0 && a.ld * size % 16 == 0 && reinterpret_cast<uintptr_t>(a.logits) % 16 == 0;
+    const RouteKernel kernel = a.logits_bf16 ? route_kernel_of<true>(a.num_experts, wide, a.softmax != 0) : route_kernel_of<false>(a.num_experts, wide, a.softmax != 0);
+    const void* fn = reinterpret_cast<const void*>(kernel);
+    const RouteLayout l = route_layout(a.num_experts, a.num_groups, a.softmax != 0);
+    const int shared = 4 * (l.eights * 8 + a.num_experts);
+    // four tokens per warp where every SM gets some warps of them
+    int tokens = a.num_tokens >= 4 * 4 * num_sms ? kTokens : 1;
+    int warps = warps_of(4 * l.warp, shared);
+    if (a.num_tokens <= warps * tokens) warps = std::max(1, (a.num_tokens + tokens - 1) / tokens);
+    const int smem = warps * 4 * l.warp + shared;
+    cudaError_t err = allow_smem(fn, smem);
+    if (err != cudaSuccess) return err;
+    const int64_t per_cta = static_cast<int64_t>(warps) * tokens, ctas = (a.num_tokens + per_cta - 1) / per_cta;
+    const int grid = ctas == 1 ? 1 : static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(num_sms) * resident_ctas(fn, warps * 32, smem)));
+    if (grid > 1) err = cudaMemsetAsync(a.count, 0, sizeof(int32_t) * a.num_experts, stream);
+    if (err != cudaSuccess) return err;
+    void* params[] = {&a, &tokens};
+    return launch_dependent(fn, dim3(grid), dim3(warps * 32), params, smem, stream);
 }
 
-cudaError_t launch_route_backward(const RouterArgs& a, int num_sms, cudaStream_t stream) {
+cudaError_t launch_route_backward(const RouterArgs& args, int num_sms, cudaStream_t stream) {
+    RouterArgs a = args;
     if (bad_router_args(a)) return cudaErrorInvalidValue;
     if (a.num_tokens == 0) return cudaSuccess;
-    const RouterKernel fn = a.logits_bf16 ? router_kernel<true, true>(a.num_experts) : router_kernel<true, false>(a.num_experts);
-    const int64_t ctas = (a.num_tokens + kRouterWarps - 1) / kRouterWarps;
-    void* params[] = {const_cast<RouterArgs*>(&a)};
-    return launch_dependent(reinterpret_cast<const void*>(fn), dim3(static_cast<unsigned>(std::min<int64_t>(ctas, 8ll * num_sms))), dim3(kRouterWarps * 32), params, 0, stream);
+    void* params[] = {&a};
+    if (a.softmax && !a.renormalize) {
+        const RouterKernel kernel = a.logits_bf16 ? backward_all_of<true>(a.num_experts) : backward_all_of<false>(a.num_experts);
+        const int64_t ctas = (a.num_tokens + 7) / 8;
+        return launch_dependent(reinterpret_cast<const void*>(kernel), dim3(static_cast<unsigned>(std::min<int64_t>(ctas, 8ll * num_sms))), dim3(256), params, 0, stream);
+    }
+    if (reinterpret_cast<uintptr_t>(a.d_logits) % 16 != 0) return cudaErrorInvalidValue;
+    const RouterKernel kernel = a.logits_bf16 ? route_backward_kernel<true> : route_backward_kernel<false>;
+    const void* fn = reinterpret_cast<const void*>(kernel);
+    const int rows = a.logits_bf16 ? 8 : 4, per_warp = 2 * rows * a.num_experts * (a.logits_bf16 ? 2 : 4), warps = warps_of(per_warp, 0), smem = warps * per_warp;
+    const cudaError_t err = allow_smem(fn, smem);
+    if (err != cudaSuccess) return err;
+    const int64_t ctas = (a.num_tokens + warps * rows - 1) / (warps * rows);
+    const int grid = static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(num_sms) * resident_ctas(fn, warps * 32, smem)));
+    return launch_dependent(fn, dim3(grid), dim3(warps * 32), params, smem, stream);
 }
 
 }  // namespace ep
