@@ -111,7 +111,7 @@ __host__ __device__ inline RouteLayout route_layout(int experts, int groups, boo
 // shuffles of a step serve four tokens.  Bound by instruction issue: about half of what is left are the exact exponentials and reciprocals.
 // 65536 x 256 fp32, 8 of 256 in 4 of 8 groups: 59 us; one token per warp, with a maximum over the warp for every expert, took 139.
 template <int kSegs, bool kBf16, bool kWide, bool kSoftmax>
-__global__ void __launch_bounds__(256) route_kernel(const RouterArgs a, const int tokens) {
+__global__ void __launch_bounds__(256, kSoftmax || kSegs > 4 ? 2 : 4) route_kernel(const RouterArgs a, const int tokens) {
     extern __shared__ __align__(16) float route_smem[];
     const RouteLayout l = route_layout(a.num_experts, a.num_groups, kSoftmax);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, E = a.num_experts, K = a.num_topk, S = l.eights, G = a.num_groups;
@@ -124,10 +124,14 @@ __global__ void __launch_bounds__(256) route_kernel(const RouterArgs a, const in
     for (int e = threadIdx.x; e < E; e += blockDim.x) s_count[e] = 0;
     ptx::wait_for_previous_kernel();
     ptx::let_next_kernel_start();
-    for (int e = threadIdx.x; e < S * 8; e += blockDim.x) s_bias[e] = a.bias != nullptr && e < E ? a.bias[e] : 0.f;
+    int odd = 0;
+    for (int e = threadIdx.x; e < S * 8; e += blockDim.x) {
+        s_bias[e] = a.bias != nullptr && e < E ? a.bias[e] : 0.f;
+        odd |= !(fabsf(s_bias[e]) < -kNone);
+    }
     // eights past the last one of a token, which the lanes below look at, hold nobody
     for (int i = lane; i < 2 * kTokens * best_pitch; i += 32) best[i] = kNone;
-    __syncthreads();
+    const bool odd_bias = __syncthreads_or(odd) != 0;
     const int size = E / G;                            // experts of a group
     const bool whole = G > 1 && size % 8 == 0;         // groups of whole eights
     const int t8 = lane >> 3, q = lane & 7;            // token and place of the lane where eight lanes have a token
@@ -146,12 +150,11 @@ __global__ void __launch_bounds__(256) route_kernel(const RouterArgs a, const in
         best[t * best_pitch + seg] = v1;
         second[t * best_pitch + seg] = v2;
     };
-    // a choice that is no number, or whose logit is -inf, is nobody's
+    // A choice that is no number, or whose logit is -inf, is nobody's.  Looked at one by one only where the eight logits do not add up to a number, or the bias
+    // holds others than numbers.
     auto settle = [&](const float (&logit)[8], float (&c)[8]) {
-        float low = fminf(fminf(fminf(c[0], c[1]), fminf(c[2], c[3])), fminf(fminf(c[4], c[5]), fminf(c[6], c[7])));
-        float odd = ((c[0] + c[1]) + (c[2] + c[3])) + ((c[4] + c[5]) + (c[6] + c[7]));      // NaN if one of them is
-        low = fminf(low, fminf(fminf(fminf(logit[0], logit[1]), fminf(logit[2], logit[3])), fminf(fminf(logit[4], logit[5]), fminf(logit[6], logit[7]))));
-        if (!(low > kNone) || !(odd == odd)) {
+        const float sum = ((logit[0] + logit[1]) + (logit[2] + logit[3])) + ((logit[4] + logit[5]) + (logit[6] + logit[7]));
+        if (odd_bias || !(fabsf(sum) < -kNone)) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (!(c[i] > kNone) || !(logit[i] > kNone)) c[i] = kNone;
@@ -296,62 +299,63 @@ __global__ void __launch_bounds__(256) route_kernel(const RouterArgs a, const in
         }
         int chosen[2] = {-1, -1};                      // experts q and q + 8 of token t8
         float* c8 = choice + (t8 < n ? t8 : 0) * S * 8 + q;
+        const uint32_t ours = 0xffu << (t8 * 8);       // this token's lanes
+        const auto larger = [](float x, float y) { return fmaxf(x, y); };
+#pragma unroll 1
         for (int k = 0; k < K; ++k) {
             float largest = m[0];
 #pragma unroll
             for (int i = 1; i < kSegs; ++i) largest = fmaxf(largest, m[i]);
-            const float wanted = over8(largest, [](float x, float y) { return fmaxf(x, y); });
-            const bool some = wanted > kNone;
-            if (!__any_sync(0xffffffffu, some)) break;
-            // the first eight that has it, its first expert
+            const float wanted = over8(largest, larger);
+            // the first eight that has it, and there the first expert
+            const int owner = __ffs(__ballot_sync(0xffffffffu, largest == wanted) & ours) - 1;
             int at = 0;
 #pragma unroll
-            for (int i = kSegs - 1; i >= 0; --i)
+            for (int i = kSegs - 1; i > 0; --i)
                 if (m[i] == wanted) at = i;
-            const uint32_t owners = __ballot_sync(0xffffffffu, largest == wanted) >> (t8 * 8) & 0xffu;
-            const int owner = __ffs(owners) - 1, seg = __shfl_sync(0xffffffffu, q * kSegs + at, t8 * 8 + owner);
+            if (m[0] == wanted) at = 0;
+            const int seg = __shfl_sync(0xffffffffu, q * kSegs + at, owner);
+            const bool some = wanted > kNone;
             float c = some ? c8[seg * 8] : kNone;
-            const uint32_t hits = __ballot_sync(0xffffffffu, c == wanted) >> (t8 * 8) & 0xffu;
-            const int place = __ffs(hits) - 1;
-            if (some && q == place) c8[seg * 8] = c = kNone;
-            const float next = over8(c, [](float x, float y) { return fmaxf(x, y); });
-            if (some && q == owner) {
+            const int hit = __ffs(__ballot_sync(0xffffffffu, c == wanted) & ours) - 1;
+            if (some && lane == hit) c8[seg * 8] = c = kNone;
+            const float next = over8(c, larger);
+            if (lane == owner) {
 #pragma unroll
                 for (int i = 0; i < kSegs; ++i)
-                    if (i == at) m[i] = next;
+                    if (i == at) m[i] = next;          // (nobody left: -inf takes its own place)
             }
             if (some && q == (k & 7)) {
-                if (k < 8) chosen[0] = seg * 8 + place;
-                else chosen[1] = seg * 8 + place;
+                if (k < 8) chosen[0] = seg * 8 + (hit & 7);
+                else chosen[1] = seg * 8 + (hit & 7);
             }
         }
-        // weights
+        // weights: the lane's first expert, and its second one where a token has more than eight
         const uint8_t* row = rows + (t8 < n ? t8 : 0) * pitch;
-        float logit[2], p[2] = {0.f, 0.f};
+        const bool two = K > 8;
+        float logit[2] = {kNone, kNone}, p[2] = {0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 2; ++i) logit[i] = chosen[i] >= 0 ? load_logit<kBf16>(row, chosen[i]) : kNone;
+        for (int i = 0; i < 2; ++i)
+            if ((i == 0 || two) && chosen[i] >= 0) logit[i] = load_logit<kBf16>(row, chosen[i]);
         if constexpr (kSoftmax) {
             // renormalised weights are taken relative to the largest chosen logit: also right where p itself would vanish
             if (a.renormalize) top = over8(max_nan(logit[0], logit[1]), max_nan), total = 1.f;
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            if (chosen[i] >= 0) {
+            if ((i == 0 || two) && chosen[i] >= 0) {
                 p[i] = kSoftmax ? __fdiv_rn(expf(logit[i] - top), total) : sigmoid(logit[i]);
                 atomicAdd(&s_count[chosen[i]], 1);
             }
-        if (a.renormalize) {
-            const float sum = sum8(p[0] + p[1]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) p[i] = sum > 0.f ? __fdiv_rn(p[i], sum) : 0.f;
-        }
+        const float sum = a.renormalize ? sum8(p[0] + p[1]) : 1.f;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int k = q + i * 8;
-            if (t8 < n && k < K) {
+            if ((i == 0 || two) && t8 < n && k < K) {
                 const int64_t out = (t0 + t8) * K + k;
                 if (a.idx_is_64) reinterpret_cast<int64_t*>(a.topk_idx)[out] = chosen[i];
                 else reinterpret_cast<int32_t*>(a.topk_idx)[out] = chosen[i];
+                if (a.renormalize) p[i] = sum > 0.f ? __fdiv_rn(p[i], sum) : 0.f;
                 a.topk_weights[out] = p[i] * a.scale;
             }
         }
@@ -398,75 +402,103 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const RouterArgs a)
         for (int p = 0; p < kParts; ++p) held[s][p][0] = held[s][p][1] = -1;
     const int64_t step = static_cast<int64_t>(gridDim.x) * warps * kRows;
     int64_t t0 = (static_cast<int64_t>(blockIdx.x) * warps + warp) * kRows;
-    while (t0 < a.num_tokens) {
+    // Ids, weights' gradients and then logits wait for one another: ids come two batches ahead, logits one
+    struct Batch {
+        int expert[kParts][2];
+        float dw[kParts][2], logit[kParts][2];
+    };
+    const bool two = K > 8;
+    auto request_ids = [&](Batch& b, int64_t first) {
 #pragma unroll
-        for (int s = 0; s < kSets; ++s) {
-            if (t0 >= a.num_tokens) break;
-            const int n = static_cast<int>(min(static_cast<int64_t>(kRows), a.num_tokens - t0));
-            T* rows = reinterpret_cast<T*>(mine + s * set_bytes);
-            float d[kParts][2];
-            int expert[kParts][2];
+        for (int p = 0; p < kParts; ++p)
 #pragma unroll
-            for (int p = 0; p < kParts; ++p) {
-                const int t = p * 4 + t8;
-                float w[2] = {0.f, 0.f}, dw[2] = {0.f, 0.f}, logit[2], slope[2] = {1.f, 1.f};
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int k = q + i * 8;
-                    expert[p][i] = t < n && k < K ? chosen_expert(a, (t0 + t) * K + k) : -1;
-                    logit[i] = kNone;
-                    if (expert[p][i] >= 0) {
-                        dw[i] = a.d_weights[(t0 + t) * K + k] * a.scale;
-                        logit[i] = load_logit<kBf16>(reinterpret_cast<const uint8_t*>(a.logits) + (t0 + t) * a.ld * sizeof(T), expert[p][i]);
-                    }
+            for (int i = 0; i < 2; ++i) {
+                const int64_t t = first + p * 4 + t8;
+                b.expert[p][i] = -1;
+                b.dw[p][i] = 0.f;
+                if ((i == 0 || two) && t < a.num_tokens && q + i * 8 < K) {
+                    const int64_t at = t * K + q + i * 8;
+                    b.expert[p][i] = chosen_expert(a, at);
+                    b.dw[p][i] = a.d_weights[at];
                 }
-                // relative to the largest chosen logit: w = p / sum p needs no other
-                const float top = a.softmax ? over8(max_nan(logit[0], logit[1]), max_nan) : 0.f;
+            }
+    };
+    auto request_logits = [&](Batch& b, int64_t first) {
+#pragma unroll
+        for (int p = 0; p < kParts; ++p)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                b.logit[p][i] = b.expert[p][i] >= 0 ? load_logit<kBf16>(reinterpret_cast<const uint8_t*>(a.logits) + (first + p * 4 + t8) * a.ld * sizeof(T), b.expert[p][i]) : kNone;
+    };
+    Batch batch[3];
+    request_ids(batch[0], t0);
+    request_ids(batch[1], t0 + step);
+    request_logits(batch[0], t0);
+    int s = 0;
+    for (; t0 < a.num_tokens; t0 += step, s ^= 1) {
+        request_logits(batch[1], t0 + step);
+        request_ids(batch[2], t0 + 2 * step);
+        const Batch& b = batch[0];
+        const int n = static_cast<int>(min(static_cast<int64_t>(kRows), a.num_tokens - t0));
+        T* rows = reinterpret_cast<T*>(mine + s * set_bytes);
+        float d[kParts][2];
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) {
+            float w[2] = {0.f, 0.f}, dw[2], slope[2] = {1.f, 1.f};
+            // relative to the largest chosen logit: w = p / sum p needs no other
+            const float top = a.softmax ? over8(max_nan(b.logit[p][0], b.logit[p][1]), max_nan) : 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                dw[i] = b.expert[p][i] >= 0 ? b.dw[p][i] * a.scale : 0.f;
+                if ((i == 0 || two) && b.expert[p][i] >= 0) {
+                    w[i] = a.softmax ? expf(b.logit[p][i] - top) : sigmoid(b.logit[p][i]);
+                    if (!a.softmax) slope[i] = sigmoid(-b.logit[p][i]);
+                }
+            }
+            float along = 0.f;
+            if (a.renormalize) {
+                const float sum = sum8(w[0] + w[1]);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    if (expert[p][i] >= 0) {
-                        w[i] = a.softmax ? expf(logit[i] - top) : sigmoid(logit[i]);
-                        if (!a.softmax) slope[i] = sigmoid(-logit[i]);
-                    }
-                float along = 0.f;
-                if (a.renormalize) {
-                    const float sum = sum8(w[0] + w[1]);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) w[i] = sum > 0.f ? __fdiv_rn(w[i], sum) : 0.f;
-                    along = sum8(dw[0] * w[0] + dw[1] * w[1]);
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i) d[p][i] = w[i] * (dw[i] - along) * slope[i];
+                    if (i == 0 || two) w[i] = sum > 0.f ? __fdiv_rn(w[i], sum) : 0.f;
+                along = sum8(dw[0] * w[0] + dw[1] * w[1]);
             }
-            // the copy that last read this set has ended; its values go, the new ones come
-            if (lane == 0) ptx::bulk_wait_read<kSets - 1>();
-            __syncwarp();
 #pragma unroll
-            for (int p = 0; p < kParts; ++p)
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (held[s][p][i] >= 0) rows[held[s][p][i]] = logit_of<T>(0.f);
-            __syncwarp();
-#pragma unroll
-            for (int p = 0; p < kParts; ++p)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    held[s][p][i] = expert[p][i] >= 0 ? (p * 4 + t8) * E + expert[p][i] : -1;
-                    if (expert[p][i] >= 0) rows[held[s][p][i]] = logit_of<T>(d[p][i]);
-                }
-            T* out = reinterpret_cast<T*>(a.d_logits) + t0 * E;
-            const int bytes = n * E * static_cast<int>(sizeof(T));
-            if (bytes % 16 == 0) {
-                ptx::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) ptx::bulk_store(out, rows, bytes);
-            } else {
-                __syncwarp();
-                for (int i = lane; i < n * E; i += 32) out[i] = rows[i];
-            }
-            if (lane == 0) ptx::bulk_commit();
-            t0 += step;
+            for (int i = 0; i < 2; ++i) d[p][i] = w[i] * (dw[i] - along) * slope[i];
         }
+        // the copy that last read this set has ended; its values go, the new ones come
+        if (lane == 0) ptx::bulk_wait_read<kSets - 1>();
+        __syncwarp();
+#pragma unroll
+        for (int p = 0; p < kParts; ++p)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int old = s == 0 ? held[0][p][i] : held[1][p][i];
+                if (old >= 0) rows[old] = logit_of<T>(0.f);
+            }
+        __syncwarp();
+#pragma unroll
+        for (int p = 0; p < kParts; ++p)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int at = b.expert[p][i] >= 0 ? (p * 4 + t8) * E + b.expert[p][i] : -1;
+                if (s == 0) held[0][p][i] = at;
+                else held[1][p][i] = at;
+                if (at >= 0) rows[at] = logit_of<T>(d[p][i]);
+            }
+        T* out = reinterpret_cast<T*>(a.d_logits) + t0 * E;
+        const int bytes = n * E * static_cast<int>(sizeof(T));
+        if (bytes % 16 == 0) {
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::bulk_store(out, rows, bytes);
+        } else {
+            __syncwarp();
+            for (int i = lane; i < n * E; i += 32) out[i] = rows[i];
+        }
+        if (lane == 0) ptx::bulk_commit();
+        batch[0] = batch[1];
+        batch[1] = batch[2];
     }
     if (lane == 0) ptx::bulk_wait_read<0>();
 }
