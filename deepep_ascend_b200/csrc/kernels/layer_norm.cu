@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(kWarpRows ? 256 : kVec == 1 ? 512 : 1024) laye
 // bytes in flight for HBM.  (Single bf16 values are read when they are needed.)
 __host__ __device__ constexpr int norm_stages(int size, int vec, int values) { return size * vec < 4 ? 0 : size * values >= 64 ? 3 : 4; }
 template <class T, class P, int kVec, int kValues, bool kWarpRows, bool kBias>
-__global__ void __launch_bounds__(kWarpRows ? 256 : kValues == 8 ? 896 : 512) layer_norm_backward_kernel(const LayerNormArgs a) {
+__global__ void __launch_bounds__(kWarpRows ? 256 : kValues == 8 && kVec == 8 ? 896 : 512) layer_norm_backward_kernel(const LayerNormArgs a) {
     extern __shared__ __align__(16) uint8_t norm_smem[];
     __shared__ float scratch[2][32][2];
     using E = typename Piece<kVec>::E;
@@ -490,7 +490,10 @@ template <class T, class P>
 NormKernel forward_kernel(const NormShape& n) {
     constexpr int kVec = 16 / sizeof(T);
     if (n.values == 0) return layer_norm_wide_kernel<T, P>;
-    if (n.vec == 1) return n.warp_rows ? layer_norm_kernel<T, P, 1, 16, true> : layer_norm_kernel<T, P, 1, 16, false>;
+    if (n.vec == 1) {
+        if (n.values == 8) return n.warp_rows ? layer_norm_kernel<T, P, 1, 8, true> : layer_norm_kernel<T, P, 1, 8, false>;
+        return layer_norm_kernel<T, P, 1, 16, false>;
+    }
     if (n.warp_rows) return n.values == kVec ? layer_norm_kernel<T, P, kVec, 1, true> : layer_norm_kernel<T, P, kVec, 4, true>;
     return layer_norm_kernel<T, P, kVec, 4, false>;
 }
@@ -505,7 +508,7 @@ NormKernel backward_kernel(bool bias) {
 template <class T, class P, int kVec>
 NormKernel backward_kernel(const NormShape& n, bool bias) {
     if (n.warp_rows) return n.values == 8 ? backward_kernel<T, P, kVec, 8, true>(bias) : backward_kernel<T, P, kVec, 16, true>(bias);
-    if constexpr (kVec == 8)
+    if constexpr (kVec != 4)
         if (n.values == 8) return backward_kernel<T, P, kVec, 8, false>(bias);
     return backward_kernel<T, P, kVec, 16, false>(bias);
 }
@@ -555,15 +558,15 @@ cudaError_t launch_rows(const void* fn, const NormShape& n, void** params, cudaS
 
 }  // namespace
 
-// Pieces of 16 bytes where every row of every operand starts on 16 bytes, single values otherwise.  Four pieces (sixteen values) per thread, so that a row has few threads;
-// one where that makes do with a warp.
+// Pieces of 16 bytes where every row of every operand starts on 16 bytes, single values otherwise.  Four pieces (eight or sixteen values) per thread, so that a row has few
+// threads; one where that makes do with a warp.
 cudaError_t launch_layer_norm(const LayerNormArgs& args, int num_sms, cudaStream_t stream) {
     if (args.hidden < 1 || args.rows < 0) return cudaErrorInvalidValue;
     if (args.rows == 0) return cudaSuccess;
     LayerNormArgs a = args;
     NormShape n{};
     n.vec = rows_on_16_bytes(a, false) ? 16 / (a.x_bf16 ? 2 : 4) : 1;
-    n.values = n.vec == 1 ? 16 : a.hidden <= 32 * n.vec ? n.vec : 4 * n.vec;
+    n.values = n.vec == 1 ? (a.hidden <= 8 * 512 ? 8 : 16) : a.hidden <= 32 * n.vec ? n.vec : 4 * n.vec;
     n.threads = static_cast<int>((static_cast<int64_t>(a.hidden) + n.values - 1) / n.values + 31) / 32 * 32;
     n.warp_rows = n.threads == 32;
     n.rows_per_cta = n.warp_rows ? 8 : 1;
@@ -580,14 +583,15 @@ cudaError_t launch_layer_norm(const LayerNormArgs& args, int num_sms, cudaStream
 
 // Backward: pieces of 16 bytes where every row of every operand starts on 16 bytes, single values otherwise.  A warp per row up to 512 channels, then a CTA of up to
 // 512 threads with sixteen values of a row each (128 registers); wider rows stay in memory.  bf16 rows that leave room for one such CTA on an SM take eight values on up to
-// 896 threads: 8192 x 7168 78 us, with sixteen 82; 16384 x 4096 101 / 81, 32768 x 2048 87 / 78.
+// 896 threads: 8192 x 7168 78 us, with sixteen 82; 16384 x 4096 101 / 81, 32768 x 2048 87 / 78.  So do single values
+// up to 4096 channels.
 // (Whether there is a bias changes nothing, so that the weights' gradient has the same bits with and without.)
 NormShape layer_norm_backward_shape(const LayerNormArgs& a, int num_sms) {
     NormShape n{};
     const int size = a.x_bf16 ? 2 : 4;
     n.vec = rows_on_16_bytes(a, true) ? 16 / size : 1;
     n.warp_rows = a.hidden <= 512;
-    n.values = a.hidden <= 256 || (n.vec == 8 && a.hidden > 16 * 256 && a.hidden <= 8 * 896) ? 8 : a.hidden <= 16 * 512 ? 16 : 0;
+    n.values = a.hidden <= 256 || (n.vec == 8 && a.hidden > 16 * 256 && a.hidden <= 8 * 896) || (n.vec == 1 && a.hidden > 512 && a.hidden <= 8 * 512) ? 8 : a.hidden <= 16 * 512 ? 16 : 0;
     n.threads = n.values == 0 ? kWideThreads : n.warp_rows ? 32 : ((a.hidden + n.values - 1) / n.values + 31) / 32 * 32;
     n.rows_per_cta = n.warp_rows ? 8 : 1;
     n.smem = norm_stages(size, n.vec, n.values) * 2 * n.values * size * n.threads * n.rows_per_cta;
