@@ -16,6 +16,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "gemm_sm100.cuh"
@@ -134,13 +135,32 @@ __device__ __forceinline__ void unpack_half(const uint4& v, float (&f)[8]) {
     }
 }
 
+// What a product reads and writes beside its operands
+struct NsStep {
+    const __half *x_in, *sq_in;
+    __half *x_out, *sq_out;
+    void* out;               // the last step's result, or null
+};
+
 // 32 x 32 values of a tile lie on a warp as four rows (i * 8 + lane / 4) of eight neighbouring columns ((lane & 3) * 8) per lane: rows are read and written in
 // whole sectors.
 struct Block {
     int row0, col0;
     __device__ __forceinline__ int row(int i) const { return row0 + i * 8 + ((threadIdx.x & 31) >> 2); }
     __device__ __forceinline__ int col() const { return col0 + (threadIdx.x & 3) * 8; }
+    __device__ __forceinline__ bool on_diagonal(int i) const { return static_cast<uint32_t>(row(i) - col()) < 8u; }      // the lane's eight of row i hold it
 };
+// Value `at` of eight (0 if there is none), which is zero afterwards.  (Looked for by blocks on the diagonal alone: 32 tests per block took ten times as long as all
+// else that is done with its values.)
+__device__ __forceinline__ float take_diagonal(float (&v)[8], int at) {
+    float d = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        d = j == at ? v[j] : d;
+        v[j] = j == at ? 0.f : v[j];
+    }
+    return d;
+}
 // From one row per lane, as tensor memory gives them
 __device__ __forceinline__ void spread(uint8_t* staging, const uint32_t (&r)[32], float (&v)[4][8]) {
     const int lane = threadIdx.x & 31;
@@ -175,9 +195,27 @@ __device__ __forceinline__ void transposed(uint8_t* staging, const uint32_t (&o)
     }
     __syncwarp();
 }
+// The block as it is (or transposed: `o` staged so) row by row, a lane per value: for results whose rows do not start on 16 bytes, where eight lanes' pieces of
+// two bytes each took twice the time of the whole product.
+template <class Write>
+__device__ __forceinline__ void by_value(uint8_t* staging, const uint32_t (&o)[4][4], const Block& b, bool transpose, Write write) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int r = i * 8 + (lane >> 2), c = (lane & 3) * 8 + j;
+            *reinterpret_cast<uint16_t*>(staging + (transpose ? c * kTransposePitch + r * 2 : r * kTransposePitch + c * 2)) = static_cast<uint16_t>(o[i][j >> 1] >> (16 * (j & 1)));
+        }
+    __syncwarp();
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+        write((transpose ? b.col0 : b.row0) + r, (transpose ? b.row0 : b.col0) + lane, *reinterpret_cast<const uint16_t*>(staging + r * kTransposePitch + lane * 2));
+    __syncwarp();
+}
 // A symmetric result's block, and its mirror image
-__device__ __forceinline__ void store_symmetric(const NsArgs& g, uint8_t* staging, int matrix, const Block& b, const float (&v)[4][8], bool mirror) {
-    __half* out = g.sq_out + static_cast<int64_t>(matrix) * g.rows * g.ld_sq;
+__device__ __forceinline__ void store_symmetric(const NsArgs& g, __half* sq_out, uint8_t* staging, int matrix, const Block& b, const float (&v)[4][8], bool mirror) {
+    __half* out = sq_out + static_cast<int64_t>(matrix) * g.rows * g.ld_sq;
     uint32_t o[4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -192,335 +230,397 @@ __device__ __forceinline__ void store_symmetric(const NsArgs& g, uint8_t* stagin
         });
 }
 // X X^T in kUnitX^2 -> O and the diagonal.  (Columns past the end are sums of zeros.)
-__device__ __forceinline__ void finish_gram(const NsArgs& g, uint8_t* staging, int matrix, const Block& b, float (&v)[4][8], bool mirror) {
+__device__ __forceinline__ void finish_gram(const NsArgs& g, __half* sq_out, uint8_t* staging, int matrix, const Block& b, float (&v)[4][8], bool mirror) {
+    if (b.row0 == b.col0)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float d = take_diagonal(v[i], b.row(i) - b.col());
+            if (b.on_diagonal(i) && b.row(i) < g.rows) g.diag[static_cast<int64_t>(matrix) * g.ld_sq + b.row(i)] = d * (1.f / (kUnitX * kUnitX));
+        }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            if (b.row(i) == b.col() + j) {
-                if (b.row(i) < g.rows) g.diag[static_cast<int64_t>(matrix) * g.ld_sq + b.row(i)] = v[i][j] * (1.f / (kUnitX * kUnitX));
-                v[i][j] = 0.f;
-            }
-            v[i][j] *= kUnitA / (kUnitX * kUnitX);
-        }
-    store_symmetric(g, staging, matrix, b, v, mirror);
+        for (int j = 0; j < 8; ++j) v[i][j] *= kUnitA / (kUnitX * kUnitX);
+    store_symmetric(g, sq_out, staging, matrix, b, v, mirror);
 }
 
-// kGram: O, d = X X^T without its diagonal, and the diagonal; kGramPart: its sums over a part of K.  kPoly: B, coef = b A + c A A without its diagonal, and a + the
-// diagonal.  kUpdate: X <- coef X + B X.
+// What a product of `mode` runs over
 template <int kMode, int kBlockN>
-__global__ void __launch_bounds__(kNsThreads, 1)
-ns_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ NsArgs g) {
-    extern __shared__ __align__(1024) uint8_t smem[];
-    constexpr int kStages = ns_stages(kBlockN), kBytesA = kTileM * 128, kBytesB = kBlockN * 128;
-    constexpr bool kSymmetric = kMode != kUpdate;
-    constexpr int kTmemColumns = 2 * kBlockN;
-    constexpr uint32_t kIdesc = umma::make_instr_desc(kTileM, kBlockN, umma::kFormatF16, false, kMode == kUpdate);
-    uint8_t* s_a = smem;
-    uint8_t* s_b = smem + kStages * kBytesA;
-    NsSmem* sm = reinterpret_cast<NsSmem*>(smem + kStages * (kBytesA + kBytesB));
-    uint8_t* s_epi = smem + kStages * (kBytesA + kBytesB) + 1024;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int num_m = (g.rows + kTileM - 1) / kTileM;
-    const int per_matrix = kSymmetric ? symmetric_tiles<kBlockN>(g.rows) : num_m * ((g.cols + kBlockN - 1) / kBlockN);
-    const int num_tiles = per_matrix * g.count, num_items = kMode == kGramPart ? num_tiles * g.k_splits : num_tiles;
-    const int num_k = ((kMode == kGram || kMode == kGramPart ? g.cols : g.rows) + kTileK - 1) / kTileK;
+struct NsWork {
+    static constexpr bool kSymmetric = kMode != kUpdate;
+    int num_m, per_matrix, num_tiles, num_items, num_k, splits;
+    __device__ __forceinline__ explicit NsWork(const NsArgs& g) {
+        num_m = (g.rows + kTileM - 1) / kTileM;
+        per_matrix = kSymmetric ? symmetric_tiles<kBlockN>(g.rows) : num_m * ((g.cols + kBlockN - 1) / kBlockN);
+        splits = kMode == kGramPart ? g.k_splits : 1;
+        num_tiles = per_matrix * g.count;
+        num_items = num_tiles * splits;
+        num_k = ((kMode == kGram || kMode == kGramPart ? g.cols : g.rows) + kTileK - 1) / kTileK;
+    }
     // the K blocks of an item: all, or those of its part
-    auto k_begin = [&](int item) { return kMode == kGramPart ? num_k * (item / num_tiles) / g.k_splits : 0; };
-    auto k_end = [&](int item) { return kMode == kGramPart ? num_k * (item / num_tiles + 1) / g.k_splits : num_k; };
-    auto tile_of = [&](int item) { return ns_tile<kBlockN, kSymmetric>(kMode == kGramPart ? item % num_tiles : item, per_matrix, num_m); };
+    __device__ __forceinline__ int k_begin(int item) const { return kMode == kGramPart ? num_k * (item / num_tiles) / splits : 0; }
+    __device__ __forceinline__ int k_end(int item) const { return kMode == kGramPart ? num_k * (item / num_tiles + 1) / splits : num_k; }
+    __device__ __forceinline__ NsTile tile(int item) const { return ns_tile<kBlockN, kSymmetric>(kMode == kGramPart ? item % num_tiles : item, per_matrix, num_m); }
+};
+template <int kBlockN>
+struct NsShared {
+    static constexpr int kStages = ns_stages(kBlockN), kBytesA = kTileM * 128, kBytesB = kBlockN * 128;
+    uint8_t *a, *b, *staging;
+    NsSmem* sm;
+    __device__ __forceinline__ explicit NsShared(uint8_t* smem)
+        : a(smem), b(smem + kStages * kBytesA), staging(smem + kStages * (kBytesA + kBytesB) + 1024), sm(reinterpret_cast<NsSmem*>(smem + kStages * (kBytesA + kBytesB))) {}
+};
+template <int kBlockN>
+using NsRing = NsPipe<ns_stages(kBlockN)>;
 
+// One thread: requests the operands of this CTA's tiles
+template <int kMode, int kBlockN>
+__device__ __forceinline__ bool ns_load(const NsArgs& g, const NsShared<kBlockN>& s, const CUtensorMap* map_a, const CUtensorMap* map_b, NsRing<kBlockN>& p, int& loads) {
+    const NsWork<kMode, kBlockN> work(g);
+    constexpr int kBytesA = NsShared<kBlockN>::kBytesA, kBytesB = NsShared<kBlockN>::kBytesB;
+    for (int item = blockIdx.x; item < work.num_items; item += gridDim.x) {
+        const NsTile t = work.tile(item);
+        const int kb1 = work.k_end(item);
+        for (int kb = work.k_begin(item); kb < kb1; ++kb) {
+            if (!ns_wait(&s.sm->empty[p.stage], p.phase ^ 1, s.sm, g.report, 1)) return false;
+            ptx::mbar_arrive_expect_tx(&s.sm->full[p.stage], kBytesA + kBytesB);
+            umma::tma_load_3d(s.a + p.stage * kBytesA, map_a, kb * kTileK, t.m * kTileM, t.g, &s.sm->full[p.stage]);
+            if constexpr (kMode == kUpdate) {
+#pragma unroll
+                for (int i = 0; i < kBlockN / 64; ++i)
+                    umma::tma_load_3d(s.b + p.stage * kBytesB + i * umma::kMnChunkBytes, map_b, t.n * kBlockN + i * 64, kb * kTileK, t.g, &s.sm->full[p.stage]);
+            } else {
+                umma::tma_load_3d(s.b + p.stage * kBytesB, map_b, kb * kTileK, t.n * kBlockN, t.g, &s.sm->full[p.stage]);
+            }
+            loads = min(loads + 1, NsShared<kBlockN>::kStages);
+            p.advance();
+        }
+    }
+    return true;
+}
+// gives what is still in flight time to land before the shared memory goes to another CTA
+template <int kBlockN>
+__device__ __forceinline__ void ns_drain(const NsShared<kBlockN>& s, NsRing<kBlockN> p, int loads) {
+    for (; loads > 0; --loads) {
+        p.phase ^= p.stage == 0;
+        p.stage = p.stage == 0 ? NsShared<kBlockN>::kStages - 1 : p.stage - 1;
+        mbar_drain(&s.sm->full[p.stage], p.phase, 1000000000ull);
+    }
+}
+// One thread: issues the products
+template <int kMode, int kBlockN>
+__device__ __forceinline__ bool ns_multiply(const NsArgs& g, const NsShared<kBlockN>& s, uint32_t tmem_base, NsRing<kBlockN>& p, int& acc, uint32_t& acc_phase) {
+    const NsWork<kMode, kBlockN> work(g);
+    constexpr uint32_t kIdesc = umma::make_instr_desc(kTileM, kBlockN, umma::kFormatF16, false, kMode == kUpdate);
+    constexpr int kBytesA = NsShared<kBlockN>::kBytesA, kBytesB = NsShared<kBlockN>::kBytesB;
+    for (int item = blockIdx.x; item < work.num_items; item += gridDim.x) {
+        if (!ns_wait(&s.sm->acc_empty[acc], acc_phase ^ 1, s.sm, g.report, 2)) return false;
+        umma::fence_after_thread_sync();
+        const int kb0 = work.k_begin(item), kb1 = work.k_end(item);
+        for (int kb = kb0; kb < kb1; ++kb) {
+            if (!ns_wait(&s.sm->full[p.stage], p.phase, s.sm, g.report, 4)) return false;
+            umma::fence_after_thread_sync();
+            const uint64_t desc_a = umma::make_smem_desc_sw128(s.a + p.stage * kBytesA);
+            const uint64_t desc_b = kMode == kUpdate ? umma::make_smem_desc_mn_sw128(s.b + p.stage * kBytesB) : umma::make_smem_desc_sw128(s.b + p.stage * kBytesB);
+            constexpr int kStepB = kMode == kUpdate ? 16 * 128 : 32;       // 16 elements of K
+#pragma unroll
+            for (int k = 0; k < kTileK / 16; ++k)
+                umma::mma_ss<false>(tmem_base + acc * kBlockN, umma::advance_desc_k(desc_a, k * 32), umma::advance_desc_k(desc_b, k * kStepB), kIdesc, kb != kb0 || k != 0);
+            umma::mma_commit(&s.sm->empty[p.stage]);
+            p.advance();
+        }
+        umma::mma_commit(&s.sm->acc_full[acc]);
+        acc ^= 1;
+        acc_phase ^= acc == 0;
+    }
+    return true;
+}
+// Eight warps: kGram: O, d = X X^T without its diagonal, and the diagonal; kGramPart: its sums over a part of K.  kPoly: B, coef = b A + c A A without its diagonal, and
+// a + the diagonal.  kUpdate: X <- coef X + B X.
+template <int kMode, int kBlockN>
+__device__ __forceinline__ bool ns_finish(const NsArgs& g, const NsStep& step, const NsShared<kBlockN>& s, uint32_t tmem_base, int& acc, uint32_t& acc_phase) {
+    const NsWork<kMode, kBlockN> work(g);
+    constexpr int kChunks = kBlockN / 2 / 32;          // 32-column blocks of a warp
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* staging = s.staging + (warp - 2) * kStagingBytes;
+    for (int item = blockIdx.x; item < work.num_items; item += gridDim.x) {
+        const NsTile t = work.tile(item);
+        const int64_t sq = static_cast<int64_t>(t.g) * g.rows * g.ld_sq, wide = static_cast<int64_t>(t.g) * g.rows * g.ld_x, diag = static_cast<int64_t>(t.g) * g.ld_sq;
+        const int width = kMode != kUpdate ? g.ld_sq : g.ld_x;
+        auto block = [&](int c) { return Block{t.m * kTileM + quad * 32, t.n * kBlockN + half * (kBlockN / 2) + c * 32}; };
+        auto empty = [&](const Block& b) { return b.row0 >= g.rows || b.col0 >= width; };
+        // What the sums are combined with is requested a block ahead, that of the first one before the sums are there: waiting for it block by block
+        // took ten times as long as the products of a tile of 256 K.
+        uint4 old[2][4], low[2][4];
+        float row_value[4], col_value[2][8];
+        auto request = [&](int c, uint4 (&o)[4], uint4 (&l)[4], float (&cv)[8]) {
+            const Block b = block(c);
+            if (empty(b)) return;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool in = b.row(i) < g.rows && b.col() < width;
+                o[i] = l[i] = make_uint4(0, 0, 0, 0);
+                if constexpr (kMode == kPoly) {
+                    if (in) o[i] = *reinterpret_cast<const uint4*>(step.sq_in + sq + static_cast<int64_t>(b.row(i)) * g.ld_sq + b.col());
+                } else if constexpr (kMode == kUpdate) {
+                    if (in) {
+                        const int64_t at = wide + static_cast<int64_t>(b.row(i)) * g.ld_x + b.col();
+                        o[i] = *reinterpret_cast<const uint4*>(step.x_in + at);
+                        l[i] = *reinterpret_cast<const uint4*>(g.x_lo + at);
+                    }
+                }
+            }
+            if constexpr (kMode == kPoly) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) cv[j] = b.col() + j < g.rows ? g.diag[diag + b.col() + j] : 0.f;
+            }
+        };
+        if constexpr (kMode == kPoly || kMode == kUpdate) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = block(0).row(i);
+                row_value[i] = row >= g.rows ? 0.f : kMode == kPoly ? g.diag[diag + row] : g.coef[diag + row];
+            }
+            request(0, old[0], low[0], col_value[0]);
+        }
+        const bool ok = ns_wait(&s.sm->acc_full[acc], acc_phase, s.sm, g.report, 5);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        umma::fence_after_thread_sync();
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+            const Block b = block(c);
+            if (kMode != kGramPart && empty(b)) break;
+            if constexpr (kMode == kPoly || kMode == kUpdate)
+                if (c + 1 < kChunks) request(c + 1, old[(c + 1) & 1], low[(c + 1) & 1], col_value[(c + 1) & 1]);
+            float v[4][8];
+            {
+                uint32_t r[32];
+                umma::tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * kBlockN + half * (kBlockN / 2) + c * 32, r);
+                umma::tmem_ld_wait();
+                spread(staging, r, v);
+            }
+            if constexpr (kMode == kGram) {
+                finish_gram(g, step.sq_out, staging, t.g, b, v, t.mirror);
+            } else if constexpr (kMode == kGramPart) {
+                // [part][tile][128][kBlockN]
+                float* part = g.parts + static_cast<int64_t>(item) * kTileM * kBlockN + (b.col0 - t.n * kBlockN + (lane & 3) * 8);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float* p = part + (b.row(i) - t.m * kTileM) * kBlockN;
+                    *reinterpret_cast<float4*>(p) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+                    *reinterpret_cast<float4*>(p + 4) = make_float4(v[i][4], v[i][5], v[i][6], v[i][7]);
+                }
+            } else if constexpr (kMode == kPoly) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float f[8];
+                    unpack_half(old[c & 1][i], f);
+                    const float di = row_value[i], coefficient = g.b + g.c * di;
+                    if (b.row0 == b.col0) {
+                        const float d = take_diagonal(v[i], b.row(i) - b.col());
+                        if (b.on_diagonal(i) && b.row(i) < g.rows) g.coef[diag + b.row(i)] = g.a + g.b * di + g.c * (di * di + d * (1.f / (kUnitA * kUnitA)));
+                    }
+                    // (B in kUnitA; O O in kUnitA^2; O is zero on the diagonal)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[i][j] = (coefficient + g.c * col_value[c & 1][j]) * f[j] + g.c * (1.f / kUnitA) * v[i][j];
+                }
+                store_symmetric(g, step.sq_out, staging, t.g, b, v, t.mirror);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float hi[8], lo[8];
+                    unpack_half(old[c & 1][i], hi);
+                    unpack_half(low[c & 1][i], lo);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[i][j] = row_value[i] * (hi[j] + lo[j] * (1.f / kUnitLo)) + v[i][j] * (1.f / kUnitA);     // in kUnitX
+                }
+                if (step.out == nullptr) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t o[4], l[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            o[j] = pack_half(v[i][2 * j], v[i][2 * j + 1]);
+                            const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&o[j]));
+                            l[j] = pack_half((v[i][2 * j] - hi.x) * kUnitLo, (v[i][2 * j + 1] - hi.y) * kUnitLo);
+                        }
+                        if (b.row(i) < g.rows && b.col() < width) {
+                            const int64_t at = wide + static_cast<int64_t>(b.row(i)) * g.ld_x + b.col();
+                            *reinterpret_cast<uint4*>(step.x_out + at) = make_uint4(o[0], o[1], o[2], o[3]);
+                            *reinterpret_cast<uint4*>(g.x_lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+                        }
+                    }
+                } else {
+                    // the last step: the result, in the caller's orientation
+                    uint16_t* dst = reinterpret_cast<uint16_t*>(step.out) + static_cast<int64_t>(t.g) * g.rows * g.cols;
+                    uint32_t o[4][4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const __nv_bfloat162 h = __floats2bfloat162_rn(v[i][2 * j] * (1.f / kUnitX), v[i][2 * j + 1] * (1.f / kUnitX));
+                            o[i][j] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                    const int out_rows = g.out_transposed ? g.cols : g.rows, out_cols = g.out_transposed ? g.rows : g.cols;
+                    if (out_cols % 8 != 0) {
+                        by_value(staging, o, b, g.out_transposed != 0, [&](int row, int col, uint16_t value) {
+                            if (row < out_rows && col < out_cols) dst[static_cast<int64_t>(row) * out_cols + col] = value;
+                        });
+                    } else if (g.out_transposed) {
+                        transposed(staging, o, b, [&](int row, int col, const uint2& four) {
+                            if (row < out_rows && col < out_cols) *reinterpret_cast<uint2*>(dst + static_cast<int64_t>(row) * out_cols + col) = four;
+                        });
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (b.row(i) < out_rows && b.col() < out_cols)
+                                *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(b.row(i)) * out_cols + b.col()) = make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
+                    }
+                }
+            }
+        }
+        umma::fence_before_thread_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&s.sm->acc_empty[acc]);
+        acc ^= 1;
+        acc_phase ^= acc == 0;
+    }
+    return true;
+}
+
+template <int kBlockN>
+__device__ __forceinline__ uint32_t ns_setup(const NsShared<kBlockN>& s) {
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kStages; ++i) {
-            ptx::mbar_init(&sm->full[i], 1);
-            ptx::mbar_init(&sm->empty[i], 1);
+        for (int i = 0; i < NsShared<kBlockN>::kStages; ++i) {
+            ptx::mbar_init(&s.sm->full[i], 1);
+            ptx::mbar_init(&s.sm->empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            ptx::mbar_init(&sm->acc_full[i], 1);
-            ptx::mbar_init(&sm->acc_empty[i], kEpiWarps);
+            ptx::mbar_init(&s.sm->acc_full[i], 1);
+            ptx::mbar_init(&s.sm->acc_empty[i], kEpiWarps);
         }
-        ptx::mbar_init(&sm->quiet, 1);
-        sm->failed = 0;
+        ptx::mbar_init(&s.sm->quiet, 1);
+        s.sm->failed = 0;
         ptx::mbar_fence_init();
-        umma::prefetch_tensormap(&map_a);
-        umma::prefetch_tensormap(&map_b);
     }
-    if (warp == 1) {
-        umma::tmem_alloc(&sm->tmem_base, kTmemColumns);
+    if (threadIdx.x >> 5 == 1) {
+        umma::tmem_alloc(&s.sm->tmem_base, 2 * kBlockN);
         umma::tmem_relinquish();
     }
     umma::fence_before_thread_sync();
     __syncthreads();
     umma::fence_after_thread_sync();
-    const uint32_t tmem_base = sm->tmem_base;
-    ptx::wait_for_previous_kernel();
-
-    if (warp == 0) {
-        if (ptx::elect_one()) {
-            NsPipe<kStages> p;
-            int loads = 0;
-            bool ok = true;
-            for (int item = blockIdx.x; item < num_items && ok; item += gridDim.x) {
-                const NsTile t = tile_of(item);
-                const int kb1 = k_end(item);
-                for (int kb = k_begin(item); kb < kb1; ++kb) {
-                    ok = ns_wait(&sm->empty[p.stage], p.phase ^ 1, sm, g.report, 1);
-                    if (!ok) break;
-                    ptx::mbar_arrive_expect_tx(&sm->full[p.stage], kBytesA + kBytesB);
-                    umma::tma_load_3d(s_a + p.stage * kBytesA, &map_a, kb * kTileK, t.m * kTileM, t.g, &sm->full[p.stage]);
-                    if constexpr (kMode == kUpdate) {
-#pragma unroll
-                        for (int i = 0; i < kBlockN / 64; ++i)
-                            umma::tma_load_3d(s_b + p.stage * kBytesB + i * umma::kMnChunkBytes, &map_b, t.n * kBlockN + i * 64, kb * kTileK, t.g, &sm->full[p.stage]);
-                    } else {
-                        umma::tma_load_3d(s_b + p.stage * kBytesB, &map_b, kb * kTileK, t.n * kBlockN, t.g, &sm->full[p.stage]);
-                    }
-                    loads = min(loads + 1, kStages);
-                    p.advance();
-                }
-            }
-            ptx::let_next_kernel_start();
-            if (!ok) {      // give what is still in flight time to land before the shared memory goes to another CTA
-                for (; loads > 0; --loads) {
-                    p.phase ^= p.stage == 0;
-                    p.stage = p.stage == 0 ? kStages - 1 : p.stage - 1;
-                    mbar_drain(&sm->full[p.stage], p.phase, 1000000000ull);
-                }
-            }
-        }
-    } else if (warp == 1) {
-        if (ptx::elect_one()) {
-            NsPipe<kStages> p;
-            int acc = 0;
-            uint32_t acc_phase = 0;
-            bool ok = true;
-            for (int item = blockIdx.x; item < num_items && ok; item += gridDim.x) {
-                ok = ns_wait(&sm->acc_empty[acc], acc_phase ^ 1, sm, g.report, 2);
-                if (!ok) break;
-                umma::fence_after_thread_sync();
-                const int kb0 = k_begin(item), kb1 = k_end(item);
-                for (int kb = kb0; kb < kb1; ++kb) {
-                    ok = ns_wait(&sm->full[p.stage], p.phase, sm, g.report, 4);
-                    if (!ok) break;
-                    umma::fence_after_thread_sync();
-                    const uint64_t desc_a = umma::make_smem_desc_sw128(s_a + p.stage * kBytesA);
-                    const uint64_t desc_b = kMode == kUpdate ? umma::make_smem_desc_mn_sw128(s_b + p.stage * kBytesB) : umma::make_smem_desc_sw128(s_b + p.stage * kBytesB);
-                    constexpr int kStepB = kMode == kUpdate ? 16 * 128 : 32;       // 16 elements of K
-#pragma unroll
-                    for (int k = 0; k < kTileK / 16; ++k)
-                        umma::mma_ss<false>(tmem_base + acc * kBlockN, umma::advance_desc_k(desc_a, k * 32), umma::advance_desc_k(desc_b, k * kStepB), kIdesc,
-                                            kb != kb0 || k != 0);
-                    umma::mma_commit(&sm->empty[p.stage]);
-                    p.advance();
-                }
-                if (!ok) break;
-                umma::mma_commit(&sm->acc_full[acc]);
-                acc ^= 1;
-                acc_phase ^= acc == 0;
-            }
-            if (!ok) {      // products still under way end before the tensor memory is given back
-                umma::mma_commit(&sm->quiet);
-                mbar_drain(&sm->quiet, 0, 1000000000ull);
-            }
-        }
-    } else {
-        constexpr int kChunks = kBlockN / 2 / 32;          // 32-column blocks of a warp
-        const int quad = warp & 3, half = (warp - 2) >> 2;
-        uint8_t* staging = s_epi + (warp - 2) * kStagingBytes;
-        int acc = 0;
-        uint32_t acc_phase = 0;
-        for (int item = blockIdx.x; item < num_items; item += gridDim.x) {
-            const NsTile t = tile_of(item);
-            const int64_t sq = static_cast<int64_t>(t.g) * g.rows * g.ld_sq, wide = static_cast<int64_t>(t.g) * g.rows * g.ld_x, diag = static_cast<int64_t>(t.g) * g.ld_sq;
-            const int width = kSymmetric ? g.ld_sq : g.ld_x;
-            auto block = [&](int c) { return Block{t.m * kTileM + quad * 32, t.n * kBlockN + half * (kBlockN / 2) + c * 32}; };
-            auto empty = [&](const Block& b) { return b.row0 >= g.rows || b.col0 >= width; };
-            // What the sums are combined with is requested a block ahead, that of the first one before the sums are there: waiting for it block by block
-            // took ten times as long as the products of a tile of 256 K.
-            uint4 old[2][4], low[2][4];
-            float row_value[4], col_value[2][8];
-            auto request = [&](int c, uint4 (&o)[4], uint4 (&l)[4], float (&cv)[8]) {
-                const Block b = block(c);
-                if (empty(b)) return;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool in = b.row(i) < g.rows && b.col() < width;
-                    o[i] = l[i] = make_uint4(0, 0, 0, 0);
-                    if constexpr (kMode == kPoly) {
-                        if (in) o[i] = *reinterpret_cast<const uint4*>(g.sq_in + sq + static_cast<int64_t>(b.row(i)) * g.ld_sq + b.col());
-                    } else if constexpr (kMode == kUpdate) {
-                        if (in) {
-                            const int64_t at = wide + static_cast<int64_t>(b.row(i)) * g.ld_x + b.col();
-                            o[i] = *reinterpret_cast<const uint4*>(g.x_in + at);
-                            l[i] = *reinterpret_cast<const uint4*>(g.x_lo + at);
-                        }
-                    }
-                }
-                if constexpr (kMode == kPoly) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) cv[j] = b.col() + j < g.rows ? g.diag[diag + b.col() + j] : 0.f;
-                }
-            };
-            if constexpr (kMode == kPoly || kMode == kUpdate) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int row = block(0).row(i);
-                    row_value[i] = row >= g.rows ? 0.f : kMode == kPoly ? g.diag[diag + row] : g.coef[diag + row];
-                }
-                request(0, old[0], low[0], col_value[0]);
-            }
-            const bool ok = ns_wait(&sm->acc_full[acc], acc_phase, sm, g.report, 5);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            umma::fence_after_thread_sync();
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-                const Block b = block(c);
-                if (kMode != kGramPart && empty(b)) break;
-                if constexpr (kMode == kPoly || kMode == kUpdate)
-                    if (c + 1 < kChunks) request(c + 1, old[(c + 1) & 1], low[(c + 1) & 1], col_value[(c + 1) & 1]);
-                float v[4][8];
-                {
-                    uint32_t r[32];
-                    umma::tmem_ld_32x32(tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + acc * kBlockN + half * (kBlockN / 2) + c * 32, r);
-                    umma::tmem_ld_wait();
-                    spread(staging, r, v);
-                }
-                if constexpr (kMode == kGram) {
-                    finish_gram(g, staging, t.g, b, v, t.mirror);
-                } else if constexpr (kMode == kGramPart) {
-                    // [part][tile][128][kBlockN]
-                    float* part = g.parts + static_cast<int64_t>(item) * kTileM * kBlockN + (b.col0 - t.n * kBlockN + (lane & 3) * 8);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float* p = part + (b.row(i) - t.m * kTileM) * kBlockN;
-                        *reinterpret_cast<float4*>(p) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
-                        *reinterpret_cast<float4*>(p + 4) = make_float4(v[i][4], v[i][5], v[i][6], v[i][7]);
-                    }
-                } else if constexpr (kMode == kPoly) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float f[8];
-                        unpack_half(old[c & 1][i], f);
-                        const float di = row_value[i];
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            if (b.row(i) == b.col() + j) {
-                                if (b.row(i) < g.rows) g.coef[diag + b.row(i)] = g.a + g.b * di + g.c * (di * di + v[i][j] * (1.f / (kUnitA * kUnitA)));
-                                v[i][j] = 0.f;
-                            } else {        // (B in kUnitA; O O in kUnitA^2)
-                                v[i][j] = (g.b + g.c * (di + col_value[c & 1][j])) * f[j] + g.c * (1.f / kUnitA) * v[i][j];
-                            }
-                        }
-                    }
-                    store_symmetric(g, staging, t.g, b, v, t.mirror);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float hi[8], lo[8];
-                        unpack_half(old[c & 1][i], hi);
-                        unpack_half(low[c & 1][i], lo);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) v[i][j] = row_value[i] * (hi[j] + lo[j] * (1.f / kUnitLo)) + v[i][j] * (1.f / kUnitA);     // in kUnitX
-                    }
-                    if (g.out == nullptr) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint32_t o[4], l[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                o[j] = pack_half(v[i][2 * j], v[i][2 * j + 1]);
-                                const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&o[j]));
-                                l[j] = pack_half((v[i][2 * j] - hi.x) * kUnitLo, (v[i][2 * j + 1] - hi.y) * kUnitLo);
-                            }
-                            if (b.row(i) < g.rows && b.col() < width) {
-                                const int64_t at = wide + static_cast<int64_t>(b.row(i)) * g.ld_x + b.col();
-                                *reinterpret_cast<uint4*>(g.x_out + at) = make_uint4(o[0], o[1], o[2], o[3]);
-                                *reinterpret_cast<uint4*>(g.x_lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
-                            }
-                        }
-                    } else {
-                        // the last step: the result, in the caller's orientation
-                        uint16_t* dst = reinterpret_cast<uint16_t*>(g.out) + static_cast<int64_t>(t.g) * g.rows * g.cols;
-                        uint32_t o[4][4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) {
-                                const __nv_bfloat162 h = __floats2bfloat162_rn(v[i][2 * j] * (1.f / kUnitX), v[i][2 * j + 1] * (1.f / kUnitX));
-                                o[i][j] = *reinterpret_cast<const uint32_t*>(&h);
-                            }
-                        if (g.out_transposed) {
-                            transposed(staging, o, b, [&](int row, int col, const uint2& four) {
-                                if (row >= g.cols) return;
-                                uint16_t* p = dst + static_cast<int64_t>(row) * g.rows + col;
-                                if (g.rows % 4 == 0) {
-                                    if (col < g.rows) *reinterpret_cast<uint2*>(p) = four;
-                                } else {
-#pragma unroll
-                                    for (int j = 0; j < 4; ++j)
-                                        if (col + j < g.rows) p[j] = static_cast<uint16_t>((j < 2 ? four.x : four.y) >> (16 * (j & 1)));
-                                }
-                            });
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                if (b.row(i) >= g.rows || b.col() >= width) continue;
-                                uint16_t* p = dst + static_cast<int64_t>(b.row(i)) * g.cols + b.col();
-                                if (g.cols % 8 == 0) {
-                                    *reinterpret_cast<uint4*>(p) = make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
-                                } else {
-#pragma unroll
-                                    for (int j = 0; j < 8; ++j)
-                                        if (b.col() + j < g.cols) p[j] = static_cast<uint16_t>(o[i][j >> 1] >> (16 * (j & 1)));
-                                }
-                            }
-                        }
-                    }
-                }
-            }
-            umma::fence_before_thread_sync();
-            __syncwarp();
-            if (lane == 0) ptx::mbar_arrive(&sm->acc_empty[acc]);
-            acc ^= 1;
-            acc_phase ^= acc == 0;
-        }
-    }
+    return s.sm->tmem_base;
+}
+template <int kBlockN>
+__device__ __forceinline__ void ns_teardown(uint32_t tmem_base) {
     umma::fence_before_thread_sync();
     __syncthreads();
-    if (warp == 1) umma::tmem_dealloc(tmem_base, kTmemColumns);
+    if (threadIdx.x >> 5 == 1) umma::tmem_dealloc(tmem_base, 2 * kBlockN);
+}
+// products still under way end before the tensor memory is given back
+template <int kBlockN>
+__device__ __forceinline__ void ns_quiet(const NsShared<kBlockN>& s) {
+    umma::mma_commit(&s.sm->quiet);
+    mbar_drain(&s.sm->quiet, 0, 1000000000ull);
 }
 
-// Adds the parts of X X^T in their order: a warp per 32 x 32 block of a tile
+// One product of one step
+template <int kMode, int kBlockN>
+__global__ void __launch_bounds__(kNsThreads, 1)
+ns_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ NsArgs g) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const NsShared<kBlockN> s(smem);
+    const int warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        umma::prefetch_tensormap(&map_a);
+        umma::prefetch_tensormap(&map_b);
+    }
+    const uint32_t tmem_base = ns_setup(s);
+    ptx::wait_for_previous_kernel();
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    NsRing<kBlockN> p;
+    if (warp == 0) {
+        if (ptx::elect_one()) {
+            int loads = 0;
+            const bool ok = ns_load<kMode, kBlockN>(g, s, &map_a, &map_b, p, loads);
+            ptx::let_next_kernel_start();
+            if (!ok) ns_drain(s, p, loads);
+        }
+    } else if (warp == 1) {
+        if (ptx::elect_one() && !ns_multiply<kMode, kBlockN>(g, s, tmem_base, p, acc, acc_phase)) ns_quiet(s);
+    } else {
+        ns_finish<kMode, kBlockN>(g, NsStep{g.x_in, g.sq_in, g.x_out, g.sq_out, g.out}, s, tmem_base, acc, acc_phase);
+    }
+    ns_teardown<kBlockN>(tmem_base);
+}
+
+// Eight rows of 32 values of a tile: the parts of X X^T added in their order, eight requested at a time.  Many small pieces, since what this takes is the way of the parts
+// through L2.
+template <int kBlockN>
+struct NsAdd {
+    static constexpr int kPieces = (kTileM / 8) * (kBlockN / 32);      // of a tile
+};
+template <int kBlockN>
+__device__ __forceinline__ void ns_add_piece(const NsArgs& g, __half* sq_out, uint8_t* staging, int tile, int piece, int per_matrix, int num_tiles) {
+    const int lane = threadIdx.x & 31;
+    const NsTile t = ns_tile<kBlockN, true>(tile, per_matrix, 0);
+    const int r = piece / (kBlockN / 32) * 8 + (lane >> 2), c = piece % (kBlockN / 32) * 32 + (lane & 3) * 8;
+    const int row0 = t.m * kTileM + piece / (kBlockN / 32) * 8, col0 = t.n * kBlockN + piece % (kBlockN / 32) * 32, row = t.m * kTileM + r, col = t.n * kBlockN + c;
+    if (row0 >= g.rows || col0 >= g.ld_sq) return;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+    const float* part = g.parts + (static_cast<int64_t>(tile) * kTileM + r) * kBlockN + c;
+    const int64_t pitch = static_cast<int64_t>(num_tiles) * kTileM * kBlockN;
+    for (int s0 = 0; s0 < g.k_splits; s0 += 8) {
+        float4 x[8], y[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+            if (s0 + s < g.k_splits) {
+                x[s] = *reinterpret_cast<const float4*>(part + (s0 + s) * pitch);
+                y[s] = *reinterpret_cast<const float4*>(part + (s0 + s) * pitch + 4);
+            }
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+            if (s0 + s < g.k_splits) {
+                v[0] += x[s].x, v[1] += x[s].y, v[2] += x[s].z, v[3] += x[s].w;
+                v[4] += y[s].x, v[5] += y[s].y, v[6] += y[s].z, v[7] += y[s].w;
+            }
+    }
+    if (row0 >= col0 && row0 < col0 + 32) {
+        const float d = take_diagonal(v, row - col);
+        if (static_cast<uint32_t>(row - col) < 8u && row < g.rows) g.diag[static_cast<int64_t>(t.g) * g.ld_sq + row] = d * (1.f / (kUnitX * kUnitX));
+    }
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = pack_half(v[2 * j] * (kUnitA / (kUnitX * kUnitX)), v[2 * j + 1] * (kUnitA / (kUnitX * kUnitX)));
+    __half* out = sq_out + static_cast<int64_t>(t.g) * g.rows * g.ld_sq;
+    if (row < g.rows && col < g.ld_sq) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row) * g.ld_sq + col) = make_uint4(o[0], o[1], o[2], o[3]);
+    if (t.mirror) {
+        // the mirror image: 32 rows of eight values
+#pragma unroll
+        for (int j = 0; j < 8; ++j) *reinterpret_cast<uint16_t*>(staging + ((lane & 3) * 8 + j) * 16 + (lane >> 2) * 2) = static_cast<uint16_t>(o[j >> 1] >> (16 * (j & 1)));
+        __syncwarp();
+        if (col0 + lane < g.rows && row0 < g.ld_sq)
+            *reinterpret_cast<uint4*>(out + static_cast<int64_t>(col0 + lane) * g.ld_sq + row0) = *reinterpret_cast<const uint4*>(staging + lane * 16);
+        __syncwarp();
+    }
+}
+
+// Adds the parts of X X^T: a warp per piece
 constexpr int kAddThreads = 128;
 template <int kBlockN>
 __global__ void __launch_bounds__(kAddThreads) ns_add_kernel(const __grid_constant__ NsArgs g) {
-    __shared__ __align__(16) uint8_t s_staging[kAddThreads / 32][kStagingBytes];
+    __shared__ __align__(16) uint8_t s_staging[kAddThreads / 32][512];
     ptx::wait_for_previous_kernel();
     ptx::let_next_kernel_start();
-    const int lane = threadIdx.x & 31, per_matrix = symmetric_tiles<kBlockN>(g.rows), num_tiles = per_matrix * g.count;
+    const int per_matrix = symmetric_tiles<kBlockN>(g.rows), num_tiles = per_matrix * g.count;
     const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kAddThreads / 32) + (threadIdx.x >> 5);
-    constexpr int kBlocks = (kTileM / 32) * (kBlockN / 32);
-    const int tile = static_cast<int>(unit / kBlocks), in_tile = static_cast<int>(unit % kBlocks);
-    if (tile >= num_tiles) return;
-    const NsTile t = ns_tile<kBlockN, true>(tile, per_matrix, 0);
-    const int r0 = in_tile / (kBlockN / 32) * 32, c0 = in_tile % (kBlockN / 32) * 32;
-    const Block b{t.m * kTileM + r0, t.n * kBlockN + c0};
-    if (b.row0 >= g.rows || b.col0 >= g.ld_sq) return;
-    float v[4][8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-    const float* part = g.parts + (static_cast<int64_t>(tile) * kTileM + r0 + (lane >> 2)) * kBlockN + c0 + (lane & 3) * 8;
-#pragma unroll 2
-    for (int s = 0; s < g.k_splits; ++s, part += static_cast<int64_t>(num_tiles) * kTileM * kBlockN)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 x = *reinterpret_cast<const float4*>(part + i * 8 * kBlockN), y = *reinterpret_cast<const float4*>(part + i * 8 * kBlockN + 4);
-            v[i][0] += x.x, v[i][1] += x.y, v[i][2] += x.z, v[i][3] += x.w;
-            v[i][4] += y.x, v[i][5] += y.y, v[i][6] += y.z, v[i][7] += y.w;
-        }
-    finish_gram(g, s_staging[threadIdx.x >> 5], t.g, b, v, t.mirror);
+    constexpr int kPieces = NsAdd<kBlockN>::kPieces;
+    if (unit < static_cast<int64_t>(num_tiles) * kPieces)
+        ns_add_piece<kBlockN>(g, g.sq_out, s_staging[threadIdx.x >> 5], static_cast<int>(unit / kPieces), static_cast<int>(unit % kPieces), per_matrix, num_tiles);
 }
 
 // ------------------------------------------------------------------------------------------------ the first X
@@ -672,13 +772,23 @@ int k_splits_of(const NsArgs& g, int num_sms) {
     return static_cast<int>(best);
 }
 
+cudaError_t allow_smem(const void* fn, int bytes) {
+    const cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (err != cudaSuccess) cudaGetLastError();      // the caller reports it
+    return err;
+}
 template <int kMode, int kBlockN>
 cudaError_t launch_product(const CUtensorMap& map_a, const CUtensorMap& map_b, const NsArgs& g, int num_sms, cudaStream_t stream) {
     const void* fn = reinterpret_cast<const void*>(ns_kernel<kMode, kBlockN>);
-    const cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, ns_smem_bytes(kBlockN));
-    if (err != cudaSuccess) {
-        cudaGetLastError();      // the caller reports it
-        return err;
+    // leave for that much shared memory is asked for once per device: a step has three launches, and they are what small matrices take
+    static std::atomic<uint64_t> allowed{0};
+    int device = 0;
+    cudaError_t err = cudaGetDevice(&device);
+    if (err != cudaSuccess) return err;
+    if (device >= 64 || (allowed.load(std::memory_order_relaxed) >> device & 1) == 0) {
+        err = allow_smem(fn, ns_smem_bytes(kBlockN));
+        if (err != cudaSuccess) return err;
+        if (device < 64) allowed.fetch_or(1ull << device, std::memory_order_relaxed);
     }
     const int64_t items = tiles_of(g, kMode, kBlockN) * (kMode == kGramPart ? g.k_splits : 1);
     void* params[] = {const_cast<CUtensorMap*>(&map_a), const_cast<CUtensorMap*>(&map_b), const_cast<NsArgs*>(&g)};
@@ -764,7 +874,7 @@ cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8
             err = launch_product<kGramPart, 128>(x_rows[from], x_cols[from], g, num_sms, stream);
             if (err != cudaSuccess) break;
             void* params[] = {&g};
-            const int64_t warps = tiles_of(g, kGram, 128) * (kTileM / 32) * (128 / 32);
+            const int64_t warps = tiles_of(g, kGram, 128) * NsAdd<128>::kPieces;
             err = launch_dependent(reinterpret_cast<const void*>(ns_add_kernel<128>), dim3(static_cast<unsigned>(warps * 32 / kAddThreads)), dim3(kAddThreads), params, 0, stream);
         } else {
             err = launch_product<kGram>(n_gram, x_rows[from], x_cols[from], g, num_sms, stream);

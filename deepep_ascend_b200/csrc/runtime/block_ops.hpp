@@ -15,6 +15,15 @@ namespace ep_host {
 
 inline int device_sms() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; }
 
+// A contiguous tensor on a part of `bytes`, an allocation that several results of one call share: making them one by one is a fifth of the time of a small call
+inline at::Tensor part_of(const at::Tensor& bytes, int64_t offset, at::IntArrayRef sizes, at::ScalarType type) {
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(bytes.storage()), bytes.key_set(), c10::scalarTypeToTypeMeta(type));
+    impl->set_storage_offset(offset / static_cast<int64_t>(c10::elementSize(type)));
+    impl->set_sizes_contiguous(sizes);
+    return at::Tensor(std::move(impl));
+}
+inline int64_t round16(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
 inline void router_logits(RouterArgs& a, const at::Tensor& logits) {
     TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && (logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16),
                 "logits must be fp32 or bf16 [tokens, experts] on a GPU");
@@ -51,9 +60,11 @@ inline std::tuple<at::Tensor, at::Tensor, at::Tensor> route(const at::Tensor& lo
                     "token_mask must be contiguous bool [tokens] on the device of the logits");
         a.token_mask = reinterpret_cast<const uint8_t*>(token_mask->data_ptr<bool>());
     }
-    at::Tensor idx = at::empty({a.num_tokens, num_topk}, logits.options().dtype(idx_is_64 ? at::kLong : at::kInt));
-    at::Tensor weights = at::empty({a.num_tokens, num_topk}, logits.options().dtype(at::kFloat));
-    at::Tensor count = at::empty({a.num_experts}, logits.options().dtype(at::kInt));
+    const int64_t pairs = a.num_tokens * num_topk, idx_bytes = round16(pairs * (idx_is_64 ? 8 : 4)), weight_bytes = round16(pairs * 4);
+    at::Tensor results = at::empty({idx_bytes + weight_bytes + 4 * a.num_experts}, logits.options().dtype(at::kByte));
+    at::Tensor idx = part_of(results, 0, {a.num_tokens, num_topk}, idx_is_64 ? at::kLong : at::kInt);
+    at::Tensor weights = part_of(results, idx_bytes, {a.num_tokens, num_topk}, at::kFloat);
+    at::Tensor count = part_of(results, idx_bytes + weight_bytes, {a.num_experts}, at::kInt);
     a.num_topk = static_cast<int>(num_topk);
     a.softmax = softmax;
     a.renormalize = renormalize;
@@ -118,7 +129,8 @@ inline std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tenso
     }
     const c10::cuda::CUDAGuard guard(x.device());
     at::Tensor y = at::empty({x.size(0), x.size(1)}, x.options());
-    at::Tensor mean = at::empty({x.size(0)}, x.options().dtype(at::kFloat)), rstd = at::empty({x.size(0)}, mean.options());
+    at::Tensor moments = at::empty({2 * round16(4 * x.size(0))}, x.options().dtype(at::kByte));
+    at::Tensor mean = part_of(moments, 0, {x.size(0)}, at::kFloat), rstd = part_of(moments, round16(4 * x.size(0)), {x.size(0)}, at::kFloat);
     a.eps = static_cast<float>(eps);
     a.y = y.data_ptr();
     a.mean = mean.data_ptr<float>();
@@ -137,10 +149,12 @@ inline std::tuple<at::Tensor, at::Tensor, std::optional<at::Tensor>> layer_norm_
         TORCH_CHECK(t->device() == x.device() && t->scalar_type() == at::kFloat && t->is_contiguous() && t->dim() == 1 && t->size(0) == x.size(0),
                     "mean and rstd must be contiguous fp32 [rows] on the device of x");
     const c10::cuda::CUDAGuard guard(x.device());
-    at::Tensor dx = at::empty({x.size(0), x.size(1)}, x.options()), dw = at::empty({x.size(1)}, weight.options());
+    at::Tensor dx = at::empty({x.size(0), x.size(1)}, x.options());
+    const int64_t width_bytes = round16(x.size(1) * weight.element_size());
+    at::Tensor sums = at::empty({width_bytes * (with_bias ? 2 : 1)}, x.options().dtype(at::kByte)), dw = part_of(sums, 0, {x.size(1)}, weight.scalar_type());
     std::optional<at::Tensor> db;
     if (with_bias) {
-        db = at::empty({x.size(1)}, weight.options());
+        db = part_of(sums, width_bytes, {x.size(1)}, weight.scalar_type());
         a.db = db->data_ptr();
     }
     a.dy = dy.data_ptr();
@@ -197,7 +211,7 @@ inline at::Tensor orthogonalize(const at::Tensor& x, int64_t steps, double a, do
         g.report.status_rank = ctx.rank;
         g.report.timeout_ns = ctx.timeout_ns;
     }
-    const int sms = num_sms > 0 ? static_cast<int>(num_sms) : device_sms();
+    const int sms = num_sms > 0 ? static_cast<int>(std::min<int64_t>(num_sms, device_sms())) : device_sms();
     const NsWorkspace w = ep::newton_schulz_workspace(g, sms);
     at::Tensor workspace = at::empty({w.bytes}, x.options().dtype(at::kByte));
     cuda_check(ep::launch_newton_schulz(g, w, workspace.data_ptr<uint8_t>(), static_cast<int>(steps), sms, at::cuda::getCurrentCUDAStream()), "orthogonalisation launch");
