@@ -10,8 +10,9 @@ from .. import _native
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
     """``x`` as a matrix of rows with contiguous channels: a view where there is one."""
-    x = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -20,8 +21,11 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     the statistics fp32, one of each per row, in ``x``'s leading shape.  ``weight`` and ``bias`` ``[H]``: both bf16 or both fp32."""
     if not x.is_cuda:
         return layer_norm_ref(x, weight, bias, eps)
-    y, mean, rstd = _native.load().layer_norm(_rows(x), weight, bias, eps)
-    return (y, mean, rstd) if x.dim() == 2 else (y.view(x.shape), mean.view(x.shape[:-1]), rstd.view(x.shape[:-1]))
+    res = _native.load().layer_norm(_rows(x), weight, bias, eps)
+    if x.dim() == 2:
+        return res
+    y, mean, rstd = res
+    return y.view(x.shape), mean.view(x.shape[:-1]), rstd.view(x.shape[:-1])
 
 
 def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
