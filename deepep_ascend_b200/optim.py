@@ -1,0 +1,44 @@
+"""Optimiser for the matrices of the library's layers: Muon, whose update is the orthogonalised momentum (``ops.muon``).
+
+An expert's matrices live whole on one rank, so the update of a stack of experts needs no communication; replicated matrices (a gate) get the
+same update on every rank from gradients that the caller has averaged.  No counterpart in the reference.
+"""
+import torch
+
+from .ops.muon import COEFFICIENTS, orthogonalize
+
+
+class Muon(torch.optim.Optimizer):
+    """``momentum = beta * momentum + grad``; ``update = orthogonalize(grad + beta * momentum)`` (``nesterov``; otherwise of the momentum);
+    ``p = p * (1 - lr * weight_decay) - lr * sqrt(max(1, rows / cols)) * update``.
+
+    Parameters are matrices or stacks of them (``[experts, rows, cols]``: every expert's matrix by itself).  The momentum is fp32."""
+
+    def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
+                 coefficients=COEFFICIENTS, eps: float = 1e-7):
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps, coefficients=coefficients, eps=eps))
+        for group in self.param_groups:
+            for p in group['params']:
+                if p.dim() < 2:
+                    raise ValueError('Muon updates matrices, got a parameter of shape %s' % (tuple(p.shape),))
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            for p in group['params']:
+                if p.grad is None:
+                    continue
+                state = self.state[p]
+                if not state:
+                    state['momentum'] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
+                m, grad = state['momentum'], p.grad.float()
+                m.mul_(group['momentum']).add_(grad)
+                update = orthogonalize(grad.add_(m, alpha=group['momentum']) if group['nesterov'] else m, group['steps'], group['coefficients'], group['eps'])
+                if group['weight_decay']:
+                    p.mul_(1.0 - group['lr'] * group['weight_decay'])
+                p.add_(update, alpha=-group['lr'] * max(1.0, p.shape[-2] / p.shape[-1])**0.5)
+        return loss
