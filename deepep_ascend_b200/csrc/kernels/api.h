@@ -550,9 +550,10 @@ struct NsArgs {
     NsReport report;
     // set by the launcher
     int ld_x, ld_sq;
-    const __half *x_in, *sq_in;       // [count, rows, ld_x], [count, rows, ld_sq]
+    const __half *x_in, *sq_in, *sq_in2;      // [count, rows, ld_x]; symmetric matrices without their diagonals [count, rows, ld_sq]
+    const float *diag_in, *diag_in2;          // ... and their diagonals [count, ld_sq]
     __half *x_out, *x_lo, *sq_out;
-    float *diag, *coef;               // [count, ld_sq]
+    float* diag_out;
     float* parts;                     // [k_splits, tiles, 128, 128] sums of X X^T over parts of K
     int k_splits;
     double* norm_parts;               // [count, num_norm_parts]
@@ -561,7 +562,7 @@ struct NsArgs {
 struct NsWorkspace {
     int64_t bytes, ld_x, ld_sq, norm_parts;
     int k_splits;
-    int64_t norms, x[2], lo, sq[2], diag[2], parts;        // byte offsets
+    int64_t norms, x[2], lo, sq[3], diag[3], parts;        // byte offsets
 };
 
 namespace ep {

@@ -3,7 +3,14 @@
 //
 //     X = G / (|G|_F + eps);     per step:  A = X X^T,  B = b A + c A A,  X = a X + B X
 //
-// The three products of a step run on the tensor cores (tcgen05, fp16 operands, 32-bit sums in tensor memory), one persistent kernel each.  A and
+// Steps may go in pairs, without the X between them. With Q = a I + B the next A is Q A Q, so that a pair is
+//
+//     A = X X^T,  Q1 = a I + b A + c A A,  T = Q1 A,  A = T Q1,  Q2 = a I + b A + c A A,  Q = Q2 Q1,  X = Q X
+//
+// where all but the first and the last are symmetric products of rows^3, computed by half: in multiply-adds 3 cols/rows + 5 halves of 2 rows^3 for
+// a pair, 6 cols/rows + 2 for two single steps.
+//
+// The products run on the tensor cores (tcgen05, fp16 operands, 32-bit sums in tensor memory), one persistent kernel each.  A and
 // B are symmetric: only tiles on and above the diagonal are computed, the others are written as their mirror images.
 //
 // Precision.  A step multiplies small singular values by up to a = 3.44, and with them whatever rounding has put there, so what is rounded
@@ -12,11 +19,15 @@
 // 1.3e-3 / 7e-3 / 6e-2, nearly all of it from rounding the X of a X and the diagonals of A and B, which are far larger than what is around them.
 // So X is carried in two halves, hi + lo 2^-11 (22 bits; the products read hi alone), and the diagonals are carried in 32 bits beside matrices
 // whose diagonal is zero:  A = O + diag(d),  A A = O O + (d_i + d_j) O + diag(d^2),  B X = (B - diag) X + diag X.  Then 5e-4 / 2e-4 / 4e-4, less than
-// the rounding of the result to bf16 (1.7e-3).
+// the rounding of the result to bf16 (1.7e-3).  In a pair the second A comes from the first, not from X, and what its small eigenvalues are off by
+// has been multiplied by a^2; the next pair starts from X again.  For matrices of 512 and more rows that gives 7e-4 / 4e-4 / 3e-4, and 2.1e-3 (single
+// steps: 7e-4) for singular values that fall off evenly by 10^3 or 10^6.  At 64 rows it would be 1.9e-3 / 1.5e-3 / 1e-3, and three steps at once 2e-3 with a
+// single strong direction, five no number at all: so only pairs, and only from 512 rows.
 #include <cuda_fp16.h>
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "common.cuh"
 #include "gemm_sm100.cuh"
@@ -37,7 +48,7 @@ __host__ __device__ constexpr int ns_stage_bytes(int block_n) { return (kTileM +
 __host__ __device__ constexpr int ns_smem_bytes(int block_n) { return ns_stages(block_n) * ns_stage_bytes(block_n) + 1024 + kEpiWarps * kStagingBytes; }
 
 // What a kernel makes of its sums
-enum { kGram = 0, kPoly = 1, kUpdate = 2, kGramPart = 3 };
+enum { kGram = 0, kPoly = 1, kUpdate = 2, kGramPart = 3, kProduct = 4 };
 
 struct NsSmem {
     uint64_t full[8], empty[8], acc_full[2], acc_empty[2], quiet;
@@ -135,13 +146,6 @@ __device__ __forceinline__ void unpack_half(const uint4& v, float (&f)[8]) {
     }
 }
 
-// What a product reads and writes beside its operands
-struct NsStep {
-    const __half *x_in, *sq_in;
-    __half *x_out, *sq_out;
-    void* out;               // the last step's result, or null
-};
-
 // 32 x 32 values of a tile lie on a warp as four rows (i * 8 + lane / 4) of eight neighbouring columns ((lane & 3) * 8) per lane: rows are read and written in
 // whole sectors.
 struct Block {
@@ -214,8 +218,8 @@ __device__ __forceinline__ void by_value(uint8_t* staging, const uint32_t (&o)[4
     __syncwarp();
 }
 // A symmetric result's block, and its mirror image
-__device__ __forceinline__ void store_symmetric(const NsArgs& g, __half* sq_out, uint8_t* staging, int matrix, const Block& b, const float (&v)[4][8], bool mirror) {
-    __half* out = sq_out + static_cast<int64_t>(matrix) * g.rows * g.ld_sq;
+__device__ __forceinline__ void store_symmetric(const NsArgs& g, uint8_t* staging, int matrix, const Block& b, const float (&v)[4][8], bool mirror) {
+    __half* out = g.sq_out + static_cast<int64_t>(matrix) * g.rows * g.ld_sq;
     uint32_t o[4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -230,18 +234,18 @@ __device__ __forceinline__ void store_symmetric(const NsArgs& g, __half* sq_out,
         });
 }
 // X X^T in kUnitX^2 -> O and the diagonal.  (Columns past the end are sums of zeros.)
-__device__ __forceinline__ void finish_gram(const NsArgs& g, __half* sq_out, uint8_t* staging, int matrix, const Block& b, float (&v)[4][8], bool mirror) {
+__device__ __forceinline__ void finish_gram(const NsArgs& g, uint8_t* staging, int matrix, const Block& b, float (&v)[4][8], bool mirror) {
     if (b.row0 == b.col0)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float d = take_diagonal(v[i], b.row(i) - b.col());
-            if (b.on_diagonal(i) && b.row(i) < g.rows) g.diag[static_cast<int64_t>(matrix) * g.ld_sq + b.row(i)] = d * (1.f / (kUnitX * kUnitX));
+            if (b.on_diagonal(i) && b.row(i) < g.rows) g.diag_out[static_cast<int64_t>(matrix) * g.ld_sq + b.row(i)] = d * (1.f / (kUnitX * kUnitX));
         }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] *= kUnitA / (kUnitX * kUnitX);
-    store_symmetric(g, sq_out, staging, matrix, b, v, mirror);
+    store_symmetric(g, staging, matrix, b, v, mirror);
 }
 
 // What a product of `mode` runs over
@@ -336,9 +340,9 @@ __device__ __forceinline__ bool ns_multiply(const NsArgs& g, const NsShared<kBlo
     return true;
 }
 // Eight warps: kGram: O, d = X X^T without its diagonal, and the diagonal; kGramPart: its sums over a part of K.  kPoly: B, coef = b A + c A A without its diagonal, and
-// a + the diagonal.  kUpdate: X <- coef X + B X.
+// a + the diagonal.  kProduct: P R of two symmetric matrices that commute, likewise.  kUpdate: X <- Q X.
 template <int kMode, int kBlockN>
-__device__ __forceinline__ bool ns_finish(const NsArgs& g, const NsStep& step, const NsShared<kBlockN>& s, uint32_t tmem_base, int& acc, uint32_t& acc_phase) {
+__device__ __forceinline__ bool ns_finish(const NsArgs& g, const NsShared<kBlockN>& s, uint32_t tmem_base, int& acc, uint32_t& acc_phase) {
     const NsWork<kMode, kBlockN> work(g);
     constexpr int kChunks = kBlockN / 2 / 32;          // 32-column blocks of a warp
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = warp & 3, half = (warp - 2) >> 2;
@@ -360,26 +364,31 @@ __device__ __forceinline__ bool ns_finish(const NsArgs& g, const NsStep& step, c
             for (int i = 0; i < 4; ++i) {
                 const bool in = b.row(i) < g.rows && b.col() < width;
                 o[i] = l[i] = make_uint4(0, 0, 0, 0);
-                if constexpr (kMode == kPoly) {
-                    if (in) o[i] = *reinterpret_cast<const uint4*>(step.sq_in + sq + static_cast<int64_t>(b.row(i)) * g.ld_sq + b.col());
+                if constexpr (kMode == kPoly || kMode == kProduct) {
+                    if (in) {
+                        const int64_t at = sq + static_cast<int64_t>(b.row(i)) * g.ld_sq + b.col();
+                        o[i] = *reinterpret_cast<const uint4*>(g.sq_in + at);
+                        if constexpr (kMode == kProduct) l[i] = *reinterpret_cast<const uint4*>(g.sq_in2 + at);
+                    }
                 } else if constexpr (kMode == kUpdate) {
                     if (in) {
                         const int64_t at = wide + static_cast<int64_t>(b.row(i)) * g.ld_x + b.col();
-                        o[i] = *reinterpret_cast<const uint4*>(step.x_in + at);
+                        o[i] = *reinterpret_cast<const uint4*>(g.x_in + at);
                         l[i] = *reinterpret_cast<const uint4*>(g.x_lo + at);
                     }
                 }
             }
-            if constexpr (kMode == kPoly) {
+            if constexpr (kMode == kPoly || kMode == kProduct) {
+                const float* values = kMode == kPoly ? g.diag_in : g.diag_in2;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) cv[j] = b.col() + j < g.rows ? g.diag[diag + b.col() + j] : 0.f;
+                for (int j = 0; j < 8; ++j) cv[j] = b.col() + j < g.rows ? values[diag + b.col() + j] : 0.f;
             }
         };
-        if constexpr (kMode == kPoly || kMode == kUpdate) {
+        if constexpr (kMode == kPoly || kMode == kUpdate || kMode == kProduct) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int row = block(0).row(i);
-                row_value[i] = row >= g.rows ? 0.f : kMode == kPoly ? g.diag[diag + row] : g.coef[diag + row];
+                row_value[i] = row >= g.rows ? 0.f : g.diag_in[diag + row];
             }
             request(0, old[0], low[0], col_value[0]);
         }
@@ -390,7 +399,7 @@ __device__ __forceinline__ bool ns_finish(const NsArgs& g, const NsStep& step, c
         for (int c = 0; c < kChunks; ++c) {
             const Block b = block(c);
             if (kMode != kGramPart && empty(b)) break;
-            if constexpr (kMode == kPoly || kMode == kUpdate)
+            if constexpr (kMode == kPoly || kMode == kUpdate || kMode == kProduct)
                 if (c + 1 < kChunks) request(c + 1, old[(c + 1) & 1], low[(c + 1) & 1], col_value[(c + 1) & 1]);
             float v[4][8];
             {
@@ -400,7 +409,7 @@ __device__ __forceinline__ bool ns_finish(const NsArgs& g, const NsStep& step, c
                 spread(staging, r, v);
             }
             if constexpr (kMode == kGram) {
-                finish_gram(g, step.sq_out, staging, t.g, b, v, t.mirror);
+                finish_gram(g, staging, t.g, b, v, t.mirror);
             } else if constexpr (kMode == kGramPart) {
                 // [part][tile][128][kBlockN]
                 float* part = g.parts + static_cast<int64_t>(item) * kTileM * kBlockN + (b.col0 - t.n * kBlockN + (lane & 3) * 8);
@@ -418,13 +427,27 @@ __device__ __forceinline__ bool ns_finish(const NsArgs& g, const NsStep& step, c
                     const float di = row_value[i], coefficient = g.b + g.c * di;
                     if (b.row0 == b.col0) {
                         const float d = take_diagonal(v[i], b.row(i) - b.col());
-                        if (b.on_diagonal(i) && b.row(i) < g.rows) g.coef[diag + b.row(i)] = g.a + g.b * di + g.c * (di * di + d * (1.f / (kUnitA * kUnitA)));
+                        if (b.on_diagonal(i) && b.row(i) < g.rows) g.diag_out[diag + b.row(i)] = g.a + g.b * di + g.c * (di * di + d * (1.f / (kUnitA * kUnitA)));
                     }
                     // (B in kUnitA; O O in kUnitA^2; O is zero on the diagonal)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[i][j] = (coefficient + g.c * col_value[c & 1][j]) * f[j] + g.c * (1.f / kUnitA) * v[i][j];
                 }
-                store_symmetric(g, step.sq_out, staging, t.g, b, v, t.mirror);
+                store_symmetric(g, staging, t.g, b, v, t.mirror);
+            } else if constexpr (kMode == kProduct) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float f[8], h[8];
+                    unpack_half(old[c & 1][i], f);
+                    unpack_half(low[c & 1][i], h);
+                    if (b.row0 == b.col0) {
+                        const float d = take_diagonal(v[i], b.row(i) - b.col());
+                        if (b.on_diagonal(i) && b.row(i) < g.rows) g.diag_out[diag + b.row(i)] = d * (1.f / (kUnitA * kUnitA)) + row_value[i] * g.diag_in2[diag + b.row(i)];
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[i][j] = row_value[i] * h[j] + f[j] * col_value[c & 1][j] + v[i][j] * (1.f / kUnitA);      // in kUnitA
+                }
+                store_symmetric(g, staging, t.g, b, v, t.mirror);
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -434,7 +457,7 @@ __device__ __forceinline__ bool ns_finish(const NsArgs& g, const NsStep& step, c
 #pragma unroll
                     for (int j = 0; j < 8; ++j) v[i][j] = row_value[i] * (hi[j] + lo[j] * (1.f / kUnitLo)) + v[i][j] * (1.f / kUnitA);     // in kUnitX
                 }
-                if (step.out == nullptr) {
+                if (g.out == nullptr) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         uint32_t o[4], l[4];
@@ -446,13 +469,13 @@ __device__ __forceinline__ bool ns_finish(const NsArgs& g, const NsStep& step, c
                         }
                         if (b.row(i) < g.rows && b.col() < width) {
                             const int64_t at = wide + static_cast<int64_t>(b.row(i)) * g.ld_x + b.col();
-                            *reinterpret_cast<uint4*>(step.x_out + at) = make_uint4(o[0], o[1], o[2], o[3]);
+                            *reinterpret_cast<uint4*>(g.x_out + at) = make_uint4(o[0], o[1], o[2], o[3]);
                             *reinterpret_cast<uint4*>(g.x_lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
                         }
                     }
                 } else {
                     // the last step: the result, in the caller's orientation
-                    uint16_t* dst = reinterpret_cast<uint16_t*>(step.out) + static_cast<int64_t>(t.g) * g.rows * g.cols;
+                    uint16_t* dst = reinterpret_cast<uint16_t*>(g.out) + static_cast<int64_t>(t.g) * g.rows * g.cols;
                     uint32_t o[4][4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
@@ -551,7 +574,7 @@ ns_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     } else if (warp == 1) {
         if (ptx::elect_one() && !ns_multiply<kMode, kBlockN>(g, s, tmem_base, p, acc, acc_phase)) ns_quiet(s);
     } else {
-        ns_finish<kMode, kBlockN>(g, NsStep{g.x_in, g.sq_in, g.x_out, g.sq_out, g.out}, s, tmem_base, acc, acc_phase);
+        ns_finish<kMode, kBlockN>(g, s, tmem_base, acc, acc_phase);
     }
     ns_teardown<kBlockN>(tmem_base);
 }
@@ -563,7 +586,7 @@ struct NsAdd {
     static constexpr int kPieces = (kTileM / 8) * (kBlockN / 32);      // of a tile
 };
 template <int kBlockN>
-__device__ __forceinline__ void ns_add_piece(const NsArgs& g, __half* sq_out, uint8_t* staging, int tile, int piece, int per_matrix, int num_tiles) {
+__device__ __forceinline__ void ns_add_piece(const NsArgs& g, uint8_t* staging, int tile, int piece, int per_matrix, int num_tiles) {
     const int lane = threadIdx.x & 31;
     const NsTile t = ns_tile<kBlockN, true>(tile, per_matrix, 0);
     const int r = piece / (kBlockN / 32) * 8 + (lane >> 2), c = piece % (kBlockN / 32) * 32 + (lane & 3) * 8;
@@ -591,12 +614,12 @@ __device__ __forceinline__ void ns_add_piece(const NsArgs& g, __half* sq_out, ui
     }
     if (row0 >= col0 && row0 < col0 + 32) {
         const float d = take_diagonal(v, row - col);
-        if (static_cast<uint32_t>(row - col) < 8u && row < g.rows) g.diag[static_cast<int64_t>(t.g) * g.ld_sq + row] = d * (1.f / (kUnitX * kUnitX));
+        if (static_cast<uint32_t>(row - col) < 8u && row < g.rows) g.diag_out[static_cast<int64_t>(t.g) * g.ld_sq + row] = d * (1.f / (kUnitX * kUnitX));
     }
     uint32_t o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) o[j] = pack_half(v[2 * j] * (kUnitA / (kUnitX * kUnitX)), v[2 * j + 1] * (kUnitA / (kUnitX * kUnitX)));
-    __half* out = sq_out + static_cast<int64_t>(t.g) * g.rows * g.ld_sq;
+    __half* out = g.sq_out + static_cast<int64_t>(t.g) * g.rows * g.ld_sq;
     if (row < g.rows && col < g.ld_sq) *reinterpret_cast<uint4*>(out + static_cast<int64_t>(row) * g.ld_sq + col) = make_uint4(o[0], o[1], o[2], o[3]);
     if (t.mirror) {
         // the mirror image: 32 rows of eight values
@@ -620,7 +643,7 @@ __global__ void __launch_bounds__(kAddThreads) ns_add_kernel(const __grid_consta
     const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kAddThreads / 32) + (threadIdx.x >> 5);
     constexpr int kPieces = NsAdd<kBlockN>::kPieces;
     if (unit < static_cast<int64_t>(num_tiles) * kPieces)
-        ns_add_piece<kBlockN>(g, g.sq_out, s_staging[threadIdx.x >> 5], static_cast<int>(unit / kPieces), static_cast<int>(unit % kPieces), per_matrix, num_tiles);
+        ns_add_piece<kBlockN>(g, s_staging[threadIdx.x >> 5], static_cast<int>(unit / kPieces), static_cast<int>(unit % kPieces), per_matrix, num_tiles);
 }
 
 // ------------------------------------------------------------------------------------------------ the first X
@@ -813,9 +836,21 @@ cudaError_t launch_first(const NsArgs& g, cudaStream_t stream) {
                             stream);
 }
 
+// Steps in pairs: for matrices of half as many columns again as rows, if that saves more products than the two additional kernels of five steps cost, and the matrices have rows
+// enough for the rounding of a pair to stay below that of the result.  In us, single steps and pairs: 1024 x 1536 139 and 162, 1024 x 2048 147 and 167, four of them 238 and
+// 234, eight 437 and 400, 16 of 512 x 2048 396 and 357, 1024 x 7168 245 and 227, 2048 x 7168 550 and 460; four of 2048 x 2560 (a quarter more) 851 and 845 or 927 and 975.
+// Coefficients under which Q could grow past what fp16 holds of a product of two (64 beside the diagonal) stay with single steps.
+bool in_pairs(const NsArgs& g) {
+    auto small = [&](float x) { return std::abs(g.a + (g.b + g.c * x) * x) <= 4.f; };
+    const float vertex = g.c == 0.f ? 0.f : std::min(std::max(-g.b / (2.f * g.c), 0.f), 1.5f);
+    if (!small(0.f) || !small(1.5f) || !small(vertex)) return false;       // (X's singular values stay below 1.22 with the coefficients in use)
+    const int64_t saved = 3ll * (g.cols - g.rows) * g.rows * g.rows * g.count;       // multiply-adds per pair
+    return g.rows >= 512 && 2ll * g.cols >= 3ll * g.rows && saved >= 12'000'000'000;
+}
+
 }  // namespace
 
-// Workspace: hi of X twice and lo once, O and B, their diagonals, sums of squares, parts of X X^T.
+// Workspace: hi of X twice and lo once, three symmetric matrices (two without pairs) and their diagonals, sums of squares, parts of X X^T.
 NsWorkspace newton_schulz_workspace(const NsArgs& g, int num_sms) {
     NsWorkspace w{};
     w.ld_x = round8(g.cols);
@@ -830,8 +865,10 @@ NsWorkspace newton_schulz_workspace(const NsArgs& g, int num_sms) {
     w.norms = take(g.count * w.norm_parts * 8);
     for (int64_t& x : w.x) x = take(g.count * g.rows * w.ld_x * 2);
     w.lo = take(g.count * g.rows * w.ld_x * 2);
-    for (int64_t& s : w.sq) s = take(g.count * g.rows * w.ld_sq * 2);
-    for (int64_t& d : w.diag) d = take(g.count * w.ld_sq * 4);
+    for (int i = 0; i < (in_pairs(g) ? 3 : 2); ++i) {
+        w.sq[i] = take(g.count * g.rows * w.ld_sq * 2);
+        w.diag[i] = take(g.count * w.ld_sq * 4);
+    }
     w.parts = take(w.k_splits > 1 ? w.k_splits * tiles_of(g, kGram, 128) * kTileM * 128 * 4 : 0);
     return w;
 }
@@ -841,53 +878,84 @@ cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8
     NsArgs g = args;
     g.ld_x = static_cast<int>(w.ld_x);
     g.ld_sq = static_cast<int>(w.ld_sq);
-    __half *x[2], *sq[2];
-    for (int i = 0; i < 2; ++i) {
-        x[i] = reinterpret_cast<__half*>(workspace + w.x[i]);
-        sq[i] = reinterpret_cast<__half*>(workspace + w.sq[i]);
-    }
     g.x_lo = reinterpret_cast<__half*>(workspace + w.lo);
-    g.diag = reinterpret_cast<float*>(workspace + w.diag[0]);
-    g.coef = reinterpret_cast<float*>(workspace + w.diag[1]);
     g.norm_parts = reinterpret_cast<double*>(workspace + w.norms);
     g.num_norm_parts = static_cast<int>(w.norm_parts);
     g.parts = reinterpret_cast<float*>(workspace + w.parts);
     g.k_splits = w.k_splits;
-    void* out = g.out;
     g.out = nullptr;
-    const int n_gram = g.k_splits > 1 ? 128 : block_n_of(g, kGram, num_sms), n_poly = block_n_of(g, kPoly, num_sms), n_update = block_n_of(g, kUpdate, num_sms);
-    CUtensorMap x_rows[2], x_cols[2], x_mn[2], o_rows, o_cols, b_rows;
-    for (int i = 0; i < 2; ++i)
-        if (!make_map(&x_rows[i], x[i], g.count, g.rows, g.cols, g.ld_x, kTileM) || !make_map(&x_cols[i], x[i], g.count, g.rows, g.cols, g.ld_x, n_gram) ||
-            !make_map(&x_mn[i], x[i], g.count, g.rows, g.cols, g.ld_x, 64))
+    const bool pairs = in_pairs(g);
+    const int n_gram = g.k_splits > 1 ? 128 : block_n_of(g, kGram, num_sms), n_square = block_n_of(g, kPoly, num_sms), n_update = block_n_of(g, kUpdate, num_sms);
+    // X in turn; symmetric matrices: their rows as the first and as the second operand
+    struct Wide {
+        __half* x;
+        CUtensorMap rows, cols, mn;
+    } x[2];
+    struct Square {
+        __half* m;
+        float* diag;
+        CUtensorMap rows, cols;
+    } sq[3];
+    for (int i = 0; i < 2; ++i) {
+        x[i].x = reinterpret_cast<__half*>(workspace + w.x[i]);
+        if (!make_map(&x[i].rows, x[i].x, g.count, g.rows, g.cols, g.ld_x, kTileM) || !make_map(&x[i].cols, x[i].x, g.count, g.rows, g.cols, g.ld_x, n_gram) ||
+            !make_map(&x[i].mn, x[i].x, g.count, g.rows, g.cols, g.ld_x, 64))
             return cudaErrorInvalidValue;
-    if (!make_map(&o_rows, sq[0], g.count, g.rows, g.rows, g.ld_sq, kTileM) || !make_map(&o_cols, sq[0], g.count, g.rows, g.rows, g.ld_sq, n_poly) ||
-        !make_map(&b_rows, sq[1], g.count, g.rows, g.rows, g.ld_sq, kTileM))
-        return cudaErrorInvalidValue;
+    }
+    for (int i = 0; i < (pairs ? 3 : 2); ++i) {
+        sq[i].m = reinterpret_cast<__half*>(workspace + w.sq[i]);
+        sq[i].diag = reinterpret_cast<float*>(workspace + w.diag[i]);
+        if (!make_map(&sq[i].rows, sq[i].m, g.count, g.rows, g.rows, g.ld_sq, kTileM) || !make_map(&sq[i].cols, sq[i].m, g.count, g.rows, g.rows, g.ld_sq, n_square))
+            return cudaErrorInvalidValue;
+    }
+    auto gram = [&](const Wide& from, const Square& to) {
+        g.sq_out = to.m;
+        g.diag_out = to.diag;
+        if (g.k_splits == 1) return launch_product<kGram>(n_gram, from.rows, from.cols, g, num_sms, stream);
+        const cudaError_t err = launch_product<kGramPart, 128>(from.rows, from.cols, g, num_sms, stream);
+        if (err != cudaSuccess) return err;
+        void* params[] = {&g};
+        const int64_t warps = tiles_of(g, kGram, 128) * NsAdd<128>::kPieces;
+        return launch_dependent(reinterpret_cast<const void*>(ns_add_kernel<128>), dim3(static_cast<unsigned>(warps * 32 / kAddThreads)), dim3(kAddThreads), params, 0, stream);
+    };
+    auto poly = [&](const Square& from, const Square& to) {
+        g.sq_in = from.m;
+        g.diag_in = from.diag;
+        g.sq_out = to.m;
+        g.diag_out = to.diag;
+        return launch_product<kPoly>(n_square, from.rows, from.cols, g, num_sms, stream);
+    };
+    auto product = [&](const Square& p, const Square& r, const Square& to) {
+        g.sq_in = p.m;
+        g.diag_in = p.diag;
+        g.sq_in2 = r.m;
+        g.diag_in2 = r.diag;
+        g.sq_out = to.m;
+        g.diag_out = to.diag;
+        return launch_product<kProduct>(n_square, p.rows, r.cols, g, num_sms, stream);
+    };
+    auto update = [&](const Square& q, const Wide& from, const Wide& to) {
+        g.diag_in = q.diag;
+        g.x_in = from.x;
+        g.x_out = to.x;
+        return launch_product<kUpdate>(n_update, q.rows, from.mn, g, num_sms, stream);
+    };
 
-    g.x_out = x[0];
+    g.x_out = x[0].x;
     cudaError_t err = g.in_bf16 ? launch_first<__nv_bfloat16>(g, stream) : launch_first<float>(g, stream);
-    for (int s = 0; s < steps && err == cudaSuccess; ++s) {
-        const int from = s & 1;
-        g.sq_out = sq[0];
-        if (g.k_splits > 1) {
-            err = launch_product<kGramPart, 128>(x_rows[from], x_cols[from], g, num_sms, stream);
-            if (err != cudaSuccess) break;
-            void* params[] = {&g};
-            const int64_t warps = tiles_of(g, kGram, 128) * NsAdd<128>::kPieces;
-            err = launch_dependent(reinterpret_cast<const void*>(ns_add_kernel<128>), dim3(static_cast<unsigned>(warps * 32 / kAddThreads)), dim3(kAddThreads), params, 0, stream);
-        } else {
-            err = launch_product<kGram>(n_gram, x_rows[from], x_cols[from], g, num_sms, stream);
+    for (int done = 0, from = 0; done < steps && err == cudaSuccess; from ^= 1) {
+        const bool pair = pairs && done + 2 <= steps;
+        done += pair ? 2 : 1;
+        err = gram(x[from], sq[0]);
+        if (err == cudaSuccess) err = poly(sq[0], sq[1]);
+        if (pair) {
+            if (err == cudaSuccess) err = product(sq[1], sq[0], sq[2]);      // T = Q1 A
+            if (err == cudaSuccess) err = product(sq[2], sq[1], sq[0]);      // A = T Q1
+            if (err == cudaSuccess) err = poly(sq[0], sq[2]);                // Q2
+            if (err == cudaSuccess) err = product(sq[2], sq[1], sq[0]);      // Q = Q2 Q1
         }
-        if (err != cudaSuccess) break;
-        g.sq_in = sq[0];
-        g.sq_out = sq[1];
-        err = launch_product<kPoly>(n_poly, o_rows, o_cols, g, num_sms, stream);
-        if (err != cudaSuccess) break;
-        g.x_in = x[from];
-        g.x_out = x[from ^ 1];
-        if (s == steps - 1) g.out = out;
-        err = launch_product<kUpdate>(n_update, b_rows, x_mn[from], g, num_sms, stream);
+        if (done == steps) g.out = args.out;
+        if (err == cudaSuccess) err = update(sq[pair ? 0 : 1], x[from], x[from ^ 1]);
     }
     return err;
 }

@@ -73,6 +73,48 @@ def test_more_tiles_than_one_wave_and_few_sms(count, rows, cols):
         assert _error(orthogonalize(x[i]), want[i]) < BOUND['strong directions']
 
 
+def _falling(count, rows, cols, orders):
+    """Singular values that fall off evenly by 10^orders."""
+    g = torch.Generator().manual_seed(orders)
+    u = torch.linalg.qr(torch.randn(count, rows, rows, generator=g, dtype=torch.float64))[0]
+    v = torch.linalg.qr(torch.randn(count, cols, rows, generator=g, dtype=torch.float64))[0]
+    return ((u * torch.logspace(0, -orders, rows, dtype=torch.float64)) @ v.mT).float()
+
+
+# Wide enough for steps in pairs, and enough of them.  Simulated in 64 bits, pairs add up to 8e-4 to the rounding of the result for the kinds above, less than
+# the bounds above leave; 2.2e-3 in another direction for singular values that fall off evenly (together 2.8e-3).
+@pytest.mark.gpu
+@pytest.mark.parametrize('kind', sorted(BOUND) + ['falling by 3', 'falling by 6'])
+@pytest.mark.parametrize('count,rows,cols', [(5, 1000, 2017), (2, 1530, 2930), (32, 512, 1032), (3, 2600, 1208)])
+def test_steps_in_pairs(count, rows, cols, kind):
+    if kind in BOUND:
+        x, bound = _matrix(kind, count, rows, cols), BOUND[kind]
+    else:
+        x, bound = _falling(count, min(rows, cols), max(rows, cols), int(kind[-1])), 3.3e-3
+        x = x.mT if rows > cols else x
+    x = x.bfloat16().cuda()
+    got, one = orthogonalize(x), orthogonalize(x[0])       # (a single one is too few)
+    assert torch.equal(orthogonalize(x), got)
+    want = _exact(x)
+    assert _error(got, want) < bound
+    assert _error(one, want[0]) < bound
+
+
+@pytest.mark.gpu
+def test_pairs_of_other_steps_and_coefficients():
+    x = _matrix('strong directions', 5, 1000, 2016).cuda()
+    for steps, coefficients in ((1, COEFFICIENTS), (2, COEFFICIENTS), (3, COEFFICIENTS), (4, COEFFICIENTS), (6, (1.875, -1.25, 0.375)), (4, (1.5, -0.5, 0.0)),
+                                (2, (6.0, -9.0, 4.0))):
+        assert _error(orthogonalize(x, steps, coefficients), _exact(x, steps, coefficients)) < 2.7e-3
+    # bad matrices are their own
+    x = x.bfloat16()
+    want = orthogonalize(x)
+    x[1, 999, 2015], x[3] = float('inf'), 0.0
+    got = orthogonalize(x)
+    assert torch.isnan(got[1]).all() and not got[3].any()
+    assert all(torch.equal(got[i], want[i]) for i in (0, 2, 4))
+
+
 @pytest.mark.parametrize('device', DEVICES)
 def test_tiny_matrices(device):
     for shape in ((1, 1, 1), (3, 1, 9), (2, 9, 1), (1, 2, 2), (4, 3, 17), (2, 8, 5)):
