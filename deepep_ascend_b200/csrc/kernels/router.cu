@@ -35,6 +35,39 @@ __device__ __forceinline__ T logit_of(float v) {
 
 __device__ __forceinline__ float sigmoid(float l) { return __frcp_rn(1.f + expf(-l)); }
 
+// 1 / x, correctly rounded, for 1 <= x < 2^118: an estimate, and one step with its residual (P. W. Markstein, Computation of elementary functions on the
+// IBM RISC System/6000 processor, 1990).  The bits of __frcp_rn for every one of these numbers, without that one's look at all others, which lets the
+// eight of a lane overlap.
+__device__ __forceinline__ float reciprocal(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return fmaf(r, fmaf(-x, r, 1.f), r);
+}
+constexpr float kLowLogit = -80.f;                               // 1 + exp(80) < 2^118
+
+// a / x, correctly rounded, of 2^-100 <= a <= 1 and 1 <= x <= 2^20 with x's correctly rounded reciprocal: a quotient that is off by less than its last place
+// and one step with its exact residual round as the quotient does (the same work's theorem on division)
+__device__ __forceinline__ float quotient(float a, float x, float inverse) {
+    float q = a * inverse;
+    q = fmaf(fmaf(-q, x, a), inverse, q);
+    return fmaf(fmaf(-q, x, a), inverse, q);
+}
+constexpr float kLowShare = 7.9e-31f;                            // over 2^-100
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float min8_nan(const float (&v)[8]) {
+    const float a = min3_nan(v[0], v[1], v[2]), b = min3_nan(v[3], v[4], v[5]);
+    return min3_nan(a, b, min3_nan(v[6], v[7], v[7]));
+}
 __device__ __forceinline__ float max_nan(float a, float b) {      // a NaN wins, as everything computed with it is one
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -141,25 +174,22 @@ __global__ void __launch_bounds__(256, kSoftmax || kSegs > 4 ? 2 : 4) route_kern
     const float inverse_s = 1.f / S, inverse_g = 1.f / G;
     // largest and second largest choice of an eight
     auto tops = [&](const float (&c)[8], int t, int seg) {
-        float v1 = c[0], v2 = kNone;
+        float hi[4], lo[4];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) {
-            v2 = fmaxf(v2, fminf(v1, c[i]));
-            v1 = fmaxf(v1, c[i]);
-        }
-        best[t * best_pitch + seg] = v1;
-        second[t * best_pitch + seg] = v2;
-    };
-    // A choice that is no number, or whose logit is -inf, is nobody's.  Looked at one by one only where the eight logits do not add up to a number, or the bias
-    // holds others than numbers.
-    auto settle = [&](const float (&logit)[8], float (&c)[8]) {
-        const float sum = ((logit[0] + logit[1]) + (logit[2] + logit[3])) + ((logit[4] + logit[5]) + (logit[6] + logit[7]));
-        if (odd_bias || !(fabsf(sum) < -kNone)) {
+        for (int i = 0; i < 4; ++i) hi[i] = fmaxf(c[i], c[i + 4]), lo[i] = fminf(c[i], c[i + 4]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (!(c[i] > kNone) || !(logit[i] > kNone)) c[i] = kNone;
-        }
+        for (int h = 2; h > 0; h /= 2)
+#pragma unroll
+            for (int i = 0; i < h; ++i) {
+                lo[i] = max3(lo[i], lo[i + h], fminf(hi[i], hi[i + h]));
+                hi[i] = fmaxf(hi[i], hi[i + h]);
+            }
+        best[t * best_pitch + seg] = hi[0];
+        second[t * best_pitch + seg] = lo[0];
     };
+    // A choice that is no number, or whose logit is -inf, is nobody's.  Looked at one by one, with the general reciprocal or quotient, only in an eight
+    // that has others than ordinary numbers, or where the bias has.
+    auto settled = [](float logit, float c) { return c > kNone && logit > kNone ? c : kNone; };
 
     const int64_t step = static_cast<int64_t>(gridDim.x) * warps * tokens;
     for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * warps + warp) * tokens; t0 < a.num_tokens; t0 += step) {
@@ -208,14 +238,19 @@ __global__ void __launch_bounds__(256, kSoftmax || kSegs > 4 ? 2 : 4) route_kern
                 const int u = u0 + lane, t = min(static_cast<int>((u + 0.5f) * inverse_s), kTokens - 1), seg = u - t * S;
                 const float sum = __shfl_sync(0xffffffffu, total, t * 8);
                 if (u < units) {
-                    float logit[8], c[8];
-                    load8<kBf16, kWide>(rows + t * pitch, seg * 8, E, logit);
+                    float c[8], b[8];
                     fetch8(choice + u * 8, c);
-                    float b[8];
                     fetch8(s_bias + seg * 8, b);
+                    if (!odd_bias && min8_nan(c) >= kLowShare) {       // (none of a logit that is -inf)
+                        const float inverse = reciprocal(sum);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) c[i] = __fdiv_rn(c[i], sum) + b[i];
-                    settle(logit, c);
+                        for (int i = 0; i < 8; ++i) c[i] = quotient(c[i], sum, inverse) + b[i];
+                    } else {
+                        float logit[8];
+                        load8<kBf16, kWide>(rows + t * pitch, seg * 8, E, logit);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) c[i] = settled(logit[i], __fdiv_rn(c[i], sum) + b[i]);
+                    }
                     store8(choice + u * 8, c);
                     tops(c, t, seg);
                 }
@@ -226,9 +261,13 @@ __global__ void __launch_bounds__(256, kSoftmax || kSegs > 4 ? 2 : 4) route_kern
                 float logit[8], c[8], b[8];
                 load8<kBf16, kWide>(rows + t * pitch, seg * 8, E, logit);
                 fetch8(s_bias + seg * 8, b);
+                if (!odd_bias && min8_nan(logit) >= kLowLogit) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) c[i] = sigmoid(logit[i]) + b[i];
-                settle(logit, c);
+                    for (int i = 0; i < 8; ++i) c[i] = reciprocal(1.f + expf(-logit[i])) + b[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) c[i] = settled(logit[i], sigmoid(logit[i]) + b[i]);
+                }
                 store8(choice + u * 8, c);
                 tops(c, t, seg);
             }
