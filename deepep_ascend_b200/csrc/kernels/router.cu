@@ -120,23 +120,26 @@ __device__ __forceinline__ void fetch8(const float* p, float (&v)[8]) {
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
 
-// Shared memory of a warp, which works on up to four tokens at a time: the choices of each, padded to whole eights; the best and second best of each eight; the
-// groups' scores; for a softmax, room for the tree.
+// Shared memory of a warp, which works on up to four tokens at a time: the choices of each (for a softmax an odd number of eights apart, so
+// that the four tokens' lanes, eight each, meet different banks); the best and second best of each eight; the groups' scores.
 constexpr int kTokens = 4;
 struct RouteLayout {
-    int eights, choice, best, group, tree, warp;       // eights of a token; offsets in floats of a token's or the warp's arrays; floats of a warp
+    int eights, pitch, best, group, warp;       // eights of a token; floats from token to token; offsets in floats of the warp's arrays; floats of a warp
 };
 __host__ __device__ inline RouteLayout route_layout(int experts, int groups, bool softmax) {
     RouteLayout l;
     l.eights = (experts + 7) / 8;
-    int width = 8;                                     // experts as a power of two, eight at least
-    while (width < experts) width *= 2;
-    l.choice = 0;
-    l.best = kTokens * l.eights * 8;
+    l.pitch = (softmax ? l.eights | 1 : l.eights) * 8;
+    l.best = kTokens * l.pitch;
     l.group = l.best + kTokens * 2 * ((l.eights + 3) / 4 * 4);
-    l.tree = l.group + (groups > 1 ? kTokens * 32 : 0);
-    l.warp = l.tree + (softmax ? kTokens * width / 2 : 0);
+    l.warp = l.group + (groups > 1 ? kTokens * 32 : 0);
     return l;
+}
+// leaf(0) + ... + leaf(kCount - 1), the upper half added to the lower one until one is left
+template <int kCount, int kFirst = 0, int kStep = 1, class F>
+__device__ __forceinline__ float sum_by_halves(const F& leaf) {
+    if constexpr (kStep >= kCount) return leaf(kFirst);
+    else return sum_by_halves<kCount, kFirst, kStep * 2>(leaf) + sum_by_halves<kCount, kFirst + kStep, kStep * 2>(leaf);
 }
 
 // A warp takes `tokens` (1 or 4) at a time.  Scores: a lane has eight neighbouring experts of one token.  Choice: eight lanes per token, each with kSegs eights
@@ -144,12 +147,14 @@ __host__ __device__ inline RouteLayout route_layout(int experts, int groups, boo
 // shuffles of a step serve four tokens.  Bound by instruction issue: about half of what is left are the exact exponentials and reciprocals.
 // 65536 x 256 fp32, 8 of 256 in 4 of 8 groups: 59 us; one token per warp, with a maximum over the warp for every expert, took 139.
 template <int kSegs, bool kBf16, bool kWide, bool kSoftmax>
-__global__ void __launch_bounds__(256, kSoftmax || kSegs > 4 ? 2 : 4) route_kernel(const RouterArgs a, const int tokens) {
+__global__ void __launch_bounds__(256, kSegs > 4 ? 3 : 4) route_kernel(const RouterArgs a, const int tokens) {
     extern __shared__ __align__(16) float route_smem[];
     const RouteLayout l = route_layout(a.num_experts, a.num_groups, kSoftmax);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, E = a.num_experts, K = a.num_topk, S = l.eights, G = a.num_groups;
     float* mine = route_smem + warp * l.warp;
-    float *choice = mine + l.choice, *best = mine + l.best, *group_score = mine + l.group, *tree = mine + l.tree;
+    float *choice = mine, *best = mine + l.best, *group_score = mine + l.group;
+    const int P = kSoftmax ? l.pitch : S * 8;
+    auto place = [&](int u, int t, int seg) { return kSoftmax ? t * P + seg * 8 : u * 8; };      // of an eight
     const int best_pitch = (S + 3) / 4 * 4;
     float* second = best + kTokens * best_pitch;
     float* s_bias = route_smem + warps * l.warp;                              // [S * 8]
@@ -203,7 +208,7 @@ __global__ void __launch_bounds__(256, kSoftmax || kSegs > 4 ? 2 : 4) route_kern
                 const int t = static_cast<int>((u + 0.5f) * inverse_s), seg = u - t * S;
                 float v[8];
                 load8<kBf16, kWide>(rows + t * pitch, seg * 8, E, v);
-                store8(choice + u * 8, v);
+                store8(choice + place(u, t, seg), v);
                 best[t * best_pitch + seg] = max_nan(max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3])), max_nan(max_nan(v[4], v[5]), max_nan(v[6], v[7])));
             }
             __syncwarp();
@@ -211,26 +216,14 @@ __global__ void __launch_bounds__(256, kSoftmax || kSegs > 4 ? 2 : 4) route_kern
             if (t8 < n)
                 for (int s = q; s < S; s += 8) top = max_nan(top, best[t8 * best_pitch + s]);
             top = over8(top, max_nan);
-            // exp(l - max) of the lane's experts q, q + 8, ..., and their sum by halves: the first level on the way to `tree`
+            // exp(l - max) of the lane's experts q, q + 8, ..., and their sum.  (With zeros up to 64 kSegs experts the tree has the same sum.)
+            total = 0.f;
             if (t8 < n) {
-                float *e = choice + t8 * S * 8 + q, *x = tree + t8 * ((l.warp - l.tree) / kTokens) + q;
-                int half = (l.warp - l.tree) / kTokens / 8;            // eights of the padded experts, by two
-                if (half == 0) {
-                    e[0] = expf(e[0] - top);
-                    total = q < E ? e[0] : 0.f;
-                } else {
-                    for (int s = 0; s < half; ++s) {
-                        float lo = 0.f, hi = 0.f;
-                        if (s < S) lo = e[s * 8] = expf(e[s * 8] - top);
-                        if (s + half < S) hi = e[(s + half) * 8] = expf(e[(s + half) * 8] - top);
-                        x[s * 8] = lo + hi;
-                    }
-                    for (half /= 2; half > 0; half /= 2)
-                        for (int s = 0; s < half; ++s) x[s * 8] += x[(s + half) * 8];
-                    total = x[0];
-                }
-            } else {
-                total = 0.f;
+                float* e = choice + t8 * P + q;
+                total = sum_by_halves<8 * kSegs>([&](int s) {
+                    if (s >= S) return 0.f;
+                    return e[s * 8] = expf(e[s * 8] - top);
+                });
             }
             total = sum8(total);
             __syncwarp();
@@ -239,7 +232,7 @@ __global__ void __launch_bounds__(256, kSoftmax || kSegs > 4 ? 2 : 4) route_kern
                 const float sum = __shfl_sync(0xffffffffu, total, t * 8);
                 if (u < units) {
                     float c[8], b[8];
-                    fetch8(choice + u * 8, c);
+                    fetch8(choice + place(u, t, seg), c);
                     fetch8(s_bias + seg * 8, b);
                     if (!odd_bias && min8_nan(c) >= kLowShare) {       // (none of a logit that is -inf)
                         const float inverse = reciprocal(sum);
@@ -251,7 +244,7 @@ __global__ void __launch_bounds__(256, kSoftmax || kSegs > 4 ? 2 : 4) route_kern
 #pragma unroll
                         for (int i = 0; i < 8; ++i) c[i] = settled(logit[i], __fdiv_rn(c[i], sum) + b[i]);
                     }
-                    store8(choice + u * 8, c);
+                    store8(choice + place(u, t, seg), c);
                     tops(c, t, seg);
                 }
             }
@@ -268,7 +261,7 @@ __global__ void __launch_bounds__(256, kSoftmax || kSegs > 4 ? 2 : 4) route_kern
 #pragma unroll
                     for (int i = 0; i < 8; ++i) c[i] = settled(logit[i], sigmoid(logit[i]) + b[i]);
                 }
-                store8(choice + u * 8, c);
+                store8(choice + place(u, t, seg), c);
                 tops(c, t, seg);
             }
         }
@@ -286,7 +279,7 @@ __global__ void __launch_bounds__(256, kSoftmax || kSegs > 4 ? 2 : 4) route_kern
                         v1 = fmaxf(v1, b1);
                     }
                 } else {
-                    const float* c = choice + t * S * 8 + g * size;
+                    const float* c = choice + t * P + g * size;
                     for (int i = 0; i < size; ++i) {
                         v2 = fmaxf(v2, fminf(v1, c[i]));
                         v1 = fmaxf(v1, c[i]);
@@ -316,11 +309,11 @@ __global__ void __launch_bounds__(256, kSoftmax || kSegs > 4 ? 2 : 4) route_kern
                     const uint32_t stay = __shfl_sync(0xffffffffu, kept, t * 8);
                     if (u < units) {
                         float c[8];
-                        fetch8(choice + u * 8, c);
+                        fetch8(choice + place(u, t, seg), c);
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
                             if (((stay >> min((seg * 8 + i) / size, 31)) & 1u) == 0) c[i] = kNone;
-                        store8(choice + u * 8, c);
+                        store8(choice + place(u, t, seg), c);
                         tops(c, t, seg);
                     }
                 }
@@ -337,7 +330,7 @@ __global__ void __launch_bounds__(256, kSoftmax || kSegs > 4 ? 2 : 4) route_kern
             m[i] = routed && seg < S && ((kept >> seg_group[i]) & 1u) != 0 ? best[t8 * best_pitch + seg] : kNone;
         }
         int chosen[2] = {-1, -1};                      // experts q and q + 8 of token t8
-        float* c8 = choice + (t8 < n ? t8 : 0) * S * 8 + q;
+        float* c8 = choice + (t8 < n ? t8 : 0) * P + q;
         const uint32_t ours = 0xffu << (t8 * 8);       // this token's lanes
         const auto larger = [](float x, float y) { return fmaxf(x, y); };
 #pragma unroll 1
