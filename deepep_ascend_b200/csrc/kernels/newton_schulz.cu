@@ -43,7 +43,8 @@ constexpr int kStagingBytes = 32 * 128;                        // per epilogue w
 constexpr int kTransposePitch = 72;                            // bytes of a staged column of 32 fp16 values
 constexpr uint64_t kNsWaitLimitNs = 4ull * 1000 * 1000 * 1000; // when the caller gives no limit
 
-__host__ __device__ constexpr int ns_stages(int block_n) { return block_n == 256 ? 4 : 6; }
+__host__ __device__ constexpr int ns_stages(int block_n) { return block_n == 128 ? 6 : 4; }
+__host__ __device__ constexpr int ns_tmem_columns(int block_n) { return block_n == 128 ? 256 : 512; }      // two accumulators, a power of two
 __host__ __device__ constexpr int ns_stage_bytes(int block_n) { return (kTileM + block_n) * 128; }
 __host__ __device__ constexpr int ns_smem_bytes(int block_n) { return ns_stages(block_n) * ns_stage_bytes(block_n) + 1024 + kEpiWarps * kStagingBytes; }
 
@@ -527,7 +528,7 @@ __device__ __forceinline__ uint32_t ns_setup(const NsShared<kBlockN>& s) {
         ptx::mbar_fence_init();
     }
     if (threadIdx.x >> 5 == 1) {
-        umma::tmem_alloc(&s.sm->tmem_base, 2 * kBlockN);
+        umma::tmem_alloc(&s.sm->tmem_base, ns_tmem_columns(kBlockN));
         umma::tmem_relinquish();
     }
     umma::fence_before_thread_sync();
@@ -539,7 +540,7 @@ template <int kBlockN>
 __device__ __forceinline__ void ns_teardown(uint32_t tmem_base) {
     umma::fence_before_thread_sync();
     __syncthreads();
-    if (threadIdx.x >> 5 == 1) umma::tmem_dealloc(tmem_base, 2 * kBlockN);
+    if (threadIdx.x >> 5 == 1) umma::tmem_dealloc(tmem_base, ns_tmem_columns(kBlockN));
 }
 // products still under way end before the tensor memory is given back
 template <int kBlockN>
@@ -778,10 +779,16 @@ int64_t symmetric_tiles_of(int rows, int block_n) { return block_n == 256 ? symm
 int64_t tiles_of(const NsArgs& g, int mode, int block_n) {
     return g.count * (mode == kUpdate ? static_cast<int64_t>((g.rows + kTileM - 1) / kTileM) * ((g.cols + block_n - 1) / block_n) : symmetric_tiles_of(g.rows, block_n));
 }
-// 256-column tiles, or 128 where their waves take less time: a tile of half the columns takes about 0.6 of it.
+// Columns of a tile: of 256, 128 and for X, whose tiles need not meet the diagonal, 192, the one whose waves take the least time, if a tile of 128 columns takes 0.6 and one of
+// 192 takes 0.8 of one of 256; the wider one of equals.
 int block_n_of(const NsArgs& g, int mode, int num_sms) {
-    auto waves = [&](int n) { return (tiles_of(g, mode, n) + num_sms - 1) / num_sms; };
-    return 10 * waves(256) <= 6 * waves(128) ? 256 : 128;
+    int best = 256;
+    int64_t least = 0;
+    for (int n = 256; n >= 128; n -= mode == kUpdate ? 64 : 128) {
+        const int64_t time = (tiles_of(g, mode, n) + num_sms - 1) / num_sms * (n / 32 + 2);
+        if (n == 256 || time < least) best = n, least = time;
+    }
+    return best;
 }
 // Parts along K of X X^T where its tiles are few and long: as in the GEMM, the K blocks that a CTA is spared against the kernel that adds the parts
 // (about 16 blocks) and the parts' way through L2 (one block per 512 KB).
@@ -819,6 +826,8 @@ cudaError_t launch_product(const CUtensorMap& map_a, const CUtensorMap& map_b, c
 }
 template <int kMode>
 cudaError_t launch_product(int block_n, const CUtensorMap& map_a, const CUtensorMap& map_b, const NsArgs& g, int num_sms, cudaStream_t stream) {
+    if constexpr (kMode == kUpdate)
+        if (block_n == 192) return launch_product<kMode, 192>(map_a, map_b, g, num_sms, stream);
     return block_n == 256 ? launch_product<kMode, 256>(map_a, map_b, g, num_sms, stream) : launch_product<kMode, 128>(map_a, map_b, g, num_sms, stream);
 }
 
