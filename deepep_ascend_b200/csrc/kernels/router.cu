@@ -347,20 +347,20 @@ __global__ void __launch_bounds__(256, kSegs > 4 ? 3 : 4) route_kernel(const Rou
                 if (m[i] == wanted) at = i;
             if (m[0] == wanted) at = 0;
             const int seg = __shfl_sync(0xffffffffu, q * kSegs + at, owner);
+            // (selects, not branches: a step has little else to do than to wait for its shuffles)
             const bool some = wanted > kNone;
-            float c = some ? c8[seg * 8] : kNone;
-            const int hit = __ffs(__ballot_sync(0xffffffffu, c == wanted) & ours) - 1;
-            if (some && lane == hit) c8[seg * 8] = c = kNone;
-            const float next = over8(c, larger);
-            if (lane == owner) {
+            float* place_c = c8 + seg * 8;
+            const float seen = *place_c;
+            const int hit = __ffs(__ballot_sync(0xffffffffu, some && seen == wanted) & ours) - 1;
+            const bool taken = lane == hit;
+            if (taken) *place_c = kNone;
+            const float next = over8(some && !taken ? seen : kNone, larger);
+            const bool owns = lane == owner;
 #pragma unroll
-                for (int i = 0; i < kSegs; ++i)
-                    if (i == at) m[i] = next;          // (nobody left: -inf takes its own place)
-            }
-            if (some && q == (k & 7)) {
-                if (k < 8) chosen[0] = seg * 8 + (hit & 7);
-                else chosen[1] = seg * 8 + (hit & 7);
-            }
+            for (int i = 0; i < kSegs; ++i) m[i] = owns && i == at ? next : m[i];          // (nobody left: -inf takes its own place)
+            const int id = some ? seg * 8 + (hit & 7) : -1;
+            chosen[0] = q == k ? id : chosen[0];
+            chosen[1] = q + 8 == k ? id : chosen[1];
         }
         // weights: the lane's first expert, and its second one where a token has more than eight
         const uint8_t* row = rows + (t8 < n ? t8 : 0) * pitch;
