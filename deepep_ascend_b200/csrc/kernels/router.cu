@@ -176,7 +176,10 @@ __global__ void __launch_bounds__(256, kSegs > 4 ? 3 : 4) route_kernel(const Rou
     int seg_group[kSegs];
 #pragma unroll
     for (int i = 0; i < kSegs; ++i) seg_group[i] = whole ? min(q * kSegs + i, S - 1) * 8 / size : 0;
-    const float inverse_s = 1.f / S, inverse_g = 1.f / G;
+    const float inverse_g = 1.f / G;
+    uint32_t token_of = 0;                             // of this lane's eights lane, lane + 32, ... of four tokens: two bits each
+#pragma unroll
+    for (int i = 0; i < kSegs; ++i) token_of |= static_cast<uint32_t>(min((lane + 32 * i) / S, kTokens - 1)) << (2 * i);
     // largest and second largest choice of an eight
     auto tops = [&](const float (&c)[8], int t, int seg) {
         float hi[4], lo[4];
@@ -204,8 +207,8 @@ __global__ void __launch_bounds__(256, kSegs > 4 ? 3 : 4) route_kernel(const Rou
         float top = 0.f, total = 1.f;                  // of the token of this lane's eight
         if constexpr (kSoftmax) {
             // logits, and the largest of each eight
-            for (int u = lane; u < units; u += 32) {
-                const int t = static_cast<int>((u + 0.5f) * inverse_s), seg = u - t * S;
+            for (uint32_t w = token_of, u = lane; u < static_cast<uint32_t>(units); u += 32, w >>= 2) {
+                const int t = w & 3, seg = u - t * S;
                 float v[8];
                 load8<kBf16, kWide>(rows + t * pitch, seg * 8, E, v);
                 store8(choice + place(u, t, seg), v);
@@ -227,8 +230,8 @@ __global__ void __launch_bounds__(256, kSegs > 4 ? 3 : 4) route_kernel(const Rou
             }
             total = sum8(total);
             __syncwarp();
-            for (int u0 = 0; u0 < units; u0 += 32) {
-                const int u = u0 + lane, t = min(static_cast<int>((u + 0.5f) * inverse_s), kTokens - 1), seg = u - t * S;
+            for (uint32_t w = token_of, u0 = 0; u0 < static_cast<uint32_t>(units); u0 += 32, w >>= 2) {
+                const int u = u0 + lane, t = w & 3, seg = u - t * S;
                 const float sum = __shfl_sync(0xffffffffu, total, t * 8);
                 if (u < units) {
                     float c[8], b[8];
@@ -249,8 +252,8 @@ __global__ void __launch_bounds__(256, kSegs > 4 ? 3 : 4) route_kernel(const Rou
                 }
             }
         } else {
-            for (int u = lane; u < units; u += 32) {
-                const int t = static_cast<int>((u + 0.5f) * inverse_s), seg = u - t * S;
+            for (uint32_t w = token_of, u = lane; u < static_cast<uint32_t>(units); u += 32, w >>= 2) {
+                const int t = w & 3, seg = u - t * S;
                 float logit[8], c[8], b[8];
                 load8<kBf16, kWide>(rows + t * pitch, seg * 8, E, logit);
                 fetch8(s_bias + seg * 8, b);
@@ -304,8 +307,8 @@ __global__ void __launch_bounds__(256, kSegs > 4 ? 3 : 4) route_kernel(const Rou
             for (int o = 4; o > 0; o >>= 1) kept |= __shfl_xor_sync(0xffffffffu, kept, o);
             if (!whole) {
                 // groups that end within an eight: their experts leave one by one
-                for (int u0 = 0; u0 < units; u0 += 32) {
-                    const int u = u0 + lane, t = min(static_cast<int>((u + 0.5f) * inverse_s), kTokens - 1), seg = u - t * S;
+                for (uint32_t w = token_of, u0 = 0; u0 < static_cast<uint32_t>(units); u0 += 32, w >>= 2) {
+                    const int u = u0 + lane, t = w & 3, seg = u - t * S;
                     const uint32_t stay = __shfl_sync(0xffffffffu, kept, t * 8);
                     if (u < units) {
                         float c[8];
