@@ -195,12 +195,35 @@ struct Raw {
     }
 };
 
-// A row belongs to one warp (blockDim.y of them per CTA) or to a whole CTA; each thread has kPieces pieces of it in registers, as they came, and
-// requests the next row's before it starts on this one.  Few threads per row: the two sums of a row are what it waits for, so an SM should
+// The sum of one value per thread over a row, on each of its threads.  The warps' sums of a CTA's row lie in shared memory, zero where there is no warp, and every
+// thread adds them up.
+template <bool kWarpRows>
+__device__ __forceinline__ float row_sum(float v, float4 (*words)[8], int& turn) {
+    float one[1] = {v};
+    float sum = warp_sums<1>(one);
+    if constexpr (!kWarpRows) {
+        float4* w = words[turn];
+        turn ^= 1;
+        if ((threadIdx.x & 31) == 0) reinterpret_cast<float*>(w)[threadIdx.x >> 5] = sum;
+        __syncthreads();
+        sum = 0.f;
+        for (int i = 0; i < static_cast<int>(blockDim.x); i += 256) {
+            const float4 p = w[i / 128], q = w[i / 128 + 1];
+            sum += ((p.x + p.y) + (p.z + p.w)) + ((q.x + q.y) + (q.z + q.w));
+        }
+    }
+    return sum;
+}
+
+// CTAs of `threads` that an SM should hold: 80 registers per thread for four pieces of 16 bytes (with 64, for more threads, they do not stay in registers)
+constexpr int norm_min_ctas(int vec, int pieces, int threads) { return (vec == 1 ? (pieces == 8 ? 1024 : 512) : pieces < 4 || threads == 1024 ? 1024 : 768) / threads; }
+
+// A row belongs to one warp (blockDim.y of them per CTA) or to a whole CTA; each thread has kPieces pieces of it in registers.  The registers that they came in take
+// the next row's as soon as they have been made numbers.  Few threads per row: the two sums of a row are what it waits for, so an SM should
 // have many rows under way, and shuffles and barriers cost by the warp.
-template <class T, class P, int kVec, int kPieces, bool kWarpRows>
-__global__ void __launch_bounds__(kWarpRows ? 256 : kVec == 1 ? 512 : 1024) layer_norm_kernel(const LayerNormArgs a) {
-    __shared__ float scratch[2][32][1];
+template <class T, class P, int kVec, int kPieces, bool kWarpRows, int kThreads>
+__global__ void __launch_bounds__(kThreads, norm_min_ctas(kVec, kPieces, kThreads)) layer_norm_kernel(const LayerNormArgs a) {
+    __shared__ float4 scratch[2][8];
     using E = typename Piece<kVec>::E;
     constexpr int kN = Piece<kVec>::kN;
     const int64_t first = blockIdx.x * blockDim.y + threadIdx.y, stride = static_cast<int64_t>(gridDim.x) * blockDim.y;
@@ -208,6 +231,10 @@ __global__ void __launch_bounds__(kWarpRows ? 256 : kVec == 1 ? 512 : 1024) laye
     const P *w = reinterpret_cast<const P*>(a.weight), *b = reinterpret_cast<const P*>(a.bias);
     const float inverse = 1.f / a.hidden;
     const int col0 = threadIdx.x * kVec, step = blockDim.x * kVec;       // columns col0 + i * step
+    if constexpr (!kWarpRows) {
+        if (threadIdx.x < 16) scratch[threadIdx.x / 8][threadIdx.x % 8] = make_float4(0.f, 0.f, 0.f, 0.f);
+        __syncthreads();
+    }
     ptx::wait_for_previous_kernel();
     ptx::let_next_kernel_start();
     Raw<T, kVec> raw[kPieces];
@@ -217,37 +244,32 @@ __global__ void __launch_bounds__(kWarpRows ? 256 : kVec == 1 ? 512 : 1024) laye
             if (col0 + i * step < a.hidden) raw[i].load(x + first * a.ldx + col0 + i * step);
     int turn = 0;
     for (int64_t row = first; row < a.rows; row += stride) {
-        Raw<T, kVec> next[kPieces];
-        if (row + stride < a.rows)
-#pragma unroll
-            for (int i = 0; i < kPieces; ++i)
-                if (col0 + i * step < a.hidden) next[i].load(x + (row + stride) * a.ldx + col0 + i * step);
+        Piece<kVec> p[kPieces];
         E acc[2] = {both<E>(0.f), both<E>(0.f)};
 #pragma unroll
         for (int i = 0; i < kPieces; ++i)
             if (col0 + i * step < a.hidden) {
-                const Piece<kVec> p = raw[i].numbers();
+                p[i] = raw[i].numbers();
 #pragma unroll
-                for (int j = 0; j < kN; ++j) acc[j & 1] = acc[j & 1] + p.v[j];
+                for (int j = 0; j < kN; ++j) acc[j & 1] = acc[j & 1] + p[i].v[j];
             }
-        float sum[1] = {total(acc[0] + acc[1])};
-        row_sums<1, kWarpRows>(sum, scratch, turn);
-        const float mean = sum[0] * inverse;
+        if (row + stride < a.rows)
+#pragma unroll
+            for (int i = 0; i < kPieces; ++i)
+                if (col0 + i * step < a.hidden) raw[i].load(x + (row + stride) * a.ldx + col0 + i * step);
+        const float mean = row_sum<kWarpRows>(total(acc[0] + acc[1]), scratch, turn) * inverse;
         const E minus_mean = both<E>(-mean);
         acc[0] = acc[1] = both<E>(0.f);
 #pragma unroll
         for (int i = 0; i < kPieces; ++i)
             if (col0 + i * step < a.hidden) {
-                const Piece<kVec> p = raw[i].numbers();
 #pragma unroll
                 for (int j = 0; j < kN; ++j) {
-                    const E d = p.v[j] + minus_mean;
-                    acc[j & 1] = mul_add(d, d, acc[j & 1]);
+                    p[i].v[j] = p[i].v[j] + minus_mean;
+                    acc[j & 1] = mul_add(p[i].v[j], p[i].v[j], acc[j & 1]);
                 }
             }
-        sum[0] = total(acc[0] + acc[1]);
-        row_sums<1, kWarpRows>(sum, scratch, turn);
-        const float rstd = rsqrtf(sum[0] * inverse + a.eps);
+        const float rstd = rsqrtf(row_sum<kWarpRows>(total(acc[0] + acc[1]), scratch, turn) * inverse + a.eps);
         const E scale = both<E>(rstd);
         T* y = reinterpret_cast<T*>(a.y) + row * a.hidden;
         auto finish = [&](auto with_bias) {
@@ -255,16 +277,16 @@ __global__ void __launch_bounds__(kWarpRows ? 256 : kVec == 1 ? 512 : 1024) laye
             for (int i = 0; i < kPieces; ++i) {
                 const int col = col0 + i * step;
                 if (col < a.hidden) {
-                    Piece<kVec> p = raw[i].numbers(), pw, pb;
+                    Piece<kVec> pw, pb;
                     pw.load(w + col);
                     if constexpr (decltype(with_bias)::value) pb.load(b + col);
 #pragma unroll
                     for (int j = 0; j < kN; ++j) {
-                        const E xh = (p.v[j] + minus_mean) * scale;
-                        if constexpr (decltype(with_bias)::value) p.v[j] = mul_add(xh, pw.v[j], pb.v[j]);
-                        else p.v[j] = xh * pw.v[j];
+                        const E xh = p[i].v[j] * scale;
+                        if constexpr (decltype(with_bias)::value) p[i].v[j] = mul_add(xh, pw.v[j], pb.v[j]);
+                        else p[i].v[j] = xh * pw.v[j];
                     }
-                    p.store(y + col);
+                    p[i].store(y + col);
                 }
             }
         };
@@ -274,8 +296,6 @@ __global__ void __launch_bounds__(kWarpRows ? 256 : kVec == 1 ? 512 : 1024) laye
             a.mean[row] = mean;
             a.rstd[row] = rstd;
         }
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) raw[i] = next[i];
     }
 }
 
@@ -492,11 +512,13 @@ NormKernel forward_kernel(const NormShape& n) {
     constexpr int kVec = 16 / sizeof(T);
     if (n.values == 0) return layer_norm_wide_kernel<T, P>;
     if (n.vec == 1) {
-        if (n.values == 8) return n.warp_rows ? layer_norm_kernel<T, P, 1, 8, true> : layer_norm_kernel<T, P, 1, 8, false>;
-        return layer_norm_kernel<T, P, 1, 16, false>;
+        if (n.values == 8) return n.warp_rows ? layer_norm_kernel<T, P, 1, 8, true, 256> : layer_norm_kernel<T, P, 1, 8, false, 512>;
+        return layer_norm_kernel<T, P, 1, 16, false, 512>;
     }
-    if (n.warp_rows) return n.values == kVec ? layer_norm_kernel<T, P, kVec, 1, true> : layer_norm_kernel<T, P, kVec, 4, true>;
-    return layer_norm_kernel<T, P, kVec, 4, false>;
+    if (n.warp_rows && n.values == kVec) return layer_norm_kernel<T, P, kVec, 1, true, 256>;
+    if (n.warp_rows) return n.values == 2 * kVec ? layer_norm_kernel<T, P, kVec, 2, true, 256> : layer_norm_kernel<T, P, kVec, 4, true, 256>;
+    if (n.threads <= 256) return layer_norm_kernel<T, P, kVec, 4, false, 256>;
+    return n.threads <= 384 ? layer_norm_kernel<T, P, kVec, 4, false, 384> : layer_norm_kernel<T, P, kVec, 4, false, 1024>;
 }
 NormKernel forward_kernel(const LayerNormArgs& a, const NormShape& n) {
     if (a.x_bf16) return a.param_bf16 ? forward_kernel<__nv_bfloat16, __nv_bfloat16>(n) : forward_kernel<__nv_bfloat16, float>(n);
@@ -560,14 +582,14 @@ cudaError_t launch_rows(const void* fn, const NormShape& n, void** params, cudaS
 }  // namespace
 
 // Pieces of 16 bytes where every row of every operand starts on 16 bytes, single values otherwise.  Four pieces (eight or sixteen values) per thread, so that a row has few
-// threads; one where that makes do with a warp.
+// threads; one or two where those make do with a warp.
 cudaError_t launch_layer_norm(const LayerNormArgs& args, int num_sms, cudaStream_t stream) {
     if (args.hidden < 1 || args.rows < 0) return cudaErrorInvalidValue;
     if (args.rows == 0) return cudaSuccess;
     LayerNormArgs a = args;
     NormShape n{};
     n.vec = rows_on_16_bytes(a, false) ? 16 / (a.x_bf16 ? 2 : 4) : 1;
-    n.values = n.vec == 1 ? (a.hidden <= 8 * 512 ? 8 : 16) : a.hidden <= 32 * n.vec ? n.vec : 4 * n.vec;
+    n.values = n.vec == 1 ? (a.hidden <= 8 * 512 ? 8 : 16) : a.hidden <= 32 * n.vec ? n.vec : a.hidden <= 64 * n.vec ? 2 * n.vec : 4 * n.vec;
     n.threads = static_cast<int>((static_cast<int64_t>(a.hidden) + n.values - 1) / n.values + 31) / 32 * 32;
     n.warp_rows = n.threads == 32;
     n.rows_per_cta = n.warp_rows ? 8 : 1;
