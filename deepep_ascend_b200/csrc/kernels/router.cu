@@ -144,8 +144,11 @@ __device__ __forceinline__ float sum_by_halves(const F& leaf) {
 
 // A warp takes `tokens` (1 or 4) at a time.  Scores: a lane has eight neighbouring experts of one token.  Choice: eight lanes per token, each with kSegs eights
 // of which it knows the largest choice; a chosen expert is found, taken out, and the new largest of its eight made by the token's eight lanes together, so that the
-// shuffles of a step serve four tokens.  Bound by instruction issue: about half of what is left are the exact exponentials and reciprocals.
-// 65536 x 256 fp32, 8 of 256 in 4 of 8 groups: 59 us; one token per warp, with a maximum over the warp for every expert, took 139.
+// shuffles of a step serve four tokens.  Bound by instruction issue (1720 per warp and four tokens, 70 % of the issue slots; DRAM 18 %): about a third are the
+// exact exponentials and reciprocals, a quarter the steps of the choice.
+// 65536 x 256 fp32, 8 of 256 in 4 of 8 groups: 42 us, 1.8 TB/s (softmax 56); one token per warp, with a maximum over the warp for every expert, took 139, steps that
+// branch 48.  Requesting the next tokens' logits into L2 ahead gained nothing (43).
+// CTAs per SM: as many as leave the registers (64, or 80 for more than 256 experts) for what a lane holds: 32768 x 512 with 64 took 81 us instead of 72.
 template <int kSegs, bool kBf16, bool kWide, bool kSoftmax>
 __global__ void __launch_bounds__(256, kSegs > 4 ? 3 : 4) route_kernel(const RouterArgs a, const int tokens) {
     extern __shared__ __align__(16) float route_smem[];
@@ -415,7 +418,7 @@ __device__ __forceinline__ int chosen_expert(const RouterArgs& a, int64_t at) {
 
 // Gradients that only chosen experts have.  A warp takes kRows tokens at a time, eight lanes for each of four; their rows, zero but for the chosen experts,
 // lie in shared memory and leave as one bulk copy (kRows rows start and end on 16 bytes for any number of experts), two sets of rows in turn.  What is
-// left to do per row is to write and clear its few values.  65536 x 256 fp32, 8 chosen: 21 us; rows put together in registers took 42.
+// left to do per row is to write and clear its few values.  65536 x 256 fp32, 8 chosen: 20 us, 3.8 TB/s; rows put together in registers took 42.
 template <bool kBf16>
 __global__ void __launch_bounds__(256) route_backward_kernel(const RouterArgs a) {
     using T = std::conditional_t<kBf16, __nv_bfloat16, float>;

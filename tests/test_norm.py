@@ -81,6 +81,14 @@ def test_many_rows(T, H):
     _check(*_make(T, H, BF16, F32, 1, 'cuda'))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [BF16, F32])
+@pytest.mark.parametrize('T,H', [(9001, 200), (9001, 512), (5001, 1040), (2001, 4104), (1001, 8200), (1001, 12280), (701, 16392), (701, 24576), (301, 32776)])
+def test_every_width_over_many_rows(T, H, dtype):
+    """One, two and four pieces of 16 bytes per thread, rows of a warp, of up to 256, 384 and 1024 threads and wider ones, each with several rows per CTA."""
+    _check(*_make(T, H, dtype, F32, 3, 'cuda'))
+
+
 @pytest.mark.parametrize('device', DEVICES)
 @pytest.mark.parametrize('std,offset', [(1e-3, 100.0), (1e-18, 0.0), (1e15, 0.0), (1.0, -1e4)])
 def test_scales_and_offsets(std, offset, device):

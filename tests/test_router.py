@@ -155,6 +155,23 @@ def test_kernel_chooses_what_32_bit_scores_say(E, K, G, TG, top, score):
             assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('score', ['sigmoid', 'softmax'])
+@pytest.mark.parametrize('E,K', [(8, 8), (40, 16), (256, 8), (1000, 16)])
+def test_scores_of_every_size(E, K, score):
+    """Bit by bit what 32-bit scores say over the whole range: logits around and beyond what the kernel's short reciprocal and quotient take, groups of eight
+    neighbours of ordinary ones, of small ones and mixed, with and without a bias of ordinary numbers."""
+    g = torch.Generator().manual_seed(E)
+    l = torch.randn(4096, E, generator=g) * torch.logspace(-3, 2.2, 4096)[:, None]
+    l[::3] -= torch.randint(0, 140, (len(l[::3]), 1), generator=g)
+    l[1::3, : E // 2] -= 75 + 10 * torch.rand(len(l[1::3]), 1, generator=g)
+    l = l.cuda()
+    for bias in (None, (torch.randn(E, generator=g) * 0.1).cuda(), torch.full((E, ), -0.5, device='cuda')):
+        want = router.route_ref(l, K, score, bias, renormalize=False)
+        got = router.route(l, K, score, bias, renormalize=False)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(got[2], want[2])
+
+
 @pytest.mark.parametrize('device', DEVICES)
 @pytest.mark.parametrize('score,renormalize', [('sigmoid', True), ('sigmoid', False), ('softmax', True), ('softmax', False)])
 @pytest.mark.parametrize('E,K', [(1, 1), (7, 3), (32, 8), (65, 6), (160, 6), (256, 8), (500, 16), (1024, 9)])
