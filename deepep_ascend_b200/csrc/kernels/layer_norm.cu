@@ -495,8 +495,12 @@ __global__ void __launch_bounds__(kReduceWarps * 32) layer_norm_reduce_kernel(co
     const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 + lane, width = static_cast<int64_t>(a.db != nullptr ? 2 : 1) * a.hidden;
     float v = 0.f;
     if (col < width)
-#pragma unroll 8
-        for (int s = warp; s < a.slices; s += kReduceWarps) v += a.partial[s * width + col];
+        for (int s0 = warp; s0 < a.slices; s0 += 8 * kReduceWarps) {        // eight requested at once
+            float p[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = s0 + i * kReduceWarps < a.slices ? a.partial[(s0 + i * kReduceWarps) * width + col] : 0.f;
+            v += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        }
     sums[warp][lane] = v;
     __syncthreads();
     v = sums[lane][warp];          // column `warp`, slice group `lane`
@@ -623,9 +627,9 @@ NormShape layer_norm_backward_shape(const LayerNormArgs& a, int num_sms) {
     n.smem = norm_stages(size, n.vec, n.values) * 2 * n.values * size * n.threads * n.rows_per_cta;
     if (n.warp_rows) n.smem = std::max(n.smem, n.rows_per_cta * 2 * a.hidden * 4);
     const int per_sm = resident_ctas(reinterpret_cast<const void*>(backward_kernel(a, n, true)), n.threads * n.rows_per_cta, n.smem);
-    // every slice of the gradient's sums costs a row of 32-bit values written and read again: at least two rows share one
+    // every slice of the gradient's sums costs a row of 32-bit values written and read again: at least four rows share one
     int64_t ctas = (static_cast<int64_t>(a.rows) + n.rows_per_cta - 1) / n.rows_per_cta;
-    ctas = std::min<int64_t>(ctas, std::max<int64_t>(num_sms, a.rows / 2));
+    ctas = std::min<int64_t>(ctas, std::max<int64_t>(num_sms, a.rows / 4));
     n.ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ctas, static_cast<int64_t>(per_sm) * num_sms)));
     return n;
 }
