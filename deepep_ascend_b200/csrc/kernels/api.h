@@ -265,6 +265,8 @@ cudaError_t launch_reduce_slots(const ReduceSlotsArgs& args, cudaStream_t stream
 namespace ep {
 // Launch of a kernel that calls wait_for_previous_kernel() before it touches global memory: it is set up while the kernel before it drains.
 cudaError_t launch_dependent(const void* fn, dim3 grid, dim3 block, void** params, size_t smem, cudaStream_t stream);
+// Leave for `smem` bytes of dynamic shared memory, and the CTAs of `threads` that then fit on an SM: asked for once per device, kernel, threads and size.  `ctas` may be null.
+cudaError_t allow_shared_memory(const void* fn, int threads, int smem, int* ctas);
 }  // namespace ep
 
 // ------------------------------------------------------------------------------------------------ tcgen05 GEMM

@@ -5,9 +5,6 @@
 //
 // Values, statistics and sums are 32-bit; a result is rounded once to its type.
 #include <algorithm>
-#include <map>
-#include <mutex>
-#include <tuple>
 #include <type_traits>
 
 #include "common.cuh"
@@ -553,20 +550,11 @@ NormKernel backward_kernel(const LayerNormArgs& a, const NormShape& n, bool bias
 }
 bool on_16_bytes(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-constexpr int kPlainSmem = 40 * 1024;      // dynamic shared memory that needs no leave (48 KB with the static one)
-
-// CTAs of a kernel that fit on an SM, asked for once per kernel and block size
-int resident_ctas(const void* fn, int threads, int smem) {
-    static std::mutex lock;
-    static std::map<std::tuple<const void*, int, int>, int> known;
-    const std::lock_guard<std::mutex> guard(lock);
-    int& n = known[{fn, threads, smem}];
-    if (n == 0) {
-        if (smem > kPlainSmem) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, threads, smem) != cudaSuccess) cudaGetLastError();
-        n = std::max(1, n);
-    }
-    return n;
+// At most `ctas` CTAs, as many as fit on the SMs.  Not asked for where every CTA has an SM: that would be a tenth of what a small call takes.
+int resident_ctas(const void* fn, int threads, int smem, int64_t ctas, int num_sms) {
+    int n = 1;
+    if (ctas > num_sms) allow_shared_memory(fn, threads, smem, &n);      // (what fails here fails again, and is reported, at the launch)
+    return static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(n) * num_sms));
 }
 
 bool rows_on_16_bytes(const LayerNormArgs& a, bool backward) {
@@ -576,12 +564,9 @@ bool rows_on_16_bytes(const LayerNormArgs& a, bool backward) {
 }
 
 cudaError_t launch_rows(const void* fn, const NormShape& n, void** params, cudaStream_t stream) {
-    if (n.smem > kPlainSmem) {
-        const cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, n.smem);
-        if (err != cudaSuccess) {
-            cudaGetLastError();      // the caller reports it
-            return err;
-        }
+    if (n.smem > 40 * 1024) {      // (48 KB with the static one need no leave)
+        const cudaError_t err = allow_shared_memory(fn, n.threads * n.rows_per_cta, n.smem, nullptr);
+        if (err != cudaSuccess) return err;
     }
     return launch_dependent(fn, dim3(n.ctas), dim3(n.threads, n.rows_per_cta), params, n.smem, stream);
 }
@@ -606,7 +591,7 @@ cudaError_t launch_layer_norm(const LayerNormArgs& args, int num_sms, cudaStream
     }
     const void* fn = reinterpret_cast<const void*>(forward_kernel(a, n));
     const int64_t ctas = (static_cast<int64_t>(a.rows) + n.rows_per_cta - 1) / n.rows_per_cta;
-    n.ctas = static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(resident_ctas(fn, n.threads * n.rows_per_cta, 0)) * num_sms));
+    n.ctas = resident_ctas(fn, n.threads * n.rows_per_cta, 0, ctas, num_sms);
     void* params[] = {&a};
     return launch_rows(fn, n, params, stream);
 }
@@ -626,11 +611,10 @@ NormShape layer_norm_backward_shape(const LayerNormArgs& a, int num_sms) {
     n.rows_per_cta = n.warp_rows ? 8 : 1;
     n.smem = norm_stages(size, n.vec, n.values) * 2 * n.values * size * n.threads * n.rows_per_cta;
     if (n.warp_rows) n.smem = std::max(n.smem, n.rows_per_cta * 2 * a.hidden * 4);
-    const int per_sm = resident_ctas(reinterpret_cast<const void*>(backward_kernel(a, n, true)), n.threads * n.rows_per_cta, n.smem);
     // every slice of the gradient's sums costs a row of 32-bit values written and read again: at least four rows share one
     int64_t ctas = (static_cast<int64_t>(a.rows) + n.rows_per_cta - 1) / n.rows_per_cta;
     ctas = std::min<int64_t>(ctas, std::max<int64_t>(num_sms, a.rows / 4));
-    n.ctas = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ctas, static_cast<int64_t>(per_sm) * num_sms)));
+    n.ctas = std::max(1, resident_ctas(reinterpret_cast<const void*>(backward_kernel(a, n, true)), n.threads * n.rows_per_cta, n.smem, ctas, num_sms));
     return n;
 }
 

@@ -2,6 +2,11 @@
 // get_dispatch_layout, and a stand-alone bf16 -> e4m3 (1x128 scales) cast.
 // Parity: barrier_impl (deep_ep/include/deep_ep/impls/barrier.cuh:11-40), get_dispatch_layout
 // (csrc/kernels/legacy/layout.cu:10-150), per_token_cast_to_fp8 (deep_ep/utils/math.py:30-39).
+#include <algorithm>
+#include <map>
+#include <mutex>
+#include <tuple>
+
 #include "common.cuh"
 
 namespace ep {
@@ -20,6 +25,30 @@ cudaError_t launch_dependent(const void* fn, dim3 grid, dim3 block, void** param
     const cudaError_t err = cudaLaunchKernelExC(&config, fn, params);
     if (err != cudaSuccess) cudaGetLastError();   // the caller reports it
     return err;
+}
+cudaError_t allow_shared_memory(const void* fn, int threads, int smem, int* ctas) {
+    static std::mutex lock;
+    static std::map<std::tuple<int, const void*, int, int>, int> known;
+    int device = 0;
+    cudaError_t err = cudaGetDevice(&device);
+    if (err != cudaSuccess) return err;
+    const std::lock_guard<std::mutex> guard(lock);
+    int& n = known[{device, fn, threads, smem}];
+    if (n == 0) {
+        // (the largest size counts: leave is never taken back from launches of another one)
+        cudaFuncAttributes now;
+        err = cudaFuncGetAttributes(&now, fn);
+        if (err == cudaSuccess && smem > now.maxDynamicSharedSizeBytes) err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        int fit = 0;
+        if (err == cudaSuccess) err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, fn, threads, smem);
+        if (err != cudaSuccess) {
+            cudaGetLastError();      // the caller reports it
+            return err;
+        }
+        n = std::max(1, fit);
+    }
+    if (ctas != nullptr) *ctas = n;
+    return cudaSuccess;
 }
 
 namespace {

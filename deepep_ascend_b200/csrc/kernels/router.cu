@@ -9,9 +9,6 @@
 // The sum of the exponentials is a tree: the experts, padded with zeros to a power of two, are halved and the upper half is added to the lower one.
 // That order is part of the definition: scores that differ in their last bit would choose another expert where two are as good.
 #include <algorithm>
-#include <map>
-#include <mutex>
-#include <tuple>
 #include <type_traits>
 
 #include "common.cuh"
@@ -617,22 +614,11 @@ bool bad_router_args(const RouterArgs& a) {
     return a.num_experts < 1 || a.num_experts > EP_MAX_EXPERTS || a.num_topk < 1 || a.num_topk > EP_MAX_TOPK || a.num_tokens < 0 || a.ld < a.num_experts;
 }
 
-// CTAs of a kernel that fit on an SM, asked for once per kernel and shape
-int resident_ctas(const void* fn, int threads, int smem) {
-    static std::mutex lock;
-    static std::map<std::tuple<const void*, int, int>, int> known;
-    const std::lock_guard<std::mutex> guard(lock);
-    int& n = known[{fn, threads, smem}];
-    if (n == 0) {
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, fn, threads, smem) != cudaSuccess) cudaGetLastError();
-        n = std::max(1, n);
-    }
-    return n;
-}
-cudaError_t allow_smem(const void* fn, int bytes) {
-    if (bytes <= 48 * 1024) return cudaSuccess;
-    const cudaError_t err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (err != cudaSuccess) cudaGetLastError();      // the caller reports it
+// CTAs of a launch, and leave for its shared memory.  Nothing is asked for small launches that need neither: it is a tenth of what they take.
+cudaError_t grid_of(const void* fn, int threads, int smem, int64_t ctas, int num_sms, int& grid) {
+    int per_sm = 1;
+    const cudaError_t err = ctas <= num_sms && smem <= 48 * 1024 ? cudaSuccess : allow_shared_memory(fn, threads, smem, &per_sm);
+    grid = static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(num_sms) * per_sm));
     return err;
 }
 // warps of a CTA: eight, or as many as have room
@@ -657,10 +643,10 @@ cudaError_t launch_route(const RouterArgs& args, int num_sms, cudaStream_t strea
     int warps = warps_of(4 * l.warp, shared);
     if (a.num_tokens <= warps * tokens) warps = std::max(1, (a.num_tokens + tokens - 1) / tokens);
     const int smem = warps * 4 * l.warp + shared;
-    cudaError_t err = allow_smem(fn, smem);
-    if (err != cudaSuccess) return err;
     const int64_t per_cta = static_cast<int64_t>(warps) * tokens, ctas = (a.num_tokens + per_cta - 1) / per_cta;
-    const int grid = ctas == 1 ? 1 : static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(num_sms) * resident_ctas(fn, warps * 32, smem)));
+    int grid = 1;
+    cudaError_t err = grid_of(fn, warps * 32, smem, ctas, num_sms, grid);
+    if (err != cudaSuccess) return err;
     if (grid > 1) err = cudaMemsetAsync(a.count, 0, sizeof(int32_t) * a.num_experts, stream);
     if (err != cudaSuccess) return err;
     void* params[] = {&a, &tokens};
@@ -681,10 +667,10 @@ cudaError_t launch_route_backward(const RouterArgs& args, int num_sms, cudaStrea
     const RouterKernel kernel = a.logits_bf16 ? route_backward_kernel<true> : route_backward_kernel<false>;
     const void* fn = reinterpret_cast<const void*>(kernel);
     const int rows = a.logits_bf16 ? 8 : 4, per_warp = 2 * rows * a.num_experts * (a.logits_bf16 ? 2 : 4), warps = warps_of(per_warp, 0), smem = warps * per_warp;
-    const cudaError_t err = allow_smem(fn, smem);
-    if (err != cudaSuccess) return err;
     const int64_t ctas = (a.num_tokens + warps * rows - 1) / (warps * rows);
-    const int grid = static_cast<int>(std::min<int64_t>(ctas, static_cast<int64_t>(num_sms) * resident_ctas(fn, warps * 32, smem)));
+    int grid = 1;
+    const cudaError_t err = grid_of(fn, warps * 32, smem, ctas, num_sms, grid);
+    if (err != cudaSuccess) return err;
     return launch_dependent(fn, dim3(grid), dim3(warps * 32), params, smem, stream);
 }
 

@@ -36,6 +36,8 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
         return layer_norm_backward_ref(dy, x, weight, mean, rstd, with_bias)
     if dy.shape != x.shape:
         raise ValueError('dy must have the shape of x, got %s and %s' % (tuple(dy.shape), tuple(x.shape)))
+    if x.dim() == 2 and mean.dim() == rstd.dim() == 1:
+        return _native.load().layer_norm_backward(_rows(dy), _rows(x), weight, mean, rstd, with_bias)
     dx, dw, db = _native.load().layer_norm_backward(_rows(dy), _rows(x), weight, mean.reshape(-1), rstd.reshape(-1), with_bias)
     return dx if x.dim() == 2 else dx.view(x.shape), dw, db
 
