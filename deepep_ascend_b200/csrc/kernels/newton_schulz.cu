@@ -249,6 +249,63 @@ __device__ __forceinline__ void finish_gram(const NsArgs& g, uint8_t* staging, i
     store_symmetric(g, staging, matrix, b, v, mirror);
 }
 
+// B X in kUnitA kUnitX, the old X and the diagonal of Q -> the new X, or (the last step) the result
+__device__ __forceinline__ void finish_update(const NsArgs& g, uint8_t* staging, int matrix, const Block& b, float (&v)[4][8], const uint4 (&old)[4], const uint4 (&low)[4],
+                                              const float (&row_value)[4]) {
+    const int64_t wide = static_cast<int64_t>(matrix) * g.rows * g.ld_x;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float hi[8], lo[8];
+        unpack_half(old[i], hi);
+        unpack_half(low[i], lo);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = row_value[i] * (hi[j] + lo[j] * (1.f / kUnitLo)) + v[i][j] * (1.f / kUnitA);     // in kUnitX
+    }
+    if (g.out == nullptr) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t o[4], l[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                o[j] = pack_half(v[i][2 * j], v[i][2 * j + 1]);
+                const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&o[j]));
+                l[j] = pack_half((v[i][2 * j] - hi.x) * kUnitLo, (v[i][2 * j + 1] - hi.y) * kUnitLo);
+            }
+            if (b.row(i) < g.rows && b.col() < g.ld_x) {
+                const int64_t at = wide + static_cast<int64_t>(b.row(i)) * g.ld_x + b.col();
+                *reinterpret_cast<uint4*>(g.x_out + at) = make_uint4(o[0], o[1], o[2], o[3]);
+                *reinterpret_cast<uint4*>(g.x_lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
+            }
+        }
+    } else {
+        // the last step: the result, in the caller's orientation
+        uint16_t* dst = reinterpret_cast<uint16_t*>(g.out) + static_cast<int64_t>(matrix) * g.rows * g.cols;
+        uint32_t o[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[i][2 * j] * (1.f / kUnitX), v[i][2 * j + 1] * (1.f / kUnitX));
+                o[i][j] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        const int out_rows = g.out_transposed ? g.cols : g.rows, out_cols = g.out_transposed ? g.rows : g.cols;
+        if (out_cols % 8 != 0) {
+            by_value(staging, o, b, g.out_transposed != 0, [&](int row, int col, uint16_t value) {
+                if (row < out_rows && col < out_cols) dst[static_cast<int64_t>(row) * out_cols + col] = value;
+            });
+        } else if (g.out_transposed) {
+            transposed(staging, o, b, [&](int row, int col, const uint2& four) {
+                if (row < out_rows && col < out_cols) *reinterpret_cast<uint2*>(dst + static_cast<int64_t>(row) * out_cols + col) = four;
+            });
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (b.row(i) < out_rows && b.col() < out_cols)
+                    *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(b.row(i)) * out_cols + b.col()) = make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
+        }
+    }
+}
+
 // What a product of `mode` runs over
 template <int kMode, int kBlockN>
 struct NsWork {
@@ -450,57 +507,7 @@ __device__ __forceinline__ bool ns_finish(const NsArgs& g, const NsShared<kBlock
                 }
                 store_symmetric(g, staging, t.g, b, v, t.mirror);
             } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float hi[8], lo[8];
-                    unpack_half(old[c & 1][i], hi);
-                    unpack_half(low[c & 1][i], lo);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[i][j] = row_value[i] * (hi[j] + lo[j] * (1.f / kUnitLo)) + v[i][j] * (1.f / kUnitA);     // in kUnitX
-                }
-                if (g.out == nullptr) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t o[4], l[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            o[j] = pack_half(v[i][2 * j], v[i][2 * j + 1]);
-                            const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&o[j]));
-                            l[j] = pack_half((v[i][2 * j] - hi.x) * kUnitLo, (v[i][2 * j + 1] - hi.y) * kUnitLo);
-                        }
-                        if (b.row(i) < g.rows && b.col() < width) {
-                            const int64_t at = wide + static_cast<int64_t>(b.row(i)) * g.ld_x + b.col();
-                            *reinterpret_cast<uint4*>(g.x_out + at) = make_uint4(o[0], o[1], o[2], o[3]);
-                            *reinterpret_cast<uint4*>(g.x_lo + at) = make_uint4(l[0], l[1], l[2], l[3]);
-                        }
-                    }
-                } else {
-                    // the last step: the result, in the caller's orientation
-                    uint16_t* dst = reinterpret_cast<uint16_t*>(g.out) + static_cast<int64_t>(t.g) * g.rows * g.cols;
-                    uint32_t o[4][4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const __nv_bfloat162 h = __floats2bfloat162_rn(v[i][2 * j] * (1.f / kUnitX), v[i][2 * j + 1] * (1.f / kUnitX));
-                            o[i][j] = *reinterpret_cast<const uint32_t*>(&h);
-                        }
-                    const int out_rows = g.out_transposed ? g.cols : g.rows, out_cols = g.out_transposed ? g.rows : g.cols;
-                    if (out_cols % 8 != 0) {
-                        by_value(staging, o, b, g.out_transposed != 0, [&](int row, int col, uint16_t value) {
-                            if (row < out_rows && col < out_cols) dst[static_cast<int64_t>(row) * out_cols + col] = value;
-                        });
-                    } else if (g.out_transposed) {
-                        transposed(staging, o, b, [&](int row, int col, const uint2& four) {
-                            if (row < out_rows && col < out_cols) *reinterpret_cast<uint2*>(dst + static_cast<int64_t>(row) * out_cols + col) = four;
-                        });
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (b.row(i) < out_rows && b.col() < out_cols)
-                                *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(b.row(i)) * out_cols + b.col()) = make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
-                    }
-                }
+                finish_update(g, staging, t.g, b, v, old[c & 1], low[c & 1], row_value);
             }
         }
         umma::fence_before_thread_sync();
@@ -552,8 +559,8 @@ __device__ __forceinline__ void ns_quiet(const NsShared<kBlockN>& s) {
 // One product of one step: a persistent CTA per SM, a warp that requests operands, one that issues the products, eight that finish tiles while the next one's products run
 // (two accumulators).  Bound by the tensor cores and, in long runs, by power: 8 x 4096 x 7168 alone takes 707 us for X X^T, 413 for a product of squares (half of either
 // is computed) and 1490 for X, 1.3 to 1.4 PFLOP/s; all 19 products in a row 14.6 ms, 1.0 PFLOP/s.  4 x 2048 x 3584: tensor pipe 72 % busy for X X^T and X, 53 to 59 % for squares
-// (tiles of 32 K blocks).  Below some 1000 rows the chain of launches is what counts: 256 x 7168 takes 120 us in 22 launches, 7.1 GFLOP; all steps in one launch whose CTAs
-// wait for one another took 147, parts along K in a cluster's shared memory 145.
+// (tiles of 32 K blocks).  Below some 1000 rows the chain of launches is what counts: 3 x 777 x 1001 takes 171 us in 17 launches, 34 GFLOP; all steps in one launch whose
+// CTAs wait for one another took 237 (183 without), parts along K in a cluster's shared memory 145 for 256 x 7168 (121 without).
 template <int kMode, int kBlockN>
 __global__ void __launch_bounds__(kNsThreads, 1)
 ns_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ NsArgs g) {
@@ -582,6 +589,186 @@ ns_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
         ns_finish<kMode, kBlockN>(g, s, tmem_base, acc, acc_phase);
     }
     ns_teardown<kBlockN>(tmem_base);
+}
+
+// Short matrices: Q and X <- Q X in one kernel, a CTA per 128 x 128 tile of X, which makes the 128 rows of B that it needs itself and writes them over those of O, as the first
+// operand of its second product.  One launch less per step, which is what these matrices take.
+// Five steps with and without, in us: 64 x 64 47 and 60, 256 x 256 80 and 92, 256 x 7168 111 and 120, 32 of 256 x 256 93 and 111.
+template <int kRows>
+struct NsStepShared {
+    static constexpr int kBlocks = kRows / kTileK, kBlockBytes = kRows * 128, kBytesX = kTileM * 128;       // blocks of 64 columns of O, of 64 rows of X
+    uint8_t *o, *x, *staging;
+    NsSmem* sm;
+    float* coef;                                       // [128] the diagonal of Q
+    __device__ __forceinline__ explicit NsStepShared(uint8_t* smem)
+        : o(smem), x(smem + kBlocks * kBlockBytes), staging(x + kBlocks * kBytesX + 1024), sm(reinterpret_cast<NsSmem*>(x + kBlocks * kBytesX)),
+          coef(reinterpret_cast<float*>(x + kBlocks * kBytesX + 512)) {}
+    static constexpr int kBytes = kBlocks * (kBlockBytes + kBytesX) + 1024 + kEpiWarps * kStagingBytes;
+    // eight neighbouring values of O or B
+    __device__ __forceinline__ uint4* at(int row, int col) const {
+        return reinterpret_cast<uint4*>(o + (col / kTileK) * kBlockBytes + row * 128 + ((((col % kTileK) / 8) ^ (row & 7)) * 16));
+    }
+};
+template <int kRows>
+__device__ __forceinline__ bool ns_step_multiply(const NsArgs& g, const NsStepShared<kRows>& s, uint32_t tmem_base, int m, int num_k) {
+    constexpr uint32_t kSquare = umma::make_instr_desc(kTileM, kRows, umma::kFormatF16), kWide = umma::make_instr_desc(kTileM, kTileM, umma::kFormatF16, false, true);
+    auto mine = [&](int kb) { return umma::make_smem_desc_sw128(s.o + kb * s.kBlockBytes + m * kTileM * 128); };
+    if (!ns_wait(&s.sm->full[0], 0, s.sm, g.report, 4)) return false;
+    umma::fence_after_thread_sync();
+    for (int kb = 0; kb < num_k; ++kb) {
+        const uint64_t desc_b = umma::make_smem_desc_sw128(s.o + kb * s.kBlockBytes);
+#pragma unroll
+        for (int k = 0; k < kTileK / 16; ++k)
+            umma::mma_ss<false>(tmem_base, umma::advance_desc_k(mine(kb), k * 32), umma::advance_desc_k(desc_b, k * 32), kSquare, kb != 0 || k != 0);
+    }
+    umma::mma_commit(&s.sm->acc_full[0]);
+    if (!ns_wait(&s.sm->acc_empty[0], 0, s.sm, g.report, 2) || !ns_wait(&s.sm->full[1], 0, s.sm, g.report, 4)) return false;
+    umma::fence_after_thread_sync();
+    for (int kb = 0; kb < num_k; ++kb) {
+        const uint64_t desc_b = umma::make_smem_desc_mn_sw128(s.x + kb * s.kBytesX);
+#pragma unroll
+        for (int k = 0; k < kTileK / 16; ++k)
+            umma::mma_ss<false>(tmem_base + kRows, umma::advance_desc_k(mine(kb), k * 32), umma::advance_desc_k(desc_b, k * 16 * 128), kWide, kb != 0 || k != 0);
+    }
+    umma::mma_commit(&s.sm->acc_full[1]);
+    return true;
+}
+template <int kRows>
+__device__ __forceinline__ void ns_step_finish(const NsArgs& g, const NsStepShared<kRows>& s, uint32_t tmem_base, const NsTile& t) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* staging = s.staging + (warp - 2) * kStagingBytes;
+    const uint32_t tmem = tmem_base + (static_cast<uint32_t>(quad * 32) << 16);
+    const float* diag = g.diag_in + static_cast<int64_t>(t.g) * g.ld_sq;
+    const int64_t wide = static_cast<int64_t>(t.g) * g.rows * g.ld_x;
+    const int row0 = t.m * kTileM + quad * 32;
+    auto sums = [&](uint32_t column, float (&v)[4][8]) {
+        uint32_t r[32];
+        umma::tmem_ld_32x32(tmem + column, r);
+        umma::tmem_ld_wait();
+        spread(staging, r, v);
+    };
+    float di[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = row0 + i * 8 + (lane >> 2);
+        di[i] = row < g.rows ? diag[row] : 0.f;
+    }
+    // (O itself as well: its values are read here)
+    bool ok = __all_sync(0xffffffffu, ns_wait(&s.sm->full[0], 0, s.sm, g.report, 4) && ns_wait(&s.sm->acc_full[0], 0, s.sm, g.report, 5));
+    umma::fence_after_thread_sync();
+    if (ok) {
+#pragma unroll 1
+        for (int c = 0; c < kRows / 64; ++c) {
+            const Block b{row0, half * (kRows / 2) + c * 32};
+            float dj[8], v[4][8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dj[j] = b.col() + j < g.rows ? diag[b.col() + j] : 0.f;
+            sums(b.col0, v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint4* at = s.at(b.row(i), b.col());
+                float f[8];
+                unpack_half(*at, f);
+                const float coefficient = g.b + g.c * di[i];
+                if (b.row0 == b.col0) {
+                    const float d = take_diagonal(v[i], b.row(i) - b.col());
+                    if (b.on_diagonal(i)) s.coef[quad * 32 + i * 8 + (lane >> 2)] = b.row(i) < g.rows ? g.a + g.b * di[i] + g.c * (di[i] * di[i] + d * (1.f / (kUnitA * kUnitA))) : 0.f;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[i][j] = (coefficient + g.c * dj[j]) * f[j] + g.c * (1.f / kUnitA) * v[i][j];
+                *at = make_uint4(pack_half(v[i][0], v[i][1]), pack_half(v[i][2], v[i][3]), pack_half(v[i][4], v[i][5]), pack_half(v[i][6], v[i][7]));
+            }
+        }
+        ptx::fence_proxy_async_smem();
+        umma::fence_before_thread_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&s.sm->acc_empty[0]);
+    }
+    // the old X, and the diagonal that other warps have made.  (Every warp comes here, whatever became of its wait.)
+    uint4 old[2][4], low[2][4];
+    auto block = [&](int c) { return Block{row0, t.n * kTileM + half * 64 + c * 32}; };
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const Block b = block(c);
+            const bool in = b.row(i) < g.rows && b.col() < g.ld_x;
+            const int64_t at = wide + static_cast<int64_t>(b.row(i)) * g.ld_x + b.col();
+            old[c][i] = in ? *reinterpret_cast<const uint4*>(g.x_in + at) : make_uint4(0, 0, 0, 0);
+            low[c][i] = in ? *reinterpret_cast<const uint4*>(g.x_lo + at) : make_uint4(0, 0, 0, 0);
+        }
+    asm volatile("bar.sync 1, %0;" ::"n"(kEpiWarps * 32) : "memory");
+    if (!ok) return;
+    float q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = s.coef[quad * 32 + i * 8 + (lane >> 2)];
+    ok = __all_sync(0xffffffffu, ns_wait(&s.sm->acc_full[1], 0, s.sm, g.report, 5));
+    if (!ok) return;
+    umma::fence_after_thread_sync();
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        const Block b = block(c);
+        if (b.row0 >= g.rows || b.col0 >= g.ld_x) break;
+        float v[4][8];
+        sums(kRows + half * 64 + c * 32, v);
+        finish_update(g, staging, t.g, b, v, old[c], low[c], q);
+    }
+}
+template <int kRows>
+__global__ void __launch_bounds__(kNsThreads, 1)
+ns_step_kernel(const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ NsArgs g) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const NsStepShared<kRows> s(smem);
+    constexpr int kColumns = kRows + kTileM <= 256 ? 256 : 512;
+    const int warp = threadIdx.x >> 5, num_m = (g.rows + kTileM - 1) / kTileM, num_k = (g.rows + kTileK - 1) / kTileK;
+    if (threadIdx.x == 0) {
+        umma::prefetch_tensormap(&map_o);
+        umma::prefetch_tensormap(&map_x);
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&s.sm->full[i], 1);
+            ptx::mbar_init(&s.sm->acc_full[i], 1);
+        }
+        ptx::mbar_init(&s.sm->acc_empty[0], kEpiWarps);
+        ptx::mbar_init(&s.sm->quiet, 1);
+        s.sm->failed = 0;
+        ptx::mbar_fence_init();
+    }
+    if (warp == 1) {
+        umma::tmem_alloc(&s.sm->tmem_base, kColumns);
+        umma::tmem_relinquish();
+    }
+    umma::fence_before_thread_sync();
+    __syncthreads();
+    umma::fence_after_thread_sync();
+    const uint32_t tmem_base = s.sm->tmem_base;
+    ptx::wait_for_previous_kernel();
+    const NsTile t = ns_tile<kTileM, false>(blockIdx.x, num_m * ((g.cols + kTileM - 1) / kTileM), num_m);
+    if (warp == 0) {
+        if (ptx::elect_one()) {
+            ptx::mbar_arrive_expect_tx(&s.sm->full[0], num_k * s.kBlockBytes);
+            for (int kb = 0; kb < num_k; ++kb)
+#pragma unroll
+                for (int r = 0; r < kRows; r += kTileM) umma::tma_load_3d(s.o + kb * s.kBlockBytes + r * 128, &map_o, kb * kTileK, r, t.g, &s.sm->full[0]);
+            ptx::mbar_arrive_expect_tx(&s.sm->full[1], num_k * s.kBytesX);
+            for (int kb = 0; kb < num_k; ++kb)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) umma::tma_load_3d(s.x + kb * s.kBytesX + i * umma::kMnChunkBytes, &map_x, t.n * kTileM + i * 64, kb * kTileK, t.g, &s.sm->full[1]);
+            ptx::let_next_kernel_start();
+            // whatever the others wait for: what was requested has landed before the shared memory goes to another CTA
+            mbar_drain(&s.sm->full[0], 0, 1000000000ull);
+            mbar_drain(&s.sm->full[1], 0, 1000000000ull);
+        }
+    } else if (warp == 1) {
+        if (ptx::elect_one() && !ns_step_multiply(g, s, tmem_base, t.m, num_k)) {
+            umma::mma_commit(&s.sm->quiet);
+            mbar_drain(&s.sm->quiet, 0, 1000000000ull);
+        }
+    } else {
+        ns_step_finish(g, s, tmem_base, t);
+    }
+    umma::fence_before_thread_sync();
+    __syncthreads();
+    if (warp == 1) umma::tmem_dealloc(tmem_base, kColumns);
 }
 
 // Eight rows of 32 values of a tile: the parts of X X^T added in their order, eight requested at a time.  Many small pieces, since what this takes is the way of the parts
@@ -812,19 +999,23 @@ cudaError_t allow_smem(const void* fn, int bytes) {
     if (err != cudaSuccess) cudaGetLastError();      // the caller reports it
     return err;
 }
-template <int kMode, int kBlockN>
-cudaError_t launch_product(const CUtensorMap& map_a, const CUtensorMap& map_b, const NsArgs& g, int num_sms, cudaStream_t stream) {
-    const void* fn = reinterpret_cast<const void*>(ns_kernel<kMode, kBlockN>);
-    // leave for that much shared memory is asked for once per device: a step has three launches, and they are what small matrices take
-    static std::atomic<uint64_t> allowed{0};
+// ... once per device: a step has few launches, and they are what small matrices take
+cudaError_t allow_once(const void* fn, int bytes, std::atomic<uint64_t>& allowed) {
     int device = 0;
     cudaError_t err = cudaGetDevice(&device);
     if (err != cudaSuccess) return err;
     if (device >= 64 || (allowed.load(std::memory_order_relaxed) >> device & 1) == 0) {
-        err = allow_smem(fn, ns_smem_bytes(kBlockN));
-        if (err != cudaSuccess) return err;
-        if (device < 64) allowed.fetch_or(1ull << device, std::memory_order_relaxed);
+        err = allow_smem(fn, bytes);
+        if (err == cudaSuccess && device < 64) allowed.fetch_or(1ull << device, std::memory_order_relaxed);
     }
+    return err;
+}
+template <int kMode, int kBlockN>
+cudaError_t launch_product(const CUtensorMap& map_a, const CUtensorMap& map_b, const NsArgs& g, int num_sms, cudaStream_t stream) {
+    const void* fn = reinterpret_cast<const void*>(ns_kernel<kMode, kBlockN>);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t err = allow_once(fn, ns_smem_bytes(kBlockN), allowed);
+    if (err != cudaSuccess) return err;
     const int64_t items = tiles_of(g, kMode, kBlockN) * (kMode == kGramPart ? g.k_splits : 1);
     void* params[] = {const_cast<CUtensorMap*>(&map_a), const_cast<CUtensorMap*>(&map_b), const_cast<NsArgs*>(&g)};
     return launch_dependent(fn, dim3(static_cast<unsigned>(std::min<int64_t>(items, num_sms))), dim3(kNsThreads), params, ns_smem_bytes(kBlockN), stream);
@@ -834,6 +1025,18 @@ cudaError_t launch_product(int block_n, const CUtensorMap& map_a, const CUtensor
     if constexpr (kMode == kUpdate)
         if (block_n == 192) return launch_product<kMode, 192>(map_a, map_b, g, num_sms, stream);
     return block_n == 256 ? launch_product<kMode, 256>(map_a, map_b, g, num_sms, stream) : launch_product<kMode, 128>(map_a, map_b, g, num_sms, stream);
+}
+
+// Short matrices whose tiles of X have an SM each: more tiles would make the polynomial again and again
+bool in_one_kernel(const NsArgs& g, int num_sms) { return g.rows <= 256 && tiles_of(g, kUpdate, kTileM) <= num_sms; }
+template <int kRows>
+cudaError_t launch_step(const CUtensorMap& map_o, const CUtensorMap& map_x, const NsArgs& g, cudaStream_t stream) {
+    const void* fn = reinterpret_cast<const void*>(ns_step_kernel<kRows>);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t err = allow_once(fn, NsStepShared<kRows>::kBytes, allowed);
+    if (err != cudaSuccess) return err;
+    void* params[] = {const_cast<CUtensorMap*>(&map_o), const_cast<CUtensorMap*>(&map_x), const_cast<NsArgs*>(&g)};
+    return launch_dependent(fn, dim3(static_cast<unsigned>(tiles_of(g, kUpdate, kTileM))), dim3(kNsThreads), params, NsStepShared<kRows>::kBytes, stream);
 }
 
 int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
@@ -898,7 +1101,7 @@ cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8
     g.parts = reinterpret_cast<float*>(workspace + w.parts);
     g.k_splits = w.k_splits;
     g.out = nullptr;
-    const bool pairs = in_pairs(g);
+    const bool pairs = in_pairs(g), one_kernel = in_one_kernel(g, num_sms);
     const int n_gram = g.k_splits > 1 ? 128 : block_n_of(g, kGram, num_sms), n_square = block_n_of(g, kPoly, num_sms), n_update = block_n_of(g, kUpdate, num_sms);
     // X in turn; symmetric matrices: their rows as the first and as the second operand
     struct Wide {
@@ -948,6 +1151,13 @@ cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8
         g.diag_out = to.diag;
         return launch_product<kProduct>(n_square, p.rows, r.cols, g, num_sms, stream);
     };
+    // X <- Q X, with Q of A
+    auto step = [&](const Square& from_a, const Wide& from, const Wide& to) {
+        g.diag_in = from_a.diag;
+        g.x_in = from.x;
+        g.x_out = to.x;
+        return g.rows <= 128 ? launch_step<128>(from_a.rows, from.mn, g, stream) : launch_step<256>(from_a.rows, from.mn, g, stream);
+    };
     auto update = [&](const Square& q, const Wide& from, const Wide& to) {
         g.diag_in = q.diag;
         g.x_in = from.x;
@@ -961,7 +1171,7 @@ cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8
         const bool pair = pairs && done + 2 <= steps;
         done += pair ? 2 : 1;
         err = gram(x[from], sq[0]);
-        if (err == cudaSuccess) err = poly(sq[0], sq[1]);
+        if (err == cudaSuccess && !one_kernel) err = poly(sq[0], sq[1]);
         if (pair) {
             if (err == cudaSuccess) err = product(sq[1], sq[0], sq[2]);      // T = Q1 A
             if (err == cudaSuccess) err = product(sq[2], sq[1], sq[0]);      // A = T Q1
@@ -969,7 +1179,7 @@ cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8
             if (err == cudaSuccess) err = product(sq[2], sq[1], sq[0]);      // Q = Q2 Q1
         }
         if (done == steps) g.out = args.out;
-        if (err == cudaSuccess) err = update(sq[pair ? 0 : 1], x[from], x[from ^ 1]);
+        if (err == cudaSuccess) err = one_kernel ? step(sq[0], x[from], x[from ^ 1]) : update(sq[pair ? 0 : 1], x[from], x[from ^ 1]);
     }
     return err;
 }

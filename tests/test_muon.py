@@ -73,6 +73,19 @@ def test_more_tiles_than_one_wave_and_few_sms(count, rows, cols):
         assert _error(orthogonalize(x[i]), want[i]) < BOUND['strong directions']
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize('kind', sorted(BOUND))
+@pytest.mark.parametrize('count,rows,cols', [(1, 256, 9000), (2, 130, 4800), (4, 128, 4096), (2, 6001, 255), (1, 129, 200), (70, 96, 250), (3, 64, 5000)])
+def test_short_matrices_in_either_form(count, rows, cols, kind):
+    """Polynomial and update in one kernel, or (more tiles than SMs) in two."""
+    x = _matrix(kind, count, rows, cols).bfloat16().cuda()
+    want = _exact(x)
+    for sms in (0, 100, 20):
+        got = orthogonalize(x, num_sms=sms)
+        assert _error(got, want) < BOUND[kind]
+        assert torch.equal(orthogonalize(x, num_sms=sms), got)
+
+
 def _falling(count, rows, cols, orders):
     """Singular values that fall off evenly by 10^orders."""
     g = torch.Generator().manual_seed(orders)
