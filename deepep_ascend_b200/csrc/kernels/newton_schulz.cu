@@ -1039,7 +1039,8 @@ cudaError_t launch_step(const CUtensorMap& map_o, const CUtensorMap& map_x, cons
     return launch_dependent(fn, dim3(static_cast<unsigned>(tiles_of(g, kUpdate, kTileM))), dim3(kNsThreads), params, NsStepShared<kRows>::kBytes, stream);
 }
 
-int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+// rows of 128 bytes: a box of rows that start elsewhere takes three times as long on its way into shared memory
+int64_t round64(int64_t n) { return (n + 63) / 64 * 64; }
 
 template <class T>
 cudaError_t launch_first(const NsArgs& g, cudaStream_t stream) {
@@ -1070,8 +1071,8 @@ bool in_pairs(const NsArgs& g) {
 // Workspace: hi of X twice and lo once, three symmetric matrices (two without pairs) and their diagonals, sums of squares, parts of X X^T.
 NsWorkspace newton_schulz_workspace(const NsArgs& g, int num_sms) {
     NsWorkspace w{};
-    w.ld_x = round8(g.cols);
-    w.ld_sq = round8(g.rows);
+    w.ld_x = round64(g.cols);
+    w.ld_sq = round64(g.rows);
     w.norm_parts = std::max<int64_t>(1, std::min<int64_t>((static_cast<int64_t>(g.rows) * g.cols + 8191) / 8192, 8 * num_sms / g.count));
     w.k_splits = k_splits_of(g, num_sms);
     auto take = [&](int64_t bytes) {
