@@ -559,7 +559,7 @@ __device__ __forceinline__ void ns_quiet(const NsShared<kBlockN>& s) {
 // One product of one step: a persistent CTA per SM, a warp that requests operands, one that issues the products, eight that finish tiles while the next one's products run
 // (two accumulators).  Bound by the tensor cores and, in long runs, by power: 8 x 4096 x 7168 alone takes 707 us for X X^T, 413 for a product of squares (half of either
 // is computed) and 1490 for X, 1.3 to 1.4 PFLOP/s; all 19 products in a row 14.6 ms, 1.0 PFLOP/s.  4 x 2048 x 3584: tensor pipe 72 % busy for X X^T and X, 53 to 59 % for squares
-// (tiles of 32 K blocks).  Below some 1000 rows the chain of launches is what counts: 3 x 777 x 1001 takes 171 us in 17 launches, 34 GFLOP; all steps in one launch whose
+// (tiles of 32 K blocks).  Below some 1000 rows the chain of launches is what counts: 3 x 777 x 1001 takes 154 us in 17 launches, 34 GFLOP; all steps in one launch whose
 // CTAs wait for one another took 237 (183 without), parts along K in a cluster's shared memory 145 for 256 x 7168 (121 without).
 template <int kMode, int kBlockN>
 __global__ void __launch_bounds__(kNsThreads, 1)
@@ -1068,7 +1068,7 @@ bool in_pairs(const NsArgs& g) {
 
 }  // namespace
 
-// Workspace: hi of X twice and lo once, three symmetric matrices (two without pairs) and their diagonals, sums of squares, parts of X X^T.
+// Workspace: hi of X twice and lo once, three symmetric matrices (two without pairs, one for short matrices) and their diagonals, sums of squares, parts of X X^T.
 NsWorkspace newton_schulz_workspace(const NsArgs& g, int num_sms) {
     NsWorkspace w{};
     w.ld_x = round64(g.cols);
@@ -1083,7 +1083,7 @@ NsWorkspace newton_schulz_workspace(const NsArgs& g, int num_sms) {
     w.norms = take(g.count * w.norm_parts * 8);
     for (int64_t& x : w.x) x = take(g.count * g.rows * w.ld_x * 2);
     w.lo = take(g.count * g.rows * w.ld_x * 2);
-    for (int i = 0; i < (in_pairs(g) ? 3 : 2); ++i) {
+    for (int i = 0; i < (in_pairs(g) ? 3 : in_one_kernel(g, num_sms) ? 1 : 2); ++i) {
         w.sq[i] = take(g.count * g.rows * w.ld_sq * 2);
         w.diag[i] = take(g.count * w.ld_sq * 4);
     }
@@ -1116,15 +1116,16 @@ cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8
     } sq[3];
     for (int i = 0; i < 2; ++i) {
         x[i].x = reinterpret_cast<__half*>(workspace + w.x[i]);
-        if (!make_map(&x[i].rows, x[i].x, g.count, g.rows, g.cols, g.ld_x, kTileM) || !make_map(&x[i].cols, x[i].x, g.count, g.rows, g.cols, g.ld_x, n_gram) ||
-            !make_map(&x[i].mn, x[i].x, g.count, g.rows, g.cols, g.ld_x, 64))
-            return cudaErrorInvalidValue;
+        if (!make_map(&x[i].rows, x[i].x, g.count, g.rows, g.cols, g.ld_x, kTileM) || !make_map(&x[i].mn, x[i].x, g.count, g.rows, g.cols, g.ld_x, 64)) return cudaErrorInvalidValue;
+        x[i].cols = x[i].rows;
+        if (n_gram != kTileM && !make_map(&x[i].cols, x[i].x, g.count, g.rows, g.cols, g.ld_x, n_gram)) return cudaErrorInvalidValue;
     }
-    for (int i = 0; i < (pairs ? 3 : 2); ++i) {
+    for (int i = 0; i < (pairs ? 3 : one_kernel ? 1 : 2); ++i) {
         sq[i].m = reinterpret_cast<__half*>(workspace + w.sq[i]);
         sq[i].diag = reinterpret_cast<float*>(workspace + w.diag[i]);
-        if (!make_map(&sq[i].rows, sq[i].m, g.count, g.rows, g.rows, g.ld_sq, kTileM) || !make_map(&sq[i].cols, sq[i].m, g.count, g.rows, g.rows, g.ld_sq, n_square))
-            return cudaErrorInvalidValue;
+        if (!make_map(&sq[i].rows, sq[i].m, g.count, g.rows, g.rows, g.ld_sq, kTileM)) return cudaErrorInvalidValue;
+        sq[i].cols = sq[i].rows;
+        if (n_square != kTileM && !make_map(&sq[i].cols, sq[i].m, g.count, g.rows, g.rows, g.ld_sq, n_square)) return cudaErrorInvalidValue;
     }
     auto gram = [&](const Wide& from, const Square& to) {
         g.sq_out = to.m;

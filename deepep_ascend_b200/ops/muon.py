@@ -21,7 +21,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Tuple[float, fl
     Matrices may be stored by rows or by columns, with any distance between rows; other strides are copied first.  The products have fp16 operands and
     32-bit sums, and carry 22 bits of X and 32 bits of the diagonals from step to step, so that the result is off by little more than its rounding to
     bf16 (where large matrices of half as many columns again as rows, or more, take two steps at once: by up to 1.6 times that, if their singular values
-    fall off evenly over several orders).  The workspace (about 6 bytes per element and 4 to 6 per element of A) comes from PyTorch's allocator.
+    fall off evenly over several orders).  The workspace (about 6 bytes per element and 2 to 6 per element of A, rows of whole 128 bytes) comes from PyTorch's allocator.
     ``num_sms``: SMs to run on (0: all).
     ``buffer``: see :func:`ops.gemm.gemm_nt`."""
     if x.dim() < 2:
