@@ -37,7 +37,7 @@ class Muon(torch.optim.Optimizer):
                     state['momentum'] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
                 m, grad = state['momentum'], p.grad.float()
                 m.mul_(group['momentum']).add_(grad)
-                update = orthogonalize(grad.add_(m, alpha=group['momentum']) if group['nesterov'] else m, group['steps'], group['coefficients'], group['eps'])
+                update = orthogonalize(torch.add(grad, m, alpha=group['momentum']) if group['nesterov'] else m, group['steps'], group['coefficients'], group['eps'])
                 if group['weight_decay']:
                     p.mul_(1.0 - group['lr'] * group['weight_decay'])
                 p.add_(update, alpha=-group['lr'] * max(1.0, p.shape[-2] / p.shape[-1])**0.5)
