@@ -22,6 +22,24 @@ class Muon(torch.optim.Optimizer):
                 if p.dim() < 2:
                     raise ValueError('Muon updates matrices, got a parameter of shape %s' % (tuple(p.shape),))
 
+    def load_state_dict(self, state_dict) -> None:
+        """As the base class's, which casts a state to its parameter's type; the momentum is taken as it was saved."""
+        given = {}
+
+        def restore(_):
+            ids = (i for group in given['param_groups'] for i in group['params'])
+            for p, i in zip((p for group in self.param_groups for p in group['params']), ids):
+                for name, value in given['state'].get(i, {}).items():
+                    self.state[p][name] = value.to(p.device, torch.float32, copy=True)
+        # (behind the caller's hooks, which may give another dict, and ahead of those that look at what was loaded)
+        hooks = (self.register_load_state_dict_pre_hook(lambda _, loaded: given.update(loaded)),
+                 self.register_load_state_dict_post_hook(restore, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None

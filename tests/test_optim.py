@@ -1,4 +1,6 @@
 """The optimiser of matrices: what it leaves alone, what it keeps between steps and across a checkpoint."""
+import copy
+
 import pytest
 import torch
 
@@ -29,3 +31,32 @@ def test_the_gradient_is_the_callers(dtype, nesterov, device):
         before = grad.clone()
         opt.step()
         assert p.grad is grad and torch.equal(grad, before)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', [F32, BF16])
+def test_a_checkpoint_keeps_every_bit(dtype, device):
+    """A run that is saved and loaded goes on as the one that was not, although the base class casts loaded states to their parameter's type."""
+    def fresh():
+        p = _parameter((2, 48, 32), dtype, device)
+        return p, Muon([p], lr=0.02, weight_decay=0.1)
+    p, opt = fresh()
+    grads = _gradients(p, 5)
+    for grad in grads[:3]:
+        p.grad = grad
+        opt.step()
+    saved, weights = copy.deepcopy(opt.state_dict()), p.detach().clone()
+    resumed, other = fresh()
+    with torch.no_grad():
+        resumed.copy_(weights)
+    other.load_state_dict(saved)
+    assert opt.state[p].keys() == other.state[resumed].keys()
+    for name, value in opt.state[p].items():
+        loaded = other.state[resumed][name]
+        assert loaded.dtype == value.dtype == F32 and loaded.device == value.device and torch.equal(loaded, value)
+        assert loaded.data_ptr() != saved['state'][0][name].data_ptr()           # what was saved is not written to by later steps
+    for grad in grads[3:]:
+        for q, o in ((p, opt), (resumed, other)):
+            q.grad = grad.clone()
+            o.step()
+        assert torch.equal(p, resumed) and torch.equal(opt.state[p]['momentum'], other.state[resumed]['momentum'])
