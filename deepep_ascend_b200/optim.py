@@ -12,7 +12,9 @@ class Muon(torch.optim.Optimizer):
     """``momentum = beta * momentum + grad``; ``update = orthogonalize(grad + beta * momentum)`` (``nesterov``; otherwise of the momentum);
     ``p = p * (1 - lr * weight_decay) - lr * sqrt(max(1, rows / cols)) * update``.
 
-    Parameters are matrices or stacks of them (``[experts, rows, cols]``: every expert's matrix by itself).  The momentum is fp32."""
+    Parameters are matrices or stacks of them (``[experts, rows, cols]``: every expert's matrix by itself).  The momentum is fp32, and so is a copy of
+    16-bit parameters (``state[p]['weight']``, 4 bytes per element) that steps are added to, since most of an update is below the last place of a bf16 weight: ``p``
+    is that copy, rounded.  Where a weight has been set by others since, its value counts."""
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
                  coefficients=COEFFICIENTS, eps: float = 1e-7):
@@ -23,7 +25,7 @@ class Muon(torch.optim.Optimizer):
                     raise ValueError('Muon updates matrices, got a parameter of shape %s' % (tuple(p.shape),))
 
     def load_state_dict(self, state_dict) -> None:
-        """As the base class's, which casts a state to its parameter's type; the momentum is taken as it was saved."""
+        """As the base class's, which casts a state to its parameter's type; what is kept in fp32 is taken as it was saved."""
         given = {}
 
         def restore(_):
@@ -51,12 +53,27 @@ class Muon(torch.optim.Optimizer):
                 if p.grad is None:
                     continue
                 state = self.state[p]
-                if not state:
+                if 'momentum' not in state:
                     state['momentum'] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
                 m, grad = state['momentum'], p.grad.float()
                 m.mul_(group['momentum']).add_(grad)
                 update = orthogonalize(torch.add(grad, m, alpha=group['momentum']) if group['nesterov'] else m, group['steps'], group['coefficients'], group['eps'])
+                w = self._weight(p, state)
                 if group['weight_decay']:
-                    p.mul_(1.0 - group['lr'] * group['weight_decay'])
-                p.add_(update, alpha=-group['lr'] * max(1.0, p.shape[-2] / p.shape[-1])**0.5)
+                    w.mul_(1.0 - group['lr'] * group['weight_decay'])
+                w.add_(update, alpha=-group['lr'] * max(1.0, p.shape[-2] / p.shape[-1])**0.5)
+                if w is not p:
+                    p.copy_(w)
         return loss
+
+    @staticmethod
+    def _weight(p, state):
+        """What a step is added to: ``p``, or the fp32 copy of a 16-bit one."""
+        if p.dtype.itemsize > 2:
+            return p
+        w = state.get('weight')
+        if w is None:
+            w = state['weight'] = p.to(torch.float32, copy=True)
+        else:
+            w.copy_(torch.where(w.to(p.dtype) == p, w, p))
+        return w

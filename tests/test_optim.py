@@ -60,3 +60,54 @@ def test_a_checkpoint_keeps_every_bit(dtype, device):
             q.grad = grad.clone()
             o.step()
         assert torch.equal(p, resumed) and torch.equal(opt.state[p]['momentum'], other.state[resumed]['momentum'])
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('lr,decay', [(1e-3, 0.0), (1e-3, 0.1), (0.02, 0.1)])
+def test_bf16_weights_move_as_fp32_ones_do(lr, decay, device):
+    """Updates far below a weight's last place add up: the weights are those of an fp32 run, rounded."""
+    p, q = _parameter((2, 96, 64), BF16, device), _parameter((2, 96, 64), BF16, device)
+    q = torch.nn.Parameter(q.detach().float())
+    a, b = Muon([p], lr=lr, weight_decay=decay), Muon([q], lr=lr, weight_decay=decay)
+    start = p.detach().clone()
+    for grad in _gradients(p, 30):
+        p.grad, q.grad = grad, grad.float()
+        a.step()
+        b.step()
+        assert torch.equal(p, q.bfloat16())
+    assert (p != start).float().mean() > 0.9
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('dtype', [F32, BF16, torch.float16])
+def test_decay_alone_shrinks_the_weights(dtype, device):
+    p = _parameter((64, 32), dtype, device)
+    opt, start = Muon([p], lr=0.01, weight_decay=0.1), p.detach().float().clone()
+    for _ in range(100):
+        p.grad = torch.zeros_like(p)
+        opt.step()
+    # 100 fp32 products are off by a rounding each, the weight by that of its type
+    half_ulp = {F32: 0.0, BF16: 2.0**-8, torch.float16: 2.0**-11}[dtype]
+    torch.testing.assert_close(p.detach().float(), start * 0.999**100, rtol=half_ulp + 202 * 2.0**-24, atol=2.0**-25)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_weights_that_others_have_changed(device):
+    """A weight that is set between two steps (loaded, clipped, tied) is the one that the next step starts from; the others go on with all their digits."""
+    p = _parameter((32, 32), BF16, device)
+    opt = Muon([p], lr=1e-3)
+    grads = _gradients(p, 12)
+    for grad in grads[:6]:
+        p.grad = grad
+        opt.step()
+    q = torch.nn.Parameter(opt.state[p]['weight'].clone())
+    with torch.no_grad():
+        p[3], q[3] = 0.0, 0.0
+        p[5, 7] = q[5, 7] = float('inf')
+    other = Muon([q], lr=1e-3)
+    other.load_state_dict({'state': {0: {'momentum': opt.state[p]['momentum']}}, 'param_groups': other.state_dict()['param_groups']})
+    for grad in grads[6:]:
+        p.grad, q.grad = grad, grad.float()
+        opt.step()
+        other.step()
+        assert torch.equal(p, q.bfloat16())
