@@ -50,7 +50,7 @@ class Muon(torch.optim.Optimizer):
                 loss = closure()
         for group in self.param_groups:
             for p in group['params']:
-                if p.grad is None:
+                if p.grad is None or p.numel() == 0:
                     continue
                 state = self.state[p]
                 if 'momentum' not in state:

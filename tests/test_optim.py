@@ -111,3 +111,15 @@ def test_weights_that_others_have_changed(device):
         opt.step()
         other.step()
         assert torch.equal(p, q.bfloat16())
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('shape', [(0, 8, 4), (4, 0), (0, 4), (2, 3, 0), (2, 2, 0, 5)])
+def test_parameters_without_elements(shape, device):
+    """A rank that holds no expert, or a layer of no width, has nothing to update."""
+    p, full = _parameter(shape, F32, device), _parameter((8, 8), F32, device)
+    opt = Muon([p, full], weight_decay=0.1)
+    before = full.detach().clone()
+    p.grad, full.grad = torch.zeros_like(p), torch.ones_like(full)
+    opt.step()
+    assert p.shape == shape and not torch.equal(full, before)
