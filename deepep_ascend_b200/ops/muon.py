@@ -3,6 +3,7 @@ it is added to the weights, here for whole stacks such as the experts' ``w13`` a
 
 No counterpart in the reference, which has no optimiser.
 """
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -21,7 +22,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Tuple[float, fl
     Matrices may be stored by rows or by columns, with any distance between rows; other strides are copied first.  The products have fp16 operands and
     32-bit sums, and carry 22 bits of X and 32 bits of the diagonals from step to step, so that the result is off by little more than its rounding to
     bf16 (where large matrices of half as many columns again as rows, or more, take two steps at once: by up to 1.6 times that, if their singular values
-    fall off evenly over several orders).  The workspace (about 6 bytes per element and 2 to 6 per element of A, rows of whole 128 bytes) comes from PyTorch's allocator.
+    fall off evenly over several orders).  The workspace comes from PyTorch's allocator: about 6 bytes per element and 2 to 6 per element of A, with rows of
+    whole 128 bytes, and for few rows the parts of A that are summed along the columns, at most 64 KB per SM.
     ``num_sms``: SMs to run on (0: all).
     ``buffer``: see :func:`ops.gemm.gemm_nt`."""
     if x.dim() < 2:
@@ -29,7 +31,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Tuple[float, fl
     if not x.is_cuda:
         res = orthogonalize_ref(x, steps, coefficients, eps)
         return res if out is None else out.copy_(res)
-    m = x if x.dim() == 3 else x.reshape(-1, x.shape[-2], x.shape[-1])
+    m = x if x.dim() == 3 else x.reshape(math.prod(x.shape[:-2]), x.shape[-2], x.shape[-1])
     if 1 not in m.stride()[1:] and 1 not in m.shape[1:]:
         m = m.contiguous()
     res = _native.load().orthogonalize(m, steps, *coefficients, eps, None if out is None else out.view(m.shape), num_sms, _core_of(buffer))

@@ -229,3 +229,13 @@ def test_refusals_of_the_statement():
         orthogonalize(torch.randn(4))
     with pytest.raises(ValueError):
         orthogonalize_ref(torch.randn(4, 4), steps=0)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('shape', [(0, 5), (5, 0), (0, 0), (0, 4, 5), (2, 0, 5), (2, 3, 0, 5), (2, 3, 5, 0), (2, 0, 4, 5)])
+def test_no_elements_in_any_number_of_axes(shape, device):
+    x = torch.empty(shape, device=device)
+    got = orthogonalize(x)
+    assert got.shape == shape and got.dtype == BF16
+    out = torch.empty(shape, dtype=BF16, device=device)
+    assert orthogonalize(x, out=out) is out
