@@ -548,6 +548,7 @@ struct NsArgs {
     void* out;                        // bf16 [count, rows, cols] contiguous, or with out_transposed [count, cols, rows]
     int out_transposed;
     int count, rows, cols;
+    int steps;
     float a, b, c, eps;
     NsReport report;
     // set by the launcher
@@ -568,6 +569,8 @@ struct NsWorkspace {
 };
 
 namespace ep {
-NsWorkspace newton_schulz_workspace(const NsArgs& args, int num_sms);      // (sizes alone are read)
-cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8_t* workspace, int steps, int num_sms, cudaStream_t stream);
+// Whether all that the steps write in 16 bits stays in their range, whatever the matrix (steps and coefficients alone are read)
+bool newton_schulz_fits(const NsArgs& args);
+NsWorkspace newton_schulz_workspace(const NsArgs& args, int num_sms);      // (sizes, steps and coefficients alone are read)
+cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8_t* workspace, int num_sms, cudaStream_t stream);
 }  // namespace ep

@@ -1054,19 +1054,57 @@ cudaError_t launch_first(const NsArgs& g, cudaStream_t stream) {
                             stream);
 }
 
+// The largest singular value that X can have before any of `steps` steps: 1 before the first one (its squares add up to 1), then the largest
+// |s (a + b s^2 + c s^4)| of s from 0 to it, a thousandth more for what rounding adds.  (The larger it is, the larger is the next one: they rise, or fall from the first on.)
+double largest_singular_value(const NsArgs& g, int steps) {
+    const double a = g.a, b = g.b, c = g.c;
+    double top = 1.001;
+    for (int i = 1; i < steps; ++i) {
+        double next = 0.0;
+        auto look = [&](double y) {                    // at s^2 = y
+            if (y >= 0.0 && y <= top * top) next = std::max(next, std::sqrt(y) * std::abs(a + (b + c * y) * y));
+        };
+        look(top * top);
+        // where the derivative 5 c y^2 + 3 b y + a is zero
+        if (c == 0.0) {
+            if (b != 0.0) look(-a / (3.0 * b));
+        } else if (const double d = 9.0 * b * b - 20.0 * a * c; d >= 0.0) {
+            look((-3.0 * b + std::sqrt(d)) / (10.0 * c));
+            look((-3.0 * b - std::sqrt(d)) / (10.0 * c));
+        }
+        if (next >= 1e3) return 1e3;
+        if (1.001 * next <= top) break;
+        top = 1.001 * next;
+    }
+    return top;
+}
+
 // Steps in pairs: for matrices of half as many columns again as rows, if that saves more products than the two additional kernels of five steps cost, and the matrices have rows
 // enough for the rounding of a pair to stay below that of the result.  In us, single steps and pairs: 1024 x 1536 139 and 162, 1024 x 2048 147 and 167, four of them 238 and
 // 234, eight 437 and 400, 16 of 512 x 2048 396 and 357, 1024 x 7168 245 and 227, 2048 x 7168 550 and 460; four of 2048 x 2560 (a quarter more) 851 and 845 or 927 and 975.
 // Coefficients under which Q could grow past what fp16 holds of a product of two (64 beside the diagonal) stay with single steps.
 bool in_pairs(const NsArgs& g) {
+    const double s = largest_singular_value(g, g.steps);
+    const float top = static_cast<float>(std::max(1.5, s * s));              // eigenvalues of A, and of Q1 A Q1, are 0 to this
     auto small = [&](float x) { return std::abs(g.a + (g.b + g.c * x) * x) <= 4.f; };
-    const float vertex = g.c == 0.f ? 0.f : std::min(std::max(-g.b / (2.f * g.c), 0.f), 1.5f);
-    if (!small(0.f) || !small(1.5f) || !small(vertex)) return false;       // (X's singular values stay below 1.22 with the coefficients in use)
+    const float vertex = g.c == 0.f ? 0.f : std::min(std::max(-g.b / (2.f * g.c), 0.f), top);
+    if (!small(0.f) || !small(top) || !small(vertex) || !(top <= 14.f)) return false;       // (T = Q1 A: 4 x 14)
     const int64_t saved = 3ll * (g.cols - g.rows) * g.rows * g.rows * g.count;       // multiply-adds per pair
     return g.rows >= 512 && 2ll * g.cols >= 3ll * g.rows && saved >= 12'000'000'000;
 }
 
 }  // namespace
+
+// What fp16 holds: 65504 / kUnitX of X's entries, which its largest singular value s bounds, and 65504 / kUnitA beside the diagonals of A and B, which half the range of their
+// eigenvalues bounds: [0, s^2], and b y + c y^2 for y from 0 to s^2.
+bool newton_schulz_fits(const NsArgs& g) {
+    if (!std::isfinite(g.a) || !std::isfinite(g.b) || !std::isfinite(g.c)) return false;
+    const double s = largest_singular_value(g, g.steps), y = s * s, limit = 60000.0;
+    auto b_of = [&](double v) { return (g.b + static_cast<double>(g.c) * v) * v; };
+    const double vertex = g.c == 0.f ? 0.0 : std::min(std::max(-g.b / (2.0 * g.c), 0.0), y);
+    const double low = std::min({0.0, b_of(vertex), b_of(y)}), high = std::max({0.0, b_of(vertex), b_of(y)});
+    return s * kUnitX <= limit && 0.5 * y * kUnitA <= limit && 0.5 * (high - low) * kUnitA <= limit;
+}
 
 // Workspace: hi of X twice and lo once, three symmetric matrices (two without pairs, one for short matrices) and their diagonals, sums of squares, parts of X X^T.
 NsWorkspace newton_schulz_workspace(const NsArgs& g, int num_sms) {
@@ -1091,8 +1129,9 @@ NsWorkspace newton_schulz_workspace(const NsArgs& g, int num_sms) {
     return w;
 }
 
-cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8_t* workspace, int steps, int num_sms, cudaStream_t stream) {
-    if (args.count < 1 || args.rows < 1 || args.rows > args.cols || steps < 1 || reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return cudaErrorInvalidValue;
+cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8_t* workspace, int num_sms, cudaStream_t stream) {
+    const int steps = args.steps;
+    if (args.count < 1 || args.rows < 1 || args.rows > args.cols || steps < 1 || !newton_schulz_fits(args) || reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return cudaErrorInvalidValue;
     NsArgs g = args;
     g.ld_x = static_cast<int>(w.ld_x);
     g.ld_sq = static_cast<int>(w.ld_sq);

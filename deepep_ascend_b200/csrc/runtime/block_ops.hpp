@@ -199,9 +199,11 @@ inline at::Tensor orthogonalize(const at::Tensor& x, int64_t steps, double a, do
     g.count = static_cast<int>(count);
     g.rows = static_cast<int>(std::min(R, C));
     g.cols = static_cast<int>(std::max(R, C));
+    g.steps = static_cast<int>(std::min<int64_t>(steps, 1 << 30));
     g.a = static_cast<float>(a);
     g.b = static_cast<float>(b);
     g.c = static_cast<float>(c);
+    TORCH_CHECK(ep::newton_schulz_fits(g), "singular values may grow beyond what the 16-bit operands of the products hold with these coefficients and steps");
     g.eps = static_cast<float>(eps);
     g.report.error = error.data_ptr<int>();
     if (report_to != nullptr) {
@@ -214,7 +216,7 @@ inline at::Tensor orthogonalize(const at::Tensor& x, int64_t steps, double a, do
     const int sms = num_sms > 0 ? static_cast<int>(std::min<int64_t>(num_sms, device_sms())) : device_sms();
     const NsWorkspace w = ep::newton_schulz_workspace(g, sms);
     at::Tensor workspace = at::empty({w.bytes}, x.options().dtype(at::kByte));
-    cuda_check(ep::launch_newton_schulz(g, w, workspace.data_ptr<uint8_t>(), static_cast<int>(steps), sms, at::cuda::getCurrentCUDAStream()), "orthogonalisation launch");
+    cuda_check(ep::launch_newton_schulz(g, w, workspace.data_ptr<uint8_t>(), sms, at::cuda::getCurrentCUDAStream()), "orthogonalisation launch");
     return res;
 }
 

@@ -24,6 +24,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Tuple[float, fl
     bf16 (where large matrices of half as many columns again as rows, or more, take two steps at once: by up to 1.6 times that, if their singular values
     fall off evenly over several orders).  The workspace comes from PyTorch's allocator: about 6 bytes per element and 2 to 6 per element of A, with rows of
     whole 128 bytes, and for few rows the parts of A that are summed along the columns, at most 64 KB per SM.
+    Refused (on a GPU) are coefficients under which singular values between 0 and 1 may come to more than some 10 before the last step (A reaches the
+    range of fp16); those that are made to move them towards one stay far below.
     ``num_sms``: SMs to run on (0: all).
     ``buffer``: see :func:`ops.gemm.gemm_nt`."""
     if x.dim() < 2:

@@ -239,3 +239,32 @@ def test_no_elements_in_any_number_of_axes(shape, device):
     assert got.shape == shape and got.dtype == BF16
     out = torch.empty(shape, dtype=BF16, device=device)
     assert orthogonalize(x, out=out) is out
+
+
+@pytest.mark.gpu
+def test_coefficients_that_leave_the_range_of_the_operands():
+    """A matrix whose norm is all in one element, or in one pair of equal rows, takes the largest singular values that steps can make.  They are right
+    up to where a step's A or B would leave fp16, and refused beyond.  (Right: the result's rounding is 2e-3, that of the operands 5e-4 per step, which a
+    step that grows with the cube of what it is given triples.)"""
+    one, pair = torch.zeros(1, 80, 96), torch.zeros(1, 80, 96)
+    one[0, 3, 5], pair[0, 2:4, 7] = 2.0, 1.0
+    for steps, coefficients in ((3, (3.0, 0.0, 0.0)), (5, (1.7, 0.0, 0.0)), (2, (2.0, 3.0, 0.0))):
+        for x in (one, pair):
+            assert _error(orthogonalize(x.cuda(), steps, coefficients), _exact(x, steps, coefficients)) < 6e-3
+    for steps, coefficients in ((2, (6.0, -9.0, 4.0)), (1, (8.2872, -23.5959, 17.3004)), (3, (4.0848, -6.8946, 2.9270)), (8, COEFFICIENTS)):
+        assert _error(orthogonalize(one.cuda(), steps, coefficients), _exact(one, steps, coefficients)) < 6e-3
+    for steps, coefficients in ((4, (3.0, 0.0, 0.0)), (5, (4.0, 0.0, 0.0)), (3, (2.0, 3.0, 0.0)), (2, (1.0, 40.0, 40.0)), (3, (8.2872, -23.5959, 17.3004)),
+                                (2, (float('nan'), 0.0, 0.0)), (2, (1.0, 0.0, float('inf'))), (1, (1.0, 0.0, float('nan')))):
+        with pytest.raises(RuntimeError, match='singular values'):
+            orthogonalize(one.cuda(), steps, coefficients)
+
+
+@pytest.mark.gpu
+def test_pairs_only_where_singular_values_stay_small():
+    """Coefficients under which they grow step by step, for matrices that would be taken in pairs.  Bound as above."""
+    x = torch.zeros(5, 1000, 2016)
+    x[:, 3:5, 5] = 2.0
+    x[1] += _matrix('normal', 1, 1000, 2016)[0]
+    for steps, coefficients in ((5, (1.7, 0.0, 0.0)), (3, (2.0, 0.05, 0.0))):
+        want = _exact(x.cuda(), steps, coefficients)
+        assert _error(orthogonalize(x.cuda(), steps, coefficients), want) < 6e-3
