@@ -3,12 +3,12 @@
 //
 //     X = G / (|G|_F + eps);     per step:  A = X X^T,  B = b A + c A A,  X = a X + B X
 //
-// Steps may go in pairs, without the X between them. With Q = a I + B the next A is Q A Q, so that a pair is
+// The first two steps may go as a pair, without the X between them. With Q = a I + B the next A is Q A Q, so that a pair is
 //
 //     A = X X^T,  Q1 = a I + b A + c A A,  T = Q1 A,  A = T Q1,  Q2 = a I + b A + c A A,  Q = Q2 Q1,  X = Q X
 //
 // where all but the first and the last are symmetric products of rows^3, computed by half: in multiply-adds 3 cols/rows + 5 halves of 2 rows^3 for
-// a pair, 6 cols/rows + 2 for two single steps.
+// the pair, 6 cols/rows + 2 for two single steps.
 //
 // The products run on the tensor cores (tcgen05, fp16 operands, 32-bit sums in tensor memory), one persistent kernel each.  A and
 // B are symmetric: only tiles on and above the diagonal are computed, the others are written as their mirror images.
@@ -19,10 +19,12 @@
 // 1.3e-3 / 7e-3 / 6e-2, nearly all of it from rounding the X of a X and the diagonals of A and B, which are far larger than what is around them.
 // So X is carried in two halves, hi + lo 2^-11 (22 bits; the products read hi alone), and the diagonals are carried in 32 bits beside matrices
 // whose diagonal is zero:  A = O + diag(d),  A A = O O + (d_i + d_j) O + diag(d^2),  B X = (B - diag) X + diag X.  Then 5e-4 / 2e-4 / 4e-4, less than
-// the rounding of the result to bf16 (1.7e-3).  In a pair the second A comes from the first, not from X, and what its small eigenvalues are off by
-// has been multiplied by a^2; the next pair starts from X again.  For matrices of 512 and more rows that gives 7e-4 / 4e-4 / 3e-4, and 2.1e-3 (single
-// steps: 7e-4) for singular values that fall off evenly by 10^3 or 10^6.  At 64 rows it would be 1.9e-3 / 1.5e-3 / 1e-3, and three steps at once 2e-3 with a
-// single strong direction, five no number at all: so only pairs, and only from 512 rows.
+// the rounding of the result to bf16 (1.7e-3).  Singular
+// values on two levels far apart take the most: 1.9e-3 for 512 rows (a fifth of them at one, the others at a thousandth), 2.9e-3 for 256, 3.9e-3, 5e-3, 8e-3 and 2e-2 for 128, 64, 32 and 16,
+// where fewer roundings average out.  In a pair the second A comes from the first, not from X, and what its small eigenvalues are off by
+// has been multiplied by a^2.  The steps after a first pair, each from its own X, make that good: the same errors as single steps for 47 spectra at 512
+// and 1024 rows.  A second pair would not: 6.8e-3, four times the rounding of the result, for a tenth of 512 singular values at one and the others at 0.1, where single steps give 6e-4.  At
+// 64 rows a pair is off by 1.9e-3 for normal numbers; three steps at once are off by 2e-3 with a single strong direction, five are no number at all: so a pair, and only from 512 rows.
 #include <cuda_fp16.h>
 
 #include <algorithm>
@@ -1079,18 +1081,18 @@ double largest_singular_value(const NsArgs& g, int steps) {
     return top;
 }
 
-// Steps in pairs: for matrices of half as many columns again as rows, if that saves more products than the two additional kernels of five steps cost, and the matrices have rows
-// enough for the rounding of a pair to stay below that of the result.  In us, single steps and pairs: 1024 x 1536 139 and 162, 1024 x 2048 147 and 167, four of them 238 and
-// 234, eight 437 and 400, 16 of 512 x 2048 396 and 357, 1024 x 7168 245 and 227, 2048 x 7168 550 and 460; four of 2048 x 2560 (a quarter more) 851 and 845 or 927 and 975.
+// The first two steps as a pair: for matrices of half as many columns again as rows, if that saves more products than its additional kernel costs, and the matrices have rows
+// enough for the rounding of a pair to stay below that of the result.  In us, five single steps and with a pair: 1024 x 1536 138 and 149, 1024 x 2048 147 and 157, four of them 238 and
+// 236, eight 438 and 417, 16 of 512 x 2048 427 and 376, 1024 x 7168 250 and 238, 2048 x 7168 535 and 484, four of them 1910 and 1715; four of 2048 x 2560 (a quarter more) 855 and 850.
 // Coefficients under which Q could grow past what fp16 holds of a product of two (64 beside the diagonal) stay with single steps.
-bool in_pairs(const NsArgs& g) {
-    const double s = largest_singular_value(g, g.steps);
+bool first_pair(const NsArgs& g) {
+    const double s = largest_singular_value(g, 2);
     const float top = static_cast<float>(std::max(1.5, s * s));              // eigenvalues of A, and of Q1 A Q1, are 0 to this
     auto small = [&](float x) { return std::abs(g.a + (g.b + g.c * x) * x) <= 4.f; };
     const float vertex = g.c == 0.f ? 0.f : std::min(std::max(-g.b / (2.f * g.c), 0.f), top);
     if (!small(0.f) || !small(top) || !small(vertex) || !(top <= 14.f)) return false;       // (T = Q1 A: 4 x 14)
-    const int64_t saved = 3ll * (g.cols - g.rows) * g.rows * g.rows * g.count;       // multiply-adds per pair
-    return g.rows >= 512 && 2ll * g.cols >= 3ll * g.rows && saved >= 12'000'000'000;
+    const int64_t saved = 3ll * (g.cols - g.rows) * g.rows * g.rows * g.count;       // multiply-adds
+    return g.steps >= 2 && g.rows >= 512 && 2ll * g.cols >= 3ll * g.rows && saved >= 12'000'000'000;
 }
 
 }  // namespace
@@ -1106,7 +1108,7 @@ bool newton_schulz_fits(const NsArgs& g) {
     return s * kUnitX <= limit && 0.5 * y * kUnitA <= limit && 0.5 * (high - low) * kUnitA <= limit;
 }
 
-// Workspace: hi of X twice and lo once, three symmetric matrices (two without pairs, one for short matrices) and their diagonals, sums of squares, parts of X X^T.
+// Workspace: hi of X twice and lo once, three symmetric matrices (two without a pair, one for short matrices) and their diagonals, sums of squares, parts of X X^T.
 NsWorkspace newton_schulz_workspace(const NsArgs& g, int num_sms) {
     NsWorkspace w{};
     w.ld_x = round64(g.cols);
@@ -1121,7 +1123,7 @@ NsWorkspace newton_schulz_workspace(const NsArgs& g, int num_sms) {
     w.norms = take(g.count * w.norm_parts * 8);
     for (int64_t& x : w.x) x = take(g.count * g.rows * w.ld_x * 2);
     w.lo = take(g.count * g.rows * w.ld_x * 2);
-    for (int i = 0; i < (in_pairs(g) ? 3 : in_one_kernel(g, num_sms) ? 1 : 2); ++i) {
+    for (int i = 0; i < (first_pair(g) ? 3 : in_one_kernel(g, num_sms) ? 1 : 2); ++i) {
         w.sq[i] = take(g.count * g.rows * w.ld_sq * 2);
         w.diag[i] = take(g.count * w.ld_sq * 4);
     }
@@ -1141,7 +1143,7 @@ cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8
     g.parts = reinterpret_cast<float*>(workspace + w.parts);
     g.k_splits = w.k_splits;
     g.out = nullptr;
-    const bool pairs = in_pairs(g), one_kernel = in_one_kernel(g, num_sms);
+    const bool pair_first = first_pair(g), one_kernel = in_one_kernel(g, num_sms);
     const int n_gram = g.k_splits > 1 ? 128 : block_n_of(g, kGram, num_sms), n_square = block_n_of(g, kPoly, num_sms), n_update = block_n_of(g, kUpdate, num_sms);
     // X in turn; symmetric matrices: their rows as the first and as the second operand
     struct Wide {
@@ -1159,7 +1161,7 @@ cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8
         x[i].cols = x[i].rows;
         if (n_gram != kTileM && !make_map(&x[i].cols, x[i].x, g.count, g.rows, g.cols, g.ld_x, n_gram)) return cudaErrorInvalidValue;
     }
-    for (int i = 0; i < (pairs ? 3 : one_kernel ? 1 : 2); ++i) {
+    for (int i = 0; i < (pair_first ? 3 : one_kernel ? 1 : 2); ++i) {
         sq[i].m = reinterpret_cast<__half*>(workspace + w.sq[i]);
         sq[i].diag = reinterpret_cast<float*>(workspace + w.diag[i]);
         if (!make_map(&sq[i].rows, sq[i].m, g.count, g.rows, g.rows, g.ld_sq, kTileM)) return cudaErrorInvalidValue;
@@ -1209,7 +1211,7 @@ cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8
     g.x_out = x[0].x;
     cudaError_t err = g.in_bf16 ? launch_first<__nv_bfloat16>(g, stream) : launch_first<float>(g, stream);
     for (int done = 0, from = 0; done < steps && err == cudaSuccess; from ^= 1) {
-        const bool pair = pairs && done + 2 <= steps;
+        const bool pair = pair_first && done == 0;
         done += pair ? 2 : 1;
         err = gram(x[from], sq[0]);
         if (err == cudaSuccess && !one_kernel) err = poly(sq[0], sq[1]);

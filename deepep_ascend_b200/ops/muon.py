@@ -20,9 +20,9 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Tuple[float, fl
     times ``X = a X + (b A + c A A) X`` with ``A = X X^T`` (of the smaller side) -> bf16, contiguous, in ``x``'s shape (``out``: its memory, which may be that of ``x``).
 
     Matrices may be stored by rows or by columns, with any distance between rows; other strides are copied first.  The products have fp16 operands and
-    32-bit sums, and carry 22 bits of X and 32 bits of the diagonals from step to step, so that the result is off by little more than its rounding to
-    bf16 (where large matrices of half as many columns again as rows, or more, take two steps at once: by up to 1.6 times that, if their singular values
-    fall off evenly over several orders).  The workspace comes from PyTorch's allocator: about 6 bytes per element and 2 to 6 per element of A, with rows of
+    32-bit sums, and carry 22 bits of X and 32 bits of the diagonals from step to step, so that the result is
+    mostly off by little more than its rounding to bf16 (1.7e-3 of its norm): 1.7e-3 to 2.3e-3.  Singular values on two levels far apart take the most: 2.7e-3 for 512 and
+    more rows, 3.5e-3 for 256, 4.5e-3, 6e-3, 9e-3 and 2e-2 for 128, 64, 32 and 16.  The workspace comes from PyTorch's allocator: about 6 bytes per element and 2 to 6 per element of A, with rows of
     whole 128 bytes, and for few rows the parts of A that are summed along the columns, at most 64 KB per SM.
     Refused (on a GPU) are coefficients under which singular values between 0 and 1 may come to more than some 10 before the last step (A reaches the
     range of fp16); those that are made to move them towards one stay far below.
