@@ -2,6 +2,8 @@
 // Parity: csrc/python_api.cpp:1-54, csrc/elastic/binding.hpp:9-44 of the reference.
 #include <torch/extension.h>
 
+#include <algorithm>
+
 #include "kernels/api.h"
 #include "runtime/block_ops.hpp"
 #include "runtime/coordinator.hpp"
@@ -966,6 +968,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           py::arg("group_top"), py::arg("renormalize"), py::arg("scale"), py::arg("token_mask"), py::arg("idx_is_64"));
     m.def("route_backward", &route_backward, py::arg("d_weights"), py::arg("logits"), py::arg("topk_idx"), py::arg("softmax"), py::arg("renormalize"),
           py::arg("scale"));
+    m.def("watched", [](const std::vector<at::Tensor>& tensors) {
+        return std::any_of(tensors.begin(), tensors.end(), [](const at::Tensor& t) { return watched({&t}); });
+    });
     m.def("layer_norm", &layer_norm, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("eps"));
     m.def("layer_norm_backward", &layer_norm_backward, py::arg("dy"), py::arg("x"), py::arg("weight"), py::arg("mean"), py::arg("rstd"), py::arg("with_bias"));
     m.def("orthogonalize", [](const at::Tensor& x, int64_t steps, double a, double b, double c, double eps, const std::optional<at::Tensor>& out, int64_t num_sms,

@@ -3,15 +3,39 @@
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <optional>
 #include <tuple>
+#include <vector>
 
 #include "../kernels/api.h"
 #include "elastic_buffer.hpp"
 
 namespace ep_host {
+
+// Whether something records, transforms or intercepts what is done with these tensors, or a tangent goes with one of them: a native call would be invisible to it (a tracer would
+// record the allocation of the results and not the launch that fills them).  Asked here since it takes a tenth of the time that the same questions take in Python.
+inline bool watched(std::initializer_list<const at::Tensor*> tensors) {
+    if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::stack_len() != 0 ||
+        c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode))
+        return true;
+    constexpr c10::DispatchKeySet kWrappers({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::Functionalize});
+    for (const at::Tensor* t : tensors)
+        if (t != nullptr && t->defined() && (t->key_set().has_any(kWrappers) || t->_fw_grad(0).defined())) return true;
+    return false;
+}
+// ... or a gradient is to be carried on through one of them
+inline bool not_for_a_kernel(std::initializer_list<const at::Tensor*> tensors) {
+    if (at::GradMode::is_enabled())
+        for (const at::Tensor* t : tensors)
+            if (t != nullptr && t->requires_grad()) return true;
+    return watched(tensors);
+}
+inline const at::Tensor* given(const std::optional<at::Tensor>& t) { return t.has_value() ? &*t : nullptr; }
 
 inline int device_sms() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; }
 
@@ -119,7 +143,10 @@ inline void norm_rows(LayerNormArgs& a, const at::Tensor& x, const at::Tensor& w
     a.weight = weight.data_ptr();
 }
 
-inline std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias, double eps) {
+// nothing: for the PyTorch statement, or the function that carries gradients
+using NormResults = std::tuple<at::Tensor, at::Tensor, at::Tensor>;
+inline std::optional<NormResults> layer_norm(const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias, double eps) {
+    if (not_for_a_kernel({&x, &weight, given(bias)})) return std::nullopt;
     LayerNormArgs a{};
     norm_rows(a, x, weight);
     if (bias.has_value()) {
@@ -136,11 +163,13 @@ inline std::tuple<at::Tensor, at::Tensor, at::Tensor> layer_norm(const at::Tenso
     a.mean = mean.data_ptr<float>();
     a.rstd = rstd.data_ptr<float>();
     cuda_check(ep::launch_layer_norm(a, device_sms(), at::cuda::getCurrentCUDAStream()), "layer norm launch");
-    return {y, mean, rstd};
+    return NormResults(y, mean, rstd);
 }
 
-inline std::tuple<at::Tensor, at::Tensor, std::optional<at::Tensor>> layer_norm_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& weight,
-                                                                                         const at::Tensor& mean, const at::Tensor& rstd, bool with_bias) {
+using NormGradients = std::tuple<at::Tensor, at::Tensor, std::optional<at::Tensor>>;
+inline std::optional<NormGradients> layer_norm_backward(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& weight, const at::Tensor& mean, const at::Tensor& rstd,
+                                                        bool with_bias) {
+    if (not_for_a_kernel({&dy, &x, &weight, &mean, &rstd})) return std::nullopt;
     LayerNormArgs a{};
     norm_rows(a, x, weight);
     TORCH_CHECK(dy.device() == x.device() && dy.scalar_type() == x.scalar_type() && dy.sizes() == x.sizes() && (dy.size(1) == 1 || dy.stride(1) == 1),
@@ -167,7 +196,7 @@ inline std::tuple<at::Tensor, at::Tensor, std::optional<at::Tensor>> layer_norm_
     a.dw = dw.data_ptr();
     a.partial = partial.data_ptr<float>();
     cuda_check(ep::launch_layer_norm_backward(a, shape, at::cuda::getCurrentCUDAStream()), "layer norm gradient launch");
-    return {dx, dw, db};
+    return NormGradients(dx, dw, db);
 }
 
 // Stack of matrices [count, rows, cols], bf16 or fp32, rows or columns contiguous -> bf16 [count, rows, cols]

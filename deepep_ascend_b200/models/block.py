@@ -14,25 +14,17 @@ import torch.nn as nn
 
 from ..buffers.elastic import ElasticBuffer
 from ..ops import gemm as G
-from ..ops.norm import layer_norm, layer_norm_backward
+from ..ops.norm import layer_norm
 from ..ops.router import route, route_backward
 from .moe import FusedMoE
 
 
-class LayerNormFunction(torch.autograd.Function):
-    """:func:`ops.norm.layer_norm` with its gradients: ``apply(x, weight, bias or None, eps) -> y``."""
+class LayerNormFunction:
+    """``apply(x, weight, bias or None, eps) -> y``: the first result of :func:`ops.norm.layer_norm`, which carries gradients itself."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = layer_norm(x, weight, bias, eps)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        ctx.with_bias = bias is not None
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        return (*layer_norm_backward(dy, x, weight, mean, rstd, with_bias=ctx.with_bias), None)
+    def apply(x, weight, bias, eps):
+        return layer_norm(x, weight, bias, eps)[0]
 
 
 class GateFunction(torch.autograd.Function):

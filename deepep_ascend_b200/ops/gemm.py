@@ -9,6 +9,7 @@ import torch
 
 from .. import _native
 
+_is_compiling, _has_torch_function = torch.compiler.is_compiling, torch.overrides.has_torch_function_variadic
 BLOCK_M = 128   # rows of one output tile; expert segments of the grouped GEMM are aligned to it
 
 
@@ -53,6 +54,17 @@ def _plain(t: torch.Tensor) -> bool:
 def _plain_cuda(t: torch.Tensor) -> bool:
     """:func:`_plain`, on the current GPU."""
     return t.is_cuda and t.device.index == torch.cuda.current_device() and _plain(t)
+
+
+def _by_type(*tensors: Optional[torch.Tensor]) -> bool:
+    """No subclass is among the tensors and nothing is being compiled: the part of :func:`_plain` that native calls cannot ask for themselves."""
+    return not _is_compiling() and (not _has_torch_function(*tensors) or all(t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors))
+
+
+def _gradient_alone(*tensors: Optional[torch.Tensor]) -> bool:
+    """Of tensors that a native call has left to the caller: a gradient is to be carried on, and nobody watches beside it."""
+    tensors = [t for t in tensors if t is not None]
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors) and not _native.load().watched(tensors)
 
 
 def quantize_weight_blocks(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
