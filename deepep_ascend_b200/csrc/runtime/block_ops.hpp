@@ -62,9 +62,11 @@ inline void router_logits(RouterArgs& a, const at::Tensor& logits) {
     a.num_experts = static_cast<int>(logits.size(1));
 }
 
-inline std::tuple<at::Tensor, at::Tensor, at::Tensor> route(const at::Tensor& logits, int64_t num_topk, bool softmax, const std::optional<at::Tensor>& bias,
-                                                            int64_t num_groups, int64_t num_topk_groups, int64_t group_top, bool renormalize, double scale,
-                                                            const std::optional<at::Tensor>& token_mask, bool idx_is_64) {
+// (nothing where a kernel is not to run, as of the norm below)
+using Routes = std::tuple<at::Tensor, at::Tensor, at::Tensor>;
+inline std::optional<Routes> route(const at::Tensor& logits, int64_t num_topk, bool softmax, const std::optional<at::Tensor>& bias, int64_t num_groups, int64_t num_topk_groups,
+                                   int64_t group_top, bool renormalize, double scale, const std::optional<at::Tensor>& token_mask, bool idx_is_64) {
+    if (not_for_a_kernel({&logits}) || watched({given(bias), given(token_mask)})) return std::nullopt;      // (the bias, which the choice alone sees, has no gradient)
     RouterArgs a{};
     router_logits(a, logits);
     TORCH_CHECK(num_groups >= 1 && num_groups <= 32 && a.num_experts % num_groups == 0, "the experts must divide into 1 to 32 groups");
@@ -101,10 +103,11 @@ inline std::tuple<at::Tensor, at::Tensor, at::Tensor> route(const at::Tensor& lo
     a.topk_weights = weights.data_ptr<float>();
     a.count = count.data_ptr<int32_t>();
     cuda_check(ep::launch_route(a, device_sms(), at::cuda::getCurrentCUDAStream()), "routing launch");
-    return {idx, weights, count};
+    return Routes(idx, weights, count);
 }
 
-inline at::Tensor route_backward(const at::Tensor& d_weights, const at::Tensor& logits, const at::Tensor& topk_idx, bool softmax, bool renormalize, double scale) {
+inline std::optional<at::Tensor> route_backward(const at::Tensor& d_weights, const at::Tensor& logits, const at::Tensor& topk_idx, bool softmax, bool renormalize, double scale) {
+    if (not_for_a_kernel({&d_weights, &logits, &topk_idx})) return std::nullopt;
     RouterArgs a{};
     router_logits(a, logits);
     TORCH_CHECK(topk_idx.device() == logits.device() && topk_idx.dim() == 2 && topk_idx.is_contiguous() && topk_idx.size(0) == a.num_tokens &&

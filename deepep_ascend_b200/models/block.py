@@ -15,7 +15,7 @@ import torch.nn as nn
 from ..buffers.elastic import ElasticBuffer
 from ..ops import gemm as G
 from ..ops.norm import layer_norm
-from ..ops.router import route, route_backward
+from ..ops.router import RouteFunction
 from .moe import FusedMoE
 
 
@@ -48,24 +48,6 @@ class GateFunction(torch.autograd.Function):
                 h, d_logits = (torch.nn.functional.pad(t, (0, 0, 0, rows - T)) for t in (h, d_logits))
             d_gate = G.gemm_kgrouped_tn(d_logits, h, torch.tensor([0, rows], dtype=torch.int32, device=h.device))[0]
         return d_h, d_gate
-
-
-class RouteFunction(torch.autograd.Function):
-    """:func:`ops.router.route` with the gradient of its weights: ``apply(logits, options) -> (topk_idx, topk_weights, count)``, ``options``
-    a dict of ``route``'s other arguments."""
-
-    @staticmethod
-    def forward(ctx, logits, options):
-        idx, weights, count = route(logits, **options)
-        ctx.save_for_backward(logits, idx)
-        ctx.options = {k: options[k] for k in ('score', 'renormalize', 'scale') if k in options}
-        ctx.mark_non_differentiable(idx, count)
-        return idx, weights, count
-
-    @staticmethod
-    def backward(ctx, _idx, d_weights, _count):
-        logits, idx = ctx.saved_tensors
-        return route_backward(d_weights.contiguous(), logits, idx, **ctx.options), None
 
 
 class MoEBlock(nn.Module):

@@ -10,6 +10,7 @@ import torch
 
 from .. import _native
 from ..buffers.elastic import topk_idx_t
+from .gemm import _by_type, _gradient_alone
 
 _SCORES = ('sigmoid', 'softmax')
 
@@ -26,25 +27,55 @@ def route(logits: torch.Tensor, num_topk: int, score: str = 'sigmoid', bias: Opt
     token's experts with ``renormalize``.  ``count[e]``: tokens that chose expert ``e``.
 
     Nobody chooses an expert whose logit is -inf, whose bias is -inf or whose choice is NaN; tokens with ``token_mask[t] == False`` choose none.
-    Places without an expert hold index -1 and weight 0, which is what ``dispatch`` takes for "no selection"."""
+    Places without an expert hold index -1 and weight 0, which is what ``dispatch`` takes for "no selection".
+
+    The weights carry a gradient to the logits, by the kernel of :func:`route_backward`.  Tracers, function transforms, dispatch modes and forward mode
+    see the PyTorch statement."""
     if score not in _SCORES:
         raise ValueError('score must be one of %s, got %r' % (_SCORES, score))
     if not logits.is_cuda:
         return route_ref(logits, num_topk, score, bias, num_groups, num_topk_groups, group_top, renormalize, scale, token_mask)
-    return _native.load().route(logits, num_topk, score == 'softmax', bias, num_groups, num_topk_groups, group_top, renormalize, scale, token_mask,
-                                topk_idx_t == torch.int64)
+    if _by_type(logits, bias, token_mask):
+        res = _native.load().route(logits, num_topk, score == 'softmax', bias, num_groups, num_topk_groups, group_top, renormalize, scale, token_mask,
+                                   topk_idx_t == torch.int64)
+        if res is not None:
+            return res
+        if _gradient_alone(logits):
+            return RouteFunction.apply(logits, dict(num_topk=num_topk, score=score, bias=bias, num_groups=num_groups, num_topk_groups=num_topk_groups,
+                                                    group_top=group_top, renormalize=renormalize, scale=scale, token_mask=token_mask))
+    return route_ref(logits, num_topk, score, bias, num_groups, num_topk_groups, group_top, renormalize, scale, token_mask)
+
+
+class RouteFunction(torch.autograd.Function):
+    """:func:`route` with the gradient of its weights: ``apply(logits, options) -> (topk_idx, topk_weights, count)``, ``options`` a dict of
+    ``route``'s other arguments."""
+
+    @staticmethod
+    def forward(ctx, logits, options):
+        idx, weights, count = route(logits, **options)
+        ctx.save_for_backward(logits, idx)
+        ctx.options = {k: options[k] for k in ('score', 'renormalize', 'scale') if k in options}
+        ctx.mark_non_differentiable(idx, count)
+        return idx, weights, count
+
+    @staticmethod
+    def backward(ctx, _idx, d_weights, _count):
+        logits, idx = ctx.saved_tensors
+        return route_backward(d_weights.contiguous(), logits, idx, **ctx.options), None
 
 
 def route_backward(d_weights: torch.Tensor, logits: torch.Tensor, topk_idx: torch.Tensor, score: str = 'sigmoid', renormalize: bool = True,
                    scale: float = 1.0) -> torch.Tensor:
     """Gradient of ``topk_weights`` with respect to the logits, the choice held fixed: ``d_weights`` fp32 ``[T, K]``, the ``logits`` and
     ``topk_idx`` of :func:`route` -> ``[T, E]`` in the logits' type.  Only a softmax without ``renormalize`` gives experts that were not chosen a
-    gradient (and reads their logits); the others' is zero, as that of a token without experts."""
+    gradient (and reads their logits); the others' is zero, as that of a token without experts.  Where this gradient is to carry gradients itself, and for
+    whoever watches, the PyTorch statement runs."""
     if score not in _SCORES:
         raise ValueError('score must be one of %s, got %r' % (_SCORES, score))
     if not logits.is_cuda:
         return route_backward_ref(d_weights, logits, topk_idx, score, renormalize, scale)
-    return _native.load().route_backward(d_weights, logits, topk_idx, score == 'softmax', renormalize, scale)
+    res = _native.load().route_backward(d_weights, logits, topk_idx, score == 'softmax', renormalize, scale) if _by_type(d_weights, logits, topk_idx) else None
+    return route_backward_ref(d_weights, logits, topk_idx, score, renormalize, scale) if res is None else res
 
 
 def _scores(logits: torch.Tensor, score: str) -> torch.Tensor:
@@ -54,10 +85,12 @@ def _scores(logits: torch.Tensor, score: str) -> torch.Tensor:
     if score == 'sigmoid':
         return 1.0 / (1.0 + torch.exp(-x))
     e = torch.exp(x - x.max(dim=-1, keepdim=True).values)
-    total = torch.nn.functional.pad(e, (0, (1 << (e.shape[-1] - 1).bit_length()) - e.shape[-1]))
-    while total.shape[-1] > 1:
-        h = total.shape[-1] // 2
-        total = total[..., :h] + total[..., h:]
+    experts = int(e.shape[-1])                                      # (a number while tracing, too)
+    width = 1 << (experts - 1).bit_length()
+    total = torch.nn.functional.pad(e, (0, width - experts))
+    while width > 1:
+        width //= 2
+        total = total[..., :width] + total[..., width:]
     return e / total
 
 
@@ -88,7 +121,7 @@ def route_ref(logits, num_topk, score='sigmoid', bias=None, num_groups=1, num_to
         # (a place that nobody fills adds nothing; a group without an eligible expert comes last)
         total = torch.where(best[..., 0] == none, none, torch.where(best == none, 0.0, best).sum(-1))
         order = torch.sort(total, dim=-1, descending=True, stable=True).indices[:, :num_topk_groups]
-        keep = torch.zeros_like(total, dtype=torch.bool).scatter_(1, order, True)
+        keep = torch.zeros_like(total).scatter(1, order, 1.0) > 0
         choice = torch.where(keep.unsqueeze(-1), groups, none).view(T, E)
     value, idx = torch.sort(choice, dim=-1, descending=True, stable=True)
     live = value[:, :num_topk] > none
@@ -99,7 +132,7 @@ def route_ref(logits, num_topk, score='sigmoid', bias=None, num_groups=1, num_to
     if renormalize:
         total = w.sum(-1, keepdim=True)
         w = torch.where(total > 0, w / total, 0.0)
-    count = torch.bincount((idx + 1).flatten(), minlength=E + 1)[1:].to(torch.int32)
+    count = torch.zeros(E + 1, dtype=torch.int32, device=idx.device).scatter_add(0, (idx + 1).flatten(), torch.ones_like(idx, dtype=torch.int32).flatten())[1:]
     return idx.to(topk_idx_t), w * scale, count
 
 
@@ -114,7 +147,7 @@ def route_backward_ref(d_weights, logits, topk_idx, score='sigmoid', renormalize
     d = torch.where(live, d * w, 0.0)                               # softmax: d loss / d logit through the chosen scores
     if score == 'sigmoid':
         d = d * (1.0 - _scores(logits, score).gather(1, at))
-    out = torch.zeros(logits.shape[0], logits.shape[1] + 1, dtype=d.dtype, device=d.device).scatter_(1, torch.where(live, at, logits.shape[1]), d)[:, :-1]
+    out = torch.zeros(logits.shape[0], logits.shape[1] + 1, dtype=d.dtype, device=d.device).scatter(1, torch.where(live, at, logits.shape[1]), d)[:, :-1]
     if score == 'softmax' and not renormalize:
         out = torch.where(live.any(-1, keepdim=True), out - _scores(logits, score) * d.sum(-1, keepdim=True), 0.0)
     return out.to(logits.dtype)

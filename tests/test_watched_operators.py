@@ -3,10 +3,11 @@ import pytest
 import torch
 
 from deepep_ascend_b200 import _native
-from deepep_ascend_b200.ops import gemm, norm
+from deepep_ascend_b200.ops import gemm, norm, router
 
 from test_plain_tensor_guard import _watchers
 
+DEVICES = ['cpu', pytest.param('cuda', marks=pytest.mark.gpu)]
 EPS = 2.0**-24
 
 
@@ -91,11 +92,11 @@ def test_a_gradient_of_the_norms_gradient():
         torch.testing.assert_close(p.double(), q, rtol=1e-4, atol=1e-4 * q.abs().max().item())
 
 
-@pytest.mark.gpu
+@pytest.mark.parametrize('device', DEVICES)
 @pytest.mark.parametrize('tracer', ['jit.trace', 'make_fx', 'functionalize', 'vmap', 'forward mode', 'dispatch mode'])
-def test_the_norm_is_seen(tracer):
+def test_the_norm_is_seen(tracer, device):
     """A recorded norm gives the result for rows that it has not seen, and a transformed one that of its statement."""
-    x, w, b = _norm_inputs('cuda', torch.float32)
+    x, w, b = _norm_inputs(device, torch.float32)
     stats = norm.layer_norm(x, w, b)[1:]
     dy = torch.randn_like(x)
     for f in (lambda x: norm.layer_norm(x, w, b)[0], lambda x: norm.layer_norm_backward(dy, x, w, *stats, with_bias=True)[0]):
@@ -114,3 +115,57 @@ def test_a_tangent_through_the_norm():
     got = torch.func.jvp(lambda x: norm.layer_norm(x, w, b)[0], (x,), (t,))[1]
     want = torch.func.jvp(lambda x: norm.layer_norm_ref(x, w.double(), b.double())[0], (x.double(),), (t.double(),))[1]
     torch.testing.assert_close(got.double(), want, rtol=1e-4, atol=1e-4)
+
+
+ROUTES = [dict(), dict(score='softmax', renormalize=False), dict(score='softmax', scale=2.5), dict(renormalize=False, num_groups=4, num_topk_groups=2)]
+
+
+@pytest.mark.parametrize('options', ROUTES)
+def test_the_routing_function_against_differences(options):
+    logits = torch.randn(4, 16, generator=torch.Generator().manual_seed(0), dtype=torch.float64).requires_grad_(True)
+    f = lambda l: router.RouteFunction.apply(l, dict(options, num_topk=3))[1]      # noqa: E731
+    assert torch.autograd.gradcheck(f, (logits,)) and torch.autograd.gradgradcheck(f, (logits,))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize('options', ROUTES)
+def test_routing_carries_gradients(options, dtype):
+    g = torch.Generator().manual_seed(1)
+    logits = torch.randn(50, 32, generator=g).to(dtype).cuda().requires_grad_(True)
+    bias = torch.randn(32, generator=g).mul(0.1).cuda().requires_grad_(True)
+    mask = (torch.arange(50) % 7 != 2).cuda()
+    idx, w, count = router.route(logits, 4, bias=bias, token_mask=mask, **options)
+    assert 'RouteFunction' in type(w.grad_fn).__name__ and not idx.requires_grad and not count.requires_grad
+    d = torch.randn_like(w)
+    got, none = torch.autograd.grad(w, (logits, bias), d, allow_unused=True)
+    assert none is None                                        # the bias counts for the choice alone
+    keep = {k: options[k] for k in ('score', 'renormalize', 'scale') if k in options}
+    with torch.no_grad():
+        assert torch.equal(got, router.route_backward(d, logits, idx, **keep))
+        again = router.route(logits, 4, bias=bias, token_mask=mask, **options)
+    assert all(torch.equal(p, q) for p, q in zip((idx, w, count), again))
+    # the gradient of a gradient, against the statement's: a few dozen roundings of 32 bits
+    if dtype == torch.float32:
+        def second(l, f):
+            first, = torch.autograd.grad((f(l, 4, bias=bias.detach().to(l.dtype), **options)[1]**3).sum(), l, create_graph=True)
+            return torch.autograd.grad((first**2).sum(), l)[0]
+        want = second(logits.detach().double().requires_grad_(True), router.route_ref)
+        torch.testing.assert_close(second(logits, router.route).double(), want, rtol=1e-4, atol=1e-4 * want.abs().max().item())
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('tracer', ['jit.trace', 'make_fx', 'functionalize', 'vmap', 'forward mode', 'dispatch mode'])
+def test_routing_is_seen(tracer, device):
+    logits = torch.randn(20, 32, device=device)
+    idx = router.route(logits, 4)[0]
+    d = torch.randn(20, 4, device=device)
+    for f in (lambda l: router.route(l, 4, num_groups=4, num_topk_groups=2)[1], lambda l: router.route(l, 4)[0] * 1, lambda l: router.route(l, 4)[2] * 1,
+              lambda l: router.route_backward(d, l, idx), lambda l: router.route_backward(d, l, idx, 'softmax', False)):
+        out = _watchers()[tracer](f, logits)
+        want = f(logits)
+        if callable(out):
+            assert all(torch.allclose(out(v), f(v), rtol=1e-5, atol=1e-5) for v in (logits, torch.randn_like(logits) * 2))
+        else:
+            out = torch.autograd.forward_ad.unpack_dual(out)[0] if tracer == 'forward mode' else out
+            assert torch.allclose(out.reshape(want.shape), want, rtol=1e-5, atol=1e-5)
