@@ -974,7 +974,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("layer_norm", &layer_norm, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("eps"));
     m.def("layer_norm_backward", &layer_norm_backward, py::arg("dy"), py::arg("x"), py::arg("weight"), py::arg("mean"), py::arg("rstd"), py::arg("with_bias"));
     m.def("orthogonalize", [](const at::Tensor& x, int64_t steps, double a, double b, double c, double eps, const std::optional<at::Tensor>& out, int64_t num_sms,
-                              ElasticBufferCore* report_to) {
+                              ElasticBufferCore* report_to) -> std::optional<at::Tensor> {
+        if (not_for_a_kernel({&x, given(out)})) return std::nullopt;
         TORCH_CHECK(x.is_cuda(), "matrices must be on a GPU");
         return orthogonalize(x, steps, a, b, c, eps, out, num_sms, gemm_error_flag(x.get_device()), report_to);
     }, py::arg("x"), py::arg("steps"), py::arg("a"), py::arg("b"), py::arg("c"), py::arg("eps"), py::arg("out") = py::none(), py::arg("num_sms") = 0,

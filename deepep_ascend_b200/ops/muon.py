@@ -9,7 +9,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native
-from .gemm import _core_of
+from .gemm import _by_type, _core_of
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 
@@ -26,18 +26,21 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients: Tuple[float, fl
     whole 128 bytes, and for few rows the parts of A that are summed along the columns, at most 64 KB per SM.
     Refused (on a GPU) are coefficients under which singular values between 0 and 1 may come to more than some 10 before the last step (A reaches the
     range of fp16); those that are made to move them towards one stay far below.
+    Tensors that carry a gradient, tracers, function transforms, dispatch modes and forward mode get the PyTorch statement.
     ``num_sms``: SMs to run on (0: all).
     ``buffer``: see :func:`ops.gemm.gemm_nt`."""
     if x.dim() < 2:
         raise ValueError('matrices are needed, got shape %s' % (tuple(x.shape),))
-    if not x.is_cuda:
-        res = orthogonalize_ref(x, steps, coefficients, eps)
-        return res if out is None else out.copy_(res)
-    m = x if x.dim() == 3 else x.reshape(math.prod(x.shape[:-2]), x.shape[-2], x.shape[-1])
-    if 1 not in m.stride()[1:] and 1 not in m.shape[1:]:
-        m = m.contiguous()
-    res = _native.load().orthogonalize(m, steps, *coefficients, eps, None if out is None else out.view(m.shape), num_sms, _core_of(buffer))
-    return res.view(x.shape) if out is None else out
+    res = None
+    if x.is_cuda and _by_type(x, out):
+        m = x if x.dim() == 3 else x.reshape(math.prod(x.shape[:-2]), x.shape[-2], x.shape[-1])
+        if 1 not in m.stride()[1:] and 1 not in m.shape[1:]:
+            m = m.contiguous()
+        res = _native.load().orthogonalize(m, steps, *coefficients, eps, None if out is None else out.view(m.shape), num_sms, _core_of(buffer))
+    if res is not None:
+        return res.view(x.shape) if out is None else out
+    res = orthogonalize_ref(x, steps, coefficients, eps)
+    return res if out is None else out.copy_(res)
 
 
 def orthogonalize_ref(x: torch.Tensor, steps: int = 5, coefficients: Tuple[float, float, float] = COEFFICIENTS, eps: float = 1e-7) -> torch.Tensor:

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from deepep_ascend_b200 import _native
-from deepep_ascend_b200.ops import gemm, norm, router
+from deepep_ascend_b200.ops import gemm, muon, norm, router
 
 from test_plain_tensor_guard import _watchers
 
@@ -169,3 +169,32 @@ def test_routing_is_seen(tracer, device):
         else:
             out = torch.autograd.forward_ad.unpack_dual(out)[0] if tracer == 'forward mode' else out
             assert torch.allclose(out.reshape(want.shape), want, rtol=1e-5, atol=1e-5)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('tracer', ['jit.trace', 'make_fx', 'functionalize', 'vmap', 'forward mode', 'dispatch mode', 'fake tensors'])
+def test_an_update_is_seen(tracer, device):
+    """Against the statement: bf16 results whose last places differ (the kernel's errors are stated where it is tested)."""
+    x = torch.randn(2, 24, 40, device=device)
+    out = _watchers()[tracer](lambda x: muon.orthogonalize(x) * 1, x)
+    if tracer == 'fake tensors':
+        assert type(out).__name__ == 'FakeTensor' and out.shape == x.shape and out.dtype == torch.bfloat16
+    elif callable(out):
+        for v in (x, torch.randn_like(x) * 3):
+            assert torch.allclose(out(v), muon.orthogonalize(v), rtol=2e-2, atol=5e-3)
+    else:
+        out = torch.autograd.forward_ad.unpack_dual(out)[0] if tracer == 'forward mode' else out
+        assert torch.allclose(out.reshape(x.shape), muon.orthogonalize(x), rtol=2e-2, atol=5e-3)
+
+
+@pytest.mark.parametrize('device', DEVICES)
+def test_an_update_carries_gradients(device):
+    x = torch.randn(3, 8, 5, generator=torch.Generator().manual_seed(0)).to(device).requires_grad_(True)
+    d = torch.randn(3, 8, 5, generator=torch.Generator().manual_seed(1)).to(device)
+    got, = torch.autograd.grad((muon.orthogonalize(x, steps=2).float() * d).sum(), x)
+    y = x.detach().double().requires_grad_(True)
+    want, = torch.autograd.grad((muon.orthogonalize_ref(y, steps=2) * d.double()).sum(), y)
+    # (what comes back through the rounding to bf16 is rounded to it)
+    assert (got.double() - want).norm() < 2.0**-7 * want.norm()
+    with torch.no_grad():
+        assert not muon.orthogonalize(x).requires_grad
