@@ -79,9 +79,11 @@ class MoEBlock(nn.Module):
 
     @torch.no_grad()
     def update_balance(self, speed: float = 1e-3, group=None) -> None:
-        """Moves every expert's bias by ``speed`` towards the mean load of the last forward pass (of all ranks of ``group``)."""
+        """Moves every expert's bias by ``speed`` towards the mean load of the last forward pass, of all ranks of ``group`` (the buffer's, if none is given), which
+        call this together and come to the same bias."""
         count = self.last_count.float()
-        if group is not None:
+        group = self.experts.buffer.group if group is None else group
+        if group is not None and torch.distributed.get_world_size(group) > 1:
             torch.distributed.all_reduce(count, group=group)
         self.balance_bias += speed * torch.sign(count.mean() - count)
 
