@@ -54,15 +54,18 @@ class MoEBlock(nn.Module):
     """``forward(x bf16 [T, hidden], token_mask bool [T] = None) -> x + FusedMoE(norm(x), route(gate(norm(x))))``.
 
     ``num_experts``: of all ranks, a multiple of 8; the experts of this rank are ``self.experts.w13`` and ``w2``, the gate is replicated.
+    ``score``, ``num_groups``, ``num_topk_groups``, ``group_top``, ``renormalize`` and ``scale`` are those of :func:`ops.router.route`.
     ``balance_bias`` (fp32 ``[num_experts]``, no parameter) is added to the scores for the choice of experts; :meth:`update_balance` moves it after
     a step so that crowded experts are chosen less.  ``self.last_count``: tokens of this rank that chose each expert in the last forward pass."""
 
     def __init__(self, buffer: ElasticBuffer, num_experts: int, hidden: int, intermediate: int, num_topk: int, score: str = 'sigmoid', num_groups: int = 1,
-                 num_topk_groups: int = 1, scale: float = 1.0, eps: float = 1e-5, norm_bias: bool = False, init_std: float = 0.02, device='cuda', **moe):
+                 num_topk_groups: int = 1, scale: float = 1.0, eps: float = 1e-5, norm_bias: bool = False, init_std: float = 0.02, device='cuda',
+                 renormalize: bool = True, group_top: int = 2, **moe):
         super().__init__()
         if num_experts % 8 or hidden % 8:
             raise ValueError('num_experts and hidden must be multiples of 8')
-        self.options = dict(num_topk=num_topk, score=score, num_groups=num_groups, num_topk_groups=num_topk_groups, scale=scale, renormalize=True)
+        self.options = dict(num_topk=num_topk, score=score, num_groups=num_groups, num_topk_groups=num_topk_groups, scale=scale, renormalize=renormalize,
+                            group_top=group_top)
         self.eps = eps
         self.norm_weight = nn.Parameter(torch.ones(hidden, device=device))
         self.norm_bias = nn.Parameter(torch.zeros(hidden, device=device)) if norm_bias else None
