@@ -28,12 +28,14 @@ class LayerNormFunction:
 
 
 class GateFunction(torch.autograd.Function):
-    """``apply(h bf16 [T, H], gate bf16 [E, H]) -> logits bf16 [T, E]`` on the tensor cores; ``H`` and ``E`` multiples of 8."""
+    """``apply(h bf16 [T, H], gate bf16 [E, H], buffer=None) -> logits bf16 [T, E]`` on the tensor cores; ``H`` and ``E`` multiples of 8.  ``buffer``: see
+    :func:`ops.gemm.gemm_nt`."""
 
     @staticmethod
-    def forward(ctx, h, gate):
+    def forward(ctx, h, gate, buffer=None):
         ctx.save_for_backward(h, gate)
-        return G.gemm_nt(h, gate)
+        ctx.buffer = buffer
+        return G.gemm_nt(h, gate, buffer=buffer)
 
     @staticmethod
     def backward(ctx, d_logits):
@@ -41,13 +43,13 @@ class GateFunction(torch.autograd.Function):
         T, d_logits = h.shape[0], d_logits.contiguous()
         d_h = d_gate = None
         if ctx.needs_input_grad[0]:
-            d_h = G.grouped_gemm_nn(d_logits, gate.unsqueeze(0), torch.zeros((T + G.BLOCK_M - 1) // G.BLOCK_M, dtype=torch.int32, device=h.device))
+            d_h = G.grouped_gemm_nn(d_logits, gate.unsqueeze(0), torch.zeros((T + G.BLOCK_M - 1) // G.BLOCK_M, dtype=torch.int32, device=h.device), buffer=ctx.buffer)
         if ctx.needs_input_grad[1]:
             rows = (T + 63) // 64 * 64                      # the sum over tokens runs in whole blocks of 64
             if rows != T:
                 h, d_logits = (torch.nn.functional.pad(t, (0, 0, 0, rows - T)) for t in (h, d_logits))
             d_gate = G.gemm_kgrouped_tn(d_logits, h, torch.tensor([0, rows], dtype=torch.int32, device=h.device))[0]
-        return d_h, d_gate
+        return d_h, d_gate, None
 
 
 class MoEBlock(nn.Module):
@@ -76,7 +78,7 @@ class MoEBlock(nn.Module):
 
     def forward(self, x: torch.Tensor, token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         h = LayerNormFunction.apply(x, self.norm_weight, self.norm_bias, self.eps)
-        logits = GateFunction.apply(h, self.gate)
+        logits = GateFunction.apply(h, self.gate, self.experts.buffer)
         idx, weights, self.last_count = RouteFunction.apply(logits, dict(self.options, bias=self.balance_bias, token_mask=token_mask))
         return x + self.experts(h, idx, weights)
 

@@ -60,7 +60,8 @@ class _Experts(torch.nn.Module):
 
 def _stand_in(block, monkeypatch):
     monkeypatch.setattr(block_module.GateFunction, 'apply', staticmethod(lambda h, gate, *_: (h @ gate.float().t()).bfloat16()))
-    block.experts = _Experts()
+    buffer, block.experts = block.experts.buffer, _Experts()
+    block.experts.buffer = buffer
 
 
 @pytest.mark.parametrize('options', [dict(), dict(num_groups=4, num_topk_groups=2, scale=2.5),
@@ -96,3 +97,29 @@ def test_the_gradient_of_a_softmax_that_is_not_renormalised(monkeypatch):
         _stand_in(block, monkeypatch)
         block(torch.randn(1, 128, generator=torch.Generator().manual_seed(2))).square().sum().backward()
         assert int((block.gate.grad.abs().sum(1) > 0).sum()) == rows
+
+
+def _gate_on_cpu(monkeypatch):
+    """The gate's products in PyTorch; returns which buffers they were given."""
+    buffers = []
+    G = block_module.G
+
+    def nn(a, b, tile_group, out=None, num_sms=0, buffer=None):
+        buffers.append(buffer)
+        return a @ b[0]
+
+    def nt(a, b, out=None, num_sms=0, buffer=None):
+        buffers.append(buffer)
+        return a @ b.t()
+    monkeypatch.setattr(G, 'gemm_nt', nt)
+    monkeypatch.setattr(G, 'grouped_gemm_nn', nn)
+    monkeypatch.setattr(G, 'gemm_kgrouped_tn', lambda a, b, off: (a.t() @ b).unsqueeze(0))
+    return buffers
+
+
+def test_waits_of_the_gates_product_report_to_the_buffer(monkeypatch):
+    buffers, block = _gate_on_cpu(monkeypatch), _block()
+    block.experts = _Experts()
+    block.experts.buffer = buffer = SimpleNamespace(group=None)
+    block(torch.randn(10, 128).bfloat16().requires_grad_(True)).float().square().sum().backward()
+    assert block.gate.grad is not None and buffers == [buffer, buffer]
