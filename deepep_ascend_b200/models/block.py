@@ -100,7 +100,7 @@ def main(steps: int = 30) -> None:
     buffer = ElasticBuffer(None, num_max_tokens_per_rank=T, hidden=H, num_topk=K)
     try:
         block = MoEBlock(buffer, E, H, I, K, num_groups=4, num_topk_groups=2, scale=2.0)
-        matrices = Muon([block.gate, block.experts.w13, block.experts.w2], lr=0.05)
+        matrices = Muon([block.gate, block.experts.w13, block.experts.w2], lr=0.05, buffer=buffer)
         vectors = torch.optim.AdamW([block.norm_weight], lr=1e-3)
         x, target = torch.randn(T, H, device='cuda').bfloat16(), torch.randn(T, H, device='cuda')
         for step in range(steps):

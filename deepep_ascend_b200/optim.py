@@ -14,11 +14,14 @@ class Muon(torch.optim.Optimizer):
 
     Parameters are matrices or stacks of them (``[experts, rows, cols]``: every expert's matrix by itself).  The momentum is fp32, and so is a copy of
     16-bit parameters (``state[p]['weight']``, 4 bytes per element) that steps are added to, since most of an update is below the last place of a bf16 weight: ``p``
-    is that copy, rounded.  Where a weight has been set by others since, its value counts."""
+    is that copy, rounded.  Where a weight has been set by others since, its value counts.  ``buffer``: see :func:`ops.gemm.gemm_nt`."""
+
+    buffer = None
 
     def __init__(self, params, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.0, steps: int = 5,
-                 coefficients=COEFFICIENTS, eps: float = 1e-7):
+                 coefficients=COEFFICIENTS, eps: float = 1e-7, buffer=None):
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps, coefficients=coefficients, eps=eps))
+        self.buffer = buffer
         for group in self.param_groups:
             for p in group['params']:
                 if p.dim() < 2:
@@ -57,7 +60,8 @@ class Muon(torch.optim.Optimizer):
                     state['momentum'] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
                 m, grad = state['momentum'], p.grad.float()
                 m.mul_(group['momentum']).add_(grad)
-                update = orthogonalize(torch.add(grad, m, alpha=group['momentum']) if group['nesterov'] else m, group['steps'], group['coefficients'], group['eps'])
+                update = orthogonalize(torch.add(grad, m, alpha=group['momentum']) if group['nesterov'] else m, group['steps'], group['coefficients'], group['eps'],
+                                       buffer=self.buffer)
                 w = self._weight(p, state)
                 if group['weight_decay']:
                     w.mul_(1.0 - group['lr'] * group['weight_decay'])

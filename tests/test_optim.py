@@ -123,3 +123,17 @@ def test_parameters_without_elements(shape, device):
     p.grad, full.grad = torch.zeros_like(p), torch.ones_like(full)
     opt.step()
     assert p.shape == shape and not torch.equal(full, before)
+
+
+def test_waits_of_the_products_report_to_the_buffer(monkeypatch):
+    from deepep_ascend_b200 import optim
+    seen = []
+    monkeypatch.setattr(optim, 'orthogonalize', lambda x, *args, buffer=None: seen.append(buffer) or x.bfloat16())
+    buffer = object()
+    for given in (None, buffer):
+        p = _parameter((8, 8), F32, 'cpu')
+        opt = Muon([p], buffer=given)
+        p.grad = torch.ones_like(p)
+        opt.step()
+        opt.load_state_dict(copy.deepcopy(opt.state_dict()))         # (a buffer is no state)
+    assert seen == [None, buffer]
