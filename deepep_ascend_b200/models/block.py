@@ -11,6 +11,7 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from ..buffers.elastic import ElasticBuffer
 from ..ops import gemm as G
@@ -38,6 +39,7 @@ class GateFunction(torch.autograd.Function):
         return G.gemm_nt(h, gate, buffer=buffer)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_logits):
         h, gate = ctx.saved_tensors
         T, d_logits = h.shape[0], d_logits.contiguous()

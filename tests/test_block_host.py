@@ -123,3 +123,19 @@ def test_waits_of_the_gates_product_report_to_the_buffer(monkeypatch):
     block.experts.buffer = buffer = SimpleNamespace(group=None)
     block(torch.randn(10, 128).bfloat16().requires_grad_(True)).float().square().sum().backward()
     assert block.gate.grad is not None and buffers == [buffer, buffer]
+
+
+def test_a_gradient_of_the_gates_gradient_is_refused(monkeypatch):
+    """The products of its backward pass carry none: terms would be missing without a word."""
+    _gate_on_cpu(monkeypatch)
+    native = block_module.GateFunction
+    h, gate = torch.randn(6, 8).bfloat16().requires_grad_(True), torch.randn(8, 8).bfloat16().requires_grad_(True)
+    for name in ('grouped_gemm_nn', 'gemm_kgrouped_tn'):             # (native calls return results without a graph)
+        f = getattr(block_module.G, name)
+        monkeypatch.setattr(block_module.G, name, lambda *a, f=f, **k: f(*a, **k).detach())
+    logits = native.apply(h, gate)
+    d = torch.autograd.grad(logits.float().square().sum(), (h, gate), create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(sum(t.float().square().sum() for t in d), h)
+    with pytest.raises(RuntimeError, match='once_differentiable'):
+        ((d[0].float() * h.float()).sum() + (d[1].float() ** 2).sum()).backward()
