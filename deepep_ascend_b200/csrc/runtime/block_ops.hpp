@@ -182,11 +182,11 @@ inline std::optional<NormGradients> layer_norm_backward(const at::Tensor& dy, co
                     "mean and rstd must be contiguous fp32 [rows] on the device of x");
     const c10::cuda::CUDAGuard guard(x.device());
     at::Tensor dx = at::empty({x.size(0), x.size(1)}, x.options());
-    const int64_t width_bytes = round16(x.size(1) * weight.element_size());
-    at::Tensor sums = at::empty({width_bytes * (with_bias ? 2 : 1)}, x.options().dtype(at::kByte)), dw = part_of(sums, 0, {x.size(1)}, weight.scalar_type());
+    // (a storage each: they become the gradients of parameters, which are kept, saved and freed one by one)
+    at::Tensor dw = at::empty({x.size(1)}, weight.options());
     std::optional<at::Tensor> db;
     if (with_bias) {
-        db = part_of(sums, width_bytes, {x.size(1)}, weight.scalar_type());
+        db = at::empty({x.size(1)}, weight.options());
         a.db = db->data_ptr();
     }
     a.dy = dy.data_ptr();

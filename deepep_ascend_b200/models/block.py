@@ -81,7 +81,8 @@ class MoEBlock(nn.Module):
     def forward(self, x: torch.Tensor, token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         h = LayerNormFunction.apply(x, self.norm_weight, self.norm_bias, self.eps)
         logits = GateFunction.apply(h, self.gate, self.experts.buffer)
-        idx, weights, self.last_count = RouteFunction.apply(logits, dict(self.options, bias=self.balance_bias, token_mask=token_mask))
+        idx, weights, count = RouteFunction.apply(logits, dict(self.options, bias=self.balance_bias, token_mask=token_mask))
+        self.last_count = count.clone()                     # (the router's results share an allocation, which this would keep)
         return x + self.experts(h, idx, weights)
 
     @torch.no_grad()

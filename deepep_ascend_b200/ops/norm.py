@@ -19,7 +19,7 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
 def layer_norm(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(x - mean) * rstd * weight (+ bias)`` over the last axis of ``x [..., H]`` (bf16 or fp32, any strides) -> ``(y like x, mean, rstd)``,
-    the statistics fp32, one of each per row, in ``x``'s leading shape.  ``weight`` and ``bias`` ``[H]``: both bf16 or both fp32.
+    the statistics fp32, one of each per row, in ``x``'s leading shape (on a GPU they share an allocation).  ``weight`` and ``bias`` ``[H]``: both bf16 or both fp32.
 
     Carries gradients, by the kernel of :func:`layer_norm_backward`.  Tracers, function transforms, dispatch modes and forward mode see the PyTorch
     statement."""

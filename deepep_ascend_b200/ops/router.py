@@ -27,7 +27,8 @@ def route(logits: torch.Tensor, num_topk: int, score: str = 'sigmoid', bias: Opt
     token's experts with ``renormalize``.  ``count[e]``: tokens that chose expert ``e``.
 
     Nobody chooses an expert whose logit is -inf, whose bias is -inf or whose choice is NaN; tokens with ``token_mask[t] == False`` choose none.
-    Places without an expert hold index -1 and weight 0, which is what ``dispatch`` takes for "no selection".
+    Places without an expert hold index -1 and weight 0, which is what ``dispatch`` takes for "no selection".  (On a GPU the three results share an allocation: keep
+    a clone of one that outlives the others.)
 
     The weights carry a gradient to the logits, by the kernel of :func:`route_backward`.  Tracers, function transforms, dispatch modes and forward mode
     see the PyTorch statement."""

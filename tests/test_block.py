@@ -111,3 +111,37 @@ def test_refusals():
             MoEBlock(buf, 12, 256, 128, 2)
     finally:
         buf.destroy()
+
+
+@pytest.mark.gpu
+def test_what_is_kept_of_a_batch_is_its_counts():
+    """`last_count` outlives the batch; its ids and weights do not, and a forward pass gives the block's own choice."""
+    from deepep_ascend_b200 import ElasticBuffer
+    from deepep_ascend_b200.models.block import MoEBlock
+    from deepep_ascend_b200.ops import gemm
+    from deepep_ascend_b200.ops.norm import layer_norm
+    from deepep_ascend_b200.ops.router import route_ref
+    torch.manual_seed(0)
+    T, H, E, K = 300, 256, 16, 3
+    buf = ElasticBuffer(None, num_max_tokens_per_rank=T, hidden=H, num_topk=K)
+    try:
+        for options in (dict(num_groups=4, num_topk_groups=2, scale=2.0), dict(score='softmax', num_groups=8, num_topk_groups=3, group_top=1, renormalize=False)):
+            block = MoEBlock(buf, E, H, 128, K, norm_bias=True, **options)
+            block.balance_bias.copy_(0.3 * torch.randn(E, device='cuda'))
+            x, mask = torch.randn(T, H, device='cuda').bfloat16(), torch.arange(T, device='cuda') % 11 != 3
+            chosen = {}
+            hook = block.experts.register_forward_pre_hook(lambda m, args: chosen.update(idx=args[1], weights=args[2]))
+            block(x, mask).float().sum().backward()
+            hook.remove()
+            with torch.no_grad():
+                logits = gemm.gemm_nt(layer_norm(x, block.norm_weight, block.norm_bias, block.eps)[0], block.gate, buffer=buf)
+            idx, weights, count = route_ref(logits, K, bias=block.balance_bias, token_mask=mask, **options)
+            plain = route_ref(logits, K, **options)[0]
+            assert torch.equal(chosen['idx'], idx) and torch.equal(block.last_count, count) and not torch.equal(plain, idx)
+            # (a sum of three weights and a few operations in another order)
+            torch.testing.assert_close(chosen['weights'].detach(), weights, rtol=1e-5, atol=1e-6)
+            assert block.last_count.untyped_storage().nbytes() == 4 * E
+            assert block.norm_weight.grad.untyped_storage().data_ptr() != block.norm_bias.grad.untyped_storage().data_ptr()
+        buf.check_status()
+    finally:
+        buf.destroy()

@@ -191,3 +191,13 @@ def test_refusals():
             layer_norm_backward(*args)
     with pytest.raises(ValueError):
         layer_norm_backward(dy[:3], x, w, mean, rstd)
+
+
+@pytest.mark.gpu
+def test_gradients_of_the_parameters_have_a_storage_each():
+    """Whatever frees, saves or resizes the one leaves the other alone."""
+    x, w, b, dy = _make(5, 72, BF16, F32, 0, 'cuda')
+    _, mean, rstd = layer_norm(x, w, b)
+    _, dw, db = layer_norm_backward(dy, x, w, mean, rstd, with_bias=True)
+    for t in (dw, db):
+        assert t.untyped_storage().nbytes() == 72 * 4 and t.storage_offset() == 0
