@@ -12,6 +12,7 @@
 #include <type_traits>
 
 #include "common.cuh"
+#include "division.cuh"
 
 namespace ep {
 
@@ -32,23 +33,8 @@ __device__ __forceinline__ T logit_of(float v) {
 
 __device__ __forceinline__ float sigmoid(float l) { return __frcp_rn(1.f + expf(-l)); }
 
-// 1 / x, correctly rounded, for 1 <= x < 2^118: an estimate, and one step with its residual (P. W. Markstein, Computation of elementary functions on the
-// IBM RISC System/6000 processor, 1990).  The bits of __frcp_rn for every one of these numbers, without that one's look at all others, which lets the
-// eight of a lane overlap.
-__device__ __forceinline__ float reciprocal(float x) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return fmaf(r, fmaf(-x, r, 1.f), r);
-}
+// (where reciprocal and quotient of division.cuh may be taken for the general ones)
 constexpr float kLowLogit = -80.f;                               // 1 + exp(80) < 2^118
-
-// a / x, correctly rounded, of 2^-100 <= a <= 1 and 1 <= x <= 2^20 with x's correctly rounded reciprocal: a quotient that is off by less than its last place
-// and one step with its exact residual round as the quotient does (the same work's theorem on division)
-__device__ __forceinline__ float quotient(float a, float x, float inverse) {
-    float q = a * inverse;
-    q = fmaf(fmaf(-q, x, a), inverse, q);
-    return fmaf(fmaf(-q, x, a), inverse, q);
-}
 constexpr float kLowShare = 7.9e-31f;                            // over 2^-100
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -143,7 +129,7 @@ __device__ __forceinline__ float sum_by_halves(const F& leaf) {
 // of which it knows the largest choice; a chosen expert is found, taken out, and the new largest of its eight made by the token's eight lanes together, so that the
 // shuffles of a step serve four tokens.  Bound by instruction issue (1720 per warp and four tokens, 70 % of the issue slots; DRAM 18 %): about a third are the
 // exact exponentials and reciprocals, a quarter the steps of the choice.
-// 65536 x 256 fp32, 8 of 256 in 4 of 8 groups: 42 us, 1.8 TB/s (softmax 56); one token per warp, with a maximum over the warp for every expert, took 139, steps that
+// 65536 x 256 fp32, 8 of 256 in 4 of 8 groups: 42 us, 1.8 TB/s (softmax 55); one token per warp, with a maximum over the warp for every expert, took 139, steps that
 // branch 48.  Requesting the next tokens' logits into L2 ahead gained nothing (43).
 // CTAs per SM: as many as leave the registers (64, or 80 for more than 256 experts) for what a lane holds: 32768 x 512 with 64 took 81 us instead of 72.
 template <int kSegs, bool kBf16, bool kWide, bool kSoftmax>

@@ -297,3 +297,20 @@ def test_refusals_of_the_statements():
             router.route(l, **kw)
     with pytest.raises(ValueError):
         router.route_backward(torch.zeros(4, 2), l, torch.zeros(4, 2, dtype=torch.int64), 'relu')
+
+
+@pytest.mark.gpu
+def test_short_divisions_have_the_bits_of_the_general_ones(tmp_path):
+    """Every reciprocal of the range that the kernel takes it in, and six thousand million quotients."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+    nvcc = shutil.which('nvcc') or '/usr/local/cuda/bin/nvcc'
+    if not Path(nvcc).exists():
+        pytest.skip('no compiler')
+    root = Path(__file__).resolve().parents[1]
+    program = tmp_path / 'division'
+    subprocess.run([nvcc, '-gencode', 'arch=compute_100a,code=sm_100a', '-O3', '-std=c++17', '-I', root / 'deepep_ascend_b200' / 'csrc' / 'kernels',
+                    root / 'tests' / 'probes' / 'division.cu', '-o', program], check=True)
+    state, reciprocals, quotients, count = subprocess.run([program], check=True, capture_output=True, text=True).stdout.split()
+    assert (state, int(reciprocals), int(quotients)) == ('cudaSuccess', 0, 0) and int(count) > 6e9
