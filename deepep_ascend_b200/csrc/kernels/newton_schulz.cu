@@ -560,7 +560,7 @@ __device__ __forceinline__ void ns_quiet(const NsShared<kBlockN>& s) {
 
 // One product of one step: a persistent CTA per SM, a warp that requests operands, one that issues the products, eight that finish tiles while the next one's products run
 // (two accumulators).  Bound by the tensor cores and, in long runs, by power: 8 x 4096 x 7168 alone takes 707 us for X X^T, 413 for a product of squares (half of either
-// is computed) and 1490 for X, 1.3 to 1.4 PFLOP/s; all 19 products in a row 14.6 ms, 1.0 PFLOP/s.  4 x 2048 x 3584: tensor pipe 72 % busy for X X^T and X, 53 to 59 % for squares
+// is computed) and 1490 for X, 1.3 to 1.4 PFLOP/s; all 16 products of five steps, behind the norm and the cast, 15.1 ms, 1.06 PFLOP/s.  4 x 2048 x 3584: tensor pipe 72 % busy for X X^T and X, 53 to 59 % for squares
 // (tiles of 32 K blocks).  Below some 1000 rows the chain of launches is what counts: 3 x 777 x 1001 takes 154 us in 17 launches, 34 GFLOP; all steps in one launch whose
 // CTAs wait for one another took 237 (183 without), parts along K in a cluster's shared memory 145 for 256 x 7168 (121 without).
 template <int kMode, int kBlockN>

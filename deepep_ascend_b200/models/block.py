@@ -58,6 +58,7 @@ class MoEBlock(nn.Module):
     """``forward(x bf16 [T, hidden], token_mask bool [T] = None) -> x + FusedMoE(norm(x), route(gate(norm(x))))``.
 
     ``num_experts``: of all ranks, a multiple of 8; the experts of this rank are ``self.experts.w13`` and ``w2``, the gate is replicated.
+    The logits are bf16 (the gate's product is rounded once), the scores that are made of them 32-bit: experts whose logits round alike tie, and go by index.
     ``score``, ``num_groups``, ``num_topk_groups``, ``group_top``, ``renormalize`` and ``scale`` are those of :func:`ops.router.route`.
     ``balance_bias`` (fp32 ``[num_experts]``, no parameter) is added to the scores for the choice of experts; :meth:`update_balance` moves it after
     a step so that crowded experts are chosen less.  ``self.last_count``: tokens of this rank that chose each expert in the last forward pass."""
