@@ -34,8 +34,9 @@ class Muon(torch.optim.Optimizer):
         def restore(_):
             ids = (i for group in given['param_groups'] for i in group['params'])
             for p, i in zip((p for group in self.param_groups for p in group['params']), ids):
-                for name, value in given['state'].get(i, {}).items():
-                    self.state[p][name] = value.to(p.device, torch.float32, copy=True)
+                saved = given['state'].get(i, {})
+                for name in saved.keys() & {'momentum', 'weight'}:
+                    self.state[p][name] = saved[name].to(p.device, torch.float32, copy=True)
         # (behind the caller's hooks, which may give another dict, and ahead of those that look at what was loaded)
         hooks = (self.register_load_state_dict_pre_hook(lambda _, loaded: given.update(loaded)),
                  self.register_load_state_dict_post_hook(restore, prepend=True))

@@ -137,3 +137,16 @@ def test_waits_of_the_products_report_to_the_buffer(monkeypatch):
         opt.step()
         opt.load_state_dict(copy.deepcopy(opt.state_dict()))         # (a buffer is no state)
     assert seen == [None, buffer]
+
+
+def test_what_others_have_put_into_a_checkpoint():
+    """Entries that are not this optimiser's come through as the base class treats them: a count of steps is no tensor."""
+    p = _parameter((8, 8), BF16, 'cpu')
+    opt = Muon([p])
+    p.grad = torch.ones_like(p)
+    opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    saved['state'][0].update(step=3, seen=torch.arange(2))
+    opt.load_state_dict(saved)
+    assert opt.state[p]['step'] == 3 and opt.state[p]['momentum'].dtype == F32
+    assert torch.equal(opt.state[p]['seen'].float(), torch.arange(2).float())
