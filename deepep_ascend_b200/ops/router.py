@@ -140,7 +140,7 @@ def route_ref(logits, num_topk, score='sigmoid', bias=None, num_groups=1, num_to
 def route_backward_ref(d_weights, logits, topk_idx, score='sigmoid', renormalize=True, scale=1.0):
     """:func:`route_backward` stated with plain PyTorch operations."""
     live, at = topk_idx >= 0, topk_idx.clamp_min(0).to(torch.int64)
-    w, d = _gathered(logits, topk_idx, score, renormalize), d_weights * scale
+    w, d = _gathered(logits, topk_idx, score, renormalize), torch.where(live, d_weights, 0.0) * scale
     if renormalize:
         total = w.sum(-1, keepdim=True)
         w = torch.where(total > 0, w / total, 0.0)

@@ -314,3 +314,17 @@ def test_short_divisions_have_the_bits_of_the_general_ones(tmp_path):
                     root / 'tests' / 'probes' / 'division.cu', '-o', program], check=True)
     state, reciprocals, quotients, count = subprocess.run([program], check=True, capture_output=True, text=True).stdout.split()
     assert (state, int(reciprocals), int(quotients)) == ('cudaSuccess', 0, 0) and int(count) > 6e9
+
+
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('score,renormalize', [('sigmoid', True), ('sigmoid', False), ('softmax', True), ('softmax', False)])
+def test_gradients_of_empty_places_count_for_nothing(score, renormalize, device):
+    """Whatever stands there: no number, or none at all."""
+    g = torch.Generator().manual_seed(0)
+    logits, d = torch.randn(9, 24, generator=g).to(device), torch.randn(9, 4, generator=g).to(device)
+    idx = router.route_ref(logits, 4, score)[0]
+    idx[2, 1], idx[4, 3], idx[5, 0], idx[7] = -1, -1, -1, -1
+    want = router.route_backward(torch.where(idx >= 0, d, 0.0), logits, idx, score, renormalize)
+    for nothing in (math.nan, math.inf, -math.inf, 1e30):
+        assert torch.equal(router.route_backward(torch.where(idx >= 0, d, nothing), logits, idx, score, renormalize), want)
+    assert torch.isfinite(want).all()
