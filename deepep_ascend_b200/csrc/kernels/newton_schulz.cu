@@ -362,7 +362,7 @@ __device__ __forceinline__ bool ns_load(const NsArgs& g, const NsShared<kBlockN>
     }
     return true;
 }
-// gives what is still in flight time to land before the shared memory goes to another CTA
+// gives what is still in flight time to land
 template <int kBlockN>
 __device__ __forceinline__ void ns_drain(const NsShared<kBlockN>& s, NsRing<kBlockN> p, int loads) {
     for (; loads > 0; --loads) {
@@ -545,17 +545,22 @@ __device__ __forceinline__ uint32_t ns_setup(const NsShared<kBlockN>& s) {
     umma::fence_after_thread_sync();
     return s.sm->tmem_base;
 }
-template <int kBlockN>
-__device__ __forceinline__ void ns_teardown(uint32_t tmem_base) {
-    umma::fence_before_thread_sync();
+// Where a wait has run out (which nobody can come to any more), what is still under way ends before its memory goes to others: what was requested has landed, and products
+// have ended, those too that were issued before the wait ran out elsewhere.
+template <class Landed>
+__device__ __forceinline__ void ns_settle(NsSmem* sm, Landed landed) {
     __syncthreads();
-    if (threadIdx.x >> 5 == 1) umma::tmem_dealloc(tmem_base, ns_tmem_columns(kBlockN));
-}
-// products still under way end before the tensor memory is given back
-template <int kBlockN>
-__device__ __forceinline__ void ns_quiet(const NsShared<kBlockN>& s) {
-    umma::mma_commit(&s.sm->quiet);
-    mbar_drain(&s.sm->quiet, 0, 1000000000ull);
+    if (sm->failed == 0) return;
+    const int warp = threadIdx.x >> 5;
+    if (warp < 2 && ptx::elect_one()) {                // (the thread that requested, or issued)
+        if (warp == 0) {
+            landed();
+        } else {
+            umma::mma_commit(&sm->quiet);
+            mbar_drain(&sm->quiet, 0, 1000000000ull);
+        }
+    }
+    __syncthreads();
 }
 
 // One product of one step: a persistent CTA per SM, a warp that requests operands, one that issues the products, eight that finish tiles while the next one's products run
@@ -578,19 +583,20 @@ ns_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUt
     int acc = 0;
     uint32_t acc_phase = 0;
     NsRing<kBlockN> p;
+    int loads = 0;
     if (warp == 0) {
         if (ptx::elect_one()) {
-            int loads = 0;
-            const bool ok = ns_load<kMode, kBlockN>(g, s, &map_a, &map_b, p, loads);
+            ns_load<kMode, kBlockN>(g, s, &map_a, &map_b, p, loads);
             ptx::let_next_kernel_start();
-            if (!ok) ns_drain(s, p, loads);
         }
     } else if (warp == 1) {
-        if (ptx::elect_one() && !ns_multiply<kMode, kBlockN>(g, s, tmem_base, p, acc, acc_phase)) ns_quiet(s);
+        if (ptx::elect_one()) ns_multiply<kMode, kBlockN>(g, s, tmem_base, p, acc, acc_phase);
     } else {
         ns_finish<kMode, kBlockN>(g, s, tmem_base, acc, acc_phase);
     }
-    ns_teardown<kBlockN>(tmem_base);
+    umma::fence_before_thread_sync();
+    ns_settle(s.sm, [&] { ns_drain(s, p, loads); });
+    if (warp == 1) umma::tmem_dealloc(tmem_base, ns_tmem_columns(kBlockN));
 }
 
 // Short matrices: Q and X <- Q X in one kernel, a CTA per 128 x 128 tile of X, which makes the 128 rows of B that it needs itself and writes them over those of O, as the first
@@ -756,20 +762,17 @@ ns_step_kernel(const __grid_constant__ CUtensorMap map_o, const __grid_constant_
 #pragma unroll
                 for (int i = 0; i < 2; ++i) umma::tma_load_3d(s.x + kb * s.kBytesX + i * umma::kMnChunkBytes, &map_x, t.n * kTileM + i * 64, kb * kTileK, t.g, &s.sm->full[1]);
             ptx::let_next_kernel_start();
-            // whatever the others wait for: what was requested has landed before the shared memory goes to another CTA
-            mbar_drain(&s.sm->full[0], 0, 1000000000ull);
-            mbar_drain(&s.sm->full[1], 0, 1000000000ull);
         }
     } else if (warp == 1) {
-        if (ptx::elect_one() && !ns_step_multiply(g, s, tmem_base, t.m, num_k)) {
-            umma::mma_commit(&s.sm->quiet);
-            mbar_drain(&s.sm->quiet, 0, 1000000000ull);
-        }
+        if (ptx::elect_one()) ns_step_multiply(g, s, tmem_base, t.m, num_k);
     } else {
         ns_step_finish(g, s, tmem_base, t);
     }
     umma::fence_before_thread_sync();
-    __syncthreads();
+    ns_settle(s.sm, [&] {
+        mbar_drain(&s.sm->full[0], 0, 1000000000ull);
+        mbar_drain(&s.sm->full[1], 0, 1000000000ull);
+    });
     if (warp == 1) umma::tmem_dealloc(tmem_base, kColumns);
 }
 

@@ -305,3 +305,48 @@ def test_two_levels_in_few_rows(rows, cols, simulated):
             x = _two_levels(1, m, n, share, low)
             x = (x.mT if rows > cols else x).cuda()
             assert _error(orthogonalize(x), _exact(x)) < 1.5 * simulated + 2e-3
+
+
+_SHORT_LIMIT = """
+import torch
+from deepep_ascend_b200 import ElasticBuffer, _native
+from deepep_ascend_b200.ops.muon import orthogonalize
+torch.manual_seed(0)
+small = torch.randn(3, 300, 500, device='cuda')
+want = orthogonalize(small)
+buf = ElasticBuffer(None, num_max_tokens_per_rank=16, hidden=256, num_topk=2)
+x = torch.randn(128, 1000000, device='cuda', dtype=torch.bfloat16)
+buf.core.set_gpu_timeout(3e-4)
+orthogonalize(x, steps=1, num_sms=1, buffer=buf)
+torch.cuda.synchronize()
+code, phase, peer, expected, observed, rank = buf.core.read_status()
+assert (code, phase, expected, rank) == (1, 14, 5, 0), (code, phase, expected, rank)
+assert _native.load().gemm_error(0) == 5
+try:
+    buf.check_status()
+except RuntimeError as e:
+    assert 'timed out' in str(e)
+else:
+    raise AssertionError('the wait was not reported')
+try:
+    orthogonalize(small, buffer=buf)
+except RuntimeError:
+    pass
+else:
+    raise AssertionError('a buffer whose wait has failed was taken')
+# the memory of the products has been given back, and what follows is right
+for _ in range(3):
+    assert torch.equal(orthogonalize(small), want)
+print('reported')
+"""
+
+
+@pytest.mark.gpu
+def test_a_wait_that_runs_out_is_reported():
+    """One SM sums 15625 blocks of K, for milliseconds, while the warps that wait for the sum have 0.3 ms.  (In a process of its own: the device's error flag stays up.)"""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, '-c', _SHORT_LIMIT], cwd=root, env=dict(os.environ, PYTHONPATH=root), capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0 and run.stdout.strip().endswith('reported'), run.stderr[-2000:]
