@@ -574,3 +574,33 @@ bool newton_schulz_fits(const NsArgs& args);
 NsWorkspace newton_schulz_workspace(const NsArgs& args, int num_sms);      // (sizes, steps and coefficients alone are read)
 cudaError_t launch_newton_schulz(const NsArgs& args, const NsWorkspace& w, uint8_t* workspace, int num_sms, cudaStream_t stream);
 }  // namespace ep
+
+// ------------------------------------------------------------------------------------------------ attention
+// A tensor [tokens, heads, dim] whose channels are contiguous
+struct HeadsView {
+    const void* data;
+    int64_t stride_token, stride_head;      // elements
+};
+// Packed sequences (attention.cu states the formulas).  Sequence i has the queries cu_q[i] .. cu_q[i + 1] and the keys cu_k[i] .. cu_k[i + 1].
+struct AttentionArgs {
+    HeadsView q, k, v;                // bf16 [tq, heads, dim], [tk, kv_heads, dim]
+    int tq, tk, heads, kv_heads, dim; // dim: a multiple of 8, at most 128
+    const int32_t *cu_q, *cu_k;       // [num_seqs + 1], or null: one sequence of all tokens
+    int num_seqs;
+    int causal;                       // query i of n sees the keys up to its place, the last query the last key
+    float scale;
+    void* o;                          // bf16 [tq, heads, dim] contiguous
+    float* lse;                       // [heads, tq]
+    // gradients
+    HeadsView d_o;                    // bf16 [tq, heads, dim]
+    HeadsView o_in;
+    const float *lse_in, *d_lse;      // [heads, tq]; d_lse or null
+    float* delta;                     // [heads, tq] workspace
+    void *dq, *dk, *dv;               // bf16, contiguous
+    NsReport report;
+};
+
+namespace ep {
+cudaError_t launch_attention(const AttentionArgs& args, int num_sms, cudaStream_t stream);
+cudaError_t launch_attention_backward(const AttentionArgs& args, int num_sms, cudaStream_t stream);
+}  // namespace ep

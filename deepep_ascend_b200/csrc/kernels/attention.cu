@@ -1,0 +1,867 @@
+// Attention of packed sequences on the tensor cores, forward and backward.  Per sequence and query head, with the keys and values of its group,
+//
+//     S = scale Q K^T (only what a query sees),   P = softmax(S),   O = P V,   lse = log sum exp(S)
+//     delta = rowsum(dO O) - d_lse,   dP = dO V^T,   dS = P (dP - delta)
+//     dV = P^T dO,   dQ = scale dS K,   dK = scale dS^T Q        (dK, dV: over the heads of the group)
+//
+// Products are tcgen05 (bf16 operands, 32-bit sums in tensor memory).  The softmax is taken in one pass over the keys with a running reference and sum, all
+// in 32 bits; P and dS are rounded to bf16, as operands of the products that follow (an unbiased 2^-9 of each term, which in a sum of many is less than
+// the rounding of the result).
+//
+// A causal query sees the keys up to its own place, both sequences ending together: query i of nq the keys 0 .. nk - nq + i of nk.
+#include <algorithm>
+#include <atomic>
+
+#include "common.cuh"
+#include "gemm_sm100.cuh"
+
+namespace ep {
+
+namespace {
+
+constexpr uint64_t kAttnWaitLimitNs = 4ull * 1000 * 1000 * 1000;      // when the caller gives no limit
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+using bf16 = __nv_bfloat16;
+
+// ------------------------------------------------------------------------------------------------ waits
+struct AttnState {
+    uint32_t tmem_base;
+    int failed;
+};
+// Bounded wait for an mbarrier phase; when it runs out the device's flag is raised, and the status block of the caller's buffer written.
+__device__ __noinline__ void attn_fail(const NsReport& r, int* failed, int code) {
+    *failed = code;
+    if (atomicCAS(r.error, 0, code) == 0 && r.status != nullptr) {
+        volatile uint64_t* st = r.status;
+        st[EP_STATUS_PHASE] = EP_PH_GEMM_PIPE;
+        st[EP_STATUS_PEER] = static_cast<uint64_t>(-1ll);
+        st[EP_STATUS_EXPECTED] = static_cast<uint64_t>(code);
+        st[EP_STATUS_OBSERVED] = blockIdx.x;
+        st[EP_STATUS_RANK] = static_cast<uint64_t>(r.status_rank);
+        __threadfence_system();
+        st[EP_STATUS_CODE] = EP_ERR_TIMEOUT;
+        __threadfence_system();
+    }
+}
+// code: 1 free stage, 2 probabilities, 4 full stage, 5 scores, 6 sums
+__device__ __forceinline__ bool attn_wait(uint64_t* bar, uint32_t parity, int* failed, const NsReport& r, int code) {
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns(), limit = r.timeout_ns != 0 ? r.timeout_ns : kAttnWaitLimitNs;
+    uint32_t spins = 0;
+    while (!ptx::mbar_try_wait(bar, parity)) {
+        if ((++spins & 63u) == 0u) {
+            if (*reinterpret_cast<volatile int*>(failed)) return false;
+            if (globaltimer_ns() - t0 > limit) {
+                attn_fail(r, failed, code);
+                return false;
+            }
+        }
+    }
+    return true;
+}
+// ... of a whole warp
+__device__ __forceinline__ bool attn_wait_warp(uint64_t* bar, uint32_t parity, int* failed, const NsReport& r, int code) {
+    return __all_sync(0xffffffffu, attn_wait(bar, parity, failed, r, code)) != 0;
+}
+
+template <int kStages>
+struct AttnRing {
+    int stage = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void advance() {
+        if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+        }
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ work
+// Blocks of kRows rows of the sequences are numbered without a count of them: sequence i has the numbers from cu[i] / kRows + i on, up to one more than it needs.
+struct AttnBlock {
+    int seq, row0, rows;             // first row of the block inside its sequence, rows of the sequence (row0 >= rows: no block has this number)
+    int start;                       // first row of the sequence
+};
+__device__ __forceinline__ int2 sequence_rows(const int32_t* cu, int i, int total) {
+    if (cu == nullptr) return make_int2(0, total);
+    const int a = min(max(cu[i], 0), total), b = min(max(cu[i + 1], a), total);
+    return make_int2(a, b - a);
+}
+template <int kRows>
+__device__ __forceinline__ AttnBlock find_block(const int32_t* cu, int num_seqs, int total, int number) {
+    int lo = 0;
+    if (cu != nullptr) {
+        int hi = num_seqs;                                        // the last i in [lo, hi) with cu[i] / kRows + i <= number
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (min(max(cu[mid], 0), total) / kRows + mid <= number) lo = mid;
+            else hi = mid;
+        }
+    }
+    const int2 s = sequence_rows(cu, lo, total);
+    const int at = number - s.x / kRows - lo;                     // (below zero: in front of the first sequence)
+    return AttnBlock{lo, at < 0 ? s.y : at * kRows, s.y, s.x};
+}
+template <int kRows>
+int64_t num_blocks(int64_t total, int64_t num_seqs) { return total / kRows + num_seqs; }
+
+// The first kThreads threads: rows that belong to no sequence get zeros (and -inf), this CTA's part of them
+template <int kThreads>
+__device__ __forceinline__ void clear_rows(const int32_t* cu, int num_seqs, int total, bf16* out, int64_t row_values, float* lse, int heads) {
+    if (cu == nullptr) return;
+    const int first = min(max(cu[0], 0), total), last = min(max(cu[num_seqs], first), total);
+    const int missing = first + total - last;
+    for (int i = blockIdx.x; i < missing; i += gridDim.x) {
+        const int row = i < first ? i : last + i - first;
+        for (int64_t c = threadIdx.x; c < row_values / 8; c += kThreads) reinterpret_cast<uint4*>(out + row * row_values)[c] = make_uint4(0, 0, 0, 0);
+        if (lse != nullptr)
+            for (int h = threadIdx.x; h < heads; h += kThreads) lse[static_cast<int64_t>(h) * total + row] = __int_as_float(0xff800000);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ operands
+// A tile of rows x 64 kChunks channels lies in shared memory as chunks of 64 channels, rows of 128 bytes with the 128-byte swizzle, as TMA writes them.  It is
+// an operand along its channels (K-major) and along its rows (MN-major: every channel a row of the operand) alike.
+template <int kRows>
+__device__ __forceinline__ uint64_t desc_channels(const uint8_t* tile, int k) {      // k-th 16 channels
+    return umma::advance_desc_k(umma::make_smem_desc_sw128(tile + (k >> 2) * kRows * 128), (k & 3) * 32);
+}
+template <int kRows>
+__device__ __forceinline__ uint64_t desc_rows(const uint8_t* tile, int k) {          // k-th 16 rows
+    const uint64_t addr = ptx::smem_u32(tile) + k * 16 * 128;
+    return ((addr & 0x3ffffull) >> 4) | (static_cast<uint64_t>(kRows * 128 >> 4) << 16) | ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+template <int kRows, int kChunks>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, int head, int row, uint64_t* bar) {
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) umma::tma_load_3d(dst + c * kRows * 128, map, c * 64, head, row, bar);
+}
+// A warp: zeros in the rows from `valid` on, which belong to others and may hold anything: a probability of zero times an infinity is a NaN
+template <int kRows, int kChunks>
+__device__ __forceinline__ void clear_tile(uint8_t* tile, int valid) {
+    const int lane = threadIdx.x & 31, pieces = (kRows - valid) * 8;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+        for (int i = lane; i < pieces; i += 32) *reinterpret_cast<uint4*>(tile + c * kRows * 128 + valid * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+}
+
+// ------------------------------------------------------------------------------------------------ numbers
+__device__ __forceinline__ float exp2_approx(float x) {              // 2 ulp; 0 for -inf
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t v;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+    return v;
+}
+__device__ __forceinline__ uint64_t f32x2(float lo, float hi) { return umma::pack_f32x2(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+constexpr float kNone = -__builtin_huge_valf();
+
+// The two groups of four warps that hold rows take registers of the third: 384 x 168 at launch = 128 x (232 + 232 + 40)
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 232;"); }
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 40;"); }
+
+// A row of sums in tensor memory, times `factor`, as bf16
+template <int kColumns>
+__device__ __forceinline__ void store_row(uint32_t tmem, float factor, bf16* row, int dim, bool write) {
+#pragma unroll
+    for (int c = 0; c < kColumns; c += 32) {
+        uint32_t r[32];
+        umma::tmem_ld_32x32(tmem + c, r);
+        umma::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; i += 8)
+            if (write && c + i < dim) {
+                uint4 v;
+                v.x = pack_bf16(__uint_as_float(r[i]) * factor, __uint_as_float(r[i + 1]) * factor);
+                v.y = pack_bf16(__uint_as_float(r[i + 2]) * factor, __uint_as_float(r[i + 3]) * factor);
+                v.z = pack_bf16(__uint_as_float(r[i + 4]) * factor, __uint_as_float(r[i + 5]) * factor);
+                v.w = pack_bf16(__uint_as_float(r[i + 6]) * factor, __uint_as_float(r[i + 7]) * factor);
+                *reinterpret_cast<uint4*>(row + c + i) = v;
+            }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ forward
+// A CTA takes 256 queries of a head as two tiles of 128, whose softmaxes (four warps each, a row per thread) and products alternate: while one tile's scores are made into
+// probabilities, the tensor cores work for the other.  Probabilities take the place of the scores in tensor memory, from where they are the first operand of the next product.
+constexpr int kFwdThreads = 384;                     // 2 x 4 warps for the softmaxes, one that requests tiles, one that issues products, two without work
+template <int kChunks>
+struct FwdShape {
+    static constexpr int kTileBytes = 128 * 128 * kChunks, kStages = kChunks == 2 ? 5 : 8;
+    static constexpr int kOut = 256;                  // tensor memory: two tiles' scores, then two tiles' sums
+    static constexpr int kSmem = (2 + kStages) * kTileBytes + 1024;
+};
+struct FwdBars {
+    uint64_t q_full[2], full[8], empty[8], s_full[2], p_full[2], o_full[2], tail, quiet;
+    AttnState st;
+    int4 block;
+};
+
+template <int kChunks>
+__global__ void __launch_bounds__(kFwdThreads, 1)
+attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                 const __grid_constant__ AttentionArgs a) {
+    using Shape = FwdShape<kChunks>;
+    constexpr int kStages = Shape::kStages, kTileBytes = Shape::kTileBytes;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t *sq = smem, *skv = smem + 2 * kTileBytes;
+    FwdBars* b = reinterpret_cast<FwdBars*>(smem + (2 + kStages) * kTileBytes);
+    const int warp = threadIdx.x >> 5;
+    const int head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
+    if (threadIdx.x == 0) {
+        umma::prefetch_tensormap(&map_q);
+        umma::prefetch_tensormap(&map_k);
+        umma::prefetch_tensormap(&map_v);
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&b->q_full[i], 1);
+            ptx::mbar_init(&b->s_full[i], 1);
+            ptx::mbar_init(&b->p_full[i], 4);
+            ptx::mbar_init(&b->o_full[i], 1);
+        }
+        for (int i = 0; i < kStages; ++i) {
+            ptx::mbar_init(&b->full[i], 1);
+            ptx::mbar_init(&b->empty[i], 1);
+        }
+        ptx::mbar_init(&b->tail, 1);
+        ptx::mbar_init(&b->quiet, 1);
+        b->st.failed = 0;
+        ptx::mbar_fence_init();
+    }
+    if (warp == 9) {
+        umma::tmem_alloc(&b->st.tmem_base, 512);
+        umma::tmem_relinquish();
+    }
+    umma::fence_before_thread_sync();
+    __syncthreads();
+    umma::fence_after_thread_sync();
+    const uint32_t tmem = b->st.tmem_base;
+    ptx::wait_for_previous_kernel();
+    ptx::let_next_kernel_start();
+    // long blocks first: those at the ends of the sequences
+    const AttnBlock blk = find_block<256>(a.cu_q, a.num_seqs, a.tq, static_cast<int>(gridDim.x / a.heads - 1 - blockIdx.x / a.heads));
+    const int2 keys = sequence_rows(a.cu_k, blk.seq, a.tk);
+    const int shift = keys.y - blk.rows;                          // query i sees the keys up to i + shift
+    // blocks of 128 keys that the tiles' rows see
+    int n[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int last = min(blk.row0 + t * 128 + 128, blk.rows) - 1;
+        const int seen = a.causal ? min(last + shift + 1, keys.y) : keys.y;
+        n[t] = blk.row0 + t * 128 >= blk.rows || seen <= 0 ? 0 : (seen + 127) / 128;
+    }
+    const int blocks = max(n[0], n[1]);
+    int* failed = &b->st.failed;
+
+    if (warp >= 8) {
+        give_registers();
+        if (warp == 8) {
+            AttnRing<kStages> p;
+            const bool one = ptx::elect_one();
+            auto request = [&](const CUtensorMap* map, int j, bool clear) {
+                if (!attn_wait_warp(&b->empty[p.stage], p.phase ^ 1, failed, a.report, 1)) return false;
+                uint8_t* tile = skv + p.stage * kTileBytes;
+                const bool tail = clear && j * 128 + 128 > keys.y;     // (the last block: at most once)
+                uint64_t* bar = tail ? &b->tail : &b->full[p.stage];
+                if (one) {
+                    ptx::mbar_arrive_expect_tx(bar, kTileBytes);
+                    load_tile<128, kChunks>(tile, map, kv_head, keys.x + j * 128, bar);
+                }
+                __syncwarp();
+                if (tail) {
+                    if (!attn_wait_warp(&b->tail, 0, failed, a.report, 4)) return false;
+                    clear_tile<128, kChunks>(tile, keys.y - j * 128);
+                    if (one) ptx::mbar_arrive(&b->full[p.stage]);
+                }
+                p.advance();
+                return true;
+            };
+            if (blocks > 0) {
+                if (one)
+                    for (int t = 0; t < 2; ++t)
+                        if (n[t] > 0) {
+                            ptx::mbar_arrive_expect_tx(&b->q_full[t], kTileBytes);
+                            load_tile<128, kChunks>(sq + t * kTileBytes, &map_q, head, blk.start + blk.row0 + t * 128, &b->q_full[t]);
+                        }
+                __syncwarp();
+                for (int j = 0; j < blocks; ++j)
+                    if (!request(&map_k, j, false) || !request(&map_v, j, true)) break;
+            }
+        } else if (warp == 9) {
+            if (ptx::elect_one() && blocks > 0) {
+                const int dim16 = (a.dim + 15) / 16;
+                const uint32_t idesc_s = umma::make_instr_desc(128, 128, umma::kFormatBF16);
+                const uint32_t idesc_o = umma::make_instr_desc(128, 16, umma::kFormatBF16, false, true) + (static_cast<uint32_t>(2 * dim16 - 2) << 17);
+                auto scores = [&](int t, const uint8_t* tile) {
+                    for (int k = 0; k < dim16; ++k)
+                        umma::mma_ss<false>(tmem + t * 128, desc_channels<128>(sq + t * kTileBytes, k), desc_channels<128>(tile, k), idesc_s, k != 0);
+                    umma::mma_commit(&b->s_full[t]);
+                };
+                AttnRing<kStages> p;
+                auto multiply = [&]() {
+                    if (!attn_wait(&b->full[0], 0, failed, a.report, 4)) return;
+                    for (int t = 0; t < 2; ++t)
+                        if (n[t] > 0) {
+                            if (!attn_wait(&b->q_full[t], 0, failed, a.report, 4)) return;
+                            umma::fence_after_thread_sync();
+                            scores(t, skv);
+                        }
+                    umma::mma_commit(&b->empty[0]);
+                    p.advance();
+                    for (int j = 0; j < blocks; ++j) {
+                        const int stage_v = p.stage;
+                        if (!attn_wait(&b->full[stage_v], p.phase, failed, a.report, 4)) return;
+                        p.advance();
+                        bool have_k = false;
+                        for (int t = 0; t < 2; ++t) {
+                            if (j >= n[t]) continue;
+                            if (!attn_wait(&b->p_full[t], j & 1, failed, a.report, 2)) return;
+                            umma::fence_after_thread_sync();
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                umma::mma_ts(tmem + Shape::kOut + t * 128, tmem + t * 128 + k * 8, desc_rows<128>(skv + stage_v * kTileBytes, k), idesc_o, j != 0 || k != 0);
+                            if (j + 1 == n[t]) {
+                                umma::mma_commit(&b->o_full[t]);
+                            } else {
+                                if (!have_k && !attn_wait(&b->full[p.stage], p.phase, failed, a.report, 4)) return;
+                                have_k = true;
+                                umma::fence_after_thread_sync();
+                                scores(t, skv + p.stage * kTileBytes);
+                            }
+                        }
+                        umma::mma_commit(&b->empty[stage_v]);
+                        if (have_k) {
+                            umma::mma_commit(&b->empty[p.stage]);
+                            p.advance();
+                        }
+                    }
+                };
+                multiply();
+            }
+        }
+    } else {
+        take_registers();
+        const int t = warp >> 2, lane_row = threadIdx.x & 127, row = blk.row0 + t * 128 + lane_row;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), ts = lanes + t * 128, to = lanes + Shape::kOut + t * 128;
+        const float c = a.scale * kLog2e;
+        const int seen = a.causal ? min(row + shift + 1, keys.y) : keys.y;      // keys that this row sees
+        const int first_seen = a.causal ? min(blk.row0 + t * 128 + shift + 1, keys.y) : keys.y;      // ... and the tile's first row
+        float ref = 0.f, sum = 0.f;
+        bool ok = true;
+        for (int j = 0; j < n[t]; ++j) {
+            ok = attn_wait_warp(&b->s_full[t], j & 1, failed, a.report, 5);
+            if (!ok) break;
+            umma::fence_after_thread_sync();
+            uint32_t s[4][32];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) umma::tmem_ld_32x32(ts + i * 32, s[i]);
+            umma::tmem_ld_wait();
+            if (j * 128 + 128 > first_seen) {
+                const int visible = seen - j * 128;
+#pragma unroll
+                for (int i = 0; i < 128; ++i)
+                    if (i >= visible) s[i >> 5][i & 31] = 0xff800000u;
+            }
+            float top[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                top[i] = __uint_as_float(s[i][0]);
+#pragma unroll
+                for (int k = 1; k < 32; ++k) top[i] = fmaxf(top[i], __uint_as_float(s[i][k]));
+            }
+            const float largest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            // The reference moves only when the largest score is more than 2^8 above it: sums and probabilities have that much room, and O is seldom multiplied.
+            if (j == 0) {
+                ref = largest == kNone ? 0.f : largest;
+            } else {
+                const bool move = (largest - ref) * c > 8.f;
+                if (__any_sync(0xffffffffu, move)) {
+                    const float factor = move ? exp2_approx((ref - largest) * c) : 1.f;
+                    sum *= factor;
+                    ref = move ? largest : ref;
+#pragma unroll
+                    for (int i = 0; i < 64 * kChunks; i += 32) {
+                        uint32_t o[32];
+                        umma::tmem_ld_32x32(to + i, o);
+                        umma::tmem_ld_wait();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
+                        umma::tmem_st_32x32(to + i, o);
+                    }
+                }
+            }
+            const uint64_t c2 = f32x2(c, c), minus = f32x2(-ref * c, -ref * c);
+            uint64_t part[2] = {f32x2(sum, 0.f), f32x2(0.f, 0.f)};
+#pragma unroll
+            for (int i = 0; i < 4; i += 2) {
+                uint32_t out[32];
+#pragma unroll
+                for (int k = 0; k < 64; k += 2) {
+                    float x, y;
+                    umma::unpack_f32x2(fma2(umma::pack_f32x2(s[i + (k >> 5)][k & 31], s[i + (k >> 5)][(k & 31) + 1]), c2, minus), x, y);
+                    x = exp2_approx(x);
+                    y = exp2_approx(y);
+                    part[(k >> 1) & 1] = add2(part[(k >> 1) & 1], f32x2(x, y));
+                    out[k >> 1] = pack_bf16(x, y);
+                }
+                umma::tmem_st_32x32(ts + i * 16, out);
+            }
+            float u, v;
+            umma::unpack_f32x2(add2(part[0], part[1]), u, v);
+            sum = u + v;
+            umma::tmem_st_wait();
+            umma::fence_before_thread_sync();
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->p_full[t]);
+        }
+        const bool in = row < blk.rows;
+        const int64_t token = blk.start + row;
+        bf16* out = reinterpret_cast<bf16*>(a.o) + (token * a.heads + head) * a.dim;
+        if (n[t] > 0) {
+            ok = ok && attn_wait_warp(&b->o_full[t], 0, failed, a.report, 6);
+            if (ok) {
+                umma::fence_after_thread_sync();
+                store_row<64 * kChunks>(to, sum == 0.f ? 0.f : 1.f / sum, out, a.dim, in);
+            }
+        } else if (in) {
+            for (int i = 0; i < a.dim; i += 8) *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
+        }
+        if (in && ok) a.lse[static_cast<int64_t>(head) * a.tq + token] = sum == 0.f ? kNone : (ref * c + log2f(sum)) * kLn2;
+        clear_rows<256>(a.cu_q, a.num_seqs, a.tq, reinterpret_cast<bf16*>(a.o), static_cast<int64_t>(a.heads) * a.dim, a.lse, a.heads);
+    }
+    umma::fence_before_thread_sync();
+    __syncthreads();
+    if (b->st.failed != 0) {
+        // (a wait has run out: what was requested or issued ends before its memory goes to others)
+        if (warp == 8) {
+            for (int i = 0; i < 2; ++i)
+                if (n[i] > 0) mbar_drain(&b->q_full[i], 0, 100000000ull);
+            for (int i = 0; i < kStages; ++i) mbar_drain(&b->full[i], 0, 100000000ull), mbar_drain(&b->full[i], 1, 100000000ull);
+        }
+        if (warp == 9 && ptx::elect_one()) {
+            umma::mma_commit(&b->quiet);
+            mbar_drain(&b->quiet, 0, 1000000000ull);
+        }
+        __syncthreads();
+    }
+    if (warp == 9) umma::tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+// delta = rowsum(dO O) - d_lse: 16 lanes per row of a head
+constexpr int kDeltaThreads = 256;
+__global__ void __launch_bounds__(kDeltaThreads) attention_delta_kernel(const __grid_constant__ AttentionArgs a) {
+    ptx::wait_for_previous_kernel();
+    ptx::let_next_kernel_start();
+    const int64_t row = (static_cast<int64_t>(blockIdx.x) * kDeltaThreads + threadIdx.x) / 16;
+    const int lane = threadIdx.x & 15, c = lane * 8;
+    const int64_t token = row / a.heads;
+    const int head = static_cast<int>(row - token * a.heads);
+    const bool in = token < a.tq;
+    float sum = 0.f;
+    if (in && c < a.dim) {
+        const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(a.d_o.data) + token * a.d_o.stride_token + head * a.d_o.stride_head + c);
+        const uint4 y = *reinterpret_cast<const uint4*>(static_cast<const bf16*>(a.o_in.data) + token * a.o_in.stride_token + head * a.o_in.stride_head + c);
+        const uint32_t u[4] = {x.x, x.y, x.z, x.w}, v[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            sum = fmaf(__uint_as_float(u[i] << 16), __uint_as_float(v[i] << 16), sum);
+            sum = fmaf(__uint_as_float(u[i] & 0xffff0000u), __uint_as_float(v[i] & 0xffff0000u), sum);
+        }
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (in && lane == 0) {
+        const int64_t at = static_cast<int64_t>(head) * a.tq + token;
+        a.delta[at] = a.d_lse != nullptr ? sum - a.d_lse[at] : sum;
+    }
+}
+
+// A CTA keeps 128 rows of one side (kKeys: keys and values, whose gradients it makes; otherwise queries and dO, for dQ) and takes those of the other side in
+// pieces of 64.  Scores and dP of a piece are products whose lanes are the kept rows, so that P and dS, written over them, are first operands of the products
+// that follow, and sums stay in tensor memory until the end: every gradient is added by one CTA, in a fixed order.  P is made twice, which costs two products of
+// seven, and spares sums of dQ in memory by many CTAs in any order.  Two groups of four warps take every other piece.
+constexpr int kBwdThreads = 384;                     // as in the forward pass
+template <int kChunks>
+struct BwdShape {
+    static constexpr int kKeptBytes = 128 * 128 * kChunks, kPieceBytes = 64 * 128 * kChunks, kStages = kChunks == 2 ? 4 : 6;
+    static constexpr int kBuffers = 256;              // tensor memory: two sums of 128 columns, then twice scores and dP of 64 columns
+    static constexpr int kStatBytes = 2 * 2 * 128 * 4;
+    static constexpr int kSmem = 2 * kKeptBytes + 2 * kStages * kPieceBytes + kStatBytes + 1024;
+};
+struct BwdBars {
+    uint64_t kept, full[8], empty[8], s_full[2], p_full[2], sums, tail, quiet;
+    AttnState st;
+};
+
+template <int kChunks, bool kKeys>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const __grid_constant__ CUtensorMap map_kept1, const __grid_constant__ CUtensorMap map_piece0,
+                          const __grid_constant__ CUtensorMap map_piece1, const __grid_constant__ AttentionArgs a) {
+    using Shape = BwdShape<kChunks>;
+    constexpr int kStages = Shape::kStages, kPieceBytes = Shape::kPieceBytes, kKeptBytes = Shape::kKeptBytes;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t *kept = smem, *pieces = smem + 2 * kKeptBytes;
+    float* stats = reinterpret_cast<float*>(pieces + 2 * kStages * kPieceBytes);
+    BwdBars* b = reinterpret_cast<BwdBars*>(pieces + 2 * kStages * kPieceBytes + Shape::kStatBytes);
+    const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads;
+    if (threadIdx.x == 0) {
+        umma::prefetch_tensormap(&map_kept0);
+        umma::prefetch_tensormap(&map_kept1);
+        umma::prefetch_tensormap(&map_piece0);
+        umma::prefetch_tensormap(&map_piece1);
+        ptx::mbar_init(&b->kept, 1);
+        for (int i = 0; i < kStages; ++i) {
+            ptx::mbar_init(&b->full[i], 1);
+            ptx::mbar_init(&b->empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&b->s_full[i], 1);
+            ptx::mbar_init(&b->p_full[i], 4);
+        }
+        ptx::mbar_init(&b->sums, 1);
+        ptx::mbar_init(&b->tail, 1);
+        ptx::mbar_init(&b->quiet, 1);
+        b->st.failed = 0;
+        ptx::mbar_fence_init();
+    }
+    if (warp == 9) {
+        umma::tmem_alloc(&b->st.tmem_base, 512);
+        umma::tmem_relinquish();
+    }
+    umma::fence_before_thread_sync();
+    __syncthreads();
+    umma::fence_after_thread_sync();
+    const uint32_t tmem = b->st.tmem_base;
+    ptx::wait_for_previous_kernel();
+    ptx::let_next_kernel_start();
+    int* failed = &b->st.failed;
+    // (kKeys: the first keys are seen by most queries; otherwise the last queries see most keys.  Long blocks first.)
+    const int heads = kKeys ? a.kv_heads : a.heads, total = kKeys ? a.tk : a.tq;
+    const int head = blockIdx.x % heads, number = blockIdx.x / heads;
+    const AttnBlock blk = find_block<128>(kKeys ? a.cu_k : a.cu_q, a.num_seqs, total, kKeys ? number : static_cast<int>(gridDim.x / heads) - 1 - number);
+    const int2 other = sequence_rows(kKeys ? a.cu_q : a.cu_k, blk.seq, kKeys ? a.tq : a.tk);
+    const int shift = kKeys ? blk.rows - other.y : other.y - blk.rows;     // query i sees the keys up to i + shift
+    // pieces [piece0, piece1) of every head
+    int piece0 = 0, piece1 = 0, n = 0;
+    if (blk.row0 < blk.rows) {
+        if (kKeys) {
+            piece0 = a.causal ? max(blk.row0 - shift, 0) / 64 : 0;
+            piece1 = (other.y + 63) / 64;
+        } else {
+            const int seen = a.causal ? min(min(blk.row0 + 128, blk.rows) + shift, other.y) : other.y;
+            piece1 = seen <= 0 ? 0 : (seen + 63) / 64;
+        }
+        n = max(piece1 - piece0, 0) * (kKeys ? group : 1);
+    }
+    const int per_head = max(piece1 - piece0, 1);
+
+    if (warp >= 8) {
+        give_registers();
+        if (warp == 8) {
+            if (n > 0) {
+                AttnRing<kStages> p;
+                const bool one = ptx::elect_one();
+                if (one) {
+                    ptx::mbar_arrive_expect_tx(&b->kept, 2 * kKeptBytes);
+                    load_tile<128, kChunks>(kept, &map_kept0, head, blk.start + blk.row0, &b->kept);
+                    load_tile<128, kChunks>(kept + kKeptBytes, &map_kept1, head, blk.start + blk.row0, &b->kept);
+                }
+                __syncwarp();
+                uint32_t tails = 0;
+                for (int i = 0; i < n; ++i) {
+                    if (!attn_wait_warp(&b->empty[p.stage], p.phase ^ 1, failed, a.report, 1)) break;
+                    const int h = kKeys ? head * group + i / per_head : head / group, piece = piece0 + i % per_head;
+                    uint8_t* tile = pieces + p.stage * 2 * kPieceBytes;
+                    const bool tail = piece * 64 + 64 > other.y;
+                    uint64_t* bar = tail ? &b->tail : &b->full[p.stage];
+                    if (one) {
+                        ptx::mbar_arrive_expect_tx(bar, 2 * kPieceBytes);
+                        load_tile<64, kChunks>(tile, &map_piece0, h, other.x + piece * 64, bar);
+                        load_tile<64, kChunks>(tile + kPieceBytes, &map_piece1, h, other.x + piece * 64, bar);
+                    }
+                    __syncwarp();
+                    if (tail) {
+                        if (!attn_wait_warp(&b->tail, tails & 1, failed, a.report, 4)) break;
+                        ++tails;
+                        clear_tile<64, kChunks>(tile, other.y - piece * 64);
+                        clear_tile<64, kChunks>(tile + kPieceBytes, other.y - piece * 64);
+                        if (one) ptx::mbar_arrive(&b->full[p.stage]);
+                    }
+                    p.advance();
+                }
+            }
+        } else if (warp == 9) {
+            if (n > 0 && ptx::elect_one()) {
+                const int dim16 = (a.dim + 15) / 16;
+                const uint32_t idesc_s = umma::make_instr_desc(128, 64, umma::kFormatBF16);
+                const uint32_t idesc_o = umma::make_instr_desc(128, 16, umma::kFormatBF16, false, true) + (static_cast<uint32_t>(2 * dim16 - 2) << 17);
+                AttnRing<kStages> p, q;                   // pieces whose scores are next, pieces whose sums are next
+                auto scores = [&](int i) {
+                    if (!attn_wait(&b->full[p.stage], p.phase, failed, a.report, 4)) return false;
+                    umma::fence_after_thread_sync();
+                    const uint8_t* tile = pieces + p.stage * 2 * kPieceBytes;
+                    const uint32_t to = tmem + Shape::kBuffers + (i & 1) * 128;
+                    for (int k = 0; k < dim16; ++k) umma::mma_ss<false>(to, desc_channels<128>(kept, k), desc_channels<64>(tile, k), idesc_s, k != 0);
+                    for (int k = 0; k < dim16; ++k)
+                        umma::mma_ss<false>(to + 64, desc_channels<128>(kept + kKeptBytes, k), desc_channels<64>(tile + kPieceBytes, k), idesc_s, k != 0);
+                    umma::mma_commit(&b->s_full[i & 1]);
+                    p.advance();
+                    return true;
+                };
+                auto multiply = [&]() {
+                    if (!attn_wait(&b->kept, 0, failed, a.report, 4)) return;
+                    if (!scores(0) || (n > 1 && !scores(1))) return;
+                    for (int i = 0; i < n; ++i) {
+                        if (!attn_wait(&b->p_full[i & 1], (i >> 1) & 1, failed, a.report, 2)) return;
+                        umma::fence_after_thread_sync();
+                        const uint8_t* tile = pieces + q.stage * 2 * kPieceBytes;
+                        const uint32_t from = tmem + Shape::kBuffers + (i & 1) * 128;
+                        if (kKeys)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) umma::mma_ts(tmem + 128, from + k * 8, desc_rows<64>(tile + kPieceBytes, k), idesc_o, i != 0 || k != 0);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) umma::mma_ts(tmem, from + 64 + k * 8, desc_rows<64>(tile, k), idesc_o, i != 0 || k != 0);
+                        umma::mma_commit(&b->empty[q.stage]);
+                        q.advance();
+                        if (i + 2 < n && !scores(i + 2)) return;
+                    }
+                    umma::mma_commit(&b->sums);
+                };
+                multiply();
+            }
+        }
+    } else {
+        take_registers();
+        const int half = warp >> 2, lane_row = threadIdx.x & 127, row = blk.row0 + lane_row;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), from = lanes + Shape::kBuffers + half * 128;
+        const float c = a.scale * kLog2e;
+        const bool in = row < blk.rows;
+        const int64_t token = blk.start + row;
+        float* mine = stats + half * 256;             // twice: 64 times -lse log2 e, 64 times -delta
+        // a statistic of a query that sees nothing, or that is none: its probabilities are zero
+        auto statistic = [&](bool is_delta, bool is_there, int h, int64_t query) {
+            if (!is_there) return is_delta ? 0.f : kNone;
+            const int64_t at = static_cast<int64_t>(h) * a.tq + query;
+            if (is_delta) return -a.delta[at];
+            const float l = a.lse_in[at];
+            return l == kNone ? kNone : -l * kLog2e;
+        };
+        auto next_statistic = [&](int i) {
+            if (i >= n) return 0.f;
+            const int at = (piece0 + i % per_head) * 64 + (lane_row & 63);
+            return statistic(lane_row >= 64, at < other.y, head * group + i / per_head, other.x + at);
+        };
+        float coming = 0.f;
+        uint64_t minus2 = 0, delta2 = 0;
+        if (kKeys) {
+            coming = next_statistic(half);
+        } else if (n > 0) {
+            const float m = statistic(false, in, head, token), d = statistic(true, in, head, token);
+            minus2 = f32x2(m, m);
+            delta2 = f32x2(d, d);
+        }
+        bool ok = true;
+        const uint64_t c2 = f32x2(c, c);
+        for (int i = half; i < n; i += 2) {
+            float* now = mine + (i >> 1 & 1) * 128;
+            if (kKeys) {
+                now[lane_row] = coming;
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+                coming = next_statistic(i + 2);
+            }
+            ok = ok && attn_wait_warp(&b->s_full[half], (i >> 1) & 1, failed, a.report, 5);
+            if (!ok) continue;                        // (the others may wait at the barrier above)
+            umma::fence_after_thread_sync();
+            uint32_t s[2][32], d[2][32];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) umma::tmem_ld_32x32(from + k * 32, s[k]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) umma::tmem_ld_32x32(from + 64 + k * 32, d[k]);
+            umma::tmem_ld_wait();
+            const int piece = piece0 + i % per_head;
+            // columns [low, high) are visible
+            int low = 0, high = 64;
+            if (kKeys) {
+                if (a.causal) low = row - shift - piece * 64;
+            } else {
+                high = (a.causal ? min(row + shift + 1, other.y) : other.y) - piece * 64;
+            }
+            const bool masked = __any_sync(0xffffffffu, low > 0 || high < 64);
+            uint32_t ps[32], ds[32];
+#pragma unroll
+            for (int k = 0; k < 64; k += 2) {
+                if (kKeys && (k & 3) == 0) {
+                    const float4 m4 = *reinterpret_cast<const float4*>(now + k), d4 = *reinterpret_cast<const float4*>(now + 64 + k);
+                    minus2 = f32x2(m4.x, m4.y);
+                    delta2 = f32x2(d4.x, d4.y);
+                } else if (kKeys) {
+                    const float2 m4 = *reinterpret_cast<const float2*>(now + k), d4 = *reinterpret_cast<const float2*>(now + 64 + k);
+                    minus2 = f32x2(m4.x, m4.y);
+                    delta2 = f32x2(d4.x, d4.y);
+                }
+                float x, y, u, v;
+                umma::unpack_f32x2(fma2(umma::pack_f32x2(s[k >> 5][k & 31], s[k >> 5][(k & 31) + 1]), c2, minus2), x, y);
+                x = exp2_approx(x);
+                y = exp2_approx(y);
+                umma::unpack_f32x2(mul2(f32x2(x, y), add2(umma::pack_f32x2(d[k >> 5][k & 31], d[k >> 5][(k & 31) + 1]), delta2)), u, v);
+                if (masked) {
+                    const bool see0 = k >= low && k < high, see1 = k + 1 >= low && k + 1 < high;
+                    x = see0 ? x : 0.f;
+                    u = see0 ? u : 0.f;
+                    y = see1 ? y : 0.f;
+                    v = see1 ? v : 0.f;
+                }
+                ps[k >> 1] = pack_bf16(x, y);
+                ds[k >> 1] = pack_bf16(u, v);
+            }
+            if (kKeys) umma::tmem_st_32x32(from, ps);
+            umma::tmem_st_32x32(from + 64, ds);
+            umma::tmem_st_wait();
+            umma::fence_before_thread_sync();
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->p_full[half]);
+        }
+        const int64_t at = (token * heads + head) * a.dim;
+        if (n > 0) {
+            ok = ok && attn_wait_warp(&b->sums, 0, failed, a.report, 6);
+            if (ok) {
+                umma::fence_after_thread_sync();
+                if (!kKeys) {
+                    const int first = half * 32 * kChunks;
+                    store_row<32 * kChunks>(lanes + first, a.scale, reinterpret_cast<bf16*>(a.dq) + at + first, a.dim - first, in);
+                } else if (half == 0) {
+                    store_row<64 * kChunks>(lanes, a.scale, reinterpret_cast<bf16*>(a.dk) + at, a.dim, in);
+                } else {
+                    store_row<64 * kChunks>(lanes + 128, 1.f, reinterpret_cast<bf16*>(a.dv) + at, a.dim, in);
+                }
+            }
+        } else if (in && half == 0) {
+            for (int i = 0; i < a.dim; i += 8) {
+                if (kKeys) {
+                    *reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.dk) + at + i) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.dv) + at + i) = make_uint4(0, 0, 0, 0);
+                } else {
+                    *reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.dq) + at + i) = make_uint4(0, 0, 0, 0);
+                }
+            }
+        }
+        const int64_t row_values = static_cast<int64_t>(heads) * a.dim;
+        if (kKeys) {
+            clear_rows<256>(a.cu_k, a.num_seqs, a.tk, reinterpret_cast<bf16*>(a.dk), row_values, nullptr, 0);
+            clear_rows<256>(a.cu_k, a.num_seqs, a.tk, reinterpret_cast<bf16*>(a.dv), row_values, nullptr, 0);
+        } else {
+            clear_rows<256>(a.cu_q, a.num_seqs, a.tq, reinterpret_cast<bf16*>(a.dq), row_values, nullptr, 0);
+        }
+    }
+    umma::fence_before_thread_sync();
+    __syncthreads();
+    if (b->st.failed != 0) {
+        // (as in the forward pass)
+        if (warp == 8 && n > 0) {
+            mbar_drain(&b->kept, 0, 100000000ull);
+            for (int i = 0; i < kStages; ++i) mbar_drain(&b->full[i], 0, 100000000ull), mbar_drain(&b->full[i], 1, 100000000ull);
+        }
+        if (warp == 9 && ptx::elect_one()) {
+            umma::mma_commit(&b->quiet);
+            mbar_drain(&b->quiet, 0, 1000000000ull);
+        }
+        __syncthreads();
+    }
+    if (warp == 9) umma::tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------------------------------------------ host
+bool make_map(CUtensorMap* map, const HeadsView& x, int64_t tokens, int64_t heads, int64_t dim, int box_rows) {
+    EncodeTiledFn encode = get_encode_fn();
+    if (encode == nullptr) return false;
+    // (a stride that nothing steps along may be anything)
+    const int64_t pitch = (dim * 2 + 15) / 16 * 16;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(heads > 1 ? x.stride_head * 2 : pitch), static_cast<cuuint64_t>(tokens > 1 ? x.stride_token * 2 : pitch)};
+    const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t steps[3] = {1, 1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(x.data), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// leave for shared memory, once per device
+cudaError_t allow_once(const void* fn, int bytes, std::atomic<uint64_t>& allowed) {
+    int device = 0;
+    cudaError_t err = cudaGetDevice(&device);
+    if (err != cudaSuccess) return err;
+    if (device >= 64 || (allowed.load(std::memory_order_relaxed) >> device & 1) == 0) {
+        err = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (err != cudaSuccess) cudaGetLastError();      // the caller reports it
+        else if (device < 64) allowed.fetch_or(1ull << device, std::memory_order_relaxed);
+    }
+    return err;
+}
+
+template <int kChunks>
+cudaError_t launch_forward(const AttentionArgs& a, cudaStream_t stream) {
+    const void* fn = reinterpret_cast<const void*>(attention_kernel<kChunks>);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t err = allow_once(fn, FwdShape<kChunks>::kSmem, allowed);
+    if (err != cudaSuccess) return err;
+    CUtensorMap q, k, v;
+    if (!make_map(&q, a.q, a.tq, a.heads, a.dim, 128) || !make_map(&k, a.k, a.tk, a.kv_heads, a.dim, 128) || !make_map(&v, a.v, a.tk, a.kv_heads, a.dim, 128))
+        return cudaErrorInvalidValue;
+    void* params[] = {&q, &k, &v, const_cast<AttentionArgs*>(&a)};
+    return launch_dependent(fn, dim3(static_cast<unsigned>(num_blocks<256>(a.tq, a.num_seqs) * a.heads)), dim3(kFwdThreads), params, FwdShape<kChunks>::kSmem, stream);
+}
+template <int kChunks, bool kKeys>
+cudaError_t launch_gradient(const AttentionArgs& a, cudaStream_t stream) {
+    const void* fn = reinterpret_cast<const void*>(attention_backward_kernel<kChunks, kKeys>);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t err = allow_once(fn, BwdShape<kChunks>::kSmem, allowed);
+    if (err != cudaSuccess) return err;
+    CUtensorMap q, k, v, d;
+    const int queries = kKeys ? 64 : 128, keys = kKeys ? 128 : 64;
+    if (!make_map(&q, a.q, a.tq, a.heads, a.dim, queries) || !make_map(&d, a.d_o, a.tq, a.heads, a.dim, queries) || !make_map(&k, a.k, a.tk, a.kv_heads, a.dim, keys) ||
+        !make_map(&v, a.v, a.tk, a.kv_heads, a.dim, keys))
+        return cudaErrorInvalidValue;
+    void* params[] = {kKeys ? &k : &q, kKeys ? &v : &d, kKeys ? &q : &k, kKeys ? &d : &v, const_cast<AttentionArgs*>(&a)};
+    const int64_t ctas = num_blocks<128>(kKeys ? a.tk : a.tq, a.num_seqs) * (kKeys ? a.kv_heads : a.heads);
+    return launch_dependent(fn, dim3(static_cast<unsigned>(ctas)), dim3(kBwdThreads), params, BwdShape<kChunks>::kSmem, stream);
+}
+template <int kChunks>
+cudaError_t launch_backward(const AttentionArgs& a, cudaStream_t stream) {
+    void* params[] = {const_cast<AttentionArgs*>(&a)};
+    const int64_t rows = static_cast<int64_t>(a.tq) * a.heads;
+    cudaError_t err = launch_dependent(reinterpret_cast<const void*>(attention_delta_kernel), dim3(static_cast<unsigned>((rows * 16 + kDeltaThreads - 1) / kDeltaThreads)),
+                                       dim3(kDeltaThreads), params, 0, stream);
+    if (err == cudaSuccess) err = launch_gradient<kChunks, true>(a, stream);
+    if (err == cudaSuccess) err = launch_gradient<kChunks, false>(a, stream);
+    return err;
+}
+
+}  // namespace
+
+cudaError_t launch_attention(const AttentionArgs& a, int num_sms, cudaStream_t stream) {
+    return a.dim <= 64 ? launch_forward<1>(a, stream) : launch_forward<2>(a, stream);
+}
+cudaError_t launch_attention_backward(const AttentionArgs& a, int num_sms, cudaStream_t stream) {
+    return a.dim <= 64 ? launch_backward<1>(a, stream) : launch_backward<2>(a, stream);
+}
+
+}  // namespace ep

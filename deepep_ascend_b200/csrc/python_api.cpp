@@ -5,6 +5,7 @@
 #include <algorithm>
 
 #include "kernels/api.h"
+#include "runtime/attention_ops.hpp"
 #include "runtime/block_ops.hpp"
 #include "runtime/coordinator.hpp"
 #include "runtime/elastic_buffer.hpp"
@@ -980,6 +981,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         return orthogonalize(x, steps, a, b, c, eps, out, num_sms, gemm_error_flag(x.get_device()), report_to);
     }, py::arg("x"), py::arg("steps"), py::arg("a"), py::arg("b"), py::arg("c"), py::arg("eps"), py::arg("out") = py::none(), py::arg("num_sms") = 0,
           py::arg("report_to") = py::none());
+    m.def("attention", [](const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const std::optional<at::Tensor>& cu_q, const std::optional<at::Tensor>& cu_k, bool causal,
+                          double scale, ElasticBufferCore* report_to) -> std::optional<std::tuple<at::Tensor, at::Tensor>> {
+        if (not_for_a_kernel({&q, &k, &v}) || watched({given(cu_q), given(cu_k)})) return std::nullopt;
+        TORCH_CHECK(q.is_cuda(), "q must be on a GPU");
+        return attention(q, k, v, cu_q, cu_k, causal, scale, gemm_error_flag(q.get_device()), report_to);
+    }, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("cu_q"), py::arg("cu_k"), py::arg("causal"), py::arg("scale"), py::arg("report_to") = py::none());
+    m.def("attention_backward", [](const at::Tensor& d_o, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& lse,
+                                   const std::optional<at::Tensor>& d_lse, const std::optional<at::Tensor>& cu_q, const std::optional<at::Tensor>& cu_k, bool causal, double scale,
+                                   ElasticBufferCore* report_to) -> std::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor>> {
+        if (not_for_a_kernel({&d_o, &q, &k, &v, &o, &lse, given(d_lse)}) || watched({given(cu_q), given(cu_k)})) return std::nullopt;
+        TORCH_CHECK(q.is_cuda(), "q must be on a GPU");
+        return attention_backward(d_o, q, k, v, o, lse, d_lse, cu_q, cu_k, causal, scale, gemm_error_flag(q.get_device()), report_to);
+    }, py::arg("d_o"), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("o"), py::arg("lse"), py::arg("d_lse"), py::arg("cu_q"), py::arg("cu_k"), py::arg("causal"),
+          py::arg("scale"), py::arg("report_to") = py::none());
     m.def("gemm_error", [](int device) { return gemm_error_flag(device).item<int>(); });
     m.def("get_dispatch_layout", &get_dispatch_layout);
     m.def("per_token_cast_to_fp8", &per_token_cast_to_fp8, py::arg("x"), py::arg("round_scale") = false,

@@ -1,0 +1,139 @@
+"""Attention on the tensor cores: packed prompts, forward and backward (``csrc/kernels/attention.cu``), and single tokens over a paged cache
+(``csrc/kernels/paged_attention.cu``).  CPU tensors take the PyTorch statements below.
+
+No counterpart in the reference, which stops at the exchange of tokens.
+"""
+from typing import Optional, Tuple
+
+import torch
+
+from .. import _native
+from .gemm import _by_type, _core_of, _gradient_alone
+
+
+def _options(q: torch.Tensor, cu_seqlens, cu_seqlens_k, scale: Optional[float]):
+    if cu_seqlens is None and cu_seqlens_k is not None:
+        raise ValueError('cu_seqlens_k goes with cu_seqlens')
+    return cu_seqlens, cu_seqlens if cu_seqlens_k is None else cu_seqlens_k, q.shape[-1]**-0.5 if scale is None else float(scale)
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, cu_seqlens_k: Optional[torch.Tensor] = None,
+              causal: bool = True, scale: Optional[float] = None, buffer=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``q [tokens, heads, dim]``, ``k`` and ``v [keys, kv_heads, dim]`` (bf16, ``dim`` a multiple of 8, at most 128) -> ``(o`` like ``q``, contiguous,
+    ``lse`` fp32 ``[heads, tokens])``: ``o = softmax(scale q k^T) v`` and ``lse = log sum exp(scale q k^T)`` within each sequence.  ``heads`` is a multiple of
+    ``kv_heads``: as many neighbouring heads share keys and values.  ``scale``: ``dim ** -0.5`` if none is given, positive.
+
+    ``cu_seqlens`` int32 ``[sequences + 1]``: where the sequences start in ``q``, and where the last one ends; none: one sequence.  ``cu_seqlens_k``: the same of ``k``
+    and ``v``, if their lengths are others (keys of earlier calls in front).  With ``causal`` both of a sequence end together: query ``i`` of ``n`` sees the keys up to
+    ``i + keys - n``.  A query that sees no key, and one that belongs to no sequence, gets zeros and an ``lse`` of -inf.
+
+    Whatever lies behind a sequence is not looked at; within one, keys and values must be numbers (a NaN reaches queries of its tile that do not see it).  Any strides;
+    heads whose channels are apart or that do not start on 16 bytes are copied first.  ``buffer``: see :func:`ops.gemm.gemm_nt`.
+
+    Both results carry gradients, by the kernels of :func:`attention_backward`.  Tracers, function transforms, dispatch modes and forward mode see the PyTorch
+    statement."""
+    cu_q, cu_k, scale = _options(q, cu_seqlens, cu_seqlens_k, scale)
+    if q.is_cuda and _by_type(q, k, v, cu_q, cu_k):
+        res = _native.load().attention(q, k, v, cu_q, cu_k, causal, scale, _core_of(buffer))
+        if res is not None:
+            return res
+        if _gradient_alone(q, k, v):
+            return _Attention.apply(q, k, v, cu_q, cu_k, causal, scale, buffer)
+    return attention_ref(q, k, v, cu_q, cu_k, causal, scale)
+
+
+class _Attention(torch.autograd.Function):
+    """``apply(q, k, v, cu_seqlens, cu_seqlens_k, causal, scale, buffer) -> (o, lse)``, both with gradients."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_q, cu_k, causal, scale, buffer):
+        o, lse = attention(q, k, v, cu_q, cu_k, causal, scale, buffer)
+        ctx.save_for_backward(q, k, v, o, lse, cu_q, cu_k)
+        ctx.options = dict(causal=causal, scale=scale, buffer=buffer)
+        ctx.set_materialize_grads(False)
+        return o, lse
+
+    @staticmethod
+    def backward(ctx, d_o, d_lse):
+        q, k, v, o, lse, cu_q, cu_k = ctx.saved_tensors
+        if d_o is None:
+            d_o = torch.zeros_like(o)
+        d_lse = None if d_lse is None else d_lse.contiguous()
+        return (*attention_backward(d_o, q, k, v, o, lse, cu_q, cu_k, d_lse=d_lse, **ctx.options), None, None, None, None, None)
+
+
+def attention_backward(d_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, lse: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
+                       cu_seqlens_k: Optional[torch.Tensor] = None, causal: bool = True, scale: Optional[float] = None, d_lse: Optional[torch.Tensor] = None,
+                       buffer=None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients of :func:`attention` from ``d_o`` (like ``o``), optionally ``d_lse`` (like ``lse``), and what the forward pass was given and returned ->
+    ``(d_q, d_k, d_v)``, contiguous.  Those of shared keys and values are added over their heads in 32 bits; every sum is taken in one order.  Queries and keys of no
+    sequence, queries that see nothing and keys that nobody sees get zeros.  Where these gradients are to carry gradients themselves, and for whoever watches, the
+    PyTorch statement runs."""
+    cu_q, cu_k, scale = _options(q, cu_seqlens, cu_seqlens_k, scale)
+    if q.is_cuda and _by_type(d_o, q, k, v, o, lse, d_lse, cu_q, cu_k):
+        res = _native.load().attention_backward(d_o, q, k, v, o, lse, d_lse, cu_q, cu_k, causal, scale, _core_of(buffer))
+        if res is not None:
+            return res
+    return attention_backward_ref(d_o, q, k, v, o, lse, cu_q, cu_k, causal, scale, d_lse)
+
+
+def _wide(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype == torch.float64 else t.float()
+
+
+def _sees(q, k, cu_q, cu_k, causal: bool) -> torch.Tensor:
+    """``[tokens, keys]``: whether a query sees a key."""
+    def place(t, cu):
+        at = torch.arange(t.shape[0], device=t.device)
+        if cu is None:
+            return torch.zeros_like(at), at, torch.full_like(at, t.shape[0])
+        cu = cu.long()
+        seq = (torch.searchsorted(cu, at, right=True) - 1).clamp(0, max(cu.numel() - 2, 0))
+        if cu.numel() < 2:
+            return torch.full_like(at, -1), at, at
+        inside = (at >= cu[seq]) & (at < cu[seq + 1])
+        return torch.where(inside, seq, -1), at - cu[seq], cu[seq + 1] - cu[seq]
+    (sq, iq, nq), (sk, ik, nk) = place(q, cu_q), place(k, cu_k)
+    sees = (sq[:, None] == sk) & (sq >= 0)[:, None]
+    return sees & (ik - nk <= (iq - nq)[:, None]) if causal else sees
+
+
+def _scores(q, k, cu_q, cu_k, causal, scale):
+    group = q.shape[1] // k.shape[1]
+    s = torch.einsum('ihd,jhd->hij', _wide(q), _wide(k).repeat_interleave(group, 1)) * scale
+    sees = _sees(q, k, cu_q, cu_k, causal)
+    return torch.where(sees, s, float('-inf')), sees, group
+
+
+def attention_ref(q, k, v, cu_seqlens=None, cu_seqlens_k=None, causal=True, scale=None):
+    """:func:`attention` stated with plain PyTorch operations (any device; what the kernel is tested against).  All scores at once."""
+    cu_q, cu_k, scale = _options(q, cu_seqlens, cu_seqlens_k, scale)
+    if k.shape[0] == 0:
+        return torch.zeros_like(q), _wide(q).new_full((q.shape[1], q.shape[0]), float('-inf'))
+    s, sees, group = _scores(q, k, cu_q, cu_k, causal, scale)
+    some = sees.any(-1)
+    top = torch.where(some, s.max(-1).values, 0.0).detach()
+    e = torch.exp(s - top.unsqueeze(-1))
+    total = torch.where(some, e.sum(-1), 1.0)
+    o = torch.einsum('hij,jhd->ihd', e / total.unsqueeze(-1), _wide(v).repeat_interleave(group, 1))
+    return o.to(q.dtype), torch.where(some, top + torch.log(total), float('-inf'))
+
+
+def attention_backward_ref(d_o, q, k, v, o, lse, cu_seqlens=None, cu_seqlens_k=None, causal=True, scale=None, d_lse=None):
+    """:func:`attention_backward` stated with plain PyTorch operations."""
+    cu_q, cu_k, scale = _options(q, cu_seqlens, cu_seqlens_k, scale)
+    if k.shape[0] == 0:
+        return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    s, sees, group = _scores(q, k, cu_q, cu_k, causal, scale)
+    p = torch.where(sees, torch.exp(s - torch.where(sees.any(-1), lse, 0.0).unsqueeze(-1)), 0.0)
+    g = _wide(d_o)
+    dp = torch.einsum('ihd,jhd->hij', g, _wide(v).repeat_interleave(group, 1))
+    delta = (g * _wide(o)).sum(-1).t()
+    if d_lse is not None:
+        delta = delta - d_lse
+    ds = torch.where(sees, p * (dp - delta.unsqueeze(-1)), 0.0) * scale
+    dq = torch.einsum('hij,jhd->ihd', ds, _wide(k).repeat_interleave(group, 1))
+    shape = (k.shape[0], k.shape[1], group, k.shape[2])
+    dk = torch.einsum('hij,ihd->jhd', ds, _wide(q)).view(shape).sum(2)
+    dv = torch.einsum('hij,ihd->jhd', p, g).view(shape).sum(2)
+    return dq.to(q.dtype), dk.to(k.dtype), dv.to(v.dtype)
