@@ -7,6 +7,7 @@
 
 #define EP_MAX_RANKS 8
 #define EP_MAX_EXPERTS 1024
+#define EP_MAX_PAGED_SEQS 4096
 #define EP_MAX_TOPK 16
 #define EP_MAX_CTAS 160
 #define EP_MAX_TILE_FLAGS 16384
@@ -603,4 +604,60 @@ struct AttentionArgs {
 namespace ep {
 cudaError_t launch_attention(const AttentionArgs& args, int num_sms, cudaStream_t stream);
 cudaError_t launch_attention_backward(const AttentionArgs& args, int num_sms, cudaStream_t stream);
+}  // namespace ep
+
+// One new token per sequence over a paged cache (paged_attention.cu)
+struct PagedAttentionArgs {
+    HeadsView q;                      // bf16 [num_seqs, heads, dim]
+    const void *k_cache, *v_cache;    // bf16 [num_pages, page_size, kv_heads, dim], strides in elements
+    int64_t stride_page, stride_slot, stride_head;
+    int64_t num_pages;
+    int page_size;
+    const int32_t* page_table;        // [num_seqs, table_width], row pitch table_pitch
+    int64_t table_pitch;
+    int table_width;
+    const int32_t* lengths;           // [num_seqs]
+    int num_seqs, heads, kv_heads, dim;
+    float scale;
+    void* o;                          // bf16 [num_seqs, heads, dim] contiguous
+    float* parts;                     // workspace of paged_attention_workspace() bytes
+};
+
+namespace ep {
+int64_t paged_attention_workspace(const PagedAttentionArgs& args, int num_sms);      // (sizes alone are read)
+cudaError_t launch_paged_attention(const PagedAttentionArgs& args, int num_sms, cudaStream_t stream);
+}  // namespace ep
+
+// ------------------------------------------------------------------------------------------------ norm and rotation of heads
+// Queries (0) and keys (1), [tokens, heads, dim] of one type (rotary.cu states the formulas)
+struct RotaryArgs {
+    HeadsView x[2], dy[2];
+    void* out[2];                     // results (or, of the gradient, those of x), contiguous
+    int heads[2];
+    const void* weight[2];            // [dim]
+    int tokens, dim, rotary;          // dim: a multiple of 8, at most 256; rotary: a multiple of 16, at most dim
+    int x_bf16, param_bf16, interleaved;
+    const float* table;               // [num_positions, rotary]: cosines, then sines
+    int64_t num_positions;
+    const void* positions;            // [tokens] int64 or int32
+    int positions_64;
+    float eps;
+    // keys and values into a paged cache
+    HeadsView v;
+    void *k_cache, *v_cache;          // or null: no cache
+    int64_t stride_page, stride_slot, stride_head;
+    int64_t num_slots;                // num_pages * page_size
+    int page_size;
+    const void* slots;                // [tokens] int64 or int32
+    int slots_64;
+    // gradient
+    void* dw[2];                      // [dim]
+    float* partial;                   // [ctas, 2, dim]
+    int ctas;
+};
+
+namespace ep {
+cudaError_t launch_rotary(const RotaryArgs& args, int num_sms, cudaStream_t stream);
+int rotary_backward_ctas(const RotaryArgs& args, int num_sms);
+cudaError_t launch_rotary_backward(const RotaryArgs& args, cudaStream_t stream);
 }  // namespace ep

@@ -995,6 +995,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         return attention_backward(d_o, q, k, v, o, lse, d_lse, cu_q, cu_k, causal, scale, gemm_error_flag(q.get_device()), report_to);
     }, py::arg("d_o"), py::arg("q"), py::arg("k"), py::arg("v"), py::arg("o"), py::arg("lse"), py::arg("d_lse"), py::arg("cu_q"), py::arg("cu_k"), py::arg("causal"),
           py::arg("scale"), py::arg("report_to") = py::none());
+    m.def("paged_attention", [](const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& page_table, const at::Tensor& lengths, double scale,
+                                const std::optional<at::Tensor>& out) -> std::optional<at::Tensor> {
+        if (not_for_a_kernel({&q, &k_cache, &v_cache, given(out)}) || watched({&page_table, &lengths})) return std::nullopt;
+        return paged_attention(q, k_cache, v_cache, page_table, lengths, scale, out);
+    }, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("page_table"), py::arg("lengths"), py::arg("scale"), py::arg("out") = py::none());
+    m.def("qk_norm_rope", &qk_norm_rope, py::arg("q"), py::arg("k"), py::arg("q_weight"), py::arg("k_weight"), py::arg("table"), py::arg("positions"), py::arg("eps"),
+          py::arg("interleaved"));
+    m.def("qk_norm_rope_append", &qk_norm_rope_append, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("q_weight"), py::arg("k_weight"), py::arg("table"), py::arg("positions"),
+          py::arg("k_cache"), py::arg("v_cache"), py::arg("slots"), py::arg("eps"), py::arg("interleaved"));
+    m.def("qk_norm_rope_backward", &qk_norm_rope_backward, py::arg("dq"), py::arg("dk"), py::arg("q"), py::arg("k"), py::arg("q_weight"), py::arg("k_weight"), py::arg("table"),
+          py::arg("positions"), py::arg("eps"), py::arg("interleaved"));
     m.def("gemm_error", [](int device) { return gemm_error_flag(device).item<int>(); });
     m.def("get_dispatch_layout", &get_dispatch_layout);
     m.def("per_token_cast_to_fp8", &per_token_cast_to_fp8, py::arg("x"), py::arg("round_scale") = false,

@@ -116,4 +116,181 @@ inline std::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor>> attention_b
     return std::make_tuple(dq, dk, dv);
 }
 
+// What paged caches [pages, page_size, kv_heads, dim] have to be
+inline void check_caches(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& like, at::ScalarType type) {
+    for (const at::Tensor* t : {&k_cache, &v_cache})
+        TORCH_CHECK(t->device() == like.device() && t->scalar_type() == type && t->dim() == 4, "caches must be [pages, page_size, kv_heads, dim], of the type and on the device of the heads");
+    TORCH_CHECK(k_cache.sizes() == v_cache.sizes() && k_cache.strides() == v_cache.strides(), "k_cache and v_cache must have one shape and one layout");
+    TORCH_CHECK(k_cache.size(1) >= 1 && k_cache.size(1) < (1 << 30) && k_cache.size(0) < (1ll << 31), "between 1 and 2^30 places per page, fewer than 2^31 pages");
+    TORCH_CHECK(k_cache.size(3) == 1 || k_cache.stride(3) == 1, "channels of the caches must be contiguous");
+    const int64_t per16 = 16 / k_cache.element_size();
+    for (int i = 0; i < 3; ++i) TORCH_CHECK(k_cache.stride(i) % per16 == 0, "heads of the caches must start on 16 bytes");
+    for (const at::Tensor* t : {&k_cache, &v_cache}) TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "heads of the caches must start on 16 bytes");
+}
+
+inline at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& page_table, const at::Tensor& lengths, double scale,
+                                  const std::optional<at::Tensor>& out) {
+    TORCH_CHECK(q.is_cuda() && q.dim() == 3 && q.scalar_type() == at::kBFloat16, "q must be bf16 [sequences, heads, dim] on a GPU");
+    const c10::cuda::CUDAGuard guard(q.device());
+    check_caches(k_cache, v_cache, q, at::kBFloat16);
+    const int64_t B = q.size(0), H = q.size(1), D = q.size(2), Hk = k_cache.size(2);
+    TORCH_CHECK(D >= 8 && D <= 128 && D % 8 == 0 && k_cache.size(3) == D, "heads must have 8 to 128 channels, a multiple of 8, in q and the caches alike");
+    TORCH_CHECK(H >= 1 && H < (1 << 16) && Hk >= 1 && H % Hk == 0, "the heads of q must be a multiple of those of the caches");
+    TORCH_CHECK(B <= EP_MAX_PAGED_SEQS, "at most ", EP_MAX_PAGED_SEQS, " sequences");
+    TORCH_CHECK(page_table.device() == q.device() && page_table.scalar_type() == at::kInt && page_table.dim() == 2 && page_table.size(0) == B &&
+                    (page_table.size(1) <= 1 || page_table.stride(1) == 1) && page_table.size(1) < (1ll << 31),
+                "page_table must be int32 [sequences, pages] with contiguous rows on the device of q");
+    TORCH_CHECK(lengths.device() == q.device() && lengths.scalar_type() == at::kInt && lengths.dim() == 1 && lengths.size(0) == B && lengths.is_contiguous(),
+                "lengths must be contiguous int32 [sequences] on the device of q");
+    TORCH_CHECK(B * (page_table.size(1) * k_cache.size(1) / 64 + 1) < (1ll << 31), "too many places in page_table");
+    TORCH_CHECK(std::isfinite(scale) && scale > 0, "scale must be positive");
+    at::Tensor o = out.has_value() ? *out : at::empty(q.sizes(), q.options());
+    TORCH_CHECK(o.device() == q.device() && o.scalar_type() == at::kBFloat16 && o.is_contiguous() && o.sizes() == q.sizes() && reinterpret_cast<uintptr_t>(o.data_ptr()) % 16 == 0,
+                "out must be contiguous bf16 of q's shape, on 16 bytes");
+    if (B == 0) return o;
+    const at::Tensor q16 = heads_of(q);
+    PagedAttentionArgs a{};
+    a.q = view_of(q16);
+    a.k_cache = k_cache.data_ptr();
+    a.v_cache = v_cache.data_ptr();
+    a.stride_page = k_cache.stride(0);
+    a.stride_slot = k_cache.stride(1);
+    a.stride_head = k_cache.stride(2);
+    a.num_pages = k_cache.size(0);
+    a.page_size = static_cast<int>(k_cache.size(1));
+    a.page_table = page_table.data_ptr<int>();
+    a.table_pitch = page_table.stride(0);
+    a.table_width = static_cast<int>(page_table.size(1));
+    a.lengths = lengths.data_ptr<int>();
+    a.num_seqs = static_cast<int>(B);
+    a.heads = static_cast<int>(H);
+    a.kv_heads = static_cast<int>(Hk);
+    a.dim = static_cast<int>(D);
+    a.scale = static_cast<float>(scale);
+    a.o = o.data_ptr();
+    at::Tensor parts;
+    if (const int64_t bytes = ep::paged_attention_workspace(a, device_sms()); bytes > 0) {
+        parts = at::empty({bytes}, q.options().dtype(at::kByte));
+        a.parts = reinterpret_cast<float*>(parts.data_ptr());
+    }
+    cuda_check(ep::launch_paged_attention(a, device_sms(), at::cuda::getCurrentCUDAStream()), "paged attention launch");
+    return o;
+}
+
+// ------------------------------------------------------------------------------------------------ norm and rotation of heads
+struct RotaryInputs {
+    at::Tensor q, k, weight[2], table, positions;      // as the kernels read them
+    RotaryArgs a{};
+};
+inline at::Tensor on16(const at::Tensor& t) { return t.is_contiguous() && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 ? t : t.clone(at::MemoryFormat::Contiguous); }
+inline RotaryInputs rotary_inputs(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_weight, const at::Tensor& k_weight, const at::Tensor& table, const at::Tensor& positions,
+                                  double eps, bool interleaved) {
+    for (const at::Tensor* t : {&q, &k})
+        TORCH_CHECK(t->is_cuda() && t->device() == q.device() && t->dim() == 3 && is_bf16_or_f32(*t) && t->scalar_type() == q.scalar_type(),
+                    "q and k must be bf16 or fp32 [tokens, heads, dim], of one type on one GPU");
+    const int64_t T = q.size(0), D = q.size(2);
+    TORCH_CHECK(k.size(0) == T && k.size(2) == D, "q and k must have the same tokens and channels");
+    TORCH_CHECK(D >= 8 && D <= 256 && D % 8 == 0, "heads must have 8 to 256 channels, a multiple of 8");
+    TORCH_CHECK(q.size(1) < (1 << 16) && k.size(1) < (1 << 16) && T < (1ll << 31) && T * (q.size(1) + 2 * k.size(1)) < (1ll << 33), "too many tokens or heads");
+    for (const at::Tensor* t : {&q_weight, &k_weight})
+        TORCH_CHECK(t->device() == q.device() && is_bf16_or_f32(*t) && t->scalar_type() == q_weight.scalar_type() && t->dim() == 1 && t->size(0) == D,
+                    "weights must be bf16 or fp32 [dim], of one type, on the device of q");
+    TORCH_CHECK(table.device() == q.device() && table.scalar_type() == at::kFloat && table.dim() == 2 && table.size(1) <= D && table.size(1) % 16 == 0,
+                "table must be fp32 [positions, rotated channels], a multiple of 16 of at most dim, on the device of q");
+    TORCH_CHECK(positions.device() == q.device() && positions.dim() == 1 && positions.size(0) == T && (positions.scalar_type() == at::kLong || positions.scalar_type() == at::kInt),
+                "positions must be int64 or int32 [tokens] on the device of q");
+    RotaryInputs in;
+    in.q = heads_of(q);
+    in.k = heads_of(k);
+    in.weight[0] = on16(q_weight);
+    in.weight[1] = on16(k_weight);
+    in.table = on16(table);
+    in.positions = positions.contiguous();
+    RotaryArgs& a = in.a;
+    a.x[0] = view_of(in.q);
+    a.x[1] = view_of(in.k);
+    a.heads[0] = static_cast<int>(q.size(1));
+    a.heads[1] = static_cast<int>(k.size(1));
+    for (int i = 0; i < 2; ++i) a.weight[i] = in.weight[i].data_ptr();
+    a.tokens = static_cast<int>(T);
+    a.dim = static_cast<int>(D);
+    a.rotary = static_cast<int>(table.size(1));
+    a.x_bf16 = q.scalar_type() == at::kBFloat16;
+    a.param_bf16 = q_weight.scalar_type() == at::kBFloat16;
+    a.interleaved = interleaved;
+    a.table = in.table.data_ptr<float>();
+    a.num_positions = table.size(0);
+    a.positions = in.positions.data_ptr();
+    a.positions_64 = in.positions.scalar_type() == at::kLong;
+    a.eps = static_cast<float>(eps);
+    return in;
+}
+// (nothing where a kernel is not to run, as of the norm)
+inline std::optional<std::tuple<at::Tensor, at::Tensor>> qk_norm_rope(const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_weight, const at::Tensor& k_weight,
+                                                                      const at::Tensor& table, const at::Tensor& positions, double eps, bool interleaved) {
+    if (not_for_a_kernel({&q, &k, &q_weight, &k_weight, &table}) || watched({&positions})) return std::nullopt;
+    const c10::cuda::CUDAGuard guard(q.device());
+    RotaryInputs in = rotary_inputs(q, k, q_weight, k_weight, table, positions, eps, interleaved);
+    at::Tensor yq = at::empty(q.sizes(), q.options()), yk = at::empty(k.sizes(), k.options());
+    if (q.size(0) == 0) return std::make_tuple(yq, yk);
+    in.a.out[0] = yq.data_ptr();
+    in.a.out[1] = yk.data_ptr();
+    cuda_check(ep::launch_rotary(in.a, device_sms(), at::cuda::getCurrentCUDAStream()), "rotation launch");
+    return std::make_tuple(yq, yk);
+}
+inline std::optional<at::Tensor> qk_norm_rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& q_weight, const at::Tensor& k_weight,
+                                                     const at::Tensor& table, const at::Tensor& positions, at::Tensor k_cache, at::Tensor v_cache, const at::Tensor& slots, double eps,
+                                                     bool interleaved) {
+    if (not_for_a_kernel({&q, &k, &v, &q_weight, &k_weight, &table, &k_cache, &v_cache}) || watched({&positions, &slots})) return std::nullopt;
+    const c10::cuda::CUDAGuard guard(q.device());
+    RotaryInputs in = rotary_inputs(q, k, q_weight, k_weight, table, positions, eps, interleaved);
+    TORCH_CHECK(v.device() == q.device() && v.scalar_type() == q.scalar_type() && v.sizes() == k.sizes(), "v must be like k");
+    check_caches(k_cache, v_cache, q, q.scalar_type());
+    TORCH_CHECK(k_cache.size(2) == k.size(1) && k_cache.size(3) == k.size(2), "the caches must have the heads and channels of k");
+    TORCH_CHECK(slots.device() == q.device() && slots.dim() == 1 && slots.size(0) == q.size(0) && (slots.scalar_type() == at::kLong || slots.scalar_type() == at::kInt),
+                "slots must be int64 or int32 [tokens] on the device of q");
+    at::Tensor yq = at::empty(q.sizes(), q.options());
+    if (q.size(0) == 0) return yq;
+    const at::Tensor v16 = heads_of(v), s = slots.contiguous();
+    RotaryArgs& a = in.a;
+    a.out[0] = yq.data_ptr();
+    a.v = view_of(v16);
+    a.k_cache = k_cache.data_ptr();
+    a.v_cache = v_cache.data_ptr();
+    a.stride_page = k_cache.stride(0);
+    a.stride_slot = k_cache.stride(1);
+    a.stride_head = k_cache.stride(2);
+    a.num_slots = k_cache.size(0) * k_cache.size(1);
+    a.page_size = static_cast<int>(k_cache.size(1));
+    a.slots = s.data_ptr();
+    a.slots_64 = s.scalar_type() == at::kLong;
+    cuda_check(ep::launch_rotary(a, device_sms(), at::cuda::getCurrentCUDAStream()), "rotation launch");
+    return yq;
+}
+using RotaryGradients = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+inline std::optional<RotaryGradients> qk_norm_rope_backward(const at::Tensor& dq, const at::Tensor& dk, const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_weight,
+                                                            const at::Tensor& k_weight, const at::Tensor& table, const at::Tensor& positions, double eps, bool interleaved) {
+    if (not_for_a_kernel({&dq, &dk, &q, &k, &q_weight, &k_weight, &table}) || watched({&positions})) return std::nullopt;
+    const c10::cuda::CUDAGuard guard(q.device());
+    RotaryInputs in = rotary_inputs(q, k, q_weight, k_weight, table, positions, eps, interleaved);
+    TORCH_CHECK(dq.device() == q.device() && dq.scalar_type() == q.scalar_type() && dq.sizes() == q.sizes() && dk.device() == q.device() && dk.scalar_type() == q.scalar_type() &&
+                    dk.sizes() == k.sizes(), "gradients must be like q and k");
+    at::Tensor dx = at::empty(q.sizes(), q.options()), dy = at::empty(k.sizes(), k.options());
+    at::Tensor dqw = at::empty(q_weight.sizes(), q_weight.options()), dkw = at::empty(k_weight.sizes(), k_weight.options());
+    if (q.size(0) == 0) return RotaryGradients(dx, dy, dqw.zero_(), dkw.zero_());
+    const at::Tensor dq16 = heads_of(dq), dk16 = heads_of(dk);
+    RotaryArgs& a = in.a;
+    a.dy[0] = view_of(dq16);
+    a.dy[1] = view_of(dk16);
+    a.out[0] = dx.data_ptr();
+    a.out[1] = dy.data_ptr();
+    a.dw[0] = dqw.data_ptr();
+    a.dw[1] = dkw.data_ptr();
+    a.ctas = ep::rotary_backward_ctas(a, device_sms());
+    at::Tensor partial = at::empty({a.ctas, 2, a.dim}, table.options());
+    a.partial = partial.data_ptr<float>();
+    cuda_check(ep::launch_rotary_backward(a, at::cuda::getCurrentCUDAStream()), "rotation gradient launch");
+    return RotaryGradients(dx, dy, dqw, dkw);
+}
+
 }  // namespace ep_host

@@ -77,32 +77,55 @@ def attention_backward(d_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: t
     return attention_backward_ref(d_o, q, k, v, o, lse, cu_q, cu_k, causal, scale, d_lse)
 
 
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, scale: Optional[float] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One new token per sequence: ``q [sequences, heads, dim]`` (bf16, ``dim`` a multiple of 8, at most 128; at most 4096 sequences) over the keys and values of a paged cache,
+    ``k_cache`` and ``v_cache [pages, page_size, kv_heads, dim]`` (as :func:`ops.rotary.qk_norm_rope_append` fills them) -> ``o`` like ``q``, contiguous, or ``out``.
+
+    Sequence ``i`` has ``lengths[i]`` keys (int32), the new token's own among them; key ``p`` stands in place ``p % page_size`` of page ``page_table[i, p // page_size]``
+    (int32 ``[sequences, at least as many pages]``).  Places behind the length are not looked at, nor are the table's.  A sequence without keys gets zeros; one that names a page which
+    the caches do not have, or is longer than its row of the table, gets no numbers (NaN), and nothing is read for it.  ``heads``, ``kv_heads`` and ``scale``: see
+    :func:`attention`.  How the work is cut depends on the lengths of the whole batch: the last bits of a result can change with the batch that it is in.
+
+    Carries no gradient of its own: where one is wanted, and for whoever watches, the PyTorch statement runs."""
+    scale = q.shape[-1]**-0.5 if scale is None else float(scale)
+    if q.is_cuda and _by_type(q, k_cache, v_cache, page_table, lengths, out):
+        res = _native.load().paged_attention(q, k_cache, v_cache, page_table, lengths, scale, out)
+        if res is not None:
+            return res
+    o = paged_attention_ref(q, k_cache, v_cache, page_table, lengths, scale)
+    return o if out is None else out.copy_(o)
+
+
 def _wide(t: torch.Tensor) -> torch.Tensor:
     return t if t.dtype == torch.float64 else t.float()
 
 
-def _sees(q, k, cu_q, cu_k, causal: bool) -> torch.Tensor:
-    """``[tokens, keys]``: whether a query sees a key."""
-    def place(t, cu):
-        at = torch.arange(t.shape[0], device=t.device)
-        if cu is None:
-            return torch.zeros_like(at), at, torch.full_like(at, t.shape[0])
-        cu = cu.long()
-        seq = (torch.searchsorted(cu, at, right=True) - 1).clamp(0, max(cu.numel() - 2, 0))
-        if cu.numel() < 2:
-            return torch.full_like(at, -1), at, at
-        inside = (at >= cu[seq]) & (at < cu[seq + 1])
-        return torch.where(inside, seq, -1), at - cu[seq], cu[seq + 1] - cu[seq]
-    (sq, iq, nq), (sk, ik, nk) = place(q, cu_q), place(k, cu_k)
-    sees = (sq[:, None] == sk) & (sq >= 0)[:, None]
-    return sees & (ik - nk <= (iq - nq)[:, None]) if causal else sees
+def _places(t, cu):
+    """Of every row: its sequence (-1: none), its place there, the sequence's length."""
+    at = torch.arange(t.shape[0], device=t.device)
+    if cu is None:
+        return torch.zeros_like(at), at, torch.full_like(at, t.shape[0])
+    if cu.numel() < 2:
+        return torch.full_like(at, -1), at, at
+    cu = cu.long()
+    seq = (torch.searchsorted(cu, at, right=True) - 1).clamp(0, cu.numel() - 2)
+    return torch.where((at >= cu[seq]) & (at < cu[seq + 1]), seq, -1), at - cu[seq], cu[seq + 1] - cu[seq]
+
+
+def _of_sequences(t, cu):
+    """``t`` in 32 bits (64 if it has them), zeros in rows of no sequence."""
+    return torch.where((_places(t, cu)[0] >= 0)[:, None, None], _wide(t), 0.0)
 
 
 def _scores(q, k, cu_q, cu_k, causal, scale):
-    group = q.shape[1] // k.shape[1]
-    s = torch.einsum('ihd,jhd->hij', _wide(q), _wide(k).repeat_interleave(group, 1)) * scale
-    sees = _sees(q, k, cu_q, cu_k, causal)
-    return torch.where(sees, s, float('-inf')), sees, group
+    """``q`` and, for every query head, ``k`` in 32 bits; scores ``[heads, tokens, keys]`` and whether a query sees a key."""
+    (sq, iq, nq), (sk, ik, nk) = _places(q, cu_q), _places(k, cu_k)
+    sees = (sq[:, None] == sk) & (sq >= 0)[:, None]
+    if causal:
+        sees = sees & (ik - nk <= (iq - nq)[:, None])
+    q, k = _of_sequences(q, cu_q), _of_sequences(k, cu_k).repeat_interleave(int(q.shape[1]) // int(k.shape[1]), 1)
+    return q, k, torch.where(sees, torch.einsum('ihd,jhd->hij', q, k) * scale, float('-inf')), sees
 
 
 def attention_ref(q, k, v, cu_seqlens=None, cu_seqlens_k=None, causal=True, scale=None):
@@ -110,13 +133,13 @@ def attention_ref(q, k, v, cu_seqlens=None, cu_seqlens_k=None, causal=True, scal
     cu_q, cu_k, scale = _options(q, cu_seqlens, cu_seqlens_k, scale)
     if k.shape[0] == 0:
         return torch.zeros_like(q), _wide(q).new_full((q.shape[1], q.shape[0]), float('-inf'))
-    s, sees, group = _scores(q, k, cu_q, cu_k, causal, scale)
+    _, _, s, sees = _scores(q, k, cu_q, cu_k, causal, scale)
     some = sees.any(-1)
     top = torch.where(some, s.max(-1).values, 0.0).detach()
     e = torch.exp(s - top.unsqueeze(-1))
     total = torch.where(some, e.sum(-1), 1.0)
-    o = torch.einsum('hij,jhd->ihd', e / total.unsqueeze(-1), _wide(v).repeat_interleave(group, 1))
-    return o.to(q.dtype), torch.where(some, top + torch.log(total), float('-inf'))
+    o = torch.einsum('hij,jhd->ihd', e / total.unsqueeze(-1), _of_sequences(v, cu_k).repeat_interleave(int(q.shape[1]) // int(k.shape[1]), 1))
+    return o.to(q.dtype).contiguous(), torch.where(some, top + torch.log(total), float('-inf'))
 
 
 def attention_backward_ref(d_o, q, k, v, o, lse, cu_seqlens=None, cu_seqlens_k=None, causal=True, scale=None, d_lse=None):
@@ -124,16 +147,40 @@ def attention_backward_ref(d_o, q, k, v, o, lse, cu_seqlens=None, cu_seqlens_k=N
     cu_q, cu_k, scale = _options(q, cu_seqlens, cu_seqlens_k, scale)
     if k.shape[0] == 0:
         return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
-    s, sees, group = _scores(q, k, cu_q, cu_k, causal, scale)
-    p = torch.where(sees, torch.exp(s - torch.where(sees.any(-1), lse, 0.0).unsqueeze(-1)), 0.0)
-    g = _wide(d_o)
-    dp = torch.einsum('ihd,jhd->hij', g, _wide(v).repeat_interleave(group, 1))
-    delta = (g * _wide(o)).sum(-1).t()
+    shape = (k.shape[0], k.shape[1], int(q.shape[1]) // int(k.shape[1]), k.shape[2])      # (numbers while tracing, too)
+    types = q.dtype, k.dtype, v.dtype
+    q, k, s, sees = _scores(q, k, cu_q, cu_k, causal, scale)
+    some = sees.any(-1)
+    p = torch.where(sees, torch.exp(s - torch.where(some, lse, 0.0).unsqueeze(-1)), 0.0)
+    g = _of_sequences(d_o, cu_q)
+    dp = torch.einsum('ihd,jhd->hij', g, _of_sequences(v, cu_k).repeat_interleave(shape[2], 1))
+    delta = (g * _of_sequences(o, cu_q)).sum(-1).t()
     if d_lse is not None:
-        delta = delta - d_lse
+        delta = delta - torch.where(some, d_lse, 0.0)
     ds = torch.where(sees, p * (dp - delta.unsqueeze(-1)), 0.0) * scale
-    dq = torch.einsum('hij,jhd->ihd', ds, _wide(k).repeat_interleave(group, 1))
-    shape = (k.shape[0], k.shape[1], group, k.shape[2])
-    dk = torch.einsum('hij,ihd->jhd', ds, _wide(q)).view(shape).sum(2)
-    dv = torch.einsum('hij,ihd->jhd', p, g).view(shape).sum(2)
-    return dq.to(q.dtype), dk.to(k.dtype), dv.to(v.dtype)
+    dq = torch.einsum('hij,jhd->ihd', ds, k)
+    dk, dv = (torch.einsum('hij,ihd->jhd', x, y).reshape(shape).sum(2) for x, y in ((ds, q), (p, g)))
+    return tuple(t.to(dtype).contiguous() for t, dtype in zip((dq, dk, dv), types))
+
+
+def paged_attention_ref(q, k_cache, v_cache, page_table, lengths, scale=None):
+    """:func:`paged_attention` stated with plain PyTorch operations (any device; what the kernel is tested against).  All places of the table at once."""
+    scale = q.shape[-1]**-0.5 if scale is None else float(scale)
+    pages, size, kv_heads, dim = k_cache.shape
+    n, group = lengths.long(), q.shape[1] // kv_heads
+    at = torch.arange(page_table.shape[1] * size, device=q.device)
+    there = at < n[:, None]
+    page = page_table.long()[:, at // size]
+    bad = (there & ((page < 0) | (page >= pages))).any(-1) | (n > at.numel())
+    page, place = torch.where(there & (page >= 0) & (page < pages), page, 0), at % size
+    if pages == 0 or at.numel() == 0:
+        o = _wide(q).new_zeros(q.shape)
+    else:
+        k, v = (torch.where(there[:, :, None, None], _wide(c[page, place]), 0.0) for c in (k_cache, v_cache))
+        s = torch.einsum('bhgd,bjhd->bhgj', _wide(q).reshape(q.shape[0], kv_heads, group, dim), k) * scale
+        s = torch.where(there[:, None, None], s, float('-inf'))
+        top = torch.where(n[:, None, None] > 0, s.amax(-1), 0.0)
+        e = torch.exp(s - top.unsqueeze(-1))
+        e = e / torch.where(n[:, None, None] > 0, e.sum(-1), 1.0).unsqueeze(-1)
+        o = torch.einsum('bhgj,bjhd->bhgd', e, v).reshape(q.shape)
+    return torch.where(bad[:, None, None], float('nan'), o).to(q.dtype)
