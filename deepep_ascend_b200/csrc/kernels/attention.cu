@@ -124,13 +124,22 @@ __device__ __forceinline__ void clear_rows(const int32_t* cu, int num_seqs, int 
 // A tile of rows x 64 kChunks channels lies in shared memory as chunks of 64 channels, rows of 128 bytes with the 128-byte swizzle, as TMA writes them.  It is
 // an operand along its channels (K-major) and along its rows (MN-major: every channel a row of the operand) alike.
 template <int kRows>
-__device__ __forceinline__ uint64_t desc_channels(const uint8_t* tile, int k) {      // k-th 16 channels
-    return umma::advance_desc_k(umma::make_smem_desc_sw128(tile + (k >> 2) * kRows * 128), (k & 3) * 32);
-}
+__device__ __forceinline__ uint64_t desc_channels(const uint8_t* tile) { return umma::make_smem_desc_sw128(tile); }
 template <int kRows>
-__device__ __forceinline__ uint64_t desc_rows(const uint8_t* tile, int k) {          // k-th 16 rows
-    const uint64_t addr = ptx::smem_u32(tile) + k * 16 * 128;
-    return ((addr & 0x3ffffull) >> 4) | (static_cast<uint64_t>(kRows * 128 >> 4) << 16) | ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
+__device__ __forceinline__ uint64_t desc_rows(const uint8_t* tile) {
+    return ((static_cast<uint64_t>(ptx::smem_u32(tile)) & 0x3ffffull) >> 4) | (static_cast<uint64_t>(kRows * 128 >> 4) << 16) | ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// D (+)= A B over the channels / over kSteps * 16 rows.  Descriptors step by constants and loops are unrolled: the one thread that issues products has 64 clocks for each.
+template <int kRowsA, int kRowsB, int kChunks>
+__device__ __forceinline__ void multiply_channels(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int dim16) {
+#pragma unroll
+    for (int k = 0; k < 4 * kChunks; ++k)
+        if (k < dim16) umma::mma_ss<false>(d, a + ((k >> 2) * kRowsA * 128 + (k & 3) * 32) / 16, b + ((k >> 2) * kRowsB * 128 + (k & 3) * 32) / 16, idesc, k != 0);
+}
+template <int kFirst, int kSteps>
+__device__ __forceinline__ void multiply_rows(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+#pragma unroll
+    for (int k = kFirst; k < kFirst + kSteps; ++k) umma::mma_ts(d, a + k * 8, b + k * 16 * 128 / 16, idesc, add || k != 0);
 }
 template <int kRows, int kChunks>
 __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, int head, int row, uint64_t* bar) {
@@ -176,6 +185,32 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     return d;
 }
 constexpr float kNone = -__builtin_huge_valf();
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 2^x of a pair without the special function unit, which makes 16 a clock of an SM and would be what the softmax waits for: x = n + f with n the nearest whole number, 2^f
+// by a polynomial of degree 4 (relative error 2.8e-6, least largest error on [-1/2, 1/2] with a constant of exactly 1, so that -127 and below give exactly 0), n added
+// to the exponent.  A NaN stays one or becomes an infinity.
+__device__ __forceinline__ uint64_t exp2_by_polynomial(uint64_t x2) {
+    float x, y;
+    umma::unpack_f32x2(x2, x, y);
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(x));
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(y));
+    x2 = f32x2(x, y);
+    const uint64_t shift = f32x2(12582912.f, 12582912.f), back = f32x2(-12582912.f, -12582912.f), minus_one = f32x2(-1.f, -1.f);
+    const uint64_t n = add2(x2, shift), f = fma2(add2(n, back), minus_one, x2);
+    uint64_t p = fma2(f, f32x2(0.009585382388763709f, 0.009585382388763709f), f32x2(0.05590662825543393f, 0.05590662825543393f));
+    p = fma2(p, f, f32x2(0.24024038166610448f, 0.24024038166610448f));
+    p = fma2(p, f, f32x2(0.6931241843387045f, 0.6931241843387045f));
+    p = fma2(p, f, f32x2(1.f, 1.f));
+    float u, v, a, b;
+    umma::unpack_f32x2(p, u, v);
+    umma::unpack_f32x2(n, a, b);
+    return umma::pack_f32x2(__float_as_uint(u) + (__float_as_uint(a) << 23), __float_as_uint(v) + (__float_as_uint(b) << 23));
+}
+constexpr int kPolynomialOf = 4;                     // of so many pairs of a row one goes by the polynomial
 
 // The two groups of four warps that hold rows take registers of the third: 384 x 168 at launch = 128 x (232 + 232 + 40)
 __device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 232;"); }
@@ -205,7 +240,7 @@ __device__ __forceinline__ void store_row(uint32_t tmem, float factor, bf16* row
 // ------------------------------------------------------------------------------------------------ forward
 // A CTA takes 256 queries of a head as two tiles of 128, whose softmaxes (four warps each, a row per thread) and products alternate: while one tile's scores are made into
 // probabilities, the tensor cores work for the other.  Probabilities take the place of the scores in tensor memory, from where they are the first operand of the next product.
-constexpr int kFwdThreads = 384;                     // 2 x 4 warps for the softmaxes, one that requests tiles, one that issues products, two without work
+constexpr int kFwdThreads = 384;                     // 2 x 4 warps for the softmaxes, one that requests tiles, two that issue products, one without work
 template <int kChunks>
 struct FwdShape {
     static constexpr int kTileBytes = 128 * 128 * kChunks, kStages = kChunks == 2 ? 5 : 8;
@@ -213,7 +248,7 @@ struct FwdShape {
     static constexpr int kSmem = (2 + kStages) * kTileBytes + 1024;
 };
 struct FwdBars {
-    uint64_t q_full[2], full[8], empty[8], s_full[2], p_full[2], o_full[2], tail, quiet;
+    uint64_t q_full[2], full[8], empty[8], s_full[2], p_full[2][2], o_full[2], tail, quiet[2];
     AttnState st;
     int4 block;
 };
@@ -236,15 +271,17 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&b->q_full[i], 1);
             ptx::mbar_init(&b->s_full[i], 1);
-            ptx::mbar_init(&b->p_full[i], 4);
+            ptx::mbar_init(&b->p_full[i][0], 4);
+            ptx::mbar_init(&b->p_full[i][1], 4);
             ptx::mbar_init(&b->o_full[i], 1);
         }
         for (int i = 0; i < kStages; ++i) {
             ptx::mbar_init(&b->full[i], 1);
-            ptx::mbar_init(&b->empty[i], 1);
+            ptx::mbar_init(&b->empty[i], 2);
         }
         ptx::mbar_init(&b->tail, 1);
-        ptx::mbar_init(&b->quiet, 1);
+        ptx::mbar_init(&b->quiet[0], 1);
+        ptx::mbar_init(&b->quiet[1], 1);
         b->st.failed = 0;
         ptx::mbar_fence_init();
     }
@@ -307,51 +344,53 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 for (int j = 0; j < blocks; ++j)
                     if (!request(&map_k, j, false) || !request(&map_v, j, true)) break;
             }
-        } else if (warp == 9) {
+        } else if (warp < 11) {
+            // a tile's products; what neither tile reads any more is free
+            const int t = warp - 9;
             if (ptx::elect_one() && blocks > 0) {
-                const int dim16 = (a.dim + 15) / 16;
-                const uint32_t idesc_s = umma::make_instr_desc(128, 128, umma::kFormatBF16);
+                const int dim16 = (a.dim + 15) / 16, mine = n[t];
+                const uint32_t idesc_s = umma::make_instr_desc(128, 128, umma::kFormatBF16), to_s = tmem + t * 128, to_o = tmem + Shape::kOut + t * 128;
                 const uint32_t idesc_o = umma::make_instr_desc(128, 16, umma::kFormatBF16, false, true) + (static_cast<uint32_t>(2 * dim16 - 2) << 17);
-                auto scores = [&](int t, const uint8_t* tile) {
-                    for (int k = 0; k < dim16; ++k)
-                        umma::mma_ss<false>(tmem + t * 128, desc_channels<128>(sq + t * kTileBytes, k), desc_channels<128>(tile, k), idesc_s, k != 0);
-                    umma::mma_commit(&b->s_full[t]);
+                const uint64_t queries = desc_channels<128>(sq + t * kTileBytes), keys_of = desc_channels<128>(skv), values_of = desc_rows<128>(skv);
+                auto free_stage = [&](int stage, bool read) {
+                    if (read) umma::mma_commit(&b->empty[stage]);
+                    else ptx::mbar_arrive(&b->empty[stage]);
                 };
                 AttnRing<kStages> p;
+                auto scores = [&]() {
+                    umma::fence_after_thread_sync();
+                    multiply_channels<128, 128, kChunks>(to_s, queries, keys_of + p.stage * (kTileBytes / 16), idesc_s, dim16);
+                    umma::mma_commit(&b->s_full[t]);
+                };
                 auto multiply = [&]() {
                     if (!attn_wait(&b->full[0], 0, failed, a.report, 4)) return;
-                    for (int t = 0; t < 2; ++t)
-                        if (n[t] > 0) {
-                            if (!attn_wait(&b->q_full[t], 0, failed, a.report, 4)) return;
-                            umma::fence_after_thread_sync();
-                            scores(t, skv);
-                        }
-                    umma::mma_commit(&b->empty[0]);
+                    if (mine > 0) {
+                        if (!attn_wait(&b->q_full[t], 0, failed, a.report, 4)) return;
+                        scores();
+                    }
+                    free_stage(0, mine > 0);
                     p.advance();
                     for (int j = 0; j < blocks; ++j) {
+                        // (the values, and the next keys, have mostly long been there)
                         const int stage_v = p.stage;
+                        const uint64_t values = values_of + stage_v * (kTileBytes / 16);
                         if (!attn_wait(&b->full[stage_v], p.phase, failed, a.report, 4)) return;
                         p.advance();
-                        bool have_k = false;
-                        for (int t = 0; t < 2; ++t) {
-                            if (j >= n[t]) continue;
-                            if (!attn_wait(&b->p_full[t], j & 1, failed, a.report, 2)) return;
+                        if (j + 1 < blocks && !attn_wait(&b->full[p.stage], p.phase, failed, a.report, 4)) return;
+                        if (j < mine) {
+                            // the first half of the probabilities as soon as it is there
+                            if (!attn_wait(&b->p_full[t][0], j & 1, failed, a.report, 2)) return;
                             umma::fence_after_thread_sync();
-#pragma unroll
-                            for (int k = 0; k < 8; ++k)
-                                umma::mma_ts(tmem + Shape::kOut + t * 128, tmem + t * 128 + k * 8, desc_rows<128>(skv + stage_v * kTileBytes, k), idesc_o, j != 0 || k != 0);
-                            if (j + 1 == n[t]) {
-                                umma::mma_commit(&b->o_full[t]);
-                            } else {
-                                if (!have_k && !attn_wait(&b->full[p.stage], p.phase, failed, a.report, 4)) return;
-                                have_k = true;
-                                umma::fence_after_thread_sync();
-                                scores(t, skv + p.stage * kTileBytes);
-                            }
+                            multiply_rows<0, 4>(to_o, to_s, values, idesc_o, j != 0);
+                            if (!attn_wait(&b->p_full[t][1], j & 1, failed, a.report, 2)) return;
+                            umma::fence_after_thread_sync();
+                            multiply_rows<4, 4>(to_o, to_s, values, idesc_o, true);
+                            if (j + 1 < mine) scores();
+                            else umma::mma_commit(&b->o_full[t]);
                         }
-                        umma::mma_commit(&b->empty[stage_v]);
-                        if (have_k) {
-                            umma::mma_commit(&b->empty[p.stage]);
+                        free_stage(stage_v, j < mine);
+                        if (j + 1 < blocks) {
+                            free_stage(p.stage, j + 1 < mine);
                             p.advance();
                         }
                     }
@@ -373,23 +412,68 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             if (!ok) break;
             umma::fence_after_thread_sync();
             uint32_t s[4][32];
+            const bool masked = j * 128 + 128 > first_seen;
+            const int visible = seen - j * 128;
+            uint32_t out[32];
+            uint64_t part[2];
+            // 16 scores at a time, in an order that keeps the special function unit fed: scaled two steps ahead, summed and rounded a step behind
+            auto scaled = [&](int i) {
+                const uint64_t c2 = f32x2(c, c), minus = f32x2(-ref * c, -ref * c);
+#pragma unroll
+                for (int k = i * 16; k < i * 16 + 16; k += 2) {
+                    float x, y;
+                    umma::unpack_f32x2(fma2(umma::pack_f32x2(s[k >> 5][k & 31], s[k >> 5][(k & 31) + 1]), c2, minus), x, y);
+                    s[k >> 5][k & 31] = __float_as_uint(x);
+                    s[k >> 5][(k & 31) + 1] = __float_as_uint(y);
+                }
+            };
+            auto powers = [&](int i) {
+#pragma unroll
+                for (int k = i * 16; k < i * 16 + 16; k += 2) {
+                    uint32_t &x = s[k >> 5][k & 31], &y = s[k >> 5][(k & 31) + 1];
+                    if ((k >> 1) % kPolynomialOf == kPolynomialOf - 1) {
+                        float u, v;
+                        umma::unpack_f32x2(exp2_by_polynomial(umma::pack_f32x2(x, y)), u, v);
+                        x = __float_as_uint(u);
+                        y = __float_as_uint(v);
+                    } else {
+                        x = __float_as_uint(exp2_approx(__uint_as_float(x)));
+                        y = __float_as_uint(exp2_approx(__uint_as_float(y)));
+                    }
+                }
+            };
+            auto rounded = [&](int i) {
+#pragma unroll
+                for (int k = i * 16; k < i * 16 + 16; k += 2) {
+                    const uint32_t x = s[k >> 5][k & 31], y = s[k >> 5][(k & 31) + 1];
+                    part[(k >> 1) & 1] = add2(part[(k >> 1) & 1], umma::pack_f32x2(x, y));
+                    out[(k & 63) >> 1] = pack_bf16(__uint_as_float(x), __uint_as_float(y));
+                }
+            };
+            auto hand_over = [&](int i) {
+                umma::tmem_st_32x32(ts + i * 32, out);
+                umma::tmem_st_wait();
+                umma::fence_before_thread_sync();
+                __syncwarp();
+                if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->p_full[t][i]);
+            };
 #pragma unroll
             for (int i = 0; i < 4; ++i) umma::tmem_ld_32x32(ts + i * 32, s[i]);
             umma::tmem_ld_wait();
-            if (j * 128 + 128 > first_seen) {
-                const int visible = seen - j * 128;
+            if (masked)
 #pragma unroll
-                for (int i = 0; i < 128; ++i)
-                    if (i >= visible) s[i >> 5][i & 31] = 0xff800000u;
+                for (int k = 0; k < 128; ++k)
+                    if (k >= visible) s[k >> 5][k & 31] = 0xff800000u;
+            float top[8];                             // (many short chains)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                auto value = [&](int k) { return __uint_as_float(s[i >> 1][(i & 1) * 16 + k]); };
+                top[i] = max3(value(0), value(1), value(2));
+#pragma unroll
+                for (int k = 3; k < 15; k += 2) top[i] = max3(top[i], value(k), value(k + 1));
+                top[i] = fmaxf(top[i], value(15));
             }
-            float top[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                top[i] = __uint_as_float(s[i][0]);
-#pragma unroll
-                for (int k = 1; k < 32; ++k) top[i] = fmaxf(top[i], __uint_as_float(s[i][k]));
-            }
-            const float largest = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            const float largest = fmaxf(max3(max3(top[0], top[1], top[2]), top[3], top[4]), max3(top[5], top[6], top[7]));
             // The reference moves only when the largest score is more than 2^8 above it: sums and probabilities have that much room, and O is seldom multiplied.
             if (j == 0) {
                 ref = largest == kNone ? 0.f : largest;
@@ -400,39 +484,33 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     sum *= factor;
                     ref = move ? largest : ref;
 #pragma unroll
-                    for (int i = 0; i < 64 * kChunks; i += 32) {
-                        uint32_t o[32];
-                        umma::tmem_ld_32x32(to + i, o);
+                    for (int i = 0; i < 64 * kChunks; i += 16) {
+                        uint32_t o[16];
+                        umma::tmem_ld_32x16(to + i, o);
                         umma::tmem_ld_wait();
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
-                        umma::tmem_st_32x32(to + i, o);
+                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
+                        umma::tmem_st_32x16(to + i, o);
                     }
                 }
             }
-            const uint64_t c2 = f32x2(c, c), minus = f32x2(-ref * c, -ref * c);
-            uint64_t part[2] = {f32x2(sum, 0.f), f32x2(0.f, 0.f)};
+            part[0] = f32x2(sum, 0.f);
+            part[1] = f32x2(0.f, 0.f);
+            scaled(0);
+            scaled(1);
+            powers(0);
 #pragma unroll
-            for (int i = 0; i < 4; i += 2) {
-                uint32_t out[32];
-#pragma unroll
-                for (int k = 0; k < 64; k += 2) {
-                    float x, y;
-                    umma::unpack_f32x2(fma2(umma::pack_f32x2(s[i + (k >> 5)][k & 31], s[i + (k >> 5)][(k & 31) + 1]), c2, minus), x, y);
-                    x = exp2_approx(x);
-                    y = exp2_approx(y);
-                    part[(k >> 1) & 1] = add2(part[(k >> 1) & 1], f32x2(x, y));
-                    out[k >> 1] = pack_bf16(x, y);
-                }
-                umma::tmem_st_32x32(ts + i * 16, out);
+            for (int i = 1; i < 8; ++i) {
+                if (i < 7) scaled(i + 1);
+                powers(i);
+                rounded(i - 1);
+                if (i == 4) hand_over(0);
             }
+            rounded(7);
+            hand_over(1);
             float u, v;
             umma::unpack_f32x2(add2(part[0], part[1]), u, v);
             sum = u + v;
-            umma::tmem_st_wait();
-            umma::fence_before_thread_sync();
-            __syncwarp();
-            if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->p_full[t]);
         }
         const bool in = row < blk.rows;
         const int64_t token = blk.start + row;
@@ -458,9 +536,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 if (n[i] > 0) mbar_drain(&b->q_full[i], 0, 100000000ull);
             for (int i = 0; i < kStages; ++i) mbar_drain(&b->full[i], 0, 100000000ull), mbar_drain(&b->full[i], 1, 100000000ull);
         }
-        if (warp == 9 && ptx::elect_one()) {
-            umma::mma_commit(&b->quiet);
-            mbar_drain(&b->quiet, 0, 1000000000ull);
+        if ((warp == 9 || warp == 10) && ptx::elect_one()) {
+            umma::mma_commit(&b->quiet[warp - 9]);
+            mbar_drain(&b->quiet[warp - 9], 0, 1000000000ull);
         }
         __syncthreads();
     }
@@ -501,7 +579,7 @@ __global__ void __launch_bounds__(kDeltaThreads) attention_delta_kernel(const __
 // pieces of 64.  Scores and dP of a piece are products whose lanes are the kept rows, so that P and dS, written over them, are first operands of the products
 // that follow, and sums stay in tensor memory until the end: every gradient is added by one CTA, in a fixed order.  P is made twice, which costs two products of
 // seven, and spares sums of dQ in memory by many CTAs in any order.  Two groups of four warps take every other piece.
-constexpr int kBwdThreads = 384;                     // as in the forward pass
+constexpr int kBwdThreads = 384;                     // 2 x 4 warps for rows, one that requests pieces, one that issues products, two without work
 template <int kChunks>
 struct BwdShape {
     static constexpr int kKeptBytes = 128 * 128 * kChunks, kPieceBytes = 64 * 128 * kChunks, kStages = kChunks == 2 ? 4 : 6;
@@ -616,15 +694,15 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                 const int dim16 = (a.dim + 15) / 16;
                 const uint32_t idesc_s = umma::make_instr_desc(128, 64, umma::kFormatBF16);
                 const uint32_t idesc_o = umma::make_instr_desc(128, 16, umma::kFormatBF16, false, true) + (static_cast<uint32_t>(2 * dim16 - 2) << 17);
+                const uint64_t kept_of = desc_channels<128>(kept), pieces_of = desc_channels<64>(pieces), rows_of = desc_rows<64>(pieces);
                 AttnRing<kStages> p, q;                   // pieces whose scores are next, pieces whose sums are next
                 auto scores = [&](int i) {
                     if (!attn_wait(&b->full[p.stage], p.phase, failed, a.report, 4)) return false;
                     umma::fence_after_thread_sync();
-                    const uint8_t* tile = pieces + p.stage * 2 * kPieceBytes;
                     const uint32_t to = tmem + Shape::kBuffers + (i & 1) * 128;
-                    for (int k = 0; k < dim16; ++k) umma::mma_ss<false>(to, desc_channels<128>(kept, k), desc_channels<64>(tile, k), idesc_s, k != 0);
-                    for (int k = 0; k < dim16; ++k)
-                        umma::mma_ss<false>(to + 64, desc_channels<128>(kept + kKeptBytes, k), desc_channels<64>(tile + kPieceBytes, k), idesc_s, k != 0);
+                    const uint64_t piece = pieces_of + p.stage * (2 * kPieceBytes / 16);
+                    multiply_channels<128, 64, kChunks>(to, kept_of, piece, idesc_s, dim16);
+                    multiply_channels<128, 64, kChunks>(to + 64, kept_of + kKeptBytes / 16, piece + kPieceBytes / 16, idesc_s, dim16);
                     umma::mma_commit(&b->s_full[i & 1]);
                     p.advance();
                     return true;
@@ -635,13 +713,10 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                     for (int i = 0; i < n; ++i) {
                         if (!attn_wait(&b->p_full[i & 1], (i >> 1) & 1, failed, a.report, 2)) return;
                         umma::fence_after_thread_sync();
-                        const uint8_t* tile = pieces + q.stage * 2 * kPieceBytes;
                         const uint32_t from = tmem + Shape::kBuffers + (i & 1) * 128;
-                        if (kKeys)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) umma::mma_ts(tmem + 128, from + k * 8, desc_rows<64>(tile + kPieceBytes, k), idesc_o, i != 0 || k != 0);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) umma::mma_ts(tmem, from + 64 + k * 8, desc_rows<64>(tile, k), idesc_o, i != 0 || k != 0);
+                        const uint64_t piece = rows_of + q.stage * (2 * kPieceBytes / 16);
+                        if (kKeys) multiply_rows<0, 4>(tmem + 128, from, piece + kPieceBytes / 16, idesc_o, i != 0);
+                        multiply_rows<0, 4>(tmem, from + 64, piece, idesc_o, i != 0);
                         umma::mma_commit(&b->empty[q.stage]);
                         q.advance();
                         if (i + 2 < n && !scores(i + 2)) return;
