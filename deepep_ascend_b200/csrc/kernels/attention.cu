@@ -106,40 +106,40 @@ __device__ __forceinline__ AttnBlock find_block(const int32_t* cu, int num_seqs,
 template <int kRows>
 int64_t num_blocks(int64_t total, int64_t num_seqs) { return total / kRows + num_seqs; }
 
-// The first kThreads threads: rows that belong to no sequence get zeros (and -inf), this CTA's part of them
+// kThreads threads: rows that belong to no sequence get zeros (and -inf), one of `parts` of them
 template <int kThreads>
-__device__ __forceinline__ void clear_rows(const int32_t* cu, int num_seqs, int total, bf16* out, int64_t row_values, float* lse, int heads) {
+__device__ __forceinline__ void clear_rows(const int32_t* cu, int num_seqs, int total, int part, int parts, bf16* out, int64_t row_values, float* lse, int heads) {
     if (cu == nullptr) return;
     const int first = min(max(cu[0], 0), total), last = min(max(cu[num_seqs], first), total);
     const int missing = first + total - last;
-    for (int i = blockIdx.x; i < missing; i += gridDim.x) {
+    for (int i = part; i < missing; i += parts) {
         const int row = i < first ? i : last + i - first;
-        for (int64_t c = threadIdx.x; c < row_values / 8; c += kThreads) reinterpret_cast<uint4*>(out + row * row_values)[c] = make_uint4(0, 0, 0, 0);
+        for (int64_t c = threadIdx.x % kThreads; c < row_values / 8; c += kThreads) reinterpret_cast<uint4*>(out + row * row_values)[c] = make_uint4(0, 0, 0, 0);
         if (lse != nullptr)
-            for (int h = threadIdx.x; h < heads; h += kThreads) lse[static_cast<int64_t>(h) * total + row] = __int_as_float(0xff800000);
+            for (int h = threadIdx.x % kThreads; h < heads; h += kThreads) lse[static_cast<int64_t>(h) * total + row] = __int_as_float(0xff800000);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ operands
 // A tile of rows x 64 kChunks channels lies in shared memory as chunks of 64 channels, rows of 128 bytes with the 128-byte swizzle, as TMA writes them.  It is
 // an operand along its channels (K-major) and along its rows (MN-major: every channel a row of the operand) alike.
+// Lower halves of the descriptors (the upper ones, of eight rows per 1024 bytes, are all alike)
+__device__ __forceinline__ uint32_t desc_channels(const uint8_t* tile) { return (ptx::smem_u32(tile) & 0x3ffffu) >> 4 | 1u << 16; }
 template <int kRows>
-__device__ __forceinline__ uint64_t desc_channels(const uint8_t* tile) { return umma::make_smem_desc_sw128(tile); }
-template <int kRows>
-__device__ __forceinline__ uint64_t desc_rows(const uint8_t* tile) {
-    return ((static_cast<uint64_t>(ptx::smem_u32(tile)) & 0x3ffffull) >> 4) | (static_cast<uint64_t>(kRows * 128 >> 4) << 16) | ((1024ull >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
+__device__ __forceinline__ uint32_t desc_rows(const uint8_t* tile) { return (ptx::smem_u32(tile) & 0x3ffffu) >> 4 | static_cast<uint32_t>(kRows * 128 >> 4) << 16; }
+__device__ __forceinline__ uint64_t desc_of(uint32_t low) { return static_cast<uint64_t>((1024u >> 4) | 1u << 14 | 2u << 29) << 32 | low; }
 // D (+)= A B over the channels / over kSteps * 16 rows.  Descriptors step by constants and loops are unrolled: the one thread that issues products has 64 clocks for each.
 template <int kRowsA, int kRowsB, int kChunks>
-__device__ __forceinline__ void multiply_channels(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int dim16) {
+__device__ __forceinline__ void multiply_channels(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, int dim16) {
 #pragma unroll
     for (int k = 0; k < 4 * kChunks; ++k)
-        if (k < dim16) umma::mma_ss<false>(d, a + ((k >> 2) * kRowsA * 128 + (k & 3) * 32) / 16, b + ((k >> 2) * kRowsB * 128 + (k & 3) * 32) / 16, idesc, k != 0);
+        if (k < dim16)
+            umma::mma_ss<false>(d, desc_of(a + ((k >> 2) * kRowsA * 128 + (k & 3) * 32) / 16), desc_of(b + ((k >> 2) * kRowsB * 128 + (k & 3) * 32) / 16), idesc, k != 0);
 }
 template <int kFirst, int kSteps>
-__device__ __forceinline__ void multiply_rows(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void multiply_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
 #pragma unroll
-    for (int k = kFirst; k < kFirst + kSteps; ++k) umma::mma_ts(d, a + k * 8, b + k * 16 * 128 / 16, idesc, add || k != 0);
+    for (int k = kFirst; k < kFirst + kSteps; ++k) umma::mma_ts(d, a + k * 8, desc_of(b + k * 16 * 128 / 16), idesc, add || k != 0);
 }
 template <int kRows, int kChunks>
 __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, int head, int row, uint64_t* bar) {
@@ -212,9 +212,9 @@ __device__ __forceinline__ uint64_t exp2_by_polynomial(uint64_t x2) {
 }
 constexpr int kPolynomialOf = 4;                     // of so many pairs of a row one goes by the polynomial
 
-// The two groups of four warps that hold rows take registers of the third: 384 x 168 at launch = 128 x (232 + 232 + 40)
-__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 232;"); }
-__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 40;"); }
+// The two groups of four warps that hold rows take registers of the third: 384 x 168 at launch = 128 x (224 + 224 + 56)
+__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); }
+__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
 
 // A row of sums in tensor memory, times `factor`, as bf16
 template <int kColumns>
@@ -224,34 +224,69 @@ __device__ __forceinline__ void store_row(uint32_t tmem, float factor, bf16* row
         uint32_t r[32];
         umma::tmem_ld_32x32(tmem + c, r);
         umma::tmem_ld_wait();
+        uint32_t v[16];
 #pragma unroll
-        for (int i = 0; i < 32; i += 8)
-            if (write && c + i < dim) {
-                uint4 v;
-                v.x = pack_bf16(__uint_as_float(r[i]) * factor, __uint_as_float(r[i + 1]) * factor);
-                v.y = pack_bf16(__uint_as_float(r[i + 2]) * factor, __uint_as_float(r[i + 3]) * factor);
-                v.z = pack_bf16(__uint_as_float(r[i + 4]) * factor, __uint_as_float(r[i + 5]) * factor);
-                v.w = pack_bf16(__uint_as_float(r[i + 6]) * factor, __uint_as_float(r[i + 7]) * factor);
-                *reinterpret_cast<uint4*>(row + c + i) = v;
-            }
+        for (int i = 0; i < 16; ++i) v[i] = pack_bf16(__uint_as_float(r[2 * i]) * factor, __uint_as_float(r[2 * i + 1]) * factor);
+        // (32 bytes at once, a sector, where rows start on them)
+        if (dim % 16 == 0) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 8)
+                if (write && c + 2 * i < dim)
+                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row + c + 2 * i), "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]),
+                                 "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+                                 : "memory");
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                if (write && c + 2 * i < dim) *reinterpret_cast<uint4*>(row + c + 2 * i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        }
     }
 }
 
 // ------------------------------------------------------------------------------------------------ forward
-// A CTA takes 256 queries of a head as two tiles of 128, whose softmaxes (four warps each, a row per thread) and products alternate: while one tile's scores are made into
+// A CTA takes two tiles of 128 queries that share keys and values, of two heads of a group or, where it has no second one, of one head, whose softmaxes (four warps each, a row per thread) and products alternate: while one tile's scores are made into
 // probabilities, the tensor cores work for the other.  Probabilities take the place of the scores in tensor memory, from where they are the first operand of the next product.
-constexpr int kFwdThreads = 384;                     // 2 x 4 warps for the softmaxes, one that requests tiles, two that issue products, one without work
+//
+// A CTA goes on with the work of CTAs that have not started (it cancels their launch and takes their place): barriers and tensor memory are set up once, and the next block's
+// queries, keys and values come while the last one's results leave.  Blocks differ in length, so who takes which is decided as they end.
+constexpr int kFwdThreads = 384;                     // 2 x 4 warps for the softmaxes, one that requests tiles, two that issue products, one that looks for work
+constexpr int kFwdReaders = 11;                      // ... of which so many do it
 template <int kChunks>
 struct FwdShape {
     static constexpr int kTileBytes = 128 * 128 * kChunks, kStages = kChunks == 2 ? 5 : 8;
     static constexpr int kOut = 256;                  // tensor memory: two tiles' scores, then two tiles' sums
     static constexpr int kSmem = (2 + kStages) * kTileBytes + 1024;
 };
-struct FwdBars {
-    uint64_t q_full[2], full[8], empty[8], s_full[2], p_full[2][2], o_full[2], tail, quiet[2];
-    AttnState st;
-    int4 block;
+struct FwdWork {
+    int start, rows;                 // as of AttnBlock; rows < 0: no more work
+    int key0, keys, kv_head;
+    int row0[2], head[2];            // of the tiles
+    int n[2];                        // blocks of 128 keys that their rows see (0: there is nothing to do but to write zeros, if there are rows)
+    __device__ __forceinline__ int blocks() const { return max(n[0], n[1]); }
 };
+struct FwdBars {
+    alignas(16) uint4 answer;        // to the request for more work
+    FwdWork work;
+    uint64_t q_full[2], q_empty[2], full[8], empty[8], s_full[2], p_full[2][2], o_full[2], work_full, work_read, answered, tail, quiet[2];
+    AttnState st;
+};
+// The next block of the grid that no CTA has started yet, or -1
+__device__ __forceinline__ void request_work(FwdBars* b) {
+    ptx::mbar_arrive_expect_tx(&b->answered, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(ptx::smem_u32(&b->answer)), "r"(ptx::smem_u32(&b->answered))
+                 : "memory");
+}
+__device__ __forceinline__ int work_of_answer(FwdBars* b) {
+    uint32_t x, got;
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .b128 a;\n .reg .b32 y, z, w;\n ld.shared.b128 a, [%2];\n clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n"
+        " selp.u32 %1, 1, 0, p;\n mov.u32 %0, 0;\n @p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, y, z, w}, a;\n}\n"
+        : "=r"(x), "=r"(got)
+        : "r"(ptx::smem_u32(&b->answer))
+        : "memory");
+    ptx::fence_proxy_async_smem();                   // (read before the next answer comes)
+    return got != 0 ? static_cast<int>(x) : -1;
+}
 
 template <int kChunks>
 __global__ void __launch_bounds__(kFwdThreads, 1)
@@ -263,25 +298,28 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     uint8_t *sq = smem, *skv = smem + 2 * kTileBytes;
     FwdBars* b = reinterpret_cast<FwdBars*>(smem + (2 + kStages) * kTileBytes);
     const int warp = threadIdx.x >> 5;
-    const int head = blockIdx.x % a.heads, kv_head = head / (a.heads / a.kv_heads);
+    int* failed = &b->st.failed;
     if (threadIdx.x == 0) {
         umma::prefetch_tensormap(&map_q);
         umma::prefetch_tensormap(&map_k);
         umma::prefetch_tensormap(&map_v);
         for (int i = 0; i < 2; ++i) {
             ptx::mbar_init(&b->q_full[i], 1);
+            ptx::mbar_init(&b->q_empty[i], 1);
             ptx::mbar_init(&b->s_full[i], 1);
             ptx::mbar_init(&b->p_full[i][0], 4);
             ptx::mbar_init(&b->p_full[i][1], 4);
             ptx::mbar_init(&b->o_full[i], 1);
+            ptx::mbar_init(&b->quiet[i], 1);
         }
         for (int i = 0; i < kStages; ++i) {
             ptx::mbar_init(&b->full[i], 1);
             ptx::mbar_init(&b->empty[i], 2);
         }
+        ptx::mbar_init(&b->work_full, 1);
+        ptx::mbar_init(&b->work_read, kFwdReaders);
+        ptx::mbar_init(&b->answered, 1);
         ptx::mbar_init(&b->tail, 1);
-        ptx::mbar_init(&b->quiet[0], 1);
-        ptx::mbar_init(&b->quiet[1], 1);
         b->st.failed = 0;
         ptx::mbar_fence_init();
     }
@@ -294,247 +332,312 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     umma::fence_after_thread_sync();
     const uint32_t tmem = b->st.tmem_base;
     ptx::wait_for_previous_kernel();
-    ptx::let_next_kernel_start();
-    // long blocks first: those at the ends of the sequences
-    const AttnBlock blk = find_block<256>(a.cu_q, a.num_seqs, a.tq, static_cast<int>(gridDim.x / a.heads - 1 - blockIdx.x / a.heads));
-    const int2 keys = sequence_rows(a.cu_k, blk.seq, a.tk);
-    const int shift = keys.y - blk.rows;                          // query i sees the keys up to i + shift
-    // blocks of 128 keys that the tiles' rows see
-    int n[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-        const int last = min(blk.row0 + t * 128 + 128, blk.rows) - 1;
-        const int seen = a.causal ? min(last + shift + 1, keys.y) : keys.y;
-        n[t] = blk.row0 + t * 128 >= blk.rows || seen <= 0 ? 0 : (seen + 127) / 128;
-    }
-    const int blocks = max(n[0], n[1]);
-    int* failed = &b->st.failed;
+    // The k-th block of this CTA, for a whole warp; false: no more
+    auto next_work = [&](int k, FwdWork& w) {
+        if (!attn_wait_warp(&b->work_full, k & 1, failed, a.report, 7)) return false;
+        w = b->work;
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->work_read);
+        return w.rows >= 0;
+    };
 
     if (warp >= 8) {
         give_registers();
         if (warp == 8) {
             AttnRing<kStages> p;
             const bool one = ptx::elect_one();
+            uint32_t tails = 0, queries[2] = {0, 0};
+            FwdWork w;
             auto request = [&](const CUtensorMap* map, int j, bool clear) {
                 if (!attn_wait_warp(&b->empty[p.stage], p.phase ^ 1, failed, a.report, 1)) return false;
                 uint8_t* tile = skv + p.stage * kTileBytes;
-                const bool tail = clear && j * 128 + 128 > keys.y;     // (the last block: at most once)
+                const bool tail = clear && j * 128 + 128 > w.keys;
                 uint64_t* bar = tail ? &b->tail : &b->full[p.stage];
                 if (one) {
                     ptx::mbar_arrive_expect_tx(bar, kTileBytes);
-                    load_tile<128, kChunks>(tile, map, kv_head, keys.x + j * 128, bar);
+                    load_tile<128, kChunks>(tile, map, w.kv_head, w.key0 + j * 128, bar);
                 }
                 __syncwarp();
                 if (tail) {
-                    if (!attn_wait_warp(&b->tail, 0, failed, a.report, 4)) return false;
-                    clear_tile<128, kChunks>(tile, keys.y - j * 128);
+                    if (!attn_wait_warp(&b->tail, tails & 1, failed, a.report, 4)) return false;
+                    ++tails;
+                    clear_tile<128, kChunks>(tile, w.keys - j * 128);
                     if (one) ptx::mbar_arrive(&b->full[p.stage]);
                 }
                 p.advance();
                 return true;
             };
-            if (blocks > 0) {
-                if (one)
+            auto load = [&]() {
+                for (int k = 0; next_work(k, w); ++k) {
+                    const int blocks = w.blocks();
+#pragma unroll
                     for (int t = 0; t < 2; ++t)
-                        if (n[t] > 0) {
-                            ptx::mbar_arrive_expect_tx(&b->q_full[t], kTileBytes);
-                            load_tile<128, kChunks>(sq + t * kTileBytes, &map_q, head, blk.start + blk.row0 + t * 128, &b->q_full[t]);
+                        if (w.n[t] > 0) {
+                            if (!attn_wait_warp(&b->q_empty[t], (queries[t] & 1) ^ 1, failed, a.report, 1)) return;
+                            ++queries[t];
+                            if (one) {
+                                ptx::mbar_arrive_expect_tx(&b->q_full[t], kTileBytes);
+                                load_tile<128, kChunks>(sq + t * kTileBytes, &map_q, w.head[t], w.start + w.row0[t], &b->q_full[t]);
+                            }
+                            __syncwarp();
                         }
-                __syncwarp();
-                for (int j = 0; j < blocks; ++j)
-                    if (!request(&map_k, j, false) || !request(&map_v, j, true)) break;
-            }
+                    for (int j = 0; j < blocks; ++j)
+                        if (!request(&map_k, j, false) || !request(&map_v, j, true)) return;
+                }
+            };
+            load();
         } else if (warp < 11) {
             // a tile's products; what neither tile reads any more is free
             const int t = warp - 9;
-            if (ptx::elect_one() && blocks > 0) {
-                const int dim16 = (a.dim + 15) / 16, mine = n[t];
-                const uint32_t idesc_s = umma::make_instr_desc(128, 128, umma::kFormatBF16), to_s = tmem + t * 128, to_o = tmem + Shape::kOut + t * 128;
-                const uint32_t idesc_o = umma::make_instr_desc(128, 16, umma::kFormatBF16, false, true) + (static_cast<uint32_t>(2 * dim16 - 2) << 17);
-                const uint64_t queries = desc_channels<128>(sq + t * kTileBytes), keys_of = desc_channels<128>(skv), values_of = desc_rows<128>(skv);
-                auto free_stage = [&](int stage, bool read) {
-                    if (read) umma::mma_commit(&b->empty[stage]);
-                    else ptx::mbar_arrive(&b->empty[stage]);
-                };
-                AttnRing<kStages> p;
-                auto scores = [&]() {
-                    umma::fence_after_thread_sync();
-                    multiply_channels<128, 128, kChunks>(to_s, queries, keys_of + p.stage * (kTileBytes / 16), idesc_s, dim16);
-                    umma::mma_commit(&b->s_full[t]);
-                };
-                auto multiply = [&]() {
-                    if (!attn_wait(&b->full[0], 0, failed, a.report, 4)) return;
-                    if (mine > 0) {
-                        if (!attn_wait(&b->q_full[t], 0, failed, a.report, 4)) return;
-                        scores();
-                    }
-                    free_stage(0, mine > 0);
+            const bool one = ptx::elect_one();
+            const int dim16 = (a.dim + 15) / 16;
+            const uint32_t idesc_s = umma::make_instr_desc(128, 128, umma::kFormatBF16), to_s = tmem + t * 128, to_o = tmem + Shape::kOut + t * 128;
+            const uint32_t idesc_o = umma::make_instr_desc(128, 16, umma::kFormatBF16, false, true) + (static_cast<uint32_t>(2 * dim16 - 2) << 17);
+            const uint32_t queries = desc_channels(sq + t * kTileBytes), keys_of = desc_channels(skv), values_of = desc_rows<128>(skv);
+            auto free_stage = [&](int stage, bool read) {
+                if (read) umma::mma_commit(&b->empty[stage]);
+                else ptx::mbar_arrive(&b->empty[stage]);
+            };
+            AttnRing<kStages> p;
+            uint32_t loads = 0, handed = 0;           // tiles of queries, blocks of probabilities so far
+            auto scores = [&](bool last) {
+                umma::fence_after_thread_sync();
+                multiply_channels<128, 128, kChunks>(to_s, queries, keys_of + p.stage * (kTileBytes / 16), idesc_s, dim16);
+                umma::mma_commit(&b->s_full[t]);
+                if (last) umma::mma_commit(&b->q_empty[t]);
+            };
+            auto multiply = [&](int blocks, int mine) {
+                if (!attn_wait(&b->full[p.stage], p.phase, failed, a.report, 4)) return;
+                if (mine > 0) {
+                    if (!attn_wait(&b->q_full[t], loads & 1, failed, a.report, 4)) return;
+                    ++loads;
+                    scores(mine == 1);
+                }
+                free_stage(p.stage, mine > 0);
+                p.advance();
+                for (int j = 0; j < blocks; ++j) {
+                    // (the values, and the next keys, have mostly long been there)
+                    const int stage_v = p.stage;
+                    const uint32_t values = values_of + stage_v * (kTileBytes / 16);
+                    if (!attn_wait(&b->full[stage_v], p.phase, failed, a.report, 4)) return;
                     p.advance();
-                    for (int j = 0; j < blocks; ++j) {
-                        // (the values, and the next keys, have mostly long been there)
-                        const int stage_v = p.stage;
-                        const uint64_t values = values_of + stage_v * (kTileBytes / 16);
-                        if (!attn_wait(&b->full[stage_v], p.phase, failed, a.report, 4)) return;
-                        p.advance();
-                        if (j + 1 < blocks && !attn_wait(&b->full[p.stage], p.phase, failed, a.report, 4)) return;
-                        if (j < mine) {
-                            // the first half of the probabilities as soon as it is there
-                            if (!attn_wait(&b->p_full[t][0], j & 1, failed, a.report, 2)) return;
-                            umma::fence_after_thread_sync();
-                            multiply_rows<0, 4>(to_o, to_s, values, idesc_o, j != 0);
-                            if (!attn_wait(&b->p_full[t][1], j & 1, failed, a.report, 2)) return;
-                            umma::fence_after_thread_sync();
-                            multiply_rows<4, 4>(to_o, to_s, values, idesc_o, true);
-                            if (j + 1 < mine) scores();
-                            else umma::mma_commit(&b->o_full[t]);
-                        }
-                        free_stage(stage_v, j < mine);
-                        if (j + 1 < blocks) {
-                            free_stage(p.stage, j + 1 < mine);
-                            p.advance();
-                        }
+                    if (j + 1 < blocks && !attn_wait(&b->full[p.stage], p.phase, failed, a.report, 4)) return;
+                    if (j < mine) {
+                        // the first half of the probabilities as soon as it is there
+                        if (!attn_wait(&b->p_full[t][0], handed & 1, failed, a.report, 2)) return;
+                        umma::fence_after_thread_sync();
+                        multiply_rows<0, 4>(to_o, to_s, values, idesc_o, j != 0);
+                        if (!attn_wait(&b->p_full[t][1], handed & 1, failed, a.report, 2)) return;
+                        ++handed;
+                        umma::fence_after_thread_sync();
+                        multiply_rows<4, 4>(to_o, to_s, values, idesc_o, true);
+                        if (j + 1 < mine) scores(j + 2 == mine);
+                        else umma::mma_commit(&b->o_full[t]);
                     }
-                };
-                multiply();
+                    free_stage(stage_v, j < mine);
+                    if (j + 1 < blocks) {
+                        free_stage(p.stage, j + 1 < mine);
+                        p.advance();
+                    }
+                }
+            };
+            FwdWork w;
+            for (int k = 0; next_work(k, w); ++k) {
+                if (one && w.blocks() > 0) multiply(w.blocks(), t == 0 ? w.n[0] : w.n[1]);
+                __syncwarp();
+            }
+        } else {
+            // looks for work: first this CTA's own
+            const int blocks = gridDim.x / a.heads;
+            int item = blockIdx.x;
+            uint32_t handed = 0;
+            bool something = true;
+            for (uint32_t answers = 0;; ++answers) {
+                FwdWork w{};
+                w.rows = -1;
+                if (item >= 0) {
+                    // 256 rows of a group's heads are as many pairs of tiles as the group has heads.  Long blocks first: those at the ends of the sequences
+                    const int number = item / a.heads, pair = item - number * a.heads, group = a.heads / a.kv_heads;
+                    const AttnBlock blk = find_block<256>(a.cu_q, a.num_seqs, a.tq, blocks - 1 - number);
+                    const int2 keys = sequence_rows(a.cu_k, blk.seq, a.tk);
+                    clear_rows<32>(a.cu_q, a.num_seqs, a.tq, item, gridDim.x, reinterpret_cast<bf16*>(a.o), static_cast<int64_t>(a.heads) * a.dim, a.lse, a.heads);
+                    w.start = blk.start;
+                    w.rows = blk.rows;
+                    w.key0 = keys.x;
+                    w.keys = keys.y;
+                    w.kv_head = pair / group;
+                    const int tile = (pair - w.kv_head * group) * 2;
+                    something = false;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const bool upper = tile + t >= group;
+                        w.row0[t] = blk.row0 + (upper ? 128 : 0);
+                        w.head[t] = w.kv_head * group + tile + t - (upper ? group : 0);
+                        const int last = min(w.row0[t] + 128, blk.rows) - 1, seen = a.causal ? min(last + keys.y - blk.rows + 1, keys.y) : keys.y;
+                        w.n[t] = w.row0[t] >= blk.rows || seen <= 0 ? 0 : (seen + 127) / 128;
+                        something |= w.row0[t] < blk.rows;
+                    }
+                }
+                if (something) {                      // (numbers without a tile are passed over)
+                    if ((threadIdx.x & 31) == 0) {
+                        b->work = w;
+                        ptx::mbar_arrive(&b->work_full);
+                    }
+                    // (a block is taken when the one before it is begun: taken earlier, it would wait here while other CTAs have none)
+                    if (w.rows < 0 || !attn_wait_warp(&b->work_read, handed & 1, failed, a.report, 7)) break;
+                    ++handed;
+                }
+                if ((threadIdx.x & 31) == 0) request_work(b);
+                if (!attn_wait_warp(&b->answered, answers & 1, failed, a.report, 7)) break;
+                item = work_of_answer(b);
+                something = true;
+                __syncwarp();
             }
         }
     } else {
         take_registers();
-        const int t = warp >> 2, lane_row = threadIdx.x & 127, row = blk.row0 + t * 128 + lane_row;
+        const int t = warp >> 2, lane_row = threadIdx.x & 127;
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), ts = lanes + t * 128, to = lanes + Shape::kOut + t * 128;
         const float c = a.scale * kLog2e;
-        const int seen = a.causal ? min(row + shift + 1, keys.y) : keys.y;      // keys that this row sees
-        const int first_seen = a.causal ? min(blk.row0 + t * 128 + shift + 1, keys.y) : keys.y;      // ... and the tile's first row
-        float ref = 0.f, sum = 0.f;
+        uint32_t made = 0, ended = 0;                 // blocks of scores, of results so far
+        FwdWork w;
         bool ok = true;
-        for (int j = 0; j < n[t]; ++j) {
-            ok = attn_wait_warp(&b->s_full[t], j & 1, failed, a.report, 5);
-            if (!ok) break;
-            umma::fence_after_thread_sync();
-            uint32_t s[4][32];
-            const bool masked = j * 128 + 128 > first_seen;
-            const int visible = seen - j * 128;
-            uint32_t out[32];
-            uint64_t part[2];
-            // 16 scores at a time, in an order that keeps the special function unit fed: scaled two steps ahead, summed and rounded a step behind
-            auto scaled = [&](int i) {
-                const uint64_t c2 = f32x2(c, c), minus = f32x2(-ref * c, -ref * c);
-#pragma unroll
-                for (int k = i * 16; k < i * 16 + 16; k += 2) {
-                    float x, y;
-                    umma::unpack_f32x2(fma2(umma::pack_f32x2(s[k >> 5][k & 31], s[k >> 5][(k & 31) + 1]), c2, minus), x, y);
-                    s[k >> 5][k & 31] = __float_as_uint(x);
-                    s[k >> 5][(k & 31) + 1] = __float_as_uint(y);
-                }
-            };
-            auto powers = [&](int i) {
-#pragma unroll
-                for (int k = i * 16; k < i * 16 + 16; k += 2) {
-                    uint32_t &x = s[k >> 5][k & 31], &y = s[k >> 5][(k & 31) + 1];
-                    if ((k >> 1) % kPolynomialOf == kPolynomialOf - 1) {
-                        float u, v;
-                        umma::unpack_f32x2(exp2_by_polynomial(umma::pack_f32x2(x, y)), u, v);
-                        x = __float_as_uint(u);
-                        y = __float_as_uint(v);
-                    } else {
-                        x = __float_as_uint(exp2_approx(__uint_as_float(x)));
-                        y = __float_as_uint(exp2_approx(__uint_as_float(y)));
-                    }
-                }
-            };
-            auto rounded = [&](int i) {
-#pragma unroll
-                for (int k = i * 16; k < i * 16 + 16; k += 2) {
-                    const uint32_t x = s[k >> 5][k & 31], y = s[k >> 5][(k & 31) + 1];
-                    part[(k >> 1) & 1] = add2(part[(k >> 1) & 1], umma::pack_f32x2(x, y));
-                    out[(k & 63) >> 1] = pack_bf16(__uint_as_float(x), __uint_as_float(y));
-                }
-            };
-            auto hand_over = [&](int i) {
-                umma::tmem_st_32x32(ts + i * 32, out);
-                umma::tmem_st_wait();
-                umma::fence_before_thread_sync();
-                __syncwarp();
-                if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->p_full[t][i]);
-            };
-#pragma unroll
-            for (int i = 0; i < 4; ++i) umma::tmem_ld_32x32(ts + i * 32, s[i]);
-            umma::tmem_ld_wait();
-            if (masked)
-#pragma unroll
-                for (int k = 0; k < 128; ++k)
-                    if (k >= visible) s[k >> 5][k & 31] = 0xff800000u;
-            float top[8];                             // (many short chains)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                auto value = [&](int k) { return __uint_as_float(s[i >> 1][(i & 1) * 16 + k]); };
-                top[i] = max3(value(0), value(1), value(2));
-#pragma unroll
-                for (int k = 3; k < 15; k += 2) top[i] = max3(top[i], value(k), value(k + 1));
-                top[i] = fmaxf(top[i], value(15));
-            }
-            const float largest = fmaxf(max3(max3(top[0], top[1], top[2]), top[3], top[4]), max3(top[5], top[6], top[7]));
-            // The reference moves only when the largest score is more than 2^8 above it: sums and probabilities have that much room, and O is seldom multiplied.
-            if (j == 0) {
-                ref = largest == kNone ? 0.f : largest;
-            } else {
-                const bool move = (largest - ref) * c > 8.f;
-                if (__any_sync(0xffffffffu, move)) {
-                    const float factor = move ? exp2_approx((ref - largest) * c) : 1.f;
-                    sum *= factor;
-                    ref = move ? largest : ref;
-#pragma unroll
-                    for (int i = 0; i < 64 * kChunks; i += 16) {
-                        uint32_t o[16];
-                        umma::tmem_ld_32x16(to + i, o);
-                        umma::tmem_ld_wait();
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
-                        umma::tmem_st_32x16(to + i, o);
-                    }
-                }
-            }
-            part[0] = f32x2(sum, 0.f);
-            part[1] = f32x2(0.f, 0.f);
-            scaled(0);
-            scaled(1);
-            powers(0);
-#pragma unroll
-            for (int i = 1; i < 8; ++i) {
-                if (i < 7) scaled(i + 1);
-                powers(i);
-                rounded(i - 1);
-                if (i == 4) hand_over(0);
-            }
-            rounded(7);
-            hand_over(1);
-            float u, v;
-            umma::unpack_f32x2(add2(part[0], part[1]), u, v);
-            sum = u + v;
-        }
-        const bool in = row < blk.rows;
-        const int64_t token = blk.start + row;
-        bf16* out = reinterpret_cast<bf16*>(a.o) + (token * a.heads + head) * a.dim;
-        if (n[t] > 0) {
-            ok = ok && attn_wait_warp(&b->o_full[t], 0, failed, a.report, 6);
-            if (ok) {
+        for (int k = 0; ok && next_work(k, w); ++k) {
+            const int row0 = t == 0 ? w.row0[0] : w.row0[1], head = t == 0 ? w.head[0] : w.head[1], row = row0 + lane_row, shift = w.keys - w.rows;
+            const int seen = a.causal ? min(row + shift + 1, w.keys) : w.keys;      // keys that this row sees
+            const int first_seen = a.causal ? min(row0 + shift + 1, w.keys) : w.keys;      // ... and the tile's first row
+            const int n = t == 0 ? w.n[0] : w.n[1];
+            float ref = 0.f, sum = 0.f;
+            for (int j = 0; j < n; ++j) {
+                ok = attn_wait_warp(&b->s_full[t], made & 1, failed, a.report, 5);
+                if (!ok) break;
+                ++made;
                 umma::fence_after_thread_sync();
-                store_row<64 * kChunks>(to, sum == 0.f ? 0.f : 1.f / sum, out, a.dim, in);
+                uint32_t s[4][32];
+                const bool masked = j * 128 + 128 > first_seen;
+                const int visible = seen - j * 128;
+                uint32_t out[32];
+                uint64_t part[2];
+                // 16 scores at a time, in an order that keeps the special function unit fed: scaled two steps ahead, summed and rounded a step behind
+                auto scaled = [&](int i) {
+                    const uint64_t c2 = f32x2(c, c), minus = f32x2(-ref * c, -ref * c);
+#pragma unroll
+                    for (int k = i * 16; k < i * 16 + 16; k += 2) {
+                        float x, y;
+                        umma::unpack_f32x2(fma2(umma::pack_f32x2(s[k >> 5][k & 31], s[k >> 5][(k & 31) + 1]), c2, minus), x, y);
+                        s[k >> 5][k & 31] = __float_as_uint(x);
+                        s[k >> 5][(k & 31) + 1] = __float_as_uint(y);
+                    }
+                };
+                auto powers = [&](int i) {
+#pragma unroll
+                    for (int k = i * 16; k < i * 16 + 16; k += 2) {
+                        uint32_t &x = s[k >> 5][k & 31], &y = s[k >> 5][(k & 31) + 1];
+                        if ((k >> 1) % kPolynomialOf == kPolynomialOf - 1) {
+                            float u, v;
+                            umma::unpack_f32x2(exp2_by_polynomial(umma::pack_f32x2(x, y)), u, v);
+                            x = __float_as_uint(u);
+                            y = __float_as_uint(v);
+                        } else {
+                            x = __float_as_uint(exp2_approx(__uint_as_float(x)));
+                            y = __float_as_uint(exp2_approx(__uint_as_float(y)));
+                        }
+                    }
+                };
+                auto rounded = [&](int i) {
+#pragma unroll
+                    for (int k = i * 16; k < i * 16 + 16; k += 2) {
+                        const uint32_t x = s[k >> 5][k & 31], y = s[k >> 5][(k & 31) + 1];
+                        part[(k >> 1) & 1] = add2(part[(k >> 1) & 1], umma::pack_f32x2(x, y));
+                        out[(k & 63) >> 1] = pack_bf16(__uint_as_float(x), __uint_as_float(y));
+                    }
+                };
+                auto hand_over = [&](int i) {
+                    umma::tmem_st_32x32(ts + i * 32, out);
+                    umma::tmem_st_wait();
+                    umma::fence_before_thread_sync();
+                    __syncwarp();
+                    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->p_full[t][i]);
+                };
+#pragma unroll
+                for (int i = 0; i < 4; ++i) umma::tmem_ld_32x32(ts + i * 32, s[i]);
+                umma::tmem_ld_wait();
+                if (masked)
+#pragma unroll
+                    for (int k = 0; k < 128; ++k)
+                        if (k >= visible) s[k >> 5][k & 31] = 0xff800000u;
+                float top[8];                             // (many short chains)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    auto value = [&](int k) { return __uint_as_float(s[i >> 1][(i & 1) * 16 + k]); };
+                    top[i] = max3(value(0), value(1), value(2));
+#pragma unroll
+                    for (int k = 3; k < 15; k += 2) top[i] = max3(top[i], value(k), value(k + 1));
+                    top[i] = fmaxf(top[i], value(15));
+                }
+                const float largest = fmaxf(max3(max3(top[0], top[1], top[2]), top[3], top[4]), max3(top[5], top[6], top[7]));
+                // The reference moves only when the largest score is more than 2^8 above it: sums and probabilities have that much room, and O is seldom multiplied.
+                if (j == 0) {
+                    ref = largest == kNone ? 0.f : largest;
+                } else {
+                    const bool move = (largest - ref) * c > 8.f;
+                    if (__any_sync(0xffffffffu, move)) {
+                        const float factor = move ? exp2_approx((ref - largest) * c) : 1.f;
+                        sum *= factor;
+                        ref = move ? largest : ref;
+#pragma unroll
+                        for (int i = 0; i < 64 * kChunks; i += 16) {
+                            uint32_t o[16];
+                            umma::tmem_ld_32x16(to + i, o);
+                            umma::tmem_ld_wait();
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * factor);
+                            umma::tmem_st_32x16(to + i, o);
+                        }
+                    }
+                }
+                part[0] = f32x2(sum, 0.f);
+                part[1] = f32x2(0.f, 0.f);
+                scaled(0);
+                scaled(1);
+                powers(0);
+#pragma unroll
+                for (int i = 1; i < 8; ++i) {
+                    if (i < 7) scaled(i + 1);
+                    powers(i);
+                    rounded(i - 1);
+                    if (i == 4) hand_over(0);
+                }
+                rounded(7);
+                hand_over(1);
+                float u, v;
+                umma::unpack_f32x2(add2(part[0], part[1]), u, v);
+                sum = u + v;
             }
-        } else if (in) {
-            for (int i = 0; i < a.dim; i += 8) *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
+            const bool in = row < w.rows;
+            const int64_t token = w.start + row;
+            bf16* out = reinterpret_cast<bf16*>(a.o) + (token * a.heads + head) * a.dim;
+            if (n > 0) {
+                ok = ok && attn_wait_warp(&b->o_full[t], ended & 1, failed, a.report, 6);
+                ++ended;
+                if (ok) {
+                    umma::fence_after_thread_sync();
+                    store_row<64 * kChunks>(to, sum == 0.f ? 0.f : 1.f / sum, out, a.dim, in);
+                }
+            } else if (in) {
+                for (int i = 0; i < a.dim; i += 8) *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
+            }
+            if (in && ok) a.lse[static_cast<int64_t>(head) * a.tq + token] = sum == 0.f ? kNone : (ref * c + log2f(sum)) * kLn2;
         }
-        if (in && ok) a.lse[static_cast<int64_t>(head) * a.tq + token] = sum == 0.f ? kNone : (ref * c + log2f(sum)) * kLn2;
-        clear_rows<256>(a.cu_q, a.num_seqs, a.tq, reinterpret_cast<bf16*>(a.o), static_cast<int64_t>(a.heads) * a.dim, a.lse, a.heads);
     }
     umma::fence_before_thread_sync();
     __syncthreads();
     if (b->st.failed != 0) {
         // (a wait has run out: what was requested or issued ends before its memory goes to others)
         if (warp == 8) {
-            for (int i = 0; i < 2; ++i)
-                if (n[i] > 0) mbar_drain(&b->q_full[i], 0, 100000000ull);
+            for (int i = 0; i < 2; ++i) mbar_drain(&b->q_full[i], 0, 100000000ull), mbar_drain(&b->q_full[i], 1, 100000000ull);
             for (int i = 0; i < kStages; ++i) mbar_drain(&b->full[i], 0, 100000000ull), mbar_drain(&b->full[i], 1, 100000000ull);
+            mbar_drain(&b->answered, 0, 100000000ull), mbar_drain(&b->answered, 1, 100000000ull);
         }
         if ((warp == 9 || warp == 10) && ptx::elect_one()) {
             umma::mma_commit(&b->quiet[warp - 9]);
@@ -694,13 +797,13 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                 const int dim16 = (a.dim + 15) / 16;
                 const uint32_t idesc_s = umma::make_instr_desc(128, 64, umma::kFormatBF16);
                 const uint32_t idesc_o = umma::make_instr_desc(128, 16, umma::kFormatBF16, false, true) + (static_cast<uint32_t>(2 * dim16 - 2) << 17);
-                const uint64_t kept_of = desc_channels<128>(kept), pieces_of = desc_channels<64>(pieces), rows_of = desc_rows<64>(pieces);
+                const uint32_t kept_of = desc_channels(kept), pieces_of = desc_channels(pieces), rows_of = desc_rows<64>(pieces);
                 AttnRing<kStages> p, q;                   // pieces whose scores are next, pieces whose sums are next
                 auto scores = [&](int i) {
                     if (!attn_wait(&b->full[p.stage], p.phase, failed, a.report, 4)) return false;
                     umma::fence_after_thread_sync();
                     const uint32_t to = tmem + Shape::kBuffers + (i & 1) * 128;
-                    const uint64_t piece = pieces_of + p.stage * (2 * kPieceBytes / 16);
+                    const uint32_t piece = pieces_of + p.stage * (2 * kPieceBytes / 16);
                     multiply_channels<128, 64, kChunks>(to, kept_of, piece, idesc_s, dim16);
                     multiply_channels<128, 64, kChunks>(to + 64, kept_of + kKeptBytes / 16, piece + kPieceBytes / 16, idesc_s, dim16);
                     umma::mma_commit(&b->s_full[i & 1]);
@@ -714,7 +817,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                         if (!attn_wait(&b->p_full[i & 1], (i >> 1) & 1, failed, a.report, 2)) return;
                         umma::fence_after_thread_sync();
                         const uint32_t from = tmem + Shape::kBuffers + (i & 1) * 128;
-                        const uint64_t piece = rows_of + q.stage * (2 * kPieceBytes / 16);
+                        const uint32_t piece = rows_of + q.stage * (2 * kPieceBytes / 16);
                         if (kKeys) multiply_rows<0, 4>(tmem + 128, from, piece + kPieceBytes / 16, idesc_o, i != 0);
                         multiply_rows<0, 4>(tmem, from + 64, piece, idesc_o, i != 0);
                         umma::mma_commit(&b->empty[q.stage]);
@@ -843,10 +946,10 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
         }
         const int64_t row_values = static_cast<int64_t>(heads) * a.dim;
         if (kKeys) {
-            clear_rows<256>(a.cu_k, a.num_seqs, a.tk, reinterpret_cast<bf16*>(a.dk), row_values, nullptr, 0);
-            clear_rows<256>(a.cu_k, a.num_seqs, a.tk, reinterpret_cast<bf16*>(a.dv), row_values, nullptr, 0);
+            clear_rows<256>(a.cu_k, a.num_seqs, a.tk, blockIdx.x, gridDim.x, reinterpret_cast<bf16*>(a.dk), row_values, nullptr, 0);
+            clear_rows<256>(a.cu_k, a.num_seqs, a.tk, blockIdx.x, gridDim.x, reinterpret_cast<bf16*>(a.dv), row_values, nullptr, 0);
         } else {
-            clear_rows<256>(a.cu_q, a.num_seqs, a.tq, reinterpret_cast<bf16*>(a.dq), row_values, nullptr, 0);
+            clear_rows<256>(a.cu_q, a.num_seqs, a.tq, blockIdx.x, gridDim.x, reinterpret_cast<bf16*>(a.dq), row_values, nullptr, 0);
         }
     }
     umma::fence_before_thread_sync();
