@@ -598,12 +598,15 @@ struct AttentionArgs {
     const float *lse_in, *d_lse;      // [heads, tq]; d_lse or null
     float* delta;                     // [heads, tq] workspace
     void *dq, *dk, *dv;               // bf16, contiguous
+    int splits;                       // parts of a group that make dk and dv by themselves
+    float* parts;                     // [splits, 2, tk, kv_heads, dim] workspace, if there are several
     NsReport report;
 };
 
 namespace ep {
-cudaError_t launch_attention(const AttentionArgs& args, int num_sms, cudaStream_t stream);
-cudaError_t launch_attention_backward(const AttentionArgs& args, int num_sms, cudaStream_t stream);
+cudaError_t launch_attention(const AttentionArgs& args, cudaStream_t stream);
+int attention_backward_splits(const AttentionArgs& args, int num_sms);
+cudaError_t launch_attention_backward(const AttentionArgs& args, cudaStream_t stream);
 }  // namespace ep
 
 // One new token per sequence over a paged cache (paged_attention.cu)

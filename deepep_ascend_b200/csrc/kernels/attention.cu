@@ -243,6 +243,22 @@ __device__ __forceinline__ void store_row(uint32_t tmem, float factor, bf16* row
     }
 }
 
+// ... as it is, in 32 bits
+template <int kColumns>
+__device__ __forceinline__ void store_part(uint32_t tmem, float factor, float* row, int dim, bool write) {
+#pragma unroll
+    for (int c = 0; c < kColumns; c += 32) {
+        uint32_t r[32];
+        umma::tmem_ld_32x32(tmem + c, r);
+        umma::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+            if (write && c + i < dim)
+                *reinterpret_cast<float4*>(row + c + i) = make_float4(__uint_as_float(r[i]) * factor, __uint_as_float(r[i + 1]) * factor, __uint_as_float(r[i + 2]) * factor,
+                                                                      __uint_as_float(r[i + 3]) * factor);
+    }
+}
+
 // ------------------------------------------------------------------------------------------------ forward
 // A CTA takes two tiles of 128 queries that share keys and values, of two heads of a group or, where it has no second one, of one head, whose softmaxes (four warps each, a row per thread) and products alternate: while one tile's scores are made into
 // probabilities, the tensor cores work for the other.  Probabilities take the place of the scores in tensor memory, from where they are the first operand of the next product.
@@ -679,19 +695,24 @@ __global__ void __launch_bounds__(kDeltaThreads) attention_delta_kernel(const __
 }
 
 // A CTA keeps 128 rows of one side (kKeys: keys and values, whose gradients it makes; otherwise queries and dO, for dQ) and takes those of the other side in
-// pieces of 64.  Scores and dP of a piece are products whose lanes are the kept rows, so that P and dS, written over them, are first operands of the products
-// that follow, and sums stay in tensor memory until the end: every gradient is added by one CTA, in a fixed order.  P is made twice, which costs two products of
-// seven, and spares sums of dQ in memory by many CTAs in any order.  Two groups of four warps take every other piece.
+// pieces of 128.  Scores and dP of a piece are products whose lanes are the kept rows, so that P and dS are first operands of the products that follow, and sums stay in
+// tensor memory until the end: every gradient is added by one CTA (or by one per part of the group, whose parts are then added), in a fixed order.  P is made twice, which
+// costs two products of seven, and spares sums of dQ in memory by many CTAs in any order.
+//
+// Two groups of four warps have 64 columns of a piece each.  P and dS take the place of dP; that of the scores is free as soon as they are in registers, so the next piece's
+// scores are made meanwhile, and their powers while dV, dK and the next dP are.  (Pieces of 64 columns with two places for each had products of half the width, which take as long
+// as whole ones: 128 rows of the first operand come from shared memory either way.)
 constexpr int kBwdThreads = 384;                     // 2 x 4 warps for rows, one that requests pieces, one that issues products, two without work
-template <int kChunks>
+template <int kChunks, bool kKeys>
 struct BwdShape {
-    static constexpr int kKeptBytes = 128 * 128 * kChunks, kPieceBytes = 64 * 128 * kChunks, kStages = kChunks == 2 ? 4 : 6;
-    static constexpr int kBuffers = 256;              // tensor memory: two sums of 128 columns, then twice scores and dP of 64 columns
+    static constexpr int kTileBytes = 128 * 128 * kChunks, kSlots = kChunks == 2 ? 5 : 8;
+    // tensor memory: sums (of keys and values, or of queries), scores, dP (once, or twice)
+    static constexpr int kScores = kKeys ? 256 : 128, kDp = kKeys ? 384 : 256, kDps = kKeys ? 1 : 2;
     static constexpr int kStatBytes = 2 * 2 * 128 * 4;
-    static constexpr int kSmem = 2 * kKeptBytes + 2 * kStages * kPieceBytes + kStatBytes + 1024;
+    static constexpr int kSmem = (2 + kSlots) * kTileBytes + kStatBytes + 1024;
 };
 struct BwdBars {
-    uint64_t kept, full[8], empty[8], s_full[2], p_full[2], sums, tail, quiet;
+    uint64_t kept, full[8], empty[8], s_full, s_read, dp_full, p_full[2], sums, tail, quiet;
     AttnState st;
 };
 
@@ -699,12 +720,12 @@ template <int kChunks, bool kKeys>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const __grid_constant__ CUtensorMap map_kept1, const __grid_constant__ CUtensorMap map_piece0,
                           const __grid_constant__ CUtensorMap map_piece1, const __grid_constant__ AttentionArgs a) {
-    using Shape = BwdShape<kChunks>;
-    constexpr int kStages = Shape::kStages, kPieceBytes = Shape::kPieceBytes, kKeptBytes = Shape::kKeptBytes;
+    using Shape = BwdShape<kChunks, kKeys>;
+    constexpr int kSlots = Shape::kSlots, kTileBytes = Shape::kTileBytes;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t *kept = smem, *pieces = smem + 2 * kKeptBytes;
-    float* stats = reinterpret_cast<float*>(pieces + 2 * kStages * kPieceBytes);
-    BwdBars* b = reinterpret_cast<BwdBars*>(pieces + 2 * kStages * kPieceBytes + Shape::kStatBytes);
+    uint8_t *kept = smem, *pieces = smem + 2 * kTileBytes;
+    float* stats = reinterpret_cast<float*>(pieces + kSlots * kTileBytes);
+    BwdBars* b = reinterpret_cast<BwdBars*>(pieces + kSlots * kTileBytes + Shape::kStatBytes);
     const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads;
     if (threadIdx.x == 0) {
         umma::prefetch_tensormap(&map_kept0);
@@ -712,14 +733,15 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
         umma::prefetch_tensormap(&map_piece0);
         umma::prefetch_tensormap(&map_piece1);
         ptx::mbar_init(&b->kept, 1);
-        for (int i = 0; i < kStages; ++i) {
+        for (int i = 0; i < kSlots; ++i) {
             ptx::mbar_init(&b->full[i], 1);
             ptx::mbar_init(&b->empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i) {
-            ptx::mbar_init(&b->s_full[i], 1);
-            ptx::mbar_init(&b->p_full[i], 4);
-        }
+        ptx::mbar_init(&b->s_full, 1);
+        ptx::mbar_init(&b->s_read, 8);
+        ptx::mbar_init(&b->dp_full, 1);
+        ptx::mbar_init(&b->p_full[0], 4);
+        ptx::mbar_init(&b->p_full[1], 4);
         ptx::mbar_init(&b->sums, 1);
         ptx::mbar_init(&b->tail, 1);
         ptx::mbar_init(&b->quiet, 1);
@@ -738,22 +760,24 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
     ptx::let_next_kernel_start();
     int* failed = &b->st.failed;
     // (kKeys: the first keys are seen by most queries; otherwise the last queries see most keys.  Long blocks first.)
-    const int heads = kKeys ? a.kv_heads : a.heads, total = kKeys ? a.tk : a.tq;
-    const int head = blockIdx.x % heads, number = blockIdx.x / heads;
-    const AttnBlock blk = find_block<128>(kKeys ? a.cu_k : a.cu_q, a.num_seqs, total, kKeys ? number : static_cast<int>(gridDim.x / heads) - 1 - number);
+    const int units = kKeys ? a.kv_heads * a.splits : a.heads, total = kKeys ? a.tk : a.tq;
+    const int unit = blockIdx.x % units, number = blockIdx.x / units;
+    const int head = kKeys ? unit / a.splits : unit, split = kKeys ? unit % a.splits : 0;      // (of keys, or of queries)
+    const int first_head = kKeys ? head * group + group * split / a.splits : 0, num_heads = kKeys ? head * group + group * (split + 1) / a.splits - first_head : 1;
+    const AttnBlock blk = find_block<128>(kKeys ? a.cu_k : a.cu_q, a.num_seqs, total, kKeys ? number : static_cast<int>(gridDim.x / units) - 1 - number);
     const int2 other = sequence_rows(kKeys ? a.cu_q : a.cu_k, blk.seq, kKeys ? a.tq : a.tk);
     const int shift = kKeys ? blk.rows - other.y : other.y - blk.rows;     // query i sees the keys up to i + shift
     // pieces [piece0, piece1) of every head
     int piece0 = 0, piece1 = 0, n = 0;
     if (blk.row0 < blk.rows) {
         if (kKeys) {
-            piece0 = a.causal ? max(blk.row0 - shift, 0) / 64 : 0;
-            piece1 = (other.y + 63) / 64;
+            piece0 = a.causal ? max(blk.row0 - shift, 0) / 128 : 0;
+            piece1 = (other.y + 127) / 128;
         } else {
             const int seen = a.causal ? min(min(blk.row0 + 128, blk.rows) + shift, other.y) : other.y;
-            piece1 = seen <= 0 ? 0 : (seen + 63) / 64;
+            piece1 = seen <= 0 ? 0 : (seen + 127) / 128;
         }
-        n = max(piece1 - piece0, 0) * (kKeys ? group : 1);
+        n = max(piece1 - piece0, 0) * num_heads;
     }
     const int per_head = max(piece1 - piece0, 1);
 
@@ -761,68 +785,88 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
         give_registers();
         if (warp == 8) {
             if (n > 0) {
-                AttnRing<kStages> p;
+                AttnRing<kSlots> p;
                 const bool one = ptx::elect_one();
                 if (one) {
-                    ptx::mbar_arrive_expect_tx(&b->kept, 2 * kKeptBytes);
+                    ptx::mbar_arrive_expect_tx(&b->kept, 2 * kTileBytes);
                     load_tile<128, kChunks>(kept, &map_kept0, head, blk.start + blk.row0, &b->kept);
-                    load_tile<128, kChunks>(kept + kKeptBytes, &map_kept1, head, blk.start + blk.row0, &b->kept);
+                    load_tile<128, kChunks>(kept + kTileBytes, &map_kept1, head, blk.start + blk.row0, &b->kept);
                 }
                 __syncwarp();
                 uint32_t tails = 0;
-                for (int i = 0; i < n; ++i) {
-                    if (!attn_wait_warp(&b->empty[p.stage], p.phase ^ 1, failed, a.report, 1)) break;
-                    const int h = kKeys ? head * group + i / per_head : head / group, piece = piece0 + i % per_head;
-                    uint8_t* tile = pieces + p.stage * 2 * kPieceBytes;
-                    const bool tail = piece * 64 + 64 > other.y;
+                auto request = [&](const CUtensorMap* map, int h, int piece) {
+                    if (!attn_wait_warp(&b->empty[p.stage], p.phase ^ 1, failed, a.report, 1)) return false;
+                    uint8_t* tile = pieces + p.stage * kTileBytes;
+                    const bool tail = piece * 128 + 128 > other.y;
                     uint64_t* bar = tail ? &b->tail : &b->full[p.stage];
                     if (one) {
-                        ptx::mbar_arrive_expect_tx(bar, 2 * kPieceBytes);
-                        load_tile<64, kChunks>(tile, &map_piece0, h, other.x + piece * 64, bar);
-                        load_tile<64, kChunks>(tile + kPieceBytes, &map_piece1, h, other.x + piece * 64, bar);
+                        ptx::mbar_arrive_expect_tx(bar, kTileBytes);
+                        load_tile<128, kChunks>(tile, map, h, other.x + piece * 128, bar);
                     }
                     __syncwarp();
                     if (tail) {
-                        if (!attn_wait_warp(&b->tail, tails & 1, failed, a.report, 4)) break;
+                        if (!attn_wait_warp(&b->tail, tails & 1, failed, a.report, 4)) return false;
                         ++tails;
-                        clear_tile<64, kChunks>(tile, other.y - piece * 64);
-                        clear_tile<64, kChunks>(tile + kPieceBytes, other.y - piece * 64);
+                        clear_tile<128, kChunks>(tile, other.y - piece * 128);
                         if (one) ptx::mbar_arrive(&b->full[p.stage]);
                     }
                     p.advance();
+                    return true;
+                };
+                for (int i = 0; i < n; ++i) {
+                    const int h = kKeys ? first_head + i / per_head : head / group, piece = piece0 + i % per_head;
+                    if (!request(&map_piece0, h, piece) || !request(&map_piece1, h, piece)) break;
                 }
             }
         } else if (warp == 9) {
             if (n > 0 && ptx::elect_one()) {
                 const int dim16 = (a.dim + 15) / 16;
-                const uint32_t idesc_s = umma::make_instr_desc(128, 64, umma::kFormatBF16);
+                const uint32_t idesc_s = umma::make_instr_desc(128, 128, umma::kFormatBF16);
                 const uint32_t idesc_o = umma::make_instr_desc(128, 16, umma::kFormatBF16, false, true) + (static_cast<uint32_t>(2 * dim16 - 2) << 17);
-                const uint32_t kept_of = desc_channels(kept), pieces_of = desc_channels(pieces), rows_of = desc_rows<64>(pieces);
-                AttnRing<kStages> p, q;                   // pieces whose scores are next, pieces whose sums are next
-                auto scores = [&](int i) {
+                const uint32_t kept_of = desc_channels(kept), pieces_of = desc_channels(pieces), rows_of = desc_rows<128>(pieces);
+                AttnRing<kSlots> p;                   // operands in the order in which they come: first and second of every piece
+                // the first products of piece i, of its first or second operand
+                auto product = [&](int which, uint32_t to, uint64_t* done, int& slot) {
                     if (!attn_wait(&b->full[p.stage], p.phase, failed, a.report, 4)) return false;
                     umma::fence_after_thread_sync();
-                    const uint32_t to = tmem + Shape::kBuffers + (i & 1) * 128;
-                    const uint32_t piece = pieces_of + p.stage * (2 * kPieceBytes / 16);
-                    multiply_channels<128, 64, kChunks>(to, kept_of, piece, idesc_s, dim16);
-                    multiply_channels<128, 64, kChunks>(to + 64, kept_of + kKeptBytes / 16, piece + kPieceBytes / 16, idesc_s, dim16);
-                    umma::mma_commit(&b->s_full[i & 1]);
+                    multiply_channels<128, 128, kChunks>(tmem + to, kept_of + which * (kTileBytes / 16), pieces_of + p.stage * (kTileBytes / 16), idesc_s, dim16);
+                    umma::mma_commit(done);
+                    slot = p.stage;
                     p.advance();
                     return true;
                 };
                 auto multiply = [&]() {
                     if (!attn_wait(&b->kept, 0, failed, a.report, 4)) return;
-                    if (!scores(0) || (n > 1 && !scores(1))) return;
+                    int slot0, slot1, next0 = 0, next1 = 0;
+                    if (!product(0, Shape::kScores, &b->s_full, slot0) || !product(1, Shape::kDp, &b->dp_full, slot1)) return;
+                    if (!kKeys) umma::mma_commit(&b->empty[slot1]);
                     for (int i = 0; i < n; ++i) {
-                        if (!attn_wait(&b->p_full[i & 1], (i >> 1) & 1, failed, a.report, 2)) return;
-                        umma::fence_after_thread_sync();
-                        const uint32_t from = tmem + Shape::kBuffers + (i & 1) * 128;
-                        const uint32_t piece = rows_of + q.stage * (2 * kPieceBytes / 16);
-                        if (kKeys) multiply_rows<0, 4>(tmem + 128, from, piece + kPieceBytes / 16, idesc_o, i != 0);
-                        multiply_rows<0, 4>(tmem, from + 64, piece, idesc_o, i != 0);
-                        umma::mma_commit(&b->empty[q.stage]);
-                        q.advance();
-                        if (i + 2 < n && !scores(i + 2)) return;
+                        const uint32_t dp = Shape::kDp + (kKeys ? 0 : (i & 1) * 128);
+                        if (i + 1 < n) {
+                            if (!attn_wait(&b->s_read, i & 1, failed, a.report, 3)) return;
+                            if (!product(0, Shape::kScores, &b->s_full, next0)) return;
+                            if (!kKeys) {
+                                // (the other place of dP: what was there is behind the products before)
+                                if (!product(1, Shape::kDp + (~i & 1) * 128, &b->dp_full, next1)) return;
+                                umma::mma_commit(&b->empty[next1]);
+                            }
+                        }
+                        const uint32_t rows0 = rows_of + slot0 * (kTileBytes / 16), rows1 = rows_of + slot1 * (kTileBytes / 16);
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            if (!attn_wait(&b->p_full[half], i & 1, failed, a.report, 2)) return;
+                            umma::fence_after_thread_sync();
+                            const uint32_t from = tmem + dp + half * 64, step = half * 4 * 16 * 128 / 16;
+                            if (kKeys) multiply_rows<0, 4>(tmem + 128, from, rows1 + step, idesc_o, i != 0 || half != 0);
+                            multiply_rows<0, 4>(tmem, from + 32, rows0 + step, idesc_o, i != 0 || half != 0);
+                        }
+                        umma::mma_commit(&b->empty[slot0]);
+                        if (kKeys) {
+                            umma::mma_commit(&b->empty[slot1]);
+                            if (i + 1 < n && !product(1, Shape::kDp, &b->dp_full, next1)) return;
+                        }
+                        slot0 = next0;
+                        slot1 = next1;
                     }
                     umma::mma_commit(&b->sums);
                 };
@@ -832,7 +876,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
     } else {
         take_registers();
         const int half = warp >> 2, lane_row = threadIdx.x & 127, row = blk.row0 + lane_row;
-        const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), from = lanes + Shape::kBuffers + half * 128;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const float c = a.scale * kLog2e;
         const bool in = row < blk.rows;
         const int64_t token = blk.start + row;
@@ -847,13 +891,13 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
         };
         auto next_statistic = [&](int i) {
             if (i >= n) return 0.f;
-            const int at = (piece0 + i % per_head) * 64 + (lane_row & 63);
-            return statistic(lane_row >= 64, at < other.y, head * group + i / per_head, other.x + at);
+            const int at = (piece0 + i % per_head) * 128 + half * 64 + (lane_row & 63);
+            return statistic(lane_row >= 64, at < other.y, first_head + i / per_head, other.x + at);
         };
         float coming = 0.f;
         uint64_t minus2 = 0, delta2 = 0;
         if (kKeys) {
-            coming = next_statistic(half);
+            coming = next_statistic(0);
         } else if (n > 0) {
             const float m = statistic(false, in, head, token), d = statistic(true, in, head, token);
             minus2 = f32x2(m, m);
@@ -861,95 +905,116 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
         }
         bool ok = true;
         const uint64_t c2 = f32x2(c, c);
-        for (int i = half; i < n; i += 2) {
-            float* now = mine + (i >> 1 & 1) * 128;
+        for (int i = 0; i < n; ++i) {
+            const float* now = mine + (i & 1) * 128;
             if (kKeys) {
-                now[lane_row] = coming;
-                asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
-                coming = next_statistic(i + 2);
+                mine[(i & 1) * 128 + lane_row] = coming;
+                if (half == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
+                else asm volatile("bar.sync 2, 128;" ::: "memory");
+                coming = next_statistic(i + 1);
             }
-            ok = ok && attn_wait_warp(&b->s_full[half], (i >> 1) & 1, failed, a.report, 5);
+            ok = ok && attn_wait_warp(&b->s_full, i & 1, failed, a.report, 5);
             if (!ok) continue;                        // (the others may wait at the barrier above)
             umma::fence_after_thread_sync();
             uint32_t s[2][32], d[2][32];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) umma::tmem_ld_32x32(from + k * 32, s[k]);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) umma::tmem_ld_32x32(from + 64 + k * 32, d[k]);
+            umma::tmem_ld_32x32(lanes + Shape::kScores + half * 64, s[0]);
+            umma::tmem_ld_32x32(lanes + Shape::kScores + half * 64 + 32, s[1]);
             umma::tmem_ld_wait();
-            const int piece = piece0 + i % per_head;
+            umma::fence_before_thread_sync();
+            __syncwarp();
+            if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->s_read);
+            const int first = (piece0 + i % per_head) * 128 + half * 64;
             // columns [low, high) are visible
             int low = 0, high = 64;
             if (kKeys) {
-                if (a.causal) low = row - shift - piece * 64;
+                if (a.causal) low = row - shift - first;
             } else {
-                high = (a.causal ? min(row + shift + 1, other.y) : other.y) - piece * 64;
+                high = (a.causal ? min(row + shift + 1, other.y) : other.y) - first;
             }
             const bool masked = __any_sync(0xffffffffu, low > 0 || high < 64);
-            uint32_t ps[32], ds[32];
 #pragma unroll
             for (int k = 0; k < 64; k += 2) {
-                if (kKeys && (k & 3) == 0) {
-                    const float4 m4 = *reinterpret_cast<const float4*>(now + k), d4 = *reinterpret_cast<const float4*>(now + 64 + k);
-                    minus2 = f32x2(m4.x, m4.y);
-                    delta2 = f32x2(d4.x, d4.y);
-                } else if (kKeys) {
-                    const float2 m4 = *reinterpret_cast<const float2*>(now + k), d4 = *reinterpret_cast<const float2*>(now + 64 + k);
-                    minus2 = f32x2(m4.x, m4.y);
-                    delta2 = f32x2(d4.x, d4.y);
+                if (kKeys) {
+                    const float2 m = *reinterpret_cast<const float2*>(now + k);
+                    minus2 = f32x2(m.x, m.y);
                 }
-                float x, y, u, v;
+                float x, y;
                 umma::unpack_f32x2(fma2(umma::pack_f32x2(s[k >> 5][k & 31], s[k >> 5][(k & 31) + 1]), c2, minus2), x, y);
-                x = exp2_approx(x);
-                y = exp2_approx(y);
-                umma::unpack_f32x2(mul2(f32x2(x, y), add2(umma::pack_f32x2(d[k >> 5][k & 31], d[k >> 5][(k & 31) + 1]), delta2)), u, v);
-                if (masked) {
-                    const bool see0 = k >= low && k < high, see1 = k + 1 >= low && k + 1 < high;
-                    x = see0 ? x : 0.f;
-                    u = see0 ? u : 0.f;
-                    y = see1 ? y : 0.f;
-                    v = see1 ? v : 0.f;
-                }
-                ps[k >> 1] = pack_bf16(x, y);
-                ds[k >> 1] = pack_bf16(u, v);
+                s[k >> 5][k & 31] = __float_as_uint(x);
+                s[k >> 5][(k & 31) + 1] = __float_as_uint(y);
             }
-            if (kKeys) umma::tmem_st_32x32(from, ps);
-            umma::tmem_st_32x32(from + 64, ds);
+            if (masked)
+#pragma unroll
+                for (int k = 0; k < 64; ++k)
+                    if (k < low || k >= high) s[k >> 5][k & 31] = 0xff800000u;
+#pragma unroll
+            for (int k = 0; k < 64; ++k) s[k >> 5][k & 31] = __float_as_uint(exp2_approx(__uint_as_float(s[k >> 5][k & 31])));
+            ok = attn_wait_warp(&b->dp_full, i & 1, failed, a.report, 5);
+            if (!ok) continue;
+            umma::fence_after_thread_sync();
+            const uint32_t dp = lanes + Shape::kDp + (kKeys ? 0 : (i & 1) * 128) + half * 64;
+            umma::tmem_ld_32x32(dp, d[0]);
+            umma::tmem_ld_32x32(dp + 32, d[1]);
+            umma::tmem_ld_wait();
+            uint32_t out[32];
+            if (kKeys) {
+#pragma unroll
+                for (int k = 0; k < 64; k += 2) out[k >> 1] = pack_bf16(__uint_as_float(s[k >> 5][k & 31]), __uint_as_float(s[k >> 5][(k & 31) + 1]));
+                umma::tmem_st_32x32(dp, out);
+            }
+#pragma unroll
+            for (int k = 0; k < 64; k += 2) {
+                if (kKeys) {
+                    const float2 m = *reinterpret_cast<const float2*>(now + 64 + k);
+                    delta2 = f32x2(m.x, m.y);
+                }
+                float u, v;
+                umma::unpack_f32x2(mul2(umma::pack_f32x2(s[k >> 5][k & 31], s[k >> 5][(k & 31) + 1]), add2(umma::pack_f32x2(d[k >> 5][k & 31], d[k >> 5][(k & 31) + 1]), delta2)), u, v);
+                out[k >> 1] = pack_bf16(u, v);
+            }
+            if (masked) {                             // (zero whatever dP is there)
+#pragma unroll
+                for (int k = 0; k < 64; k += 2) {
+                    const uint32_t keep = (k >= low && k < high ? 0xffffu : 0u) | (k + 1 >= low && k + 1 < high ? 0xffff0000u : 0u);
+                    out[k >> 1] &= keep;
+                }
+            }
+            umma::tmem_st_32x32(dp + 32, out);
             umma::tmem_st_wait();
             umma::fence_before_thread_sync();
             __syncwarp();
             if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->p_full[half]);
         }
-        const int64_t at = (token * heads + head) * a.dim;
+        const int64_t at = (token * (kKeys ? a.kv_heads : a.heads) + head) * a.dim;
+        const float factor = kKeys && half == 1 ? 1.f : a.scale;
+        bf16* out = reinterpret_cast<bf16*>(kKeys ? (half == 0 ? a.dk : a.dv) : a.dq) + at;
+        float* part = nullptr;
+        if (kKeys && a.splits > 1) part = a.parts + (static_cast<int64_t>(split) * 2 + half) * a.tk * a.kv_heads * a.dim + at;
         if (n > 0) {
             ok = ok && attn_wait_warp(&b->sums, 0, failed, a.report, 6);
             if (ok) {
                 umma::fence_after_thread_sync();
                 if (!kKeys) {
                     const int first = half * 32 * kChunks;
-                    store_row<32 * kChunks>(lanes + first, a.scale, reinterpret_cast<bf16*>(a.dq) + at + first, a.dim - first, in);
-                } else if (half == 0) {
-                    store_row<64 * kChunks>(lanes, a.scale, reinterpret_cast<bf16*>(a.dk) + at, a.dim, in);
+                    store_row<32 * kChunks>(lanes + first, factor, out + first, a.dim - first, in);
+                } else if (part != nullptr) {
+                    store_part<64 * kChunks>(lanes + half * 128, factor, part, a.dim, in);
                 } else {
-                    store_row<64 * kChunks>(lanes + 128, 1.f, reinterpret_cast<bf16*>(a.dv) + at, a.dim, in);
+                    store_row<64 * kChunks>(lanes + half * 128, factor, out, a.dim, in);
                 }
             }
-        } else if (in && half == 0) {
+        } else if (in && (kKeys || half == 0)) {
             for (int i = 0; i < a.dim; i += 8) {
-                if (kKeys) {
-                    *reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.dk) + at + i) = make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.dv) + at + i) = make_uint4(0, 0, 0, 0);
-                } else {
-                    *reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.dq) + at + i) = make_uint4(0, 0, 0, 0);
-                }
+                if (part != nullptr) *reinterpret_cast<uint4*>(part + i) = *reinterpret_cast<uint4*>(part + i + 4) = make_uint4(0, 0, 0, 0);
+                else *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
             }
         }
-        const int64_t row_values = static_cast<int64_t>(heads) * a.dim;
-        if (kKeys) {
+        const int64_t row_values = static_cast<int64_t>(kKeys ? a.kv_heads : a.heads) * a.dim;
+        if (!kKeys) {
+            clear_rows<256>(a.cu_q, a.num_seqs, a.tq, blockIdx.x, gridDim.x, reinterpret_cast<bf16*>(a.dq), row_values, nullptr, 0);
+        } else if (part == nullptr) {
             clear_rows<256>(a.cu_k, a.num_seqs, a.tk, blockIdx.x, gridDim.x, reinterpret_cast<bf16*>(a.dk), row_values, nullptr, 0);
             clear_rows<256>(a.cu_k, a.num_seqs, a.tk, blockIdx.x, gridDim.x, reinterpret_cast<bf16*>(a.dv), row_values, nullptr, 0);
-        } else {
-            clear_rows<256>(a.cu_q, a.num_seqs, a.tq, blockIdx.x, gridDim.x, reinterpret_cast<bf16*>(a.dq), row_values, nullptr, 0);
         }
     }
     umma::fence_before_thread_sync();
@@ -958,7 +1023,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
         // (as in the forward pass)
         if (warp == 8 && n > 0) {
             mbar_drain(&b->kept, 0, 100000000ull);
-            for (int i = 0; i < kStages; ++i) mbar_drain(&b->full[i], 0, 100000000ull), mbar_drain(&b->full[i], 1, 100000000ull);
+            for (int i = 0; i < kSlots; ++i) mbar_drain(&b->full[i], 0, 100000000ull), mbar_drain(&b->full[i], 1, 100000000ull);
         }
         if (warp == 9 && ptx::elect_one()) {
             umma::mma_commit(&b->quiet);
@@ -967,6 +1032,29 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
         __syncthreads();
     }
     if (warp == 9) umma::tmem_dealloc(tmem, 512);
+}
+
+// The parts of dK and dV, in their order; rows of no sequence get zeros
+constexpr int kAddThreads = 256;
+__global__ void __launch_bounds__(kAddThreads) attention_add_kernel(const __grid_constant__ AttentionArgs a) {
+    ptx::wait_for_previous_kernel();
+    ptx::let_next_kernel_start();
+    const int64_t row_values = static_cast<int64_t>(a.kv_heads) * a.dim, values = a.tk * row_values;
+    const int64_t at = (static_cast<int64_t>(blockIdx.x) * kAddThreads + threadIdx.x) * 4;
+    if (at >= values) return;
+    const int row = static_cast<int>(at / row_values), first = a.cu_k == nullptr ? 0 : a.cu_k[0], last = a.cu_k == nullptr ? a.tk : a.cu_k[a.num_seqs];
+    const bool in = row >= first && row < last;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (in)
+#pragma unroll 4
+            for (int i = 0; i < a.splits; ++i) {
+                const float4 x = *reinterpret_cast<const float4*>(a.parts + (static_cast<int64_t>(i) * 2 + which) * values + at);
+                sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+            }
+        *reinterpret_cast<uint2*>(static_cast<bf16*>(which == 0 ? a.dk : a.dv) + at) = make_uint2(pack_bf16(sum.x, sum.y), pack_bf16(sum.z, sum.w));
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -1008,37 +1096,48 @@ cudaError_t launch_forward(const AttentionArgs& a, cudaStream_t stream) {
     return launch_dependent(fn, dim3(static_cast<unsigned>(num_blocks<256>(a.tq, a.num_seqs) * a.heads)), dim3(kFwdThreads), params, FwdShape<kChunks>::kSmem, stream);
 }
 template <int kChunks, bool kKeys>
-cudaError_t launch_gradient(const AttentionArgs& a, cudaStream_t stream) {
+cudaError_t launch_gradient(const AttentionArgs& a, const CUtensorMap& q, const CUtensorMap& d, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t stream) {
     const void* fn = reinterpret_cast<const void*>(attention_backward_kernel<kChunks, kKeys>);
     static std::atomic<uint64_t> allowed{0};
-    const cudaError_t err = allow_once(fn, BwdShape<kChunks>::kSmem, allowed);
+    const cudaError_t err = allow_once(fn, BwdShape<kChunks, kKeys>::kSmem, allowed);
     if (err != cudaSuccess) return err;
-    CUtensorMap q, k, v, d;
-    const int queries = kKeys ? 64 : 128, keys = kKeys ? 128 : 64;
-    if (!make_map(&q, a.q, a.tq, a.heads, a.dim, queries) || !make_map(&d, a.d_o, a.tq, a.heads, a.dim, queries) || !make_map(&k, a.k, a.tk, a.kv_heads, a.dim, keys) ||
-        !make_map(&v, a.v, a.tk, a.kv_heads, a.dim, keys))
-        return cudaErrorInvalidValue;
-    void* params[] = {kKeys ? &k : &q, kKeys ? &v : &d, kKeys ? &q : &k, kKeys ? &d : &v, const_cast<AttentionArgs*>(&a)};
-    const int64_t ctas = num_blocks<128>(kKeys ? a.tk : a.tq, a.num_seqs) * (kKeys ? a.kv_heads : a.heads);
-    return launch_dependent(fn, dim3(static_cast<unsigned>(ctas)), dim3(kBwdThreads), params, BwdShape<kChunks>::kSmem, stream);
+    const CUtensorMap* maps[4] = {kKeys ? &k : &q, kKeys ? &v : &d, kKeys ? &q : &k, kKeys ? &d : &v};
+    void* params[] = {const_cast<CUtensorMap*>(maps[0]), const_cast<CUtensorMap*>(maps[1]), const_cast<CUtensorMap*>(maps[2]), const_cast<CUtensorMap*>(maps[3]),
+                      const_cast<AttentionArgs*>(&a)};
+    const int64_t ctas = num_blocks<128>(kKeys ? a.tk : a.tq, a.num_seqs) * (kKeys ? a.kv_heads * a.splits : a.heads);
+    return launch_dependent(fn, dim3(static_cast<unsigned>(ctas)), dim3(kBwdThreads), params, BwdShape<kChunks, kKeys>::kSmem, stream);
 }
 template <int kChunks>
 cudaError_t launch_backward(const AttentionArgs& a, cudaStream_t stream) {
+    CUtensorMap q, k, v, d;
+    if (!make_map(&q, a.q, a.tq, a.heads, a.dim, 128) || !make_map(&d, a.d_o, a.tq, a.heads, a.dim, 128) || !make_map(&k, a.k, a.tk, a.kv_heads, a.dim, 128) ||
+        !make_map(&v, a.v, a.tk, a.kv_heads, a.dim, 128))
+        return cudaErrorInvalidValue;
     void* params[] = {const_cast<AttentionArgs*>(&a)};
     const int64_t rows = static_cast<int64_t>(a.tq) * a.heads;
     cudaError_t err = launch_dependent(reinterpret_cast<const void*>(attention_delta_kernel), dim3(static_cast<unsigned>((rows * 16 + kDeltaThreads - 1) / kDeltaThreads)),
                                        dim3(kDeltaThreads), params, 0, stream);
-    if (err == cudaSuccess) err = launch_gradient<kChunks, true>(a, stream);
-    if (err == cudaSuccess) err = launch_gradient<kChunks, false>(a, stream);
+    if (err == cudaSuccess) err = launch_gradient<kChunks, true>(a, q, d, k, v, stream);
+    if (err == cudaSuccess) err = launch_gradient<kChunks, false>(a, q, d, k, v, stream);
+    if (err == cudaSuccess && a.splits > 1) {
+        const int64_t values = static_cast<int64_t>(a.tk) * a.kv_heads * a.dim;
+        err = launch_dependent(reinterpret_cast<const void*>(attention_add_kernel), dim3(static_cast<unsigned>((values / 4 + kAddThreads - 1) / kAddThreads)), dim3(kAddThreads), params, 0,
+                               stream);
+    }
     return err;
 }
 
 }  // namespace
 
-cudaError_t launch_attention(const AttentionArgs& a, int num_sms, cudaStream_t stream) {
+cudaError_t launch_attention(const AttentionArgs& a, cudaStream_t stream) {
     return a.dim <= 64 ? launch_forward<1>(a, stream) : launch_forward<2>(a, stream);
 }
-cudaError_t launch_attention_backward(const AttentionArgs& a, int num_sms, cudaStream_t stream) {
+// Parts of a group whose gradients of keys and values are made by CTAs of their own, and then added (8 bytes per part and value each way): as many as give every SM two.
+int attention_backward_splits(const AttentionArgs& a, int num_sms) {
+    const int64_t ctas = std::max<int64_t>(1, std::max(a.tk / 128, 1) * a.kv_heads);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(a.heads / a.kv_heads, 2 * num_sms / ctas)));
+}
+cudaError_t launch_attention_backward(const AttentionArgs& a, cudaStream_t stream) {
     return a.dim <= 64 ? launch_backward<1>(a, stream) : launch_backward<2>(a, stream);
 }
 

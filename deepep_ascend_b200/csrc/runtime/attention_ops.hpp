@@ -82,7 +82,7 @@ inline std::optional<std::tuple<at::Tensor, at::Tensor>> attention(const at::Ten
     in.a.o = o.data_ptr();
     in.a.lse = lse.data_ptr<float>();
     report_through(in.a.report, error, report_to);
-    cuda_check(ep::launch_attention(in.a, device_sms(), at::cuda::getCurrentCUDAStream()), "attention launch");
+    cuda_check(ep::launch_attention(in.a, at::cuda::getCurrentCUDAStream()), "attention launch");
     return std::make_tuple(o, lse);
 }
 
@@ -108,11 +108,17 @@ inline std::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor>> attention_b
     in.a.lse_in = lse.data_ptr<float>();
     in.a.d_lse = d_lse.has_value() ? d_lse->data_ptr<float>() : nullptr;
     in.a.delta = delta.data_ptr<float>();
+    in.a.splits = ep::attention_backward_splits(in.a, device_sms());
+    at::Tensor parts;
+    if (in.a.splits > 1) {
+        parts = at::empty({in.a.splits, 2, k.numel()}, lse.options());
+        in.a.parts = parts.data_ptr<float>();
+    }
     in.a.dq = dq.data_ptr();
     in.a.dk = dk.data_ptr();
     in.a.dv = dv.data_ptr();
     report_through(in.a.report, error, report_to);
-    cuda_check(ep::launch_attention_backward(in.a, device_sms(), at::cuda::getCurrentCUDAStream()), "attention gradient launch");
+    cuda_check(ep::launch_attention_backward(in.a, at::cuda::getCurrentCUDAStream()), "attention gradient launch");
     return std::make_tuple(dq, dk, dv);
 }
 
