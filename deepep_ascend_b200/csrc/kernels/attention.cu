@@ -212,9 +212,16 @@ __device__ __forceinline__ uint64_t exp2_by_polynomial(uint64_t x2) {
 }
 constexpr int kPolynomialOf = 4;                     // of so many pairs of a row one goes by the polynomial
 
-// The two groups of four warps that hold rows take registers of the third: 384 x 168 at launch = 128 x (224 + 224 + 56)
-__device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 224;"); }
-__device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 56;"); }
+// The two groups of four warps that hold rows take registers of the third: 384 x 168 at launch = 128 x (2 rows' + the others')
+constexpr int kFwdRegisters = 224, kBwdRegisters = 208;
+template <int kRows>
+__device__ __forceinline__ void take_registers() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRows));
+}
+template <int kRows>
+__device__ __forceinline__ void give_registers() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(3 * 168 - 2 * kRows));
+}
 
 // A row of sums in tensor memory, times `factor`, as bf16
 template <int kColumns>
@@ -287,12 +294,14 @@ struct FwdBars {
     AttnState st;
 };
 // The next block of the grid that no CTA has started yet, or -1
-__device__ __forceinline__ void request_work(FwdBars* b) {
+template <class Bars>
+__device__ __forceinline__ void request_work(Bars* b) {
     ptx::mbar_arrive_expect_tx(&b->answered, 16);
     asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(ptx::smem_u32(&b->answer)), "r"(ptx::smem_u32(&b->answered))
                  : "memory");
 }
-__device__ __forceinline__ int work_of_answer(FwdBars* b) {
+template <class Bars>
+__device__ __forceinline__ int work_of_answer(Bars* b) {
     uint32_t x, got;
     asm volatile(
         "{\n .reg .pred p;\n .reg .b128 a;\n .reg .b32 y, z, w;\n ld.shared.b128 a, [%2];\n clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n"
@@ -358,7 +367,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     };
 
     if (warp >= 8) {
-        give_registers();
+        give_registers<kFwdRegisters>();
         if (warp == 8) {
             AttnRing<kStages> p;
             const bool one = ptx::elect_one();
@@ -511,7 +520,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             }
         }
     } else {
-        take_registers();
+        take_registers<kFwdRegisters>();
         const int t = warp >> 2, lane_row = threadIdx.x & 127;
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), ts = lanes + t * 128, to = lanes + Shape::kOut + t * 128;
         const float c = a.scale * kLog2e;
@@ -702,7 +711,8 @@ __global__ void __launch_bounds__(kDeltaThreads) attention_delta_kernel(const __
 // Two groups of four warps have 64 columns of a piece each.  P and dS take the place of dP; that of the scores is free as soon as they are in registers, so the next piece's
 // scores are made meanwhile, and their powers while dV, dK and the next dP are.  (Pieces of 64 columns with two places for each had products of half the width, which take as long
 // as whole ones: 128 rows of the first operand come from shared memory either way.)
-constexpr int kBwdThreads = 384;                     // 2 x 4 warps for rows, one that requests pieces, one that issues products, two without work
+constexpr int kBwdThreads = 384;                     // 2 x 4 warps for rows, one that requests pieces, one that issues products, one that looks for work, one without any
+constexpr int kBwdReaders = 10;
 template <int kChunks, bool kKeys>
 struct BwdShape {
     static constexpr int kTileBytes = 128 * 128 * kChunks, kSlots = kChunks == 2 ? 5 : 8;
@@ -711,8 +721,17 @@ struct BwdShape {
     static constexpr int kStatBytes = 2 * 2 * 128 * 4;
     static constexpr int kSmem = (2 + kSlots) * kTileBytes + kStatBytes + 1024;
 };
+struct BwdWork {
+    int start, row0, rows;           // as of AttnBlock; rows < 0: no more work
+    int other0, others;              // rows of the other side
+    int head, first_head, split;     // kept head, first head of the pieces
+    int piece0, per_head, n;         // pieces [piece0, piece0 + per_head) of every head, pieces in all
+};
+// (dP and what is made of it in turn by pieces: with two places for dP, the next one's can be there before a slow warp has looked for this one's)
 struct BwdBars {
-    uint64_t kept, full[8], empty[8], s_full, s_read, dp_full, p_full[2], sums, tail, quiet;
+    alignas(16) uint4 answer;
+    BwdWork work;
+    uint64_t kept, kept_empty, full[8], empty[8], s_full, s_read, dp_full[2], p_full[2][2], stats_full[2], sums, drained, work_full, work_read, answered, tail, quiet;
     AttnState st;
 };
 
@@ -733,15 +752,23 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
         umma::prefetch_tensormap(&map_piece0);
         umma::prefetch_tensormap(&map_piece1);
         ptx::mbar_init(&b->kept, 1);
+        ptx::mbar_init(&b->kept_empty, 1);
+        ptx::mbar_init(&b->drained, 8);
+        ptx::mbar_init(&b->work_full, 1);
+        ptx::mbar_init(&b->work_read, kBwdReaders);
+        ptx::mbar_init(&b->answered, 1);
         for (int i = 0; i < kSlots; ++i) {
             ptx::mbar_init(&b->full[i], 1);
             ptx::mbar_init(&b->empty[i], 1);
         }
         ptx::mbar_init(&b->s_full, 1);
         ptx::mbar_init(&b->s_read, 8);
-        ptx::mbar_init(&b->dp_full, 1);
-        ptx::mbar_init(&b->p_full[0], 4);
-        ptx::mbar_init(&b->p_full[1], 4);
+        for (int i = 0; i < 2; ++i) {
+            ptx::mbar_init(&b->dp_full[i], 1);
+            ptx::mbar_init(&b->p_full[i][0], 4);
+            ptx::mbar_init(&b->p_full[i][1], 4);
+            ptx::mbar_init(&b->stats_full[i], 4);
+        }
         ptx::mbar_init(&b->sums, 1);
         ptx::mbar_init(&b->tail, 1);
         ptx::mbar_init(&b->quiet, 1);
@@ -757,272 +784,339 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
     umma::fence_after_thread_sync();
     const uint32_t tmem = b->st.tmem_base;
     ptx::wait_for_previous_kernel();
-    ptx::let_next_kernel_start();
     int* failed = &b->st.failed;
-    // (kKeys: the first keys are seen by most queries; otherwise the last queries see most keys.  Long blocks first.)
-    const int units = kKeys ? a.kv_heads * a.splits : a.heads, total = kKeys ? a.tk : a.tq;
-    const int unit = blockIdx.x % units, number = blockIdx.x / units;
-    const int head = kKeys ? unit / a.splits : unit, split = kKeys ? unit % a.splits : 0;      // (of keys, or of queries)
-    const int first_head = kKeys ? head * group + group * split / a.splits : 0, num_heads = kKeys ? head * group + group * (split + 1) / a.splits - first_head : 1;
-    const AttnBlock blk = find_block<128>(kKeys ? a.cu_k : a.cu_q, a.num_seqs, total, kKeys ? number : static_cast<int>(gridDim.x / units) - 1 - number);
-    const int2 other = sequence_rows(kKeys ? a.cu_q : a.cu_k, blk.seq, kKeys ? a.tq : a.tk);
-    const int shift = kKeys ? blk.rows - other.y : other.y - blk.rows;     // query i sees the keys up to i + shift
-    // pieces [piece0, piece1) of every head
-    int piece0 = 0, piece1 = 0, n = 0;
-    if (blk.row0 < blk.rows) {
-        if (kKeys) {
-            piece0 = a.causal ? max(blk.row0 - shift, 0) / 128 : 0;
-            piece1 = (other.y + 127) / 128;
-        } else {
-            const int seen = a.causal ? min(min(blk.row0 + 128, blk.rows) + shift, other.y) : other.y;
-            piece1 = seen <= 0 ? 0 : (seen + 127) / 128;
-        }
-        n = max(piece1 - piece0, 0) * num_heads;
-    }
-    const int per_head = max(piece1 - piece0, 1);
+    // The k-th block of this CTA, for a whole warp; false: no more
+    auto next_work = [&](int k, BwdWork& w) {
+        if (!attn_wait_warp(&b->work_full, k & 1, failed, a.report, 7)) return false;
+        w = b->work;
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->work_read);
+        return w.rows >= 0;
+    };
 
     if (warp >= 8) {
-        give_registers();
+        give_registers<kBwdRegisters>();
         if (warp == 8) {
-            if (n > 0) {
-                AttnRing<kSlots> p;
-                const bool one = ptx::elect_one();
+            AttnRing<kSlots> p;
+            const bool one = ptx::elect_one();
+            uint32_t tails = 0, blocks = 0;
+            BwdWork w;
+            auto request = [&](const CUtensorMap* map, int h, int piece) {
+                if (!attn_wait_warp(&b->empty[p.stage], p.phase ^ 1, failed, a.report, 1)) return false;
+                uint8_t* tile = pieces + p.stage * kTileBytes;
+                const bool tail = piece * 128 + 128 > w.others;
+                uint64_t* bar = tail ? &b->tail : &b->full[p.stage];
                 if (one) {
-                    ptx::mbar_arrive_expect_tx(&b->kept, 2 * kTileBytes);
-                    load_tile<128, kChunks>(kept, &map_kept0, head, blk.start + blk.row0, &b->kept);
-                    load_tile<128, kChunks>(kept + kTileBytes, &map_kept1, head, blk.start + blk.row0, &b->kept);
+                    ptx::mbar_arrive_expect_tx(bar, kTileBytes);
+                    load_tile<128, kChunks>(tile, map, h, w.other0 + piece * 128, bar);
                 }
                 __syncwarp();
-                uint32_t tails = 0;
-                auto request = [&](const CUtensorMap* map, int h, int piece) {
-                    if (!attn_wait_warp(&b->empty[p.stage], p.phase ^ 1, failed, a.report, 1)) return false;
-                    uint8_t* tile = pieces + p.stage * kTileBytes;
-                    const bool tail = piece * 128 + 128 > other.y;
-                    uint64_t* bar = tail ? &b->tail : &b->full[p.stage];
+                if (tail) {
+                    if (!attn_wait_warp(&b->tail, tails & 1, failed, a.report, 4)) return false;
+                    ++tails;
+                    clear_tile<128, kChunks>(tile, w.others - piece * 128);
+                    if (one) ptx::mbar_arrive(&b->full[p.stage]);
+                }
+                p.advance();
+                return true;
+            };
+            auto load = [&]() {
+                for (int k = 0; next_work(k, w); ++k) {
+                    if (w.n == 0) continue;
+                    if (!attn_wait_warp(&b->kept_empty, (blocks & 1) ^ 1, failed, a.report, 1)) return;
+                    ++blocks;
                     if (one) {
-                        ptx::mbar_arrive_expect_tx(bar, kTileBytes);
-                        load_tile<128, kChunks>(tile, map, h, other.x + piece * 128, bar);
+                        ptx::mbar_arrive_expect_tx(&b->kept, 2 * kTileBytes);
+                        load_tile<128, kChunks>(kept, &map_kept0, w.head, w.start + w.row0, &b->kept);
+                        load_tile<128, kChunks>(kept + kTileBytes, &map_kept1, w.head, w.start + w.row0, &b->kept);
                     }
                     __syncwarp();
-                    if (tail) {
-                        if (!attn_wait_warp(&b->tail, tails & 1, failed, a.report, 4)) return false;
-                        ++tails;
-                        clear_tile<128, kChunks>(tile, other.y - piece * 128);
-                        if (one) ptx::mbar_arrive(&b->full[p.stage]);
+                    for (int i = 0; i < w.n; ++i) {
+                        const int h = kKeys ? w.first_head + i / w.per_head : w.head / group, piece = w.piece0 + i % w.per_head;
+                        if (!request(&map_piece0, h, piece) || !request(&map_piece1, h, piece)) return;
                     }
-                    p.advance();
-                    return true;
-                };
-                for (int i = 0; i < n; ++i) {
-                    const int h = kKeys ? first_head + i / per_head : head / group, piece = piece0 + i % per_head;
-                    if (!request(&map_piece0, h, piece) || !request(&map_piece1, h, piece)) break;
                 }
-            }
+            };
+            load();
         } else if (warp == 9) {
-            if (n > 0 && ptx::elect_one()) {
-                const int dim16 = (a.dim + 15) / 16;
-                const uint32_t idesc_s = umma::make_instr_desc(128, 128, umma::kFormatBF16);
-                const uint32_t idesc_o = umma::make_instr_desc(128, 16, umma::kFormatBF16, false, true) + (static_cast<uint32_t>(2 * dim16 - 2) << 17);
-                const uint32_t kept_of = desc_channels(kept), pieces_of = desc_channels(pieces), rows_of = desc_rows<128>(pieces);
-                AttnRing<kSlots> p;                   // operands in the order in which they come: first and second of every piece
-                // the first products of piece i, of its first or second operand
-                auto product = [&](int which, uint32_t to, uint64_t* done, int& slot) {
-                    if (!attn_wait(&b->full[p.stage], p.phase, failed, a.report, 4)) return false;
-                    umma::fence_after_thread_sync();
-                    multiply_channels<128, 128, kChunks>(tmem + to, kept_of + which * (kTileBytes / 16), pieces_of + p.stage * (kTileBytes / 16), idesc_s, dim16);
-                    umma::mma_commit(done);
-                    slot = p.stage;
-                    p.advance();
-                    return true;
-                };
-                auto multiply = [&]() {
-                    if (!attn_wait(&b->kept, 0, failed, a.report, 4)) return;
-                    int slot0, slot1, next0 = 0, next1 = 0;
-                    if (!product(0, Shape::kScores, &b->s_full, slot0) || !product(1, Shape::kDp, &b->dp_full, slot1)) return;
-                    if (!kKeys) umma::mma_commit(&b->empty[slot1]);
-                    for (int i = 0; i < n; ++i) {
-                        const uint32_t dp = Shape::kDp + (kKeys ? 0 : (i & 1) * 128);
-                        if (i + 1 < n) {
-                            if (!attn_wait(&b->s_read, i & 1, failed, a.report, 3)) return;
-                            if (!product(0, Shape::kScores, &b->s_full, next0)) return;
-                            if (!kKeys) {
-                                // (the other place of dP: what was there is behind the products before)
-                                if (!product(1, Shape::kDp + (~i & 1) * 128, &b->dp_full, next1)) return;
-                                umma::mma_commit(&b->empty[next1]);
-                            }
+            const bool one = ptx::elect_one();
+            const int dim16 = (a.dim + 15) / 16;
+            const uint32_t idesc_s = umma::make_instr_desc(128, 128, umma::kFormatBF16);
+            const uint32_t idesc_o = umma::make_instr_desc(128, 16, umma::kFormatBF16, false, true) + (static_cast<uint32_t>(2 * dim16 - 2) << 17);
+            const uint32_t kept_of = desc_channels(kept), pieces_of = desc_channels(pieces), rows_of = desc_rows<128>(pieces);
+            AttnRing<kSlots> p;                       // operands in the order in which they come: first and second of every piece
+            uint32_t made = 0, blocks = 0;            // pieces, blocks so far
+            // the first products of a piece, of its first or second operand
+            auto product = [&](int which, uint32_t to, uint64_t* done, int& slot) {
+                if (!attn_wait(&b->full[p.stage], p.phase, failed, a.report, 4)) return false;
+                umma::fence_after_thread_sync();
+                multiply_channels<128, 128, kChunks>(tmem + to, kept_of + which * (kTileBytes / 16), pieces_of + p.stage * (kTileBytes / 16), idesc_s, dim16);
+                umma::mma_commit(done);
+                slot = p.stage;
+                p.advance();
+                return true;
+            };
+            auto multiply = [&](int n) {
+                if (!attn_wait(&b->kept, blocks & 1, failed, a.report, 4)) return;
+                int slot0, slot1, next0 = 0, next1 = 0;
+                if (!product(0, Shape::kScores, &b->s_full, slot0) || !product(1, Shape::kDp + (kKeys ? 0 : (made & 1) * 128), &b->dp_full[made & 1], slot1)) return;
+                if (!kKeys) umma::mma_commit(&b->empty[slot1]);
+                if (n == 1) umma::mma_commit(&b->kept_empty);
+                // (the sums of the block before have been read)
+                if (blocks > 0 && !attn_wait(&b->drained, (blocks - 1) & 1, failed, a.report, 6)) return;
+                ++blocks;
+                for (int i = 0; i < n; ++i, ++made) {
+                    const uint32_t dp = Shape::kDp + (kKeys ? 0 : (made & 1) * 128);
+                    if (i + 1 < n) {
+                        if (!attn_wait(&b->s_read, made & 1, failed, a.report, 3)) return;
+                        if (!product(0, Shape::kScores, &b->s_full, next0)) return;
+                        if (!kKeys) {
+                            // (the other place of dP: what was there is behind the products before)
+                            if (!product(1, Shape::kDp + (~made & 1) * 128, &b->dp_full[~made & 1], next1)) return;
+                            umma::mma_commit(&b->empty[next1]);
+                            if (i + 2 == n) umma::mma_commit(&b->kept_empty);
                         }
-                        const uint32_t rows0 = rows_of + slot0 * (kTileBytes / 16), rows1 = rows_of + slot1 * (kTileBytes / 16);
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            if (!attn_wait(&b->p_full[half], i & 1, failed, a.report, 2)) return;
-                            umma::fence_after_thread_sync();
-                            const uint32_t from = tmem + dp + half * 64, step = half * 4 * 16 * 128 / 16;
-                            if (kKeys) multiply_rows<0, 4>(tmem + 128, from, rows1 + step, idesc_o, i != 0 || half != 0);
-                            multiply_rows<0, 4>(tmem, from + 32, rows0 + step, idesc_o, i != 0 || half != 0);
-                        }
-                        umma::mma_commit(&b->empty[slot0]);
-                        if (kKeys) {
-                            umma::mma_commit(&b->empty[slot1]);
-                            if (i + 1 < n && !product(1, Shape::kDp, &b->dp_full, next1)) return;
-                        }
-                        slot0 = next0;
-                        slot1 = next1;
                     }
-                    umma::mma_commit(&b->sums);
-                };
-                multiply();
+                    const uint32_t rows0 = rows_of + slot0 * (kTileBytes / 16), rows1 = rows_of + slot1 * (kTileBytes / 16);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        if (!attn_wait(&b->p_full[half][made & 1], made >> 1 & 1, failed, a.report, 2)) return;
+                        umma::fence_after_thread_sync();
+                        const uint32_t from = tmem + dp + half * 64, step = half * 4 * 16 * 128 / 16;
+                        if (kKeys) multiply_rows<0, 4>(tmem + 128, from, rows1 + step, idesc_o, i != 0 || half != 0);
+                        multiply_rows<0, 4>(tmem, from + 32, rows0 + step, idesc_o, i != 0 || half != 0);
+                    }
+                    umma::mma_commit(&b->empty[slot0]);
+                    if (kKeys) {
+                        umma::mma_commit(&b->empty[slot1]);
+                        if (i + 1 < n) {
+                            if (!product(1, Shape::kDp, &b->dp_full[~made & 1], next1)) return;
+                            if (i + 2 == n) umma::mma_commit(&b->kept_empty);
+                        }
+                    }
+                    slot0 = next0;
+                    slot1 = next1;
+                }
+                umma::mma_commit(&b->sums);
+                // (nobody waits for the last piece's scores to be read)
+            };
+            BwdWork w;
+            for (int k = 0; next_work(k, w); ++k) {
+                if (one && w.n > 0) multiply(w.n);
+                __syncwarp();
+            }
+        } else if (warp == 10) {
+            // looks for work: first this CTA's own
+            const int units = kKeys ? a.kv_heads * a.splits : a.heads;
+            int item = blockIdx.x;
+            uint32_t handed = 0;
+            for (uint32_t answers = 0;; ++answers) {
+                BwdWork w{};
+                w.rows = -1;
+                bool something = true;
+                if (item >= 0) {
+                    // (kKeys: the first keys are seen by most queries; otherwise the last queries see most keys.  Long blocks first.)
+                    const int unit = item % units, number = item / units;
+                    w.head = kKeys ? unit / a.splits : unit;      // (of keys, or of queries)
+                    w.split = kKeys ? unit % a.splits : 0;
+                    w.first_head = kKeys ? w.head * group + group * w.split / a.splits : 0;
+                    const int num_heads = kKeys ? w.head * group + group * (w.split + 1) / a.splits - w.first_head : 1;
+                    const AttnBlock blk =
+                        find_block<128>(kKeys ? a.cu_k : a.cu_q, a.num_seqs, kKeys ? a.tk : a.tq, kKeys ? number : static_cast<int>(gridDim.x / units) - 1 - number);
+                    const int2 other = sequence_rows(kKeys ? a.cu_q : a.cu_k, blk.seq, kKeys ? a.tq : a.tk);
+                    const int shift = kKeys ? blk.rows - other.y : other.y - blk.rows;
+                    w.start = blk.start;
+                    w.row0 = blk.row0;
+                    w.rows = blk.rows;
+                    w.other0 = other.x;
+                    w.others = other.y;
+                    something = blk.row0 < blk.rows;
+                    int piece1 = (other.y + 127) / 128;
+                    if (kKeys) {
+                        w.piece0 = a.causal ? max(blk.row0 - shift, 0) / 128 : 0;
+                    } else if (a.causal) {
+                        const int seen = min(min(blk.row0 + 128, blk.rows) + shift, other.y);
+                        piece1 = seen <= 0 ? 0 : (seen + 127) / 128;
+                    }
+                    w.per_head = max(piece1 - w.piece0, 0);
+                    w.n = w.per_head * num_heads;
+                    const int64_t row_values = static_cast<int64_t>(kKeys ? a.kv_heads : a.heads) * a.dim;
+                    if (!kKeys) {
+                        clear_rows<32>(a.cu_q, a.num_seqs, a.tq, item, gridDim.x, reinterpret_cast<bf16*>(a.dq), row_values, nullptr, 0);
+                    } else if (a.splits == 1) {
+                        clear_rows<32>(a.cu_k, a.num_seqs, a.tk, item, gridDim.x, reinterpret_cast<bf16*>(a.dk), row_values, nullptr, 0);
+                        clear_rows<32>(a.cu_k, a.num_seqs, a.tk, item, gridDim.x, reinterpret_cast<bf16*>(a.dv), row_values, nullptr, 0);
+                    }
+                }
+                if (something) {                      // (numbers without a block are passed over)
+                    if ((threadIdx.x & 31) == 0) {
+                        b->work = w;
+                        ptx::mbar_arrive(&b->work_full);
+                    }
+                    if (w.rows < 0 || !attn_wait_warp(&b->work_read, handed & 1, failed, a.report, 7)) break;
+                    ++handed;
+                }
+                if ((threadIdx.x & 31) == 0) request_work(b);
+                if (!attn_wait_warp(&b->answered, answers & 1, failed, a.report, 7)) break;
+                item = work_of_answer(b);
+                __syncwarp();
             }
         }
     } else {
-        take_registers();
-        const int half = warp >> 2, lane_row = threadIdx.x & 127, row = blk.row0 + lane_row;
+        take_registers<kBwdRegisters>();
+        const int half = warp >> 2, lane_row = threadIdx.x & 127;
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const float c = a.scale * kLog2e;
-        const bool in = row < blk.rows;
-        const int64_t token = blk.start + row;
         float* mine = stats + half * 256;             // twice: 64 times -lse log2 e, 64 times -delta
-        // a statistic of a query that sees nothing, or that is none: its probabilities are zero
-        auto statistic = [&](bool is_delta, bool is_there, int h, int64_t query) {
-            if (!is_there) return is_delta ? 0.f : kNone;
-            const int64_t at = static_cast<int64_t>(h) * a.tq + query;
-            if (is_delta) return -a.delta[at];
-            const float l = a.lse_in[at];
-            return l == kNone ? kNone : -l * kLog2e;
-        };
-        auto next_statistic = [&](int i) {
-            if (i >= n) return 0.f;
-            const int at = (piece0 + i % per_head) * 128 + half * 64 + (lane_row & 63);
-            return statistic(lane_row >= 64, at < other.y, first_head + i / per_head, other.x + at);
-        };
-        float coming = 0.f;
-        uint64_t minus2 = 0, delta2 = 0;
-        if (kKeys) {
-            coming = next_statistic(0);
-        } else if (n > 0) {
-            const float m = statistic(false, in, head, token), d = statistic(true, in, head, token);
-            minus2 = f32x2(m, m);
-            delta2 = f32x2(d, d);
-        }
-        bool ok = true;
         const uint64_t c2 = f32x2(c, c);
-        for (int i = 0; i < n; ++i) {
-            const float* now = mine + (i & 1) * 128;
+        uint32_t made = 0, ended = 0;                 // pieces, blocks so far
+        bool ok = true;
+        BwdWork w;
+        for (int k = 0; ok && next_work(k, w); ++k) {
+            const int row = w.row0 + lane_row, shift = kKeys ? w.rows - w.others : w.others - w.rows;     // query i sees the keys up to i + shift
+            const bool in = row < w.rows;
+            const int64_t token = w.start + row;
+            // a statistic of a query that sees nothing, or that is none: its probabilities are zero
+            auto statistic = [&](bool is_delta, bool is_there, int h, int64_t query) {
+                if (!is_there) return is_delta ? 0.f : kNone;
+                const int64_t at = static_cast<int64_t>(h) * a.tq + query;
+                if (is_delta) return -a.delta[at];
+                const float l = a.lse_in[at];
+                return l == kNone ? kNone : -l * kLog2e;
+            };
+            auto next_statistic = [&](int i) {
+                if (i >= w.n) return 0.f;
+                const int at = (w.piece0 + i % w.per_head) * 128 + half * 64 + (lane_row & 63);
+                return statistic(lane_row >= 64, at < w.others, w.first_head + i / w.per_head, w.other0 + at);
+            };
+            float coming = 0.f;
+            uint64_t minus2 = 0, delta2 = 0;
             if (kKeys) {
-                mine[(i & 1) * 128 + lane_row] = coming;
-                if (half == 0) asm volatile("bar.sync 1, 128;" ::: "memory");
-                else asm volatile("bar.sync 2, 128;" ::: "memory");
-                coming = next_statistic(i + 1);
+                coming = next_statistic(0);
+            } else if (w.n > 0) {
+                const float m = statistic(false, in, w.head, token), d = statistic(true, in, w.head, token);
+                minus2 = f32x2(m, m);
+                delta2 = f32x2(d, d);
             }
-            ok = ok && attn_wait_warp(&b->s_full, i & 1, failed, a.report, 5);
-            if (!ok) continue;                        // (the others may wait at the barrier above)
-            umma::fence_after_thread_sync();
-            uint32_t s[2][32], d[2][32];
-            umma::tmem_ld_32x32(lanes + Shape::kScores + half * 64, s[0]);
-            umma::tmem_ld_32x32(lanes + Shape::kScores + half * 64 + 32, s[1]);
-            umma::tmem_ld_wait();
-            umma::fence_before_thread_sync();
-            __syncwarp();
-            if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->s_read);
-            const int first = (piece0 + i % per_head) * 128 + half * 64;
-            // columns [low, high) are visible
-            int low = 0, high = 64;
-            if (kKeys) {
-                if (a.causal) low = row - shift - first;
-            } else {
-                high = (a.causal ? min(row + shift + 1, other.y) : other.y) - first;
-            }
-            const bool masked = __any_sync(0xffffffffu, low > 0 || high < 64);
-#pragma unroll
-            for (int k = 0; k < 64; k += 2) {
+            for (int i = 0; i < w.n; ++i, ++made) {
+                const float* now = mine + (made & 1) * 128;
                 if (kKeys) {
-                    const float2 m = *reinterpret_cast<const float2*>(now + k);
-                    minus2 = f32x2(m.x, m.y);
+                    mine[(made & 1) * 128 + lane_row] = coming;
+                    __syncwarp();
+                    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->stats_full[half]);
+                    coming = next_statistic(i + 1);
+                    ok = attn_wait_warp(&b->stats_full[half], made & 1, failed, a.report, 6);
+                    if (!ok) break;
                 }
-                float x, y;
-                umma::unpack_f32x2(fma2(umma::pack_f32x2(s[k >> 5][k & 31], s[k >> 5][(k & 31) + 1]), c2, minus2), x, y);
-                s[k >> 5][k & 31] = __float_as_uint(x);
-                s[k >> 5][(k & 31) + 1] = __float_as_uint(y);
-            }
-            if (masked)
-#pragma unroll
-                for (int k = 0; k < 64; ++k)
-                    if (k < low || k >= high) s[k >> 5][k & 31] = 0xff800000u;
-#pragma unroll
-            for (int k = 0; k < 64; ++k) s[k >> 5][k & 31] = __float_as_uint(exp2_approx(__uint_as_float(s[k >> 5][k & 31])));
-            ok = attn_wait_warp(&b->dp_full, i & 1, failed, a.report, 5);
-            if (!ok) continue;
-            umma::fence_after_thread_sync();
-            const uint32_t dp = lanes + Shape::kDp + (kKeys ? 0 : (i & 1) * 128) + half * 64;
-            umma::tmem_ld_32x32(dp, d[0]);
-            umma::tmem_ld_32x32(dp + 32, d[1]);
-            umma::tmem_ld_wait();
-            uint32_t out[32];
-            if (kKeys) {
-#pragma unroll
-                for (int k = 0; k < 64; k += 2) out[k >> 1] = pack_bf16(__uint_as_float(s[k >> 5][k & 31]), __uint_as_float(s[k >> 5][(k & 31) + 1]));
-                umma::tmem_st_32x32(dp, out);
-            }
-#pragma unroll
-            for (int k = 0; k < 64; k += 2) {
+                ok = attn_wait_warp(&b->s_full, made & 1, failed, a.report, 5);
+                if (!ok) break;
+                umma::fence_after_thread_sync();
+                uint32_t s[2][32], d[2][32];
+                umma::tmem_ld_32x32(lanes + Shape::kScores + half * 64, s[0]);
+                umma::tmem_ld_32x32(lanes + Shape::kScores + half * 64 + 32, s[1]);
+                umma::tmem_ld_wait();
+                umma::fence_before_thread_sync();
+                __syncwarp();
+                if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->s_read);
+                const int first = (w.piece0 + i % w.per_head) * 128 + half * 64;
+                // columns [low, high) are visible
+                int low = 0, high = 64;
                 if (kKeys) {
-                    const float2 m = *reinterpret_cast<const float2*>(now + 64 + k);
-                    delta2 = f32x2(m.x, m.y);
+                    if (a.causal) low = row - shift - first;
+                } else {
+                    high = (a.causal ? min(row + shift + 1, w.others) : w.others) - first;
                 }
-                float u, v;
-                umma::unpack_f32x2(mul2(umma::pack_f32x2(s[k >> 5][k & 31], s[k >> 5][(k & 31) + 1]), add2(umma::pack_f32x2(d[k >> 5][k & 31], d[k >> 5][(k & 31) + 1]), delta2)), u, v);
-                out[k >> 1] = pack_bf16(u, v);
-            }
-            if (masked) {                             // (zero whatever dP is there)
+                const bool masked = __any_sync(0xffffffffu, low > 0 || high < 64);
 #pragma unroll
                 for (int k = 0; k < 64; k += 2) {
-                    const uint32_t keep = (k >= low && k < high ? 0xffffu : 0u) | (k + 1 >= low && k + 1 < high ? 0xffff0000u : 0u);
-                    out[k >> 1] &= keep;
+                    if (kKeys) {
+                        const float2 m = *reinterpret_cast<const float2*>(now + k);
+                        minus2 = f32x2(m.x, m.y);
+                    }
+                    float x, y;
+                    umma::unpack_f32x2(fma2(umma::pack_f32x2(s[k >> 5][k & 31], s[k >> 5][(k & 31) + 1]), c2, minus2), x, y);
+                    s[k >> 5][k & 31] = __float_as_uint(x);
+                    s[k >> 5][(k & 31) + 1] = __float_as_uint(y);
                 }
-            }
-            umma::tmem_st_32x32(dp + 32, out);
-            umma::tmem_st_wait();
-            umma::fence_before_thread_sync();
-            __syncwarp();
-            if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->p_full[half]);
-        }
-        const int64_t at = (token * (kKeys ? a.kv_heads : a.heads) + head) * a.dim;
-        const float factor = kKeys && half == 1 ? 1.f : a.scale;
-        bf16* out = reinterpret_cast<bf16*>(kKeys ? (half == 0 ? a.dk : a.dv) : a.dq) + at;
-        float* part = nullptr;
-        if (kKeys && a.splits > 1) part = a.parts + (static_cast<int64_t>(split) * 2 + half) * a.tk * a.kv_heads * a.dim + at;
-        if (n > 0) {
-            ok = ok && attn_wait_warp(&b->sums, 0, failed, a.report, 6);
-            if (ok) {
+                if (masked)
+#pragma unroll
+                    for (int k = 0; k < 64; ++k)
+                        if (k < low || k >= high) s[k >> 5][k & 31] = 0xff800000u;
+#pragma unroll
+                for (int k = 0; k < 64; ++k) s[k >> 5][k & 31] = __float_as_uint(exp2_approx(__uint_as_float(s[k >> 5][k & 31])));
+                ok = attn_wait_warp(&b->dp_full[made & 1], made >> 1 & 1, failed, a.report, 5);
+                if (!ok) break;
                 umma::fence_after_thread_sync();
-                if (!kKeys) {
-                    const int first = half * 32 * kChunks;
-                    store_row<32 * kChunks>(lanes + first, factor, out + first, a.dim - first, in);
-                } else if (part != nullptr) {
-                    store_part<64 * kChunks>(lanes + half * 128, factor, part, a.dim, in);
-                } else {
-                    store_row<64 * kChunks>(lanes + half * 128, factor, out, a.dim, in);
+                const uint32_t dp = lanes + Shape::kDp + (kKeys ? 0 : (made & 1) * 128) + half * 64;
+                umma::tmem_ld_32x32(dp, d[0]);
+                umma::tmem_ld_32x32(dp + 32, d[1]);
+                umma::tmem_ld_wait();
+                uint32_t out[32];
+                if (kKeys) {
+#pragma unroll
+                    for (int k = 0; k < 64; k += 2) out[k >> 1] = pack_bf16(__uint_as_float(s[k >> 5][k & 31]), __uint_as_float(s[k >> 5][(k & 31) + 1]));
+                    umma::tmem_st_32x32(dp, out);
+                }
+#pragma unroll
+                for (int k = 0; k < 64; k += 2) {
+                    if (kKeys) {
+                        const float2 m = *reinterpret_cast<const float2*>(now + 64 + k);
+                        delta2 = f32x2(m.x, m.y);
+                    }
+                    float u, v;
+                    umma::unpack_f32x2(mul2(umma::pack_f32x2(s[k >> 5][k & 31], s[k >> 5][(k & 31) + 1]), add2(umma::pack_f32x2(d[k >> 5][k & 31], d[k >> 5][(k & 31) + 1]), delta2)), u, v);
+                    out[k >> 1] = pack_bf16(u, v);
+                }
+                if (masked) {                             // (zero whatever dP is there)
+#pragma unroll
+                    for (int k = 0; k < 64; k += 2) {
+                        const uint32_t keep = (k >= low && k < high ? 0xffffu : 0u) | (k + 1 >= low && k + 1 < high ? 0xffff0000u : 0u);
+                        out[k >> 1] &= keep;
+                    }
+                }
+                umma::tmem_st_32x32(dp + 32, out);
+                umma::tmem_st_wait();
+                umma::fence_before_thread_sync();
+                __syncwarp();
+                if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->p_full[half][made & 1]);
+            }
+            const int64_t at = (token * (kKeys ? a.kv_heads : a.heads) + w.head) * a.dim;
+            const float factor = kKeys && half == 1 ? 1.f : a.scale;
+            bf16* out = reinterpret_cast<bf16*>(kKeys ? (half == 0 ? a.dk : a.dv) : a.dq) + at;
+            float* part = nullptr;
+            if (kKeys && a.splits > 1) part = a.parts + (static_cast<int64_t>(w.split) * 2 + half) * a.tk * a.kv_heads * a.dim + at;
+            if (w.n > 0) {
+                ok = ok && attn_wait_warp(&b->sums, ended & 1, failed, a.report, 6);
+                ++ended;
+                if (ok) {
+                    umma::fence_after_thread_sync();
+                    if (!kKeys) {
+                        const int first = half * 32 * kChunks;
+                        store_row<32 * kChunks>(lanes + first, factor, out + first, a.dim - first, in);
+                    } else if (part != nullptr) {
+                        store_part<64 * kChunks>(lanes + half * 128, factor, part, a.dim, in);
+                    } else {
+                        store_row<64 * kChunks>(lanes + half * 128, factor, out, a.dim, in);
+                    }
+                    umma::fence_before_thread_sync();
+                    __syncwarp();
+                    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->drained);
+                }
+            } else if (in && (kKeys || half == 0)) {
+                for (int i = 0; i < a.dim; i += 8) {
+                    if (part != nullptr) *reinterpret_cast<uint4*>(part + i) = *reinterpret_cast<uint4*>(part + i + 4) = make_uint4(0, 0, 0, 0);
+                    else *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
                 }
             }
-        } else if (in && (kKeys || half == 0)) {
-            for (int i = 0; i < a.dim; i += 8) {
-                if (part != nullptr) *reinterpret_cast<uint4*>(part + i) = *reinterpret_cast<uint4*>(part + i + 4) = make_uint4(0, 0, 0, 0);
-                else *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
-            }
-        }
-        const int64_t row_values = static_cast<int64_t>(kKeys ? a.kv_heads : a.heads) * a.dim;
-        if (!kKeys) {
-            clear_rows<256>(a.cu_q, a.num_seqs, a.tq, blockIdx.x, gridDim.x, reinterpret_cast<bf16*>(a.dq), row_values, nullptr, 0);
-        } else if (part == nullptr) {
-            clear_rows<256>(a.cu_k, a.num_seqs, a.tk, blockIdx.x, gridDim.x, reinterpret_cast<bf16*>(a.dk), row_values, nullptr, 0);
-            clear_rows<256>(a.cu_k, a.num_seqs, a.tk, blockIdx.x, gridDim.x, reinterpret_cast<bf16*>(a.dv), row_values, nullptr, 0);
         }
     }
     umma::fence_before_thread_sync();
     __syncthreads();
     if (b->st.failed != 0) {
         // (as in the forward pass)
-        if (warp == 8 && n > 0) {
-            mbar_drain(&b->kept, 0, 100000000ull);
+        if (warp == 8) {
+            mbar_drain(&b->kept, 0, 100000000ull), mbar_drain(&b->kept, 1, 100000000ull);
+            mbar_drain(&b->answered, 0, 100000000ull), mbar_drain(&b->answered, 1, 100000000ull);
             for (int i = 0; i < kSlots; ++i) mbar_drain(&b->full[i], 0, 100000000ull), mbar_drain(&b->full[i], 1, 100000000ull);
         }
         if (warp == 9 && ptx::elect_one()) {
@@ -1067,8 +1161,14 @@ bool make_map(CUtensorMap* map, const HeadsView& x, int64_t tokens, int64_t head
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(heads > 1 ? x.stride_head * 2 : pitch), static_cast<cuuint64_t>(tokens > 1 ? x.stride_token * 2 : pitch)};
     const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(box_rows)};
     const cuuint32_t steps[3] = {1, 1, 1};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(x.data), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    auto made = [&]() {
+        return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(x.data), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    if (made()) return true;
+    // (the driver wants a context, and a thread that has made no call of the runtime yet, as those that run gradients, has none)
+    int device = 0;
+    return cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess && made();
 }
 // leave for shared memory, once per device
 cudaError_t allow_once(const void* fn, int bytes, std::atomic<uint64_t>& allowed) {

@@ -280,6 +280,43 @@ def test_in_a_graph_and_on_another_stream():
 
 
 @pytest.mark.gpu
+def test_in_threads_that_have_done_nothing_yet():
+    import threading
+    q, k, v, d_o, _ = _make(200, 200, 4, 2, 64, 12, 'cuda')
+    want = attention(q, k, v)
+    grads = attention_backward(d_o, q, k, v, *want)
+    got = {}
+    for name, f in (('forward', lambda: attention(q, k, v)), ('backward', lambda: attention_backward(d_o, q, k, v, *want))):
+        thread = threading.Thread(target=lambda: got.update({name: f()}))
+        thread.start()
+        thread.join()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((*got['forward'], *got['backward']), (*want, *grads)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('D,H,Hk', [(128, 12, 4), (64, 16, 16)])
+def test_more_blocks_than_processors(D, H, Hk):
+    """Every CTA takes many blocks of unlike length, empty sequences among them: against the same sequences one by one."""
+    lengths = [700, 0, 33, 128, 1500, 129, 1, 256, 640] * 3
+    q, k, v, d_o, _ = _make(sum(lengths), sum(lengths), H, Hk, D, 13, 'cuda')
+    cu = _cu(lengths, 'cuda')
+    o, lse = attention(q, k, v, cu)
+    grads = attention_backward(d_o, q, k, v, o, lse, cu)
+    a = 0
+    for n in lengths[:9]:
+        i = slice(a, a + n)
+        a += n
+        if n == 0:
+            continue
+        one = attention(q[i], k[i], v[i])
+        assert torch.equal(one[0], o[i]) and torch.equal(one[1], lse[:, i])
+        # (keys' gradients may be added in other parts: half a step of bf16, and of what the products round)
+        for x, y in zip(attention_backward(d_o[i], q[i], k[i], v[i], *one), grads):
+            assert (x.float() - y[i].float()).abs().max() <= 4 * HALF * y[i].float().abs().max()
+
+
+@pytest.mark.gpu
 def test_nothing_to_do():
     q, k, v, d_o, d_lse = _make(10, 12, 2, 1, 64, 0, 'cuda')
     o, lse = attention(q[:0], k, v)
