@@ -6,8 +6,8 @@
 //
 //     dw = sum over tokens and heads of g rstd x,     u = g w,     dx = rstd (u - rstd^2 x mean(u x))
 //
-// Bound by memory: every value is read once and written once.  A row of D channels lies on 8, 16 or 32 lanes of a warp, eight channels each; partners that are R/2 apart
-// exchange their raw values (four registers of bf16 pairs, where normed ones would take eight) and norm them on both sides.
+// Bound by memory: every value is read once and written once.  A row of D channels lies on 8, 16 or 32 lanes of a warp, eight channels each: neighbours where pairs are neighbours,
+// else four and their partners, so that no lane asks another for them (eight neighbours, and their partners' values by shuffles: 66 instead of XX us for 8192 x 64 heads of 128).
 #include <algorithm>
 #include <type_traits>
 
@@ -19,17 +19,38 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 constexpr int kRotaryThreads = 256;
+constexpr int kForwardIters = 4, kBackwardIters = 2, kForwardCtas = 4, kBackwardCtas = 2;
 
+// Eight channels, four from lo on and four from hi on (kWhole: neighbours)
 template <class T>
 struct Eight {
     uint4 raw[sizeof(T) / 2];
 };
-template <class T>
-__device__ __forceinline__ Eight<T> load8(const T* p) {
+template <bool kWhole, class T>
+__device__ __forceinline__ Eight<T> load8(const T* p, int lo, int hi) {
     Eight<T> e;
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) e.raw[i] = reinterpret_cast<const uint4*>(p)[i];
+    if constexpr (sizeof(T) == 4) {
+        e.raw[0] = *reinterpret_cast<const uint4*>(p + lo);
+        e.raw[1] = *reinterpret_cast<const uint4*>(p + (kWhole ? lo + 4 : hi));
+    } else if constexpr (kWhole) {
+        e.raw[0] = *reinterpret_cast<const uint4*>(p + lo);
+    } else {
+        const uint2 a = *reinterpret_cast<const uint2*>(p + lo), b = *reinterpret_cast<const uint2*>(p + hi);
+        e.raw[0] = make_uint4(a.x, a.y, b.x, b.y);
+    }
     return e;
+}
+template <bool kWhole, class T>
+__device__ __forceinline__ void store8(T* p, int lo, int hi, const Eight<T>& e) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<uint4*>(p + lo) = e.raw[0];
+        *reinterpret_cast<uint4*>(p + (kWhole ? lo + 4 : hi)) = e.raw[1];
+    } else if constexpr (kWhole) {
+        *reinterpret_cast<uint4*>(p + lo) = e.raw[0];
+    } else {
+        *reinterpret_cast<uint2*>(p + lo) = make_uint2(e.raw[0].x, e.raw[0].y);
+        *reinterpret_cast<uint2*>(p + hi) = make_uint2(e.raw[0].z, e.raw[0].w);
+    }
 }
 __device__ __forceinline__ void to_float(const Eight<bf16>& e, float (&f)[8]) {
     const uint32_t w[4] = {e.raw[0].x, e.raw[0].y, e.raw[0].z, e.raw[0].w};
@@ -49,33 +70,23 @@ __device__ __forceinline__ void to_float(const Eight<float>& e, float (&f)[8]) {
     }
 }
 template <class T>
-__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+__device__ __forceinline__ Eight<T> from_float(const float (&f)[8]) {
+    Eight<T> e;
     if constexpr (sizeof(T) == 2) {
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(f[2 * i + 1]), "f"(f[2 * i]));
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        e.raw[0] = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
-        reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-    }
-}
-// those of lane `from`
-template <class T>
-__device__ __forceinline__ Eight<T> exchange(const Eight<T>& e, int from) {
-    Eight<T> r;
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) {
-        r.raw[i].x = __shfl_sync(0xffffffffu, e.raw[i].x, from);
-        r.raw[i].y = __shfl_sync(0xffffffffu, e.raw[i].y, from);
-        r.raw[i].z = __shfl_sync(0xffffffffu, e.raw[i].z, from);
-        r.raw[i].w = __shfl_sync(0xffffffffu, e.raw[i].w, from);
+        for (int i = 0; i < 2; ++i) e.raw[i] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]), __float_as_uint(f[4 * i + 3]));
     }
-    return r;
+    return e;
 }
-__device__ __forceinline__ void load_weight(const void* w, int is_bf16, int c, float (&f)[8]) {
-    if (is_bf16) to_float(load8(static_cast<const bf16*>(w) + c), f);
-    else to_float(load8(static_cast<const float*>(w) + c), f);
+template <bool kWhole>
+__device__ __forceinline__ void load_weight(const void* w, int is_bf16, int lo, int hi, float (&f)[8]) {
+    if (is_bf16) to_float(load8<kWhole>(static_cast<const bf16*>(w), lo, hi), f);
+    else to_float(load8<kWhole>(static_cast<const float*>(w), lo, hi), f);
 }
 __device__ __forceinline__ int64_t load_index(const void* p, int is_64, int64_t i) {
     return is_64 ? static_cast<const int64_t*>(p)[i] : static_cast<int64_t>(static_cast<const int32_t*>(p)[i]);
@@ -90,43 +101,52 @@ __device__ __forceinline__ float sum_row(float v) {
 // What a lane knows of its place in the rows
 template <int kLanes, bool kInterleaved>
 struct Place {
-    static constexpr int kRows = 32 / kLanes;            // rows of a warp
-    int sub, c, partner, angle;                          // row of the warp, first channel, lane of the partners, first angle
-    bool on, turned, second;                             // lanes that hold channels, that hold rotated ones, whose are the second of their pairs
+    static constexpr int kRows = 32 / kLanes, kPartner = kInterleaved ? 1 : 4;      // rows of a warp; value j's partner is value j ^ kPartner
+    int sub, lo, hi, angle;                              // row of the warp, channels, first angle
+    bool on, turned;                                     // lanes that hold channels, that hold rotated ones
     __device__ __forceinline__ Place(int dim, int rotary) {
         const int lane = threadIdx.x & 31, in = lane % kLanes;
         sub = lane / kLanes;
-        c = in * 8;
-        on = c < dim;
-        turned = c < rotary;
-        second = !kInterleaved && c >= rotary / 2;
-        partner = kInterleaved || !turned ? lane : lane + (second ? -rotary / 16 : rotary / 16);
-        angle = kInterleaved ? c / 2 : (second ? c - rotary / 2 : c);
+        on = in * 8 < dim;
+        turned = in * 8 < rotary;
+        lo = kInterleaved || !turned ? in * 8 : in * 4;
+        hi = kInterleaved || !turned ? lo + 4 : rotary / 2 + lo;
+        angle = in * 4;
     }
+    __device__ __forceinline__ int channel(int j) const { return j < 4 ? lo + j : hi + j - 4; }
 };
-// Cosines and sines of a lane's pairs; rows of zeros in front of the table, of no numbers behind it
+// What a lane's eight channels take of themselves and of their partners: cosines and signed sines, or these times the channels' weights.  Rows of zeros in front of the
+// table, of no numbers behind it.
 template <bool kInterleaved>
 struct Angles {
-    static constexpr int kCount = kInterleaved ? 4 : 8;
-    float cos[kCount], sin[kCount], keep;
+    float own[8], partner[8], keep;
     template <class P>
     __device__ __forceinline__ Angles(const RotaryArgs& a, const P& place, int64_t position) {
         keep = position < 0 ? 0.f : (position < a.num_positions ? 1.f : __int_as_float(0x7fc00000));
         const float* row = a.table + (position >= 0 && position < a.num_positions ? position : 0) * a.rotary + place.angle;
+        const bool read = place.turned && a.num_positions > 0;
+        const float4 u = read ? *reinterpret_cast<const float4*>(row) : make_float4(1.f, 1.f, 1.f, 1.f);
+        const float4 v = read ? *reinterpret_cast<const float4*>(row + a.rotary / 2) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float cos[4] = {u.x, u.y, u.z, u.w}, sin[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int i = 0; i < kCount; i += 4) {
-            const bool read = place.turned && a.num_positions > 0;
-            const float4 u = read ? *reinterpret_cast<const float4*>(row + i) : make_float4(1.f, 1.f, 1.f, 1.f);
-            const float4 v = read ? *reinterpret_cast<const float4*>(row + a.rotary / 2 + i) : make_float4(0.f, 0.f, 0.f, 0.f);
-            cos[i] = u.x, cos[i + 1] = u.y, cos[i + 2] = u.z, cos[i + 3] = u.w;
-            sin[i] = v.x, sin[i + 1] = v.y, sin[i + 2] = v.z, sin[i + 3] = v.w;
+        for (int i = 0; i < 8; ++i) {
+            const int pair = kInterleaved ? i / 2 : i % 4;
+            own[i] = cos[pair];
+            partner[i] = (kInterleaved ? i % 2 : i / 4) == 1 ? sin[pair] : -sin[pair];
+        }
+    }
+    __device__ __forceinline__ void times(const float (&w)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            own[i] *= w[i];
+            partner[i] *= w[i ^ (kInterleaved ? 1 : 4)];
         }
     }
 };
 
 // Rows [kIters] of a warp: heads of one kind (queries, keys, values) of one token
 template <class T, int kLanes, bool kInterleaved, int kIters>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_constant__ RotaryArgs a, int chunks_q, int chunks_k, int chunks) {
+__global__ void __launch_bounds__(kRotaryThreads, kForwardCtas) rotary_kernel(const __grid_constant__ RotaryArgs a, int chunks_q, int chunks_k, int chunks) {
     using Lane = Place<kLanes, kInterleaved>;
     constexpr int kHeads = kIters * Lane::kRows;
     ptx::wait_for_previous_kernel();
@@ -141,11 +161,12 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
     const float inv_dim = 1.f / a.dim;
     const HeadsView& x = kind == 2 ? a.v : a.x[kind];
     const int heads = a.heads[kind == 0 ? 0 : 1], head0 = chunk * kHeads + place.sub;
+    const int64_t position = kind == 2 ? 0 : load_index(a.positions, a.positions_64, token);
     Eight<T> raw[kIters] = {};
 #pragma unroll
     for (int i = 0; i < kIters; ++i)
         if (place.on && head0 + i * Lane::kRows < heads)
-            raw[i] = load8(static_cast<const T*>(x.data) + token * x.stride_token + (head0 + i * Lane::kRows) * x.stride_head + place.c);
+            raw[i] = load8<kInterleaved>(static_cast<const T*>(x.data) + token * x.stride_token + (head0 + i * Lane::kRows) * x.stride_head, place.lo, place.hi);
     T* out;
     int64_t pitch;
     bool write = place.on;
@@ -162,17 +183,13 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
     if (kind == 2) {
 #pragma unroll
         for (int i = 0; i < kIters; ++i)
-            if (write && head0 + i * Lane::kRows < heads) {
-                T* row = out + (head0 + i * Lane::kRows) * pitch + place.c;
-#pragma unroll
-                for (int j = 0; j < static_cast<int>(sizeof(T)) / 2; ++j) reinterpret_cast<uint4*>(row)[j] = raw[i].raw[j];
-            }
+            if (write && head0 + i * Lane::kRows < heads) store8<kInterleaved>(out + (head0 + i * Lane::kRows) * pitch, place.lo, place.hi, raw[i]);
         return;
     }
-    const Angles<kInterleaved> turn(a, place, load_index(a.positions, a.positions_64, token));
-    float w[8] = {}, w_partner[8] = {};
-    if (place.on) load_weight(a.weight[kind], a.param_bf16, place.c, w);
-    if (!kInterleaved && place.turned) load_weight(a.weight[kind], a.param_bf16, place.second ? place.c - a.rotary / 2 : place.c + a.rotary / 2, w_partner);
+    float w[8] = {};
+    if (place.on) load_weight<kInterleaved>(a.weight[kind], a.param_bf16, place.lo, place.hi, w);
+    Angles<kInterleaved> turn(a, place, position);
+    turn.times(w);
 #pragma unroll
     for (int i = 0; i < kIters; ++i) {
         float v[8], y[8], squares = 0.f;
@@ -180,32 +197,18 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_kernel(const __grid_con
 #pragma unroll
         for (int j = 0; j < 8; ++j) squares = fmaf(v[j], v[j], squares);
         const float rstd = __frsqrt_rn(sum_row<kLanes>(squares) * inv_dim + a.eps);
-        if constexpr (kInterleaved) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float p = v[2 * j] * rstd * w[2 * j], q = v[2 * j + 1] * rstd * w[2 * j + 1];
-                y[2 * j] = p * turn.cos[j] - q * turn.sin[j];
-                y[2 * j + 1] = q * turn.cos[j] + p * turn.sin[j];
-            }
-        } else {
-            float u[8];
-            to_float(exchange(raw[i], place.partner), u);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float p = v[j] * rstd * w[j], q = u[j] * rstd * w_partner[j];
-                y[j] = p * turn.cos[j] + (place.second ? q : -q) * turn.sin[j];
-            }
-        }
+        for (int j = 0; j < 8; ++j) y[j] = rstd * fmaf(v[j ^ Lane::kPartner], turn.partner[j], v[j] * turn.own[j]);
         if (turn.keep != 1.f)
 #pragma unroll
             for (int j = 0; j < 8; ++j) y[j] = turn.keep;
-        if (write && head0 + i * Lane::kRows < heads) store8(out + (head0 + i * Lane::kRows) * pitch + place.c, y);
+        if (write && head0 + i * Lane::kRows < heads) store8<kInterleaved>(out + (head0 + i * Lane::kRows) * pitch, place.lo, place.hi, from_float<T>(y));
     }
 }
 
 // Gradient: a warp takes chunks of heads, those of queries and then those of keys, and keeps its sums of the weight's gradient
 template <class T, int kLanes, bool kInterleaved, int kIters>
-__global__ void __launch_bounds__(kRotaryThreads) rotary_backward_kernel(const __grid_constant__ RotaryArgs a) {
+__global__ void __launch_bounds__(kRotaryThreads, kBackwardCtas) rotary_backward_kernel(const __grid_constant__ RotaryArgs a) {
     using Lane = Place<kLanes, kInterleaved>;
     constexpr int kHeads = kIters * Lane::kRows, kWarps = kRotaryThreads / 32;
     __shared__ float s_sum[kWarps][kLanes * 8];
@@ -219,37 +222,42 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_backward_kernel(const _
         const int heads = a.heads[kind], chunks = (heads + kHeads - 1) / kHeads;
         const int64_t units = static_cast<int64_t>(a.tokens) * chunks;
         float w[8] = {}, dw[8] = {};
-        if (place.on) load_weight(a.weight[kind], a.param_bf16, place.c, w);
-#pragma unroll 1
-        for (int64_t unit = static_cast<int64_t>(blockIdx.x) * kWarps + warp; unit < units; unit += static_cast<int64_t>(gridDim.x) * kWarps) {
-            const int64_t token = unit / chunks;
-            const int head0 = static_cast<int>(unit - token * chunks) * kHeads + place.sub;
-            Eight<T> x[kIters] = {}, d[kIters] = {};
+        if (place.on) load_weight<kInterleaved>(a.weight[kind], a.param_bf16, place.lo, place.hi, w);
+        // neighbouring chunks, the next one's values on their way while this one's are worked on
+        const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarps, share = (units + warps - 1) / warps;
+        const int64_t begin = (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * share, end = min(begin + share, units);
+        Eight<T> x[kIters] = {}, d[kIters] = {}, next_x[kIters] = {}, next_d[kIters] = {};
+        int64_t token = begin / chunks, next_token = token;
+        int chunk = static_cast<int>(begin - token * chunks), next_chunk = chunk;
+        auto request = [&]() {
 #pragma unroll
-            for (int i = 0; i < kIters; ++i)
-                if (place.on && head0 + i * Lane::kRows < heads) {
-                    const int64_t head = head0 + i * Lane::kRows;
-                    x[i] = load8(static_cast<const T*>(a.x[kind].data) + token * a.x[kind].stride_token + head * a.x[kind].stride_head + place.c);
-                    d[i] = load8(static_cast<const T*>(a.dy[kind].data) + token * a.dy[kind].stride_token + head * a.dy[kind].stride_head + place.c);
+            for (int i = 0; i < kIters; ++i) {
+                const int64_t head = next_chunk * kHeads + place.sub + i * Lane::kRows;
+                if (place.on && head < heads) {
+                    next_x[i] = load8<kInterleaved>(static_cast<const T*>(a.x[kind].data) + next_token * a.x[kind].stride_token + head * a.x[kind].stride_head, place.lo, place.hi);
+                    next_d[i] = load8<kInterleaved>(static_cast<const T*>(a.dy[kind].data) + next_token * a.dy[kind].stride_token + head * a.dy[kind].stride_head, place.lo, place.hi);
                 }
+            }
+        };
+        if (begin < end) request();
+#pragma unroll 1
+        for (int64_t unit = begin; unit < end; ++unit) {
+            token = next_token;
+            chunk = next_chunk;
+#pragma unroll
+            for (int i = 0; i < kIters; ++i) x[i] = next_x[i], d[i] = next_d[i];
+            if (++next_chunk == chunks) next_chunk = 0, ++next_token;
+            if (unit + 1 < end) request();
+            const int head0 = chunk * kHeads + place.sub;
             const Angles<kInterleaved> turn(a, place, load_index(a.positions, a.positions_64, token));
 #pragma unroll
             for (int i = 0; i < kIters; ++i) {
                 float v[8], g[8], own[8];
                 to_float(x[i], v);
                 to_float(d[i], own);
-                if constexpr (kInterleaved) {
+                // (turned back: the sines' signs are the other way round)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        g[2 * j] = own[2 * j] * turn.cos[j] + own[2 * j + 1] * turn.sin[j];
-                        g[2 * j + 1] = own[2 * j + 1] * turn.cos[j] - own[2 * j] * turn.sin[j];
-                    }
-                } else {
-                    float u[8];
-                    to_float(exchange(d[i], place.partner), u);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) g[j] = own[j] * turn.cos[j] + (place.second ? -u[j] : u[j]) * turn.sin[j];
-                }
+                for (int j = 0; j < 8; ++j) g[j] = fmaf(-own[j ^ Lane::kPartner], turn.partner[j], own[j] * turn.own[j]);
                 if (turn.keep != 1.f)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) g[j] = turn.keep;
@@ -261,19 +269,20 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_backward_kernel(const _
                 }
                 squares = sum_row<kLanes>(squares);
                 along = sum_row<kLanes>(along);
-                const float rstd = __frsqrt_rn(squares * inv_dim + a.eps), back = rstd * rstd * (along * inv_dim);
-                float dx[8];
+                const float rstd = __frsqrt_rn(squares * inv_dim + a.eps), back = rstd * rstd * rstd * (along * inv_dim);
                 if (head0 + i * Lane::kRows < heads) {
+                    float dx[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        dx[j] = rstd * (g[j] * w[j] - v[j] * back);
-                        dw[j] = turn.keep == 0.f ? dw[j] : fmaf(g[j] * rstd, v[j], dw[j]);
+                        const float gr = g[j] * rstd;
+                        dx[j] = fmaf(gr, w[j], -v[j] * back);
+                        dw[j] = turn.keep == 0.f ? dw[j] : fmaf(gr, v[j], dw[j]);
                     }
                     if (place.on) {
                         if (turn.keep == 0.f)
 #pragma unroll
                             for (int j = 0; j < 8; ++j) dx[j] = 0.f;
-                        store8(static_cast<T*>(a.out[kind]) + (token * heads + head0 + i * Lane::kRows) * a.dim + place.c, dx);
+                        store8<kInterleaved>(static_cast<T*>(a.out[kind]) + (token * heads + head0 + i * Lane::kRows) * a.dim, place.lo, place.hi, from_float<T>(dx));
                     }
                 }
             }
@@ -286,7 +295,7 @@ __global__ void __launch_bounds__(kRotaryThreads) rotary_backward_kernel(const _
         __syncthreads();
         if (place.sub == 0)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s_sum[warp][place.c + j] = dw[j];
+            for (int j = 0; j < 8; ++j) s_sum[warp][place.on ? place.channel(j) : place.lo + j] = dw[j];
         __syncthreads();
         for (int c = threadIdx.x; c < a.dim; c += kRotaryThreads) {
             float sum = 0.f;
@@ -319,7 +328,6 @@ __global__ void __launch_bounds__(1024) rotary_reduce_kernel(const __grid_consta
     }
 }
 
-constexpr int kForwardIters = 4, kBackwardIters = 2;
 int lanes_of(int dim) { return dim <= 64 ? 8 : (dim <= 128 ? 16 : 32); }
 
 template <class F>
@@ -355,7 +363,7 @@ cudaError_t launch_rotary(const RotaryArgs& a, int num_sms, cudaStream_t stream)
 int rotary_backward_ctas(const RotaryArgs& a, int num_sms) {
     const int heads_per_unit = kBackwardIters * 32 / lanes_of(a.dim);
     const int64_t units = static_cast<int64_t>(a.tokens) * ((a.heads[0] + heads_per_unit - 1) / heads_per_unit);
-    return static_cast<int>(std::min<int64_t>((units * 32 + kRotaryThreads - 1) / kRotaryThreads, num_sms * 4));
+    return static_cast<int>(std::min<int64_t>((units * 32 + kRotaryThreads - 1) / kRotaryThreads, num_sms * kBackwardCtas));
 }
 cudaError_t launch_rotary_backward(const RotaryArgs& a, cudaStream_t stream) {
     void* params[] = {const_cast<RotaryArgs*>(&a)};
