@@ -7,7 +7,7 @@
 //     dw = sum over tokens and heads of g rstd x,     u = g w,     dx = rstd (u - rstd^2 x mean(u x))
 //
 // Bound by memory: every value is read once and written once.  A row of D channels lies on 8, 16 or 32 lanes of a warp, eight channels each: neighbours where pairs are neighbours,
-// else four and their partners, so that no lane asks another for them (eight neighbours, and their partners' values by shuffles: 66 instead of XX us for 8192 x 64 heads of 128).
+// else four and their partners, so that no lane asks another for them (eight neighbours, and their partners' values by shuffles: 66 instead of 63 us for 8192 x 64 heads of 128).  What 16-bit heads take beyond that is instruction issue, so values go in pairs.
 #include <algorithm>
 #include <type_traits>
 
@@ -19,7 +19,33 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 constexpr int kRotaryThreads = 256;
-constexpr int kForwardIters = 4, kBackwardIters = 2, kForwardCtas = 4, kBackwardCtas = 2;
+// Rows of a lane group that a warp has at once, and CTAs of an SM: what is on its way at a time.  8192 x 64 heads of 128, bf16: 59 us (two rows: 67, eight on three CTAs: 66); gradients 94 (two
+// rows: 101, three CTAs 109), where four rows of 32-bit values do not fit the registers (4096 x 40 heads: 86 us instead of 48).
+constexpr int kForwardIters = 4, kForwardCtas = 4, kBackwardCtas = 2;
+__host__ __device__ constexpr int backward_iters(int value_bytes) { return value_bytes == 2 ? 4 : 2; }
+
+// Two values at once
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ float both(uint64_t v) {
+    float a, b;
+    unpair(v, a, b);
+    return a + b;
+}
 
 // Eight channels, four from lo on and four from hi on (kWhole: neighbours)
 template <class T>
@@ -52,39 +78,53 @@ __device__ __forceinline__ void store8(T* p, int lo, int hi, const Eight<T>& e) 
         *reinterpret_cast<uint2*>(p + hi) = make_uint2(e.raw[0].z, e.raw[0].w);
     }
 }
-__device__ __forceinline__ void to_float(const Eight<bf16>& e, float (&f)[8]) {
+__device__ __forceinline__ void to_float(const Eight<bf16>& e, uint64_t (&f)[4]) {
     const uint32_t w[4] = {e.raw[0].x, e.raw[0].y, e.raw[0].z, e.raw[0].w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        f[2 * i] = __uint_as_float(w[i] << 16);
-        f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+    for (int i = 0; i < 4; ++i) f[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
 }
-__device__ __forceinline__ void to_float(const Eight<float>& e, float (&f)[8]) {
+__device__ __forceinline__ void to_float(const Eight<float>& e, uint64_t (&f)[4]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        f[4 * i] = __uint_as_float(e.raw[i].x);
-        f[4 * i + 1] = __uint_as_float(e.raw[i].y);
-        f[4 * i + 2] = __uint_as_float(e.raw[i].z);
-        f[4 * i + 3] = __uint_as_float(e.raw[i].w);
+        f[2 * i] = pair(__uint_as_float(e.raw[i].x), __uint_as_float(e.raw[i].y));
+        f[2 * i + 1] = pair(__uint_as_float(e.raw[i].z), __uint_as_float(e.raw[i].w));
     }
 }
 template <class T>
-__device__ __forceinline__ Eight<T> from_float(const float (&f)[8]) {
+__device__ __forceinline__ Eight<T> from_float(const uint64_t (&f)[4]) {
     Eight<T> e;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpair(f[i], v[2 * i], v[2 * i + 1]);
     if constexpr (sizeof(T) == 2) {
         uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(f[2 * i + 1]), "f"(f[2 * i]));
+        for (int i = 0; i < 4; ++i) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i]) : "f"(v[2 * i + 1]), "f"(v[2 * i]));
         e.raw[0] = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) e.raw[i] = make_uint4(__float_as_uint(f[4 * i]), __float_as_uint(f[4 * i + 1]), __float_as_uint(f[4 * i + 2]), __float_as_uint(f[4 * i + 3]));
+        for (int i = 0; i < 2; ++i) e.raw[i] = make_uint4(__float_as_uint(v[4 * i]), __float_as_uint(v[4 * i + 1]), __float_as_uint(v[4 * i + 2]), __float_as_uint(v[4 * i + 3]));
     }
     return e;
 }
+template <class T>
+__device__ __forceinline__ Eight<T> all_of(float x) {
+    const uint64_t v[4] = {pair(x, x), pair(x, x), pair(x, x), pair(x, x)};
+    return from_float<T>(v);
+}
+// ... of the partners of a lane's channels
+template <bool kInterleaved>
+__device__ __forceinline__ uint64_t partner_of(const uint64_t (&v)[4], int i) {
+    if constexpr (kInterleaved) {
+        float a, b;
+        unpair(v[i], a, b);
+        return pair(b, a);
+    } else {
+        return v[i ^ 2];
+    }
+}
 template <bool kWhole>
-__device__ __forceinline__ void load_weight(const void* w, int is_bf16, int lo, int hi, float (&f)[8]) {
+__device__ __forceinline__ void load_weight(const void* w, int is_bf16, int lo, int hi, uint64_t (&f)[4]) {
     if (is_bf16) to_float(load8<kWhole>(static_cast<const bf16*>(w), lo, hi), f);
     else to_float(load8<kWhole>(static_cast<const float*>(w), lo, hi), f);
 }
@@ -101,7 +141,7 @@ __device__ __forceinline__ float sum_row(float v) {
 // What a lane knows of its place in the rows
 template <int kLanes, bool kInterleaved>
 struct Place {
-    static constexpr int kRows = 32 / kLanes, kPartner = kInterleaved ? 1 : 4;      // rows of a warp; value j's partner is value j ^ kPartner
+    static constexpr int kRows = 32 / kLanes;            // of a warp
     int sub, lo, hi, angle;                              // row of the warp, channels, first angle
     bool on, turned;                                     // lanes that hold channels, that hold rotated ones
     __device__ __forceinline__ Place(int dim, int rotary) {
@@ -119,28 +159,34 @@ struct Place {
 // table, of no numbers behind it.
 template <bool kInterleaved>
 struct Angles {
-    float own[8], partner[8], keep;
+    uint64_t own[4], partner[4];
+    float keep;
     template <class P>
     __device__ __forceinline__ Angles(const RotaryArgs& a, const P& place, int64_t position) {
         keep = position < 0 ? 0.f : (position < a.num_positions ? 1.f : __int_as_float(0x7fc00000));
         const float* row = a.table + (position >= 0 && position < a.num_positions ? position : 0) * a.rotary + place.angle;
         const bool read = place.turned && a.num_positions > 0;
-        const float4 u = read ? *reinterpret_cast<const float4*>(row) : make_float4(1.f, 1.f, 1.f, 1.f);
-        const float4 v = read ? *reinterpret_cast<const float4*>(row + a.rotary / 2) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float cos[4] = {u.x, u.y, u.z, u.w}, sin[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int pair = kInterleaved ? i / 2 : i % 4;
-            own[i] = cos[pair];
-            partner[i] = (kInterleaved ? i % 2 : i / 4) == 1 ? sin[pair] : -sin[pair];
+        const float4 c = read ? *reinterpret_cast<const float4*>(row) : make_float4(1.f, 1.f, 1.f, 1.f);
+        const float4 s = read ? *reinterpret_cast<const float4*>(row + a.rotary / 2) : make_float4(0.f, 0.f, 0.f, 0.f);
+        if constexpr (kInterleaved) {
+            own[0] = pair(c.x, c.x), own[1] = pair(c.y, c.y), own[2] = pair(c.z, c.z), own[3] = pair(c.w, c.w);
+            partner[0] = pair(-s.x, s.x), partner[1] = pair(-s.y, s.y), partner[2] = pair(-s.z, s.z), partner[3] = pair(-s.w, s.w);
+        } else {
+            own[0] = own[2] = pair(c.x, c.y), own[1] = own[3] = pair(c.z, c.w);
+            partner[0] = pair(-s.x, -s.y), partner[1] = pair(-s.z, -s.w), partner[2] = pair(s.x, s.y), partner[3] = pair(s.z, s.w);
         }
     }
-    __device__ __forceinline__ void times(const float (&w)[8]) {
+    __device__ __forceinline__ void times(const uint64_t (&w)[4]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            own[i] *= w[i];
-            partner[i] *= w[i ^ (kInterleaved ? 1 : 4)];
+        for (int i = 0; i < 4; ++i) {
+            own[i] = mul2(own[i], w[i]);
+            partner[i] = mul2(partner[i], partner_of<kInterleaved>(w, i));
         }
+    }
+    // (the other way round: the sines' signs)
+    __device__ __forceinline__ void back() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) partner[i] ^= 0x8000000080000000ull;
     }
 };
 
@@ -151,10 +197,10 @@ __global__ void __launch_bounds__(kRotaryThreads, kForwardCtas) rotary_kernel(co
     constexpr int kHeads = kIters * Lane::kRows;
     ptx::wait_for_previous_kernel();
     ptx::let_next_kernel_start();
-    const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kRotaryThreads / 32) + (threadIdx.x >> 5);
-    const int64_t token = unit / chunks;
+    const uint32_t unit = blockIdx.x * (kRotaryThreads / 32) + (threadIdx.x >> 5);      // (fewer than 2^32)
+    const int64_t token = unit / static_cast<uint32_t>(chunks);
     if (token >= a.tokens) return;
-    int chunk = static_cast<int>(unit - token * chunks);
+    int chunk = static_cast<int>(unit - static_cast<uint32_t>(token) * chunks);
     const int kind = chunk < chunks_q ? 0 : (chunk < chunks_q + chunks_k ? 1 : 2);
     chunk -= kind == 0 ? 0 : (kind == 1 ? chunks_q : chunks_q + chunks_k);
     const Lane place(a.dim, a.rotary);
@@ -186,23 +232,30 @@ __global__ void __launch_bounds__(kRotaryThreads, kForwardCtas) rotary_kernel(co
             if (write && head0 + i * Lane::kRows < heads) store8<kInterleaved>(out + (head0 + i * Lane::kRows) * pitch, place.lo, place.hi, raw[i]);
         return;
     }
-    float w[8] = {};
+    uint64_t w[4] = {};
     if (place.on) load_weight<kInterleaved>(a.weight[kind], a.param_bf16, place.lo, place.hi, w);
     Angles<kInterleaved> turn(a, place, position);
+    out += head0 * pitch;
+    if (turn.keep != 1.f) {
+        const Eight<T> fill = all_of<T>(turn.keep);
+#pragma unroll
+        for (int i = 0; i < kIters; ++i)
+            if (write && head0 + i * Lane::kRows < heads) store8<kInterleaved>(out + i * Lane::kRows * pitch, place.lo, place.hi, fill);
+        return;
+    }
     turn.times(w);
 #pragma unroll
     for (int i = 0; i < kIters; ++i) {
-        float v[8], y[8], squares = 0.f;
+        uint64_t v[4], squares = 0;
         to_float(raw[i], v);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) squares = fmaf(v[j], v[j], squares);
-        const float rstd = __frsqrt_rn(sum_row<kLanes>(squares) * inv_dim + a.eps);
+        for (int j = 0; j < 4; ++j) squares = fma2(v[j], v[j], squares);
+        const float rstd = __frsqrt_rn(sum_row<kLanes>(both(squares)) * inv_dim + a.eps);
+        const uint64_t rstd2 = pair(rstd, rstd);
+        uint64_t y[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = rstd * fmaf(v[j ^ Lane::kPartner], turn.partner[j], v[j] * turn.own[j]);
-        if (turn.keep != 1.f)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = turn.keep;
-        if (write && head0 + i * Lane::kRows < heads) store8<kInterleaved>(out + (head0 + i * Lane::kRows) * pitch, place.lo, place.hi, from_float<T>(y));
+        for (int j = 0; j < 4; ++j) y[j] = mul2(rstd2, fma2(partner_of<kInterleaved>(v, j), turn.partner[j], mul2(v[j], turn.own[j])));
+        if (write && head0 + i * Lane::kRows < heads) store8<kInterleaved>(out + i * Lane::kRows * pitch, place.lo, place.hi, from_float<T>(y));
     }
 }
 
@@ -221,7 +274,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kBackwardCtas) rotary_backward
     for (int kind = 0; kind < 2; ++kind) {
         const int heads = a.heads[kind], chunks = (heads + kHeads - 1) / kHeads;
         const int64_t units = static_cast<int64_t>(a.tokens) * chunks;
-        float w[8] = {}, dw[8] = {};
+        uint64_t w[4] = {}, dw[4] = {};
         if (place.on) load_weight<kInterleaved>(a.weight[kind], a.param_bf16, place.lo, place.hi, w);
         // neighbouring chunks, the next one's values on their way while this one's are worked on
         const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarps, share = (units + warps - 1) / warps;
@@ -233,6 +286,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kBackwardCtas) rotary_backward
 #pragma unroll
             for (int i = 0; i < kIters; ++i) {
                 const int64_t head = next_chunk * kHeads + place.sub + i * Lane::kRows;
+                next_x[i] = next_d[i] = Eight<T>{};
                 if (place.on && head < heads) {
                     next_x[i] = load8<kInterleaved>(static_cast<const T*>(a.x[kind].data) + next_token * a.x[kind].stride_token + head * a.x[kind].stride_head, place.lo, place.hi);
                     next_d[i] = load8<kInterleaved>(static_cast<const T*>(a.dy[kind].data) + next_token * a.dy[kind].stride_token + head * a.dy[kind].stride_head, place.lo, place.hi);
@@ -249,53 +303,57 @@ __global__ void __launch_bounds__(kRotaryThreads, kBackwardCtas) rotary_backward
             if (++next_chunk == chunks) next_chunk = 0, ++next_token;
             if (unit + 1 < end) request();
             const int head0 = chunk * kHeads + place.sub;
-            const Angles<kInterleaved> turn(a, place, load_index(a.positions, a.positions_64, token));
+            Angles<kInterleaved> turn(a, place, load_index(a.positions, a.positions_64, token));
+            turn.back();
+            T* out = static_cast<T*>(a.out[kind]) + (token * heads + head0) * a.dim;
+            if (turn.keep != 1.f) {
+                const Eight<T> fill = all_of<T>(turn.keep);
+#pragma unroll
+                for (int i = 0; i < kIters; ++i)
+                    if (place.on && head0 + i * Lane::kRows < heads) store8<kInterleaved>(out + i * Lane::kRows * a.dim, place.lo, place.hi, fill);
+                if (turn.keep != 0.f)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) dw[j] = pair(turn.keep, turn.keep);
+                continue;
+            }
 #pragma unroll
             for (int i = 0; i < kIters; ++i) {
-                float v[8], g[8], own[8];
+                // (rows that are not there are zeros)
+                uint64_t v[4], g[4], own[4], squares = 0, along = 0;
                 to_float(x[i], v);
                 to_float(d[i], own);
-                // (turned back: the sines' signs are the other way round)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) g[j] = fmaf(-own[j ^ Lane::kPartner], turn.partner[j], own[j] * turn.own[j]);
-                if (turn.keep != 1.f)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) g[j] = turn.keep;
-                float squares = 0.f, along = 0.f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    squares = fmaf(v[j], v[j], squares);
-                    along = fmaf(g[j] * w[j], v[j], along);
+                for (int j = 0; j < 4; ++j) {
+                    g[j] = fma2(partner_of<kInterleaved>(own, j), turn.partner[j], mul2(own[j], turn.own[j]));
+                    squares = fma2(v[j], v[j], squares);
+                    along = fma2(mul2(g[j], w[j]), v[j], along);
                 }
-                squares = sum_row<kLanes>(squares);
-                along = sum_row<kLanes>(along);
-                const float rstd = __frsqrt_rn(squares * inv_dim + a.eps), back = rstd * rstd * rstd * (along * inv_dim);
-                if (head0 + i * Lane::kRows < heads) {
-                    float dx[8];
+                const float mean = sum_row<kLanes>(both(squares)) * inv_dim, with = sum_row<kLanes>(both(along)) * inv_dim;
+                const float rstd = __frsqrt_rn(mean + a.eps), back = -rstd * rstd * rstd * with;
+                const bool there = head0 + i * Lane::kRows < heads;
+                const uint64_t rstd2 = pair(rstd, rstd), back2 = pair(back, back);
+                uint64_t dx[4];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float gr = g[j] * rstd;
-                        dx[j] = fmaf(gr, w[j], -v[j] * back);
-                        dw[j] = turn.keep == 0.f ? dw[j] : fmaf(gr, v[j], dw[j]);
-                    }
-                    if (place.on) {
-                        if (turn.keep == 0.f)
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) dx[j] = 0.f;
-                        store8<kInterleaved>(static_cast<T*>(a.out[kind]) + (token * heads + head0 + i * Lane::kRows) * a.dim, place.lo, place.hi, from_float<T>(dx));
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    const uint64_t gr = mul2(g[j], rstd2);
+                    dx[j] = fma2(gr, w[j], mul2(v[j], back2));
+                    dw[j] = fma2(gr, v[j], dw[j]);
                 }
+                if (there && place.on) store8<kInterleaved>(out + i * Lane::kRows * a.dim, place.lo, place.hi, from_float<T>(dx));
             }
         }
+        float sums[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) unpair(dw[j], sums[2 * j], sums[2 * j + 1]);
         // rows of a warp, then warps
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int o = kLanes; o < 32; o <<= 1) dw[j] += __shfl_xor_sync(0xffffffffu, dw[j], o);
+            for (int o = kLanes; o < 32; o <<= 1) sums[j] += __shfl_xor_sync(0xffffffffu, sums[j], o);
         __syncthreads();
         if (place.sub == 0)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) s_sum[warp][place.on ? place.channel(j) : place.lo + j] = dw[j];
+            for (int j = 0; j < 8; ++j) s_sum[warp][place.on ? place.channel(j) : place.lo + j] = sums[j];
         __syncthreads();
         for (int c = threadIdx.x; c < a.dim; c += kRotaryThreads) {
             float sum = 0.f;
@@ -355,20 +413,20 @@ cudaError_t launch_rotary(const RotaryArgs& a, int num_sms, cudaStream_t stream)
         };
         // few rows: one at a time, on more warps
         const int64_t rows = static_cast<int64_t>(a.tokens) * (a.heads[0] + 2 * a.heads[1]);
-        if (rows < static_cast<int64_t>(num_sms) * 16 * kRows * kForwardIters) return launch(reinterpret_cast<const void*>(rotary_kernel<T, kLanes, kInterleaved, 1>), 1);
+        if (rows < static_cast<int64_t>(num_sms) * 32 * kRows * kForwardIters) return launch(reinterpret_cast<const void*>(rotary_kernel<T, kLanes, kInterleaved, 1>), 1);
         return launch(reinterpret_cast<const void*>(rotary_kernel<T, kLanes, kInterleaved, kForwardIters>), kForwardIters);
     });
 }
 
 int rotary_backward_ctas(const RotaryArgs& a, int num_sms) {
-    const int heads_per_unit = kBackwardIters * 32 / lanes_of(a.dim);
+    const int heads_per_unit = backward_iters(a.x_bf16 ? 2 : 4) * 32 / lanes_of(a.dim);
     const int64_t units = static_cast<int64_t>(a.tokens) * ((a.heads[0] + heads_per_unit - 1) / heads_per_unit);
     return static_cast<int>(std::min<int64_t>((units * 32 + kRotaryThreads - 1) / kRotaryThreads, num_sms * kBackwardCtas));
 }
 cudaError_t launch_rotary_backward(const RotaryArgs& a, cudaStream_t stream) {
     void* params[] = {const_cast<RotaryArgs*>(&a)};
     const cudaError_t err = with_shape(a, [&](auto type, auto lanes, auto interleaved) {
-        const void* fn = reinterpret_cast<const void*>(rotary_backward_kernel<decltype(type), decltype(lanes)::value, decltype(interleaved)::value, kBackwardIters>);
+        const void* fn = reinterpret_cast<const void*>(rotary_backward_kernel<decltype(type), decltype(lanes)::value, decltype(interleaved)::value, backward_iters(sizeof(type))>);
         return launch_dependent(fn, dim3(a.ctas), dim3(kRotaryThreads), params, 0, stream);
     });
     if (err != cudaSuccess) return err;

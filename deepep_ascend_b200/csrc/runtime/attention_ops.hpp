@@ -197,7 +197,7 @@ inline RotaryInputs rotary_inputs(const at::Tensor& q, const at::Tensor& k, cons
     const int64_t T = q.size(0), D = q.size(2);
     TORCH_CHECK(k.size(0) == T && k.size(2) == D, "q and k must have the same tokens and channels");
     TORCH_CHECK(D >= 8 && D <= 256 && D % 8 == 0, "heads must have 8 to 256 channels, a multiple of 8");
-    TORCH_CHECK(q.size(1) < (1 << 16) && k.size(1) < (1 << 16) && T < (1ll << 31) && T * (q.size(1) + 2 * k.size(1)) < (1ll << 33), "too many tokens or heads");
+    TORCH_CHECK(q.size(1) < (1 << 16) && k.size(1) < (1 << 16) && T < (1ll << 31) && T * (q.size(1) + 2 * k.size(1)) < (1ll << 31), "too many tokens or heads");
     for (const at::Tensor* t : {&q_weight, &k_weight})
         TORCH_CHECK(t->device() == q.device() && is_bf16_or_f32(*t) && t->scalar_type() == q_weight.scalar_type() && t->dim() == 1 && t->size(0) == D,
                     "weights must be bf16 or fp32 [dim], of one type, on the device of q");
