@@ -8,6 +8,7 @@
 // Statistics and sums are 32 bits, probabilities are rounded to bf16 as operands.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -16,17 +17,20 @@ namespace ep {
 namespace {
 
 using bf16 = __nv_bfloat16;
-constexpr int kPagedWarps = 4, kPagedThreads = kPagedWarps * 32, kTileKeys = 16 * kPagedWarps, kHeadRows = 16, kPagedStages = 3;
-constexpr int kLeastTiles = 8;                       // of a CTA: shorter stretches would cost more in joining than they spare
+constexpr int kHeadRows = 16, kPagedStages = 3;
+constexpr int kManyPairs = 2;                        // per SM
+constexpr int kPairKeys = 512;                       // what a CTA takes of a pair where none has more
 constexpr float kPagedLog2e = 1.4426950408889634f;
 constexpr float kLowest = -__builtin_huge_valf();
 
-template <int kDim>
+// kWarps of a CTA share a tile, 16 keys each.  As many CTAs as the shared memory of an SM holds
+template <int kDim, int kWarps>
 struct PagedShape {
+    static constexpr int kThreads = kWarps * 32, kTileKeys = kWarps * 16, kCtas = (kDim == 128 ? 8 : 16) / kWarps;
     static constexpr int kRowBytes = kDim * 2, kStageBytes = 2 * 16 * kRowBytes, kWarpBytes = kPagedStages * kStageBytes;
-    static constexpr int kRing = kPagedWarps * kWarpBytes;
+    static constexpr int kRing = kWarps * kWarpBytes;
     static constexpr int kPartFloats = kHeadRows * kDim + 2 * kHeadRows;      // sums, references, totals
-    static_assert(kPagedWarps * kHeadRows * kDim * 4 <= kRing, "the warps' sums lie in the ring");
+    static_assert(kWarps * kHeadRows * kDim * 4 <= kRing, "the warps' sums lie in the ring");
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -60,16 +64,19 @@ __device__ __forceinline__ int keys_of(const PagedAttentionArgs& a, int seq) {  
     const int64_t n = a.lengths[seq];
     return static_cast<int>(max(static_cast<int64_t>(0), min(n, capacity(a))));
 }
-__host__ __device__ __forceinline__ int tiles_of_keys(int keys) { return (keys + kTileKeys - 1) / kTileKeys; }
+template <int kTileKeys>
+__host__ __device__ __forceinline__ int tiles_of_keys(int keys) {
+    return (keys + kTileKeys - 1) / kTileKeys;
+}
 // Every thread of a CTA of kThreads: first[i] = tiles in front of sequence i (of one key head), first[num_seqs] = all
-template <int kThreads>
+template <int kThreads, int kTileKeys>
 __device__ __forceinline__ void count_tiles(const PagedAttentionArgs& a, int* first) {
     __shared__ int s_warp[kThreads / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int before = 0;
     for (int base = 0; base < a.num_seqs; base += kThreads) {
         const int i = base + threadIdx.x;
-        const int n = i < a.num_seqs ? tiles_of_keys(keys_of(a, i)) : 0;
+        const int n = i < a.num_seqs ? tiles_of_keys<kTileKeys>(keys_of(a, i)) : 0;
         int upto = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -95,7 +102,7 @@ struct Stretch {
     int64_t total, share;            // tiles in all, tiles of a CTA
     __device__ __forceinline__ Stretch(int tiles, int units, int ctas) {
         total = static_cast<int64_t>(tiles) * units;
-        share = max((total + ctas - 1) / ctas, static_cast<int64_t>(kLeastTiles));
+        share = max((total + ctas - 1) / ctas, static_cast<int64_t>(1));
     }
 };
 struct Pair {
@@ -122,10 +129,11 @@ template <int kDim>
 struct WarpState {
     float o[kDim / 8][4], top[2], sum[2];
 };
-template <int kDim>
+template <int kDim, int kWarps>
 __device__ __forceinline__ void attend(const PagedAttentionArgs& a, uint8_t* ring, uint32_t* bad_tiles, int seq, int kv_head, int head0, int rows, int tile0, int tile1,
                                        WarpState<kDim>& st) {
-    using Shape = PagedShape<kDim>;
+    using Shape = PagedShape<kDim, kWarps>;
+    constexpr int kTileKeys = Shape::kTileKeys;
     constexpr int kPieces = kDim / 8, kPassRows = 32 / kPieces;      // 16-byte pieces of a row, rows of one copy instruction
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int keys = keys_of(a, seq), pieces = a.dim / 8;
@@ -274,7 +282,7 @@ __device__ __forceinline__ void attend(const PagedAttentionArgs& a, uint8_t* rin
 }
 
 // Result (part == null) or part of a pair, from its warps' states
-template <int kDim>
+template <int kDim, int kWarps>
 __device__ __forceinline__ void join_warps(const PagedAttentionArgs& a, uint8_t* ring, float* s_top, float* s_sum, const WarpState<kDim>& st, int seq, int head0, int rows,
                                            float* part, bool broken) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -293,7 +301,7 @@ __device__ __forceinline__ void join_warps(const PagedAttentionArgs& a, uint8_t*
         const int row = h * 8 + (lane >> 2);
         float top = kLowest;
 #pragma unroll
-        for (int w = 0; w < kPagedWarps; ++w) top = fmaxf(top, s_top[w * kHeadRows + row]);
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_top[w * kHeadRows + row]);
         const float factor = st.top[h] == kLowest ? 0.f : ex2((st.top[h] - top) * c);
         if (row < rows)
 #pragma unroll
@@ -301,14 +309,14 @@ __device__ __forceinline__ void join_warps(const PagedAttentionArgs& a, uint8_t*
                 *reinterpret_cast<float2*>(sums + (warp * kHeadRows + row) * kDim + i * 8 + (lane & 3) * 2) = make_float2(st.o[i][2 * h] * factor, st.o[i][2 * h + 1] * factor);
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < rows * (kDim / 4); i += kPagedThreads) {
+    for (int i = threadIdx.x; i < rows * (kDim / 4); i += kWarps * 32) {
         const int row = i / (kDim / 4), d = i % (kDim / 4) * 4;
         float top = kLowest, sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kPagedWarps; ++w) top = fmaxf(top, s_top[w * kHeadRows + row]);
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_top[w * kHeadRows + row]);
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < kPagedWarps; ++w) {
+        for (int w = 0; w < kWarps; ++w) {
             const float t = s_top[w * kHeadRows + row], u = s_sum[w * kHeadRows + row];
             sum += t == kLowest && u == 0.f ? 0.f : u * ex2((t - top) * c);
             const float4 x = *reinterpret_cast<const float4*>(sums + (w * kHeadRows + row) * kDim + d);
@@ -329,31 +337,32 @@ __device__ __forceinline__ void join_warps(const PagedAttentionArgs& a, uint8_t*
     __syncthreads();
 }
 
+template <int kThreads>
 __device__ __forceinline__ void clear_results(const PagedAttentionArgs& a, int seq) {
     uint2* out = reinterpret_cast<uint2*>(static_cast<bf16*>(a.o) + static_cast<int64_t>(seq) * a.heads * a.dim);
     const uint32_t v = a.lengths[seq] > 0 ? 0x7fc07fc0u : 0u;      // (a table without places)
-    for (int i = threadIdx.x; i < a.heads * a.dim / 4; i += kPagedThreads) out[i] = make_uint2(v, v);
+    for (int i = threadIdx.x; i < a.heads * a.dim / 4; i += kThreads) out[i] = make_uint2(v, v);
 }
 
 // kSplit: a CTA takes an equal stretch of all tiles; otherwise it takes a pair
-template <int kDim, bool kSplit>
-__global__ void __launch_bounds__(kPagedThreads, 2) paged_attention_kernel(const __grid_constant__ PagedAttentionArgs a) {
-    using Shape = PagedShape<kDim>;
+template <int kDim, int kWarps, bool kSplit>
+__global__ void __launch_bounds__(kWarps * 32, PagedShape<kDim, kWarps>::kCtas) paged_attention_kernel(const __grid_constant__ PagedAttentionArgs a) {
+    using Shape = PagedShape<kDim, kWarps>;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float s_top[kPagedWarps * kHeadRows], s_sum[kPagedWarps * kHeadRows];
-    __shared__ uint32_t s_bad[kPagedWarps * kPagedStages];
+    __shared__ float s_top[kWarps * kHeadRows], s_sum[kWarps * kHeadRows];
+    __shared__ uint32_t s_bad[kWarps * kPagedStages];
     const int chunks = chunks_of(a), units = a.kv_heads * chunks, group = a.heads / a.kv_heads;
     ptx::wait_for_previous_kernel();
     ptx::let_next_kernel_start();
     auto run = [&](int seq, int unit, int tile0, int tile1, float* part) {
         const int kv_head = unit / chunks, first = (unit - kv_head * chunks) * kHeadRows, rows = min(group - first, kHeadRows);
         WarpState<kDim> st;
-        attend<kDim>(a, smem, s_bad, seq, kv_head, kv_head * group + first, rows, tile0, tile1, st);
-        join_warps<kDim>(a, smem, s_top, s_sum, st, seq, kv_head * group + first, rows, part, a.lengths[seq] > capacity(a));
+        attend<kDim, kWarps>(a, smem, s_bad, seq, kv_head, kv_head * group + first, rows, tile0, tile1, st);
+        join_warps<kDim, kWarps>(a, smem, s_top, s_sum, st, seq, kv_head * group + first, rows, part, a.lengths[seq] > capacity(a));
     };
     if constexpr (kSplit) {
         int* first = reinterpret_cast<int*>(smem + Shape::kRing);
-        count_tiles<kPagedThreads>(a, first);
+        count_tiles<Shape::kThreads, Shape::kTileKeys>(a, first);
         const Stretch all(first[a.num_seqs], units, gridDim.x);
         int64_t at = all.share * blockIdx.x;
         const int64_t end = min(at + all.share, all.total);
@@ -367,24 +376,27 @@ __global__ void __launch_bounds__(kPagedThreads, 2) paged_attention_kernel(const
             at = until;
         }
         for (int seq = blockIdx.x; seq < a.num_seqs; seq += gridDim.x)
-            if (first[seq + 1] == first[seq]) clear_results(a, seq);
+            if (first[seq + 1] == first[seq]) clear_results<Shape::kThreads>(a, seq);
     } else {
-        const int seq = blockIdx.x / units, tiles = tiles_of_keys(keys_of(a, seq));
+        const int seq = blockIdx.x / units, tiles = tiles_of_keys<Shape::kTileKeys>(keys_of(a, seq));
         if (tiles > 0) run(seq, blockIdx.x % units, 0, tiles, nullptr);
-        else if (blockIdx.x % units == 0) clear_results(a, seq);
+        else if (blockIdx.x % units == 0) clear_results<Shape::kThreads>(a, seq);
     }
 }
 
-// Joins the pair that begins in stretch blockIdx.x and ends in a later one; a fourth of its heads
-template <int kDim>
-__global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const __grid_constant__ PagedAttentionArgs a) {
-    using Shape = PagedShape<kDim>;
+// Joins the pair that begins in stretch blockIdx.x and ends in a later one: warps_per_head of eight warps add up the parts of a head
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32;
+template <int kDim, int kWarps>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttentionArgs a, int warps_per_head) {
+    using Shape = PagedShape<kDim, kWarps>;
+    constexpr int kPer = kDim / 32;                  // channels of a lane
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float s_sum[kJoinWarps], s_value[kJoinWarps][kDim];
     int* first = reinterpret_cast<int*>(smem);
     ptx::wait_for_previous_kernel();
     ptx::let_next_kernel_start();
     const int chunks = chunks_of(a), units = a.kv_heads * chunks, group = a.heads / a.kv_heads;
-    count_tiles<kPagedThreads>(a, first);
+    count_tiles<kJoinThreads, Shape::kTileKeys>(a, first);
     const Stretch all(first[a.num_seqs], units, gridDim.x);
     const int64_t begin = all.share * blockIdx.x, end = begin + all.share;
     if (end >= all.total) return;
@@ -393,24 +405,35 @@ __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const __grid_
     const int last = static_cast<int>((p.begin + p.tiles - 1) / all.share);
     const int kv_head = p.unit / chunks, chunk = p.unit - kv_head * chunks, rows = min(group - chunk * kHeadRows, kHeadRows);
     const float c = a.scale * kPagedLog2e;
-    // 32 lanes by kDim / 32 channels per row
-    const int row = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    constexpr int kPer = kDim / 32;
-    if (row >= rows) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y * (kJoinWarps / warps_per_head) + warp / warps_per_head, mine = warp % warps_per_head;
+    const bool in = row < rows;
     auto part = [&](int cta) { return a.parts + (static_cast<int64_t>(cta) * 2 + (cta == static_cast<int>(blockIdx.x) ? 1 : 0)) * Shape::kPartFloats; };
-    float top = kLowest;
-    for (int cta = blockIdx.x + lane; cta <= last; cta += 32) top = fmaxf(top, part(cta)[kHeadRows * kDim + row]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float sum = 0.f, v[kPer] = {};
-#pragma unroll 4
-    for (int cta = blockIdx.x; cta <= last; ++cta) {
-        const float* from = part(cta);
-        const float t = from[kHeadRows * kDim + row], u = from[kHeadRows * kDim + kHeadRows + row];
-        const float factor = t == kLowest ? 0.f : ex2((t - top) * c);
-        sum += t == kLowest ? u * 0.f : u * factor;      // (a broken part's total is no number)
+    if (in) {
+        float top = kLowest;
+#pragma unroll 8
+        for (int cta = blockIdx.x + lane; cta <= last; cta += 32) top = fmaxf(top, part(cta)[kHeadRows * kDim + row]);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) v[i] = fmaf(from[row * kDim + lane * kPer + i], factor, v[i]);
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll 8
+        for (int cta = blockIdx.x + mine; cta <= last; cta += warps_per_head) {
+            const float* from = part(cta);
+            const float t = from[kHeadRows * kDim + row], u = from[kHeadRows * kDim + kHeadRows + row];
+            const float factor = t == kLowest ? 0.f : ex2((t - top) * c);
+            sum += t == kLowest ? u * 0.f : u * factor;      // (a broken part's total is no number)
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) v[i] = fmaf(from[row * kDim + lane * kPer + i], factor, v[i]);
+        }
+    }
+    if (lane == 0) s_sum[warp] = sum;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) s_value[warp][lane * kPer + i] = v[i];
+    __syncthreads();
+    if (!in || mine != 0) return;
+    for (int w = 1; w < warps_per_head; ++w) {
+        sum += s_sum[warp + w];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) v[i] += s_value[warp + w][lane * kPer + i];
     }
     const float inv = 1.f / sum;
     if (lane * kPer < a.dim) {
@@ -422,18 +445,24 @@ __global__ void __launch_bounds__(kPagedThreads) paged_join_kernel(const __grid_
 
 // ------------------------------------------------------------------------------------------------ host
 int units_of(const PagedAttentionArgs& a) { return a.kv_heads * ((a.heads / a.kv_heads + kHeadRows - 1) / kHeadRows); }
-// Sequences that cannot be longer than a stretch's least length: a CTA per pair, and nothing to join
-bool in_pairs(const PagedAttentionArgs& a) { return static_cast<int64_t>(a.table_width) * a.page_size <= kLeastTiles * kTileKeys; }
+int64_t capacity_of(const PagedAttentionArgs& a) { return static_cast<int64_t>(a.table_width) * a.page_size; }
+// Sequences that cannot be long: a CTA per pair, and nothing to join
+bool in_pairs(const PagedAttentionArgs& a) { return capacity_of(a) <= kPairKeys; }
+// Where pairs are many, most of what a CTA does is to begin and to end one: CTAs of one warp, eight times as many, do so beside one another.  Few pairs are cut into fewer stretches by
+// CTAs of four warps, whose parts are fewer to join.
+bool by_warps(const PagedAttentionArgs& a, int num_sms) { return static_cast<int64_t>(a.num_seqs) * units_of(a) >= kManyPairs * num_sms; }
+template <class Shape>
 int stretches(const PagedAttentionArgs& a, int num_sms) {
-    const int64_t most = (static_cast<int64_t>(a.table_width) * a.page_size + kTileKeys - 1) / kTileKeys * a.num_seqs * units_of(a);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(num_sms * 2, (most + kLeastTiles - 1) / kLeastTiles)));
+    const int64_t most = (capacity_of(a) + Shape::kTileKeys - 1) / Shape::kTileKeys * a.num_seqs * units_of(a);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(num_sms * Shape::kCtas, most)));
 }
-template <int kDim>
+template <int kDim, int kWarps>
 cudaError_t launch(const PagedAttentionArgs& a, int num_sms, cudaStream_t stream) {
-    using Shape = PagedShape<kDim>;
+    using Shape = PagedShape<kDim, kWarps>;
     const bool pairs = in_pairs(a);
-    const void* fn = pairs ? reinterpret_cast<const void*>(paged_attention_kernel<kDim, false>) : reinterpret_cast<const void*>(paged_attention_kernel<kDim, true>);
-    const int counts = (a.num_seqs + 1) * 4, most = Shape::kRing + (EP_MAX_PAGED_SEQS + 1) * 4;
+    const void* fn = pairs ? reinterpret_cast<const void*>(paged_attention_kernel<kDim, kWarps, false>) : reinterpret_cast<const void*>(paged_attention_kernel<kDim, kWarps, true>);
+    int counts = (a.num_seqs + 1) * 4;
+    const int most = Shape::kRing + (EP_MAX_PAGED_SEQS + 1) * 4;
     static std::atomic<uint64_t> allowed[2];
     int device = 0;
     cudaError_t err = cudaGetDevice(&device);
@@ -447,22 +476,37 @@ cudaError_t launch(const PagedAttentionArgs& a, int num_sms, cudaStream_t stream
         if (device < 64) allowed[pairs].fetch_or(1ull << device, std::memory_order_relaxed);
     }
     void* params[] = {const_cast<PagedAttentionArgs*>(&a)};
-    if (pairs) return launch_dependent(fn, dim3(static_cast<unsigned>(a.num_seqs * units_of(a))), dim3(kPagedThreads), params, Shape::kRing, stream);
-    const int ctas = stretches(a, num_sms);
-    err = launch_dependent(fn, dim3(ctas), dim3(kPagedThreads), params, Shape::kRing + counts, stream);
+    const int64_t num_pairs = static_cast<int64_t>(a.num_seqs) * units_of(a);
+    if (pairs) return launch_dependent(fn, dim3(static_cast<unsigned>(num_pairs)), dim3(Shape::kThreads), params, Shape::kRing, stream);
+    const int ctas = stretches<Shape>(a, num_sms);
+    err = launch_dependent(fn, dim3(ctas), dim3(Shape::kThreads), params, Shape::kRing + counts, stream);
     if (err != cudaSuccess) return err;
-    return launch_dependent(reinterpret_cast<const void*>(paged_join_kernel<kDim>), dim3(ctas, (std::min(a.heads / a.kv_heads, kHeadRows) + 3) / 4), dim3(kPagedThreads), params, counts,
-                            stream);
+    // warps for the parts that a pair may have
+    int warps_per_head = 1;
+    while (warps_per_head < kJoinWarps && ctas / num_pairs >= 8 * warps_per_head) warps_per_head *= 2;
+    const int heads = std::min(a.heads / a.kv_heads, kHeadRows), per_cta = kJoinWarps / warps_per_head;
+    void* join_params[] = {const_cast<PagedAttentionArgs*>(&a), &warps_per_head};
+    return launch_dependent(reinterpret_cast<const void*>(paged_join_kernel<kDim, kWarps>), dim3(ctas, (heads + per_cta - 1) / per_cta), dim3(kJoinThreads), join_params, counts, stream);
+}
+template <class F>
+auto with_shape(const PagedAttentionArgs& a, int num_sms, F f) {
+    using One = std::integral_constant<int, 1>;
+    using Four = std::integral_constant<int, 4>;
+    if (a.dim <= 64) return by_warps(a, num_sms) ? f(std::integral_constant<int, 64>{}, One{}) : f(std::integral_constant<int, 64>{}, Four{});
+    return by_warps(a, num_sms) ? f(std::integral_constant<int, 128>{}, One{}) : f(std::integral_constant<int, 128>{}, Four{});
 }
 
 }  // namespace
 
 int64_t paged_attention_workspace(const PagedAttentionArgs& a, int num_sms) {
     if (in_pairs(a)) return 0;
-    return static_cast<int64_t>(stretches(a, num_sms)) * 2 * (a.dim <= 64 ? PagedShape<64>::kPartFloats : PagedShape<128>::kPartFloats) * 4;
+    return with_shape(a, num_sms, [&](auto dim, auto warps) {
+        using Shape = PagedShape<decltype(dim)::value, decltype(warps)::value>;
+        return static_cast<int64_t>(stretches<Shape>(a, num_sms)) * 2 * Shape::kPartFloats * 4;
+    });
 }
 cudaError_t launch_paged_attention(const PagedAttentionArgs& a, int num_sms, cudaStream_t stream) {
-    return a.dim <= 64 ? launch<64>(a, num_sms, stream) : launch<128>(a, num_sms, stream);
+    return with_shape(a, num_sms, [&](auto dim, auto warps) { return launch<decltype(dim)::value, decltype(warps)::value>(a, num_sms, stream); });
 }
 
 }  // namespace ep
