@@ -624,6 +624,7 @@ struct PagedAttentionArgs {
     float scale;
     void* o;                          // bf16 [num_seqs, heads, dim] contiguous
     float* parts;                     // workspace of paged_attention_workspace() bytes
+    int4* open_pairs;                 // set by the launcher
 };
 
 namespace ep {

@@ -361,6 +361,7 @@ __global__ void __launch_bounds__(kWarps * 32, PagedShape<kDim, kWarps>::kCtas) 
         join_warps<kDim, kWarps>(a, smem, s_top, s_sum, st, seq, kv_head * group + first, rows, part, a.lengths[seq] > capacity(a));
     };
     if constexpr (kSplit) {
+        int4 open = make_int4(0, 0, 0, 0);           // the pair that begins here and ends in a later stretch: sequence, unit, last stretch, whether there is one
         int* first = reinterpret_cast<int*>(smem + Shape::kRing);
         count_tiles<Shape::kThreads, Shape::kTileKeys>(a, first);
         const Stretch all(first[a.num_seqs], units, gridDim.x);
@@ -373,8 +374,10 @@ __global__ void __launch_bounds__(kWarps * 32, PagedShape<kDim, kWarps>::kCtas) 
             const bool whole = at == p.begin && until == p.begin + p.tiles;
             float* part = whole ? nullptr : a.parts + (static_cast<int64_t>(blockIdx.x) * 2 + (p.begin >= begin ? 1 : 0)) * Shape::kPartFloats;
             run(p.seq, p.unit, static_cast<int>(at - p.begin), static_cast<int>(until - p.begin), part);
+            if (!whole && p.begin >= begin) open = make_int4(p.seq, p.unit, static_cast<int>((p.begin + p.tiles - 1) / all.share), 1);
             at = until;
         }
+        if (threadIdx.x == 0) a.open_pairs[blockIdx.x] = open;
         for (int seq = blockIdx.x; seq < a.num_seqs; seq += gridDim.x)
             if (first[seq + 1] == first[seq]) clear_results<Shape::kThreads>(a, seq);
     } else {
@@ -390,20 +393,13 @@ template <int kDim, int kWarps>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ PagedAttentionArgs a, int warps_per_head) {
     using Shape = PagedShape<kDim, kWarps>;
     constexpr int kPer = kDim / 32;                  // channels of a lane
-    extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_sum[kJoinWarps], s_value[kJoinWarps][kDim];
-    int* first = reinterpret_cast<int*>(smem);
     ptx::wait_for_previous_kernel();
     ptx::let_next_kernel_start();
-    const int chunks = chunks_of(a), units = a.kv_heads * chunks, group = a.heads / a.kv_heads;
-    count_tiles<kJoinThreads, Shape::kTileKeys>(a, first);
-    const Stretch all(first[a.num_seqs], units, gridDim.x);
-    const int64_t begin = all.share * blockIdx.x, end = begin + all.share;
-    if (end >= all.total) return;
-    const Pair p = find_pair(first, a.num_seqs, units, end - 1);
-    if (p.begin < begin || p.begin + p.tiles <= end) return;
-    const int last = static_cast<int>((p.begin + p.tiles - 1) / all.share);
-    const int kv_head = p.unit / chunks, chunk = p.unit - kv_head * chunks, rows = min(group - chunk * kHeadRows, kHeadRows);
+    const int4 p = a.open_pairs[blockIdx.x];
+    if (p.w == 0) return;
+    const int last = p.z, chunks = chunks_of(a), group = a.heads / a.kv_heads;
+    const int kv_head = p.y / chunks, chunk = p.y - kv_head * chunks, rows = min(group - chunk * kHeadRows, kHeadRows);
     const float c = a.scale * kPagedLog2e;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.y * (kJoinWarps / warps_per_head) + warp / warps_per_head, mine = warp % warps_per_head;
     const bool in = row < rows;
@@ -421,8 +417,11 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
             const float t = from[kHeadRows * kDim + row], u = from[kHeadRows * kDim + kHeadRows + row];
             const float factor = t == kLowest ? 0.f : ex2((t - top) * c);
             sum += t == kLowest ? u * 0.f : u * factor;      // (a broken part's total is no number)
+            float x[kPer];
+            if constexpr (kPer == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(from + row * kDim + lane * 4);
+            else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(from + row * kDim + lane * 2);
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) v[i] = fmaf(from[row * kDim + lane * kPer + i], factor, v[i]);
+            for (int i = 0; i < kPer; ++i) v[i] = fmaf(x[i], factor, v[i]);
         }
     }
     if (lane == 0) s_sum[warp] = sum;
@@ -437,7 +436,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     }
     const float inv = 1.f / sum;
     if (lane * kPer < a.dim) {
-        bf16* out = static_cast<bf16*>(a.o) + (static_cast<int64_t>(p.seq) * a.heads + kv_head * group + chunk * kHeadRows + row) * a.dim + lane * kPer;
+        bf16* out = static_cast<bf16*>(a.o) + (static_cast<int64_t>(p.x) * a.heads + kv_head * group + chunk * kHeadRows + row) * a.dim + lane * kPer;
 #pragma unroll
         for (int i = 0; i < kPer; i += 2) *reinterpret_cast<uint32_t*>(out + i) = pack2(v[i] * inv, v[i + 1] * inv);
     }
@@ -457,11 +456,11 @@ int stretches(const PagedAttentionArgs& a, int num_sms) {
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(num_sms * Shape::kCtas, most)));
 }
 template <int kDim, int kWarps>
-cudaError_t launch(const PagedAttentionArgs& a, int num_sms, cudaStream_t stream) {
+cudaError_t launch(PagedAttentionArgs a, int num_sms, cudaStream_t stream) {
     using Shape = PagedShape<kDim, kWarps>;
     const bool pairs = in_pairs(a);
     const void* fn = pairs ? reinterpret_cast<const void*>(paged_attention_kernel<kDim, kWarps, false>) : reinterpret_cast<const void*>(paged_attention_kernel<kDim, kWarps, true>);
-    int counts = (a.num_seqs + 1) * 4;
+    const int counts = (a.num_seqs + 1) * 4;
     const int most = Shape::kRing + (EP_MAX_PAGED_SEQS + 1) * 4;
     static std::atomic<uint64_t> allowed[2];
     int device = 0;
@@ -475,18 +474,19 @@ cudaError_t launch(const PagedAttentionArgs& a, int num_sms, cudaStream_t stream
         }
         if (device < 64) allowed[pairs].fetch_or(1ull << device, std::memory_order_relaxed);
     }
-    void* params[] = {const_cast<PagedAttentionArgs*>(&a)};
+    void* params[] = {&a};
     const int64_t num_pairs = static_cast<int64_t>(a.num_seqs) * units_of(a);
     if (pairs) return launch_dependent(fn, dim3(static_cast<unsigned>(num_pairs)), dim3(Shape::kThreads), params, Shape::kRing, stream);
     const int ctas = stretches<Shape>(a, num_sms);
+    a.open_pairs = reinterpret_cast<int4*>(a.parts + static_cast<int64_t>(ctas) * 2 * Shape::kPartFloats);
     err = launch_dependent(fn, dim3(ctas), dim3(Shape::kThreads), params, Shape::kRing + counts, stream);
     if (err != cudaSuccess) return err;
     // warps for the parts that a pair may have
     int warps_per_head = 1;
     while (warps_per_head < kJoinWarps && ctas / num_pairs >= 8 * warps_per_head) warps_per_head *= 2;
     const int heads = std::min(a.heads / a.kv_heads, kHeadRows), per_cta = kJoinWarps / warps_per_head;
-    void* join_params[] = {const_cast<PagedAttentionArgs*>(&a), &warps_per_head};
-    return launch_dependent(reinterpret_cast<const void*>(paged_join_kernel<kDim, kWarps>), dim3(ctas, (heads + per_cta - 1) / per_cta), dim3(kJoinThreads), join_params, counts, stream);
+    void* join_params[] = {&a, &warps_per_head};
+    return launch_dependent(reinterpret_cast<const void*>(paged_join_kernel<kDim, kWarps>), dim3(ctas, (heads + per_cta - 1) / per_cta), dim3(kJoinThreads), join_params, 0, stream);
 }
 template <class F>
 auto with_shape(const PagedAttentionArgs& a, int num_sms, F f) {
@@ -502,7 +502,7 @@ int64_t paged_attention_workspace(const PagedAttentionArgs& a, int num_sms) {
     if (in_pairs(a)) return 0;
     return with_shape(a, num_sms, [&](auto dim, auto warps) {
         using Shape = PagedShape<decltype(dim)::value, decltype(warps)::value>;
-        return static_cast<int64_t>(stretches<Shape>(a, num_sms)) * 2 * Shape::kPartFloats * 4;
+        return static_cast<int64_t>(stretches<Shape>(a, num_sms)) * (2 * Shape::kPartFloats * 4 + 16);      // (parts, then open_pairs)
     });
 }
 cudaError_t launch_paged_attention(const PagedAttentionArgs& a, int num_sms, cudaStream_t stream) {
