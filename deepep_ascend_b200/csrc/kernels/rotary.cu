@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kForwardCtas) rotary_kernel(co
     for (int i = 0; i < kIters; ++i)
         if (place.on && head0 + i * Lane::kRows < heads)
             raw[i] = load8<kInterleaved>(static_cast<const T*>(x.data) + token * x.stride_token + (head0 + i * Lane::kRows) * x.stride_head, place.lo, place.hi);
-    T* out;
+    T *out, *too = nullptr;                              // (keys may go to a cache and to a result)
     int64_t pitch;
     bool write = place.on;
     if (kind == 0 || a.k_cache == nullptr) {
@@ -225,6 +225,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kForwardCtas) rotary_kernel(co
         const int64_t page = slot / a.page_size;
         out = static_cast<T*>(kind == 1 ? a.k_cache : a.v_cache) + page * a.stride_page + (slot - page * a.page_size) * a.stride_slot;
         pitch = a.stride_head;
+        if (kind == 1 && a.out[1] != nullptr) too = static_cast<T*>(a.out[1]) + (token * heads + head0) * a.dim;
     }
     if (kind == 2) {
 #pragma unroll
@@ -240,7 +241,10 @@ __global__ void __launch_bounds__(kRotaryThreads, kForwardCtas) rotary_kernel(co
         const Eight<T> fill = all_of<T>(turn.keep);
 #pragma unroll
         for (int i = 0; i < kIters; ++i)
-            if (write && head0 + i * Lane::kRows < heads) store8<kInterleaved>(out + i * Lane::kRows * pitch, place.lo, place.hi, fill);
+            if (head0 + i * Lane::kRows < heads) {
+                if (write) store8<kInterleaved>(out + i * Lane::kRows * pitch, place.lo, place.hi, fill);
+                if (too != nullptr && place.on) store8<kInterleaved>(too + i * Lane::kRows * a.dim, place.lo, place.hi, fill);
+            }
         return;
     }
     turn.times(w);
@@ -255,7 +259,11 @@ __global__ void __launch_bounds__(kRotaryThreads, kForwardCtas) rotary_kernel(co
         uint64_t y[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) y[j] = mul2(rstd2, fma2(partner_of<kInterleaved>(v, j), turn.partner[j], mul2(v[j], turn.own[j])));
-        if (write && head0 + i * Lane::kRows < heads) store8<kInterleaved>(out + i * Lane::kRows * pitch, place.lo, place.hi, from_float<T>(y));
+        if (head0 + i * Lane::kRows < heads) {
+            const Eight<T> e = from_float<T>(y);
+            if (write) store8<kInterleaved>(out + i * Lane::kRows * pitch, place.lo, place.hi, e);
+            if (too != nullptr && place.on) store8<kInterleaved>(too + i * Lane::kRows * a.dim, place.lo, place.hi, e);
+        }
     }
 }
 

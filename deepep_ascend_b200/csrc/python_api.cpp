@@ -1003,7 +1003,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("qk_norm_rope", &qk_norm_rope, py::arg("q"), py::arg("k"), py::arg("q_weight"), py::arg("k_weight"), py::arg("table"), py::arg("positions"), py::arg("eps"),
           py::arg("interleaved"));
     m.def("qk_norm_rope_append", &qk_norm_rope_append, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("q_weight"), py::arg("k_weight"), py::arg("table"), py::arg("positions"),
-          py::arg("k_cache"), py::arg("v_cache"), py::arg("slots"), py::arg("eps"), py::arg("interleaved"));
+          py::arg("k_cache"), py::arg("v_cache"), py::arg("slots"), py::arg("eps"), py::arg("interleaved"), py::arg("keep_k"));
     m.def("qk_norm_rope_backward", &qk_norm_rope_backward, py::arg("dq"), py::arg("dk"), py::arg("q"), py::arg("k"), py::arg("q_weight"), py::arg("k_weight"), py::arg("table"),
           py::arg("positions"), py::arg("eps"), py::arg("interleaved"));
     m.def("gemm_error", [](int device) { return gemm_error_flag(device).item<int>(); });

@@ -244,9 +244,9 @@ inline std::optional<std::tuple<at::Tensor, at::Tensor>> qk_norm_rope(const at::
     cuda_check(ep::launch_rotary(in.a, device_sms(), at::cuda::getCurrentCUDAStream()), "rotation launch");
     return std::make_tuple(yq, yk);
 }
-inline std::optional<at::Tensor> qk_norm_rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& q_weight, const at::Tensor& k_weight,
+inline std::optional<std::tuple<at::Tensor, std::optional<at::Tensor>>> qk_norm_rope_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& q_weight, const at::Tensor& k_weight,
                                                      const at::Tensor& table, const at::Tensor& positions, at::Tensor k_cache, at::Tensor v_cache, const at::Tensor& slots, double eps,
-                                                     bool interleaved) {
+                                                     bool interleaved, bool keep_k) {
     if (not_for_a_kernel({&q, &k, &v, &q_weight, &k_weight, &table, &k_cache, &v_cache}) || watched({&positions, &slots})) return std::nullopt;
     const c10::cuda::CUDAGuard guard(q.device());
     RotaryInputs in = rotary_inputs(q, k, q_weight, k_weight, table, positions, eps, interleaved);
@@ -256,10 +256,13 @@ inline std::optional<at::Tensor> qk_norm_rope_append(const at::Tensor& q, const 
     TORCH_CHECK(slots.device() == q.device() && slots.dim() == 1 && slots.size(0) == q.size(0) && (slots.scalar_type() == at::kLong || slots.scalar_type() == at::kInt),
                 "slots must be int64 or int32 [tokens] on the device of q");
     at::Tensor yq = at::empty(q.sizes(), q.options());
-    if (q.size(0) == 0) return yq;
+    std::optional<at::Tensor> yk;
+    if (keep_k) yk = at::empty(k.sizes(), k.options());
+    if (q.size(0) == 0) return std::make_tuple(yq, yk);
     const at::Tensor v16 = heads_of(v), s = slots.contiguous();
     RotaryArgs& a = in.a;
     a.out[0] = yq.data_ptr();
+    if (keep_k) a.out[1] = yk->data_ptr();
     a.v = view_of(v16);
     a.k_cache = k_cache.data_ptr();
     a.v_cache = v_cache.data_ptr();
@@ -271,7 +274,7 @@ inline std::optional<at::Tensor> qk_norm_rope_append(const at::Tensor& q, const 
     a.slots = s.data_ptr();
     a.slots_64 = s.scalar_type() == at::kLong;
     cuda_check(ep::launch_rotary(a, device_sms(), at::cuda::getCurrentCUDAStream()), "rotation launch");
-    return yq;
+    return std::make_tuple(yq, yk);
 }
 using RotaryGradients = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
 inline std::optional<RotaryGradients> qk_norm_rope_backward(const at::Tensor& dq, const at::Tensor& dk, const at::Tensor& q, const at::Tensor& k, const at::Tensor& q_weight,

@@ -3,7 +3,7 @@ straight into a paged cache.  CPU tensors take the PyTorch statements below.
 
 No counterpart in the reference, which stops at the exchange of tokens.
 """
-from typing import Optional, Tuple
+from typing import Tuple, Union
 
 import torch
 
@@ -63,17 +63,19 @@ def qk_norm_rope_backward(dq: torch.Tensor, dk: torch.Tensor, q: torch.Tensor, k
 
 
 def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor, table: torch.Tensor, positions: torch.Tensor,
-                        k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, eps: float = 1e-6, interleaved: bool = False) -> torch.Tensor:
-    """:func:`qk_norm_rope` whose keys, with the values ``v`` (like ``k``) as they are, go to their places in paged caches -> the queries.
+                        k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, eps: float = 1e-6, interleaved: bool = False,
+                        keep_k: bool = False) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """:func:`qk_norm_rope` whose keys, with the values ``v`` (like ``k``) as they are, go to their places in paged caches -> the queries, or with ``keep_k``
+    ``(queries, keys)``, for a prompt whose attention is taken at once.
 
     ``k_cache`` and ``v_cache [pages, page_size, kv_heads, dim]``: of the heads' type, one layout, channels contiguous, heads on 16 bytes (views of one
     allocation, or with the heads in front of the places, are as good).  Token ``t`` goes to place ``slots[t] % page_size`` of page ``slots[t] // page_size`` (int64 or int32); tokens whose
     slot is not in the caches go nowhere.  Slots that several tokens name hold one of them.  What is in the caches carries no gradient."""
     if q.is_cuda and _by_type(q, k, v, q_weight, k_weight, table, positions, k_cache, v_cache, slots):
-        res = _native.load().qk_norm_rope_append(q, k, v, q_weight, k_weight, table, positions, k_cache, v_cache, slots, eps, interleaved)
+        res = _native.load().qk_norm_rope_append(q, k, v, q_weight, k_weight, table, positions, k_cache, v_cache, slots, eps, interleaved, keep_k)
         if res is not None:
-            return res
-    return qk_norm_rope_append_ref(q, k, v, q_weight, k_weight, table, positions, k_cache, v_cache, slots, eps, interleaved)
+            return res if keep_k else res[0]
+    return qk_norm_rope_append_ref(q, k, v, q_weight, k_weight, table, positions, k_cache, v_cache, slots, eps, interleaved, keep_k)
 
 
 def _wide(t: torch.Tensor) -> torch.Tensor:
@@ -121,7 +123,7 @@ def qk_norm_rope_backward_ref(dq, dk, q, k, q_weight, k_weight, table, positions
     return (*dx, *dw)
 
 
-def qk_norm_rope_append_ref(q, k, v, q_weight, k_weight, table, positions, k_cache, v_cache, slots, eps=1e-6, interleaved=False):
+def qk_norm_rope_append_ref(q, k, v, q_weight, k_weight, table, positions, k_cache, v_cache, slots, eps=1e-6, interleaved=False, keep_k=False):
     """:func:`qk_norm_rope_append` stated with plain PyTorch operations."""
     q, k = qk_norm_rope_ref(q, k, q_weight, k_weight, table, positions, eps, interleaved)
     pages, size = k_cache.shape[:2]
@@ -129,4 +131,4 @@ def qk_norm_rope_append_ref(q, k, v, q_weight, k_weight, table, positions, k_cac
     at = slots[keep].long()
     for cache, new in ((k_cache, k), (v_cache, v)):
         cache[at // size, at % size] = new[keep].detach()
-    return q
+    return (q, k) if keep_k else q

@@ -146,6 +146,9 @@ def test_into_paged_caches(T, Hq, Hk, D, size, dtype, index, layout, device):
         keep = (slots >= 0) & (slots < pages * size)
         want[slots[keep].long()] = new[keep]
         assert torch.equal(cache.reshape(-1, Hk, D), want)
+    # the keys as a result too, those that go nowhere among them
+    again = qk_norm_rope_append(given['q'], given['k'], v, qw, kw, table, positions, k_cache, v_cache, slots, keep_k=True)
+    assert torch.equal(again[0], q) and torch.equal(again[1], k)
 
 
 @pytest.mark.gpu
