@@ -53,7 +53,7 @@ inline PackedInputs packed_inputs(const at::Tensor& q, const at::Tensor& k, cons
         a.cu_k = cu_k->data_ptr<int>();
     }
     TORCH_CHECK((q.size(0) / 128 + a.num_seqs) * q.size(1) < (1ll << 31) && (k.size(0) / 128 + a.num_seqs) * q.size(1) < (1ll << 31) &&
-                    q.size(0) * q.size(1) < (1ll << 34), "too much work for one launch");
+                    q.size(0) * q.size(1) < (1ll << 34) && (q.size(0) / 128 + 1) * (q.size(1) / k.size(1)) < (1ll << 31), "too much work for one launch");
     in.q = heads_of(q);
     in.k = heads_of(k);
     in.v = heads_of(v);
@@ -148,7 +148,7 @@ inline at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache
                 "page_table must be int32 [sequences, pages] with contiguous rows on the device of q");
     TORCH_CHECK(lengths.device() == q.device() && lengths.scalar_type() == at::kInt && lengths.dim() == 1 && lengths.size(0) == B && lengths.is_contiguous(),
                 "lengths must be contiguous int32 [sequences] on the device of q");
-    TORCH_CHECK(B * (page_table.size(1) * k_cache.size(1) / 64 + 1) < (1ll << 31), "too many places in page_table");
+    TORCH_CHECK(page_table.size(1) * k_cache.size(1) < (1ll << 31) - 65536 && B * (page_table.size(1) * k_cache.size(1) / 16 + 1) < (1ll << 31), "too many places in page_table");
     TORCH_CHECK(std::isfinite(scale) && scale > 0, "scale must be positive");
     at::Tensor o = out.has_value() ? *out : at::empty(q.sizes(), q.options());
     TORCH_CHECK(o.device() == q.device() && o.scalar_type() == at::kBFloat16 && o.is_contiguous() && o.sizes() == q.sizes() && reinterpret_cast<uintptr_t>(o.data_ptr()) % 16 == 0,
@@ -253,6 +253,7 @@ inline std::optional<std::tuple<at::Tensor, std::optional<at::Tensor>>> qk_norm_
     TORCH_CHECK(v.device() == q.device() && v.scalar_type() == q.scalar_type() && v.sizes() == k.sizes(), "v must be like k");
     check_caches(k_cache, v_cache, q, q.scalar_type());
     TORCH_CHECK(k_cache.size(2) == k.size(1) && k_cache.size(3) == k.size(2), "the caches must have the heads and channels of k");
+    for (int i = 0; i < 3; ++i) TORCH_CHECK(k_cache.size(i) <= 1 || k_cache.stride(i) > 0, "places and heads of the caches must not share memory");
     TORCH_CHECK(slots.device() == q.device() && slots.dim() == 1 && slots.size(0) == q.size(0) && (slots.scalar_type() == at::kLong || slots.scalar_type() == at::kInt),
                 "slots must be int64 or int32 [tokens] on the device of q");
     at::Tensor yq = at::empty(q.sizes(), q.options());
