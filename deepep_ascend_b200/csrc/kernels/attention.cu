@@ -20,6 +20,7 @@ namespace ep {
 namespace {
 
 constexpr uint64_t kAttnWaitLimitNs = 4ull * 1000 * 1000 * 1000;      // when the caller gives no limit
+constexpr uint64_t kLandNs = 10ull * 1000 * 1000;                     // after a failure: what a copy is given to land (a phase that nothing is on its way for takes it all)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 using bf16 = __nv_bfloat16;
@@ -271,7 +272,13 @@ __device__ __forceinline__ void store_part(uint32_t tmem, float factor, float* r
 // probabilities, the tensor cores work for the other.  Probabilities take the place of the scores in tensor memory, from where they are the first operand of the next product.
 //
 // A CTA goes on with the work of CTAs that have not started (it cancels their launch and takes their place): barriers and tensor memory are set up once, and the next block's
-// queries, keys and values come while the last one's results leave.  Blocks differ in length, so who takes which is decided as they end.
+// queries, keys and values come while the last one's results leave.  Blocks differ in length, so who takes which is decided as they end.  (31 prompts of 264 tokens, 56 heads of 128: 268 us with
+// a CTA for every block, 150 so.)
+//
+// Long sequences are bound by power: 16384 tokens, 56 heads of 128, 3.0 to 3.4 ms, 1.1 to 1.3 PFLOP/s at SM clocks of 1.4 to 1.55 GHz, the tensor pipe busy in 67 % of them.  What the clocks go by is the
+// chain of a tile's block of 128 keys, some 3000 of which two tiles share: 70 for the scores into registers, 370 for their largest, 1050 for the powers, 100 for their way back, 512 + 512 for
+// the products and as much for the barriers between, which lie in the shared memory that the products read at its full rate.  So a quarter of the powers by polynomial, the first half of
+// the probabilities handed over early and an issuing thread for each tile took it from 3650 clocks to 3030.
 constexpr int kFwdThreads = 384;                     // 2 x 4 warps for the softmaxes, one that requests tiles, two that issue products, one that looks for work
 constexpr int kFwdReaders = 11;                      // ... of which so many do it
 template <int kChunks>
@@ -660,9 +667,10 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     if (b->st.failed != 0) {
         // (a wait has run out: what was requested or issued ends before its memory goes to others)
         if (warp == 8) {
-            for (int i = 0; i < 2; ++i) mbar_drain(&b->q_full[i], 0, 100000000ull), mbar_drain(&b->q_full[i], 1, 100000000ull);
-            for (int i = 0; i < kStages; ++i) mbar_drain(&b->full[i], 0, 100000000ull), mbar_drain(&b->full[i], 1, 100000000ull);
-            mbar_drain(&b->answered, 0, 100000000ull), mbar_drain(&b->answered, 1, 100000000ull);
+            for (int i = 0; i < 2; ++i) mbar_drain(&b->q_full[i], 0, kLandNs), mbar_drain(&b->q_full[i], 1, kLandNs);
+            for (int i = 0; i < kStages; ++i) mbar_drain(&b->full[i], 0, kLandNs), mbar_drain(&b->full[i], 1, kLandNs);
+            mbar_drain(&b->answered, 0, kLandNs), mbar_drain(&b->answered, 1, kLandNs);
+            mbar_drain(&b->tail, 0, kLandNs), mbar_drain(&b->tail, 1, kLandNs);
         }
         if ((warp == 9 || warp == 10) && ptx::elect_one()) {
             umma::mma_commit(&b->quiet[warp - 9]);
@@ -707,6 +715,9 @@ __global__ void __launch_bounds__(kDeltaThreads) attention_delta_kernel(const __
 // pieces of 128.  Scores and dP of a piece are products whose lanes are the kept rows, so that P and dS are first operands of the products that follow, and sums stay in
 // tensor memory until the end: every gradient is added by one CTA (or by one per part of the group, whose parts are then added), in a fixed order.  P is made twice, which
 // costs two products of seven, and spares sums of dQ in memory by many CTAs in any order.
+//
+// 16384 tokens, 56 heads of 128: 11.5 ms, 0.84 PFLOP/s counted as five products and 1.17 as seven, bound by power as the forward pass; two documents of 4096: 1.4 to 1.6 ms.  Short sequences are bound
+// by the chain of a piece, some 2200 clocks, and by what a block takes to begin and to end.
 //
 // Two groups of four warps have 64 columns of a piece each.  P and dS take the place of dP; that of the scores is free as soon as they are in registers, so the next piece's
 // scores are made meanwhile, and their powers while dV, dK and the next dP are.  (Pieces of 64 columns with two places for each had products of half the width, which take as long
@@ -1120,9 +1131,10 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
     if (b->st.failed != 0) {
         // (as in the forward pass)
         if (warp == 8) {
-            mbar_drain(&b->kept, 0, 100000000ull), mbar_drain(&b->kept, 1, 100000000ull);
-            mbar_drain(&b->answered, 0, 100000000ull), mbar_drain(&b->answered, 1, 100000000ull);
-            for (int i = 0; i < kSlots; ++i) mbar_drain(&b->full[i], 0, 100000000ull), mbar_drain(&b->full[i], 1, 100000000ull);
+            mbar_drain(&b->kept, 0, kLandNs), mbar_drain(&b->kept, 1, kLandNs);
+            mbar_drain(&b->answered, 0, kLandNs), mbar_drain(&b->answered, 1, kLandNs);
+            mbar_drain(&b->tail, 0, kLandNs), mbar_drain(&b->tail, 1, kLandNs);
+            for (int i = 0; i < kSlots; ++i) mbar_drain(&b->full[i], 0, kLandNs), mbar_drain(&b->full[i], 1, kLandNs);
         }
         if (warp == 9 && ptx::elect_one()) {
             umma::mma_commit(&b->quiet);

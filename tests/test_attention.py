@@ -348,3 +348,58 @@ def test_refusals():
     for bad in (dict(d_o=d_o[:5]), dict(d_o=d_o.float()), dict(o=o[:, :2]), dict(lse=lse.t()), dict(lse=lse.double()), dict(d_lse=d_lse[:1])):
         with pytest.raises(RuntimeError):
             attention_backward(**{**dict(d_o=d_o, q=q, k=k, v=v, o=o, lse=lse, cu_seqlens=cu), **bad})
+
+
+_SHORT_LIMIT = """
+import torch
+from deepep_ascend_b200 import ElasticBuffer, _native
+from deepep_ascend_b200.ops.attention import attention, attention_backward
+torch.manual_seed(0)
+make = lambda n: [torch.randn(n, 1, 64, device='cuda').bfloat16() for _ in range(4)]
+q, k, v, g = make(1000)
+want = attention(q, k, v)
+grads = attention_backward(g, q, k, v, *want)
+buf = ElasticBuffer(None, num_max_tokens_per_rank=16, hidden=256, num_topk=2)
+assert torch.equal(attention(q, k, v, buffer=buf)[0], want[0])
+assert all(torch.equal(a, b) for a, b in zip(attention_backward(g, q, k, v, *want, buffer=buf), grads))
+torch.cuda.synchronize()
+buf.check_status()
+x, y, z, d = make(100000)
+if BACKWARD:
+    o, lse = attention(x, y, z, causal=False)
+    torch.cuda.synchronize()
+buf.core.set_gpu_timeout(3e-4)
+if BACKWARD:
+    attention_backward(d, x, y, z, o, lse, causal=False, buffer=buf)
+else:
+    attention(x, y, z, causal=False, buffer=buf)
+torch.cuda.synchronize()
+code, phase, peer, expected, observed, rank = buf.core.read_status()
+assert (code, phase, rank) == (1, 14, 0) and expected in (1, 7), (code, phase, expected, rank)
+assert _native.load().gemm_error(0) == expected
+try:
+    buf.check_status()
+except RuntimeError as e:
+    assert 'timed out' in str(e)
+else:
+    raise AssertionError('the wait was not reported')
+# shared and tensor memory have been given back, and what follows is right
+for _ in range(3):
+    o, lse = attention(q, k, v)
+    assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+    assert all(torch.equal(a, b) for a, b in zip(attention_backward(g, q, k, v, *want), grads))
+print('reported')
+"""
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('backward', [False, True])
+def test_a_wait_that_runs_out_is_reported(backward):
+    """A block of 128 rows against 100000 takes a millisecond, while who waits for its end has 0.3.  (In a process of its own: the device's error flag stays up.)"""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, '-c', _SHORT_LIMIT.replace('BACKWARD', str(backward))], cwd=root, env=dict(os.environ, PYTHONPATH=root), capture_output=True, text=True,
+                         timeout=120)
+    assert run.returncode == 0 and run.stdout.strip().endswith('reported'), run.stderr[-2000:]
