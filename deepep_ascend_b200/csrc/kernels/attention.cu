@@ -213,15 +213,15 @@ __device__ __forceinline__ uint64_t exp2_by_polynomial(uint64_t x2) {
 }
 constexpr int kPolynomialOf = 4;                     // of so many pairs of a row one goes by the polynomial
 
-// The two groups of four warps that hold rows take registers of the third: 384 x 168 at launch = 128 x (2 rows' + the others')
-constexpr int kFwdRegisters = 224, kBwdRegisters = 208;
-template <int kRows>
+// The groups of four warps that hold rows take registers of the other one: 384 x 168 at launch = 128 x (2 rows' + the others'), 256 x 128 = 128 x (rows' + the others')
+constexpr int kFwdRegisters = 224, kFwdRegistersOfTwo = 200, kBwdRegisters = 208;
+template <int kRegisters>
 __device__ __forceinline__ void take_registers() {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRows));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegisters));
 }
-template <int kRows>
+template <int kRegisters>
 __device__ __forceinline__ void give_registers() {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(3 * 168 - 2 * kRows));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters));
 }
 
 // A row of sums in tensor memory, times `factor`, as bf16
@@ -279,13 +279,16 @@ __device__ __forceinline__ void store_part(uint32_t tmem, float factor, float* r
 // chain of a tile's block of 128 keys, some 3000 of which two tiles share: 70 for the scores into registers, 370 for their largest, 1050 for the powers, 100 for their way back, 512 + 512 for
 // the products and as much for the barriers between, which lie in the shared memory that the products read at its full rate.  So a quarter of the powers by polynomial, the first half of
 // the probabilities handed over early and an issuing thread for each tile took it from 3650 clocks to 3030.
-constexpr int kFwdThreads = 384;                     // 2 x 4 warps for the softmaxes, one that requests tiles, two that issue products, one that looks for work
-constexpr int kFwdReaders = 11;                      // ... of which so many do it
-template <int kChunks>
+// Short sequences have one tile per CTA and two CTAs on an SM, one of which works while the other begins or ends a block; two tiles read keys and values from L2 once for both.
+template <int kChunks, int kTiles>
 struct FwdShape {
-    static constexpr int kTileBytes = 128 * 128 * kChunks, kStages = kChunks == 2 ? 5 : 8;
-    static constexpr int kOut = 256;                  // tensor memory: two tiles' scores, then two tiles' sums
-    static constexpr int kSmem = (2 + kStages) * kTileBytes + 1024;
+    // four warps per tile for its softmax; one that requests tiles, one per tile that issues products, one that looks for work, and to make up four more one without any
+    static constexpr int kRowWarps = 4 * kTiles, kLoadWarp = kRowWarps, kMultiplyWarp = kRowWarps + 1, kWorkWarp = kRowWarps + 1 + kTiles;
+    static constexpr int kThreads = kRowWarps * 32 + 128, kReaders = kRowWarps + 1 + kTiles, kRegisters = kTiles == 2 ? kFwdRegisters : kFwdRegistersOfTwo;
+    static constexpr int kLaunchRegisters = kTiles == 2 ? 168 : 128;
+    static constexpr int kTileBytes = 128 * 128 * kChunks, kStages = kTiles == 2 ? (kChunks == 2 ? 5 : 8) : (kChunks == 2 ? 2 : 5);
+    static constexpr int kOut = kTiles * 128, kColumns = kTiles * 256;      // tensor memory: the tiles' scores, then their sums
+    static constexpr int kSmem = (kTiles + kStages) * kTileBytes + 1024;
 };
 struct FwdWork {
     int start, rows;                 // as of AttnBlock; rows < 0: no more work
@@ -320,15 +323,15 @@ __device__ __forceinline__ int work_of_answer(Bars* b) {
     return got != 0 ? static_cast<int>(x) : -1;
 }
 
-template <int kChunks>
-__global__ void __launch_bounds__(kFwdThreads, 1)
+template <int kChunks, int kTiles>
+__global__ void __launch_bounds__(FwdShape<kChunks, kTiles>::kThreads, 3 - kTiles)
 attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                  const __grid_constant__ AttentionArgs a) {
-    using Shape = FwdShape<kChunks>;
+    using Shape = FwdShape<kChunks, kTiles>;
     constexpr int kStages = Shape::kStages, kTileBytes = Shape::kTileBytes;
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t *sq = smem, *skv = smem + 2 * kTileBytes;
-    FwdBars* b = reinterpret_cast<FwdBars*>(smem + (2 + kStages) * kTileBytes);
+    uint8_t *sq = smem, *skv = smem + kTiles * kTileBytes;
+    FwdBars* b = reinterpret_cast<FwdBars*>(smem + (kTiles + kStages) * kTileBytes);
     const int warp = threadIdx.x >> 5;
     int* failed = &b->st.failed;
     if (threadIdx.x == 0) {
@@ -346,17 +349,17 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         }
         for (int i = 0; i < kStages; ++i) {
             ptx::mbar_init(&b->full[i], 1);
-            ptx::mbar_init(&b->empty[i], 2);
+            ptx::mbar_init(&b->empty[i], kTiles);
         }
         ptx::mbar_init(&b->work_full, 1);
-        ptx::mbar_init(&b->work_read, kFwdReaders);
+        ptx::mbar_init(&b->work_read, Shape::kReaders);
         ptx::mbar_init(&b->answered, 1);
         ptx::mbar_init(&b->tail, 1);
         b->st.failed = 0;
         ptx::mbar_fence_init();
     }
-    if (warp == 9) {
-        umma::tmem_alloc(&b->st.tmem_base, 512);
+    if (warp == Shape::kMultiplyWarp) {
+        umma::tmem_alloc(&b->st.tmem_base, Shape::kColumns);
         umma::tmem_relinquish();
     }
     umma::fence_before_thread_sync();
@@ -373,9 +376,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         return w.rows >= 0;
     };
 
-    if (warp >= 8) {
-        give_registers<kFwdRegisters>();
-        if (warp == 8) {
+    if (warp >= Shape::kRowWarps) {
+        give_registers<(kTiles + 1) * Shape::kLaunchRegisters - kTiles * Shape::kRegisters>();
+        if (warp == Shape::kLoadWarp) {
             AttnRing<kStages> p;
             const bool one = ptx::elect_one();
             uint32_t tails = 0, queries[2] = {0, 0};
@@ -403,7 +406,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 for (int k = 0; next_work(k, w); ++k) {
                     const int blocks = w.blocks();
 #pragma unroll
-                    for (int t = 0; t < 2; ++t)
+                    for (int t = 0; t < kTiles; ++t)
                         if (w.n[t] > 0) {
                             if (!attn_wait_warp(&b->q_empty[t], (queries[t] & 1) ^ 1, failed, a.report, 1)) return;
                             ++queries[t];
@@ -418,9 +421,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 }
             };
             load();
-        } else if (warp < 11) {
-            // a tile's products; what neither tile reads any more is free
-            const int t = warp - 9;
+        } else if (warp < Shape::kWorkWarp) {
+            // a tile's products; what no tile reads any more is free
+            const int t = warp - Shape::kMultiplyWarp;
             const bool one = ptx::elect_one();
             const int dim16 = (a.dim + 15) / 16;
             const uint32_t idesc_s = umma::make_instr_desc(128, 128, umma::kFormatBF16), to_s = tmem + t * 128, to_o = tmem + Shape::kOut + t * 128;
@@ -478,7 +481,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 if (one && w.blocks() > 0) multiply(w.blocks(), t == 0 ? w.n[0] : w.n[1]);
                 __syncwarp();
             }
-        } else {
+        } else if (warp == Shape::kWorkWarp) {
             // looks for work: first this CTA's own
             const int blocks = gridDim.x / a.heads;
             int item = blockIdx.x;
@@ -488,20 +491,20 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 FwdWork w{};
                 w.rows = -1;
                 if (item >= 0) {
-                    // 256 rows of a group's heads are as many pairs of tiles as the group has heads.  Long blocks first: those at the ends of the sequences
-                    const int number = item / a.heads, pair = item - number * a.heads, group = a.heads / a.kv_heads;
-                    const AttnBlock blk = find_block<256>(a.cu_q, a.num_seqs, a.tq, blocks - 1 - number);
+                    // 256 rows of a group's heads are as many pairs of tiles as the group has heads (128 rows: as many tiles).  Long blocks first: those at the ends of the sequences
+                    const int number = item / a.heads, unit = item - number * a.heads, group = a.heads / a.kv_heads;
+                    const AttnBlock blk = find_block<128 * kTiles>(a.cu_q, a.num_seqs, a.tq, blocks - 1 - number);
                     const int2 keys = sequence_rows(a.cu_k, blk.seq, a.tk);
                     clear_rows<32>(a.cu_q, a.num_seqs, a.tq, item, gridDim.x, reinterpret_cast<bf16*>(a.o), static_cast<int64_t>(a.heads) * a.dim, a.lse, a.heads);
                     w.start = blk.start;
                     w.rows = blk.rows;
                     w.key0 = keys.x;
                     w.keys = keys.y;
-                    w.kv_head = pair / group;
-                    const int tile = (pair - w.kv_head * group) * 2;
+                    w.kv_head = unit / group;
+                    const int tile = (unit - w.kv_head * group) * kTiles;
                     something = false;
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
+                    for (int t = 0; t < kTiles; ++t) {
                         const bool upper = tile + t >= group;
                         w.row0[t] = blk.row0 + (upper ? 128 : 0);
                         w.head[t] = w.kv_head * group + tile + t - (upper ? group : 0);
@@ -527,7 +530,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             }
         }
     } else {
-        take_registers<kFwdRegisters>();
+        take_registers<Shape::kRegisters>();
         const int t = warp >> 2, lane_row = threadIdx.x & 127;
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), ts = lanes + t * 128, to = lanes + Shape::kOut + t * 128;
         const float c = a.scale * kLog2e;
@@ -666,19 +669,19 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     __syncthreads();
     if (b->st.failed != 0) {
         // (a wait has run out: what was requested or issued ends before its memory goes to others)
-        if (warp == 8) {
-            for (int i = 0; i < 2; ++i) mbar_drain(&b->q_full[i], 0, kLandNs), mbar_drain(&b->q_full[i], 1, kLandNs);
+        if (warp == Shape::kLoadWarp) {
+            for (int i = 0; i < kTiles; ++i) mbar_drain(&b->q_full[i], 0, kLandNs), mbar_drain(&b->q_full[i], 1, kLandNs);
             for (int i = 0; i < kStages; ++i) mbar_drain(&b->full[i], 0, kLandNs), mbar_drain(&b->full[i], 1, kLandNs);
             mbar_drain(&b->answered, 0, kLandNs), mbar_drain(&b->answered, 1, kLandNs);
             mbar_drain(&b->tail, 0, kLandNs), mbar_drain(&b->tail, 1, kLandNs);
         }
-        if ((warp == 9 || warp == 10) && ptx::elect_one()) {
-            umma::mma_commit(&b->quiet[warp - 9]);
-            mbar_drain(&b->quiet[warp - 9], 0, 1000000000ull);
+        if (warp >= Shape::kMultiplyWarp && warp < Shape::kWorkWarp && ptx::elect_one()) {
+            umma::mma_commit(&b->quiet[warp - Shape::kMultiplyWarp]);
+            mbar_drain(&b->quiet[warp - Shape::kMultiplyWarp], 0, 1000000000ull);
         }
         __syncthreads();
     }
-    if (warp == 9) umma::tmem_dealloc(tmem, 512);
+    if (warp == Shape::kMultiplyWarp) umma::tmem_dealloc(tmem, Shape::kColumns);
 }
 
 // ------------------------------------------------------------------------------------------------ backward
@@ -811,7 +814,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
     };
 
     if (warp >= 8) {
-        give_registers<kBwdRegisters>();
+        give_registers<3 * 168 - 2 * kBwdRegisters>();
         if (warp == 8) {
             AttnRing<kSlots> p;
             const bool one = ptx::elect_one();
@@ -1201,17 +1204,23 @@ cudaError_t allow_once(const void* fn, int bytes, std::atomic<uint64_t>& allowed
     return err;
 }
 
-template <int kChunks>
+template <int kChunks, int kTiles>
 cudaError_t launch_forward(const AttentionArgs& a, cudaStream_t stream) {
-    const void* fn = reinterpret_cast<const void*>(attention_kernel<kChunks>);
+    using Shape = FwdShape<kChunks, kTiles>;
+    const void* fn = reinterpret_cast<const void*>(attention_kernel<kChunks, kTiles>);
     static std::atomic<uint64_t> allowed{0};
-    const cudaError_t err = allow_once(fn, FwdShape<kChunks>::kSmem, allowed);
+    const cudaError_t err = allow_once(fn, Shape::kSmem, allowed);
     if (err != cudaSuccess) return err;
     CUtensorMap q, k, v;
     if (!make_map(&q, a.q, a.tq, a.heads, a.dim, 128) || !make_map(&k, a.k, a.tk, a.kv_heads, a.dim, 128) || !make_map(&v, a.v, a.tk, a.kv_heads, a.dim, 128))
         return cudaErrorInvalidValue;
     void* params[] = {&q, &k, &v, const_cast<AttentionArgs*>(&a)};
-    return launch_dependent(fn, dim3(static_cast<unsigned>(num_blocks<256>(a.tq, a.num_seqs) * a.heads)), dim3(kFwdThreads), params, FwdShape<kChunks>::kSmem, stream);
+    return launch_dependent(fn, dim3(static_cast<unsigned>(num_blocks<128 * kTiles>(a.tq, a.num_seqs) * a.heads)), dim3(Shape::kThreads), params, Shape::kSmem, stream);
+}
+constexpr int kShortKeys = 1024;
+template <int kChunks>
+cudaError_t launch_forward(const AttentionArgs& a, cudaStream_t stream) {
+    return a.tk / std::max(a.num_seqs, 1) <= kShortKeys ? launch_forward<kChunks, 1>(a, stream) : launch_forward<kChunks, 2>(a, stream);
 }
 template <int kChunks, bool kKeys>
 cudaError_t launch_gradient(const AttentionArgs& a, const CUtensorMap& q, const CUtensorMap& d, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t stream) {
