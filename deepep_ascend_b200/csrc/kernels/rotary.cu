@@ -7,7 +7,8 @@
 //     dw = sum over tokens and heads of g rstd x,     u = g w,     dx = rstd (u - rstd^2 x mean(u x))
 //
 // Bound by memory: every value is read once and written once.  A row of D channels lies on 8, 16 or 32 lanes of a warp, eight channels each: neighbours where pairs are neighbours,
-// else four and their partners, so that no lane asks another for them (eight neighbours, and their partners' values by shuffles: 66 instead of 63 us for 8192 x 64 heads of 128).  What 16-bit heads take beyond that is instruction issue, so values go in pairs.
+// else four and their partners, so that no lane asks another for them (eight neighbours, and their partners' values by shuffles: 3 us more for 8192 x 64 heads of 128).  What 16-bit heads take beyond that is instruction issue,
+// so values go in pairs and 1/sqrt is CUDA's of 2 ulp (the one that rounds to nearest: 59 instead of 54 us).
 #include <algorithm>
 #include <type_traits>
 
@@ -19,8 +20,8 @@ namespace {
 
 using bf16 = __nv_bfloat16;
 constexpr int kRotaryThreads = 256;
-// Rows of a lane group that a warp has at once, and CTAs of an SM: what is on its way at a time.  8192 x 64 heads of 128, bf16: 59 us (two rows: 67, eight on three CTAs: 66); gradients 94 (two
-// rows: 101, three CTAs 109), where four rows of 32-bit values do not fit the registers (4096 x 40 heads: 86 us instead of 48).
+// Rows of a lane group that a warp has at once, and CTAs of an SM: what is on its way at a time.  8192 x 64 heads of 128, bf16: 54 us (three CTAs: 62; two rows: 8 us more, eight
+// on three CTAs: 7 more, two times four behind one another: 10 more, by the registers that they take from the loads); gradients 91 (two rows: 7 more, three CTAs: 15 more), where four rows of 32-bit values do not fit the registers (4096 x 40 heads: 86 us instead of 48).
 constexpr int kForwardIters = 4, kForwardCtas = 4, kBackwardCtas = 2;
 __host__ __device__ constexpr int backward_iters(int value_bytes) { return value_bytes == 2 ? 4 : 2; }
 
@@ -254,7 +255,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kForwardCtas) rotary_kernel(co
         to_float(raw[i], v);
 #pragma unroll
         for (int j = 0; j < 4; ++j) squares = fma2(v[j], v[j], squares);
-        const float rstd = __frsqrt_rn(sum_row<kLanes>(both(squares)) * inv_dim + a.eps);
+        const float rstd = rsqrtf(sum_row<kLanes>(both(squares)) * inv_dim + a.eps);
         const uint64_t rstd2 = pair(rstd, rstd);
         uint64_t y[4];
 #pragma unroll
@@ -337,7 +338,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kBackwardCtas) rotary_backward
                     along = fma2(mul2(g[j], w[j]), v[j], along);
                 }
                 const float mean = sum_row<kLanes>(both(squares)) * inv_dim, with = sum_row<kLanes>(both(along)) * inv_dim;
-                const float rstd = __frsqrt_rn(mean + a.eps), back = -rstd * rstd * rstd * with;
+                const float rstd = rsqrtf(mean + a.eps), back = -rstd * rstd * rstd * with;
                 const bool there = head0 + i * Lane::kRows < heads;
                 const uint64_t rstd2 = pair(rstd, rstd), back2 = pair(back, back);
                 uint64_t dx[4];
