@@ -79,7 +79,7 @@ struct AttnRing {
 };
 
 // ------------------------------------------------------------------------------------------------ work
-// Blocks of kRows rows of the sequences are numbered without a count of them: sequence i has the numbers from cu[i] / kRows + i on, up to one more than it needs.
+// Blocks of `rows` rows of the sequences are numbered without a count of them: sequence i has the numbers from cu[i] / rows + i on, up to one more than it needs.
 struct AttnBlock {
     int seq, row0, rows;             // first row of the block inside its sequence, rows of the sequence (row0 >= rows: no block has this number)
     int start;                       // first row of the sequence
@@ -89,23 +89,21 @@ __device__ __forceinline__ int2 sequence_rows(const int32_t* cu, int i, int tota
     const int a = min(max(cu[i], 0), total), b = min(max(cu[i + 1], a), total);
     return make_int2(a, b - a);
 }
-template <int kRows>
-__device__ __forceinline__ AttnBlock find_block(const int32_t* cu, int num_seqs, int total, int number) {
+__device__ __forceinline__ AttnBlock find_block(const int32_t* cu, int num_seqs, int total, int number, int rows) {
     int lo = 0;
     if (cu != nullptr) {
-        int hi = num_seqs;                                        // the last i in [lo, hi) with cu[i] / kRows + i <= number
+        int hi = num_seqs;                                        // the last i in [lo, hi) with cu[i] / rows + i <= number
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
-            if (min(max(cu[mid], 0), total) / kRows + mid <= number) lo = mid;
+            if (min(max(cu[mid], 0), total) / rows + mid <= number) lo = mid;
             else hi = mid;
         }
     }
     const int2 s = sequence_rows(cu, lo, total);
-    const int at = number - s.x / kRows - lo;                     // (below zero: in front of the first sequence)
-    return AttnBlock{lo, at < 0 ? s.y : at * kRows, s.y, s.x};
+    const int at = number - s.x / rows - lo;                     // (below zero: in front of the first sequence)
+    return AttnBlock{lo, at < 0 ? s.y : at * rows, s.y, s.x};
 }
-template <int kRows>
-int64_t num_blocks(int64_t total, int64_t num_seqs) { return total / kRows + num_seqs; }
+int64_t num_blocks(int64_t total, int64_t num_seqs, int rows) { return total / rows + num_seqs; }
 
 // kThreads threads: rows that belong to no sequence get zeros (and -inf), one of `parts` of them
 template <int kThreads>
@@ -287,6 +285,9 @@ __device__ __forceinline__ void store_part(uint32_t tmem, float factor, float* r
 // the products and as much for the barriers between, which lie in the shared memory that the products read at its full rate.  So a quarter of the powers by polynomial, the first half of
 // the probabilities handed over early and an issuing thread for each tile took it from 3650 clocks to 3030.
 // Short sequences have one tile per CTA and two CTAs on an SM, one of which works while the other begins or ends a block; two tiles read keys and values from L2 once for both.
+// That tile takes the heads of a group together, each of as many queries as fill 128 rows (7 heads: 18), so that few rows stay empty where a sequence ends: 31 prompts of 264 tokens
+// 125 -> 90 us, 200 of 30 tokens (32 heads) 97 -> 46, 8 of 1000 152 either way.
+constexpr int kPackedHeads = 16;
 template <int kChunks, int kTiles>
 struct FwdShape {
     // four warps per tile for its softmax; one that requests tiles, one per tile that issues products, one that looks for work, and to make up four more one without any
@@ -336,6 +337,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                  const __grid_constant__ AttentionArgs a) {
     using Shape = FwdShape<kChunks, kTiles>;
     constexpr int kStages = Shape::kStages, kTileBytes = Shape::kTileBytes;
+    const int pack = kTiles == 1 ? a.pack : 1, tokens = 128 / pack;      // heads and tokens of a tile
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *sq = smem, *skv = smem + kTiles * kTileBytes;
     FwdBars* b = reinterpret_cast<FwdBars*>(smem + (kTiles + kStages) * kTileBytes);
@@ -369,6 +371,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         umma::tmem_alloc(&b->st.tmem_base, Shape::kColumns);
         umma::tmem_relinquish();
     }
+    if (kTiles == 1 && warp == Shape::kLoadWarp) clear_tile<128, kChunks>(sq, tokens * pack);      // (rows that no query has)
     umma::fence_before_thread_sync();
     __syncthreads();
     umma::fence_after_thread_sync();
@@ -418,7 +421,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                             if (!attn_wait_warp(&b->q_empty[t], (queries[t] & 1) ^ 1, failed, a.report, 1)) return;
                             ++queries[t];
                             if (one) {
-                                ptx::mbar_arrive_expect_tx(&b->q_full[t], kTileBytes);
+                                ptx::mbar_arrive_expect_tx(&b->q_full[t], kTiles == 1 ? tokens * pack * 128 * kChunks : kTileBytes);
                                 load_tile<128, kChunks>(sq + t * kTileBytes, &map_q, w.head[t], w.start + w.row0[t], &b->q_full[t]);
                             }
                             __syncwarp();
@@ -490,7 +493,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
             }
         } else if (warp == Shape::kWorkWarp) {
             // looks for work: first this CTA's own
-            const int blocks = gridDim.x / a.heads;
+            const int units = a.heads / pack, blocks = gridDim.x / units;
             int item = blockIdx.x;
             uint32_t handed = 0;
             bool something = true;
@@ -498,9 +501,9 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 FwdWork w{};
                 w.rows = -1;
                 if (item >= 0) {
-                    // 256 rows of a group's heads are as many pairs of tiles as the group has heads (128 rows: as many tiles).  Long blocks first: those at the ends of the sequences
-                    const int number = item / a.heads, unit = item - number * a.heads, group = a.heads / a.kv_heads;
-                    const AttnBlock blk = find_block<128 * kTiles>(a.cu_q, a.num_seqs, a.tq, blocks - 1 - number);
+                    // two tiles: 256 rows of a group's heads are as many pairs of tiles as the group has heads.  Long blocks first: those at the ends of the sequences
+                    const int number = item / units, unit = item - number * units, group = a.heads / a.kv_heads / pack;
+                    const AttnBlock blk = find_block(a.cu_q, a.num_seqs, a.tq, blocks - 1 - number, kTiles * tokens);
                     const int2 keys = sequence_rows(a.cu_k, blk.seq, a.tk);
                     clear_rows<32>(a.cu_q, a.num_seqs, a.tq, item, gridDim.x, reinterpret_cast<bf16*>(a.o), static_cast<int64_t>(a.heads) * a.dim, a.lse, a.heads);
                     w.start = blk.start;
@@ -514,8 +517,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     for (int t = 0; t < kTiles; ++t) {
                         const bool upper = tile + t >= group;
                         w.row0[t] = blk.row0 + (upper ? 128 : 0);
-                        w.head[t] = w.kv_head * group + tile + t - (upper ? group : 0);
-                        const int last = min(w.row0[t] + 128, blk.rows) - 1, seen = a.causal ? min(last + keys.y - blk.rows + 1, keys.y) : keys.y;
+                        w.head[t] = (w.kv_head * group + tile + t - (upper ? group : 0)) * pack;
+                        const int last = min(w.row0[t] + tokens, blk.rows) - 1, seen = a.causal ? min(last + keys.y - blk.rows + 1, keys.y) : keys.y;
                         w.n[t] = w.row0[t] >= blk.rows || seen <= 0 ? 0 : (seen + 127) / 128;
                         something |= w.row0[t] < blk.rows;
                     }
@@ -542,10 +545,11 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16), ts = lanes + t * 128, to = lanes + Shape::kOut + t * 128;
         const float c = a.scale * kLog2e;
         uint32_t made = 0, ended = 0;                 // blocks of scores, of results so far
+        const int token_of = lane_row / pack, head_of = lane_row - token_of * pack;
         FwdWork w;
         bool ok = true;
         for (int k = 0; ok && next_work(k, w); ++k) {
-            const int row0 = t == 0 ? w.row0[0] : w.row0[1], head = t == 0 ? w.head[0] : w.head[1], row = row0 + lane_row, shift = w.keys - w.rows;
+            const int row0 = t == 0 ? w.row0[0] : w.row0[1], head = (t == 0 ? w.head[0] : w.head[1]) + head_of, row = row0 + token_of, shift = w.keys - w.rows;
             const int seen = a.causal ? min(row + shift + 1, w.keys) : w.keys;      // keys that this row sees
             const int first_seen = a.causal ? min(row0 + shift + 1, w.keys) : w.keys;      // ... and the tile's first row
             const int n = t == 0 ? w.n[0] : w.n[1];
@@ -655,7 +659,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                 umma::unpack_f32x2(add2(part[0], part[1]), u, v);
                 sum = u + v;
             }
-            const bool in = row < w.rows;
+            const bool in = row < w.rows && token_of < tokens;
             const int64_t token = w.start + row;
             bf16* out = reinterpret_cast<bf16*>(a.o) + (token * a.heads + head) * a.dim;
             if (n > 0) {
@@ -947,7 +951,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                     w.first_head = kKeys ? w.head * group + group * w.split / a.splits : 0;
                     const int num_heads = kKeys ? w.head * group + group * (w.split + 1) / a.splits - w.first_head : 1;
                     const AttnBlock blk =
-                        find_block<128>(kKeys ? a.cu_k : a.cu_q, a.num_seqs, kKeys ? a.tk : a.tq, kKeys ? number : static_cast<int>(gridDim.x / units) - 1 - number);
+                        find_block(kKeys ? a.cu_k : a.cu_q, a.num_seqs, kKeys ? a.tk : a.tq, kKeys ? number : static_cast<int>(gridDim.x / units) - 1 - number, 128);
                     const int2 other = sequence_rows(kKeys ? a.cu_q : a.cu_k, blk.seq, kKeys ? a.tq : a.tk);
                     const int shift = kKeys ? blk.rows - other.y : other.y - blk.rows;
                     w.start = blk.start;
@@ -1179,14 +1183,14 @@ __global__ void __launch_bounds__(kAddThreads) attention_add_kernel(const __grid
 }
 
 // ------------------------------------------------------------------------------------------------ host
-bool make_map(CUtensorMap* map, const HeadsView& x, int64_t tokens, int64_t heads, int64_t dim, int box_rows) {
+bool make_map(CUtensorMap* map, const HeadsView& x, int64_t tokens, int64_t heads, int64_t dim, int box_rows, int box_heads = 1) {
     EncodeTiledFn encode = get_encode_fn();
     if (encode == nullptr) return false;
     // (a stride that nothing steps along may be anything)
     const int64_t pitch = (dim * 2 + 15) / 16 * 16;
     const cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(tokens)};
     const cuuint64_t strides[2] = {static_cast<cuuint64_t>(heads > 1 ? x.stride_head * 2 : pitch), static_cast<cuuint64_t>(tokens > 1 ? x.stride_token * 2 : pitch)};
-    const cuuint32_t box[3] = {64, 1, static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_rows)};
     const cuuint32_t steps[3] = {1, 1, 1};
     auto made = [&]() {
         return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(x.data), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -1211,17 +1215,21 @@ cudaError_t allow_once(const void* fn, int bytes, std::atomic<uint64_t>& allowed
 }
 
 template <int kChunks, int kTiles>
-cudaError_t launch_forward(const AttentionArgs& a, cudaStream_t stream) {
+cudaError_t launch_forward(AttentionArgs a, cudaStream_t stream) {
     using Shape = FwdShape<kChunks, kTiles>;
     const void* fn = reinterpret_cast<const void*>(attention_kernel<kChunks, kTiles>);
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t err = allow_once(fn, Shape::kSmem, allowed);
     if (err != cudaSuccess) return err;
+    // Heads that a single tile takes of as many tokens as fill it: all of a group, or as many as divide it
+    a.pack = kTiles == 1 ? std::min(a.heads / a.kv_heads, kPackedHeads) : 1;
+    while (a.heads / a.kv_heads % a.pack != 0) --a.pack;
+    const int tokens = 128 / a.pack;
     CUtensorMap q, k, v;
-    if (!make_map(&q, a.q, a.tq, a.heads, a.dim, 128) || !make_map(&k, a.k, a.tk, a.kv_heads, a.dim, 128) || !make_map(&v, a.v, a.tk, a.kv_heads, a.dim, 128))
+    if (!make_map(&q, a.q, a.tq, a.heads, a.dim, tokens, a.pack) || !make_map(&k, a.k, a.tk, a.kv_heads, a.dim, 128) || !make_map(&v, a.v, a.tk, a.kv_heads, a.dim, 128))
         return cudaErrorInvalidValue;
-    void* params[] = {&q, &k, &v, const_cast<AttentionArgs*>(&a)};
-    return launch_dependent(fn, dim3(static_cast<unsigned>(num_blocks<128 * kTiles>(a.tq, a.num_seqs) * a.heads)), dim3(Shape::kThreads), params, Shape::kSmem, stream);
+    void* params[] = {&q, &k, &v, &a};
+    return launch_dependent(fn, dim3(static_cast<unsigned>(num_blocks(a.tq, a.num_seqs, kTiles * tokens) * (a.heads / a.pack))), dim3(Shape::kThreads), params, Shape::kSmem, stream);
 }
 constexpr int kShortKeys = 1024;
 template <int kChunks>
@@ -1237,7 +1245,7 @@ cudaError_t launch_gradient(const AttentionArgs& a, const CUtensorMap& q, const 
     const CUtensorMap* maps[4] = {kKeys ? &k : &q, kKeys ? &v : &d, kKeys ? &q : &k, kKeys ? &d : &v};
     void* params[] = {const_cast<CUtensorMap*>(maps[0]), const_cast<CUtensorMap*>(maps[1]), const_cast<CUtensorMap*>(maps[2]), const_cast<CUtensorMap*>(maps[3]),
                       const_cast<AttentionArgs*>(&a)};
-    const int64_t ctas = num_blocks<128>(kKeys ? a.tk : a.tq, a.num_seqs) * (kKeys ? a.kv_heads * a.splits : a.heads);
+    const int64_t ctas = num_blocks(kKeys ? a.tk : a.tq, a.num_seqs, 128) * (kKeys ? a.kv_heads * a.splits : a.heads);
     return launch_dependent(fn, dim3(static_cast<unsigned>(ctas)), dim3(kBwdThreads), params, BwdShape<kChunks, kKeys>::kSmem, stream);
 }
 template <int kChunks>

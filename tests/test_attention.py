@@ -98,6 +98,15 @@ def test_against_the_formulas(lq, lk, H, Hk, D, causal, device):
     _check(*_make(sum(lq), sum(lk), H, Hk, D, sum(lk) + D, device), lq, lk, causal)
 
 
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('causal', [True, False])
+@pytest.mark.parametrize('group', [5, 11, 12, 17, 26, 48])
+def test_groups_of_heads(group, causal, device):
+    """Numbers of heads that do not divide 128, or have no divisor that a tile could take; sequences that end inside a tile."""
+    lq, lk = [1, 30, 23, 131], [1, 30, 140, 131]
+    _check(*_make(sum(lq), sum(lk), 2 * group, 2, 32, group, device), lq, lk, causal)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('lq,lk,H,Hk,D,causal', [([1100], [1100], 2, 1, 128, True), ([513, 700], [1900, 700], 4, 2, 64, True), ([640], [1333], 2, 2, 128, False)])
 def test_longer_sequences(lq, lk, H, Hk, D, causal):
