@@ -278,7 +278,7 @@ __device__ __forceinline__ void store_part(uint32_t tmem, float factor, float* r
 //
 // A CTA goes on with the work of CTAs that have not started (it cancels their launch and takes their place): barriers and tensor memory are set up once, and the next block's
 // queries, keys and values come while the last one's results leave.  Blocks differ in length, so who takes which is decided as they end.  (31 prompts of 264 tokens, 56 heads of 128: 268 us with
-// a CTA for every block, 150 so.)
+// a CTA for every block, 150 so at the time.)
 //
 // Long sequences are bound by power: 16384 tokens, 56 heads of 128, 3.0 to 3.4 ms, 1.1 to 1.3 PFLOP/s at SM clocks of 1.4 to 1.55 GHz, the tensor pipe busy in 67 % of them.  What the clocks go by is the
 // chain of a tile's block of 128 keys, some 3000 of which two tiles share: 70 for the scores into registers, 370 for their largest, 1050 for the powers, 100 for their way back, 512 + 512 for
@@ -730,7 +730,8 @@ __global__ void __launch_bounds__(kDeltaThreads) attention_delta_kernel(const __
 // costs two products of seven, and spares sums of dQ in memory by many CTAs in any order.
 //
 // 16384 tokens, 56 heads of 128: 11.5 ms, 0.84 PFLOP/s counted as five products and 1.17 as seven, bound by power as the forward pass; two documents of 4096: 1.4 to 1.6 ms.  Short sequences are bound
-// by the chain of a piece, some 2200 clocks, and by what a block takes to begin and to end.
+// by the chain of a piece, some 2200 clocks, and by what a block takes to begin and to end.  There, too, tiles of queries take heads of a group together (31 x 264 tokens, 56 heads: 385 -> 280 us,
+// 200 x 30, 32 heads: 324 -> 155).
 //
 // Two groups of four warps have 64 columns of a piece each.  P and dS take the place of dP; that of the scores is free as soon as they are in registers, so the next piece's
 // scores are made meanwhile, and their powers while dV, dK and the next dP are.  (Pieces of 64 columns with two places for each had products of half the width, which take as long
@@ -748,8 +749,11 @@ struct BwdShape {
 struct BwdWork {
     int start, row0, rows;           // as of AttnBlock; rows < 0: no more work
     int other0, others;              // rows of the other side
-    int head, first_head, split;     // kept head, first head of the pieces
-    int piece0, per_head, n;         // pieces [piece0, piece0 + per_head) of every head, pieces in all
+    int head, first_head, split;     // (first) kept head, first head of the pieces
+    int piece0, per_head, first, n;  // pieces [piece0, piece0 + per_head) of every head (or of `pack` at once); of all of them n from `first` on
+    // the head and the piece of the i-th
+    __device__ __forceinline__ int head_of(int i, int pack) const { return first_head + (first + i) / per_head * pack; }
+    __device__ __forceinline__ int piece_of(int i) const { return piece0 + (first + i) % per_head; }
 };
 // (dP and what is made of it in turn by pieces: with two places for dP, the next one's can be there before a slow warp has looked for this one's)
 struct BwdBars {
@@ -770,6 +774,8 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
     float* stats = reinterpret_cast<float*>(pieces + kSlots * kTileBytes);
     BwdBars* b = reinterpret_cast<BwdBars*>(pieces + kSlots * kTileBytes + Shape::kStatBytes);
     const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads;
+    // queries lie in tiles of `tokens` times `pack` heads, keys in tiles of 128
+    const int pack = a.pack, tokens = 128 / pack, step = kKeys ? tokens : 128;
     if (threadIdx.x == 0) {
         umma::prefetch_tensormap(&map_kept0);
         umma::prefetch_tensormap(&map_kept1);
@@ -803,6 +809,9 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
         umma::tmem_alloc(&b->st.tmem_base, 512);
         umma::tmem_relinquish();
     }
+    if (warp == 8) {                                     // (rows that no query has)
+        for (int i = kKeys ? 2 : 0; i < (kKeys ? 2 + kSlots : 2); ++i) clear_tile<128, kChunks>(smem + i * kTileBytes, tokens * pack);
+    }
     umma::fence_before_thread_sync();
     __syncthreads();
     umma::fence_after_thread_sync();
@@ -833,17 +842,17 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
             auto request = [&](const CUtensorMap* map, int h, int piece) {
                 if (!attn_wait_warp(&b->empty[p.stage], p.phase ^ 1, failed, a.report, 1)) return false;
                 uint8_t* tile = pieces + p.stage * kTileBytes;
-                const bool tail = piece * 128 + 128 > w.others;
+                const bool tail = piece * step + step > w.others;
                 uint64_t* bar = tail ? &b->tail : &b->full[p.stage];
                 if (one) {
-                    ptx::mbar_arrive_expect_tx(bar, kTileBytes);
-                    load_tile<128, kChunks>(tile, map, h, w.other0 + piece * 128, bar);
+                    ptx::mbar_arrive_expect_tx(bar, kKeys ? tokens * pack * 128 * kChunks : kTileBytes);
+                    load_tile<128, kChunks>(tile, map, h, w.other0 + piece * step, bar);
                 }
                 __syncwarp();
                 if (tail) {
                     if (!attn_wait_warp(&b->tail, tails & 1, failed, a.report, 4)) return false;
                     ++tails;
-                    clear_tile<128, kChunks>(tile, w.others - piece * 128);
+                    clear_tile<128, kChunks>(tile, (w.others - piece * step) * (kKeys ? pack : 1));
                     if (one) ptx::mbar_arrive(&b->full[p.stage]);
                 }
                 p.advance();
@@ -855,13 +864,13 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                     if (!attn_wait_warp(&b->kept_empty, (blocks & 1) ^ 1, failed, a.report, 1)) return;
                     ++blocks;
                     if (one) {
-                        ptx::mbar_arrive_expect_tx(&b->kept, 2 * kTileBytes);
+                        ptx::mbar_arrive_expect_tx(&b->kept, 2 * (kKeys ? kTileBytes : tokens * pack * 128 * kChunks));
                         load_tile<128, kChunks>(kept, &map_kept0, w.head, w.start + w.row0, &b->kept);
                         load_tile<128, kChunks>(kept + kTileBytes, &map_kept1, w.head, w.start + w.row0, &b->kept);
                     }
                     __syncwarp();
                     for (int i = 0; i < w.n; ++i) {
-                        const int h = kKeys ? w.first_head + i / w.per_head : w.head / group, piece = w.piece0 + i % w.per_head;
+                        const int h = kKeys ? w.head_of(i, pack) : w.head / group, piece = w.piece_of(i);
                         if (!request(&map_piece0, h, piece) || !request(&map_piece1, h, piece)) return;
                     }
                 }
@@ -936,7 +945,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
             }
         } else if (warp == 10) {
             // looks for work: first this CTA's own
-            const int units = kKeys ? a.kv_heads * a.splits : a.heads;
+            const int units = kKeys ? a.kv_heads * a.splits : a.heads / pack;
             int item = blockIdx.x;
             uint32_t handed = 0;
             for (uint32_t answers = 0;; ++answers) {
@@ -946,12 +955,11 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                 if (item >= 0) {
                     // (kKeys: the first keys are seen by most queries; otherwise the last queries see most keys.  Long blocks first.)
                     const int unit = item % units, number = item / units;
-                    w.head = kKeys ? unit / a.splits : unit;      // (of keys, or of queries)
+                    w.head = kKeys ? unit / a.splits : unit * pack;      // (of keys, or of queries)
                     w.split = kKeys ? unit % a.splits : 0;
-                    w.first_head = kKeys ? w.head * group + group * w.split / a.splits : 0;
-                    const int num_heads = kKeys ? w.head * group + group * (w.split + 1) / a.splits - w.first_head : 1;
+                    w.first_head = kKeys ? w.head * group : 0;
                     const AttnBlock blk =
-                        find_block(kKeys ? a.cu_k : a.cu_q, a.num_seqs, kKeys ? a.tk : a.tq, kKeys ? number : static_cast<int>(gridDim.x / units) - 1 - number, 128);
+                        find_block(kKeys ? a.cu_k : a.cu_q, a.num_seqs, kKeys ? a.tk : a.tq, kKeys ? number : static_cast<int>(gridDim.x / units) - 1 - number, kKeys ? 128 : tokens);
                     const int2 other = sequence_rows(kKeys ? a.cu_q : a.cu_k, blk.seq, kKeys ? a.tq : a.tk);
                     const int shift = kKeys ? blk.rows - other.y : other.y - blk.rows;
                     w.start = blk.start;
@@ -960,15 +968,18 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                     w.other0 = other.x;
                     w.others = other.y;
                     something = blk.row0 < blk.rows;
-                    int piece1 = (other.y + 127) / 128;
+                    int piece1 = (other.y + step - 1) / step;
                     if (kKeys) {
-                        w.piece0 = a.causal ? max(blk.row0 - shift, 0) / 128 : 0;
+                        w.piece0 = a.causal ? max(blk.row0 - shift, 0) / step : 0;
                     } else if (a.causal) {
-                        const int seen = min(min(blk.row0 + 128, blk.rows) + shift, other.y);
+                        const int seen = min(min(blk.row0 + tokens, blk.rows) + shift, other.y);
                         piece1 = seen <= 0 ? 0 : (seen + 127) / 128;
                     }
                     w.per_head = max(piece1 - w.piece0, 0);
-                    w.n = w.per_head * num_heads;
+                    // (a part of the group's pieces, of all heads)
+                    const int64_t all = static_cast<int64_t>(w.per_head) * (kKeys ? group / pack : 1);
+                    w.first = static_cast<int>(kKeys ? all * w.split / a.splits : 0);
+                    w.n = static_cast<int>((kKeys ? all * (w.split + 1) / a.splits : all) - w.first);
                     const int64_t row_values = static_cast<int64_t>(kKeys ? a.kv_heads : a.heads) * a.dim;
                     if (!kKeys) {
                         clear_rows<32>(a.cu_q, a.num_seqs, a.tq, item, gridDim.x, reinterpret_cast<bf16*>(a.dq), row_values, nullptr, 0);
@@ -998,13 +1009,15 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
         const float c = a.scale * kLog2e;
         float* mine = stats + half * 256;             // twice: 64 times -lse log2 e, 64 times -delta
         const uint64_t c2 = f32x2(c, c);
+        const int column = kKeys ? half * 64 + (lane_row & 63) : lane_row, token_of = column / pack, head_of = column - token_of * pack;      // of what this thread reads statistics of
         uint32_t made = 0, ended = 0;                 // pieces, blocks so far
         bool ok = true;
         BwdWork w;
         for (int k = 0; ok && next_work(k, w); ++k) {
-            const int row = w.row0 + lane_row, shift = kKeys ? w.rows - w.others : w.others - w.rows;     // query i sees the keys up to i + shift
-            const bool in = row < w.rows;
+            const int row = w.row0 + (kKeys ? lane_row : token_of), shift = kKeys ? w.rows - w.others : w.others - w.rows;     // query i sees the keys up to i + shift
+            const bool in = row < w.rows && (kKeys || token_of < tokens);
             const int64_t token = w.start + row;
+            const int head = w.head + (kKeys ? 0 : head_of);
             // a statistic of a query that sees nothing, or that is none: its probabilities are zero
             auto statistic = [&](bool is_delta, bool is_there, int h, int64_t query) {
                 if (!is_there) return is_delta ? 0.f : kNone;
@@ -1015,15 +1028,15 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
             };
             auto next_statistic = [&](int i) {
                 if (i >= w.n) return 0.f;
-                const int at = (w.piece0 + i % w.per_head) * 128 + half * 64 + (lane_row & 63);
-                return statistic(lane_row >= 64, at < w.others, w.first_head + i / w.per_head, w.other0 + at);
+                const int at = w.piece_of(i) * tokens + token_of;
+                return statistic(lane_row >= 64, token_of < tokens && at < w.others, w.head_of(i, pack) + head_of, w.other0 + at);
             };
             float coming = 0.f;
             uint64_t minus2 = 0, delta2 = 0;
             if (kKeys) {
                 coming = next_statistic(0);
             } else if (w.n > 0) {
-                const float m = statistic(false, in, w.head, token), d = statistic(true, in, w.head, token);
+                const float m = statistic(false, in, head, token), d = statistic(true, in, head, token);
                 minus2 = f32x2(m, m);
                 delta2 = f32x2(d, d);
             }
@@ -1047,13 +1060,13 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                 umma::fence_before_thread_sync();
                 __syncwarp();
                 if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->s_read);
-                const int first = (w.piece0 + i % w.per_head) * 128 + half * 64;
+                const int first = w.piece_of(i) * step;
                 // columns [low, high) are visible
                 int low = 0, high = 64;
                 if (kKeys) {
-                    if (a.causal) low = row - shift - first;
+                    if (a.causal) low = min(max(row - shift - first, 0), tokens) * pack - half * 64;
                 } else {
-                    high = (a.causal ? min(row + shift + 1, w.others) : w.others) - first;
+                    high = (a.causal ? min(row + shift + 1, w.others) : w.others) - first - half * 64;
                 }
                 const bool masked = __any_sync(0xffffffffu, low > 0 || high < 64);
 #pragma unroll
@@ -1109,7 +1122,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                 __syncwarp();
                 if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->p_full[half][made & 1]);
             }
-            const int64_t at = (token * (kKeys ? a.kv_heads : a.heads) + w.head) * a.dim;
+            const int64_t at = (token * (kKeys ? a.kv_heads : a.heads) + head) * a.dim;
             const float factor = kKeys && half == 1 ? 1.f : a.scale;
             bf16* out = reinterpret_cast<bf16*>(kKeys ? (half == 0 ? a.dk : a.dv) : a.dq) + at;
             float* part = nullptr;
@@ -1214,6 +1227,17 @@ cudaError_t allow_once(const void* fn, int bytes, std::atomic<uint64_t>& allowed
     return err;
 }
 
+// Sequences of so many keys or fewer on average are short: tiles of queries take heads together, and the forward pass one tile per CTA.  56 heads of 128: forward 8 x 1000 tokens 152 us either way,
+// 4 x 2048 with single tiles 5 % more; gradients of 16 x 450 285 instead of 320 us, 9 x 830 407 instead of 424, 8 x 1000 471 instead of 474 (32 heads, 8 x 1024: 292 instead of 285).
+constexpr int kShortKeys = 1024;
+bool short_sequences(const AttentionArgs& a) { return a.tk / std::max(a.num_seqs, 1) <= kShortKeys; }
+// Heads that a tile takes of as many tokens as fill it: all of a group, or as many as divide it
+int packed_heads(const AttentionArgs& a) {
+    const int group = a.heads / a.kv_heads;
+    int pack = std::min(group, kPackedHeads);
+    while (group % pack != 0) --pack;
+    return pack;
+}
 template <int kChunks, int kTiles>
 cudaError_t launch_forward(AttentionArgs a, cudaStream_t stream) {
     using Shape = FwdShape<kChunks, kTiles>;
@@ -1221,9 +1245,7 @@ cudaError_t launch_forward(AttentionArgs a, cudaStream_t stream) {
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t err = allow_once(fn, Shape::kSmem, allowed);
     if (err != cudaSuccess) return err;
-    // Heads that a single tile takes of as many tokens as fill it: all of a group, or as many as divide it
-    a.pack = kTiles == 1 ? std::min(a.heads / a.kv_heads, kPackedHeads) : 1;
-    while (a.heads / a.kv_heads % a.pack != 0) --a.pack;
+    a.pack = kTiles == 1 ? packed_heads(a) : 1;
     const int tokens = 128 / a.pack;
     CUtensorMap q, k, v;
     if (!make_map(&q, a.q, a.tq, a.heads, a.dim, tokens, a.pack) || !make_map(&k, a.k, a.tk, a.kv_heads, a.dim, 128) || !make_map(&v, a.v, a.tk, a.kv_heads, a.dim, 128))
@@ -1231,10 +1253,9 @@ cudaError_t launch_forward(AttentionArgs a, cudaStream_t stream) {
     void* params[] = {&q, &k, &v, &a};
     return launch_dependent(fn, dim3(static_cast<unsigned>(num_blocks(a.tq, a.num_seqs, kTiles * tokens) * (a.heads / a.pack))), dim3(Shape::kThreads), params, Shape::kSmem, stream);
 }
-constexpr int kShortKeys = 1024;
 template <int kChunks>
 cudaError_t launch_forward(const AttentionArgs& a, cudaStream_t stream) {
-    return a.tk / std::max(a.num_seqs, 1) <= kShortKeys ? launch_forward<kChunks, 1>(a, stream) : launch_forward<kChunks, 2>(a, stream);
+    return short_sequences(a) ? launch_forward<kChunks, 1>(a, stream) : launch_forward<kChunks, 2>(a, stream);
 }
 template <int kChunks, bool kKeys>
 cudaError_t launch_gradient(const AttentionArgs& a, const CUtensorMap& q, const CUtensorMap& d, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t stream) {
@@ -1245,16 +1266,17 @@ cudaError_t launch_gradient(const AttentionArgs& a, const CUtensorMap& q, const 
     const CUtensorMap* maps[4] = {kKeys ? &k : &q, kKeys ? &v : &d, kKeys ? &q : &k, kKeys ? &d : &v};
     void* params[] = {const_cast<CUtensorMap*>(maps[0]), const_cast<CUtensorMap*>(maps[1]), const_cast<CUtensorMap*>(maps[2]), const_cast<CUtensorMap*>(maps[3]),
                       const_cast<AttentionArgs*>(&a)};
-    const int64_t ctas = num_blocks(kKeys ? a.tk : a.tq, a.num_seqs, 128) * (kKeys ? a.kv_heads * a.splits : a.heads);
+    const int64_t ctas = kKeys ? num_blocks(a.tk, a.num_seqs, 128) * a.kv_heads * a.splits : num_blocks(a.tq, a.num_seqs, 128 / a.pack) * (a.heads / a.pack);
     return launch_dependent(fn, dim3(static_cast<unsigned>(ctas)), dim3(kBwdThreads), params, BwdShape<kChunks, kKeys>::kSmem, stream);
 }
 template <int kChunks>
-cudaError_t launch_backward(const AttentionArgs& a, cudaStream_t stream) {
+cudaError_t launch_backward(AttentionArgs a, cudaStream_t stream) {
     CUtensorMap q, k, v, d;
-    if (!make_map(&q, a.q, a.tq, a.heads, a.dim, 128) || !make_map(&d, a.d_o, a.tq, a.heads, a.dim, 128) || !make_map(&k, a.k, a.tk, a.kv_heads, a.dim, 128) ||
+    a.pack = short_sequences(a) ? packed_heads(a) : 1;
+    if (!make_map(&q, a.q, a.tq, a.heads, a.dim, 128 / a.pack, a.pack) || !make_map(&d, a.d_o, a.tq, a.heads, a.dim, 128 / a.pack, a.pack) || !make_map(&k, a.k, a.tk, a.kv_heads, a.dim, 128) ||
         !make_map(&v, a.v, a.tk, a.kv_heads, a.dim, 128))
         return cudaErrorInvalidValue;
-    void* params[] = {const_cast<AttentionArgs*>(&a)};
+    void* params[] = {&a};
     const int64_t rows = static_cast<int64_t>(a.tq) * a.heads;
     cudaError_t err = launch_dependent(reinterpret_cast<const void*>(attention_delta_kernel), dim3(static_cast<unsigned>((rows * 16 + kDeltaThreads - 1) / kDeltaThreads)),
                                        dim3(kDeltaThreads), params, 0, stream);
