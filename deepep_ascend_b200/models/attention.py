@@ -29,8 +29,10 @@ def positions_of(cu_seqlens: Optional[torch.Tensor], num_tokens: int, device=Non
 def slots_of(page_table: torch.Tensor, positions: torch.Tensor, page_size: int) -> torch.Tensor:
     """int64 slots (as of :func:`ops.rotary.qk_norm_rope_append`) of one position per row of ``page_table``; -1 for a negative one, or one that the row has no page for."""
     page = torch.div(positions, page_size, rounding_mode='floor').long()
+    if page_table.shape[1] == 0:
+        return torch.full_like(page, -1)
     there = (positions >= 0) & (page < page_table.shape[1])
-    entry = page_table.gather(1, page.clamp(0, max(page_table.shape[1] - 1, 0)).unsqueeze(1)).squeeze(1).long()
+    entry = page_table.gather(1, page.clamp(0, page_table.shape[1] - 1).unsqueeze(1)).squeeze(1).long()
     return torch.where(there & (entry >= 0), entry * page_size + positions % page_size, -1)
 
 

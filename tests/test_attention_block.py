@@ -23,6 +23,11 @@ def test_slots():
     assert slots_of(table, torch.tensor([-1, 3, 32]), 16).tolist() == [-1, -1, -1]
 
 
+def test_a_table_without_pages():
+    """Has a slot for nobody; nothing is looked up in it."""
+    assert slots_of(torch.empty(2, 0, dtype=torch.int32), torch.tensor([0, -1]), 16).tolist() == [-1, -1]
+
+
 def test_sizes_that_do_not_fit():
     for bad in (dict(hidden=100), dict(head_dim=136), dict(head_dim=60), dict(num_heads=5), dict(rotary_dim=24), dict(rotary_dim=80)):
         with pytest.raises(ValueError):
