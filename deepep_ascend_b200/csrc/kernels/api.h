@@ -598,6 +598,7 @@ struct AttentionArgs {
     const float *lse_in, *d_lse;      // [heads, tq]; d_lse or null
     float* delta;                     // [heads, tq] workspace
     void *dq, *dk, *dv;               // bf16, contiguous
+    int num_sms;
     int pack;                         // heads of a tile of queries, set by the launch
     int splits;                       // parts of a group that make dk and dv by themselves
     float* parts;                     // [splits, 2, tk, kv_heads, dim] workspace, if there are several
@@ -606,7 +607,7 @@ struct AttentionArgs {
 
 namespace ep {
 cudaError_t launch_attention(const AttentionArgs& args, cudaStream_t stream);
-int attention_backward_splits(const AttentionArgs& args, int num_sms);
+int attention_backward_splits(const AttentionArgs& args);
 cudaError_t launch_attention_backward(const AttentionArgs& args, cudaStream_t stream);
 }  // namespace ep
 

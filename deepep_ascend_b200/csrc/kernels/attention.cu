@@ -284,7 +284,7 @@ __device__ __forceinline__ void store_part(uint32_t tmem, float factor, float* r
 // chain of a tile's block of 128 keys, some 3000 of which two tiles share: 70 for the scores into registers, 370 for their largest, 1050 for the powers, 100 for their way back, 512 + 512 for
 // the products and as much for the barriers between, which lie in the shared memory that the products read at its full rate.  So a quarter of the powers by polynomial, the first half of
 // the probabilities handed over early and an issuing thread for each tile took it from 3650 clocks to 3030.
-// Short sequences have one tile per CTA and two CTAs on an SM, one of which works while the other begins or ends a block; two tiles read keys and values from L2 once for both.
+// Small tasks have one tile per CTA and two CTAs on an SM, one of which works while the other begins or ends a block; two tiles read keys and values from L2 once for both.
 // That tile takes the heads of a group together, each of as many queries as fill 128 rows (7 heads: 18), so that few rows stay empty where a sequence ends: 31 prompts of 264 tokens
 // 125 -> 90 us, 200 of 30 tokens (32 heads) 97 -> 46, 8 of 1000 152 either way.
 constexpr int kPackedHeads = 16;
@@ -337,7 +337,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                  const __grid_constant__ AttentionArgs a) {
     using Shape = FwdShape<kChunks, kTiles>;
     constexpr int kStages = Shape::kStages, kTileBytes = Shape::kTileBytes;
-    const int pack = kTiles == 1 ? a.pack : 1, tokens = 128 / pack;      // heads and tokens of a tile
+    const int pack = a.pack, tokens = 128 / pack;      // heads and tokens of a tile
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *sq = smem, *skv = smem + kTiles * kTileBytes;
     FwdBars* b = reinterpret_cast<FwdBars*>(smem + (kTiles + kStages) * kTileBytes);
@@ -371,7 +371,8 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         umma::tmem_alloc(&b->st.tmem_base, Shape::kColumns);
         umma::tmem_relinquish();
     }
-    if (kTiles == 1 && warp == Shape::kLoadWarp) clear_tile<128, kChunks>(sq, tokens * pack);      // (rows that no query has)
+    if (warp == Shape::kLoadWarp)
+        for (int t = 0; t < kTiles; ++t) clear_tile<128, kChunks>(sq + t * kTileBytes, tokens * pack);      // (rows that no query has)
     umma::fence_before_thread_sync();
     __syncthreads();
     umma::fence_after_thread_sync();
@@ -421,7 +422,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                             if (!attn_wait_warp(&b->q_empty[t], (queries[t] & 1) ^ 1, failed, a.report, 1)) return;
                             ++queries[t];
                             if (one) {
-                                ptx::mbar_arrive_expect_tx(&b->q_full[t], kTiles == 1 ? tokens * pack * 128 * kChunks : kTileBytes);
+                                ptx::mbar_arrive_expect_tx(&b->q_full[t], tokens * pack * 128 * kChunks);
                                 load_tile<128, kChunks>(sq + t * kTileBytes, &map_q, w.head[t], w.start + w.row0[t], &b->q_full[t]);
                             }
                             __syncwarp();
@@ -516,7 +517,7 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 #pragma unroll
                     for (int t = 0; t < kTiles; ++t) {
                         const bool upper = tile + t >= group;
-                        w.row0[t] = blk.row0 + (upper ? 128 : 0);
+                        w.row0[t] = blk.row0 + (upper ? tokens : 0);
                         w.head[t] = (w.kv_head * group + tile + t - (upper ? group : 0)) * pack;
                         const int last = min(w.row0[t] + tokens, blk.rows) - 1, seen = a.causal ? min(last + keys.y - blk.rows + 1, keys.y) : keys.y;
                         w.n[t] = w.row0[t] >= blk.rows || seen <= 0 ? 0 : (seen + 127) / 128;
@@ -1227,10 +1228,13 @@ cudaError_t allow_once(const void* fn, int bytes, std::atomic<uint64_t>& allowed
     return err;
 }
 
-// Sequences of so many keys or fewer on average are short: tiles of queries take heads together, and the forward pass one tile per CTA.  56 heads of 128: forward 8 x 1000 tokens 152 us either way,
-// 4 x 2048 with single tiles 5 % more; gradients of 16 x 450 285 instead of 320 us, 9 x 830 407 instead of 424, 8 x 1000 471 instead of 474 (32 heads, 8 x 1024: 292 instead of 285).
-constexpr int kShortKeys = 1024;
-bool short_sequences(const AttentionArgs& a) { return a.tk / std::max(a.num_seqs, 1) <= kShortKeys; }
+// Small tasks are sequences of so many keys or fewer on average, or few tiles for the SMs: tiles of queries take heads together, and the forward pass one tile per CTA.  Forward: 8 x 1000 tokens of 56
+// heads 150 instead of 157 us, 8 x 1500 of 32 heads 196 instead of 221, 8 x 2000 of 56 485 instead of 471; one of 4096 with 16 heads (512 tiles) 81 instead of 97, with 32 (1024) 126 instead of 131, with 56
+// (1792) 223 instead of 213, one of 8192 with 16 (1024) 234 instead of 229.  Gradients (heads together or not): 16 x 450 285 instead of 320, 8 x 1500 598 instead of 620 to 637.
+constexpr int kShortKeys = 2048, kFewTiles = 6;      // (tiles: per SM)
+bool is_small(const AttentionArgs& a) {
+    return a.tk / std::max(a.num_seqs, 1) <= kShortKeys || static_cast<int64_t>(a.tq) * a.heads / 128 < static_cast<int64_t>(kFewTiles) * a.num_sms;
+}
 // Heads that a tile takes of as many tokens as fill it: all of a group, or as many as divide it
 int packed_heads(const AttentionArgs& a) {
     const int group = a.heads / a.kv_heads;
@@ -1245,7 +1249,7 @@ cudaError_t launch_forward(AttentionArgs a, cudaStream_t stream) {
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t err = allow_once(fn, Shape::kSmem, allowed);
     if (err != cudaSuccess) return err;
-    a.pack = kTiles == 1 ? packed_heads(a) : 1;
+    a.pack = is_small(a) ? packed_heads(a) : 1;
     const int tokens = 128 / a.pack;
     CUtensorMap q, k, v;
     if (!make_map(&q, a.q, a.tq, a.heads, a.dim, tokens, a.pack) || !make_map(&k, a.k, a.tk, a.kv_heads, a.dim, 128) || !make_map(&v, a.v, a.tk, a.kv_heads, a.dim, 128))
@@ -1255,7 +1259,7 @@ cudaError_t launch_forward(AttentionArgs a, cudaStream_t stream) {
 }
 template <int kChunks>
 cudaError_t launch_forward(const AttentionArgs& a, cudaStream_t stream) {
-    return short_sequences(a) ? launch_forward<kChunks, 1>(a, stream) : launch_forward<kChunks, 2>(a, stream);
+    return is_small(a) ? launch_forward<kChunks, 1>(a, stream) : launch_forward<kChunks, 2>(a, stream);
 }
 template <int kChunks, bool kKeys>
 cudaError_t launch_gradient(const AttentionArgs& a, const CUtensorMap& q, const CUtensorMap& d, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t stream) {
@@ -1272,7 +1276,7 @@ cudaError_t launch_gradient(const AttentionArgs& a, const CUtensorMap& q, const 
 template <int kChunks>
 cudaError_t launch_backward(AttentionArgs a, cudaStream_t stream) {
     CUtensorMap q, k, v, d;
-    a.pack = short_sequences(a) ? packed_heads(a) : 1;
+    a.pack = is_small(a) ? packed_heads(a) : 1;
     if (!make_map(&q, a.q, a.tq, a.heads, a.dim, 128 / a.pack, a.pack) || !make_map(&d, a.d_o, a.tq, a.heads, a.dim, 128 / a.pack, a.pack) || !make_map(&k, a.k, a.tk, a.kv_heads, a.dim, 128) ||
         !make_map(&v, a.v, a.tk, a.kv_heads, a.dim, 128))
         return cudaErrorInvalidValue;
@@ -1296,9 +1300,9 @@ cudaError_t launch_attention(const AttentionArgs& a, cudaStream_t stream) {
     return a.dim <= 64 ? launch_forward<1>(a, stream) : launch_forward<2>(a, stream);
 }
 // Parts of a group whose gradients of keys and values are made by CTAs of their own, and then added (8 bytes per part and value each way): as many as give every SM two.
-int attention_backward_splits(const AttentionArgs& a, int num_sms) {
+int attention_backward_splits(const AttentionArgs& a) {
     const int64_t ctas = std::max<int64_t>(1, std::max(a.tk / 128, 1) * a.kv_heads);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(a.heads / a.kv_heads, 2 * num_sms / ctas)));
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(a.heads / a.kv_heads, 2 * a.num_sms / ctas)));
 }
 cudaError_t launch_attention_backward(const AttentionArgs& a, cudaStream_t stream) {
     return a.dim <= 64 ? launch_backward<1>(a, stream) : launch_backward<2>(a, stream);

@@ -67,6 +67,7 @@ inline PackedInputs packed_inputs(const at::Tensor& q, const at::Tensor& k, cons
     a.dim = static_cast<int>(q.size(2));
     a.causal = causal;
     a.scale = static_cast<float>(scale);
+    a.num_sms = device_sms();
     return in;
 }
 
@@ -108,7 +109,7 @@ inline std::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor>> attention_b
     in.a.lse_in = lse.data_ptr<float>();
     in.a.d_lse = d_lse.has_value() ? d_lse->data_ptr<float>() : nullptr;
     in.a.delta = delta.data_ptr<float>();
-    in.a.splits = ep::attention_backward_splits(in.a, device_sms());
+    in.a.splits = ep::attention_backward_splits(in.a);
     at::Tensor parts;
     if (in.a.splits > 1) {
         parts = at::empty({in.a.splits, 2, k.numel()}, lse.options());
