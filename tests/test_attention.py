@@ -113,6 +113,34 @@ def test_longer_sequences(lq, lk, H, Hk, D, causal):
     _check(*_make(sum(lq), sum(lk), H, Hk, D, 3, 'cuda'), lq, lk, causal)
 
 
+@pytest.mark.gpu
+def test_long_sequences_of_many_heads():
+    """Enough tiles of long sequences that a CTA takes two, of heads apart."""
+    lq = [2000, 2110]
+    _check(*_make(sum(lq), sum(lq), 28, 4, 72, 6, 'cuda'), lq, lq, True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('H,Hk,D,causal', [(70, 10, 128, True), (70, 10, 64, False), (64, 64, 40, True), (72, 24, 104, True)])
+def test_many_heads_are_what_few_are(H, Hk, D, causal):
+    """Rows do not depend on one another: a launch with many tiles, and those of its heads by themselves, have the same bits."""
+    lq, lk = [2049, 2311], [2049, 2400]
+    q, k, v, d_o, d_lse = _make(sum(lq), sum(lk), H, Hk, D, 7, 'cuda')
+    cq, ck = _cu(lq, 'cuda'), _cu(lk, 'cuda')
+    o, lse = attention(q, k, v, cq, ck, causal)
+    dq, dk, dv = attention_backward(d_o, q, k, v, o, lse, cq, ck, causal, d_lse=d_lse)
+    group = H // Hk
+    for h in range(0, Hk, max(1, Hk // 3)):
+        a, b = slice(h * group, h * group + group), slice(h, h + 1)
+        some = attention(q[:, a], k[:, b], v[:, b], cq, ck, causal)
+        assert torch.equal(o[:, a], some[0]) and torch.equal(lse[a], some[1])
+        grads = attention_backward(d_o[:, a], q[:, a], k[:, b], v[:, b], *some, cq, ck, causal, d_lse=d_lse[a].contiguous())
+        assert torch.equal(dq[:, a], grads[0])
+        # (sums over the heads may be in another order: within a rounding of the size that they have on the whole)
+        for x, y in ((dk[:, b], grads[1]), (dv[:, b], grads[2])):
+            assert float((x.float() - y.float()).norm()) <= 2 * HALF * float(y.float().norm())
+
+
 @pytest.mark.parametrize('device', DEVICES)
 def test_one_sequence_and_a_scale(device):
     q, k, v, d_o, d_lse = _make(150, 190, 4, 2, 64, 1, device)
