@@ -649,8 +649,9 @@ struct RotaryArgs {
     int positions_64;
     float eps;
     // keys and values into a paged cache
+    int append;                       // whether they go there (a cache without pages has no address either)
     HeadsView v;
-    void *k_cache, *v_cache;          // or null: no cache
+    void *k_cache, *v_cache;
     int64_t stride_page, stride_slot, stride_head;
     int64_t num_slots;                // num_pages * page_size
     int page_size;

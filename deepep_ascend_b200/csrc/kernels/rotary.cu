@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kForwardCtas) rotary_kernel(co
     T *out, *too = nullptr;                              // (keys may go to a cache and to a result)
     int64_t pitch;
     bool write = place.on;
-    if (kind == 0 || a.k_cache == nullptr) {
+    if (kind == 0 || !a.append) {
         out = static_cast<T*>(a.out[kind]) + token * heads * a.dim;
         pitch = a.dim;
     } else {
@@ -415,7 +415,7 @@ cudaError_t launch_rotary(const RotaryArgs& a, int num_sms, cudaStream_t stream)
         constexpr bool kInterleaved = decltype(interleaved)::value;
         auto launch = [&](const void* fn, int iters) {
             auto chunks_of = [&](int heads) { return (heads + iters * kRows - 1) / (iters * kRows); };
-            int chunks_q = chunks_of(a.heads[0]), chunks_k = chunks_of(a.heads[1]), chunks = chunks_q + chunks_k * (a.k_cache != nullptr ? 2 : 1);
+            int chunks_q = chunks_of(a.heads[0]), chunks_k = chunks_of(a.heads[1]), chunks = chunks_q + chunks_k * (a.append ? 2 : 1);
             const int64_t ctas = (static_cast<int64_t>(a.tokens) * chunks * 32 + kRotaryThreads - 1) / kRotaryThreads;
             void* params[] = {const_cast<RotaryArgs*>(&a), &chunks_q, &chunks_k, &chunks};
             return launch_dependent(fn, dim3(static_cast<unsigned>(ctas)), dim3(kRotaryThreads), params, 0, stream);

@@ -158,8 +158,9 @@ inline at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache
     const at::Tensor q16 = heads_of(q);
     PagedAttentionArgs a{};
     a.q = view_of(q16);
-    a.k_cache = k_cache.data_ptr();
-    a.v_cache = v_cache.data_ptr();
+    // (caches without pages have no address: nothing is read, and pointers are stepped from one that is there)
+    a.k_cache = k_cache.numel() != 0 ? k_cache.data_ptr() : q16.data_ptr();
+    a.v_cache = k_cache.numel() != 0 ? v_cache.data_ptr() : q16.data_ptr();
     a.stride_page = k_cache.stride(0);
     a.stride_slot = k_cache.stride(1);
     a.stride_head = k_cache.stride(2);
@@ -265,6 +266,7 @@ inline std::optional<std::tuple<at::Tensor, std::optional<at::Tensor>>> qk_norm_
     RotaryArgs& a = in.a;
     a.out[0] = yq.data_ptr();
     if (keep_k) a.out[1] = yk->data_ptr();
+    a.append = 1;
     a.v = view_of(v16);
     a.k_cache = k_cache.data_ptr();
     a.v_cache = v_cache.data_ptr();

@@ -141,6 +141,17 @@ def test_no_tokens():
 
 
 @pytest.mark.gpu
+def test_a_cache_without_pages():
+    """A prompt is what it is without a cache; a single token, which has no place for its key, gets no numbers, and one of no sequence comes back."""
+    block = _block(4)
+    x = torch.randn(20, 256, device='cuda').bfloat16()
+    cache = block.new_cache(0, 16)
+    assert torch.equal(block.prefill(x, cache, torch.arange(20, device='cuda')), block(x).detach())
+    y = block.decode(x[:2], cache, torch.zeros(2, 1, dtype=torch.int32, device='cuda'), torch.tensor([1, 0], dtype=torch.int32, device='cuda'))
+    assert y[0].isnan().all() and torch.equal(y[1], x[1])
+
+
+@pytest.mark.gpu
 def test_a_layer_runs(capsys):
     from deepep_ascend_b200.models import attention
     attention.main(steps=3, new_tokens=3)

@@ -117,6 +117,16 @@ def test_pages_that_are_none(lengths, device):
     assert not o[:3].any() and o[3].isnan().all()
 
 
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('width', [1, 100])
+def test_caches_without_pages(width, device):
+    """Every page is one that they do not have."""
+    q, k, v, _, _ = _make([1, 1, 1], 4, 2, 64, 16, 13, device)
+    table = torch.zeros(3, width, dtype=torch.int32, device=device)
+    o = paged_attention(q, k[:0].clone(), v[:0].clone(), table, torch.tensor([1, 0, 16 * width], dtype=torch.int32, device=device))
+    assert o[0].isnan().all() and not o[1].any() and o[2].isnan().all()
+
+
 @pytest.mark.gpu
 def test_the_same_bits_and_graphs():
     """Graphs of one shape, each with data of its own, replayed in turn; lengths that change between replays."""

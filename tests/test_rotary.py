@@ -151,6 +151,18 @@ def test_into_paged_caches(T, Hq, Hk, D, size, dtype, index, layout, device):
     assert torch.equal(again[0], q) and torch.equal(again[1], k)
 
 
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('keep_k', [False, True])
+def test_caches_without_pages(keep_k, device):
+    """Have a place for nobody: nothing is written, and the results are those of any caches."""
+    given, qw, kw, table, positions = _make(5, 4, 2, 64, 32, BF16, F32, 9, device)
+    want = qk_norm_rope(given['q'], given['k'], qw, kw, table, positions)
+    k_cache, v_cache = _caches(0, 16, 2, 64, BF16, device, 'plain')
+    for slots in (torch.arange(5, device=device), torch.tensor([-1, 0, 2**31 - 1, 7, -16], dtype=torch.int32, device=device)):
+        out = qk_norm_rope_append(given['q'], given['k'], given['dk'], qw, kw, table, positions, k_cache, v_cache, slots, keep_k=keep_k)
+        assert torch.equal(out[0] if keep_k else out, want[0]) and (not keep_k or torch.equal(out[1], want[1]))
+
+
 @pytest.mark.gpu
 def test_strides_and_alignment():
     given, qw, kw, table, positions = _make(37, 6, 2, 96, 64, BF16, F32, 3, 'cuda')
