@@ -160,19 +160,17 @@ __device__ __forceinline__ void attend(const PagedAttentionArgs& a, uint8_t* rin
 
     const bf16 *k_head = static_cast<const bf16*>(a.k_cache) + kv_head * a.stride_head, *v_head = static_cast<const bf16*>(a.v_cache) + kv_head * a.stride_head;
     const int32_t* table = a.page_table + seq * a.table_pitch;
-    // lanes 0 to 15: the page of a key of the tile
-    auto page_of = [&](int tile) {
-        const int key = tile * kTileKeys + warp * 16 + (lane & 15);
-        return tile < tile1 && key < keys ? table[static_cast<uint32_t>(key) / static_cast<uint32_t>(a.page_size)] : -2;
-    };
+    // lanes 0 to 15: a key of the tile, and its page, which may be any number
+    auto key_of = [&](int tile) { return tile * kTileKeys + warp * 16 + (lane & 15); };
+    auto page_of = [&](int tile) { return tile < tile1 && key_of(tile) < keys ? table[static_cast<uint32_t>(key_of(tile)) / static_cast<uint32_t>(a.page_size)] : -1; };
     int page = page_of(tile0);
     auto request = [&](int tile, int stage) {
         if (tile < tile1) {
-            const int key = tile * kTileKeys + warp * 16 + (lane & 15);
+            const int key = key_of(tile);
             const bool there = page >= 0 && page < a.num_pages;
             const int64_t at = there ? page * a.stride_page + static_cast<int64_t>(static_cast<uint32_t>(key) % static_cast<uint32_t>(a.page_size)) * a.stride_slot : -1;
             // keys of the sequence whose page is none
-            const uint32_t bad = __ballot_sync(0xffffffffu, !there && page != -2) & 0xffffu;
+            const uint32_t bad = __ballot_sync(0xffffffffu, !there && key < keys) & 0xffffu;
             if (lane == 0) bad_tiles[warp * kPagedStages + stage] = bad;
             page = page_of(tile + 1);
             const uint32_t to = base + stage * Shape::kStageBytes;

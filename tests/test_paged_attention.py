@@ -118,6 +118,20 @@ def test_pages_that_are_none(lengths, device):
 
 
 @pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('page', [-1, -2, -3, -2**31, 2**31 - 1])
+@pytest.mark.parametrize('n', [30, 5000])
+def test_any_number_that_is_no_page(n, page, device):
+    """First, in the middle and last of a sequence's pages; in tables that cut the work and in those that do not."""
+    lengths = [n, 20, n, n - 5]
+    q, k, v, table, lens = _make(lengths, 4, 2, 64, 16, 14, device)
+    for b, at in ((0, 0), (2, n // 32), (3, (n - 6) // 16)):
+        table[b, at] = page
+    o = paged_attention(q, k, v, table, lens)
+    assert all(o[b].isnan().all() for b in (0, 2, 3))
+    _check(q, k, v, table, lens, skip=(0, 2, 3))
+
+
+@pytest.mark.parametrize('device', DEVICES)
 @pytest.mark.parametrize('width', [1, 100])
 def test_caches_without_pages(width, device):
     """Every page is one that they do not have."""
