@@ -600,6 +600,7 @@ struct AttentionArgs {
     void *dq, *dk, *dv;               // bf16, contiguous
     int num_sms;
     int pack;                         // heads of a tile of queries, set by the launch
+    int key_ctas;                     // of the gradients' CTAs those of keys, which come first, set by the launch
     int splits;                       // parts of a group that make dk and dv by themselves
     float* parts;                     // [splits, 2, tk, kv_heads, dim] workspace, if there are several
     NsReport report;

@@ -11,6 +11,7 @@
 // A causal query sees the keys up to its own place, both sequences ending together: query i of nq the keys 0 .. nk - nq + i of nk.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "common.cuh"
 #include "gemm_sm100.cuh"
@@ -739,15 +740,20 @@ __global__ void __launch_bounds__(kDeltaThreads) attention_delta_kernel(const __
 // as whole ones: 128 rows of the first operand come from shared memory either way.)
 constexpr int kBwdThreads = 384;                     // 2 x 4 warps for rows, one that requests pieces, one that issues products, one that looks for work, one without any
 constexpr int kBwdReaders = 10;
-template <int kChunks, bool kKeys>
+template <int kChunks>
 struct BwdShape {
     static constexpr int kTileBytes = 128 * 128 * kChunks, kSlots = kChunks == 2 ? 5 : 8;
-    // tensor memory: sums (of keys and values, or of queries), scores, dP (once, or twice)
-    static constexpr int kScores = kKeys ? 256 : 128, kDp = kKeys ? 384 : 256, kDps = kKeys ? 1 : 2;
     static constexpr int kStatBytes = 2 * 2 * 128 * 4;
     static constexpr int kSmem = (2 + kSlots) * kTileBytes + kStatBytes + 1024;
 };
+// Tensor memory of a block: sums (of keys and values, or of queries), scores, dP (once, or, of queries, in turn by pieces)
+template <bool kKeys>
+struct BwdColumns {
+    static constexpr uint32_t kScores = kKeys ? 256 : 128;
+    static __device__ __forceinline__ uint32_t dp(uint32_t piece) { return kKeys ? 384 : 256 + (piece & 1) * 128; }
+};
 struct BwdWork {
+    int keys;                        // whether the block is one of keys
     int start, row0, rows;           // as of AttnBlock; rows < 0: no more work
     int other0, others;              // rows of the other side
     int head, first_head, split;     // (first) kept head, first head of the pieces
@@ -763,12 +769,17 @@ struct BwdBars {
     uint64_t kept, kept_empty, full[8], empty[8], s_full, s_read, dp_full[2], p_full[2][2], stats_full[2], sums, drained, work_full, work_read, answered, tail, quiet;
     AttnState st;
 };
+static_assert(sizeof(BwdBars) <= 1024, "what BwdShape leaves for it");
 
-template <int kChunks, bool kKeys>
+// Blocks of keys and blocks of queries are one launch, those of keys first: a CTA takes either as they come, so that the SMs which the last keys leave free go on with queries (1000 tokens of 8
+// heads of 128: 25 us, with a launch for each 40; two documents of 4096, 56 heads: 1420 to 1470, 1640 to 1670).  Both read delta, which the kernel before this one makes, and nothing that the other makes.
+template <int kChunks>
 __global__ void __launch_bounds__(kBwdThreads, 1)
-attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const __grid_constant__ CUtensorMap map_kept1, const __grid_constant__ CUtensorMap map_piece0,
-                          const __grid_constant__ CUtensorMap map_piece1, const __grid_constant__ AttentionArgs a) {
-    using Shape = BwdShape<kChunks, kKeys>;
+attention_backward_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_q,
+                          const __grid_constant__ CUtensorMap map_d, const __grid_constant__ AttentionArgs a) {
+    using Shape = BwdShape<kChunks>;
+    using Keys = std::true_type;
+    using Queries = std::false_type;
     constexpr int kSlots = Shape::kSlots, kTileBytes = Shape::kTileBytes;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t *kept = smem, *pieces = smem + 2 * kTileBytes;
@@ -776,12 +787,12 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
     BwdBars* b = reinterpret_cast<BwdBars*>(pieces + kSlots * kTileBytes + Shape::kStatBytes);
     const int warp = threadIdx.x >> 5, group = a.heads / a.kv_heads;
     // queries lie in tiles of `tokens` times `pack` heads, keys in tiles of 128
-    const int pack = a.pack, tokens = 128 / pack, step = kKeys ? tokens : 128;
+    const int pack = a.pack, tokens = 128 / pack;
     if (threadIdx.x == 0) {
-        umma::prefetch_tensormap(&map_kept0);
-        umma::prefetch_tensormap(&map_kept1);
-        umma::prefetch_tensormap(&map_piece0);
-        umma::prefetch_tensormap(&map_piece1);
+        umma::prefetch_tensormap(&map_k);
+        umma::prefetch_tensormap(&map_v);
+        umma::prefetch_tensormap(&map_q);
+        umma::prefetch_tensormap(&map_d);
         ptx::mbar_init(&b->kept, 1);
         ptx::mbar_init(&b->kept_empty, 1);
         ptx::mbar_init(&b->drained, 8);
@@ -811,18 +822,13 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
         umma::tmem_relinquish();
     }
     if (warp == 8) {                                     // (rows that no query has)
-        for (int i = kKeys ? 2 : 0; i < (kKeys ? 2 + kSlots : 2); ++i) clear_tile<128, kChunks>(smem + i * kTileBytes, tokens * pack);
+        for (int i = 0; i < 2 + kSlots; ++i) clear_tile<128, kChunks>(smem + i * kTileBytes, tokens * pack);
     }
     umma::fence_before_thread_sync();
     __syncthreads();
     umma::fence_after_thread_sync();
     const uint32_t tmem = b->st.tmem_base;
-    // The kernel of keys lets that of queries in when it has seen what was before it, which that one needs no more of: its CTAs take the SMs that are free, and end behind it (what is
-    // launched next may read both).  1000 tokens, 8 heads: 45 us one after the other, 32 so
-    if (kKeys) {
-        ptx::wait_for_previous_kernel();
-        ptx::let_next_kernel_start();
-    }
+    ptx::wait_for_previous_kernel();
     int* failed = &b->st.failed;
     // The k-th block of this CTA, for a whole warp; false: no more
     auto next_work = [&](int k, BwdWork& w) {
@@ -838,11 +844,18 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
         if (warp == 8) {
             AttnRing<kSlots> p;
             const bool one = ptx::elect_one();
-            uint32_t tails = 0, blocks = 0;
-            BwdWork w;
-            auto request = [&](const CUtensorMap* map, int h, int piece) {
+            uint32_t tails = 0, blocks = 0, whole = 0;   // whole: stages (bits) whose last tile was one of keys, with rows that no query has
+            auto request = [&](auto kind, const BwdWork& w, const CUtensorMap* map, int h, int piece) {
+                constexpr bool kKeys = decltype(kind)::value;
+                const int step = kKeys ? tokens : 128;
                 if (!attn_wait_warp(&b->empty[p.stage], p.phase ^ 1, failed, a.report, 1)) return false;
                 uint8_t* tile = pieces + p.stage * kTileBytes;
+                if (!kKeys) {
+                    whole |= 1u << p.stage;
+                } else if (whole >> p.stage & 1u) {
+                    clear_tile<128, kChunks>(tile, tokens * pack);
+                    whole &= ~(1u << p.stage);
+                }
                 const bool tail = piece * step + step > w.others;
                 uint64_t* bar = tail ? &b->tail : &b->full[p.stage];
                 if (one) {
@@ -859,24 +872,26 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                 p.advance();
                 return true;
             };
-            auto load = [&]() {
-                for (int k = 0; next_work(k, w); ++k) {
-                    if (w.n == 0) continue;
-                    if (!attn_wait_warp(&b->kept_empty, (blocks & 1) ^ 1, failed, a.report, 1)) return;
-                    ++blocks;
-                    if (one) {
-                        ptx::mbar_arrive_expect_tx(&b->kept, 2 * (kKeys ? kTileBytes : tokens * pack * 128 * kChunks));
-                        load_tile<128, kChunks>(kept, &map_kept0, w.head, w.start + w.row0, &b->kept);
-                        load_tile<128, kChunks>(kept + kTileBytes, &map_kept1, w.head, w.start + w.row0, &b->kept);
-                    }
-                    __syncwarp();
-                    for (int i = 0; i < w.n; ++i) {
-                        const int h = kKeys ? w.head_of(i, pack) : w.head / group, piece = w.piece_of(i);
-                        if (!request(&map_piece0, h, piece) || !request(&map_piece1, h, piece)) return;
-                    }
+            auto load = [&](auto kind, const BwdWork& w) {
+                constexpr bool kKeys = decltype(kind)::value;
+                if (w.n == 0) return true;
+                if (!attn_wait_warp(&b->kept_empty, (blocks & 1) ^ 1, failed, a.report, 1)) return false;
+                ++blocks;
+                if (one) {
+                    ptx::mbar_arrive_expect_tx(&b->kept, 2 * (kKeys ? kTileBytes : tokens * pack * 128 * kChunks));
+                    load_tile<128, kChunks>(kept, kKeys ? &map_k : &map_q, w.head, w.start + w.row0, &b->kept);
+                    load_tile<128, kChunks>(kept + kTileBytes, kKeys ? &map_v : &map_d, w.head, w.start + w.row0, &b->kept);
                 }
+                __syncwarp();
+                for (int i = 0; i < w.n; ++i) {
+                    const int h = kKeys ? w.head_of(i, pack) : w.head / group, piece = w.piece_of(i);
+                    if (!request(kind, w, kKeys ? &map_q : &map_k, h, piece) || !request(kind, w, kKeys ? &map_d : &map_v, h, piece)) return false;
+                }
+                return true;
             };
-            load();
+            BwdWork w;
+            for (int k = 0; next_work(k, w); ++k)
+                if (!(w.keys ? load(Keys{}, w) : load(Queries{}, w))) break;
         } else if (warp == 9) {
             const bool one = ptx::elect_one();
             const int dim16 = (a.dim + 15) / 16;
@@ -885,6 +900,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
             const uint32_t kept_of = desc_channels(kept), pieces_of = desc_channels(pieces), rows_of = desc_rows<128>(pieces);
             AttnRing<kSlots> p;                       // operands in the order in which they come: first and second of every piece
             uint32_t made = 0, blocks = 0;            // pieces, blocks so far
+            int keys_before = 0;                      // kind of the block before
             // the first products of a piece, of its first or second operand
             auto product = [&](int which, uint32_t to, uint64_t* done, int& slot) {
                 if (!attn_wait(&b->full[p.stage], p.phase, failed, a.report, 4)) return false;
@@ -895,23 +911,27 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                 p.advance();
                 return true;
             };
-            auto multiply = [&](int n) {
+            auto multiply = [&](auto kind, int n) {
+                constexpr bool kKeys = decltype(kind)::value;
+                using Columns = BwdColumns<kKeys>;
+                // (the sums of the block before have been read: of another kind, they lie where this one's first products go)
+                if (blocks > 0 && keys_before != kKeys && !attn_wait(&b->drained, (blocks - 1) & 1, failed, a.report, 6)) return;
+                keys_before = kKeys;
                 if (!attn_wait(&b->kept, blocks & 1, failed, a.report, 4)) return;
                 int slot0, slot1, next0 = 0, next1 = 0;
-                if (!product(0, Shape::kScores, &b->s_full, slot0) || !product(1, Shape::kDp + (kKeys ? 0 : (made & 1) * 128), &b->dp_full[made & 1], slot1)) return;
+                if (!product(0, Columns::kScores, &b->s_full, slot0) || !product(1, Columns::dp(made), &b->dp_full[made & 1], slot1)) return;
                 if (!kKeys) umma::mma_commit(&b->empty[slot1]);
                 if (n == 1) umma::mma_commit(&b->kept_empty);
-                // (the sums of the block before have been read)
                 if (blocks > 0 && !attn_wait(&b->drained, (blocks - 1) & 1, failed, a.report, 6)) return;
                 ++blocks;
                 for (int i = 0; i < n; ++i, ++made) {
-                    const uint32_t dp = Shape::kDp + (kKeys ? 0 : (made & 1) * 128);
+                    const uint32_t dp = Columns::dp(made);
                     if (i + 1 < n) {
                         if (!attn_wait(&b->s_read, made & 1, failed, a.report, 3)) return;
-                        if (!product(0, Shape::kScores, &b->s_full, next0)) return;
+                        if (!product(0, Columns::kScores, &b->s_full, next0)) return;
                         if (!kKeys) {
                             // (the other place of dP: what was there is behind the products before)
-                            if (!product(1, Shape::kDp + (~made & 1) * 128, &b->dp_full[~made & 1], next1)) return;
+                            if (!product(1, Columns::dp(made + 1), &b->dp_full[~made & 1], next1)) return;
                             umma::mma_commit(&b->empty[next1]);
                             if (i + 2 == n) umma::mma_commit(&b->kept_empty);
                         }
@@ -929,7 +949,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                     if (kKeys) {
                         umma::mma_commit(&b->empty[slot1]);
                         if (i + 1 < n) {
-                            if (!product(1, Shape::kDp, &b->dp_full[~made & 1], next1)) return;
+                            if (!product(1, Columns::dp(made + 1), &b->dp_full[~made & 1], next1)) return;
                             if (i + 2 == n) umma::mma_commit(&b->kept_empty);
                         }
                     }
@@ -941,12 +961,14 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
             };
             BwdWork w;
             for (int k = 0; next_work(k, w); ++k) {
-                if (one && w.n > 0) multiply(w.n);
+                if (one && w.n > 0) {
+                    if (w.keys) multiply(Keys{}, w.n);
+                    else multiply(Queries{}, w.n);
+                }
                 __syncwarp();
             }
         } else if (warp == 10) {
             // looks for work: first this CTA's own
-            const int units = kKeys ? a.kv_heads * a.splits : a.heads / pack;
             int item = blockIdx.x;
             uint32_t handed = 0;
             for (uint32_t answers = 0;; ++answers) {
@@ -954,15 +976,17 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                 w.rows = -1;
                 bool something = true;
                 if (item >= 0) {
-                    // (kKeys: the first keys are seen by most queries; otherwise the last queries see most keys.  Long blocks first.)
-                    const int unit = item % units, number = item / units;
-                    w.head = kKeys ? unit / a.splits : unit * pack;      // (of keys, or of queries)
-                    w.split = kKeys ? unit % a.splits : 0;
-                    w.first_head = kKeys ? w.head * group : 0;
-                    const AttnBlock blk =
-                        find_block(kKeys ? a.cu_k : a.cu_q, a.num_seqs, kKeys ? a.tk : a.tq, kKeys ? number : static_cast<int>(gridDim.x / units) - 1 - number, kKeys ? 128 : tokens);
-                    const int2 other = sequence_rows(kKeys ? a.cu_q : a.cu_k, blk.seq, kKeys ? a.tq : a.tk);
-                    const int shift = kKeys ? blk.rows - other.y : other.y - blk.rows;
+                    // (keys: the first ones are seen by most queries; queries: the last ones see most keys.  Long blocks first.)
+                    const bool keys = item < a.key_ctas;
+                    const int units = keys ? a.kv_heads * a.splits : a.heads / pack, mine = keys ? item : item - a.key_ctas, all_mine = keys ? a.key_ctas : gridDim.x - a.key_ctas;
+                    const int unit = mine % units, number = mine / units, step = keys ? tokens : 128;
+                    w.keys = keys;
+                    w.head = keys ? unit / a.splits : unit * pack;      // (of keys, or of queries)
+                    w.split = keys ? unit % a.splits : 0;
+                    w.first_head = keys ? w.head * group : 0;
+                    const AttnBlock blk = find_block(keys ? a.cu_k : a.cu_q, a.num_seqs, keys ? a.tk : a.tq, keys ? number : all_mine / units - 1 - number, keys ? 128 : tokens);
+                    const int2 other = sequence_rows(keys ? a.cu_q : a.cu_k, blk.seq, keys ? a.tq : a.tk);
+                    const int shift = keys ? blk.rows - other.y : other.y - blk.rows;
                     w.start = blk.start;
                     w.row0 = blk.row0;
                     w.rows = blk.rows;
@@ -970,7 +994,7 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                     w.others = other.y;
                     something = blk.row0 < blk.rows;
                     int piece1 = (other.y + step - 1) / step;
-                    if (kKeys) {
+                    if (keys) {
                         w.piece0 = a.causal ? max(blk.row0 - shift, 0) / step : 0;
                     } else if (a.causal) {
                         const int seen = min(min(blk.row0 + tokens, blk.rows) + shift, other.y);
@@ -978,15 +1002,15 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                     }
                     w.per_head = max(piece1 - w.piece0, 0);
                     // (a part of the group's pieces, of all heads)
-                    const int64_t all = static_cast<int64_t>(w.per_head) * (kKeys ? group / pack : 1);
-                    w.first = static_cast<int>(kKeys ? all * w.split / a.splits : 0);
-                    w.n = static_cast<int>((kKeys ? all * (w.split + 1) / a.splits : all) - w.first);
-                    const int64_t row_values = static_cast<int64_t>(kKeys ? a.kv_heads : a.heads) * a.dim;
-                    if (!kKeys) {
-                        clear_rows<32>(a.cu_q, a.num_seqs, a.tq, item, gridDim.x, reinterpret_cast<bf16*>(a.dq), row_values, nullptr, 0);
+                    const int64_t all = static_cast<int64_t>(w.per_head) * (keys ? group / pack : 1);
+                    w.first = static_cast<int>(keys ? all * w.split / a.splits : 0);
+                    w.n = static_cast<int>((keys ? all * (w.split + 1) / a.splits : all) - w.first);
+                    const int64_t row_values = static_cast<int64_t>(keys ? a.kv_heads : a.heads) * a.dim;
+                    if (!keys) {
+                        clear_rows<32>(a.cu_q, a.num_seqs, a.tq, mine, all_mine, reinterpret_cast<bf16*>(a.dq), row_values, nullptr, 0);
                     } else if (a.splits == 1) {
-                        clear_rows<32>(a.cu_k, a.num_seqs, a.tk, item, gridDim.x, reinterpret_cast<bf16*>(a.dk), row_values, nullptr, 0);
-                        clear_rows<32>(a.cu_k, a.num_seqs, a.tk, item, gridDim.x, reinterpret_cast<bf16*>(a.dv), row_values, nullptr, 0);
+                        clear_rows<32>(a.cu_k, a.num_seqs, a.tk, mine, all_mine, reinterpret_cast<bf16*>(a.dk), row_values, nullptr, 0);
+                        clear_rows<32>(a.cu_k, a.num_seqs, a.tk, mine, all_mine, reinterpret_cast<bf16*>(a.dv), row_values, nullptr, 0);
                     }
                 }
                 if (something) {                      // (numbers without a block are passed over)
@@ -1008,13 +1032,15 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
         const int half = warp >> 2, lane_row = threadIdx.x & 127;
         const uint32_t lanes = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
         const float c = a.scale * kLog2e;
-        float* mine = stats + half * 256;             // twice: 64 times -lse log2 e, 64 times -delta
+        float* stats_of_half = stats + half * 256;    // twice: 64 times -lse log2 e, 64 times -delta
         const uint64_t c2 = f32x2(c, c);
-        const int column = kKeys ? half * 64 + (lane_row & 63) : lane_row, token_of = column / pack, head_of = column - token_of * pack;      // of what this thread reads statistics of
-        uint32_t made = 0, ended = 0;                 // pieces, blocks so far
-        bool ok = true;
-        BwdWork w;
-        for (int k = 0; ok && next_work(k, w); ++k) {
+        uint32_t made = 0, told = 0, ended = 0;       // pieces, pieces with statistics, blocks so far
+        // A block; false: a wait has run out
+        auto rows = [&](auto kind, const BwdWork& w) {
+            constexpr bool kKeys = decltype(kind)::value;
+            using Columns = BwdColumns<kKeys>;
+            const int step = kKeys ? tokens : 128;
+            const int column = kKeys ? half * 64 + (lane_row & 63) : lane_row, token_of = column / pack, head_of = column - token_of * pack;      // of what this thread reads statistics of
             const int row = w.row0 + (kKeys ? lane_row : token_of), shift = kKeys ? w.rows - w.others : w.others - w.rows;     // query i sees the keys up to i + shift
             const bool in = row < w.rows && (kKeys || token_of < tokens);
             const int64_t token = w.start + row;
@@ -1042,21 +1068,20 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                 delta2 = f32x2(d, d);
             }
             for (int i = 0; i < w.n; ++i, ++made) {
-                const float* now = mine + (made & 1) * 128;
+                float* now = stats_of_half + (told & 1) * 128;
                 if (kKeys) {
-                    mine[(made & 1) * 128 + lane_row] = coming;
+                    now[lane_row] = coming;
                     __syncwarp();
                     if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->stats_full[half]);
                     coming = next_statistic(i + 1);
-                    ok = attn_wait_warp(&b->stats_full[half], made & 1, failed, a.report, 6);
-                    if (!ok) break;
+                    if (!attn_wait_warp(&b->stats_full[half], told & 1, failed, a.report, 6)) return false;
+                    ++told;
                 }
-                ok = attn_wait_warp(&b->s_full, made & 1, failed, a.report, 5);
-                if (!ok) break;
+                if (!attn_wait_warp(&b->s_full, made & 1, failed, a.report, 5)) return false;
                 umma::fence_after_thread_sync();
                 uint32_t s[2][32], d[2][32];
-                umma::tmem_ld_32x32(lanes + Shape::kScores + half * 64, s[0]);
-                umma::tmem_ld_32x32(lanes + Shape::kScores + half * 64 + 32, s[1]);
+                umma::tmem_ld_32x32(lanes + Columns::kScores + half * 64, s[0]);
+                umma::tmem_ld_32x32(lanes + Columns::kScores + half * 64 + 32, s[1]);
                 umma::tmem_ld_wait();
                 umma::fence_before_thread_sync();
                 __syncwarp();
@@ -1087,10 +1112,9 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
                         if (k < low || k >= high) s[k >> 5][k & 31] = 0xff800000u;
 #pragma unroll
                 for (int k = 0; k < 64; ++k) s[k >> 5][k & 31] = __float_as_uint(exp2_approx(__uint_as_float(s[k >> 5][k & 31])));
-                ok = attn_wait_warp(&b->dp_full[made & 1], made >> 1 & 1, failed, a.report, 5);
-                if (!ok) break;
+                if (!attn_wait_warp(&b->dp_full[made & 1], made >> 1 & 1, failed, a.report, 5)) return false;
                 umma::fence_after_thread_sync();
-                const uint32_t dp = lanes + Shape::kDp + (kKeys ? 0 : (made & 1) * 128) + half * 64;
+                const uint32_t dp = lanes + Columns::dp(made) + half * 64;
                 umma::tmem_ld_32x32(dp, d[0]);
                 umma::tmem_ld_32x32(dp + 32, d[1]);
                 umma::tmem_ld_wait();
@@ -1129,29 +1153,31 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
             float* part = nullptr;
             if (kKeys && a.splits > 1) part = a.parts + (static_cast<int64_t>(w.split) * 2 + half) * a.tk * a.kv_heads * a.dim + at;
             if (w.n > 0) {
-                ok = ok && attn_wait_warp(&b->sums, ended & 1, failed, a.report, 6);
+                if (!attn_wait_warp(&b->sums, ended & 1, failed, a.report, 6)) return false;
                 ++ended;
-                if (ok) {
-                    umma::fence_after_thread_sync();
-                    if (!kKeys) {
-                        const int first = half * 32 * kChunks;
-                        store_row<32 * kChunks>(lanes + first, factor, out + first, a.dim - first, in);
-                    } else if (part != nullptr) {
-                        store_part<64 * kChunks>(lanes + half * 128, factor, part, a.dim, in);
-                    } else {
-                        store_row<64 * kChunks>(lanes + half * 128, factor, out, a.dim, in);
-                    }
-                    umma::fence_before_thread_sync();
-                    __syncwarp();
-                    if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->drained);
+                umma::fence_after_thread_sync();
+                if (!kKeys) {
+                    const int first = half * 32 * kChunks;
+                    store_row<32 * kChunks>(lanes + first, factor, out + first, a.dim - first, in);
+                } else if (part != nullptr) {
+                    store_part<64 * kChunks>(lanes + half * 128, factor, part, a.dim, in);
+                } else {
+                    store_row<64 * kChunks>(lanes + half * 128, factor, out, a.dim, in);
                 }
+                umma::fence_before_thread_sync();
+                __syncwarp();
+                if ((threadIdx.x & 31) == 0) ptx::mbar_arrive(&b->drained);
             } else if (in && (kKeys || half == 0)) {
                 for (int i = 0; i < a.dim; i += 8) {
                     if (part != nullptr) *reinterpret_cast<uint4*>(part + i) = *reinterpret_cast<uint4*>(part + i + 4) = make_uint4(0, 0, 0, 0);
                     else *reinterpret_cast<uint4*>(out + i) = make_uint4(0, 0, 0, 0);
                 }
             }
-        }
+            return true;
+        };
+        BwdWork w;
+        for (int k = 0; next_work(k, w); ++k)
+            if (!(w.keys ? rows(Keys{}, w) : rows(Queries{}, w))) break;
     }
     umma::fence_before_thread_sync();
     __syncthreads();
@@ -1170,7 +1196,6 @@ attention_backward_kernel(const __grid_constant__ CUtensorMap map_kept0, const _
         __syncthreads();
     }
     if (warp == 9) umma::tmem_dealloc(tmem, 512);
-    if (!kKeys) ptx::wait_for_previous_kernel();
 }
 
 // The parts of dK and dV, in their order; rows of no sequence get zeros
@@ -1261,18 +1286,6 @@ template <int kChunks>
 cudaError_t launch_forward(const AttentionArgs& a, cudaStream_t stream) {
     return is_small(a) ? launch_forward<kChunks, 1>(a, stream) : launch_forward<kChunks, 2>(a, stream);
 }
-template <int kChunks, bool kKeys>
-cudaError_t launch_gradient(const AttentionArgs& a, const CUtensorMap& q, const CUtensorMap& d, const CUtensorMap& k, const CUtensorMap& v, cudaStream_t stream) {
-    const void* fn = reinterpret_cast<const void*>(attention_backward_kernel<kChunks, kKeys>);
-    static std::atomic<uint64_t> allowed{0};
-    const cudaError_t err = allow_once(fn, BwdShape<kChunks, kKeys>::kSmem, allowed);
-    if (err != cudaSuccess) return err;
-    const CUtensorMap* maps[4] = {kKeys ? &k : &q, kKeys ? &v : &d, kKeys ? &q : &k, kKeys ? &d : &v};
-    void* params[] = {const_cast<CUtensorMap*>(maps[0]), const_cast<CUtensorMap*>(maps[1]), const_cast<CUtensorMap*>(maps[2]), const_cast<CUtensorMap*>(maps[3]),
-                      const_cast<AttentionArgs*>(&a)};
-    const int64_t ctas = kKeys ? num_blocks(a.tk, a.num_seqs, 128) * a.kv_heads * a.splits : num_blocks(a.tq, a.num_seqs, 128 / a.pack) * (a.heads / a.pack);
-    return launch_dependent(fn, dim3(static_cast<unsigned>(ctas)), dim3(kBwdThreads), params, BwdShape<kChunks, kKeys>::kSmem, stream);
-}
 template <int kChunks>
 cudaError_t launch_backward(AttentionArgs a, cudaStream_t stream) {
     CUtensorMap q, k, v, d;
@@ -1280,12 +1293,17 @@ cudaError_t launch_backward(AttentionArgs a, cudaStream_t stream) {
     if (!make_map(&q, a.q, a.tq, a.heads, a.dim, 128 / a.pack, a.pack) || !make_map(&d, a.d_o, a.tq, a.heads, a.dim, 128 / a.pack, a.pack) || !make_map(&k, a.k, a.tk, a.kv_heads, a.dim, 128) ||
         !make_map(&v, a.v, a.tk, a.kv_heads, a.dim, 128))
         return cudaErrorInvalidValue;
-    void* params[] = {&a};
+    const void* fn = reinterpret_cast<const void*>(attention_backward_kernel<kChunks>);
+    static std::atomic<uint64_t> allowed{0};
+    cudaError_t err = allow_once(fn, BwdShape<kChunks>::kSmem, allowed);
+    if (err != cudaSuccess) return err;
+    const int64_t key_ctas = num_blocks(a.tk, a.num_seqs, 128) * a.kv_heads * a.splits, ctas = key_ctas + num_blocks(a.tq, a.num_seqs, 128 / a.pack) * (a.heads / a.pack);
+    a.key_ctas = static_cast<int>(key_ctas);
+    void *params[] = {&a}, *maps_and_args[] = {&k, &v, &q, &d, &a};
     const int64_t rows = static_cast<int64_t>(a.tq) * a.heads;
-    cudaError_t err = launch_dependent(reinterpret_cast<const void*>(attention_delta_kernel), dim3(static_cast<unsigned>((rows * 16 + kDeltaThreads - 1) / kDeltaThreads)),
-                                       dim3(kDeltaThreads), params, 0, stream);
-    if (err == cudaSuccess) err = launch_gradient<kChunks, true>(a, q, d, k, v, stream);
-    if (err == cudaSuccess) err = launch_gradient<kChunks, false>(a, q, d, k, v, stream);
+    err = launch_dependent(reinterpret_cast<const void*>(attention_delta_kernel), dim3(static_cast<unsigned>((rows * 16 + kDeltaThreads - 1) / kDeltaThreads)), dim3(kDeltaThreads), params, 0,
+                           stream);
+    if (err == cudaSuccess) err = launch_dependent(fn, dim3(static_cast<unsigned>(ctas)), dim3(kBwdThreads), maps_and_args, BwdShape<kChunks>::kSmem, stream);
     if (err == cudaSuccess && a.splits > 1) {
         const int64_t values = static_cast<int64_t>(a.tk) * a.kv_heads * a.dim;
         err = launch_dependent(reinterpret_cast<const void*>(attention_add_kernel), dim3(static_cast<unsigned>((values / 4 + kAddThreads - 1) / kAddThreads)), dim3(kAddThreads), params, 0,

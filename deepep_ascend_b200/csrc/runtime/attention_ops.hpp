@@ -100,6 +100,7 @@ inline std::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor>> attention_b
     if (d_lse.has_value())
         TORCH_CHECK(d_lse->device() == q.device() && d_lse->scalar_type() == at::kFloat && d_lse->is_contiguous() && d_lse->sizes() == lse.sizes(),
                     "the gradient of lse must be like lse, and contiguous");
+    TORCH_CHECK((q.size(0) / 128 + k.size(0) / 128 + 2 * static_cast<int64_t>(in.a.num_seqs)) * q.size(1) < (1ll << 31), "too much work for one launch");
     at::Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(k.sizes(), k.options());
     if (q.numel() == 0 || k.numel() == 0 || in.a.num_seqs == 0) return std::make_tuple(dq.zero_(), dk.zero_(), dv.zero_());
     const at::Tensor d16 = heads_of(d_o), o16 = heads_of(o);

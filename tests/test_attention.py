@@ -166,6 +166,26 @@ def test_what_lies_behind_the_sequences_is_not_looked_at(D, device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('H,Hk,D', [(14, 2, 128), (6, 6, 64), (22, 2, 32)])
+def test_sequences_do_not_reach_one_another(H, Hk, D, device='cuda'):
+    """One that holds no numbers anywhere, between others that share its tiles: theirs, results and gradients, keep their bits."""
+    lq, lk = [100, 50, 1, 290], [100, 61, 1, 290]
+    q, k, v, d_o, d_lse = _make(441, 452, H, Hk, D, 15, device)
+    cq, ck = _cu(lq, device), _cu(lk, device)
+    kept = attention(q, k, v, cq, ck)
+    want = attention_backward(d_o, q, k, v, *kept, cq, ck, d_lse=d_lse)
+    bad = [t.clone() for t in (q, k, v, d_o)]
+    for t, a, n in zip(bad, (100, 100, 100, 100), (50, 61, 61, 50)):
+        t[a:a + n] = float('nan')
+    o, lse = attention(*bad[:3], cq, ck)
+    grads = attention_backward(bad[3], *bad[:3], o, lse, cq, ck, d_lse=d_lse)
+    rows, keys = (torch.cat([torch.arange(100), torch.arange(100 + n, 391 + n)]).to(device) for n in (50, 61))
+    assert torch.equal(o[rows], kept[0][rows]) and torch.equal(lse[:, rows], kept[1][:, rows])
+    assert all(torch.equal(a[i], b[i]) for a, b, i in zip(grads, want, (rows, keys, keys)))
+    assert o[100:150].isnan().all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('cu_q,cu_k', [([9, 40, 100], [30, 80, 120]), ([0, 400, 100], [0, 50, 900]), ([0, 50, 30], [0, 90, 20]), ([-5, 30, 100], [0, 50, 120])])
 def test_bounds_that_are_out_of_order_stay_inside(cu_q, cu_k):
     """Gaps in front give zeros; whatever the bounds are, nothing outside the tensors is read or written."""

@@ -59,3 +59,29 @@ def test_every_device_spin_is_bounded():
                 if not re.search(r'timeout_ns|kWaitLimitNs|globaltimer|gemm_timer|limit', window):
                     offenders.append('%s:%d' % (p.name, i + 1))
     assert not offenders, offenders
+
+
+def test_dependent_kernels_wait_before_they_read():
+    """What a kernel may read of earlier ones is promised to the grid that waits: every kernel that uses the pair waits by itself, whatever its template arguments are, before it lets the next one
+    start and before it calls for anything in global memory (setup of barriers and tensor memory may come first)."""
+    checked = 0
+    for p in (REPO / 'deepep_ascend_b200' / 'csrc' / 'kernels').glob('*.cu'):
+        text = re.sub(r'//[^\n]*', '', p.read_text())
+        for m in re.finditer(r'__global__', text):
+            start = text.index('{', text.index(')', text.index('const __grid_constant__', m.end())) if 'const __grid_constant__' in text[m.end():m.end() + 400] else m.end())
+            depth, end = 1, start + 1
+            while depth:
+                depth += {'{': 1, '}': -1}.get(text[end], 0)
+                end += 1
+            body = text[start + 1:end - 1]
+            waits = [w.start() for w in re.finditer(r'wait_for_previous_kernel\(\)', body)]
+            if not waits and 'let_next_kernel_start' not in body:
+                continue
+            checked += 1
+            first = min(waits, default=0)
+            line = body[body.rfind('\n', 0, first) + 1:body.find('\n', first)].strip()
+            assert waits and line == 'ptx::wait_for_previous_kernel();', (p.name, line)
+            assert body[:first].count('{') == body[:first].count('}'), (p.name, 'the wait is conditional')
+            assert 'let_next_kernel_start' not in body[:first], p.name
+            assert not re.search(r'\bnext_work\(|\btma_load|\bload8\b|->data', body[:first]), p.name
+    assert checked > 10
