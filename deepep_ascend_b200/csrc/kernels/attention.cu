@@ -185,14 +185,15 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     return d;
 }
 constexpr float kNone = -__builtin_huge_valf();
+// (a NaN if one of them is)
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 // 2^x of a pair without the special function unit, which makes 16 a clock of an SM and would be what the softmax waits for: x = n + f with n the nearest whole number, 2^f
-// by a polynomial of degree 4 (relative error 2.8e-6, least largest error on [-1/2, 1/2] with a constant of exactly 1, so that -127 and below give exactly 0), n added
-// to the exponent.  A NaN stays one or becomes an infinity.
+// by a polynomial of degree 4 (relative error 2.87e-6, least largest error on [-1/2, 1/2] with a constant of exactly 1, so that -127 and below give exactly 0), n added
+// to the exponent.  A NaN may become any number: a row that has one is told by its largest score.
 __device__ __forceinline__ uint64_t exp2_by_polynomial(uint64_t x2) {
     float x, y;
     umma::unpack_f32x2(x2, x, y);
@@ -620,14 +621,15 @@ attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
                     top[i] = max3(value(0), value(1), value(2));
 #pragma unroll
                     for (int k = 3; k < 15; k += 2) top[i] = max3(top[i], value(k), value(k + 1));
-                    top[i] = fmaxf(top[i], value(15));
+                    top[i] = max3(top[i], value(15), value(15));
                 }
-                const float largest = fmaxf(max3(max3(top[0], top[1], top[2]), top[3], top[4]), max3(top[5], top[6], top[7]));
+                const float largest = max3(max3(max3(top[0], top[1], top[2]), top[3], top[4]), max3(top[5], top[6], top[7]), kNone);
                 // The reference moves only when the largest score is more than 2^8 above it: sums and probabilities have that much room, and O is seldom multiplied.
+                // With a score that is no number the reference is none either, and so are the row's sum, result and lse.
                 if (j == 0) {
                     ref = largest == kNone ? 0.f : largest;
                 } else {
-                    const bool move = (largest - ref) * c > 8.f;
+                    const bool move = !((largest - ref) * c <= 8.f);
                     if (__any_sync(0xffffffffu, move)) {
                         const float factor = move ? exp2_approx((ref - largest) * c) : 1.f;
                         sum *= factor;

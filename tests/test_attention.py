@@ -185,6 +185,20 @@ def test_sequences_do_not_reach_one_another(H, Hk, D, device='cuda'):
     assert o[100:150].isnan().all()
 
 
+@pytest.mark.parametrize('H,n,device', [(2, 300, 'cpu'), pytest.param(2, 300, 'cuda', marks=pytest.mark.gpu), pytest.param(56, 2200, 'cuda', marks=pytest.mark.gpu)])
+def test_a_key_that_is_no_number(H, n, device):
+    """Wherever it stands, who sees it gets no numbers, in both results; who does not keeps what there was."""
+    q, k, v, _, _ = _make(n, n, H, 1, 64, 16, device)
+    o, lse = attention(q, k, v)
+    for at in [*range(16, 24), 130, 135, 255, n - 1]:
+        for bad in (float('nan'), float('inf')):
+            x = k.clone()
+            x[at] = bad if bad != bad else (x[at].sign() * bad)      # (products of both signs: their sum is no number)
+            got = attention(q, x, v)
+            assert got[0][at:].isnan().all() and got[1][:, at:].isnan().all(), (at, bad)
+            assert torch.equal(got[0][:at], o[:at]) and torch.equal(got[1][:, :at], lse[:, :at])
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('cu_q,cu_k', [([9, 40, 100], [30, 80, 120]), ([0, 400, 100], [0, 50, 900]), ([0, 50, 30], [0, 90, 20]), ([-5, 30, 100], [0, 50, 120])])
 def test_bounds_that_are_out_of_order_stay_inside(cu_q, cu_k):
