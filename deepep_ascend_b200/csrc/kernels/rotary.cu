@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kRotaryThreads, kBackwardCtas) rotary_backward
         const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarps, share = (units + warps - 1) / warps;
         const int64_t begin = (static_cast<int64_t>(blockIdx.x) * kWarps + warp) * share, end = min(begin + share, units);
         Eight<T> x[kIters] = {}, d[kIters] = {}, next_x[kIters] = {}, next_d[kIters] = {};
-        int64_t token = begin / chunks, next_token = token;
+        int64_t token = begin / max(chunks, 1), next_token = token;      // (no chunks: no heads of this kind)
         int chunk = static_cast<int>(begin - token * chunks), next_chunk = chunk;
         auto request = [&]() {
 #pragma unroll
@@ -429,7 +429,7 @@ cudaError_t launch_rotary(const RotaryArgs& a, int num_sms, cudaStream_t stream)
 
 int rotary_backward_ctas(const RotaryArgs& a, int num_sms) {
     const int heads_per_unit = backward_iters(a.x_bf16 ? 2 : 4) * 32 / lanes_of(a.dim);
-    const int64_t units = static_cast<int64_t>(a.tokens) * ((a.heads[0] + heads_per_unit - 1) / heads_per_unit);
+    const int64_t units = std::max<int64_t>(static_cast<int64_t>(a.tokens) * ((std::max(a.heads[0], a.heads[1]) + heads_per_unit - 1) / heads_per_unit), 1);
     return static_cast<int>(std::min<int64_t>((units * 32 + kRotaryThreads - 1) / kRotaryThreads, num_sms * kBackwardCtas));
 }
 cudaError_t launch_rotary_backward(const RotaryArgs& a, cudaStream_t stream) {

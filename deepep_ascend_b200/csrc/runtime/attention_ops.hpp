@@ -241,7 +241,7 @@ inline std::optional<std::tuple<at::Tensor, at::Tensor>> qk_norm_rope(const at::
     const c10::cuda::CUDAGuard guard(q.device());
     RotaryInputs in = rotary_inputs(q, k, q_weight, k_weight, table, positions, eps, interleaved);
     at::Tensor yq = at::empty(q.sizes(), q.options()), yk = at::empty(k.sizes(), k.options());
-    if (q.size(0) == 0) return std::make_tuple(yq, yk);
+    if (q.numel() == 0 && k.numel() == 0) return std::make_tuple(yq, yk);
     in.a.out[0] = yq.data_ptr();
     in.a.out[1] = yk.data_ptr();
     cuda_check(ep::launch_rotary(in.a, device_sms(), at::cuda::getCurrentCUDAStream()), "rotation launch");
@@ -262,7 +262,7 @@ inline std::optional<std::tuple<at::Tensor, std::optional<at::Tensor>>> qk_norm_
     at::Tensor yq = at::empty(q.sizes(), q.options());
     std::optional<at::Tensor> yk;
     if (keep_k) yk = at::empty(k.sizes(), k.options());
-    if (q.size(0) == 0) return std::make_tuple(yq, yk);
+    if (q.numel() == 0 && k.numel() == 0) return std::make_tuple(yq, yk);
     const at::Tensor v16 = heads_of(v), s = slots.contiguous();
     RotaryArgs& a = in.a;
     a.out[0] = yq.data_ptr();
@@ -291,7 +291,7 @@ inline std::optional<RotaryGradients> qk_norm_rope_backward(const at::Tensor& dq
                     dk.sizes() == k.sizes(), "gradients must be like q and k");
     at::Tensor dx = at::empty(q.sizes(), q.options()), dy = at::empty(k.sizes(), k.options());
     at::Tensor dqw = at::empty(q_weight.sizes(), q_weight.options()), dkw = at::empty(k_weight.sizes(), k_weight.options());
-    if (q.size(0) == 0) return RotaryGradients(dx, dy, dqw.zero_(), dkw.zero_());
+    if (q.numel() == 0 && k.numel() == 0) return RotaryGradients(dx, dy, dqw.zero_(), dkw.zero_());
     const at::Tensor dq16 = heads_of(dq), dk16 = heads_of(dk);
     RotaryArgs& a = in.a;
     a.dy[0] = view_of(dq16);

@@ -242,6 +242,30 @@ def test_in_two_graphs():
         assert all(torch.equal(a, b) for a, b in zip(out, ref))
 
 
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('Hq,Hk', [(0, 3), (3, 0), (0, 0)])
+@pytest.mark.parametrize('T', [4, 700])
+def test_without_heads(T, Hq, Hk, device):
+    """Of one kind, or of both: the other one's results and gradients are what they are beside heads."""
+    given, qw, kw, table, positions = _make(T, 3, 3, 64, 32, BF16, F32, 17, device)
+    want = qk_norm_rope(given['q'], given['k'], qw, kw, table, positions)
+    grads = qk_norm_rope_backward(given['dq'], given['dk'], given['q'], given['k'], qw, kw, table, positions)
+    q, dq, k, dk = given['q'][:, :Hq], given['dq'][:, :Hq], given['k'][:, :Hk], given['dk'][:, :Hk]
+    out = qk_norm_rope(q, k, qw, kw, table, positions)
+    assert torch.equal(out[0], want[0][:, :Hq]) and torch.equal(out[1], want[1][:, :Hk])
+    got = qk_norm_rope_backward(dq, dk, q, k, qw, kw, table, positions)
+    assert torch.equal(got[0], grads[0][:, :Hq]) and torch.equal(got[1], grads[1][:, :Hk])
+    # (the weights' sums may be in another order: of 64 rows in 32 bits, or 3 T)
+    for x, y, H in ((got[2], grads[2], Hq), (got[3], grads[3], Hk)):
+        assert not x.any() if H == 0 else torch.allclose(x, y, rtol=0, atol=(3 * T + 64) * EPS * 3 * T * 16)
+    behind = torch.full_like(positions, 10**6)
+    got = qk_norm_rope_backward(dq, dk, q, k, qw, kw, table, behind)
+    assert all(not x.any() if H == 0 else x.isnan().all() for x, H in ((got[2], Hq), (got[3], Hk)))
+    k_cache, v_cache = _caches(T, 1, Hk, 64, BF16, device, 'plain')
+    append = qk_norm_rope_append(q, k, k, qw, kw, table, positions, k_cache, v_cache, torch.arange(T, device=device), keep_k=True)
+    assert all(torch.equal(a, b) for a, b in zip(append, out)) and torch.equal(k_cache[:, 0], out[1])
+
+
 @pytest.mark.gpu
 def test_nothing_to_do():
     given, qw, kw, table, positions = _make(4, 2, 1, 64, 64, BF16, F32, 8, 'cuda')
