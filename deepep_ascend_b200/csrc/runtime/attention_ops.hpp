@@ -1,5 +1,7 @@
 // Tensor front end of the attention half of a layer: argument checks, result tensors, launches on the current stream.
 #pragma once
+#include <cmath>
+
 #include "block_ops.hpp"
 
 namespace ep_host {
@@ -27,6 +29,12 @@ inline void report_through(NsReport& report, at::Tensor& error, ElasticBufferCor
     }
 }
 
+// Scores are multiplied by scale log2 e in 32 bits: with zero there, those that are hidden (-inf) would be no numbers
+inline void check_scale(double scale) {
+    const float s = static_cast<float>(scale);
+    TORCH_CHECK(s > 0 && std::isnormal(s) && std::isfinite(s * 1.5f), "scale must be positive, and neither too small nor too large for 32 bits");
+}
+
 struct PackedInputs {
     at::Tensor q, k, v;                // as the kernels read them
     AttentionArgs a{};
@@ -39,7 +47,7 @@ inline PackedInputs packed_inputs(const at::Tensor& q, const at::Tensor& k, cons
     TORCH_CHECK(q.size(2) >= 8 && q.size(2) <= 128 && q.size(2) % 8 == 0, "heads must have 8 to 128 channels, a multiple of 8");
     TORCH_CHECK(k.size(1) >= 1 && q.size(1) >= 1 && q.size(1) % k.size(1) == 0, "the heads of q must be a multiple of those of k");
     TORCH_CHECK(q.size(0) < (1ll << 30) && k.size(0) < (1ll << 30) && q.size(1) < (1 << 16), "too many tokens or heads");
-    TORCH_CHECK(std::isfinite(scale) && scale > 0, "scale must be positive");
+    check_scale(scale);
     TORCH_CHECK(cu_q.has_value() == cu_k.has_value(), "cu_seqlens of queries and keys go together");
     PackedInputs in;
     AttentionArgs& a = in.a;
@@ -151,7 +159,7 @@ inline at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache
     TORCH_CHECK(lengths.device() == q.device() && lengths.scalar_type() == at::kInt && lengths.dim() == 1 && lengths.size(0) == B && lengths.is_contiguous(),
                 "lengths must be contiguous int32 [sequences] on the device of q");
     TORCH_CHECK(page_table.size(1) * k_cache.size(1) < (1ll << 31) - 65536 && B * (page_table.size(1) * k_cache.size(1) / 16 + 1) < (1ll << 31), "too many places in page_table");
-    TORCH_CHECK(std::isfinite(scale) && scale > 0, "scale must be positive");
+    check_scale(scale);
     at::Tensor o = out.has_value() ? *out : at::empty(q.sizes(), q.options());
     TORCH_CHECK(o.device() == q.device() && o.scalar_type() == at::kBFloat16 && o.is_contiguous() && o.sizes() == q.sizes() && reinterpret_cast<uintptr_t>(o.data_ptr()) % 16 == 0,
                 "out must be contiguous bf16 of q's shape, on 16 bytes");

@@ -21,7 +21,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Opt
               causal: bool = True, scale: Optional[float] = None, buffer=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """``q [tokens, heads, dim]``, ``k`` and ``v [keys, kv_heads, dim]`` (bf16, ``dim`` a multiple of 8, at most 128) -> ``(o`` like ``q``, contiguous,
     ``lse`` fp32 ``[heads, tokens])``: ``o = softmax(scale q k^T) v`` and ``lse = log sum exp(scale q k^T)`` within each sequence.  ``heads`` is a multiple of
-    ``kv_heads``: as many neighbouring heads share keys and values.  ``scale``: ``dim ** -0.5`` if none is given, positive.
+    ``kv_heads``: as many neighbouring heads share keys and values.  ``scale``: ``dim ** -0.5`` if none is given, positive (a normal number of 32 bits).
 
     ``cu_seqlens`` int32 ``[sequences + 1]``: where the sequences start in ``q``, and where the last one ends; none: one sequence.  ``cu_seqlens_k``: the same of ``k``
     and ``v``, if their lengths are others (keys of earlier calls in front).  With ``causal`` both of a sequence end together: query ``i`` of ``n`` sees the keys up to

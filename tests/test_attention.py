@@ -403,6 +403,13 @@ def test_nothing_to_do():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('scale', [1e-50, 1e-39, 3e38, 1e300, -1.0, float('nan')])
+def test_scales_that_32_bits_do_not_hold(scale):
+    with pytest.raises(RuntimeError, match='scale'):
+        attention(*_make(10, 10, 2, 1, 64, 0, 'cuda')[:3], scale=scale)
+
+
+@pytest.mark.gpu
 def test_refusals():
     q, k, v, d_o, d_lse = _make(10, 10, 4, 2, 64, 0, 'cuda')
     cu = _cu([10], 'cuda')

@@ -211,6 +211,13 @@ def test_a_gradient_goes_through_the_statement():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('scale', [1e-50, 1e-39, 3e38, 1e300, -1.0, float('nan')])
+def test_scales_that_32_bits_do_not_hold(scale):
+    with pytest.raises(RuntimeError, match='scale'):
+        paged_attention(*_make([20], 4, 2, 64, 16, 12, 'cuda'), scale)
+
+
+@pytest.mark.gpu
 def test_refusals():
     q, k, v, table, lengths = _make([20, 30], 4, 2, 64, 16, 12, 'cuda')
     ok = dict(q=q, k_cache=k, v_cache=v, page_table=table, lengths=lengths)
