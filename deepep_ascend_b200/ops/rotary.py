@@ -85,9 +85,12 @@ def _wide(t: torch.Tensor) -> torch.Tensor:
 def _angles(table, positions, like):
     """Cosines and sines of every token (``[T, 1, R / 2]``), and whether its position is in front of the table and in it (``[T, 1, 1]``)."""
     at = positions.long()
+    inside = at < table.shape[0]
+    if table.shape[0] == 0:                                          # (any row: nobody is in it)
+        table = table.new_zeros(1, table.shape[1])
     rows = table[at.clamp(0, table.shape[0] - 1)].to(_wide(like).dtype).unsqueeze(1)
     half = table.shape[1] // 2
-    return rows[..., :half], rows[..., half:], (at < 0)[:, None, None], (at < table.shape[0])[:, None, None]
+    return rows[..., :half], rows[..., half:], (at < 0)[:, None, None], inside[:, None, None]
 
 
 def _turn(x, cos, sin, interleaved):

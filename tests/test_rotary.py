@@ -266,6 +266,17 @@ def test_without_heads(T, Hq, Hk, device):
     assert all(torch.equal(a, b) for a, b in zip(append, out)) and torch.equal(k_cache[:, 0], out[1])
 
 
+@pytest.mark.parametrize('device', DEVICES)
+def test_a_table_without_positions(device):
+    """Nobody has one: no numbers, and zeros for padding."""
+    given, qw, kw, table, positions = _make(4, 2, 1, 64, 64, BF16, F32, 8, device)
+    positions[2] = -1
+    rest = [0, 1, 3]
+    for t in (*qk_norm_rope(given['q'], given['k'], qw, kw, table[:0], positions),
+              *qk_norm_rope_backward(given['dq'], given['dk'], given['q'], given['k'], qw, kw, table[:0], positions)[:2]):
+        assert t[rest].isnan().all() and not t[2].any()
+
+
 @pytest.mark.gpu
 def test_nothing_to_do():
     given, qw, kw, table, positions = _make(4, 2, 1, 64, 64, BF16, F32, 8, 'cuda')
