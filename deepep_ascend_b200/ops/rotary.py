@@ -70,7 +70,8 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_wei
 
     ``k_cache`` and ``v_cache [pages, page_size, kv_heads, dim]``: of the heads' type, one layout, channels contiguous, heads on 16 bytes (views of one
     allocation, or with the heads in front of the places, are as good).  Token ``t`` goes to place ``slots[t] % page_size`` of page ``slots[t] // page_size`` (int64 or int32); tokens whose
-    slot is not in the caches go nowhere.  Slots that several tokens name hold one of them.  What is in the caches carries no gradient."""
+    slot is not in the caches go nowhere.  What a place holds that several tokens name is not said.  What is in the caches carries no gradient; where
+    the queries are to carry one (or the keys beside them), and for whoever watches, the PyTorch statement runs."""
     if q.is_cuda and _by_type(q, k, v, q_weight, k_weight, table, positions, k_cache, v_cache, slots):
         res = _native.load().qk_norm_rope_append(q, k, v, q_weight, k_weight, table, positions, k_cache, v_cache, slots, eps, interleaved, keep_k)
         if res is not None:
@@ -130,8 +131,12 @@ def qk_norm_rope_append_ref(q, k, v, q_weight, k_weight, table, positions, k_cac
     """:func:`qk_norm_rope_append` stated with plain PyTorch operations."""
     q, k = qk_norm_rope_ref(q, k, q_weight, k_weight, table, positions, eps, interleaved)
     pages, size = k_cache.shape[:2]
-    keep = ((slots >= 0) & (slots < pages * size)).nonzero().squeeze(-1)
-    at = slots[keep].long()
-    for cache, new in ((k_cache, k), (v_cache, v)):
-        cache[at // size, at % size] = new[keep].detach()
+    if pages * size > 0 and slots.shape[0] > 0:
+        # (in shapes that do not depend on the slots: tokens without a place write what one that has one writes or, where nobody has, what stands in the first place)
+        keep = (slots >= 0) & (slots < pages * size)
+        some, one = keep.any(), keep.int().argmax(0, keepdim=True)
+        at = torch.where(keep, slots.long(), torch.where(some, slots.long().index_select(0, one), 0))
+        for cache, new in ((k_cache, k), (v_cache, v)):
+            new = new.detach()
+            cache[at // size, at % size] = torch.where(keep[:, None, None], new, torch.where(some, new.index_select(0, one), cache[:1, 0]))
     return (q, k) if keep_k else q

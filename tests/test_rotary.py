@@ -163,6 +163,49 @@ def test_caches_without_pages(keep_k, device):
         assert torch.equal(out[0] if keep_k else out, want[0]) and (not keep_k or torch.equal(out[1], want[1]))
 
 
+@pytest.mark.parametrize('slots', [[3, -1, 40, 0, 31, -5], [-1, 32, 99, -2, 40, 50], [7, 6, 5, 4, 3, 2], [-1, -1, -1, -1, -1, 9]])
+@pytest.mark.parametrize('device', DEVICES)
+def test_the_statement_appends_without_looking(slots, device):
+    """Its shapes do not depend on the slots, and nobody waits for them: on a GPU it can be captured into a graph, with gradients to carry as well."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+    given, qw, kw, table, positions = _make(6, 3, 2, 32, 16, F32, F32, 18, device)
+    leaf = given['q'].clone().requires_grad_(True)
+    at, caches = torch.full((6,), -1, device=device), _caches(2, 16, 2, 32, F32, device, 'fused')
+
+    def f(at, k_cache, v_cache):
+        return R.qk_norm_rope_append(leaf, given['k'], given['dk'], qw, kw, table, positions, k_cache, v_cache, at)
+
+    class Seen(TorchDispatchMode):
+        names = set()
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.add(func.overloadpacket.__name__)
+            return func(*args, **(kwargs or {}))
+    with Seen() as seen:
+        f(at, *caches)
+    assert not seen.names & {'nonzero', '_local_scalar_dense', 'item'} and 'index_put_' in seen.names
+    want = [c.clone().view(32, 2, 32) for c in caches]
+    for i, s in enumerate(slots):
+        if 0 <= s < 32:
+            want[0][s], want[1][s] = qk_norm_rope(given['q'], given['k'], qw, kw, table, positions)[1][i], given['dk'][i]
+    if device == 'cuda':
+        f(at, *caches)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = f(at, *caches)
+        at.copy_(torch.tensor(slots))
+        graph.replay()
+    else:
+        at.copy_(torch.tensor(slots))
+        out = f(at, *caches)
+    assert out.requires_grad
+    # (two ways to the same norm in 32 bits)
+    assert torch.allclose(caches[0].reshape(32, 2, 32), want[0], rtol=1e-5, atol=1e-5) and torch.equal(caches[1].reshape(32, 2, 32), want[1])
+    assert all(torch.equal(c[~hit], torch.full_like(c[~hit], 7.0)) for c in (x.reshape(32, 2, 32) for x in caches)
+               for hit in [torch.tensor([p in slots for p in range(32)], device=device)])
+
+
 @pytest.mark.gpu
 def test_strides_and_alignment():
     given, qw, kw, table, positions = _make(37, 6, 2, 96, 64, BF16, F32, 3, 'cuda')
