@@ -132,6 +132,11 @@ inline std::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor>> attention_b
     return std::make_tuple(dq, dk, dv);
 }
 
+// A caller's tensor has been written: who keeps it for a gradient hears of it, as of any operation in place
+inline void note_written(const at::Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // What paged caches [pages, page_size, kv_heads, dim] have to be
 inline void check_caches(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& like, at::ScalarType type) {
     for (const at::Tensor* t : {&k_cache, &v_cache})
@@ -191,6 +196,7 @@ inline at::Tensor paged_attention(const at::Tensor& q, const at::Tensor& k_cache
         a.parts = reinterpret_cast<float*>(parts.data_ptr());
     }
     cuda_check(ep::launch_paged_attention(a, device_sms(), at::cuda::getCurrentCUDAStream()), "paged attention launch");
+    if (out.has_value()) note_written(o);
     return o;
 }
 
@@ -287,6 +293,8 @@ inline std::optional<std::tuple<at::Tensor, std::optional<at::Tensor>>> qk_norm_
     a.slots = s.data_ptr();
     a.slots_64 = s.scalar_type() == at::kLong;
     cuda_check(ep::launch_rotary(a, device_sms(), at::cuda::getCurrentCUDAStream()), "rotation launch");
+    note_written(k_cache);
+    note_written(v_cache);
     return std::make_tuple(yq, yk);
 }
 using RotaryGradients = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;

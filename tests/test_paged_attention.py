@@ -201,6 +201,19 @@ def test_it_is_seen(tracer, device):
         assert torch.allclose(out.reshape(q.shape).float(), f(q).float(), rtol=8 * HALF, atol=8 * HALF)
 
 
+@pytest.mark.parametrize('device', DEVICES)
+def test_a_result_that_a_gradient_needs(device):
+    """Whoever kept what is given for the result hears that it has been written."""
+    args = _make([20, 3], 2, 1, 16, 8, 10, device)
+    out, w = torch.zeros_like(args[0]), torch.ones((), device=device, requires_grad=True)
+    y = (out * w).sum()
+    assert paged_attention(*args, out=out) is out or out.any()
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.backward()
+    with torch.inference_mode():
+        assert torch.equal(paged_attention(*args, out=torch.zeros_like(out)), out)
+
+
 @pytest.mark.gpu
 def test_a_gradient_goes_through_the_statement():
     q, k, v, table, lengths = _make([20, 3], 2, 1, 16, 8, 11, 'cuda')

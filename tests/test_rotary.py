@@ -206,6 +206,25 @@ def test_the_statement_appends_without_looking(slots, device):
                for hit in [torch.tensor([p in slots for p in range(32)], device=device)])
 
 
+@pytest.mark.parametrize('device', DEVICES)
+@pytest.mark.parametrize('layout', ['plain', 'fused'])
+def test_caches_that_a_gradient_needs(layout, device):
+    """Whoever kept them hears that they have been written; inference tensors have nobody to tell."""
+    given, qw, kw, table, positions = _make(4, 2, 1, 32, 16, F32, F32, 19, device)
+    args = given['q'], given['k'], given['dk'], qw, kw, table, positions
+    for which in range(2):
+        caches = _caches(2, 16, 1, 32, F32, device, layout)
+        w = torch.ones((), device=device, requires_grad=True)
+        y = (caches[which] * w).sum()
+        qk_norm_rope_append(*args, *caches, torch.arange(4, device=device))
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            y.backward()
+    with torch.inference_mode():
+        caches = _caches(2, 16, 1, 32, F32, device, layout)
+        qk_norm_rope_append(*args, *caches, torch.arange(4, device=device))
+        assert (caches[0][0, :4] != 7).all() and torch.equal(caches[1][0, :4], given['dk'])
+
+
 @pytest.mark.gpu
 def test_strides_and_alignment():
     given, qw, kw, table, positions = _make(37, 6, 2, 96, 64, BF16, F32, 3, 'cuda')
