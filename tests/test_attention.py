@@ -200,6 +200,30 @@ def test_a_key_that_is_no_number(H, n, device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('H', [1, 512])
+def test_powers(H):
+    """2^x of the keys whose powers go by a polynomial, seen in lse: 128 keys of score 0, which the reference stays at, and of the 128 behind them those 32 with score x, the others far below.
+
+    x is exact in bf16 halves, its product with scale log2 e off by 2^-23 of it, the polynomial by 2.9e-6; the sum of 160 terms, its logarithm and their product by 2^-24 of their size each."""
+    x = torch.cat([torch.arange(-160, -20) + 0.3125, torch.arange(-20 * 128, 8 * 128 - 1) / 128]).double()
+    tokens = x.numel()
+    high = x.bfloat16().double()
+    low = (x - high).bfloat16().double()
+    assert (high + low == x).all()
+    q, k = torch.zeros(tokens, H, 8), torch.zeros(256, 1, 8)
+    q[:, :, 0], q[:, :, 1], q[:, :, 2] = high[:, None], low[:, None], 1.0
+    by_polynomial = torch.arange(128) % 8 >= 6
+    k[128:][by_polynomial, :, :2] = 1.0
+    k[128:][~by_polynomial, :, 2] = -1000.0
+    scale = float(torch.tensor(2.0).log())
+    lse = attention(q.bfloat16().cuda(), k.bfloat16().cuda(), torch.ones(256, 1, 8, dtype=BF16, device='cuda'), causal=False, scale=scale)[1].double().cpu()
+    part = 32 * 2.0**x
+    want = torch.log(128 + part)
+    err = part / (128 + part) * (2.9e-6 + x.abs() * 2.0**-23) + 8 * 2.0**-24 * (1 + want) + 160 * 2.0**-24
+    assert ((lse - want).abs() <= err).all(), float(((lse - want).abs() - err).max())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('cu_q,cu_k', [([9, 40, 100], [30, 80, 120]), ([0, 400, 100], [0, 50, 900]), ([0, 50, 30], [0, 90, 20]), ([-5, 30, 100], [0, 50, 120])])
 def test_bounds_that_are_out_of_order_stay_inside(cu_q, cu_k):
     """Gaps in front give zeros; whatever the bounds are, nothing outside the tensors is read or written."""

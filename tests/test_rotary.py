@@ -226,6 +226,27 @@ def test_caches_that_a_gradient_needs(layout, device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('layout', ['plain', 'heads first'])
+@pytest.mark.parametrize('T,Hq,Hk,D,rotary,dtype', [(900, 33, 11, 128, 128, BF16), (1600, 33, 11, 64, 32, BF16), (600, 33, 11, 256, 256, BF16), (600, 14, 10, 192, 96, F32), (3, 5, 2, 192, 192, BF16),
+                                                    (2, 4, 1, 256, 64, F32)])
+def test_prompts_into_paged_caches(T, Hq, Hk, D, rotary, dtype, layout):
+    """Enough rows that a warp takes several at once, heads that do not divide by them, and the widest heads."""
+    given, qw, kw, table, positions = _make(T, Hq, Hk, D, rotary, dtype, F32, T, 'cuda')
+    q, k = qk_norm_rope(given['q'], given['k'], qw, kw, table, positions)
+    _check(given, qw, kw, table, positions, False)
+    pages, size = T // 48 + 3, 48
+    k_cache, v_cache = _caches(pages, size, Hk, D, dtype, 'cuda', layout)
+    slots = torch.randperm(pages * size, generator=torch.Generator().manual_seed(T))[:T].cuda()
+    slots[1] = -1
+    out = qk_norm_rope_append(given['q'], given['k'], given['dk'], qw, kw, table, positions, k_cache, v_cache, slots, keep_k=True)
+    assert torch.equal(out[0], q) and torch.equal(out[1], k)
+    for cache, new in ((k_cache, k), (v_cache, given['dk'])):
+        want = torch.full((pages * size, Hk, D), 7.0, dtype=dtype, device='cuda')
+        want[slots[slots >= 0]] = new[slots >= 0]
+        assert torch.equal(cache.reshape(-1, Hk, D), want)
+
+
+@pytest.mark.gpu
 def test_strides_and_alignment():
     given, qw, kw, table, positions = _make(37, 6, 2, 96, 64, BF16, F32, 3, 'cuda')
     want = qk_norm_rope(given['q'], given['k'], qw, kw, table, positions)
