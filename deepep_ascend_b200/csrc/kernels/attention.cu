@@ -46,7 +46,7 @@ __device__ __noinline__ void attn_fail(const NsReport& r, int* failed, int code)
         __threadfence_system();
     }
 }
-// code: 1 free stage, 2 probabilities, 4 full stage, 5 scores, 6 sums
+// code: 1 free stage, 2 probabilities, 3 scores that have been read, 4 full stage, 5 scores, 6 sums and statistics, 7 work
 __device__ __forceinline__ bool attn_wait(uint64_t* bar, uint32_t parity, int* failed, const NsReport& r, int code) {
     if (ptx::mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns(), limit = r.timeout_ns != 0 ? r.timeout_ns : kAttnWaitLimitNs;
@@ -282,13 +282,13 @@ __device__ __forceinline__ void store_part(uint32_t tmem, float factor, float* r
 // queries, keys and values come while the last one's results leave.  Blocks differ in length, so who takes which is decided as they end.  (31 prompts of 264 tokens, 56 heads of 128: 268 us with
 // a CTA for every block, 150 so at the time.)
 //
-// Long sequences are bound by power: 16384 tokens, 56 heads of 128, 3.0 to 3.4 ms, 1.1 to 1.3 PFLOP/s at SM clocks of 1.4 to 1.55 GHz, the tensor pipe busy in 67 % of them.  What the clocks go by is the
+// Long sequences are bound by power: 16384 tokens, 56 heads of 128, 3.0 to 3.5 ms, 1.1 to 1.3 PFLOP/s at SM clocks of 1.4 to 1.55 GHz, the tensor pipe busy in 67 % of them.  What the clocks go by is the
 // chain of a tile's block of 128 keys, some 3000 of which two tiles share: 70 for the scores into registers, 370 for their largest, 1050 for the powers, 100 for their way back, 512 + 512 for
 // the products and as much for the barriers between, which lie in the shared memory that the products read at its full rate.  So a quarter of the powers by polynomial, the first half of
 // the probabilities handed over early and an issuing thread for each tile took it from 3650 clocks to 3030.
 // Small tasks have one tile per CTA and two CTAs on an SM, one of which works while the other begins or ends a block; two tiles read keys and values from L2 once for both.
 // That tile takes the heads of a group together, each of as many queries as fill 128 rows (7 heads: 18), so that few rows stay empty where a sequence ends: 31 prompts of 264 tokens
-// 125 -> 90 us, 200 of 30 tokens (32 heads) 97 -> 46, 8 of 1000 152 either way.
+// 125 -> 90 us (to 103 on other GPUs), 200 of 30 tokens (32 heads) 97 -> 46, 8 of 1000 152 either way.
 constexpr int kPackedHeads = 16;
 template <int kChunks, int kTiles>
 struct FwdShape {
@@ -733,8 +733,8 @@ __global__ void __launch_bounds__(kDeltaThreads) attention_delta_kernel(const __
 // tensor memory until the end: every gradient is added by one CTA (or by one per part of the group, whose parts are then added), in a fixed order.  P is made twice, which
 // costs two products of seven, and spares sums of dQ in memory by many CTAs in any order.
 //
-// 16384 tokens, 56 heads of 128: 11.5 ms, 0.84 PFLOP/s counted as five products and 1.17 as seven, bound by power as the forward pass; two documents of 4096: 1.4 to 1.6 ms.  Short sequences are bound
-// by the chain of a piece, some 2200 clocks, and by what a block takes to begin and to end.  There, too, tiles of queries take heads of a group together (31 x 264 tokens, 56 heads: 385 -> 280 us,
+// 16384 tokens, 56 heads of 128: 11.5 ms, 0.84 PFLOP/s counted as five products and 1.17 as seven, bound by power as the forward pass; two documents of 4096: 1.4 to 1.7 ms.  Short sequences are bound
+// by the chain of a piece, some 2200 clocks, and by what a block takes to begin and to end.  There, too, tiles of queries take heads of a group together (31 x 264 tokens, 56 heads: 385 -> 280 to 291 us,
 // 200 x 30, 32 heads: 324 -> 155).
 //
 // Two groups of four warps have 64 columns of a piece each.  P and dS take the place of dP; that of the scores is free as soon as they are in registers, so the next piece's
@@ -1257,7 +1257,7 @@ cudaError_t allow_once(const void* fn, int bytes, std::atomic<uint64_t>& allowed
 
 // Small tasks are sequences of so many keys or fewer on average, or few tiles for the SMs: tiles of queries take heads together, and the forward pass one tile per CTA.  Forward: 8 x 1000 tokens of 56
 // heads 150 instead of 157 us, 8 x 1500 of 32 heads 196 instead of 221, 8 x 2000 of 56 485 instead of 471; one of 4096 with 16 heads (512 tiles) 81 instead of 97, with 32 (1024) 126 instead of 131, with 56
-// (1792) 223 instead of 213, one of 8192 with 16 (1024) 234 instead of 229.  Gradients (heads together or not): 16 x 450 285 instead of 320, 8 x 1500 598 instead of 620 to 637.
+// (1792) 223 instead of 213, one of 8192 with 16 (1024) 234 instead of 229.  The average decides: a long prompt beside many short ones goes the way of the short ones.  Gradients (heads together or not): 16 x 450 285 instead of 320, 8 x 1500 598 instead of 620 to 637.
 constexpr int kShortKeys = 2048, kFewTiles = 6;      // (tiles: per SM)
 bool is_small(const AttentionArgs& a) {
     return a.tk / std::max(a.num_seqs, 1) <= kShortKeys || static_cast<int64_t>(a.tq) * a.heads / 128 < static_cast<int64_t>(kFewTiles) * a.num_sms;

@@ -1,9 +1,11 @@
 // Attention of one new token per sequence over a paged cache:  o = softmax(scale q K^T) V  per query head, with the keys and values of its group's head, the first
 // lengths[i] places of the sequence, place p in page page_table[i, p / page_size].
 //
-// Bound by memory: every key and value is read once, 4 D bytes for 4 D operations per query head of the group.  So the work is cut into tiles of 64 keys of a (sequence, key
-// head), in one line, and every CTA takes an equal stretch of it, whatever the lengths; a pair whose tiles lie with several CTAs is joined by a second kernel.  A warp has
-// 16 keys of each tile, its own ring of asynchronous copies in shared memory and its own softmax in registers, so that no warp waits for another before a pair's end.
+// Bound by memory: every key and value is read once for 16 query heads of a group (once more for every further 16 that a group has), 4 D bytes for 4 D operations per query head.
+// A pair is a sequence and 16 query heads of a key head.  The pairs' keys are cut into tiles, 16 keys for each of a CTA's warps (one where pairs are many, otherwise four), in
+// one line, and every CTA takes an equal stretch of it, whatever the lengths; a pair whose tiles lie with several CTAs is joined by a second kernel.  Where no sequence can have
+// more than 512 keys a CTA takes a pair, and nothing is joined.  A warp has its own ring of asynchronous copies in shared memory and its own softmax in registers, so that no
+// warp waits for another before a pair's end.
 // Products are 16 x 8 x 16 (mma.sync): up to 16 query heads of a group are the rows, a thousandth of the tensor cores' rate, which is not what this waits for.
 // Statistics and sums are 32 bits, probabilities are rounded to bf16 as operands.
 #include <algorithm>

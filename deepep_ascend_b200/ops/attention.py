@@ -27,11 +27,14 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Opt
     and ``v``, if their lengths are others (keys of earlier calls in front).  With ``causal`` both of a sequence end together: query ``i`` of ``n`` sees the keys up to
     ``i + keys - n``.  A query that sees no key, and one that belongs to no sequence, gets zeros and an ``lse`` of -inf.
 
-    Whatever lies behind a sequence is not looked at; within one, keys and values must be numbers (a NaN reaches queries of its tile that do not see it).  Any strides;
+    Scores, sums and ``lse`` are 32 bits; probabilities (and in the gradients what is made of them) are rounded to bf16 where they go into a product, so results are off by up to two
+    roundings of bf16 of their terms.  Whatever lies behind a sequence is not looked at; within one, keys and values must be numbers (a value that is none reaches queries of its tile
+    that do not see it).  Any strides;
     heads whose channels are apart or that do not start on 16 bytes are copied first.  ``buffer``: see :func:`ops.gemm.gemm_nt`.
 
-    Both results carry gradients, by the kernels of :func:`attention_backward`.  Tracers, function transforms, dispatch modes and forward mode see the PyTorch
-    statement."""
+    Both results carry gradients, by the kernels of :func:`attention_backward`.  Tracers, function transforms, dispatch modes (selective
+    checkpoints are one) and forward mode see the PyTorch statement, which takes any floating type and holds the scores of all queries and all keys at once, ``4 heads tokens keys`` bytes
+    several times over: for real batches it is too large."""
     cu_q, cu_k, scale = _options(q, cu_seqlens, cu_seqlens_k, scale)
     if q.is_cuda and _by_type(q, k, v, cu_q, cu_k):
         res = _native.load().attention(q, k, v, cu_q, cu_k, causal, scale, _core_of(buffer))
@@ -68,7 +71,7 @@ def attention_backward(d_o: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: t
     """Gradients of :func:`attention` from ``d_o`` (like ``o``), optionally ``d_lse`` (like ``lse``), and what the forward pass was given and returned ->
     ``(d_q, d_k, d_v)``, contiguous.  Those of shared keys and values are added over their heads in 32 bits; every sum is taken in one order.  Queries and keys of no
     sequence, queries that see nothing and keys that nobody sees get zeros.  Where these gradients are to carry gradients themselves, and for whoever watches, the
-    PyTorch statement runs."""
+    PyTorch statement runs (of any floating type, with all scores at once)."""
     cu_q, cu_k, scale = _options(q, cu_seqlens, cu_seqlens_k, scale)
     if q.is_cuda and _by_type(d_o, q, k, v, o, lse, d_lse, cu_q, cu_k):
         res = _native.load().attention_backward(d_o, q, k, v, o, lse, d_lse, cu_q, cu_k, causal, scale, _core_of(buffer))
@@ -84,7 +87,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     Sequence ``i`` has ``lengths[i]`` keys (int32), the new token's own among them; key ``p`` stands in place ``p % page_size`` of page ``page_table[i, p // page_size]``
     (int32 ``[sequences, at least as many pages]``).  Places behind the length are not looked at, nor are the table's.  A sequence without keys gets zeros; one that names a page which
-    the caches do not have, or is longer than its row of the table, gets no numbers (NaN), and nothing is read for it.  ``heads``, ``kv_heads`` and ``scale``: see
+    the caches do not have, or is longer than its row of the table, gets no numbers (NaN); what its other pages hold may be read, nothing outside the caches and the table is.
+    Probabilities are rounded to bf16 where they go into the product with the values.  ``heads``, ``kv_heads`` and ``scale``: see
     :func:`attention`.  How the work is cut depends on the lengths of the whole batch: the last bits of a result can change with the batch that it is in.
 
     Carries no gradient of its own: where one is wanted, and for whoever watches, the PyTorch statement runs."""
